@@ -1,0 +1,233 @@
+// Attention over cache pages that also adds up, per cached key, the weight it received: what a cache that is to drop keys
+// goes by.  For every new token t of a request (n new ones, L keys in the cache with them) and query head h of KV head g
+//   s[j] = cap(scale q . k[j]),  j <= L - n + t;     p[j] = exp(s[j]) / (sum_j exp(s[j]) + exp(sink[h]));     out = sum_j p[j] v[j]
+//   scores_out[g][j] = (j < L - n ? scores[g][j] : 0) + sum over t and the heads of g of p[j];     births[g][j] = position, j new
+// A key's sum needs the rows' final normaliser, so there are two passes: the rows' (output and log-sum), then the keys'.
+//
+// The kernels of this file take any type, size and page size and compute in fp32.
+//   rows: a block holds 16 rows (token, head) of a KV head; 32 keys at a time in shared memory, lane <-> key for the scores,
+//     lane <-> column for the output.
+//   keys: a block holds 32 keys of a request and KV head and walks the rows that see them, lane <-> key, the warps' sums added
+//     in a fixed order at the end.
+// No sum is shared between blocks, so results do not depend on the order in which blocks run.
+#include <math.h>
+
+#include "nhv_common.cuh"
+
+namespace {
+
+constexpr int SA_WARPS = 4, SA_ROWS_PER_WARP = 4, SA_ROWS = SA_WARPS * SA_ROWS_PER_WARP, SA_KEYS = 32, SA_MAX_D = 256;
+constexpr float SA_LOG2E = 1.4426950408889634f;
+
+struct ScoredArgs {
+  const void* q;
+  void* out;
+  const void* pages;
+  const float* scores;      // [n_pages, nkv, page_size], what the keys had
+  float* scores_out;        // the same with this step's weights (may be scores itself)
+  int* births;              // [n_pages, nkv, page_size] or null
+  const int* positions;     // per new token, with births
+  const int* block_table;
+  const int* cu_q;
+  const int* kv_len;
+  const float* sinks;       // per query head, or null
+  float* lse;               // [nkv][n_tokens * G]: log2 of a row's sum; +inf for a row that sees nothing
+  int q_stride, out_stride, bt_stride, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages;
+  int max_keys;             // what the caller says of kv_len: no table is read beyond it
+  float scale, softcap;
+};
+
+// The request of row tile `tile`, its tiles counted in tokens of `per_tile`; -1 behind the last one.
+__device__ __forceinline__ int find_tile(const int* cu_q, int n_seqs, int per_tile, int& tile) {
+  for (int s = 0; s < n_seqs; ++s) {
+    const int nt = (cu_q[s + 1] - cu_q[s] + per_tile - 1) / per_tile;
+    if (tile < nt) return s;
+    tile -= nt;
+  }
+  return -1;
+}
+
+// The element of a key's row in the pages, or -1 where the request has no page for it.
+__device__ __forceinline__ long long key_row(const ScoredArgs& a, int seq, int j, int kvh, int plane) {
+  const int page = a.block_table[(size_t)seq * a.bt_stride + j / a.page_size];
+  if (page < 0 || page >= a.n_pages) return -1;
+  return ((((long long)page * 2 + plane) * a.nkv + kvh) * a.page_size + j % a.page_size) * a.d;
+}
+
+__device__ __forceinline__ float capped(float s, float cap) { return cap > 0.f ? cap * tanhf(s / cap) : s; }
+
+template <typename T>
+__global__ void __launch_bounds__(SA_WARPS * 32) scored_rows_kernel(const ScoredArgs a) {
+  extern __shared__ float smem[];
+  __shared__ long long k_at[SA_KEYS], v_at[SA_KEYS];
+  pdl_prologue();
+  const int G = a.nq / a.nkv, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a tile is a whole number of tokens where a group fits the 16 rows, else 16 heads of one token
+  const int per_tile = SA_ROWS / G > 0 ? SA_ROWS / G : 1, head_blocks = (G + SA_ROWS - 1) / SA_ROWS;
+  int tile = blockIdx.x / head_blocks;
+  const int g0 = (blockIdx.x % head_blocks) * SA_ROWS, gs = min(G - g0, SA_ROWS);
+  const int seq = find_tile(a.cu_q, a.n_seqs, per_tile, tile);
+  if (seq < 0) return;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), t0 = tile * per_tile;
+  const int rows = min(per_tile, n - t0) * gs, d = a.d, ks = d + 1;
+  float* Qs = smem;                       // [16][d]
+  float* Ks = Qs + SA_ROWS * d;           // [32][d + 1]
+  float* Vs = Ks + SA_KEYS * ks;          // [32][d]
+  float* Ps = Vs + SA_KEYS * d;           // [warps][32]
+  const T* q = (const T*)a.q;
+  const T* pages = (const T*)a.pages;
+  for (int i = threadIdx.x; i < rows * d; i += blockDim.x) {
+    const int r = i / d, c = i - r * d;
+    Qs[i] = to_f32<T>(q[(size_t)(first + t0 + r / gs) * a.q_stride + (size_t)(kvh * G + g0 + r % gs) * d + c]);
+  }
+  float m[SA_ROWS_PER_WARP], l[SA_ROWS_PER_WARP], o[SA_ROWS_PER_WARP][SA_MAX_D / 32];
+#pragma unroll
+  for (int i = 0; i < SA_ROWS_PER_WARP; ++i) {
+    const int r = warp * SA_ROWS_PER_WARP + i;
+    const bool sink = a.sinks && r < rows;
+    m[i] = sink ? a.sinks[kvh * G + g0 + r % gs] : -INFINITY;
+    l[i] = sink ? 1.f : 0.f;
+#pragma unroll
+    for (int c = 0; c < SA_MAX_D / 32; ++c) o[i][c] = 0.f;
+  }
+  const int last = min(total - n + t0 + (rows - 1) / gs, total - 1);       // the newest key that a row of the tile sees
+  for (int j0 = 0; j0 <= last; j0 += SA_KEYS) {
+    __syncthreads();
+    if (threadIdx.x < SA_KEYS) {
+      const int j = j0 + threadIdx.x;
+      k_at[threadIdx.x] = j <= last ? key_row(a, seq, j, kvh, 0) : -1;
+      v_at[threadIdx.x] = j <= last ? key_row(a, seq, j, kvh, 1) : -1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < SA_KEYS * d; i += blockDim.x) {
+      const int r = i / d, c = i - r * d;
+      Ks[r * ks + c] = k_at[r] >= 0 ? to_f32<T>(pages[k_at[r] + c]) : 0.f;
+      Vs[i] = v_at[r] >= 0 ? to_f32<T>(pages[v_at[r] + c]) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SA_ROWS_PER_WARP; ++i) {
+      const int r = warp * SA_ROWS_PER_WARP + i;
+      if (r >= rows) break;
+      const int hi = total - n + t0 + r / gs;
+      const bool sees = j0 + lane <= hi && k_at[lane] >= 0;
+      float s = 0.f;
+      for (int c = 0; c < d; ++c) s = fmaf(Qs[r * d + c], Ks[lane * ks + c], s);
+      s = sees ? capped(s * a.scale, a.softcap) : -INFINITY;
+      const float top = warp_max(s);
+      const unsigned live = __ballot_sync(0xffffffffu, sees);
+      if (!live) continue;
+      const float m_new = fmaxf(m[i], top), ref = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = expf(m[i] - ref), p = sees ? expf(s - ref) : 0.f;
+      l[i] = l[i] * alpha + warp_sum(p);
+      m[i] = m_new;
+      Ps[warp * SA_KEYS + lane] = p;
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < SA_MAX_D / 32; ++c) {
+        if (c * 32 + lane < d) {
+          float acc = 0.f;
+          for (int k = 0; k < SA_KEYS; ++k)
+            if (live >> k & 1) acc = fmaf(Ps[warp * SA_KEYS + k], Vs[k * d + c * 32 + lane], acc);   // a key out of sight may hold anything
+          o[i][c] = o[i][c] * alpha + acc;
+        }
+      }
+      __syncwarp();
+    }
+  }
+  T* out = (T*)a.out;
+#pragma unroll
+  for (int i = 0; i < SA_ROWS_PER_WARP; ++i) {
+    const int r = warp * SA_ROWS_PER_WARP + i;
+    if (r >= rows) break;
+    const int token = first + t0 + r / gs, head = g0 + r % gs;
+    const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
+#pragma unroll
+    for (int c = 0; c < SA_MAX_D / 32; ++c)
+      if (c * 32 + lane < d) out[(size_t)token * a.out_stride + (size_t)(kvh * G + head) * d + c * 32 + lane] = from_f32<T>(o[i][c] * inv);
+    if (lane == 0) a.lse[((size_t)kvh * a.n_tokens + token) * G + head] = l[i] == 0.f ? INFINITY : fmaf(m[i], SA_LOG2E, log2f(l[i]));
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SA_WARPS * 32) scored_keys_kernel(const ScoredArgs a) {
+  extern __shared__ float smem[];
+  __shared__ float part[SA_WARPS][SA_KEYS];
+  pdl_prologue();
+  const int G = a.nq / a.nkv, kvh = blockIdx.y, seq = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), j0 = blockIdx.x * SA_KEYS;
+  if (j0 >= total) return;
+  const int d = a.d, ks = d + 1, j = j0 + lane;
+  float* Ks = smem;                       // [32][d + 1]
+  float* Qs = Ks + SA_KEYS * ks;          // [warps][d]
+  const T* q = (const T*)a.q;
+  const T* pages = (const T*)a.pages;
+  for (int i = threadIdx.x; i < SA_KEYS * d; i += blockDim.x) {
+    const int r = i / d, c = i - r * d;
+    const long long at = j0 + r < total ? key_row(a, seq, j0 + r, kvh, 0) : -1;
+    Ks[r * ks + c] = at >= 0 ? to_f32<T>(pages[at + c]) : 0.f;
+  }
+  __syncthreads();
+  const long long mine = j < total ? key_row(a, seq, j, kvh, 0) : -1;
+  const int t_first = max(0, j0 - (total - n));        // the first token that sees a key of the block
+  float w = 0.f;
+  for (int r = t_first * G + warp; r < n * G; r += SA_WARPS) {
+    const int t = r / G, h = r - t * G;
+    __syncwarp();
+    for (int c = lane; c < d; c += 32) Qs[warp * d + c] = to_f32<T>(q[(size_t)(first + t) * a.q_stride + (size_t)(kvh * G + h) * d + c]);
+    __syncwarp();
+    float s = 0.f;
+    for (int c = 0; c < d; ++c) s = fmaf(Qs[warp * d + c], Ks[lane * ks + c], s);
+    if (j <= total - n + t)
+      w += exp2f(fmaf(capped(s * a.scale, a.softcap), SA_LOG2E, -a.lse[((size_t)kvh * a.n_tokens + first + t) * G + h]));
+  }
+  part[warp][lane] = w;
+  __syncthreads();
+  if (warp == 0 && mine >= 0) {
+    float sum = part[0][lane];
+    for (int k = 1; k < SA_WARPS; ++k) sum += part[k][lane];
+    const int page = a.block_table[(size_t)seq * a.bt_stride + j / a.page_size];
+    const size_t at = ((size_t)page * a.nkv + kvh) * a.page_size + j % a.page_size;
+    const bool fresh = j >= total - n;
+    a.scores_out[at] = (fresh ? 0.f : a.scores[at]) + sum;
+    if (fresh && a.births) a.births[at] = a.positions[first + j - (total - n)];
+  }
+}
+
+template <typename T>
+int launch_simt(const ScoredArgs& a, int max_kv_len, cudaStream_t stream) {
+  static std::atomic<uint64_t> rows_done{0}, keys_done{0};
+  const int G = a.nq / a.nkv, per_tile = SA_ROWS / G > 0 ? SA_ROWS / G : 1, head_blocks = (G + SA_ROWS - 1) / SA_ROWS;
+  const size_t rows_smem = sizeof(float) * (SA_ROWS * a.d + SA_KEYS * (a.d + 1) + SA_KEYS * a.d + SA_WARPS * SA_KEYS);
+  const size_t keys_smem = sizeof(float) * (SA_KEYS * (a.d + 1) + SA_WARPS * a.d);
+  const long long tiles = ((long long)a.n_tokens / per_tile + a.n_seqs) * head_blocks;
+  NHV_REQUIRE(tiles < (1LL << 31), "scored attention: %lld tiles of new tokens are beyond the grid's reach", tiles);
+  NHV_REQUIRE(a.n_seqs <= 65535, "scored attention: %d requests are beyond the grid's reach", a.n_seqs);
+  NHV_CUDA(nhv_allow_smem((const void*)scored_rows_kernel<T>, 96 * 1024, rows_done), "scored attention");
+  NHV_CUDA(nhv_allow_smem((const void*)scored_keys_kernel<T>, 96 * 1024, keys_done), "scored attention");
+  NHV_CUDA(nhv_launch(scored_rows_kernel<T>, dim3((unsigned)tiles, a.nkv), SA_WARPS * 32, rows_smem, stream, a), "scored attention");
+  NHV_CUDA(nhv_launch(scored_keys_kernel<T>, dim3((max_kv_len + SA_KEYS - 1) / SA_KEYS, a.nkv, a.n_seqs), SA_WARPS * 32, keys_smem, stream, a),
+           "scored attention");
+  return 0;
+}
+
+}  // namespace
+
+NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* out, int out_stride, const void* kv_pages,
+                                 const float* scores, float* scores_out, int* births, const int* positions, const int* block_table,
+                                 int bt_stride, const int* cu_q, const int* kv_len, int n_seqs, int n_tokens, int min_new, int max_new,
+                                 int max_kv_len, int nq, int nkv, int d, int page_size, int n_pages, float scale, const float* sinks,
+                                 float softcap, float* lse, cudaStream_t stream) {
+  NHV_REQUIRE(dtype == NHV_F32 || dtype == NHV_BF16, "scored attention: unknown type %d", dtype);
+  NHV_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "scored attention: %d query heads do not divide into %d KV heads", nq, nkv);
+  NHV_REQUIRE(d > 0 && d <= SA_MAX_D, "scored attention: head size %d is not in 1..%d", d, SA_MAX_D);
+  NHV_REQUIRE(page_size > 0 && n_pages > 0 && bt_stride >= 0 && nkv <= 65535, "scored attention: bad page geometry");
+  NHV_REQUIRE(n_seqs >= 0 && n_tokens >= 0 && min_new >= 0 && max_new >= min_new && max_kv_len >= max_new,
+              "scored attention: %d to %d new tokens with up to %d keys", min_new, max_new, max_kv_len);
+  NHV_REQUIRE(softcap >= 0.f, "scored attention: the cap on the scores is positive");
+  NHV_REQUIRE(!births == !positions || n_tokens == 0, "scored attention: births and positions go together");
+  if (n_seqs == 0 || max_kv_len == 0) return 0;
+  const ScoredArgs a{q, out, kv_pages, scores, scores_out, births, positions, block_table, cu_q, kv_len, sinks, lse,
+                     q_stride, out_stride, bt_stride, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages, max_kv_len, scale, softcap};
+  return dtype == NHV_F32 ? launch_simt<float>(a, max_kv_len, stream) : launch_simt<__nv_bfloat16>(a, max_kv_len, stream);
+}

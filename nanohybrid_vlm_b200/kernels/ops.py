@@ -1175,6 +1175,125 @@ def attention(out, q, kv_pages, tables, batch, nq: int, nkv: int, head_dim: int,
                        nq, nkv, head_dim, scale, window)
 
 
+def _page_geometry(kv_pages, nkv: int, scores, births, block_table, n_seqs: int, max_kv_len: int) -> tuple[int, int, int]:
+    """(number of pages, page size, head size), with what the kernels over scored pages assume checked."""
+    _need_cuda(kv_pages, scores, births, block_table)
+    if kv_pages is not None and (kv_pages.dim() != 5 or kv_pages.shape[1] != 2 or kv_pages.shape[2] != nkv or not kv_pages.is_contiguous()):
+        raise KernelError(f"pages are [n_pages, 2, {nkv}, page_size, head_dim] and contiguous, not {tuple(kv_pages.shape)}")
+    if scores.dim() != 3 or scores.shape[1] != nkv or scores.dtype != torch.float32 or not scores.is_contiguous():
+        raise KernelError(f"scores are [n_pages, {nkv}, page_size] float32 and contiguous, not {tuple(scores.shape)} {scores.dtype}")
+    n_pages, _, page_size = scores.shape
+    if kv_pages is not None and (kv_pages.shape[0] != n_pages or kv_pages.shape[3] != page_size):
+        raise KernelError(f"scores {tuple(scores.shape)} do not go with pages {tuple(kv_pages.shape)}")
+    if births is not None and (births.shape != scores.shape or births.dtype != torch.int32 or not births.is_contiguous()):
+        raise KernelError(f"births are int32 of the scores' shape {tuple(scores.shape)} and contiguous, not {tuple(births.shape)} {births.dtype}")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < n_seqs or block_table.stride(1) != 1:
+        raise KernelError(f"the block table has a row of int32 pages for each of the {n_seqs} requests")
+    if n_pages == 0 or page_size == 0 or max_kv_len > block_table.shape[1] * page_size:
+        raise KernelError(f"{max_kv_len} keys do not fit a block table of {block_table.shape[1]} pages of {page_size}")
+    return n_pages, page_size, 0 if kv_pages is None else kv_pages.shape[4]
+
+
+def _int_array(name: str, t, n: int) -> None:
+    _need_cuda(t)
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < n or t.stride(0) != 1:
+        raise KernelError(f"{name} is an int32 array of {n} entries, not {tuple(t.shape)} {t.dtype}")
+
+
+def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs: int, min_new: int, max_new: int, max_kv_len: int,
+                     nq: int, nkv: int, head_dim: int, scale: float, births=None, positions=None, sinks=None,
+                     softcap: float | None = None, scores_out=None) -> None:
+    """Causal attention of the step's new tokens over the paged cache, with the weight that every cached key received.
+
+    out, q [T, nq * head_dim] (rows may lie further apart), pages [n_pages, 2, nkv, page_size, head_dim] with the new keys and values
+    stored, scores [n_pages, nkv, page_size] float32: what the keys have gathered so far.  Of request i, tokens cu_q[i] .. cu_q[i + 1]
+    are new and its keys are the first kv_len[i] slots of its pages; a token sees all slots up to its own.  The new tokens'
+    weights, summed over the tokens and over the query heads of a KV head, are added to the scores of the request's keys
+    (new keys start from nothing) and written to ``scores_out`` (None: ``scores`` itself; slots of no request stay as they are).
+    ``births`` [n_pages, nkv, page_size] int32: receives ``positions`` [T] int32 for the new keys.  ``sinks`` and ``softcap`` as in
+    ``attention_tensor_core``.  ``min_new``, ``max_new``, ``max_kv_len``: the least and the most new tokens of a request, the most keys.
+    Scores, weights and sums are float32 and added in a fixed order: the same call gives the same bits."""
+    n_pages, page_size, d = _page_geometry(kv_pages, nkv, scores, births, block_table, n_seqs, max_kv_len)
+    _need_cuda(out, q, sinks)
+    if nq <= 0 or nkv <= 0 or nq % nkv:
+        raise KernelError(f"{nq} query heads do not divide into {nkv} KV heads")
+    if d != head_dim or not 0 < head_dim <= 256:
+        raise KernelError(f"attention with scores takes heads of 1 to 256 elements, the pages' own: not {head_dim} with pages of {d}")
+    T = q.shape[0]
+    if (q.dim() != 2 or q.shape != out.shape or q.shape[1] != nq * head_dim or q.stride(1) != 1 or out.stride(1) != 1
+            or not q.dtype == out.dtype == kv_pages.dtype):
+        raise KernelError(f"q and the output are [tokens, {nq * head_dim}] in the pages' type with neighbouring columns")
+    _int_array("cu_q", cu_q, n_seqs + 1)
+    _int_array("kv_len", kv_len, n_seqs)
+    if (births is None) != (positions is None):
+        raise KernelError("births and positions go together")
+    if positions is not None:
+        _int_array("positions", positions, T)
+    if not 0 <= min_new <= max_new <= max_kv_len or not min_new * n_seqs <= T <= max_new * n_seqs:
+        raise KernelError(f"{T} new tokens of {n_seqs} requests are not {min_new} to {max_new} each, among {max_kv_len} keys")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != nq or not sinks.is_contiguous()):
+        raise KernelError(f"sinks are {nq} float32 numbers")
+    if softcap is not None and not softcap > 0:
+        raise KernelError("the cap on the scores is positive")
+    if scores_out is None:
+        scores_out = scores
+    elif scores_out.shape != scores.shape or scores_out.dtype != torch.float32 or not scores_out.is_contiguous():
+        raise KernelError(f"scores_out is float32 of the scores' shape {tuple(scores.shape)} and contiguous")
+    _need_cuda(scores_out)
+    lse = torch.empty(T * nq, dtype=torch.float32, device=q.device)
+    call("nhv_attention_scored", dtype_code(q), q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv_pages.data_ptr(),
+         scores.data_ptr(), scores_out.data_ptr(), _ptr(births), _ptr(positions), block_table.data_ptr(), block_table.stride(0),
+         cu_q.data_ptr(), kv_len.data_ptr(), n_seqs, T, min_new, max_new, max_kv_len, nq, nkv, head_dim, page_size, n_pages, float(scale),
+         _ptr(sinks), float(softcap or 0.0), lse.data_ptr(), stream_ptr())
+
+
+def select_keys(sources, targets, scores, births, block_table, kv_len, seen, budgets, n_seqs: int, max_kv_len: int, keep_first: int,
+                keep_recent: int) -> None:
+    """Which keys leave a cache that is to hold ``budgets[i]`` keys of request i, said as moves that close the gaps.
+
+    Per request and KV head, the keys of positions below ``keep_first`` and of the last ``keep_recent`` positions before
+    ``seen[i]`` (the position of the request's next token) count as +inf, scores that are no numbers as less than any; the
+    ``budgets[i]`` largest of the first kv_len[i] slots stay, of equal ones those in the lowest slots.  ``sources``, ``targets`` [n_seqs,
+    nkv, M] int32: the i-th kept slot at or above the budget and the i-th dropped slot below it, -1 behind the last.  M has to reach
+    the largest kv_len[i] - budgets[i], or the largest budget if that is less (else the next check of the kernels raises)."""
+    nkv = scores.shape[1] if scores.dim() == 3 else 0
+    n_pages, page_size, _ = _page_geometry(None, nkv, scores, births, block_table, n_seqs, max_kv_len)
+    if births is None:
+        raise KernelError("the choice of keys needs their births")
+    for name, t in (("kv_len", kv_len), ("seen", seen), ("budgets", budgets)):
+        _int_array(name, t, n_seqs)
+    moves = _moves(sources, targets, n_seqs, nkv)
+    if keep_first < 0 or keep_recent < 0 or max_kv_len < 0:
+        raise KernelError("kept first and recent keys, and keys, are counted from 0")
+    call("nhv_select_keys", sources.data_ptr(), targets.data_ptr(), scores.data_ptr(), births.data_ptr(), block_table.data_ptr(),
+         block_table.stride(0), kv_len.data_ptr(), seen.data_ptr(), budgets.data_ptr(), n_seqs, max_kv_len, nkv, page_size, n_pages, moves,
+         keep_first, keep_recent, stream_ptr())
+
+
+def _moves(sources, targets, n_seqs: int, nkv: int) -> int:
+    _need_cuda(sources, targets)
+    for t in (sources, targets):
+        if t.dim() != 3 or t.shape[:2] != (n_seqs, nkv) or t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"sources and targets are [{n_seqs}, {nkv}, moves] int32 and contiguous, not {tuple(t.shape)} {t.dtype}")
+    if sources.shape != targets.shape:
+        raise KernelError("there are as many sources as targets")
+    return sources.shape[2]
+
+
+def move_keys(kv_pages, scores, births, block_table, sources, targets, n_seqs: int) -> None:
+    """Carry out the moves of ``select_keys`` in place: key, value, score and birth of every source slot go to its target slot.
+    Afterwards the request's keys fill its first min(kv_len, budget) slots.  Sources keep what they held."""
+    nkv = scores.shape[1] if scores.dim() == 3 else 0
+    n_pages, page_size, d = _page_geometry(kv_pages, nkv, scores, births, block_table, n_seqs, 0)
+    if births is None:
+        raise KernelError("the moves of keys take their births along")
+    dtype_code(kv_pages)
+    moves = _moves(sources, targets, n_seqs, nkv)
+    call("nhv_move_keys", kv_pages.data_ptr(), scores.data_ptr(), births.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+         block_table.shape[1], sources.data_ptr(), targets.data_ptr(), n_seqs, nkv, page_size, n_pages, moves, d * kv_pages.element_size(),
+         stream_ptr())
+
+
 FUSE_DECODE_QK = True             # tests switch it off to compare with the two-kernel form
 USE_TMA_DECODE = True             # tests switch it off to reach the mma.sync decode kernel at the same shapes
 
@@ -1692,7 +1811,7 @@ def _register_library_sources() -> None:
     import ctypes
     from .library import load_library
     lib = load_library()
-    for name in ("gemm_slab", "gemm_stream_k", "gemm_tcgen05", "moe_tcgen05", "gemm_f32_tcgen05"):
+    for name in ("gemm_slab", "gemm_stream_k", "gemm_tcgen05", "moe_tcgen05", "gemm_f32_tcgen05", "key_eviction"):
         word = getattr(lib, f"nhv_{name}_error_word")
         word.restype, word.argtypes = ctypes.c_void_p, []
         take = getattr(lib, f"nhv_{name}_error")

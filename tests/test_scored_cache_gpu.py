@@ -1,0 +1,489 @@
+"""Attention that adds up the weight of every cached key, the choice of the keys that stay and the moves that close the gaps,
+each against its definition in 64 bits on the CPU: lengths from none to thousands, heads and pages of odd sizes, pools of NaN,
+masked places that hold no numbers, scores with ties, infinities and NaN.
+
+The bounds are derived, not fitted.  A score is a sum of D products in 32 bits: its error is taken as 4 sqrt(D) units of 2^-24 of
+the sum of the products' magnitudes (a random walk with room), that of a capped one as eight units of the cap more.  A weight's
+relative error is then twice that, and sums of up to L terms add sqrt(L) units; the exponential and the division 2^-20; weights
+below 2^-126, the smallest 32-bit number that is not flushed, may be none.  In bfloat16
+the weights are rounded to 8 bits for the second product and the output once more: 2^-8 of the largest value."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F64 = torch.float64
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from nanohybrid_vlm_b200.kernels import ops
+    return ops
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+class Case:
+    """Requests with ``news`` new tokens among ``lens`` keys over pages in no order, in a pool that starts as NaN."""
+
+    def __init__(self, news, lens, nq, nkv, d, page, dtype, cap=None, sinks=False, seed=0, spread=1.5, width=0):
+        g = torch.Generator().manual_seed(seed)
+        self.news, self.lens, self.nq, self.nkv, self.d, self.page, self.dtype, self.cap = news, lens, nq, nkv, d, page, dtype, cap
+        counts = [-(-L // page) for L in lens]
+        self.n_pages = sum(counts) + 3
+        ids = torch.randperm(self.n_pages, generator=g).tolist()
+        self.table = torch.full((len(lens), max(counts + [1]) + width), -1, dtype=torch.int32)
+        self.pages = torch.full((self.n_pages, 2, nkv, page, d), math.nan, dtype=dtype)
+        self.scores = torch.full((self.n_pages, nkv, page), math.nan)
+        self.births = torch.full((self.n_pages, nkv, page), -7, dtype=torch.int32)
+        self.scale = d ** -0.5
+        T = sum(news)
+        self.q = (torch.randn(T, nq * d, generator=g) * spread).to(dtype)
+        self.sinks = torch.randn(nq, generator=g) if sinks else None
+        self.cu = [0]
+        self.positions = []
+        for s, (n, L) in enumerate(zip(news, lens)):
+            self.table[s, :counts[s]] = torch.tensor([ids.pop() for _ in range(counts[s])], dtype=torch.int32)
+            self.cu.append(self.cu[-1] + n)
+            self.positions += [1000 * s + L - n + t for t in range(n)]
+            for j in range(L):
+                p, o = int(self.table[s, j // page]), j % page
+                self.pages[p, :, :, o] = torch.randn(2, nkv, d, generator=g).to(dtype)
+                self.scores[p, :, o] = torch.rand(nkv, generator=g) * 3
+                self.births[p, :, o] = j
+                if j >= L - n:
+                    self.scores[p, :, o] = math.nan         # a new key has none yet
+        self.lens_t, self.cu_t = i32(lens), i32(self.cu)
+
+    def keys(self, s, g, plane):
+        L = self.lens[s]
+        rows = [self.pages[int(self.table[s, j // self.page]), plane, g, j % self.page] for j in range(L)]
+        return torch.stack(rows).to(F64) if rows else torch.zeros(0, self.d, dtype=F64)
+
+    def of(self, per_page, s, g):
+        return torch.stack([per_page[int(self.table[s, j // self.page]), g, j % self.page] for j in range(self.lens[s])]) \
+            if self.lens[s] else torch.zeros(0)
+
+    def want(self):
+        """(output, per request [nkv, L] the new weights, bounds of both) in 64 bits."""
+        G = self.nq // self.nkv
+        out, out_tol = torch.zeros(self.q.shape, dtype=F64), torch.zeros(self.q.shape, dtype=F64)
+        weights, tols = [], []
+        for s, (n, L) in enumerate(zip(self.news, self.lens)):
+            w_s, t_s = torch.zeros(self.nkv, L, dtype=F64), torch.zeros(self.nkv, L, dtype=F64)
+            for g in range(self.nkv):
+                k, v = self.keys(s, g, 0), self.keys(s, g, 1)
+                for h in range(g * G, (g + 1) * G):
+                    rows = slice(self.cu[s], self.cu[s] + n)
+                    x = self.q[rows, h * self.d:(h + 1) * self.d].to(F64)
+                    z = x @ k.T * self.scale
+                    err = (x.abs() @ k.abs().T * self.scale).amax() * 4 * math.sqrt(self.d) * 2 ** -24 if n and L else 0.0
+                    if self.cap:
+                        z = self.cap * torch.tanh(z / self.cap)
+                        err += 8 * self.cap * 2 ** -24
+                    for t in range(n):
+                        z[t, L - n + t + 1:] = -torch.inf
+                    norm = torch.logsumexp(z, 1, keepdim=True)
+                    if self.sinks is not None:
+                        norm = torch.logaddexp(norm, self.sinks[h].to(F64))
+                    p = torch.exp(z - norm)
+                    rel = 2 * err + math.sqrt(max(L, n * G)) * 2 ** -24 + 2 ** -20
+                    out[rows, h * self.d:(h + 1) * self.d] = p @ v
+                    # the weights' error times the values they weigh, and what is rounded to 8 bits
+                    unit = 2 ** -8 if self.dtype == torch.bfloat16 else 0.0
+                    out_tol[rows, h * self.d:(h + 1) * self.d] = (p @ v.abs()) * (rel + unit) + 2 ** -20 * (p @ v.abs())
+                    w_s[g] += p.sum(0)
+                    t_s[g] += p.sum(0) * rel + n * 2.0 ** -126      # a weight below the smallest 32-bit number is none
+            weights.append(w_s)
+            tols.append(t_s)
+        return out, out_tol, weights, tols
+
+    def run(self, ops, in_place=False, q=None, births=True, table=None):
+        dev = dict(q=(self.q if q is None else q).cuda(), pages=self.pages.cuda(), scores=self.scores.cuda(), births=self.births.cuda(),
+                   table=(self.table if table is None else table).cuda())
+        out = torch.full_like(dev["q"], math.nan)
+        scores_out = dev["scores"] if in_place else torch.full_like(dev["scores"], 5.0)
+        ops.attention_scored(out, dev["q"], dev["pages"], dev["scores"], dev["table"], self.cu_t, self.lens_t, len(self.lens),
+                             min(self.news), max(self.news), max(self.lens), self.nq, self.nkv, self.d, self.scale,
+                             births=dev["births"] if births else None, positions=i32(self.positions) if births else None,
+                             sinks=None if self.sinks is None else self.sinks.cuda(), softcap=self.cap,
+                             scores_out=None if in_place else scores_out)
+        torch.cuda.synchronize()
+        ops.raise_wait_errors()
+        return out.cpu(), scores_out.cpu(), dev["births"].cpu()
+
+    def check(self, out, scores_out, births=None, rows=None):
+        want, tol, weights, tols = self.want()
+        err = (out.to(F64) - want).abs()
+        rows = slice(None) if rows is None else rows
+        assert not torch.isnan(out[rows].float()).any()
+        assert (err <= tol)[rows].all(), (err / tol.clamp(min=1e-30))[rows].max()
+        touched = torch.zeros_like(self.scores, dtype=torch.bool)
+        for s, (n, L) in enumerate(zip(self.news, self.lens)):
+            for g in range(self.nkv):
+                old = self.of(self.scores, s, g).to(F64)
+                old[L - n:] = 0
+                got = self.of(scores_out, s, g).to(F64)
+                bound = tols[s][g] + (old + weights[s][g]) * 2 ** -22
+                diff = (got - old - weights[s][g]).abs()
+                assert (diff <= bound).all(), (s, g, (diff / bound.clamp(min=1e-30)).max())
+            for j in range(L):
+                touched[int(self.table[s, j // self.page]), :, j % self.page] = True
+        if births is not None:
+            expect = self.births.clone()
+            for s, (n, L) in enumerate(zip(self.news, self.lens)):
+                for t in range(n):
+                    j = L - n + t
+                    expect[int(self.table[s, j // self.page]), :, j % self.page] = self.positions[self.cu[s] + t]
+            assert torch.equal(births, expect)
+        return touched
+
+
+SHAPES = [(4, 2, 16, 16), (6, 2, 32, 8), (8, 8, 64, 64), (12, 4, 64, 16), (16, 2, 128, 256), (8, 2, 128, 32), (6, 1, 96, 24), (5, 1, 80, 7),
+          (3, 3, 256, 64), (40, 2, 64, 64), (2, 1, 33, 5), (7, 7, 8, 1), (4, 4, 192, 64), (64, 1, 128, 64)]
+LENGTHS = {
+    "single": ([1, 1, 1, 1], [1, 2, 65, 300]),
+    "prompts": ([70, 1, 33, 129], [70, 40, 97, 300]),
+    "few": ([3, 5, 0, 2], [200, 5, 17, 131]),
+    "one": ([1], [1]),
+}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page", SHAPES)
+@pytest.mark.parametrize("lengths", LENGTHS)
+def test_outputs_weights_and_births(ops, dtype, nq, nkv, d, page, lengths):
+    c = Case(*LENGTHS[lengths], nq, nkv, d, page, dtype, seed=nq * d + page)
+    out, scores_out, births = c.run(ops)
+    touched = c.check(out, scores_out, births)
+    assert (scores_out[~touched] == 5.0).all()              # slots of no request stay as they are
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page", [(8, 2, 128, 64), (6, 2, 32, 8), (12, 4, 64, 16)])
+@pytest.mark.parametrize("cap,sinks,spread", [(30.0, False, 1.5), (2.0, True, 20.0), (None, True, 1.5), (50.0, True, 60.0)])
+def test_caps_and_sinks(ops, dtype, nq, nkv, d, page, cap, sinks, spread):
+    for lengths in ("single", "prompts", "few"):
+        c = Case(*LENGTHS[lengths], nq, nkv, d, page, dtype, cap=cap, sinks=sinks, spread=spread, seed=3)
+        c.check(*c.run(ops))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page,news,lens", [
+    (8, 2, 128, 256, [1, 1], [5000, 3]),                    # one long request beside a short one
+    (8, 1, 64, 64, [1], [9001]),
+    (4, 1, 128, 64, [700], [700]),
+    (2, 1, 128, 64, [300, 40], [2900, 40]),
+    (4, 4, 64, 32, [17, 1, 600], [4000, 2000, 601]),
+    (16, 2, 128, 64, [4, 9, 2], [3000, 700, 2]),
+    (16, 1, 64, 8, [130] * 3, [130, 1000, 260]),
+])
+def test_long_requests(ops, dtype, nq, nkv, d, page, news, lens):
+    c = Case(news, lens, nq, nkv, d, page, dtype, seed=len(lens) + page)
+    c.check(*c.run(ops))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_requests(ops, dtype):
+    lens = [1 + (37 * i) % 90 for i in range(150)]
+    c = Case([1 + i % 3 if lens[i] > 3 else 1 for i in range(150)], lens, 4, 2, 64, 64, dtype, seed=8)
+    c.check(*c.run(ops))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths", ["single", "prompts"])
+def test_in_place_rows_apart_and_a_wide_table(ops, dtype, lengths):
+    c = Case(*LENGTHS[lengths], 8, 2, 64, 64, dtype, seed=5, width=3)
+    T = c.q.shape[0]
+    wide = torch.full((T, 8 * 64 + 64), math.nan, dtype=dtype)
+    wide[:, :8 * 64] = c.q
+    q = wide.cuda()[:, :8 * 64]
+    out = torch.full((T, 8 * 64 + 32), 9.0, dtype=dtype, device="cuda")
+    scores, births, pages = c.scores.cuda(), c.births.cuda(), c.pages.cuda()
+    table = torch.full((len(c.lens), c.table.shape[1] + 5), 12345, dtype=torch.int32)
+    table[:, :c.table.shape[1]] = c.table
+    ops.attention_scored(out[:, :8 * 64], q, pages, scores, table.cuda()[:, :c.table.shape[1]], c.cu_t, c.lens_t, len(c.lens), min(c.news),
+                         max(c.news), max(c.lens), 8, 2, 64, c.scale, births=births, positions=i32(c.positions))
+    c.check(out[:, :8 * 64].cpu(), scores.cpu(), births.cpu())
+    assert (out[:, 8 * 64:] == 9.0).all()
+    again, scores_again, _ = c.run(ops, births=False)       # without births, and out of place: the same numbers
+    assert torch.equal(out[:, :8 * 64].cpu(), again)
+    L = c.lens[-1]
+    assert torch.equal(c.of(scores.cpu(), len(c.lens) - 1, 1)[:L], c.of(scores_again, len(c.lens) - 1, 1)[:L])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,page", [(128, 64), (32, 8), (64, 256)])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_what_a_token_does_not_see_does_not_reach_it(ops, dtype, d, page, what):
+    """Key or value of the token in the middle of a portion is no number: earlier tokens do not notice, and later ones of a
+    request of their own neither."""
+    n = 80
+    c = Case([n, 1, 50], [n + 40, 30, 50], 4, 2, d, page, dtype, seed=d)
+    clean, scores_clean, _ = c.run(ops)
+    bad = 40 + 45                                           # the slot of the first request's 46th new token
+    for plane in (0, 1):
+        pages = c.pages.clone()
+        c.pages[int(c.table[0, bad // page]), plane, :, bad % page] = what
+        out, scores_out, _ = c.run(ops)
+        c.pages = pages
+        assert torch.equal(out[:45], clean[:45]) and torch.equal(out[n:], clean[n:])
+        if plane == 1:
+            assert not torch.isfinite(out[45:n].float()).any()          # p v of a value that is no number, for every later token
+            for s in range(3):                                          # weights do not depend on values
+                assert torch.equal(c.of(scores_out, s, 0), c.of(scores_clean, s, 0))
+        for s in (1, 2):
+            assert torch.equal(c.of(scores_out, s, 1), c.of(scores_clean, s, 1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_of_any_size(ops, dtype):
+    """Products that reach the ends of the exponential: one key takes all, or all keys tie."""
+    c = Case([9, 1], [90, 70], 4, 2, 64, 64, dtype, seed=2, spread=300.0)
+    c.check(*c.run(ops))
+    c = Case([9, 1], [90, 70], 4, 2, 64, 64, dtype, seed=2, spread=0.0)
+    out, scores_out, births = c.run(ops)
+    c.check(out, scores_out, births)
+    c = Case([9, 1], [90, 70], 4, 2, 64, 64, dtype, seed=2, spread=1e-30)
+    c.check(*c.run(ops))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths", ["single", "prompts", "few"])
+def test_the_same_call_gives_the_same_bits_on_any_stream(ops, dtype, lengths):
+    c = Case(*LENGTHS[lengths], 8, 2, 128, 64, dtype, seed=4)
+    first = c.run(ops)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        second = c.run(ops)
+    assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(first[:2], second[:2]))
+
+
+def test_requests_without_keys_and_entries_without_pages(ops):
+    for dtype in DTYPES:
+        # an entry that only pads a batch: one token, no page
+        c = Case([1, 1, 0], [30, 1, 0], 4, 2, 64, 64, dtype, seed=6)
+        c.table[1] = -1
+        out, scores_out, _ = c.run(ops)
+        assert (out[1] == 0).all() and not torch.isnan(out.float()).any()
+        c = Case([20, 0], [20, 45], 4, 2, 64, 64, dtype, seed=6)        # a request that brings nothing keeps its scores
+        _, scores_out, _ = c.run(ops)
+        assert torch.equal(c.of(scores_out, 1, 0), c.of(c.scores, 1, 0))
+
+
+def test_refusals_of_attention(ops):
+    from nanohybrid_vlm_b200.kernels.library import KernelError
+    c = Case([2, 1], [40, 30], 4, 2, 64, 16, torch.bfloat16)
+    base = dict(out=torch.empty_like(c.q).cuda(), q=c.q.cuda(), kv_pages=c.pages.cuda(), scores=c.scores.cuda(), block_table=c.table.cuda(),
+                cu_q=c.cu_t, kv_len=c.lens_t, n_seqs=2, min_new=1, max_new=2, max_kv_len=40, nq=4, nkv=2, head_dim=64, scale=0.125)
+    ops.attention_scored(**base)
+    wrong = [dict(q=c.q), dict(q=c.q.float().cuda()), dict(nq=3), dict(nkv=4), dict(head_dim=32), dict(scores=c.scores.cuda()[:, :1]),
+             dict(scores=c.scores.cuda().half()), dict(scores=c.scores.cuda()[:-1]), dict(block_table=c.table.cuda().long()),
+             dict(block_table=c.table.cuda()[:1]), dict(max_kv_len=100000), dict(cu_q=c.cu_t[:2]), dict(kv_len=c.lens_t.long()), dict(min_new=3),
+             dict(max_new=1), dict(births=c.births.cuda()), dict(positions=i32(c.positions)), dict(births=c.births.cuda(), positions=i32([1])),
+             dict(births=c.births.cuda().float(), positions=i32(c.positions)), dict(sinks=torch.zeros(3).cuda()), dict(softcap=-1.0), dict(softcap=0.0),
+             dict(scores_out=c.scores.cuda()[1:]), dict(out=torch.empty(3, 8).cuda()), dict(kv_pages=c.pages.cuda().transpose(2, 3)),
+             dict(kv_pages=c.pages.cuda().half(), q=c.q.cuda().half(), out=c.q.cuda().half())]
+    for change in wrong:
+        with pytest.raises(KernelError):
+            ops.attention_scored(**{**base, **change})
+    big = Case([1], [3], 1, 1, 257, 4, torch.float32)
+    with pytest.raises(KernelError):
+        big.run(ops)
+
+
+# ---------------------------------------------------------------- which keys stay
+def choose(scores, births, lens, seen, budgets, keep_first, keep_recent):
+    """The definition, slot by slot: per request and head the moves (source, target) in order."""
+    out = []
+    for s, L in enumerate(lens):
+        per_head = []
+        for g in range(scores[s].shape[0]):
+            def value(j):
+                b, x = int(births[s][g, j]), float(scores[s][g, j])
+                if b < keep_first or b >= seen[s] - keep_recent:
+                    return math.inf
+                return x
+            vals = [value(j) for j in range(L)]
+            order = sorted(range(L), key=lambda j: (math.isnan(vals[j]), -vals[j] if not math.isnan(vals[j]) else 0.0, j))
+            kept = set(order[:max(0, budgets[s])])
+            sources = [j for j in range(L) if j in kept and j >= budgets[s]]
+            targets = [j for j in range(L) if j not in kept and j < budgets[s]]
+            per_head.append(list(zip(sources, targets)))
+        out.append(per_head)
+    return out
+
+
+class Pool:
+    def __init__(self, lens, nkv, page, seed=0, d=0, dtype=torch.float32):
+        g = torch.Generator().manual_seed(seed)
+        counts = [-(-L // page) for L in lens]
+        n_pages = sum(counts) + 2
+        ids = torch.randperm(n_pages, generator=g).tolist()
+        self.lens, self.nkv, self.page, self.n_pages = lens, nkv, page, n_pages
+        self.table = torch.full((len(lens), max(counts + [1])), -1, dtype=torch.int32)
+        for s, c in enumerate(counts):
+            self.table[s, :c] = torch.tensor([ids.pop() for _ in range(c)], dtype=torch.int32)
+        self.scores = torch.full((n_pages, nkv, page), math.nan)
+        self.births = torch.full((n_pages, nkv, page), -1, dtype=torch.int32)
+        if d:
+            self.pages = torch.randn(n_pages, 2, nkv, page, d, generator=g).to(dtype)
+        self.gen = g
+
+    def fill(self, scores, births):
+        """Lists per request of [nkv, L]."""
+        for s, L in enumerate(self.lens):
+            for p in range(-(-L // self.page)):
+                a, b = p * self.page, min(L, (p + 1) * self.page)
+                self.scores[int(self.table[s, p]), :, :b - a] = scores[s][:, a:b]
+                self.births[int(self.table[s, p]), :, :b - a] = births[s][:, a:b]
+
+    def random(self, ties, order=True):
+        scores, births = [], []
+        for L in self.lens:
+            x = torch.randn(self.nkv, L, generator=self.gen).exp()
+            scores.append((x * 4).round() / 4 if ties else x)
+            b = torch.stack([torch.randperm(2 * L + 1, generator=self.gen)[:L] for _ in range(self.nkv)]) if L else torch.zeros(self.nkv, 0)
+            births.append((b.sort(1).values if order else b).int())
+        self.fill(scores, births)
+        return scores, births
+
+    def select(self, ops, seen, budgets, keep_first, keep_recent, room=None):
+        M = max([0] + [min(max(0, b), max(0, L - b)) for L, b in zip(self.lens, budgets)]) if room is None else room
+        sources = torch.full((len(self.lens), self.nkv, M), 99, dtype=torch.int32, device="cuda")
+        targets = torch.full_like(sources, 99)
+        ops.select_keys(sources, targets, self.scores.cuda(), self.births.cuda(), self.table.cuda(), i32(self.lens), i32(seen), i32(budgets),
+                        len(self.lens), max(self.lens), keep_first, keep_recent)
+        return sources, targets
+
+    def check(self, ops, scores, births, seen, budgets, keep_first, keep_recent, room=None):
+        sources, targets = self.select(ops, seen, budgets, keep_first, keep_recent, room)
+        ops.raise_wait_errors()
+        want = choose(scores, births, self.lens, seen, budgets, keep_first, keep_recent)
+        for s in range(len(self.lens)):
+            for g in range(self.nkv):
+                got = list(zip(sources[s, g].tolist(), targets[s, g].tolist()))
+                n = len(want[s][g])
+                assert got[:n] == want[s][g] and all(x == (-1, -1) for x in got[n:]), (s, g)
+        return sources, targets
+
+
+@pytest.mark.parametrize("nkv,page,lens,budgets", [
+    (2, 16, [100, 31, 64, 1, 0], [40, 31, 1, 1, 5]),
+    (1, 1, [57], [20]),
+    (3, 7, [2000, 1999, 600], [600, 1, 599]),
+    (8, 256, [2304, 2049, 700, 2304], [2048, 2048, 2048, 0]),
+    (1, 64, [9000], [4500]),
+    (2, 256, [40001, 12], [4096, 4096]),
+    (4, 32, [600], [599]),
+    (1, 16, [70000], [69000]),
+])
+@pytest.mark.parametrize("ties", [False, True])
+@pytest.mark.parametrize("keep_first,keep_recent", [(0, 0), (4, 9), (3, 100000)])
+def test_the_keys_that_stay(ops, nkv, page, lens, budgets, ties, keep_first, keep_recent):
+    p = Pool(lens, nkv, page, seed=page + len(lens))
+    scores, births = p.random(ties, order=page != 32)
+    p.check(ops, scores, births, [2 * L + 1 for L in lens], budgets, keep_first, keep_recent)
+
+
+def test_scores_that_are_alike_infinite_or_no_numbers(ops):
+    L = 300
+    p = Pool([L, L, L, L], 2, 16, seed=1)
+    scores, births = p.random(False)
+    odd = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0, 1e-45, -1e-45, 3.4e38, -3.4e38, 1.0])
+    scores[0] = odd.repeat(2, L // 10)
+    scores[1] = torch.full((2, L), 2.5)
+    scores[2] = torch.full((2, L), math.nan)
+    scores[3] = torch.where(torch.arange(L) % 2 == 0, 0.0, -0.0).repeat(2, 1)
+    p.fill(scores, births)
+    for budget in (1, 29, 30, 31, 150, 299):
+        p.check(ops, scores, births, [2 * L + 1] * 4, [budget] * 4, 0, 0)
+    p.check(ops, scores, births, [2 * L + 1] * 4, [150] * 4, 7, 30)
+
+
+def test_room_for_moves(ops):
+    from nanohybrid_vlm_b200.kernels.library import KernelError
+    p = Pool([64], 1, 16, seed=2)
+    scores = [torch.arange(64).float().view(1, -1)]
+    births = [torch.arange(64, dtype=torch.int32).view(1, -1)]
+    p.fill(scores, births)
+    p.check(ops, scores, births, [64], [20], 0, 0, room=20)
+    p.check(ops, scores, births, [64], [20], 0, 0, room=50)
+    p.select(ops, [64], [20], 0, 0, room=19)                # one too few: the next check of the kernels says so
+    with pytest.raises(KernelError, match="key_eviction"):
+        ops.raise_wait_errors()
+    ops.raise_wait_errors()
+
+
+def test_refusals_of_the_choice_and_the_moves(ops):
+    from nanohybrid_vlm_b200.kernels.library import KernelError
+    p = Pool([40], 2, 16, seed=3, d=8)
+    p.random(False)
+    moves = torch.full((1, 2, 20), -1, dtype=torch.int32, device="cuda")
+    base = dict(sources=moves, targets=moves.clone(), scores=p.scores.cuda(), births=p.births.cuda(), block_table=p.table.cuda(), kv_len=i32([40]),
+                seen=i32([40]), budgets=i32([20]), n_seqs=1, max_kv_len=40, keep_first=0, keep_recent=0)
+    ops.select_keys(**base)
+    for change in (dict(sources=moves[:, :1]), dict(targets=moves[..., :10].contiguous()), dict(sources=moves.long()), dict(scores=p.scores),
+                   dict(births=None), dict(births=p.births.cuda().long()), dict(kv_len=i32([])), dict(seen=torch.zeros(1).cuda()), dict(budgets=i32([])),
+                   dict(max_kv_len=1000), dict(keep_first=-1), dict(keep_recent=-1), dict(block_table=p.table.cuda().long())):
+        with pytest.raises(KernelError):
+            ops.select_keys(**{**base, **change})
+    base = dict(kv_pages=p.pages.cuda(), scores=p.scores.cuda(), births=p.births.cuda(), block_table=p.table.cuda(), sources=moves, targets=moves, n_seqs=1)
+    ops.move_keys(**base)
+    for change in (dict(kv_pages=p.pages), dict(kv_pages=p.pages.cuda().half()), dict(kv_pages=p.pages.cuda()[:-1]), dict(births=None),
+                   dict(sources=moves[:, :1]), dict(n_seqs=2), dict(scores=p.scores.cuda().double())):
+        with pytest.raises(KernelError):
+            ops.move_keys(**{**base, **change})
+
+
+# ---------------------------------------------------------------- the moves
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nkv,d,page,lens,budgets", [
+    (2, 64, 16, [100, 31, 64, 0], [40, 31, 1, 5]),
+    (1, 33, 7, [500], [200]),
+    (8, 128, 256, [2304, 700], [2048, 600]),
+    (3, 8, 64, [1000], [10]),
+    (2, 256, 32, [90], [45]),
+    (1, 1, 1, [20], [7]),
+])
+def test_the_moves(ops, dtype, nkv, d, page, lens, budgets):
+    p = Pool(lens, nkv, page, seed=d, d=d, dtype=dtype)
+    scores, births = p.random(False)
+    sources, targets = p.select(ops, [2 * L + 1 for L in lens], budgets, 2, 5)
+    pages, sc, bi = p.pages.cuda(), p.scores.cuda(), p.births.cuda()
+    for _ in range(2):                                      # twice is the same as once
+        ops.move_keys(pages, sc, bi, p.table.cuda(), sources, targets, len(lens))
+    want_pages, want_sc, want_bi = p.pages.clone(), p.scores.clone(), p.births.clone()
+    for s in range(len(lens)):
+        for g in range(nkv):
+            for a, b in zip(sources[s, g].tolist(), targets[s, g].tolist()):
+                if a < 0:
+                    continue
+                pa, pb = int(p.table[s, a // page]), int(p.table[s, b // page])
+                want_pages[pb, :, g, b % page] = p.pages[pa, :, g, a % page]
+                want_sc[pb, g, b % page] = p.scores[pa, g, a % page]
+                want_bi[pb, g, b % page] = p.births[pa, g, a % page]
+    assert torch.equal(pages.cpu(), want_pages) and torch.equal(bi.cpu(), want_bi)
+    assert torch.equal(sc.cpu().nan_to_num(-1.0), want_sc.nan_to_num(-1.0))
+    # what stays are the largest scores, whatever order they lie in
+    for s, (L, b) in enumerate(zip(lens, budgets)):
+        at = [(int(p.table[s, j // page]), j % page) for j in range(min(L, b))]
+        for g in range(nkv):
+            kept = sorted(int(bi[q, g, o]) for q, o in at)
+            held = [(int(births[s][g, j]), float(scores[s][g, j])) for j in range(L)]
+            held = [(math.inf if t < 2 or t >= 2 * L + 1 - 5 else x, t) for t, x in held]
+            assert kept == sorted(t for _, t in sorted(held, key=lambda v: -v[0])[:b])
+
+
+def test_moves_beyond_the_table_move_nothing(ops):
+    p = Pool([40], 1, 16, seed=3, d=8)
+    p.random(False)
+    bad = torch.tensor([[[1000, 5, -1, 39]]], dtype=torch.int32, device="cuda")
+    to = torch.tensor([[[1, 4000, 3, -1]]], dtype=torch.int32, device="cuda")
+    pages, sc, bi = p.pages.cuda(), p.scores.cuda(), p.births.cuda()
+    ops.move_keys(pages, sc, bi, p.table.cuda(), bad, to, 1)
+    assert torch.equal(pages.cpu(), p.pages) and torch.equal(bi.cpu(), p.births)
