@@ -1,0 +1,80 @@
+// What the kernels of attention with scored keys share: their arguments, and the passes behind a split over the keys.
+#pragma once
+#include <math.h>
+
+#include "nhv_common.cuh"
+
+constexpr float SA_LOG2E = 1.4426950408889634f;
+constexpr int SA_MAX_D = 256;
+
+struct ScoredArgs {
+  const void* q;
+  void* out;
+  const void* pages;
+  const float* scores;      // [n_pages, nkv, page_size], what the keys had
+  float* scores_out;        // the same with this step's weights (may be scores itself)
+  int* births;              // [n_pages, nkv, page_size] or null
+  const int* positions;     // per new token, with births
+  const int* block_table;
+  const int* cu_q;
+  const int* kv_len;
+  const float* sinks;       // per query head, or null
+  float* lse;               // [nkv][n_tokens * G]: log2 of a row's sum; +inf for a row that sees nothing
+  int q_stride, out_stride, bt_stride, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages;
+  int max_keys;             // what the caller says of kv_len: no table is read beyond it
+  int min_rows, max_rows;   // a kernel takes the requests whose new tokens times G lie in this range (both included)
+  float scale, softcap;
+};
+
+__device__ __forceinline__ bool scored_takes(const ScoredArgs& a, int n) {
+  const int rows = n * (a.nq / a.nkv);
+  return rows >= a.min_rows && rows <= a.max_rows;
+}
+
+// The request of row tile `tile`, its tiles counted in tokens of `per_tile`; -1 behind the last one.
+__device__ __forceinline__ int find_tile(const ScoredArgs& a, int per_tile, int& tile) {
+  for (int s = 0; s < a.n_seqs; ++s) {
+    const int n = a.cu_q[s + 1] - a.cu_q[s];
+    if (!scored_takes(a, n)) continue;
+    const int nt = (n + per_tile - 1) / per_tile;
+    if (tile < nt) return s;
+    tile -= nt;
+  }
+  return -1;
+}
+
+// The element of a key's row in the pages, or -1 where the request has no page for it.
+__device__ __forceinline__ long long key_row(const ScoredArgs& a, int seq, int j, int kvh, int plane) {
+  const int page = a.block_table[(size_t)seq * a.bt_stride + j / a.page_size];
+  if (page < 0 || page >= a.n_pages) return -1;
+  return ((((long long)page * 2 + plane) * a.nkv + kvh) * a.page_size + j % a.page_size) * a.d;
+}
+
+// A key's sum of weights goes to its score, and a new key's position to its birth.  `fresh`: j - (keys before this step).
+__device__ __forceinline__ void store_weight(const ScoredArgs& a, int seq, int first, int kvh, int j, int fresh, float sum) {
+  const int page = a.block_table[(size_t)seq * a.bt_stride + j / a.page_size];
+  if (page < 0 || page >= a.n_pages) return;
+  const size_t at = ((size_t)page * a.nkv + kvh) * a.page_size + j % a.page_size;
+  a.scores_out[at] = (fresh >= 0 ? 0.f : a.scores[at]) + sum;
+  if (fresh >= 0 && a.births) a.births[at] = a.positions[first + fresh];
+}
+
+__device__ __forceinline__ float scored_exp2(float x) {     // 2^x; -inf gives 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---- requests with few rows (scored_attention_short.cu): the keys are split over blocks, the scores kept for the second pass
+struct ShortPlan {
+  int rows;                 // rows kept per key: the most of a request, rounded up to 2
+  int split_keys, splits;   // keys of a block, blocks of a request's KV head
+  int group;                // requests per pair of launches (the scores kept are bounded)
+  size_t keys;              // places for keys of a (request, KV head)
+  size_t floats;            // of scratch
+};
+// Whether requests of up to `rows` rows can go this way.
+bool scored_short_takes(int dtype, int rows, int d);
+ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d);
+// The requests with a.min_rows to a.max_rows rows: output, scores and births.  `work`: plan.floats floats.
+int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* work, cudaStream_t stream);

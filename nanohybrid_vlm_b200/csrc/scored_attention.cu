@@ -10,49 +10,11 @@
 //   keys: a block holds 32 keys of a request and KV head and walks the rows that see them, lane <-> key, the warps' sums added
 //     in a fixed order at the end.
 // No sum is shared between blocks, so results do not depend on the order in which blocks run.
-#include <math.h>
-
-#include "nhv_common.cuh"
+#include "nhv_scored.cuh"
 
 namespace {
 
-constexpr int SA_WARPS = 4, SA_ROWS_PER_WARP = 4, SA_ROWS = SA_WARPS * SA_ROWS_PER_WARP, SA_KEYS = 32, SA_MAX_D = 256;
-constexpr float SA_LOG2E = 1.4426950408889634f;
-
-struct ScoredArgs {
-  const void* q;
-  void* out;
-  const void* pages;
-  const float* scores;      // [n_pages, nkv, page_size], what the keys had
-  float* scores_out;        // the same with this step's weights (may be scores itself)
-  int* births;              // [n_pages, nkv, page_size] or null
-  const int* positions;     // per new token, with births
-  const int* block_table;
-  const int* cu_q;
-  const int* kv_len;
-  const float* sinks;       // per query head, or null
-  float* lse;               // [nkv][n_tokens * G]: log2 of a row's sum; +inf for a row that sees nothing
-  int q_stride, out_stride, bt_stride, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages;
-  int max_keys;             // what the caller says of kv_len: no table is read beyond it
-  float scale, softcap;
-};
-
-// The request of row tile `tile`, its tiles counted in tokens of `per_tile`; -1 behind the last one.
-__device__ __forceinline__ int find_tile(const int* cu_q, int n_seqs, int per_tile, int& tile) {
-  for (int s = 0; s < n_seqs; ++s) {
-    const int nt = (cu_q[s + 1] - cu_q[s] + per_tile - 1) / per_tile;
-    if (tile < nt) return s;
-    tile -= nt;
-  }
-  return -1;
-}
-
-// The element of a key's row in the pages, or -1 where the request has no page for it.
-__device__ __forceinline__ long long key_row(const ScoredArgs& a, int seq, int j, int kvh, int plane) {
-  const int page = a.block_table[(size_t)seq * a.bt_stride + j / a.page_size];
-  if (page < 0 || page >= a.n_pages) return -1;
-  return ((((long long)page * 2 + plane) * a.nkv + kvh) * a.page_size + j % a.page_size) * a.d;
-}
+constexpr int SA_WARPS = 4, SA_ROWS_PER_WARP = 4, SA_ROWS = SA_WARPS * SA_ROWS_PER_WARP, SA_KEYS = 32;
 
 __device__ __forceinline__ float capped(float s, float cap) { return cap > 0.f ? cap * tanhf(s / cap) : s; }
 
@@ -66,7 +28,7 @@ __global__ void __launch_bounds__(SA_WARPS * 32) scored_rows_kernel(const Scored
   const int per_tile = SA_ROWS / G > 0 ? SA_ROWS / G : 1, head_blocks = (G + SA_ROWS - 1) / SA_ROWS;
   int tile = blockIdx.x / head_blocks;
   const int g0 = (blockIdx.x % head_blocks) * SA_ROWS, gs = min(G - g0, SA_ROWS);
-  const int seq = find_tile(a.cu_q, a.n_seqs, per_tile, tile);
+  const int seq = find_tile(a, per_tile, tile);
   if (seq < 0) return;
   const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), t0 = tile * per_tile;
   const int rows = min(per_tile, n - t0) * gs, d = a.d, ks = d + 1;
@@ -156,7 +118,7 @@ __global__ void __launch_bounds__(SA_WARPS * 32) scored_keys_kernel(const Scored
   pdl_prologue();
   const int G = a.nq / a.nkv, kvh = blockIdx.y, seq = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), j0 = blockIdx.x * SA_KEYS;
-  if (j0 >= total) return;
+  if (j0 >= total || !scored_takes(a, n)) return;
   const int d = a.d, ks = d + 1, j = j0 + lane;
   float* Ks = smem;                       // [32][d + 1]
   float* Qs = Ks + SA_KEYS * ks;          // [warps][d]
@@ -168,7 +130,6 @@ __global__ void __launch_bounds__(SA_WARPS * 32) scored_keys_kernel(const Scored
     Ks[r * ks + c] = at >= 0 ? to_f32<T>(pages[at + c]) : 0.f;
   }
   __syncthreads();
-  const long long mine = j < total ? key_row(a, seq, j, kvh, 0) : -1;
   const int t_first = max(0, j0 - (total - n));        // the first token that sees a key of the block
   float w = 0.f;
   for (int r = t_first * G + warp; r < n * G; r += SA_WARPS) {
@@ -183,14 +144,10 @@ __global__ void __launch_bounds__(SA_WARPS * 32) scored_keys_kernel(const Scored
   }
   part[warp][lane] = w;
   __syncthreads();
-  if (warp == 0 && mine >= 0) {
+  if (warp == 0 && j < total) {
     float sum = part[0][lane];
     for (int k = 1; k < SA_WARPS; ++k) sum += part[k][lane];
-    const int page = a.block_table[(size_t)seq * a.bt_stride + j / a.page_size];
-    const size_t at = ((size_t)page * a.nkv + kvh) * a.page_size + j % a.page_size;
-    const bool fresh = j >= total - n;
-    a.scores_out[at] = (fresh ? 0.f : a.scores[at]) + sum;
-    if (fresh && a.births) a.births[at] = a.positions[first + j - (total - n)];
+    store_weight(a, seq, first, kvh, j, j - (total - n), sum);
   }
 }
 
@@ -202,7 +159,6 @@ int launch_simt(const ScoredArgs& a, int max_kv_len, cudaStream_t stream) {
   const size_t keys_smem = sizeof(float) * (SA_KEYS * (a.d + 1) + SA_WARPS * a.d);
   const long long tiles = ((long long)a.n_tokens / per_tile + a.n_seqs) * head_blocks;
   NHV_REQUIRE(tiles < (1LL << 31), "scored attention: %lld tiles of new tokens are beyond the grid's reach", tiles);
-  NHV_REQUIRE(a.n_seqs <= 65535, "scored attention: %d requests are beyond the grid's reach", a.n_seqs);
   NHV_CUDA(nhv_allow_smem((const void*)scored_rows_kernel<T>, 96 * 1024, rows_done), "scored attention");
   NHV_CUDA(nhv_allow_smem((const void*)scored_keys_kernel<T>, 96 * 1024, keys_done), "scored attention");
   NHV_CUDA(nhv_launch(scored_rows_kernel<T>, dim3((unsigned)tiles, a.nkv), SA_WARPS * 32, rows_smem, stream, a), "scored attention");
@@ -213,11 +169,39 @@ int launch_simt(const ScoredArgs& a, int max_kv_len, cudaStream_t stream) {
 
 }  // namespace
 
+// What a call needs beside its arguments, and which kernels take which requests: those of up to `short_rows` rows the kernels of
+// scored_attention_short.cu, the others the ones of this file.
+struct ScoredPlan {
+  int short_rows;           // -1: none go that way
+  ShortPlan few;
+  size_t floats;            // of scratch
+};
+
+static ScoredPlan scored_plan(int dtype, int n_seqs, int n_tokens, int min_new, int max_new, int max_keys, int nq, int nkv, int d) {
+  ScoredPlan p = {};
+  p.short_rows = -1;
+  p.floats = ((size_t)n_tokens * nq + 3) / 4 * 4;
+  const int G = nq / nkv, most = d <= 128 ? 16 : 8;
+  if (scored_short_takes(dtype, min_new * G, d)) {
+    p.short_rows = most;
+    const int rows = (max_new > most ? most : max_new) * G;
+    p.few = scored_short_plan(dtype, n_seqs, rows > most ? most : rows, max_keys, nkv, d);
+    p.floats += p.few.floats;
+  }
+  return p;
+}
+
+// Kilobytes of scratch that nhv_attention_scored wants for a call of these sizes.
+NHV_API int nhv_attention_scored_kilobytes(int dtype, int n_seqs, int n_tokens, int min_new, int max_new, int max_kv_len, int nq, int nkv, int d) {
+  if (n_seqs <= 0 || nkv <= 0 || nq < nkv || d <= 0) return 0;
+  return (int)(scored_plan(dtype, n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d).floats * sizeof(float) / 1024 + 1);
+}
+
 NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* out, int out_stride, const void* kv_pages,
                                  const float* scores, float* scores_out, int* births, const int* positions, const int* block_table,
                                  int bt_stride, const int* cu_q, const int* kv_len, int n_seqs, int n_tokens, int min_new, int max_new,
                                  int max_kv_len, int nq, int nkv, int d, int page_size, int n_pages, float scale, const float* sinks,
-                                 float softcap, float* lse, cudaStream_t stream) {
+                                 float softcap, float* work, int work_kilobytes, cudaStream_t stream) {
   NHV_REQUIRE(dtype == NHV_F32 || dtype == NHV_BF16, "scored attention: unknown type %d", dtype);
   NHV_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "scored attention: %d query heads do not divide into %d KV heads", nq, nkv);
   NHV_REQUIRE(d > 0 && d <= SA_MAX_D, "scored attention: head size %d is not in 1..%d", d, SA_MAX_D);
@@ -227,7 +211,21 @@ NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* o
   NHV_REQUIRE(softcap >= 0.f, "scored attention: the cap on the scores is positive");
   NHV_REQUIRE(!births == !positions || n_tokens == 0, "scored attention: births and positions go together");
   if (n_seqs == 0 || max_kv_len == 0) return 0;
-  const ScoredArgs a{q, out, kv_pages, scores, scores_out, births, positions, block_table, cu_q, kv_len, sinks, lse,
-                     q_stride, out_stride, bt_stride, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages, max_kv_len, scale, softcap};
+  NHV_REQUIRE(n_seqs <= 65535, "scored attention: %d requests are beyond the grid's reach", n_seqs);
+  // rows that 16-byte loads cannot take go to the kernels of this file
+  const bool wide = d % 8 == 0 && q_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)kv_pages % 16 == 0;
+  const ScoredPlan plan = scored_plan(dtype, n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d);
+  NHV_REQUIRE((size_t)work_kilobytes * 1024 >= plan.floats * sizeof(float) && (uintptr_t)work % 16 == 0, "scored attention: %d kilobytes of scratch are too few",
+              work_kilobytes);
+  ScoredArgs a{q, out, kv_pages, scores, scores_out, births, positions, block_table, cu_q, kv_len, sinks, work,
+               q_stride, out_stride, bt_stride, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages, max_kv_len, 0, 0x7fffffff, scale, softcap};
+  if (wide && plan.short_rows >= 0) {
+    a.max_rows = plan.short_rows;
+    const int rc = scored_short_launch(dtype, a, plan.few, work + ((size_t)n_tokens * nq + 3) / 4 * 4, stream);
+    if (rc) return rc;
+    if (max_new * (nq / nkv) <= plan.short_rows) return 0;
+    a.min_rows = plan.short_rows + 1;
+    a.max_rows = 0x7fffffff;
+  }
   return dtype == NHV_F32 ? launch_simt<float>(a, max_kv_len, stream) : launch_simt<__nv_bfloat16>(a, max_kv_len, stream);
 }

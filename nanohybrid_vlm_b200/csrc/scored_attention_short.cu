@@ -1,0 +1,456 @@
+// Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), up to 16 of
+// them: decoded tokens, drafts.  All the work is to read the keys and values once.
+//
+// First kernel: a block per (part of a request's keys, KV head, request), its warps independent of one another.  A warp takes 16
+// keys at a time straight from the pages into registers and forms S^T = K Q^T (m16n8k16, the 16 keys as M, up to 8 rows as N) and
+// O^T += V^T P^T.  No shared memory is between the pages and the products: which element of a head stands at which index of the
+// product is free as long as both operands agree, so a lane takes 16 consecutive bytes of a row and its registers are the fragment
+// as they are.  For V^T two keys' elements have to share a register, which one byte permutation each does.  The next keys'
+// loads are sent as soon as the products have used the registers; the next tile's page is looked up one tile ahead.
+//   P goes into the second product as two bfloat16 parts, the rounded value and what the rounding left (an error of 2^-16 where
+//   one part has 2^-9): the tensor pipe is idle most of the time here.
+//   The running maximum moves only when it grows by more than 2^8, so that most tiles leave the sums as they are.
+//   The warps' sums meet in shared memory; the block leaves one partial sum (fp32) and the scores of its keys.
+// Second kernel: the parts' sums are joined, a block per (request, KV head) for the output and blocks of keys for the weights: a
+// thread per key adds exp2(score - log-sum) over the rows.  Two kernels instead of one that reads the keys twice: a score is 4
+// bytes a row where a key is 2 d.
+//
+// A key out of sight may hold anything: its score is replaced, its value not loaded.  Where only some of a request's rows see a
+// key (several new tokens), the second product is made token by token with the values that the token sees.
+#include "nhv_scored.cuh"
+
+namespace {
+
+constexpr int SH_WARPS = 4, SH_THREADS = SH_WARPS * 32, FIN_THREADS = 256;
+constexpr float SH_GROW = 8.0f;                  // log2 units
+constexpr size_t SH_MOST_SCORES = (size_t)1 << 28;        // floats of scores kept at once (1 GiB)
+
+struct ShortArgs {
+  ScoredArgs a;
+  NhvScoreCap cap;
+  float* kept;              // [group][nkv][keys][rows] scores in log2 units
+  float* part_o;            // [group][nkv][splits][rows][d]
+  float* part_ml;           // [group][nkv][splits][rows][2]: reference and sum
+  size_t keys;
+  int rows, split_keys, splits, first_seq;
+};
+
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {      // an 8 x 8 tile of 16-bit numbers over the warp
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ float low_of(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float high_of(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// DB: blocks of 64 elements of a head; NT: blocks of 8 rows; BY16: pages hold a multiple of 16 keys.
+template <int DB, int NT, bool BY16>
+__global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short_kernel(const ShortArgs w) {
+  extern __shared__ float smem[];                 // [warps][rows][d + 2] sums, then [warps][rows][2]
+  const ScoredArgs& a = w.a;
+  pdl_prologue();
+  const int seq = w.first_seq + blockIdx.z, kvh = blockIdx.y, G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), R = n * G, d = a.d;
+  const int begin = blockIdx.x * w.split_keys, end = min(total, begin + w.split_keys);
+  if (begin >= end || n <= 0 || !scored_takes(a, n)) return;
+  const int ra = lane >> 2, rc = lane & 3;
+  const __nv_bfloat16* q = (const __nv_bfloat16*)a.q;
+  const __nv_bfloat16* pages = (const __nv_bfloat16*)a.pages;
+  const int* table = a.block_table + (size_t)seq * a.bt_stride;
+  const size_t v_plane = (size_t)a.nkv * a.page_size * d;
+
+  // the product's B operand: row ra (+ 8), elements 32 i + 8 rc ..
+  uint4 qf[NT][2 * DB];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = t * 8 + ra;
+#pragma unroll
+    for (int i = 0; i < 2 * DB; ++i) {
+      const int e = 32 * i + 8 * rc;
+      qf[t][i] = make_uint4(0, 0, 0, 0);
+      if (r < R && e < d) qf[t][i] = *reinterpret_cast<const uint4*>(q + (size_t)(first + r / G) * a.q_stride + (size_t)(kvh * G + r % G) * d + e);
+    }
+  }
+  float o[NT][DB][4][4];                          // O^T: element 64 b + 8 ra + 2 u (+ 1), rows 2 rc (+ 1)
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t][0] = m[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o[t][b][u][0] = o[t][b][u][1] = o[t][b][u][2] = o[t][b][u][3] = 0.f;
+  }
+  uint4 kr[2][2 * DB], vr[4][DB];
+  // where a tile's keys lie: the page of the tile (BY16), looked up a tile ahead of its loads
+  auto page_at = [&](int j) -> int {
+    const int page = j < end ? table[j / a.page_size] : -1;
+    return page < a.n_pages ? page : -1;
+  };
+  auto row_at = [&](int j, int tile_page, int tile_off, int in_tile) -> const __nv_bfloat16* {
+    int page = tile_page, off = tile_off + in_tile;
+    if (!BY16) {
+      page = page_at(j);
+      off = j % a.page_size;
+    }
+    return page < 0 || j >= end ? nullptr : pages + (((size_t)page * 2 * a.nkv + kvh) * a.page_size + off) * d;
+  };
+  auto load_keys = [&](int j0, int page, int off) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const __nv_bfloat16* row = row_at(j0 + ra + 8 * h, page, off, ra + 8 * h);
+#pragma unroll
+      for (int i = 0; i < 2 * DB; ++i) {
+        const int e = 32 * i + 8 * rc;
+        kr[h][i] = row && e < d ? load16(row + e) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  auto load_values = [&](int j0, int page, int off) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int in_tile = 2 * rc + (h & 1) + 8 * (h >> 1);
+      const __nv_bfloat16* row = row_at(j0 + in_tile, page, off, in_tile);
+#pragma unroll
+      for (int b = 0; b < DB; ++b) {
+        const int e = 64 * b + 8 * ra;
+        vr[h][b] = row && e < d ? load16(row + v_plane + e) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  auto second_product = [&](const uint32_t (&p)[NT][2][2]) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b) {
+      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vr[0][b]);
+      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vr[1][b]);
+      const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vr[2][b]);
+      const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vr[3][b]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t a0 = __byte_perm(v0[u], v1[u], 0x5410), a1 = __byte_perm(v0[u], v1[u], 0x7632);
+        const uint32_t a2 = __byte_perm(v2[u], v3[u], 0x5410), a3 = __byte_perm(v2[u], v3[u], 0x7632);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          mma16816(o[t][b][u], a0, a1, a2, a3, p[t][0][0], p[t][0][1]);
+          mma16816(o[t][b][u], a0, a1, a2, a3, p[t][1][0], p[t][1][1]);
+        }
+      }
+    }
+  };
+  float* kept = w.kept + ((size_t)blockIdx.z * a.nkv + kvh) * w.keys * w.rows;
+  const float scale_log2 = w.cap.in != 0.f ? 1.0f : a.scale * SA_LOG2E;
+
+  const int step = 16 * SH_WARPS;
+  int j0 = begin + 16 * warp;
+  int page = page_at(j0), off = BY16 ? j0 % a.page_size : 0;
+  int page_next = page_at(j0 + step);
+  if (j0 < end) {
+    load_keys(j0, page, off);
+    load_values(j0, page, off);
+  }
+  for (; j0 < end; j0 += step) {
+    float s[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * DB; ++i) {
+        mma16816(s[t], kr[0][i].x, kr[1][i].x, kr[0][i].y, kr[1][i].y, qf[t][i].x, qf[t][i].y);
+        mma16816(s[t], kr[0][i].z, kr[1][i].z, kr[0][i].w, kr[1][i].w, qf[t][i].z, qf[t][i].w);
+      }
+    }
+    const int at_page = page, off_next = BY16 ? (j0 + step) % a.page_size : 0;
+    page = page_next;
+    off = off_next;
+    load_keys(j0 + step, page, off);
+    page_next = page_at(j0 + 2 * step);
+
+    // scores in log2 units; -inf for what a row does not see
+    const bool edge = j0 + 15 > total - n;
+    if (w.cap.in != 0.f) nhv_cap_tile(s, w.cap);
+    bool grow = false;
+    float top[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[t][e] *= scale_log2;
+      if (edge || (BY16 && at_page < 0) || !BY16 || j0 + 16 > end) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + ra + 8 * (e >> 1), r = t * 8 + 2 * rc + (e & 1);
+          bool sees = j < end && r < R && j <= total - n + r / G;
+          if (BY16) sees = sees && at_page >= 0;
+          else sees = sees && page_at(j) >= 0;
+          if (!sees) s[t][e] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = fmaxf(s[t][e], s[t][2 + e]);
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
+        top[t][e] = x;
+        grow |= x > m[t][e] + SH_GROW;
+      }
+      if (t * 8 + 2 * rc < w.rows) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (j0 + ra + 8 * h < end) *reinterpret_cast<float2*>(kept + (size_t)(j0 + ra + 8 * h) * w.rows + t * 8 + 2 * rc) = make_float2(s[t][2 * h], s[t][2 * h + 1]);
+      }
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (top[t][e] > m[t][e] + SH_GROW) {
+            const float alpha = scored_exp2(m[t][e] - top[t][e]);      // 0 when the row had seen nothing
+            m[t][e] = top[t][e];
+            l[t][e] *= alpha;
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                o[t][b][u][e] *= alpha;
+                o[t][b][u][2 + e] *= alpha;
+              }
+          }
+        }
+    }
+    uint32_t p[NT][2][2];                          // [rounded, what that left][keys 0-7, 8-15]
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          x[e] = scored_exp2(s[t][2 * h + e] - (m[t][e] == -INFINITY ? 0.f : m[t][e]));
+          l[t][e] += x[e];
+        }
+        const uint32_t hi = pack2(x[0], x[1]);
+        p[t][0][h] = transposed(hi);
+        p[t][1][h] = transposed(pack2(x[0] - low_of(hi), x[1] - high_of(hi)));
+      }
+    if (!edge || n == 1) {
+      second_product(p);
+    } else {
+      // token by token, with the values up to its own key
+      for (int tok = 0; tok < n; ++tok) {
+        const int hi_key = total - n + tok;
+        if (tok + 1 < n && hi_key < j0) continue;             // earlier tokens see nothing of this tile
+        uint32_t own[NT][2][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const bool mine = (t * 8 + ra) / G == tok;
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) own[t][k][h] = mine ? p[t][k][h] : 0u;
+        }
+        uint4 all[4][DB];
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+          for (int b = 0; b < DB; ++b) {
+            all[h][b] = vr[h][b];
+            if (j0 + 2 * rc + (h & 1) + 8 * (h >> 1) > hi_key) vr[h][b] = make_uint4(0, 0, 0, 0);
+          }
+        second_product(own);
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+          for (int b = 0; b < DB; ++b) vr[h][b] = all[h][b];
+      }
+    }
+    load_values(j0 + step, page, off);
+  }
+
+  // the warps' sums joined
+  const int row_len = d + 2;
+  float* so = smem;
+  float* sml = smem + SH_WARPS * w.rows * row_len;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[t][e];
+#pragma unroll
+      for (int k = 4; k < 32; k <<= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
+      const int r = t * 8 + 2 * rc + e;
+      if (r < w.rows) {
+        if (ra == 0) {
+          sml[(warp * w.rows + r) * 2] = m[t][e];
+          sml[(warp * w.rows + r) * 2 + 1] = x;
+        }
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int at = 64 * b + 8 * ra + 2 * u;
+            if (at < d) *reinterpret_cast<float2*>(so + (warp * w.rows + r) * row_len + at) = make_float2(o[t][b][u][e], o[t][b][u][2 + e]);
+          }
+      }
+    }
+  __syncthreads();
+  const size_t part = (((size_t)blockIdx.z * a.nkv + kvh) * w.splits + blockIdx.x) * w.rows;
+  for (int i = threadIdx.x; i < R * (d / 2); i += SH_THREADS) {
+    const int r = i / (d / 2), c = 2 * (i - r * (d / 2));
+    float ref = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < SH_WARPS; ++k) ref = fmaxf(ref, sml[(k * w.rows + r) * 2]);
+    const float use = ref == -INFINITY ? 0.f : ref;
+    float sum = 0.f;
+    float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < SH_WARPS; ++k) {
+      const float f = scored_exp2(sml[(k * w.rows + r) * 2] - use);
+      const float2 x = *reinterpret_cast<const float2*>(so + (k * w.rows + r) * row_len + c);
+      sum = fmaf(f, sml[(k * w.rows + r) * 2 + 1], sum);
+      v.x = fmaf(f, x.x, v.x);
+      v.y = fmaf(f, x.y, v.y);
+    }
+    *reinterpret_cast<float2*>(w.part_o + (part + r) * d + c) = v;
+    if (c == 0) *reinterpret_cast<float2*>(w.part_ml + (part + r) * 2) = make_float2(ref, sum);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(FIN_THREADS) scored_short_finish_kernel(const ShortArgs w, const int key_blocks, const int per_block) {
+  __shared__ float s_ref[16], s_inv[16], s_lse[16];
+  const ScoredArgs& a = w.a;
+  pdl_prologue();
+  const int seq = w.first_seq + blockIdx.z, kvh = blockIdx.y, G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), R = n * G, d = a.d;
+  if (!scored_takes(a, n)) return;
+  const bool output = blockIdx.x == key_blocks;
+  if (!output && blockIdx.x * per_block >= total) return;
+  const int parts = (total + w.split_keys - 1) / w.split_keys;
+  const size_t part = ((size_t)blockIdx.z * a.nkv + kvh) * w.splits * w.rows;
+  for (int r = warp; r < R; r += FIN_THREADS / 32) {
+    float ref = -INFINITY, sum = 0.f;
+    for (int k = lane; k < parts; k += 32) ref = fmaxf(ref, w.part_ml[(part + (size_t)k * w.rows + r) * 2]);
+    ref = warp_max(ref);
+    const float sink = a.sinks ? a.sinks[kvh * G + r % G] * SA_LOG2E : -INFINITY;
+    ref = fmaxf(ref, sink);
+    const float use = ref == -INFINITY ? 0.f : ref;
+    for (int k = lane; k < parts; k += 32) {
+      const float2 ml = *reinterpret_cast<const float2*>(w.part_ml + (part + (size_t)k * w.rows + r) * 2);
+      sum = fmaf(scored_exp2(ml.x - use), ml.y, sum);
+    }
+    sum = warp_sum(sum) + scored_exp2(sink - use);
+    if (lane == 0) {
+      s_ref[r] = use;
+      s_inv[r] = sum == 0.f ? 0.f : 1.0f / sum;
+      s_lse[r] = sum == 0.f ? INFINITY : use + log2f(sum);
+    }
+  }
+  __syncthreads();
+  if (output) {
+    T* out = (T*)a.out;
+    for (int i = threadIdx.x; i < R * d; i += FIN_THREADS) {
+      const int r = i / d, c = i - r * d;
+      float v = 0.f;
+      for (int k = 0; k < parts; ++k) {
+        const size_t at = part + (size_t)k * w.rows + r;
+        v = fmaf(scored_exp2(w.part_ml[at * 2] - s_ref[r]), w.part_o[at * d + c], v);
+      }
+      out[(size_t)(first + r / G) * a.out_stride + (size_t)(kvh * G + r % G) * d + c] = from_f32<T>(v * s_inv[r]);
+    }
+    return;
+  }
+  const float* kept = w.kept + ((size_t)blockIdx.z * a.nkv + kvh) * w.keys * w.rows;
+  for (int j = blockIdx.x * per_block + threadIdx.x; j < min(total, (int)(blockIdx.x + 1) * per_block); j += FIN_THREADS) {
+    float sum = 0.f;
+    for (int r = 0; r < R; r += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(kept + (size_t)j * w.rows + r);
+      sum += scored_exp2(x.x - s_lse[r]);
+      if (r + 1 < R) sum += scored_exp2(x.y - s_lse[r + 1]);
+    }
+    store_weight(a, seq, first, kvh, j, j - (total - n), sum);
+  }
+}
+
+template <int DB, int NT>
+int launch_split(const ShortArgs& w, dim3 grid, size_t smem, cudaStream_t stream) {
+  static std::atomic<uint64_t> done16{0}, done{0};
+  if (w.a.page_size % 16 == 0) {
+    NHV_CUDA(nhv_allow_smem((const void*)scored_short_kernel<DB, NT, true>, 100 * 1024, done16), "scored attention");
+    NHV_CUDA(nhv_launch(scored_short_kernel<DB, NT, true>, grid, SH_THREADS, smem, stream, w), "scored attention");
+  } else {
+    NHV_CUDA(nhv_allow_smem((const void*)scored_short_kernel<DB, NT, false>, 100 * 1024, done), "scored attention");
+    NHV_CUDA(nhv_launch(scored_short_kernel<DB, NT, false>, grid, SH_THREADS, smem, stream, w), "scored attention");
+  }
+  return 0;
+}
+
+}  // namespace
+
+bool scored_short_takes(int dtype, int rows, int d) {
+  // 16 rows of heads above 128 would need more registers than a thread has
+  return dtype == NHV_BF16 && d % 8 == 0 && d <= SA_MAX_D && rows <= (d <= 128 ? 16 : 8);
+}
+
+ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d) {
+  ShortPlan p = {};
+  p.rows = (max_rows + 1) / 2 * 2;
+  // Four times as many blocks as run at once (three an SM), so that requests of unlike length even out, and no fewer than 64 keys a
+  // block (a tile per warp).
+  const long long keys = (long long)n_seqs * nkv * max_keys, want = (keys + 4 * 444 - 1) / (4 * 444);
+  p.split_keys = (int)((want + 63) / 64 * 64);
+  if (p.split_keys < 64) p.split_keys = 64;
+  p.splits = (max_keys + p.split_keys - 1) / p.split_keys;
+  p.keys = (size_t)p.splits * p.split_keys;
+  const size_t per_request = (size_t)nkv * p.rows * (p.keys + (size_t)p.splits * (d + 2));
+  p.group = (int)(SH_MOST_SCORES / per_request);
+  if (p.group < 1) p.group = 1;
+  if (p.group > n_seqs) p.group = n_seqs;
+  p.floats = per_request * p.group;
+  return p;
+}
+
+int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* work, cudaStream_t stream) {
+  ShortArgs w = {};
+  w.a = a;
+  w.cap = nhv_score_cap(a.scale, a.softcap);
+  w.keys = plan.keys;
+  w.rows = plan.rows;
+  w.split_keys = plan.split_keys;
+  w.splits = plan.splits;
+  const size_t pairs = (size_t)plan.group * a.nkv;
+  w.kept = work;
+  w.part_o = w.kept + pairs * plan.keys * plan.rows;
+  w.part_ml = w.part_o + pairs * plan.splits * plan.rows * a.d;
+  const int db = (a.d + 63) / 64;
+  const size_t smem = sizeof(float) * SH_WARPS * plan.rows * (a.d + 4);
+  const int per_block = plan.keys > 4096 ? 1024 : 256, key_blocks = (a.max_keys + per_block - 1) / per_block;
+  for (int s = 0; s < a.n_seqs; s += plan.group) {
+    w.first_seq = s;
+    const int count = a.n_seqs - s < plan.group ? a.n_seqs - s : plan.group;
+    const dim3 grid(plan.splits, a.nkv, count);
+    int rc = 0;
+    if (plan.rows <= 8)
+      rc = db == 1 ? launch_split<1, 1>(w, grid, smem, stream) : db == 2 ? launch_split<2, 1>(w, grid, smem, stream)
+           : db == 3 ? launch_split<3, 1>(w, grid, smem, stream) : launch_split<4, 1>(w, grid, smem, stream);
+    else
+      rc = db == 1 ? launch_split<1, 2>(w, grid, smem, stream) : launch_split<2, 2>(w, grid, smem, stream);
+    if (rc) return rc;
+    NHV_CUDA(nhv_launch(scored_short_finish_kernel<__nv_bfloat16>, dim3(key_blocks + 1, a.nkv, count), FIN_THREADS, 0, stream, w, key_blocks, per_block),
+             "scored attention");
+  }
+  return 0;
+}

@@ -1240,11 +1240,13 @@ def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs
     elif scores_out.shape != scores.shape or scores_out.dtype != torch.float32 or not scores_out.is_contiguous():
         raise KernelError(f"scores_out is float32 of the scores' shape {tuple(scores.shape)} and contiguous")
     _need_cuda(scores_out)
-    lse = torch.empty(T * nq, dtype=torch.float32, device=q.device)
-    call("nhv_attention_scored", dtype_code(q), q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv_pages.data_ptr(),
+    dt = dtype_code(q)
+    kilobytes = library.load_library().nhv_attention_scored_kilobytes(dt, n_seqs, T, min_new, max_new, max_kv_len, nq, nkv, head_dim)
+    work = torch.empty(kilobytes * 256, dtype=torch.float32, device=q.device)
+    call("nhv_attention_scored", dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv_pages.data_ptr(),
          scores.data_ptr(), scores_out.data_ptr(), _ptr(births), _ptr(positions), block_table.data_ptr(), block_table.stride(0),
          cu_q.data_ptr(), kv_len.data_ptr(), n_seqs, T, min_new, max_new, max_kv_len, nq, nkv, head_dim, page_size, n_pages, float(scale),
-         _ptr(sinks), float(softcap or 0.0), lse.data_ptr(), stream_ptr())
+         _ptr(sinks), float(softcap or 0.0), work.data_ptr(), kilobytes, stream_ptr())
 
 
 def select_keys(sources, targets, scores, births, block_table, kv_len, seen, budgets, n_seqs: int, max_kv_len: int, keep_first: int,
