@@ -78,3 +78,14 @@ bool scored_short_takes(int dtype, int rows, int d);
 ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d);
 // The requests with a.min_rows to a.max_rows rows: output, scores and births.  `work`: plan.floats floats.
 int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* work, cudaStream_t stream);
+
+// ---- requests with many rows, bfloat16 (scored_attention_tcgen05.cu)
+struct LongPlan {
+  int splits, split_tiles;  // parts of a request's keys in the rows' pass, tiles of keys of one part
+  int chunks, chunk_tiles;  // parts of a request's rows in the keys' pass, tiles of rows of one part
+  size_t keys;              // places for keys of a (request, KV head)
+  size_t floats;            // of scratch
+};
+bool scored_long_takes(int dtype, int nq, int nkv, int d, int page_size, float scale);
+LongPlan scored_long_plan(int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d);
+int scored_long_launch(ScoredArgs a, const LongPlan& plan, float* work, cudaStream_t stream);

@@ -170,31 +170,42 @@ int launch_simt(const ScoredArgs& a, int max_kv_len, cudaStream_t stream) {
 }  // namespace
 
 // What a call needs beside its arguments, and which kernels take which requests: those of up to `short_rows` rows the kernels of
-// scored_attention_short.cu, the others the ones of this file.
+// scored_attention_short.cu, the others the ones of scored_attention_tcgen05.cu, and what neither takes the kernels of this file.
 struct ScoredPlan {
   int short_rows;           // -1: none go that way
+  bool many;                // requests above that go to the tcgen05 kernels
   ShortPlan few;
+  LongPlan rest;
   size_t floats;            // of scratch
 };
 
-static ScoredPlan scored_plan(int dtype, int n_seqs, int n_tokens, int min_new, int max_new, int max_keys, int nq, int nkv, int d) {
+static ScoredPlan scored_plan(int dtype, int n_seqs, int n_tokens, int min_new, int max_new, int max_keys, int nq, int nkv, int d, int page_size,
+                              float scale) {
   ScoredPlan p = {};
   p.short_rows = -1;
-  p.floats = ((size_t)n_tokens * nq + 3) / 4 * 4;
   const int G = nq / nkv, most = d <= 128 ? 16 : 8;
+  size_t floats = 0;
   if (scored_short_takes(dtype, min_new * G, d)) {
     p.short_rows = most;
-    const int rows = (max_new > most ? most : max_new) * G;
+    const int rows = max_new > most ? most : max_new * G;
     p.few = scored_short_plan(dtype, n_seqs, rows > most ? most : rows, max_keys, nkv, d);
-    p.floats += p.few.floats;
+    floats = p.few.floats;
   }
+  p.many = max_new > most || max_new * G > p.short_rows;
+  if (p.many) p.many = scored_long_takes(dtype, nq, nkv, d, page_size, scale);
+  if (p.many) {
+    p.rest = scored_long_plan(n_seqs, n_tokens, max_new, max_keys, nq, nkv, d);
+    if (p.rest.floats > floats) floats = p.rest.floats;      // one after the other in the same scratch
+  }
+  p.floats = ((size_t)n_tokens * nq + 3) / 4 * 4 + floats;
   return p;
 }
 
 // Kilobytes of scratch that nhv_attention_scored wants for a call of these sizes.
-NHV_API int nhv_attention_scored_kilobytes(int dtype, int n_seqs, int n_tokens, int min_new, int max_new, int max_kv_len, int nq, int nkv, int d) {
-  if (n_seqs <= 0 || nkv <= 0 || nq < nkv || d <= 0) return 0;
-  return (int)(scored_plan(dtype, n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d).floats * sizeof(float) / 1024 + 1);
+NHV_API int nhv_attention_scored_kilobytes(int dtype, int n_seqs, int n_tokens, int min_new, int max_new, int max_kv_len, int nq, int nkv, int d,
+                                           int page_size, float scale) {
+  if (n_seqs <= 0 || nkv <= 0 || nq < nkv || d <= 0 || page_size <= 0) return 0;
+  return (int)(scored_plan(dtype, n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d, page_size, scale).floats * sizeof(float) / 1024 + 1);
 }
 
 NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* out, int out_stride, const void* kv_pages,
@@ -213,19 +224,22 @@ NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* o
   if (n_seqs == 0 || max_kv_len == 0) return 0;
   NHV_REQUIRE(n_seqs <= 65535, "scored attention: %d requests are beyond the grid's reach", n_seqs);
   // rows that 16-byte loads cannot take go to the kernels of this file
-  const bool wide = d % 8 == 0 && q_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)kv_pages % 16 == 0;
-  const ScoredPlan plan = scored_plan(dtype, n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d);
+  const bool wide = d % 8 == 0 && q_stride % 8 == 0 && out_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 &&
+                    (uintptr_t)kv_pages % 16 == 0;
+  const ScoredPlan plan = scored_plan(dtype, n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d, page_size, scale);
   NHV_REQUIRE((size_t)work_kilobytes * 1024 >= plan.floats * sizeof(float) && (uintptr_t)work % 16 == 0, "scored attention: %d kilobytes of scratch are too few",
               work_kilobytes);
   ScoredArgs a{q, out, kv_pages, scores, scores_out, births, positions, block_table, cu_q, kv_len, sinks, work,
                q_stride, out_stride, bt_stride, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages, max_kv_len, 0, 0x7fffffff, scale, softcap};
+  float* scratch = work + ((size_t)n_tokens * nq + 3) / 4 * 4;
   if (wide && plan.short_rows >= 0) {
     a.max_rows = plan.short_rows;
-    const int rc = scored_short_launch(dtype, a, plan.few, work + ((size_t)n_tokens * nq + 3) / 4 * 4, stream);
+    const int rc = scored_short_launch(dtype, a, plan.few, scratch, stream);
     if (rc) return rc;
-    if (max_new * (nq / nkv) <= plan.short_rows) return 0;
+    if (max_new <= plan.short_rows && max_new * (nq / nkv) <= plan.short_rows) return 0;
     a.min_rows = plan.short_rows + 1;
     a.max_rows = 0x7fffffff;
   }
+  if (wide && plan.many) return scored_long_launch(a, plan.rest, scratch, stream);
   return dtype == NHV_F32 ? launch_simt<float>(a, max_kv_len, stream) : launch_simt<__nv_bfloat16>(a, max_kv_len, stream);
 }

@@ -1,0 +1,859 @@
+// Attention with scored keys for requests that bring many rows (a row: a new token and a query head of one KV head), bfloat16, on
+// the 5th-generation tensor cores: tcgen05.mma with the accumulators in tensor memory, operands brought by TMA.
+//
+// The rows' pass: O = softmax(Q K^T) V, and each row's log-sum.  A block owns two tiles of up to 128 rows (whole tokens; heads above
+// 128: one tile) of a KV head and walks the keys in tiles of 128 (heads above 128: 64).  Warp 0, one lane: TMA, keys and
+// values through one ring of stages, straight from the pages, in boxes of as many rows as divide the page size and 128.
+// Warp 1, one lane: the MMAs, S = Q K^T and O += P V.  Warps 4-7 and 8-11: one thread per row of the first and the second tile;
+// it reads its row of S, takes maximum and exponentials, writes P (bfloat16) over S.  While one tile is in its softmax the other's
+// products run.  The products of a tile run in order, so a finished S says that the P V before it is finished too: P may be
+// written and O rescaled without another wait.  O is rescaled only when a row's maximum grew by more than 2^8.
+//   Where the grid would leave SMs idle the keys are split over blocks, whose sums a small kernel joins.
+// The keys' pass: w[j] = sum over the rows that see j of exp2(s - log-sum).  S^T = K Q^T with the keys as M: a lane of tensor
+// memory is a key and its columns are rows, so a thread adds up its key's weights with no exchange at all.  The block's keys stay
+// in shared memory, the tiles of rows stream through a ring.  Under the causal mask a request's first keys are seen by all rows
+// and its last by few; so the rows are cut into chunks, a block per (key tile, chunk), and the chunks' sums added in their order.
+// Making S a second time costs 2 D operations a pair where keeping P would write and read 4 bytes a pair, eight times the time.
+//
+// A key out of sight may hold anything.  Its score is replaced.  Its value would reach the rows that do not see it as 0 times no
+// number, so tiles of which some row sees a part have their values looked through: what is not finite is taken out of shared
+// memory, and the rows that do see it get it back at the end, from the pages.
+//
+// Every wait on an mbarrier is bounded: one that runs out sets the file's error word, the roles leave their loops, the producer
+// waits (bounded) for its copies in flight, and the block frees its tensor memory and returns.
+#define NHV_WAIT_LIMIT (1u << 22)
+#include "nhv_async.cuh"
+#include "nhv_scored.cuh"
+
+namespace {
+
+typedef __nv_bfloat16 bf16;
+constexpr int BM = 128;                          // rows of a tile = lanes of tensor memory
+constexpr float RESCALE_STEP = 8.0f;             // log2 units
+constexpr int SMS = 148;
+
+template <int DB> struct Rows {                  // DB: blocks of 64 elements (128 bytes) of a head
+  static constexpr int NQ = DB <= 2 ? 2 : 1;     // tiles of rows a block
+  static constexpr int BN = DB <= 2 ? 128 : 64;  // keys of a tile
+  static constexpr int THREADS = 128 + NQ * 128;
+  static constexpr int Q_BYTES = DB * BM * 128, STAGE = DB * BN * 128;
+  static constexpr int STAGES = DB == 1 ? 8 : 5;
+  static constexpr int SMEM = 1024 + 1024 + NQ * Q_BYTES + STAGES * STAGE;       // barriers and flags, alignment, tiles
+  static constexpr uint32_t S_COL = 0, O_COL = NQ * BN;
+  static constexpr uint32_t TMEM_COLS = 512;
+};
+template <int DB> struct Keys {
+  static constexpr int BN = 128;                 // rows of a tile = columns of S^T
+  static constexpr int THREADS = 192;
+  static constexpr int K_BYTES = DB * BM * 128, STAGE = DB * BN * 128;
+  static constexpr int STAGES = DB == 1 ? 4 : DB == 2 ? 2 : 1;     // two blocks an SM (tensor memory has room for two), above 128 one
+  static constexpr int SMEM = 1024 + 1024 + 1024 + K_BYTES + STAGES * STAGE;
+  static constexpr uint32_t TMEM_COLS = 256;     // two buffers
+};
+
+struct alignas(64) LongArgs {
+  CUtensorMap kv_map;       // the pool as [n_pages * 2 * nkv * page_size, d], boxes of 64 columns x `box` rows
+  CUtensorMap q_map;        // q as [n_tokens, nq, d], boxes of 64 columns x G heads x tokens of a tile
+  ScoredArgs a;
+  NhvScoreCap cap;
+  float scale_log2;
+  float* part_o;            // [splits][nkv][n_tokens * G][d]
+  float* part_ml;           // [splits][nkv][n_tokens * G][2]
+  float* part_w;            // [n_seqs][nkv][chunks][keys]
+  size_t keys;
+  int splits, split_tiles, chunks, chunk_tiles, key_tiles;
+  int tokens, box;          // tokens of a tile of rows; rows of a TMA box of the pages
+};
+
+// ---- tensor memory and tcgen05
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot_in_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(slot_in_smem)), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// The same with the A operand in tensor memory (one row per lane, two bfloat16 per 32-bit column).
+__device__ __forceinline__ void tc_mma_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// 32 consecutive columns of this thread's lane (no wait: tmem_ld_wait() before the values are used)
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t (&r)[32], uint32_t taddr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
+// Shared-memory matrix descriptor, 128-byte swizzle.  K-major operand (Q, K): rows of 128 bytes, groups of 8 rows 1024 bytes apart
+// (stride offset), the leading offset unused.  MN-major operand (V as it lies in the cache: a row of 128 bytes holds 64 elements of
+// one key): the stride offset is the step between groups of 8 keys, the leading offset the step between blocks of 64 elements.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading_bytes, uint32_t stride_bytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)((leading_bytes >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)((stride_bytes >> 4) & 0x3FFF) << 32;
+  d |= (uint64_t)1 << 46;                            // descriptor version of this architecture
+  d |= (uint64_t)2 << 61;                            // 128-byte swizzle
+  return d;
+}
+// Instruction descriptor: bf16 x bf16 -> fp32, A K-major, M x N; B K-major or MN-major.
+__device__ __forceinline__ uint32_t instr_desc(int m, int n, bool b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
+// A pair of bfloat16 with what is not finite taken out; `bad` says whether there was any.
+__device__ __forceinline__ uint32_t finite_pair(uint32_t v, bool& bad) {
+  const bool lo = (v & 0x7f80u) == 0x7f80u, hi = (v & 0x7f800000u) == 0x7f800000u;
+  bad |= lo | hi;
+  return (lo ? 0u : v & 0xffffu) | (hi ? 0u : v & 0xffff0000u);
+}
+// 32 scores capped (see nhv_cap_tile).
+__device__ __forceinline__ void cap32(uint32_t (&sr)[32], const NhvScoreCap& c) {
+  float s[8][4];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i >> 2][i & 3] = __uint_as_float(sr[i]);
+  nhv_cap_tile(s, c);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) sr[i] = __float_as_uint(s[i >> 2][i & 3]);
+}
+
+// Loads `BN` keys or values of a request, from key0 on, into one stage: boxes of p.box rows, which lie in one page each.  Boxes at
+// or behind `total` and those without a page bring some other row of the pool: their scores are replaced and their values cleared.
+template <int DB, int BN>
+__device__ __forceinline__ void load_tile(unsigned char* stage, const LongArgs& p, const int* table, int key0, int total, int kvh, int plane, uint64_t* bar) {
+  mbar_expect_tx(bar, DB * BN * 128);
+  const int step = p.box < BN ? p.box : BN;
+  for (int r = 0; r < BN; r += step) {
+    const int j = key0 + r < total ? key0 + r : total - 1;
+    int page = table[j / p.a.page_size];
+    page = page < 0 || page >= p.a.n_pages ? 0 : page;
+    const int row = ((page * 2 + plane) * p.a.nkv + kvh) * p.a.page_size + (j % p.a.page_size) / step * step;
+#pragma unroll
+    for (int b = 0; b < DB; ++b) tma_load_2d(stage + b * (BN * 128) + r * 128, &p.kv_map, b * 64, row, bar);
+  }
+}
+template <int DB>
+__device__ __forceinline__ void load_rows(unsigned char* stage, const LongArgs& p, int token, int kvh, int G, uint64_t* bar) {
+  mbar_expect_tx(bar, DB * p.tokens * G * 128);
+#pragma unroll
+  for (int b = 0; b < DB; ++b) tma_load_3d(stage + b * (BM * 128), &p.q_map, b * 64, kvh * G, token, bar);
+}
+
+template <int DB>
+__global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kernel(const __grid_constant__ LongArgs p) {
+  using C = Rows<DB>;
+  constexpr int NQ = C::NQ, BN = C::BN, STAGES = C::STAGES;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw);
+  uint64_t* full = bars;                   // [STAGES]
+  uint64_t* empty = bars + 8;              // [STAGES]
+  uint64_t* s_full = bars + 16;            // [NQ]
+  uint64_t* p_ready = bars + 18;           // [NQ]
+  uint64_t* o_full = bars + 20;            // [NQ]
+  uint64_t* q_full = bars + 22;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  int* s_abort = reinterpret_cast<int*>(bars + 25);
+  int* s_missing = reinterpret_cast<int*>(bars + 26);
+  uint32_t* s_bad = reinterpret_cast<uint32_t*>(bars + 32);       // [8 tiles][4]: keys whose values are not all finite
+  const uint32_t raw = smem_u32(smem_raw);
+  unsigned char* tiles = smem_raw + (((raw + 1024 + 1023u) & ~1023u) - raw);
+  unsigned char* q_s = tiles;                          // [NQ][Q_BYTES]
+  unsigned char* kv_s = q_s + NQ * C::Q_BYTES;         // [STAGES][STAGE]
+
+  const ScoredArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int q = 0; q < NQ; ++q) {
+      mbar_init(&s_full[q], 1);
+      mbar_init(&p_ready[q], 128);
+      mbar_init(&o_full[q], 1);
+    }
+    mbar_init(q_full, 1);
+    *s_abort = 0;
+    *s_missing = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&p.kv_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&p.q_map) : "memory");
+  }
+  if (threadIdx.x < 32) s_bad[threadIdx.x] = 0;
+  if (warp == 1) tmem_alloc(tmem_slot, C::TMEM_COLS);
+  pdl_prologue();
+
+  // which request, which rows, which keys: within a request the last tokens, which see the most, come first
+  const int G = a.nq / a.nkv, kvh = blockIdx.x, per_block = NQ * p.tokens;
+  int tile = blockIdx.y;
+  const int seq = find_tile(a, per_block, tile);
+  int first = 0, n = 0, total = 0, t0 = 0, key_begin = 0;
+  int nt[2] = {0, 0};                                  // tiles of keys that the rows of tile q see, of this block's part
+  if (seq >= 0) {
+    first = a.cu_q[seq];
+    n = a.cu_q[seq + 1] - first;
+    total = min(a.kv_len[seq], a.max_keys);
+    t0 = ((n + per_block - 1) / per_block - 1 - tile) * per_block;
+    key_begin = (int)blockIdx.z * p.split_tiles * BN;
+    for (int q = 0; q < NQ; ++q) {
+      const int t_last = min(t0 + (q + 1) * p.tokens, n) - 1;
+      if (t_last < t0 + q * p.tokens) continue;
+      const int seen = total - n + t_last + 1 - key_begin;
+      nt[q] = seen <= 0 ? 0 : min((seen + BN - 1) / BN, p.split_tiles);
+    }
+    const int* table = a.block_table + (size_t)seq * a.bt_stride;
+    const int page_end = (min(key_begin + max(nt[0], nt[1]) * BN, total) + a.page_size - 1) / a.page_size;
+    for (int i = key_begin / a.page_size + threadIdx.x; i < page_end; i += C::THREADS)
+      if (table[i] < 0 || table[i] >= a.n_pages) *s_missing = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int n_tiles = max(nt[0], nt[1]);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0 && n_tiles > 0) {
+      const int* table = a.block_table + (size_t)seq * a.bt_stride;
+      mbar_expect_tx(q_full, (uint32_t)((nt[0] > 0) + (nt[1] > 0)) * DB * p.tokens * G * 128);
+      for (int q = 0; q < NQ; ++q)
+        if (nt[q] > 0) {
+#pragma unroll
+          for (int b = 0; b < DB; ++b) tma_load_3d(q_s + q * C::Q_BYTES + b * (BM * 128), &p.q_map, b * 64, kvh * G, first + t0 + q * p.tokens, q_full);
+        }
+      bool ok = true;
+      int sent = 0;
+      for (int i = 0; i < 2 * n_tiles && ok; ++i) {
+        const int st = i % STAGES;
+        if (i >= STAGES) ok = mbar_wait(&empty[st], (uint32_t)(i / STAGES - 1) & 1, 1);
+        if (!ok) break;
+        load_tile<DB, BN>(kv_s + st * C::STAGE, p, table, key_begin + (i >> 1) * BN, total, kvh, i & 1, &full[st]);
+        sent = i + 1;
+      }
+      if (!ok) {
+        *s_abort = 1;
+        mbar_wait(q_full, 0, 2);
+        for (int i = max(0, sent - STAGES); i < sent; ++i) mbar_wait(&full[i % STAGES], (uint32_t)(i / STAGES) & 1, 2);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0 && n_tiles > 0) {
+      const uint32_t idesc_s = instr_desc(BM, BN, false), idesc_o = instr_desc(BM, DB * 64, true);
+      const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024);
+      const uint64_t k_desc = smem_desc(smem_u32(kv_s), 16, 1024);
+      const uint64_t v_desc = smem_desc(smem_u32(kv_s), BN * 128, 1024);
+      bool ok = mbar_wait(q_full, 0, 3);
+      tc_fence_after();
+      auto stage_ready = [&](int i) { return mbar_wait(&full[i % STAGES], (uint32_t)(i / STAGES) & 1, 4); };
+      auto first_product = [&](int q, int j) {
+        const uint64_t kd = k_desc + (uint64_t)(((2 * j) % STAGES) * (C::STAGE >> 4)), qd = q_desc + (uint64_t)(q * (C::Q_BYTES >> 4));
+#pragma unroll
+        for (int kk = 0; kk < DB * 4; ++kk)
+          tc_mma(tmem_base + C::S_COL + q * BN, qd + (uint64_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
+                 kd + (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+        tc_commit(&s_full[q]);
+      };
+      auto second_product = [&](int q, int j) {
+        const uint64_t vd = v_desc + (uint64_t)(((2 * j + 1) % STAGES) * (C::STAGE >> 4));
+        const uint32_t pa = tmem_base + C::S_COL + q * BN;           // P lies over the first half of S
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)                          // 8 columns of P and 16 rows of V per 16 keys
+          tc_mma_a_tmem(tmem_base + C::O_COL + q * (DB * 64), pa + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), idesc_o,
+                        (j > 0 || kk > 0) ? 1u : 0u);
+      };
+      if (ok) ok = stage_ready(0);
+      if (ok) {
+        tc_fence_after();
+        for (int q = 0; q < NQ; ++q)
+          if (nt[q] > 0) first_product(q, 0);
+        tc_commit(&empty[0]);
+      }
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        bool have_v = false, have_k = false;
+        for (int q = 0; q < NQ && ok; ++q) {
+          if (j >= nt[q]) continue;
+          ok = mbar_wait(&p_ready[q], (uint32_t)j & 1, 5);
+          if (ok && !have_v) ok = stage_ready(2 * j + 1);
+          have_v = true;
+          if (!ok) break;
+          tc_fence_after();
+          second_product(q, j);
+          if (j + 1 < nt[q]) {
+            if (!have_k) ok = stage_ready(2 * j + 2);
+            have_k = true;
+            if (!ok) break;
+            tc_fence_after();
+            first_product(q, j + 1);
+          } else {
+            tc_commit(&o_full[q]);
+          }
+        }
+        if (!ok) break;
+        tc_commit(&empty[(2 * j + 1) % STAGES]);
+        if (j + 1 < n_tiles) tc_commit(&empty[(2 * j + 2) % STAGES]);
+      }
+      if (!ok) *s_abort = 1;
+    }
+    __syncwarp();
+  } else if (warp >= 4 && seq >= 0) {
+    // ------------------------------------------------------------------ softmax and output: a thread per row
+    const int q = (warp - 4) >> 2, quarter = warp & 3, R = quarter * 32 + lane;
+    const int tq = R / G, g = R - tq * G, token = t0 + q * p.tokens + tq;
+    const bool valid = tq < p.tokens && token < n;
+    const int row_hi = valid ? total - n + token : -1;                 // the newest key that the row sees
+    const int all_hi = total - n + t0 + q * p.tokens;                  // every row of the tile sees keys up to here
+    const int tiles_q = nt[q];
+    const bool missing = *s_missing != 0;
+    const int* table = a.block_table + (size_t)seq * a.bt_stride;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_addr = lane_addr + C::S_COL + q * BN, o_addr = lane_addr + C::O_COL + q * (DB * 64);
+    float m = -INFINITY, l = 0.f;
+    // the first tile of which some row of the block does not see all; the notes on values begin there
+    const int first_edge = max(0, total - n + t0 + 1 - key_begin) / BN;
+    bool ok = true, any_bad = false;
+    for (int j = 0; j < tiles_q; ++j) {
+      const int key0 = key_begin + j * BN;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[q], (uint32_t)j & 1, 6));
+      if (!ok) break;
+      tc_fence_after();
+      // the maximum first; scores that a cap or a mask changes go back to where they were
+      const bool edge = key0 + BN - 1 > all_hi;                        // some row does not see some key of the tile
+      const bool masked = edge || missing;
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) {
+        uint32_t sr[32];
+        tmem_ld32_nowait(sr, s_addr + c * 32);
+        tmem_ld_wait();
+        if (p.cap.in != 0.f) cap32(sr, p.cap);
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (key0 + c * 32 + i > row_hi) sr[i] = 0xFF800000u;       // -inf
+          if (missing) {
+            for (int i = 0; i < 32; ++i) {
+              const int at = min(key0 + c * 32 + i, total - 1), page = table[at / a.page_size];
+              const bool gone = page < 0 || page >= a.n_pages;
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (k == i && gone) sr[k] = 0xFF800000u;
+            }
+          }
+        }
+        if (masked || p.cap.in != 0.f) tmem_st32(s_addr + c * 32, sr);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          mx0 = max3(mx0, __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+          mx1 = max3(mx1, __uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3]));
+        }
+      }
+      if (masked || p.cap.in != 0.f) tmem_st_wait();
+      float mx = fmaxf(mx0, mx1);
+      mx *= p.scale_log2;
+      const bool grow = mx > m + RESCALE_STEP;                         // also the first keys a row sees
+      float alpha = 1.f;
+      if (grow) {
+        alpha = scored_exp2(m - mx);                                   // 0 when the row had seen nothing
+        m = mx;
+        l *= alpha;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < DB * 64; c0 += 32) {
+          uint32_t o[32];
+          tmem_ld32_nowait(o, o_addr + c0);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(o_addr + c0, o);
+        }
+      }
+      const float neg_ref = m == -INFINITY ? 0.f : -m;
+      float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+#pragma unroll
+      for (int c = 0; c < BN / 64; ++c) {
+        uint32_t sr[2][32], pk[32];
+        tmem_ld32_nowait(sr[0], s_addr + c * 64);
+        tmem_ld32_nowait(sr[1], s_addr + c * 64 + 32);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+          const float p0 = scored_exp2(fmaf(__uint_as_float(sr[i >> 5][i & 31]), p.scale_log2, neg_ref));
+          const float p1 = scored_exp2(fmaf(__uint_as_float(sr[i >> 5][(i & 31) + 1]), p.scale_log2, neg_ref));
+          const float p2 = scored_exp2(fmaf(__uint_as_float(sr[i >> 5][(i & 31) + 2]), p.scale_log2, neg_ref));
+          const float p3 = scored_exp2(fmaf(__uint_as_float(sr[i >> 5][(i & 31) + 3]), p.scale_log2, neg_ref));
+          pk[i >> 1] = pack_bf16(p0, p1);
+          pk[(i >> 1) + 1] = pack_bf16(p2, p3);
+          l0 += p0; l1 += p1; l2 += p2; l3 += p3;                      // the row's sum in fp32, before the rounding to bfloat16
+        }
+        tmem_st32(s_addr + c * 32, pk);
+      }
+      l += (l0 + l1) + (l2 + l3);
+      tmem_st_wait();
+      if ((masked || key0 + BN - 1 > total - n + t0) && (q == 0 || j >= nt[0])) {
+        // Values that some row of the block does not see: not finite ones, and rows that are no key of the request, are taken out.
+        // The first tile's group does it for both: its product comes first.
+        const int st = (2 * j + 1) % STAGES;
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)((2 * j + 1) / STAGES) & 1, 7));
+        if (!ok) break;
+        unsigned char* v = kv_s + st * C::STAGE;
+        for (int id = threadIdx.x & 127; id < BN * DB * 8; id += 128) {
+          const int row = id / (DB * 8), rem = id - row * (DB * 8), at_key = min(key0 + row, total - 1);
+          uint4* at = reinterpret_cast<uint4*>(v + (rem >> 3) * (BN * 128) + row * 128 + ((rem & 7) << 4));
+          const int page = missing ? table[at_key / a.page_size] : 0;
+          if (key0 + row >= total || page < 0 || page >= a.n_pages) {
+            *at = make_uint4(0, 0, 0, 0);
+          } else if (j >= first_edge) {
+            uint4 x = *at;
+            bool bad = false;
+            x.x = finite_pair(x.x, bad); x.y = finite_pair(x.y, bad); x.z = finite_pair(x.z, bad); x.w = finite_pair(x.w, bad);
+            if (bad) {
+              atomicOr(&s_bad[((j - first_edge) & 7) * 4 + (row >> 5)], 1u << (row & 31));
+              *at = x;
+            }
+          }
+        }
+        fence_async_smem();
+      }
+      tc_fence_before();
+      mbar_arrive(&p_ready[q]);
+    }
+    if (ok && tiles_q > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], 0, 8));
+    if (ok) {
+      tc_fence_after();
+      // the notes on values: made before the products that o_full covers
+      for (int i = 0; i < 32; ++i) any_bad |= *(volatile uint32_t*)&s_bad[i] != 0;
+      const size_t row = (size_t)kvh * a.n_tokens * G + (size_t)(first + token) * G + g;
+      const bool whole = p.splits == 1;
+      float inv = 1.f;
+      if (whole) {
+        const float sink = a.sinks && valid ? a.sinks[kvh * G + g] * SA_LOG2E : -INFINITY;
+        float ref = fmaxf(m, sink);
+        if (ref == -INFINITY) ref = 0.f;
+        // the sink: one more term of the sum
+        const float f = scored_exp2(m - ref), sum = fmaf(l, f, scored_exp2(sink - ref));
+        inv = sum == 0.f ? 0.f : f / sum;
+        if (valid) a.lse[row] = sum == 0.f ? INFINITY : ref + log2f(sum);
+      } else if (valid) {
+        float* ml = p.part_ml + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * 2;
+        ml[0] = m;
+        ml[1] = l;
+      }
+      bf16* dst = (bf16*)a.out + (size_t)(first + token) * a.out_stride + (size_t)(kvh * G + g) * a.d;
+      float* part = p.part_o + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * a.d;
+#pragma unroll 1
+      for (int c0 = 0; c0 < DB * 64; c0 += 32) {
+        uint32_t o[32];
+        if (tiles_q > 0) {
+          tmem_ld32_nowait(o, o_addr + c0);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (valid && any_bad) {
+          // values taken out above, back to the rows that see them: p v, of what is not finite in v
+          for (int w = 0; w < 32; ++w) {
+            for (uint32_t bits = s_bad[w]; bits; bits &= bits - 1) {
+              const int key = key_begin + (first_edge + (w >> 2)) * BN + (w & 3) * 32 + __ffs(bits) - 1;
+              if (key > row_hi) continue;
+              const long long k_at = key_row(a, seq, key, kvh, 0), v_at = key_row(a, seq, key, kvh, 1);
+              if (k_at < 0) continue;
+              const bf16* qr = (const bf16*)a.q + (size_t)(first + token) * a.q_stride + (size_t)(kvh * G + g) * a.d;
+              float s = 0.f;
+              for (int e = 0; e < a.d; ++e) s = fmaf(to_f32(qr[e]), to_f32(((const bf16*)a.pages)[k_at + e]), s);
+              if (a.softcap > 0.f) s = a.softcap * tanhf(s * a.scale / a.softcap) * SA_LOG2E;
+              else s *= p.scale_log2;
+              const float weight = scored_exp2(s + (m == -INFINITY ? 0.f : -m));
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float x = c0 + i < a.d ? to_f32(((const bf16*)a.pages)[v_at + c0 + i]) : 0.f;
+                if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(fmaf(weight, x, __uint_as_float(o[i])));
+              }
+            }
+          }
+        }
+        if (valid && whole) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 x;
+            x.x = pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+            x.y = pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+            x.z = pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+            x.w = pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+            if (c0 + i < a.d) *reinterpret_cast<uint4*>(dst + c0 + i) = x;
+          }
+        } else if (valid) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            if (c0 + i < a.d)
+              *reinterpret_cast<uint4*>(part + c0 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+        __syncwarp();
+      }
+    } else {
+      *s_abort = 1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// The sums of a row's parts joined: a warp per row.
+__global__ void __launch_bounds__(256) scored_rows_join_kernel(const __grid_constant__ LongArgs p) {
+  pdl_prologue();
+  const ScoredArgs& a = p.a;
+  const int G = a.nq / a.nkv, lane = threadIdx.x & 31;
+  const size_t rows = (size_t)a.nkv * a.n_tokens * G, row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int kvh = (int)(row / ((size_t)a.n_tokens * G)), r = (int)(row - (size_t)kvh * a.n_tokens * G), token = r / G, head = kvh * G + r % G;
+  int seq = 0;
+  while (seq + 1 < a.n_seqs && a.cu_q[seq + 1] <= token) ++seq;
+  if (!scored_takes(a, a.cu_q[seq + 1] - a.cu_q[seq])) return;
+  const float sink = a.sinks ? a.sinks[head] * SA_LOG2E : -INFINITY;
+  float ref = sink;
+  for (int s = 0; s < p.splits; ++s) ref = fmaxf(ref, p.part_ml[(s * rows + row) * 2]);
+  if (ref == -INFINITY) ref = 0.f;
+  float sum = scored_exp2(sink - ref);
+  for (int s = 0; s < p.splits; ++s) sum = fmaf(p.part_ml[(s * rows + row) * 2 + 1], scored_exp2(p.part_ml[(s * rows + row) * 2] - ref), sum);
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  bf16* dst = (bf16*)a.out + (size_t)token * a.out_stride + (size_t)head * a.d;
+  for (int c = 2 * lane; c < a.d; c += 64) {
+    float2 v = make_float2(0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+      const float f = scored_exp2(p.part_ml[(s * rows + row) * 2] - ref);
+      const float2 x = *reinterpret_cast<const float2*>(p.part_o + (s * rows + row) * a.d + c);
+      v.x = fmaf(f, x.x, v.x);
+      v.y = fmaf(f, x.y, v.y);
+    }
+    *reinterpret_cast<uint32_t*>(dst + c) = pack_bf16(v.x * inv, v.y * inv);
+  }
+  if (lane == 0) a.lse[row] = sum == 0.f ? INFINITY : ref + log2f(sum);
+}
+
+// The tiles of rows [begin, end) of a request that see keys of tile `key0`, in chunk `chunk`.
+__device__ __forceinline__ void chunk_range(const LongArgs& p, int n, int total, int key0, int chunk, int& begin, int& end) {
+  const int first = max(0, key0 - (total - n)) / p.tokens, tiles = (n + p.tokens - 1) / p.tokens;
+  begin = max(first, chunk * p.chunk_tiles);
+  end = min(tiles, (chunk + 1) * p.chunk_tiles);
+}
+
+template <int DB>
+__global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_keys_tcgen05_kernel(const __grid_constant__ LongArgs p) {
+  using C = Keys<DB>;
+  constexpr int STAGES = C::STAGES;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw);
+  uint64_t* full = bars;                   // [STAGES]
+  uint64_t* empty = bars + 4;              // [STAGES]
+  uint64_t* s_full = bars + 8;             // [2]
+  uint64_t* s_free = bars + 10;            // [2]
+  uint64_t* k_full = bars + 12;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  int* s_abort = reinterpret_cast<int*>(bars + 15);
+  float* s_lse = reinterpret_cast<float*>(smem_raw + 1024);        // [2][128]
+  const uint32_t raw = smem_u32(smem_raw);
+  unsigned char* tiles = smem_raw + (((raw + 2048 + 1023u) & ~1023u) - raw);
+  unsigned char* k_s = tiles;
+  unsigned char* q_s = k_s + C::K_BYTES;               // [STAGES][STAGE]
+
+  const ScoredArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_free[s], 128);
+    }
+    mbar_init(k_full, 1);
+    *s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&p.kv_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&p.q_map) : "memory");
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, C::TMEM_COLS);
+  pdl_prologue();
+
+  const int G = a.nq / a.nkv, kvh = blockIdx.x, seq = blockIdx.z;
+  const int chunk = blockIdx.y / p.key_tiles, key0 = (blockIdx.y - chunk * p.key_tiles) * BM;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
+  int begin = 0, end = 0;
+  const bool mine = key0 < total && scored_takes(a, n);
+  if (mine) chunk_range(p, n, total, key0, chunk, begin, end);
+  const int n_tiles = max(0, end - begin);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0 && n_tiles > 0) {
+      load_tile<DB, BM>(k_s, p, a.block_table + (size_t)seq * a.bt_stride, key0, total, kvh, 0, k_full);
+      bool ok = true;
+      int sent = 0;
+      for (int i = 0; i < n_tiles && ok; ++i) {
+        const int st = i % STAGES;
+        if (i >= STAGES) ok = mbar_wait(&empty[st], (uint32_t)(i / STAGES - 1) & 1, 11);
+        if (!ok) break;
+        load_rows<DB>(q_s + st * C::STAGE, p, first + (begin + i) * p.tokens, kvh, G, &full[st]);
+        sent = i + 1;
+      }
+      if (!ok) {
+        *s_abort = 1;
+        mbar_wait(k_full, 0, 12);
+        for (int i = max(0, sent - STAGES); i < sent; ++i) mbar_wait(&full[i % STAGES], (uint32_t)(i / STAGES) & 1, 12);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && n_tiles > 0) {
+      const uint32_t idesc = instr_desc(BM, C::BN, false);
+      const uint64_t k_desc = smem_desc(smem_u32(k_s), 16, 1024), q_desc = smem_desc(smem_u32(q_s), 16, 1024);
+      bool ok = mbar_wait(k_full, 0, 13);
+      for (int i = 0; i < n_tiles && ok; ++i) {
+        const int st = i % STAGES, buf = i & 1;
+        ok = mbar_wait(&full[st], (uint32_t)(i / STAGES) & 1, 14);
+        if (ok && i >= 2) ok = mbar_wait(&s_free[buf], (uint32_t)(i / 2 - 1) & 1, 15);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t qd = q_desc + (uint64_t)(st * (C::STAGE >> 4));
+#pragma unroll
+        for (int kk = 0; kk < DB * 4; ++kk)
+          tc_mma(tmem_base + buf * C::BN, k_desc + (uint64_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
+                 qd + (uint64_t)(((kk >> 2) * (C::BN * 128) + (kk & 3) * 32) >> 4), idesc, kk > 0 ? 1u : 0u);
+        tc_commit(&empty[st]);
+        tc_commit(&s_full[buf]);
+      }
+      if (!ok) *s_abort = 1;
+    }
+    __syncwarp();
+  } else if (mine) {
+    // ------------------------------------------------------------------ a thread per key
+    const int quarter = warp & 3, at = quarter * 32 + lane, key = key0 + at;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const float* lse = a.lse + ((size_t)kvh * a.n_tokens + first) * G;
+    const int rows = n * G, tile_rows = p.tokens * G;
+    auto lse_of = [&](int i) {                          // of the tile's row `at`
+      const int r = (begin + i) * tile_rows + at;
+      return i < n_tiles && at < tile_rows && r < rows ? lse[r] : INFINITY;
+    };
+    float next = lse_of(0), sum = 0.f;
+    bool ok = true;
+    for (int i = 0; i < n_tiles; ++i) {
+      const int buf = i & 1, t_first = (begin + i) * p.tokens;
+      s_lse[buf * 128 + at] = next;
+      next = lse_of(i + 1);
+      group_sync(1);                                    // all come here in every round, also behind a wait that ran out
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buf], (uint32_t)(i / 2) & 1, 16));
+      if (!ok) continue;
+      tc_fence_after();
+      // rows behind the request's last and those that do not see every key of the tile
+      const bool masked = key0 + BM - 1 > total - n + t_first || (begin + i + 1) * tile_rows > rows || tile_rows < C::BN;
+      // the first column that this key is seen by, and the first behind the rows
+      const int lo = (key - (total - n) - t_first) * G, hi = min(tile_rows, rows - (begin + i) * tile_rows);
+      float w0 = 0.f, w1 = 0.f, w2 = 0.f, w3 = 0.f;
+#pragma unroll
+      for (int c = 0; c < C::BN / 32; ++c) {
+        uint32_t s[32];
+        tmem_ld32_nowait(s, lane_addr + buf * C::BN + c * 32);
+        tmem_ld_wait();
+        if (c == C::BN / 32 - 1) {
+          tc_fence_before();
+          mbar_arrive(&s_free[buf]);
+        }
+        if (p.cap.in != 0.f) cap32(s, p.cap);
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 ls = *reinterpret_cast<const float4*>(s_lse + buf * 128 + c * 32 + k);
+          float x0 = scored_exp2(fmaf(__uint_as_float(s[k]), p.scale_log2, -ls.x)), x1 = scored_exp2(fmaf(__uint_as_float(s[k + 1]), p.scale_log2, -ls.y));
+          float x2 = scored_exp2(fmaf(__uint_as_float(s[k + 2]), p.scale_log2, -ls.z)), x3 = scored_exp2(fmaf(__uint_as_float(s[k + 3]), p.scale_log2, -ls.w));
+          if (masked) {
+            const int r = c * 32 + k;
+            x0 = r >= lo && r < hi ? x0 : 0.f;
+            x1 = r + 1 >= lo && r + 1 < hi ? x1 : 0.f;
+            x2 = r + 2 >= lo && r + 2 < hi ? x2 : 0.f;
+            x3 = r + 3 >= lo && r + 3 < hi ? x3 : 0.f;
+          }
+          w0 += x0; w1 += x1; w2 += x2; w3 += x3;
+        }
+      }
+      sum += (w0 + w1) + (w2 + w3);
+    }
+    if (!ok) *s_abort = 1;
+    else if (key < total) {
+      if (p.chunks == 1) store_weight(a, seq, first, kvh, key, key - (total - n), sum);
+      else if (n_tiles > 0) p.part_w[(((size_t)seq * a.nkv + kvh) * p.chunks + chunk) * p.keys + key] = sum;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// The chunks' sums added in their order: a thread per key.
+__global__ void __launch_bounds__(256) scored_keys_join_kernel(const __grid_constant__ LongArgs p) {
+  pdl_prologue();
+  const ScoredArgs& a = p.a;
+  const int seq = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
+  if (key >= total || !scored_takes(a, n)) return;
+  float sum = 0.f;
+  for (int c = 0; c < p.chunks; ++c) {
+    int begin, end;
+    chunk_range(p, n, total, key / BM * BM, c, begin, end);
+    if (begin < end) sum += p.part_w[(((size_t)seq * a.nkv + kvh) * p.chunks + c) * p.keys + key];
+  }
+  store_weight(a, seq, first, kvh, key, key - (total - n), sum);
+}
+
+bool make_q_map(CUtensorMap* map, const ScoredArgs& a, int tokens) {
+  const long long dims[3] = {a.d, a.nq, a.n_tokens}, strides[3] = {2, (long long)a.d * 2, (long long)a.q_stride * 2};
+  const int box[3] = {64, a.nq / a.nkv, tokens};
+  return nhv_make_map_bf16_nd(map, a.q, 3, dims, strides, box);
+}
+
+int divisor(int a, int b) { return b == 0 ? a : divisor(b, a % b); }
+
+template <int DB>
+int launch_long(const LongArgs& p, int row_tiles, cudaStream_t stream) {
+  static std::atomic<uint64_t> rows_done{0}, keys_done{0};
+  const ScoredArgs& a = p.a;
+  NHV_CUDA(nhv_allow_smem((const void*)scored_rows_tcgen05_kernel<DB>, Rows<DB>::SMEM, rows_done), "scored attention (tcgen05)");
+  NHV_CUDA(nhv_allow_smem((const void*)scored_keys_tcgen05_kernel<DB>, Keys<DB>::SMEM, keys_done), "scored attention (tcgen05)");
+  NHV_CUDA(nhv_launch(scored_rows_tcgen05_kernel<DB>, dim3(a.nkv, row_tiles, p.splits), Rows<DB>::THREADS, Rows<DB>::SMEM, stream, p),
+           "scored attention (tcgen05)");
+  if (p.splits > 1)
+    NHV_CUDA(nhv_launch(scored_rows_join_kernel, dim3((unsigned)(((long long)a.n_tokens * a.nq + 7) / 8)), 256, 0, stream, p), "scored attention (tcgen05)");
+  NHV_CUDA(nhv_launch(scored_keys_tcgen05_kernel<DB>, dim3(a.nkv, p.key_tiles * p.chunks, a.n_seqs), Keys<DB>::THREADS, Keys<DB>::SMEM, stream, p),
+           "scored attention (tcgen05)");
+  if (p.chunks > 1)
+    NHV_CUDA(nhv_launch(scored_keys_join_kernel, dim3((a.max_keys + 255) / 256, a.nkv, a.n_seqs), 256, 0, stream, p), "scored attention (tcgen05)");
+  return 0;
+}
+
+}  // namespace
+
+NHV_API int nhv_scored_tcgen05_error() { return nhv_wait_error_take(); }
+NHV_API void* nhv_scored_tcgen05_error_word() { return nhv_wait_error_address(); }
+
+bool scored_long_takes(int dtype, int nq, int nkv, int d, int page_size, float scale) {
+  return scale > 0.f && dtype == NHV_BF16 && d % 8 == 0 && d <= SA_MAX_D && nq / nkv <= BM && page_size % 8 == 0;
+}
+
+LongPlan scored_long_plan(int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
+  LongPlan p = {};
+  const int G = nq / nkv, tokens = BM / G, per_block = (d <= 128 ? 2 : 1) * tokens, bn = d <= 128 ? 128 : 64;
+  const long long blocks = ((long long)n_tokens / per_block + n_seqs) * nkv;       // at most
+  // the rows' pass: parts of the keys only where whole walks would leave most SMs idle, and no part below eight tiles
+  const int tiles = (max_keys + bn - 1) / bn;
+  long long splits = SMS / blocks;
+  if (splits > tiles / 8) splits = tiles / 8;
+  p.splits = splits < 1 ? 1 : (int)splits;
+  p.split_tiles = (tiles + p.splits - 1) / p.splits;
+  // the keys' pass: chunks of rows so that a few blocks come to each place that runs at once (two an SM)
+  const long long row_tiles = ((long long)max_new + tokens - 1) / tokens, key_tiles = (max_keys + BM - 1) / BM;
+  const long long pairs = ((long long)n_tokens / tokens + n_seqs) * key_tiles * nkv;
+  long long chunk = pairs / (2 * SMS * 8);
+  if (chunk < 4) chunk = 4;
+  if (chunk > row_tiles) chunk = row_tiles < 1 ? 1 : row_tiles;
+  p.chunk_tiles = (int)chunk;
+  p.chunks = (int)((row_tiles + chunk - 1) / chunk);
+  if (p.chunks < 1) p.chunks = 1;
+  p.keys = (size_t)key_tiles * BM;
+  const size_t rows = (size_t)n_tokens * nq;
+  p.floats = (p.splits > 1 ? p.splits * rows * (d + 2) : 0) + (p.chunks > 1 ? (size_t)n_seqs * nkv * p.chunks * p.keys : 0);
+  return p;
+}
+
+int scored_long_launch(ScoredArgs a, const LongPlan& plan, float* work, cudaStream_t stream) {
+  const int G = a.nq / a.nkv;
+  LongArgs p;
+  p.a = a;
+  p.cap = nhv_score_cap(a.scale, a.softcap);
+  p.scale_log2 = a.softcap > 0.f ? 1.0f : a.scale * SA_LOG2E;
+  p.tokens = BM / G;
+  p.splits = plan.splits;
+  p.split_tiles = plan.split_tiles;
+  p.chunks = plan.chunks;
+  p.chunk_tiles = plan.chunk_tiles;
+  p.keys = plan.keys;
+  p.key_tiles = (int)(plan.keys / BM);
+  const size_t rows = (size_t)a.n_tokens * a.nq;
+  p.part_o = work;
+  p.part_ml = p.part_o + (plan.splits > 1 ? plan.splits * rows * a.d : 0);
+  p.part_w = p.part_ml + (plan.splits > 1 ? plan.splits * rows * 2 : 0);
+  const int db = (a.d + 63) / 64, nq_tiles = db <= 2 ? 2 : 1, bn = db <= 2 ? 128 : 64;
+  p.box = divisor(a.page_size, bn);
+  const long long pool = (long long)a.n_pages * 2 * a.nkv * a.page_size;
+  NHV_REQUIRE(pool < (1LL << 31), "scored attention (tcgen05): the pool's %lld rows are beyond a 32-bit coordinate", pool);
+  NHV_REQUIRE(nhv_make_map_bf16(&p.kv_map, a.pages, pool, a.d, a.d, 64, p.box), "scored attention (tcgen05): cannot encode the tensor map of the pool");
+  NHV_REQUIRE(make_q_map(&p.q_map, a, p.tokens), "scored attention (tcgen05): cannot encode the tensor map of q");
+  const long long row_tiles = (long long)a.n_tokens / (nq_tiles * p.tokens) + a.n_seqs;
+  NHV_REQUIRE(row_tiles <= 65535 && (long long)p.key_tiles * p.chunks <= 65535, "scored attention (tcgen05): %lld tiles of rows, %d of keys in %d chunks are beyond the grid's reach",
+              row_tiles, p.key_tiles, p.chunks);
+  switch (db) {
+    case 1: return launch_long<1>(p, (int)row_tiles, stream);
+    case 2: return launch_long<2>(p, (int)row_tiles, stream);
+    case 3: return launch_long<3>(p, (int)row_tiles, stream);
+    default: return launch_long<4>(p, (int)row_tiles, stream);
+  }
+}

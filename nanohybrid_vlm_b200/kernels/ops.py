@@ -1241,7 +1241,8 @@ def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs
         raise KernelError(f"scores_out is float32 of the scores' shape {tuple(scores.shape)} and contiguous")
     _need_cuda(scores_out)
     dt = dtype_code(q)
-    kilobytes = library.load_library().nhv_attention_scored_kilobytes(dt, n_seqs, T, min_new, max_new, max_kv_len, nq, nkv, head_dim)
+    kilobytes = library.load_library().nhv_attention_scored_kilobytes(dt, n_seqs, T, min_new, max_new, max_kv_len, nq, nkv, head_dim, page_size,
+                                                                      float(scale))
     work = torch.empty(kilobytes * 256, dtype=torch.float32, device=q.device)
     call("nhv_attention_scored", dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv_pages.data_ptr(),
          scores.data_ptr(), scores_out.data_ptr(), _ptr(births), _ptr(positions), block_table.data_ptr(), block_table.stride(0),
@@ -1813,7 +1814,7 @@ def _register_library_sources() -> None:
     import ctypes
     from .library import load_library
     lib = load_library()
-    for name in ("gemm_slab", "gemm_stream_k", "gemm_tcgen05", "moe_tcgen05", "gemm_f32_tcgen05", "key_eviction"):
+    for name in ("gemm_slab", "gemm_stream_k", "gemm_tcgen05", "moe_tcgen05", "gemm_f32_tcgen05", "key_eviction", "scored_tcgen05"):
         word = getattr(lib, f"nhv_{name}_error_word")
         word.restype, word.argtypes = ctypes.c_void_p, []
         take = getattr(lib, f"nhv_{name}_error")

@@ -6,7 +6,7 @@ The bounds are derived, not fitted.  A score is a sum of D products in 32 bits: 
 the sum of the products' magnitudes (a random walk with room), that of a capped one as eight units of the cap more.  A weight's
 relative error is then twice that, and sums of up to L terms add sqrt(L) units; the exponential and the division 2^-20; weights
 below 2^-126, the smallest 32-bit number that is not flushed, may be none.  In bfloat16
-the weights are rounded to 8 bits for the second product and the output once more: 2^-8 of the largest value."""
+the weights are rounded to 8 bits for the second product and the output once more, each by up to 2^-8 of what is rounded."""
 import math
 
 import pytest
@@ -94,7 +94,7 @@ class Case:
                     rel = 2 * err + math.sqrt(max(L, n * G)) * 2 ** -24 + 2 ** -20
                     out[rows, h * self.d:(h + 1) * self.d] = p @ v
                     # the weights' error times the values they weigh, and what is rounded to 8 bits
-                    unit = 2 ** -8 if self.dtype == torch.bfloat16 else 0.0
+                    unit = 2 * 2 ** -8 if self.dtype == torch.bfloat16 else 0.0
                     out_tol[rows, h * self.d:(h + 1) * self.d] = (p @ v.abs()) * (rel + unit) + 2 ** -20 * (p @ v.abs())
                     w_s[g] += p.sum(0)
                     t_s[g] += p.sum(0) * rel + n * 2.0 ** -126      # a weight below the smallest 32-bit number is none
