@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
   }
 }
 
+// Blocks [0, key_blocks): weights of `per_block` keys each, the others FIN_THREADS elements of the output each.
 template <typename T>
 __global__ void __launch_bounds__(FIN_THREADS) scored_short_finish_kernel(const ShortArgs w, const int key_blocks, const int per_block) {
   __shared__ float s_ref[16], s_inv[16], s_lse[16];
@@ -337,21 +338,22 @@ __global__ void __launch_bounds__(FIN_THREADS) scored_short_finish_kernel(const 
   const int seq = w.first_seq + blockIdx.z, kvh = blockIdx.y, G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), R = n * G, d = a.d;
   if (!scored_takes(a, n)) return;
-  const bool output = blockIdx.x == key_blocks;
-  if (!output && blockIdx.x * per_block >= total) return;
+  const bool output = blockIdx.x >= key_blocks;
+  const int i = ((int)blockIdx.x - key_blocks) * FIN_THREADS + threadIdx.x;       // of the output
+  if (output ? i - (int)threadIdx.x >= R * d : (int)blockIdx.x * per_block >= total) return;
   const int parts = (total + w.split_keys - 1) / w.split_keys;
   const size_t part = ((size_t)blockIdx.z * a.nkv + kvh) * w.splits * w.rows;
   for (int r = warp; r < R; r += FIN_THREADS / 32) {
-    float ref = -INFINITY, sum = 0.f;
-    for (int k = lane; k < parts; k += 32) ref = fmaxf(ref, w.part_ml[(part + (size_t)k * w.rows + r) * 2]);
-    ref = warp_max(ref);
     const float sink = a.sinks ? a.sinks[kvh * G + r % G] * SA_LOG2E : -INFINITY;
-    ref = fmaxf(ref, sink);
-    const float use = ref == -INFINITY ? 0.f : ref;
-    for (int k = lane; k < parts; k += 32) {
-      const float2 ml = *reinterpret_cast<const float2*>(w.part_ml + (part + (size_t)k * w.rows + r) * 2);
-      sum = fmaf(scored_exp2(ml.x - use), ml.y, sum);
+    float ref = sink, sum = 0.f;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (k0 + lane < parts) ml = *reinterpret_cast<const float2*>(w.part_ml + (part + (size_t)(k0 + lane) * w.rows + r) * 2);
+      const float top = fmaxf(ref, warp_max(ml.x)), use = top == -INFINITY ? 0.f : top;
+      sum = sum * scored_exp2(ref - use) + ml.y * scored_exp2(ml.x - use);
+      ref = top;
     }
+    const float use = ref == -INFINITY ? 0.f : ref;
     sum = warp_sum(sum) + scored_exp2(sink - use);
     if (lane == 0) {
       s_ref[r] = use;
@@ -361,20 +363,22 @@ __global__ void __launch_bounds__(FIN_THREADS) scored_short_finish_kernel(const 
   }
   __syncthreads();
   if (output) {
-    T* out = (T*)a.out;
-    for (int i = threadIdx.x; i < R * d; i += FIN_THREADS) {
-      const int r = i / d, c = i - r * d;
-      float v = 0.f;
-      for (int k = 0; k < parts; ++k) {
-        const size_t at = part + (size_t)k * w.rows + r;
-        v = fmaf(scored_exp2(w.part_ml[at * 2] - s_ref[r]), w.part_o[at * d + c], v);
-      }
-      out[(size_t)(first + r / G) * a.out_stride + (size_t)(kvh * G + r % G) * d + c] = from_f32<T>(v * s_inv[r]);
-    }
+    if (i >= R * d) return;
+    const int r = i / d, c = i - r * d;
+    const float ref = s_ref[r];
+    const float* ml = w.part_ml + (part + r) * 2;
+    const float* po = w.part_o + (part + r) * d + c;
+    const size_t step = w.rows;
+    float v = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) v = fmaf(scored_exp2(ml[k * step * 2] - ref), po[k * step * d], v);
+    ((T*)a.out)[(size_t)(first + r / G) * a.out_stride + (size_t)(kvh * G + r % G) * d + c] = from_f32<T>(v * s_inv[r]);
     return;
   }
   const float* kept = w.kept + ((size_t)blockIdx.z * a.nkv + kvh) * w.keys * w.rows;
-  for (int j = blockIdx.x * per_block + threadIdx.x; j < min(total, (int)(blockIdx.x + 1) * per_block); j += FIN_THREADS) {
+  const int end = min(total, (int)(blockIdx.x + 1) * per_block);
+#pragma unroll 4
+  for (int j = blockIdx.x * per_block + threadIdx.x; j < end; j += FIN_THREADS) {
     float sum = 0.f;
     for (int r = 0; r < R; r += 2) {
       const float2 x = *reinterpret_cast<const float2*>(kept + (size_t)j * w.rows + r);
@@ -437,7 +441,9 @@ int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* w
   w.part_ml = w.part_o + pairs * plan.splits * plan.rows * a.d;
   const int db = (a.d + 63) / 64;
   const size_t smem = sizeof(float) * SH_WARPS * plan.rows * (a.d + 4);
-  const int per_block = plan.keys > 4096 ? 1024 : 256, key_blocks = (a.max_keys + per_block - 1) / per_block;
+  // weights: 256 keys a block, 1,024 where there are blocks enough
+  const int per_block = (long long)plan.group * a.nkv * plan.keys > 4 * 1024 * 1024 / 8 ? 1024 : 256;
+  const int key_blocks = (a.max_keys + per_block - 1) / per_block, out_blocks = (plan.rows * a.d + FIN_THREADS - 1) / FIN_THREADS;
   for (int s = 0; s < a.n_seqs; s += plan.group) {
     w.first_seq = s;
     const int count = a.n_seqs - s < plan.group ? a.n_seqs - s : plan.group;
@@ -449,7 +455,7 @@ int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* w
     else
       rc = db == 1 ? launch_split<1, 2>(w, grid, smem, stream) : launch_split<2, 2>(w, grid, smem, stream);
     if (rc) return rc;
-    NHV_CUDA(nhv_launch(scored_short_finish_kernel<__nv_bfloat16>, dim3(key_blocks + 1, a.nkv, count), FIN_THREADS, 0, stream, w, key_blocks, per_block),
+    NHV_CUDA(nhv_launch(scored_short_finish_kernel<__nv_bfloat16>, dim3(key_blocks + out_blocks, a.nkv, count), FIN_THREADS, 0, stream, w, key_blocks, per_block),
              "scored attention");
   }
   return 0;
