@@ -65,6 +65,29 @@ __device__ __forceinline__ float scored_exp2(float x) {     // 2^x; -inf gives 0
   return y;
 }
 
+// Parts of the two passes: the keys of a request cut for the rows' pass (`splits`), its rows cut for the keys' pass (`chunks`).
+struct ScoredParts {
+  float* o;                 // [splits][nkv][n_tokens * G][d], with splits > 1
+  float* ml;                // [splits][nkv][n_tokens * G][2]: reference and sum, in log2 units
+  float* w;                 // [n_seqs][nkv][chunks][keys], with chunks > 1
+  size_t keys;              // places for keys of a (request, KV head)
+  int splits, split_tiles;  // parts of a request's keys, tiles of keys of one part
+  int chunks, chunk_tiles;  // parts of a request's rows, tiles of rows of one part
+  int tile_rows, tile_keys; // of the keys' pass
+};
+// The tiles of rows [begin, end) of chunk `chunk` that see some key of the tile of keys at key0.
+__device__ __forceinline__ void chunk_range(const ScoredParts& p, int n, int G, int total, int key0, int chunk, int& begin, int& end) {
+  const int t = key0 - (total - n), first = t > 0 ? t * G / p.tile_rows : 0, tiles = (n * G + p.tile_rows - 1) / p.tile_rows;
+  begin = first > chunk * p.chunk_tiles ? first : chunk * p.chunk_tiles;
+  end = tiles < (chunk + 1) * p.chunk_tiles ? tiles : (chunk + 1) * p.chunk_tiles;
+}
+// Fills in splits and chunks and the scratch they take; `row_tile` and `key_tile`: of the rows' pass; blocks that run at once in each.
+size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d, int row_tile, int key_tile,
+                    int rows_at_once, int keys_at_once);
+void scored_place(ScoredParts& p, float* work, int n_tokens, int nq, int d);
+int scored_join_rows(int dtype, const ScoredArgs& a, const ScoredParts& p, cudaStream_t stream);
+int scored_join_keys(const ScoredArgs& a, const ScoredParts& p, cudaStream_t stream);
+
 // ---- requests with few rows (scored_attention_short.cu): the keys are split over blocks, the scores kept for the second pass
 struct ShortPlan {
   int rows;                 // rows kept per key: the most of a request, rounded up to 2
@@ -80,12 +103,6 @@ ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, i
 int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* work, cudaStream_t stream);
 
 // ---- requests with many rows, bfloat16 (scored_attention_tcgen05.cu)
-struct LongPlan {
-  int splits, split_tiles;  // parts of a request's keys in the rows' pass, tiles of keys of one part
-  int chunks, chunk_tiles;  // parts of a request's rows in the keys' pass, tiles of rows of one part
-  size_t keys;              // places for keys of a (request, KV head)
-  size_t floats;            // of scratch
-};
 bool scored_long_takes(int dtype, int nq, int nkv, int d, int page_size, float scale);
-LongPlan scored_long_plan(int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d);
-int scored_long_launch(ScoredArgs a, const LongPlan& plan, float* work, cudaStream_t stream);
+size_t scored_long_plan(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d);     // floats of scratch
+int scored_long_launch(ScoredArgs a, const ScoredParts& p, cudaStream_t stream);

@@ -4,208 +4,508 @@
 //   scores_out[g][j] = (j < L - n ? scores[g][j] : 0) + sum over t and the heads of g of p[j];     births[g][j] = position, j new
 // A key's sum needs the rows' final normaliser, so there are two passes: the rows' (output and log-sum), then the keys'.
 //
-// The kernels of this file take any type, size and page size and compute in fp32.
-//   rows: a block holds 16 rows (token, head) of a KV head; 32 keys at a time in shared memory, lane <-> key for the scores,
-//     lane <-> column for the output.
-//   keys: a block holds 32 keys of a request and KV head and walks the rows that see them, lane <-> key, the warps' sums added
-//     in a fixed order at the end.
-// No sum is shared between blocks, so results do not depend on the order in which blocks run.
+// The entry point, and kernels for any type, size and page size that compute in fp32 on the CUDA cores (the 32-bit path, and what
+// the tensor-core kernels of scored_attention_short.cu and scored_attention_tcgen05.cu refuse).
+//   rows: 128 threads hold 8 RPT rows (row = token * G + head, of one request and KV head) and walk the keys in tiles of 64 through
+//     shared memory.  A thread makes RPT x 4 scores from 16-byte reads along the head and RPT x 4 DB outputs, two multiply-adds
+//     an instruction; P passes through shared memory, over the keys.  RPT is 8, and 1 or 2 where no request has more rows.
+//   keys: 64 keys stay in shared memory, the tiles of rows pass by; a thread adds up the weights of its 4 keys, the eight row groups
+//     meet in shared memory at the end.
+// What bounds them is multiply-adds: 4 D a pair in the first, 2 D in the second, of 128 a cycle and SM.
+// Long walks over the keys are split over blocks where there are few tiles of rows, and rows into chunks in the keys' pass; two
+// small kernels join the parts in a fixed order.  No sum depends on the order in which blocks run.
+//
+// A key out of sight may hold anything: its score is replaced, and in tiles of which some row sees only a part its value is left
+// out of that row's sum instead of being multiplied by 0.
 #include "nhv_scored.cuh"
 
 namespace {
 
-constexpr int SA_WARPS = 4, SA_ROWS_PER_WARP = 4, SA_ROWS = SA_WARPS * SA_ROWS_PER_WARP, SA_KEYS = 32;
+constexpr int SA_THREADS = 128, SA_KEYS = 64;
 
-__device__ __forceinline__ float capped(float s, float cap) { return cap > 0.f ? cap * tanhf(s / cap) : s; }
+struct TileArgs {
+  ScoredArgs a;
+  ScoredParts p;
+  int vec;                  // rows of q and of the pages can be read four elements at a time
+};
 
+template <typename T> __device__ __forceinline__ float4 load4(const T* p);
+template <> __device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+
+// `rows` rows of d elements at base + at[r] into shared memory, `stride` floats apart, as fp32; at[r] < 0: zeros.  The last four
+// columns that d reaches into are filled up with zeros.
 template <typename T>
-__global__ void __launch_bounds__(SA_WARPS * 32) scored_rows_kernel(const ScoredArgs a) {
-  extern __shared__ float smem[];
-  __shared__ long long k_at[SA_KEYS], v_at[SA_KEYS];
+__device__ __forceinline__ void load_rows(float* dst, int stride, const T* base, const long long* at, int rows, int d, bool vec) {
+  const int per_row = (d + 3) / 4;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < rows * per_row; i += SA_THREADS) {
+    const int r = i / per_row, c = (i - r * per_row) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (at[r] >= 0) {
+      const T* src = base + at[r] + c;
+      if (vec) {
+        v = load4<T>(src);
+      } else {
+        v.x = to_f32<T>(src[0]);
+        if (c + 1 < d) v.y = to_f32<T>(src[1]);
+        if (c + 2 < d) v.z = to_f32<T>(src[2]);
+        if (c + 3 < d) v.w = to_f32<T>(src[3]);
+      }
+    }
+    *reinterpret_cast<float4*>(dst + r * stride + c) = v;
+  }
+}
+
+// s[i][k] = row (ty RPT + i) . key (tx + 16 k)
+template <int RPT>
+__device__ __forceinline__ void tile_scores(float (&s)[RPT][4], const float* Qs, const float* Ks, int stride, int d, int ty, int tx) {
+  f32x2 acc[RPT][4];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[i][k] = 0ull;
+  for (int c = 0; c < d; c += 4) {
+    f32x2 kk[4][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(Ks + (tx + 16 * k) * stride + c);
+      kk[k][0] = v.x;
+      kk[k][1] = v.y;
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(Qs + (ty * RPT + i) * stride + c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[i][k] = f2_fma(q.y, kk[k][1], f2_fma(q.x, kk[k][0], acc[i][k]));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RPT; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float x, y;
+      f2_unpack(acc[i][k], x, y);
+      s[i][k] = x + y;
+    }
+}
+// in log2 units
+__device__ __forceinline__ float scaled(float s, const ScoredArgs& a) {
+  s *= a.scale;
+  return (a.softcap > 0.f ? a.softcap * tanhf(s / a.softcap) : s) * SA_LOG2E;
+}
+
+// DB: blocks of 64 elements of a head.
+template <typename T, int DB, int RPT>
+__global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_rows_kernel(const TileArgs t) {
+  extern __shared__ __align__(16) float smem[];
+  __shared__ long long s_at[SA_KEYS], s_v[SA_KEYS];
+  constexpr int ROWS = 8 * RPT, DP = 64 * DB, STRIDE = DP + 4, PS = SA_KEYS + 4;
+  float* Qs = smem;                       // [ROWS][STRIDE]
+  float* Ks = Qs + ROWS * STRIDE;         // [64][STRIDE], and then P [ROWS][PS]
+  float* Vs = Ks + SA_KEYS * STRIDE;      // [64][DP]
+  float* Ps = Ks;
   pdl_prologue();
-  const int G = a.nq / a.nkv, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // a tile is a whole number of tokens where a group fits the 16 rows, else 16 heads of one token
-  const int per_tile = SA_ROWS / G > 0 ? SA_ROWS / G : 1, head_blocks = (G + SA_ROWS - 1) / SA_ROWS;
-  int tile = blockIdx.x / head_blocks;
-  const int g0 = (blockIdx.x % head_blocks) * SA_ROWS, gs = min(G - g0, SA_ROWS);
-  const int seq = find_tile(a, per_tile, tile);
+  const ScoredArgs& a = t.a;
+  const int G = a.nq / a.nkv, kvh = blockIdx.y, tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, d = a.d;
+  // which request, which rows: the last ones, which see the most, come first
+  int tile = blockIdx.x, seq = -1;
+  for (int s = 0; s < a.n_seqs; ++s) {
+    const int n = a.cu_q[s + 1] - a.cu_q[s];
+    if (!scored_takes(a, n)) continue;
+    const int nt = (n * G + ROWS - 1) / ROWS;
+    if (tile < nt) {
+      seq = s;
+      tile = nt - 1 - tile;
+      break;
+    }
+    tile -= nt;
+  }
   if (seq < 0) return;
-  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), t0 = tile * per_tile;
-  const int rows = min(per_tile, n - t0) * gs, d = a.d, ks = d + 1;
-  float* Qs = smem;                       // [16][d]
-  float* Ks = Qs + SA_ROWS * d;           // [32][d + 1]
-  float* Vs = Ks + SA_KEYS * ks;          // [32][d]
-  float* Ps = Vs + SA_KEYS * d;           // [warps][32]
-  const T* q = (const T*)a.q;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), r0 = tile * ROWS;
+  const int rows = min(ROWS, n * G - r0), key_begin = (int)blockIdx.z * t.p.split_tiles * SA_KEYS;
+  const int last = min(total - n + (r0 + rows - 1) / G, total - 1);            // the newest key that a row of the tile sees
+  const int all = total - n + r0 / G;                                          // every row sees keys up to here
+  const int key_end = min(last + 1, key_begin + t.p.split_tiles * SA_KEYS);
   const T* pages = (const T*)a.pages;
-  for (int i = threadIdx.x; i < rows * d; i += blockDim.x) {
-    const int r = i / d, c = i - r * d;
-    Qs[i] = to_f32<T>(q[(size_t)(first + t0 + r / gs) * a.q_stride + (size_t)(kvh * G + g0 + r % gs) * d + c]);
-  }
-  float m[SA_ROWS_PER_WARP], l[SA_ROWS_PER_WARP], o[SA_ROWS_PER_WARP][SA_MAX_D / 32];
+  if (tid < ROWS) s_at[tid] = tid < rows ? (long long)(first + (r0 + tid) / G) * a.q_stride + (long long)(kvh * G + (r0 + tid) % G) * d : -1;
+  __syncthreads();
+  load_rows<T>(Qs, STRIDE, (const T*)a.q, s_at, ROWS, d, t.vec);
+
+  float m[RPT], l[RPT];
+  f32x2 o[RPT][2 * DB];                   // columns 64 b + 4 tx .. + 3
+  int hi[RPT];
 #pragma unroll
-  for (int i = 0; i < SA_ROWS_PER_WARP; ++i) {
-    const int r = warp * SA_ROWS_PER_WARP + i;
-    const bool sink = a.sinks && r < rows;
-    m[i] = sink ? a.sinks[kvh * G + g0 + r % gs] : -INFINITY;
-    l[i] = sink ? 1.f : 0.f;
+  for (int i = 0; i < RPT; ++i) {
+    const int r = ty * RPT + i;
+    hi[i] = r < rows ? min(total - n + (r0 + r) / G, total - 1) : -1;
+    m[i] = -INFINITY;
+    l[i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < SA_MAX_D / 32; ++c) o[i][c] = 0.f;
+    for (int c = 0; c < 2 * DB; ++c) o[i][c] = 0ull;
   }
-  const int last = min(total - n + t0 + (rows - 1) / gs, total - 1);       // the newest key that a row of the tile sees
-  for (int j0 = 0; j0 <= last; j0 += SA_KEYS) {
+  for (int j0 = key_begin; j0 < key_end; j0 += SA_KEYS) {
     __syncthreads();
-    if (threadIdx.x < SA_KEYS) {
-      const int j = j0 + threadIdx.x;
-      k_at[threadIdx.x] = j <= last ? key_row(a, seq, j, kvh, 0) : -1;
-      v_at[threadIdx.x] = j <= last ? key_row(a, seq, j, kvh, 1) : -1;
+    if (tid < SA_KEYS) {
+      const int j = j0 + tid;
+      s_at[tid] = j < key_end ? key_row(a, seq, j, kvh, 0) : -1;
+      s_v[tid] = j < key_end ? key_row(a, seq, j, kvh, 1) : -1;
+    }
+    // some row does not see some key of the tile
+    const bool masked = __syncthreads_or(tid < SA_KEYS && s_at[tid & (SA_KEYS - 1)] < 0) || j0 + SA_KEYS - 1 > all;
+    load_rows<T>(Ks, STRIDE, pages, s_at, SA_KEYS, d, t.vec);
+    load_rows<T>(Vs, DP, pages, s_v, SA_KEYS, d, t.vec);
+    __syncthreads();
+    float s[RPT][4];
+    tile_scores<RPT>(s, Qs, Ks, STRIDE, d, ty, tx);
+    uint32_t sees = 0xffffffffu;          // bit 4 i + k
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        s[i][k] = scaled(s[i][k], a);
+        if (masked && (j0 + tx + 16 * k > hi[i] || s_at[tx + 16 * k] < 0)) {
+          s[i][k] = -INFINITY;
+          sees &= ~(1u << (4 * i + k));
+        }
+        top = fmaxf(top, s[i][k]);
+      }
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float ref = fmaxf(m[i], top), use = ref == -INFINITY ? 0.f : ref, alpha = scored_exp2(m[i] - use);
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        s[i][k] = scored_exp2(s[i][k] - use);
+        sum += s[i][k];
+      }
+      l[i] = fmaf(l[i], alpha, sum);      // this thread's keys; the sixteen threads of a row meet at the end
+      m[i] = ref;
+      const f32x2 aa = f2_pack(alpha, alpha);
+#pragma unroll
+      for (int c = 0; c < 2 * DB; ++c) o[i][c] = f2_mul(o[i][c], aa);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < SA_KEYS * d; i += blockDim.x) {
-      const int r = i / d, c = i - r * d;
-      Ks[r * ks + c] = k_at[r] >= 0 ? to_f32<T>(pages[k_at[r] + c]) : 0.f;
-      Vs[i] = v_at[r] >= 0 ? to_f32<T>(pages[v_at[r] + c]) : 0.f;
-    }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) Ps[(ty * RPT + i) * PS + tx + 16 * k] = s[i][k];
     __syncthreads();
+    if (!masked) {
+#pragma unroll 2
+      for (int j = 0; j < SA_KEYS; j += 4) {
+        float4 p[RPT];
 #pragma unroll
-    for (int i = 0; i < SA_ROWS_PER_WARP; ++i) {
-      const int r = warp * SA_ROWS_PER_WARP + i;
-      if (r >= rows) break;
-      const int hi = total - n + t0 + r / gs;
-      const bool sees = j0 + lane <= hi && k_at[lane] >= 0;
-      float s = 0.f;
-      for (int c = 0; c < d; ++c) s = fmaf(Qs[r * d + c], Ks[lane * ks + c], s);
-      s = sees ? capped(s * a.scale, a.softcap) : -INFINITY;
-      const float top = warp_max(s);
-      const unsigned live = __ballot_sync(0xffffffffu, sees);
-      if (!live) continue;
-      const float m_new = fmaxf(m[i], top), ref = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = expf(m[i] - ref), p = sees ? expf(s - ref) : 0.f;
-      l[i] = l[i] * alpha + warp_sum(p);
-      m[i] = m_new;
-      Ps[warp * SA_KEYS + lane] = p;
-      __syncwarp();
+        for (int i = 0; i < RPT; ++i) p[i] = *reinterpret_cast<const float4*>(Ps + (ty * RPT + i) * PS + j);
 #pragma unroll
-      for (int c = 0; c < SA_MAX_D / 32; ++c) {
-        if (c * 32 + lane < d) {
-          float acc = 0.f;
-          for (int k = 0; k < SA_KEYS; ++k)
-            if (live >> k & 1) acc = fmaf(Ps[warp * SA_KEYS + k], Vs[k * d + c * 32 + lane], acc);   // a key out of sight may hold anything
-          o[i][c] = o[i][c] * alpha + acc;
+        for (int k = 0; k < 4; ++k) {
+          f32x2 v[2 * DB];
+#pragma unroll
+          for (int b = 0; b < DB; ++b) {
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(Vs + (j + k) * DP + 64 * b + 4 * tx);
+            v[2 * b] = x.x;
+            v[2 * b + 1] = x.y;
+          }
+#pragma unroll
+          for (int i = 0; i < RPT; ++i) {
+            const float pk = k == 0 ? p[i].x : k == 1 ? p[i].y : k == 2 ? p[i].z : p[i].w;
+            const f32x2 pp = f2_pack(pk, pk);
+#pragma unroll
+            for (int c = 0; c < 2 * DB; ++c) o[i][c] = f2_fma(pp, v[c], o[i][c]);
+          }
         }
       }
-      __syncwarp();
+    } else {
+      for (int j = 0; j < SA_KEYS && j0 + j < key_end; ++j) {
+        if (s_at[j] < 0) continue;
+        f32x2 v[2 * DB];
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(Vs + j * DP + 64 * b + 4 * tx);
+          v[2 * b] = x.x;
+          v[2 * b + 1] = x.y;
+        }
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+          if (j0 + j > hi[i]) continue;
+          const float pk = Ps[(ty * RPT + i) * PS + j];
+          const f32x2 pp = f2_pack(pk, pk);
+#pragma unroll
+          for (int c = 0; c < 2 * DB; ++c) o[i][c] = f2_fma(pp, v[c], o[i][c]);
+        }
+      }
     }
   }
   T* out = (T*)a.out;
 #pragma unroll
-  for (int i = 0; i < SA_ROWS_PER_WARP; ++i) {
-    const int r = warp * SA_ROWS_PER_WARP + i;
-    if (r >= rows) break;
-    const int token = first + t0 + r / gs, head = g0 + r % gs;
-    const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
+  for (int i = 0; i < RPT; ++i) {
+    float sum = l[i];
 #pragma unroll
-    for (int c = 0; c < SA_MAX_D / 32; ++c)
-      if (c * 32 + lane < d) out[(size_t)token * a.out_stride + (size_t)(kvh * G + head) * d + c * 32 + lane] = from_f32<T>(o[i][c] * inv);
-    if (lane == 0) a.lse[((size_t)kvh * a.n_tokens + token) * G + head] = l[i] == 0.f ? INFINITY : fmaf(m[i], SA_LOG2E, log2f(l[i]));
+    for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const int r = ty * RPT + i;
+    if (r >= rows) continue;
+    const int token = first + (r0 + r) / G, head = kvh * G + (r0 + r) % G;
+    const size_t row = (size_t)kvh * a.n_tokens * G + (size_t)first * G + r0 + r;
+    const bool whole = t.p.splits == 1;
+    float inv = 1.f;
+    if (whole) {
+      const float sink = a.sinks ? a.sinks[head] * SA_LOG2E : -INFINITY, ref = fmaxf(m[i], sink), use = ref == -INFINITY ? 0.f : ref;
+      const float f = scored_exp2(m[i] - use);
+      sum = fmaf(sum, f, scored_exp2(sink - use));
+      inv = sum == 0.f ? 0.f : f / sum;
+      if (tx == 0) a.lse[row] = sum == 0.f ? INFINITY : use + log2f(sum);
+    } else if (tx == 0) {
+      float* ml = t.p.ml + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * 2;
+      ml[0] = m[i];
+      ml[1] = sum;
+    }
+#pragma unroll
+    for (int c = 0; c < 2 * DB; ++c) {
+      float x, y;
+      f2_unpack(o[i][c], x, y);
+      const int at = 64 * (c >> 1) + 4 * tx + 2 * (c & 1);
+      if (whole) {
+        T* dst = out + (size_t)token * a.out_stride + (size_t)head * d + at;
+        if (at < d) dst[0] = from_f32<T>(x * inv);
+        if (at + 1 < d) dst[1] = from_f32<T>(y * inv);
+      } else {
+        float* dst = t.p.o + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * d + at;
+        if (at < d) dst[0] = x;
+        if (at + 1 < d) dst[1] = y;
+      }
+    }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SA_WARPS * 32) scored_keys_kernel(const ScoredArgs a) {
-  extern __shared__ float smem[];
-  __shared__ float part[SA_WARPS][SA_KEYS];
+template <typename T, int DB, int RPT>
+__global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_keys_kernel(const TileArgs t) {
+  extern __shared__ __align__(16) float smem[];
+  __shared__ long long s_at[SA_KEYS];
+  __shared__ float s_lse[64], s_part[8][SA_KEYS];
+  constexpr int ROWS = 8 * RPT, STRIDE = 64 * DB + 4;
+  float* Qs = smem;                       // [ROWS][STRIDE]
+  float* Ks = Qs + ROWS * STRIDE;         // [64][STRIDE]
   pdl_prologue();
-  const int G = a.nq / a.nkv, kvh = blockIdx.y, seq = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), j0 = blockIdx.x * SA_KEYS;
-  if (j0 >= total || !scored_takes(a, n)) return;
-  const int d = a.d, ks = d + 1, j = j0 + lane;
-  float* Ks = smem;                       // [32][d + 1]
-  float* Qs = Ks + SA_KEYS * ks;          // [warps][d]
-  const T* q = (const T*)a.q;
-  const T* pages = (const T*)a.pages;
-  for (int i = threadIdx.x; i < SA_KEYS * d; i += blockDim.x) {
-    const int r = i / d, c = i - r * d;
-    const long long at = j0 + r < total ? key_row(a, seq, j0 + r, kvh, 0) : -1;
-    Ks[r * ks + c] = at >= 0 ? to_f32<T>(pages[at + c]) : 0.f;
-  }
+  const ScoredArgs& a = t.a;
+  const int G = a.nq / a.nkv, kvh = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, d = a.d;
+  const int tiles = (int)(t.p.keys / SA_KEYS), chunk = blockIdx.x / tiles, key0 = (blockIdx.x - chunk * tiles) * SA_KEYS;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
+  if (key0 >= total || !scored_takes(a, n)) return;
+  int begin, end;
+  chunk_range(t.p, n, G, total, key0, chunk, begin, end);
+  if (t.p.chunks > 1 && begin >= end) return;
+  if (tid < SA_KEYS) s_at[tid] = key0 + tid < total ? key_row(a, seq, key0 + tid, kvh, 0) : -1;
   __syncthreads();
-  const int t_first = max(0, j0 - (total - n));        // the first token that sees a key of the block
-  float w = 0.f;
-  for (int r = t_first * G + warp; r < n * G; r += SA_WARPS) {
-    const int t = r / G, h = r - t * G;
-    __syncwarp();
-    for (int c = lane; c < d; c += 32) Qs[warp * d + c] = to_f32<T>(q[(size_t)(first + t) * a.q_stride + (size_t)(kvh * G + h) * d + c]);
-    __syncwarp();
-    float s = 0.f;
-    for (int c = 0; c < d; ++c) s = fmaf(Qs[warp * d + c], Ks[lane * ks + c], s);
-    if (j <= total - n + t)
-      w += exp2f(fmaf(capped(s * a.scale, a.softcap), SA_LOG2E, -a.lse[((size_t)kvh * a.n_tokens + first + t) * G + h]));
+  load_rows<T>(Ks, STRIDE, (const T*)a.pages, s_at, SA_KEYS, d, t.vec);
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = begin; i0 < end; ++i0) {
+    const int r0 = i0 * ROWS, rows = min(ROWS, n * G - r0);
+    __syncthreads();
+    if (tid < ROWS) {
+      s_at[tid] = tid < rows ? (long long)(first + (r0 + tid) / G) * a.q_stride + (long long)(kvh * G + (r0 + tid) % G) * d : -1;
+      s_lse[tid] = tid < rows ? a.lse[(size_t)kvh * a.n_tokens * G + (size_t)first * G + r0 + tid] : INFINITY;
+    }
+    __syncthreads();
+    load_rows<T>(Qs, STRIDE, (const T*)a.q, s_at, ROWS, d, t.vec);
+    __syncthreads();
+    float s[RPT][4];
+    tile_scores<RPT>(s, Qs, Ks, STRIDE, d, ty, tx);
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const int r = ty * RPT + i, hi = r < rows ? total - n + (r0 + r) / G : -1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float p = scored_exp2(scaled(s[i][k], a) - s_lse[r]);
+        if (key0 + tx + 16 * k <= hi) w[k] += p;
+      }
+    }
   }
-  part[warp][lane] = w;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s_part[ty][tx + 16 * k] = w[k];
   __syncthreads();
-  if (warp == 0 && j < total) {
-    float sum = part[0][lane];
-    for (int k = 1; k < SA_WARPS; ++k) sum += part[k][lane];
-    store_weight(a, seq, first, kvh, j, j - (total - n), sum);
+  if (tid < SA_KEYS && key0 + tid < total) {
+    float sum = 0.f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) sum += s_part[y][tid];
+    if (t.p.chunks == 1) store_weight(a, seq, first, kvh, key0 + tid, key0 + tid - (total - n), sum);
+    else t.p.w[(((size_t)seq * a.nkv + kvh) * t.p.chunks + chunk) * t.p.keys + key0 + tid] = sum;
   }
 }
 
+// The sums of a row's parts joined: a warp per row.
 template <typename T>
-int launch_simt(const ScoredArgs& a, int max_kv_len, cudaStream_t stream) {
+__global__ void __launch_bounds__(256) scored_join_rows_kernel(const ScoredArgs a, const ScoredParts p) {
+  pdl_prologue();
+  const int G = a.nq / a.nkv, lane = threadIdx.x & 31;
+  const size_t rows = (size_t)a.nkv * a.n_tokens * G, row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int kvh = (int)(row / ((size_t)a.n_tokens * G)), r = (int)(row - (size_t)kvh * a.n_tokens * G), token = r / G, head = kvh * G + r % G;
+  int seq = 0;
+  while (seq + 1 < a.n_seqs && a.cu_q[seq + 1] <= token) ++seq;
+  if (!scored_takes(a, a.cu_q[seq + 1] - a.cu_q[seq])) return;
+  const float sink = a.sinks ? a.sinks[head] * SA_LOG2E : -INFINITY;
+  float ref = sink;
+  for (int s = 0; s < p.splits; ++s) ref = fmaxf(ref, p.ml[(s * rows + row) * 2]);
+  if (ref == -INFINITY) ref = 0.f;
+  float sum = scored_exp2(sink - ref);
+  for (int s = 0; s < p.splits; ++s) sum = fmaf(p.ml[(s * rows + row) * 2 + 1], scored_exp2(p.ml[(s * rows + row) * 2] - ref), sum);
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  T* dst = (T*)a.out + (size_t)token * a.out_stride + (size_t)head * a.d;
+  for (int c = lane; c < a.d; c += 32) {
+    float v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) v = fmaf(scored_exp2(p.ml[(s * rows + row) * 2] - ref), p.o[(s * rows + row) * a.d + c], v);
+    dst[c] = from_f32<T>(v * inv);
+  }
+  if (lane == 0) a.lse[row] = sum == 0.f ? INFINITY : ref + log2f(sum);
+}
+
+// The chunks' sums added in their order: a thread per key.
+__global__ void __launch_bounds__(256) scored_join_keys_kernel(const ScoredArgs a, const ScoredParts p) {
+  pdl_prologue();
+  const int seq = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
+  if (key >= total || !scored_takes(a, n)) return;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < p.chunks; ++c) {
+    int begin, end;
+    chunk_range(p, n, a.nq / a.nkv, total, key / p.tile_keys * p.tile_keys, c, begin, end);
+    if (begin < end) sum += p.w[(((size_t)seq * a.nkv + kvh) * p.chunks + c) * p.keys + key];
+  }
+  store_weight(a, seq, first, kvh, key, key - (total - n), sum);
+}
+
+template <typename T, int DB, int RPT>
+int launch_tiles(const TileArgs& t, cudaStream_t stream) {
   static std::atomic<uint64_t> rows_done{0}, keys_done{0};
-  const int G = a.nq / a.nkv, per_tile = SA_ROWS / G > 0 ? SA_ROWS / G : 1, head_blocks = (G + SA_ROWS - 1) / SA_ROWS;
-  const size_t rows_smem = sizeof(float) * (SA_ROWS * a.d + SA_KEYS * (a.d + 1) + SA_KEYS * a.d + SA_WARPS * SA_KEYS);
-  const size_t keys_smem = sizeof(float) * (SA_KEYS * (a.d + 1) + SA_WARPS * a.d);
-  const long long tiles = ((long long)a.n_tokens / per_tile + a.n_seqs) * head_blocks;
-  NHV_REQUIRE(tiles < (1LL << 31), "scored attention: %lld tiles of new tokens are beyond the grid's reach", tiles);
-  NHV_CUDA(nhv_allow_smem((const void*)scored_rows_kernel<T>, 96 * 1024, rows_done), "scored attention");
-  NHV_CUDA(nhv_allow_smem((const void*)scored_keys_kernel<T>, 96 * 1024, keys_done), "scored attention");
-  NHV_CUDA(nhv_launch(scored_rows_kernel<T>, dim3((unsigned)tiles, a.nkv), SA_WARPS * 32, rows_smem, stream, a), "scored attention");
-  NHV_CUDA(nhv_launch(scored_keys_kernel<T>, dim3((max_kv_len + SA_KEYS - 1) / SA_KEYS, a.nkv, a.n_seqs), SA_WARPS * 32, keys_smem, stream, a),
-           "scored attention");
-  return 0;
+  constexpr int ROWS = 8 * RPT, STRIDE = 64 * DB + 4;
+  constexpr size_t rows_smem = sizeof(float) * (ROWS * STRIDE + SA_KEYS * STRIDE + SA_KEYS * 64 * DB), keys_smem = sizeof(float) * (ROWS + SA_KEYS) * STRIDE;
+  const ScoredArgs& a = t.a;
+  const long long tiles = (long long)a.n_tokens * (a.nq / a.nkv) / ROWS + a.n_seqs, key_tiles = (long long)(t.p.keys / SA_KEYS) * t.p.chunks;
+  NHV_REQUIRE(tiles < (1LL << 31) && key_tiles < (1LL << 31), "scored attention: %lld tiles of rows, %lld of keys are beyond the grid's reach", tiles, key_tiles);
+  NHV_CUDA(nhv_allow_smem((const void*)scored_rows_kernel<T, DB, RPT>, (int)rows_smem, rows_done), "scored attention");
+  NHV_CUDA(nhv_allow_smem((const void*)scored_keys_kernel<T, DB, RPT>, (int)keys_smem, keys_done), "scored attention");
+  NHV_CUDA(nhv_launch(scored_rows_kernel<T, DB, RPT>, dim3((unsigned)tiles, a.nkv, t.p.splits), SA_THREADS, rows_smem, stream, t), "scored attention");
+  int rc = scored_join_rows(sizeof(T) == 4 ? NHV_F32 : NHV_BF16, a, t.p, stream);
+  if (rc) return rc;
+  NHV_CUDA(nhv_launch(scored_keys_kernel<T, DB, RPT>, dim3((unsigned)key_tiles, a.nkv, a.n_seqs), SA_THREADS, keys_smem, stream, t), "scored attention");
+  return scored_join_keys(a, t.p, stream);
+}
+
+template <typename T, int RPT>
+int launch_tiles(const TileArgs& t, cudaStream_t stream) {
+  return t.a.d <= 64 ? launch_tiles<T, 1, RPT>(t, stream) : t.a.d <= 128 ? launch_tiles<T, 2, RPT>(t, stream) : launch_tiles<T, 4, RPT>(t, stream);
+}
+
+// Rows of a tile, by eight: 64, or 8 or 16 where no request has more (fp32 alone: bfloat16 has its own kernels for few rows).
+int rows_per_thread(int dtype, int max_new, int G) {
+  const long long rows = (long long)max_new * G;
+  return dtype == NHV_BF16 || rows > 16 ? 8 : rows > 8 ? 2 : 1;
+}
+
+size_t tile_parts(ScoredParts& p, int dtype, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
+  p.tile_rows = 8 * rows_per_thread(dtype, max_new, nq / nkv);
+  p.tile_keys = SA_KEYS;
+  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, p.tile_rows, SA_KEYS, 2 * 148, 2 * 148);
 }
 
 }  // namespace
 
+size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d, int row_tile, int key_tile,
+                    int rows_at_once, int keys_at_once) {
+  const int G = nq / nkv;
+  // the rows' pass: parts of the keys only where whole walks would leave most SMs idle, and no part below eight tiles
+  const long long blocks = ((long long)n_tokens * G / row_tile + n_seqs) * nkv;        // at most
+  const int tiles = (max_keys + key_tile - 1) / key_tile;
+  long long splits = rows_at_once / blocks;
+  if (splits > tiles / 8) splits = tiles / 8;
+  if (splits < 1) splits = 1;
+  p.split_tiles = (int)((tiles + splits - 1) / splits);
+  p.splits = (tiles + p.split_tiles - 1) / p.split_tiles;
+  // the keys' pass: chunks of rows so that a few blocks come to each place that runs at once
+  const long long row_tiles = ((long long)max_new * G + p.tile_rows - 1) / p.tile_rows, key_tiles = (max_keys + p.tile_keys - 1) / p.tile_keys;
+  const long long pairs = ((long long)n_tokens * G / p.tile_rows + n_seqs) * key_tiles * nkv;
+  long long chunk = pairs / (keys_at_once * 8LL);
+  if (chunk < 4) chunk = 4;
+  if (chunk > row_tiles) chunk = row_tiles < 1 ? 1 : row_tiles;
+  p.chunk_tiles = (int)chunk;
+  p.chunks = (int)((row_tiles + chunk - 1) / chunk);
+  if (p.chunks < 1) p.chunks = 1;
+  p.keys = (size_t)key_tiles * p.tile_keys;
+  const size_t rows = (size_t)n_tokens * nq;
+  return (p.splits > 1 ? p.splits * rows * (d + 2) : 0) + (p.chunks > 1 ? (size_t)n_seqs * nkv * p.chunks * p.keys : 0) + 8;
+}
+
+void scored_place(ScoredParts& p, float* work, int n_tokens, int nq, int d) {
+  const size_t rows = p.splits > 1 ? (size_t)p.splits * n_tokens * nq : 0;
+  p.o = work;
+  p.ml = p.o + (rows * d + 3) / 4 * 4;
+  p.w = p.ml + rows * 2;
+}
+
+int scored_join_rows(int dtype, const ScoredArgs& a, const ScoredParts& p, cudaStream_t stream) {
+  if (p.splits <= 1) return 0;
+  const dim3 grid((unsigned)(((long long)a.n_tokens * a.nq + 7) / 8));
+  if (dtype == NHV_F32) NHV_CUDA(nhv_launch(scored_join_rows_kernel<float>, grid, 256, 0, stream, a, p), "scored attention");
+  else NHV_CUDA(nhv_launch(scored_join_rows_kernel<__nv_bfloat16>, grid, 256, 0, stream, a, p), "scored attention");
+  return 0;
+}
+
+int scored_join_keys(const ScoredArgs& a, const ScoredParts& p, cudaStream_t stream) {
+  if (p.chunks <= 1) return 0;
+  NHV_CUDA(nhv_launch(scored_join_keys_kernel, dim3((a.max_keys + 255) / 256, a.nkv, a.n_seqs), 256, 0, stream, a, p), "scored attention");
+  return 0;
+}
+
 // What a call needs beside its arguments, and which kernels take which requests: those of up to `short_rows` rows the kernels of
 // scored_attention_short.cu, the others the ones of scored_attention_tcgen05.cu, and what neither takes the kernels of this file.
 struct ScoredPlan {
-  int short_rows;           // -1: none go that way
-  bool many;                // requests above that go to the tcgen05 kernels
+  bool wide;                // rows that 16-byte loads can take
+  int short_rows;           // -1: none go the short way
+  bool rest, many;          // there may be others; they go to the tcgen05 kernels
   ShortPlan few;
-  LongPlan rest;
+  ScoredParts parts;
   size_t floats;            // of scratch
 };
 
-static ScoredPlan scored_plan(int dtype, int n_seqs, int n_tokens, int min_new, int max_new, int max_keys, int nq, int nkv, int d, int page_size,
-                              float scale) {
+static ScoredPlan scored_plan(int dtype, bool wide, int n_seqs, int n_tokens, int min_new, int max_new, int max_keys, int nq, int nkv, int d,
+                              int page_size, float scale) {
   ScoredPlan p = {};
+  p.wide = wide && d % 8 == 0;
   p.short_rows = -1;
   const int G = nq / nkv, most = d <= 128 ? 16 : 8;
-  size_t floats = 0;
-  if (scored_short_takes(dtype, min_new * G, d)) {
+  size_t few = 0, rest = 0;
+  if (p.wide && min_new <= most && scored_short_takes(dtype, min_new * G, d)) {
     p.short_rows = most;
     const int rows = max_new > most ? most : max_new * G;
     p.few = scored_short_plan(dtype, n_seqs, rows > most ? most : rows, max_keys, nkv, d);
-    floats = p.few.floats;
+    few = p.few.floats;
   }
-  p.many = max_new > most || max_new * G > p.short_rows;
-  if (p.many) p.many = scored_long_takes(dtype, nq, nkv, d, page_size, scale);
-  if (p.many) {
-    p.rest = scored_long_plan(n_seqs, n_tokens, max_new, max_keys, nq, nkv, d);
-    if (p.rest.floats > floats) floats = p.rest.floats;      // one after the other in the same scratch
+  p.rest = p.short_rows < 0 || max_new > most || max_new * G > most;
+  if (p.rest) {
+    p.many = p.wide && scored_long_takes(dtype, nq, nkv, d, page_size, scale);
+    rest = p.many ? scored_long_plan(p.parts, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d)
+                  : tile_parts(p.parts, dtype, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d);
   }
-  p.floats = ((size_t)n_tokens * nq + 3) / 4 * 4 + floats;
+  p.floats = ((size_t)n_tokens * nq + 3) / 4 * 4 + (few > rest ? few : rest);       // one after the other in the same scratch
   return p;
 }
 
-// Kilobytes of scratch that nhv_attention_scored wants for a call of these sizes.
-NHV_API int nhv_attention_scored_kilobytes(int dtype, int n_seqs, int n_tokens, int min_new, int max_new, int max_kv_len, int nq, int nkv, int d,
-                                           int page_size, float scale) {
-  if (n_seqs <= 0 || nkv <= 0 || nq < nkv || d <= 0 || page_size <= 0) return 0;
-  return (int)(scored_plan(dtype, n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d, page_size, scale).floats * sizeof(float) / 1024 + 1);
+static bool scored_wide(const void* q, int q_stride, const void* out, int out_stride, const void* kv_pages) {
+  return q_stride % 8 == 0 && out_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)kv_pages % 16 == 0;
+}
+
+// Kilobytes of scratch that nhv_attention_scored wants for a call of these arguments.
+NHV_API int nhv_attention_scored_kilobytes(int dtype, const void* q, int q_stride, const void* out, int out_stride, const void* kv_pages, int n_seqs,
+                                           int n_tokens, int min_new, int max_new, int max_kv_len, int nq, int nkv, int d, int page_size, float scale) {
+  if (n_seqs <= 0 || nkv <= 0 || nq < nkv || d <= 0 || page_size <= 0 || max_kv_len <= 0) return 0;
+  return (int)(scored_plan(dtype, scored_wide(q, q_stride, out, out_stride, kv_pages), n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d, page_size, scale)
+                       .floats * sizeof(float) / 1024 + 1);
 }
 
 NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* out, int out_stride, const void* kv_pages,
@@ -223,23 +523,27 @@ NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* o
   NHV_REQUIRE(!births == !positions || n_tokens == 0, "scored attention: births and positions go together");
   if (n_seqs == 0 || max_kv_len == 0) return 0;
   NHV_REQUIRE(n_seqs <= 65535, "scored attention: %d requests are beyond the grid's reach", n_seqs);
-  // rows that 16-byte loads cannot take go to the kernels of this file
-  const bool wide = d % 8 == 0 && q_stride % 8 == 0 && out_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 &&
-                    (uintptr_t)kv_pages % 16 == 0;
-  const ScoredPlan plan = scored_plan(dtype, n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d, page_size, scale);
+  ScoredPlan plan = scored_plan(dtype, scored_wide(q, q_stride, out, out_stride, kv_pages), n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d,
+                                page_size, scale);
   NHV_REQUIRE((size_t)work_kilobytes * 1024 >= plan.floats * sizeof(float) && (uintptr_t)work % 16 == 0, "scored attention: %d kilobytes of scratch are too few",
               work_kilobytes);
   ScoredArgs a{q, out, kv_pages, scores, scores_out, births, positions, block_table, cu_q, kv_len, sinks, work,
                q_stride, out_stride, bt_stride, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages, max_kv_len, 0, 0x7fffffff, scale, softcap};
   float* scratch = work + ((size_t)n_tokens * nq + 3) / 4 * 4;
-  if (wide && plan.short_rows >= 0) {
+  if (plan.short_rows >= 0) {
     a.max_rows = plan.short_rows;
     const int rc = scored_short_launch(dtype, a, plan.few, scratch, stream);
-    if (rc) return rc;
-    if (max_new <= plan.short_rows && max_new * (nq / nkv) <= plan.short_rows) return 0;
+    if (rc || !plan.rest) return rc;
     a.min_rows = plan.short_rows + 1;
     a.max_rows = 0x7fffffff;
   }
-  if (wide && plan.many) return scored_long_launch(a, plan.rest, scratch, stream);
-  return dtype == NHV_F32 ? launch_simt<float>(a, max_kv_len, stream) : launch_simt<__nv_bfloat16>(a, max_kv_len, stream);
+  scored_place(plan.parts, scratch, n_tokens, nq, d);
+  if (plan.many) return scored_long_launch(a, plan.parts, stream);
+  const TileArgs t{a, plan.parts, d % 4 == 0 && q_stride % 4 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)kv_pages % 16 == 0};
+  if (dtype == NHV_BF16) return launch_tiles<__nv_bfloat16, 8>(t, stream);
+  switch (rows_per_thread(dtype, max_new, nq / nkv)) {
+    case 1: return launch_tiles<float, 1>(t, stream);
+    case 2: return launch_tiles<float, 2>(t, stream);
+    default: return launch_tiles<float, 8>(t, stream);
+  }
 }

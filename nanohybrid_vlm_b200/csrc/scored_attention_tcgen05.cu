@@ -57,11 +57,8 @@ struct alignas(64) LongArgs {
   ScoredArgs a;
   NhvScoreCap cap;
   float scale_log2;
-  float* part_o;            // [splits][nkv][n_tokens * G][d]
-  float* part_ml;           // [splits][nkv][n_tokens * G][2]
-  float* part_w;            // [n_seqs][nkv][chunks][keys]
-  size_t keys;
-  int splits, split_tiles, chunks, chunk_tiles, key_tiles;
+  ScoredParts parts;
+  int key_tiles;
   int tokens, box;          // tokens of a tile of rows; rows of a TMA box of the pages
 };
 
@@ -240,12 +237,12 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
     n = a.cu_q[seq + 1] - first;
     total = min(a.kv_len[seq], a.max_keys);
     t0 = ((n + per_block - 1) / per_block - 1 - tile) * per_block;
-    key_begin = (int)blockIdx.z * p.split_tiles * BN;
+    key_begin = (int)blockIdx.z * p.parts.split_tiles * BN;
     for (int q = 0; q < NQ; ++q) {
       const int t_last = min(t0 + (q + 1) * p.tokens, n) - 1;
       if (t_last < t0 + q * p.tokens) continue;
       const int seen = total - n + t_last + 1 - key_begin;
-      nt[q] = seen <= 0 ? 0 : min((seen + BN - 1) / BN, p.split_tiles);
+      nt[q] = seen <= 0 ? 0 : min((seen + BN - 1) / BN, p.parts.split_tiles);
     }
     const int* table = a.block_table + (size_t)seq * a.bt_stride;
     const int page_end = (min(key_begin + max(nt[0], nt[1]) * BN, total) + a.page_size - 1) / a.page_size;
@@ -473,7 +470,7 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
       // the notes on values: made before the products that o_full covers
       for (int i = 0; i < 32; ++i) any_bad |= *(volatile uint32_t*)&s_bad[i] != 0;
       const size_t row = (size_t)kvh * a.n_tokens * G + (size_t)(first + token) * G + g;
-      const bool whole = p.splits == 1;
+      const bool whole = p.parts.splits == 1;
       float inv = 1.f;
       if (whole) {
         const float sink = a.sinks && valid ? a.sinks[kvh * G + g] * SA_LOG2E : -INFINITY;
@@ -484,12 +481,12 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
         inv = sum == 0.f ? 0.f : f / sum;
         if (valid) a.lse[row] = sum == 0.f ? INFINITY : ref + log2f(sum);
       } else if (valid) {
-        float* ml = p.part_ml + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * 2;
+        float* ml = p.parts.ml + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * 2;
         ml[0] = m;
         ml[1] = l;
       }
       bf16* dst = (bf16*)a.out + (size_t)(first + token) * a.out_stride + (size_t)(kvh * G + g) * a.d;
-      float* part = p.part_o + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * a.d;
+      float* part = p.parts.o + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * a.d;
 #pragma unroll 1
       for (int c0 = 0; c0 < DB * 64; c0 += 32) {
         uint32_t o[32];
@@ -552,45 +549,6 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
   }
 }
 
-// The sums of a row's parts joined: a warp per row.
-__global__ void __launch_bounds__(256) scored_rows_join_kernel(const __grid_constant__ LongArgs p) {
-  pdl_prologue();
-  const ScoredArgs& a = p.a;
-  const int G = a.nq / a.nkv, lane = threadIdx.x & 31;
-  const size_t rows = (size_t)a.nkv * a.n_tokens * G, row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int kvh = (int)(row / ((size_t)a.n_tokens * G)), r = (int)(row - (size_t)kvh * a.n_tokens * G), token = r / G, head = kvh * G + r % G;
-  int seq = 0;
-  while (seq + 1 < a.n_seqs && a.cu_q[seq + 1] <= token) ++seq;
-  if (!scored_takes(a, a.cu_q[seq + 1] - a.cu_q[seq])) return;
-  const float sink = a.sinks ? a.sinks[head] * SA_LOG2E : -INFINITY;
-  float ref = sink;
-  for (int s = 0; s < p.splits; ++s) ref = fmaxf(ref, p.part_ml[(s * rows + row) * 2]);
-  if (ref == -INFINITY) ref = 0.f;
-  float sum = scored_exp2(sink - ref);
-  for (int s = 0; s < p.splits; ++s) sum = fmaf(p.part_ml[(s * rows + row) * 2 + 1], scored_exp2(p.part_ml[(s * rows + row) * 2] - ref), sum);
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  bf16* dst = (bf16*)a.out + (size_t)token * a.out_stride + (size_t)head * a.d;
-  for (int c = 2 * lane; c < a.d; c += 64) {
-    float2 v = make_float2(0.f, 0.f);
-    for (int s = 0; s < p.splits; ++s) {
-      const float f = scored_exp2(p.part_ml[(s * rows + row) * 2] - ref);
-      const float2 x = *reinterpret_cast<const float2*>(p.part_o + (s * rows + row) * a.d + c);
-      v.x = fmaf(f, x.x, v.x);
-      v.y = fmaf(f, x.y, v.y);
-    }
-    *reinterpret_cast<uint32_t*>(dst + c) = pack_bf16(v.x * inv, v.y * inv);
-  }
-  if (lane == 0) a.lse[row] = sum == 0.f ? INFINITY : ref + log2f(sum);
-}
-
-// The tiles of rows [begin, end) of a request that see keys of tile `key0`, in chunk `chunk`.
-__device__ __forceinline__ void chunk_range(const LongArgs& p, int n, int total, int key0, int chunk, int& begin, int& end) {
-  const int first = max(0, key0 - (total - n)) / p.tokens, tiles = (n + p.tokens - 1) / p.tokens;
-  begin = max(first, chunk * p.chunk_tiles);
-  end = min(tiles, (chunk + 1) * p.chunk_tiles);
-}
-
 template <int DB>
 __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_keys_tcgen05_kernel(const __grid_constant__ LongArgs p) {
   using C = Keys<DB>;
@@ -635,7 +593,7 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
   const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
   int begin = 0, end = 0;
   const bool mine = key0 < total && scored_takes(a, n);
-  if (mine) chunk_range(p, n, total, key0, chunk, begin, end);
+  if (mine) chunk_range(p.parts, n, G, total, key0, chunk, begin, end);
   const int n_tiles = max(0, end - begin);
   tc_fence_before();
   __syncthreads();
@@ -737,8 +695,8 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
     }
     if (!ok) *s_abort = 1;
     else if (key < total) {
-      if (p.chunks == 1) store_weight(a, seq, first, kvh, key, key - (total - n), sum);
-      else if (n_tiles > 0) p.part_w[(((size_t)seq * a.nkv + kvh) * p.chunks + chunk) * p.keys + key] = sum;
+      if (p.parts.chunks == 1) store_weight(a, seq, first, kvh, key, key - (total - n), sum);
+      else if (n_tiles > 0) p.parts.w[(((size_t)seq * a.nkv + kvh) * p.parts.chunks + chunk) * p.parts.keys + key] = sum;
     }
   }
   tc_fence_before();
@@ -747,22 +705,6 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
     tc_fence_after();
     tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
-}
-
-// The chunks' sums added in their order: a thread per key.
-__global__ void __launch_bounds__(256) scored_keys_join_kernel(const __grid_constant__ LongArgs p) {
-  pdl_prologue();
-  const ScoredArgs& a = p.a;
-  const int seq = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
-  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
-  if (key >= total || !scored_takes(a, n)) return;
-  float sum = 0.f;
-  for (int c = 0; c < p.chunks; ++c) {
-    int begin, end;
-    chunk_range(p, n, total, key / BM * BM, c, begin, end);
-    if (begin < end) sum += p.part_w[(((size_t)seq * a.nkv + kvh) * p.chunks + c) * p.keys + key];
-  }
-  store_weight(a, seq, first, kvh, key, key - (total - n), sum);
 }
 
 bool make_q_map(CUtensorMap* map, const ScoredArgs& a, int tokens) {
@@ -779,15 +721,13 @@ int launch_long(const LongArgs& p, int row_tiles, cudaStream_t stream) {
   const ScoredArgs& a = p.a;
   NHV_CUDA(nhv_allow_smem((const void*)scored_rows_tcgen05_kernel<DB>, Rows<DB>::SMEM, rows_done), "scored attention (tcgen05)");
   NHV_CUDA(nhv_allow_smem((const void*)scored_keys_tcgen05_kernel<DB>, Keys<DB>::SMEM, keys_done), "scored attention (tcgen05)");
-  NHV_CUDA(nhv_launch(scored_rows_tcgen05_kernel<DB>, dim3(a.nkv, row_tiles, p.splits), Rows<DB>::THREADS, Rows<DB>::SMEM, stream, p),
+  NHV_CUDA(nhv_launch(scored_rows_tcgen05_kernel<DB>, dim3(a.nkv, row_tiles, p.parts.splits), Rows<DB>::THREADS, Rows<DB>::SMEM, stream, p),
            "scored attention (tcgen05)");
-  if (p.splits > 1)
-    NHV_CUDA(nhv_launch(scored_rows_join_kernel, dim3((unsigned)(((long long)a.n_tokens * a.nq + 7) / 8)), 256, 0, stream, p), "scored attention (tcgen05)");
-  NHV_CUDA(nhv_launch(scored_keys_tcgen05_kernel<DB>, dim3(a.nkv, p.key_tiles * p.chunks, a.n_seqs), Keys<DB>::THREADS, Keys<DB>::SMEM, stream, p),
+  int rc = scored_join_rows(NHV_BF16, a, p.parts, stream);
+  if (rc) return rc;
+  NHV_CUDA(nhv_launch(scored_keys_tcgen05_kernel<DB>, dim3(a.nkv, p.key_tiles * p.parts.chunks, a.n_seqs), Keys<DB>::THREADS, Keys<DB>::SMEM, stream, p),
            "scored attention (tcgen05)");
-  if (p.chunks > 1)
-    NHV_CUDA(nhv_launch(scored_keys_join_kernel, dim3((a.max_keys + 255) / 256, a.nkv, a.n_seqs), 256, 0, stream, p), "scored attention (tcgen05)");
-  return 0;
+  return scored_join_keys(a, p.parts, stream);
 }
 
 }  // namespace
@@ -799,48 +739,21 @@ bool scored_long_takes(int dtype, int nq, int nkv, int d, int page_size, float s
   return scale > 0.f && dtype == NHV_BF16 && d % 8 == 0 && d <= SA_MAX_D && nq / nkv <= BM && page_size % 8 == 0;
 }
 
-LongPlan scored_long_plan(int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
-  LongPlan p = {};
-  const int G = nq / nkv, tokens = BM / G, per_block = (d <= 128 ? 2 : 1) * tokens, bn = d <= 128 ? 128 : 64;
-  const long long blocks = ((long long)n_tokens / per_block + n_seqs) * nkv;       // at most
-  // the rows' pass: parts of the keys only where whole walks would leave most SMs idle, and no part below eight tiles
-  const int tiles = (max_keys + bn - 1) / bn;
-  long long splits = SMS / blocks;
-  if (splits > tiles / 8) splits = tiles / 8;
-  p.splits = splits < 1 ? 1 : (int)splits;
-  p.split_tiles = (tiles + p.splits - 1) / p.splits;
-  // the keys' pass: chunks of rows so that a few blocks come to each place that runs at once (two an SM)
-  const long long row_tiles = ((long long)max_new + tokens - 1) / tokens, key_tiles = (max_keys + BM - 1) / BM;
-  const long long pairs = ((long long)n_tokens / tokens + n_seqs) * key_tiles * nkv;
-  long long chunk = pairs / (2 * SMS * 8);
-  if (chunk < 4) chunk = 4;
-  if (chunk > row_tiles) chunk = row_tiles < 1 ? 1 : row_tiles;
-  p.chunk_tiles = (int)chunk;
-  p.chunks = (int)((row_tiles + chunk - 1) / chunk);
-  if (p.chunks < 1) p.chunks = 1;
-  p.keys = (size_t)key_tiles * BM;
-  const size_t rows = (size_t)n_tokens * nq;
-  p.floats = (p.splits > 1 ? p.splits * rows * (d + 2) : 0) + (p.chunks > 1 ? (size_t)n_seqs * nkv * p.chunks * p.keys : 0);
-  return p;
+size_t scored_long_plan(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
+  const int G = nq / nkv, tokens = BM / G;
+  p.tile_rows = tokens * G;
+  p.tile_keys = BM;
+  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, (d <= 128 ? 2 : 1) * tokens * G, d <= 128 ? 128 : 64, SMS, 2 * SMS);
 }
 
-int scored_long_launch(ScoredArgs a, const LongPlan& plan, float* work, cudaStream_t stream) {
-  const int G = a.nq / a.nkv;
+int scored_long_launch(ScoredArgs a, const ScoredParts& parts, cudaStream_t stream) {
   LongArgs p;
   p.a = a;
   p.cap = nhv_score_cap(a.scale, a.softcap);
   p.scale_log2 = a.softcap > 0.f ? 1.0f : a.scale * SA_LOG2E;
-  p.tokens = BM / G;
-  p.splits = plan.splits;
-  p.split_tiles = plan.split_tiles;
-  p.chunks = plan.chunks;
-  p.chunk_tiles = plan.chunk_tiles;
-  p.keys = plan.keys;
-  p.key_tiles = (int)(plan.keys / BM);
-  const size_t rows = (size_t)a.n_tokens * a.nq;
-  p.part_o = work;
-  p.part_ml = p.part_o + (plan.splits > 1 ? plan.splits * rows * a.d : 0);
-  p.part_w = p.part_ml + (plan.splits > 1 ? plan.splits * rows * 2 : 0);
+  p.parts = parts;
+  p.tokens = BM / (a.nq / a.nkv);
+  p.key_tiles = (int)(parts.keys / BM);
   const int db = (a.d + 63) / 64, nq_tiles = db <= 2 ? 2 : 1, bn = db <= 2 ? 128 : 64;
   p.box = divisor(a.page_size, bn);
   const long long pool = (long long)a.n_pages * 2 * a.nkv * a.page_size;
@@ -848,8 +761,8 @@ int scored_long_launch(ScoredArgs a, const LongPlan& plan, float* work, cudaStre
   NHV_REQUIRE(nhv_make_map_bf16(&p.kv_map, a.pages, pool, a.d, a.d, 64, p.box), "scored attention (tcgen05): cannot encode the tensor map of the pool");
   NHV_REQUIRE(make_q_map(&p.q_map, a, p.tokens), "scored attention (tcgen05): cannot encode the tensor map of q");
   const long long row_tiles = (long long)a.n_tokens / (nq_tiles * p.tokens) + a.n_seqs;
-  NHV_REQUIRE(row_tiles <= 65535 && (long long)p.key_tiles * p.chunks <= 65535, "scored attention (tcgen05): %lld tiles of rows, %d of keys in %d chunks are beyond the grid's reach",
-              row_tiles, p.key_tiles, p.chunks);
+  NHV_REQUIRE(row_tiles <= 65535 && (long long)p.key_tiles * parts.chunks <= 65535, "scored attention (tcgen05): %lld tiles of rows, %d of keys in %d chunks are beyond the grid's reach",
+              row_tiles, p.key_tiles, parts.chunks);
   switch (db) {
     case 1: return launch_long<1>(p, (int)row_tiles, stream);
     case 2: return launch_long<2>(p, (int)row_tiles, stream);

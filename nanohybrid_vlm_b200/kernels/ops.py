@@ -1241,8 +1241,9 @@ def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs
         raise KernelError(f"scores_out is float32 of the scores' shape {tuple(scores.shape)} and contiguous")
     _need_cuda(scores_out)
     dt = dtype_code(q)
-    kilobytes = library.load_library().nhv_attention_scored_kilobytes(dt, n_seqs, T, min_new, max_new, max_kv_len, nq, nkv, head_dim, page_size,
-                                                                      float(scale))
+    kilobytes = library.load_library().nhv_attention_scored_kilobytes(
+        dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv_pages.data_ptr(), n_seqs, T, min_new, max_new, max_kv_len, nq, nkv,
+        head_dim, page_size, float(scale))
     work = torch.empty(kilobytes * 256, dtype=torch.float32, device=q.device)
     call("nhv_attention_scored", dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv_pages.data_ptr(),
          scores.data_ptr(), scores_out.data_ptr(), _ptr(births), _ptr(positions), block_table.data_ptr(), block_table.stride(0),
