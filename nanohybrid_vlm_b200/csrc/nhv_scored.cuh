@@ -81,9 +81,10 @@ __device__ __forceinline__ void chunk_range(const ScoredParts& p, int n, int G, 
   begin = first > chunk * p.chunk_tiles ? first : chunk * p.chunk_tiles;
   end = tiles < (chunk + 1) * p.chunk_tiles ? tiles : (chunk + 1) * p.chunk_tiles;
 }
-// Fills in splits and chunks and the scratch they take; `row_tile` and `key_tile`: of the rows' pass; blocks that run at once in each.
+// Fills in splits and chunks and the scratch they take; `row_tile` and `key_tile`: of the rows' pass, which takes
+// about `tile_cycles` for one of each; blocks that run at once in either pass.
 size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d, int row_tile, int key_tile,
-                    int rows_at_once, int keys_at_once);
+                    double tile_cycles, int rows_at_once, int keys_at_once);
 void scored_place(ScoredParts& p, float* work, int n_tokens, int nq, int d);
 int scored_join_rows(int dtype, const ScoredArgs& a, const ScoredParts& p, cudaStream_t stream);
 int scored_join_keys(const ScoredArgs& a, const ScoredParts& p, cudaStream_t stream);

@@ -6,12 +6,15 @@
 //
 // The entry point, and kernels for any type, size and page size that compute in fp32 on the CUDA cores (the 32-bit path, and what
 // the tensor-core kernels of scored_attention_short.cu and scored_attention_tcgen05.cu refuse).
-//   rows: 128 threads hold 8 RPT rows (row = token * G + head, of one request and KV head) and walk the keys in tiles of 64 through
+//   rows: 256 threads hold 16 RPT rows (row = token * G + head, of one request and KV head) and walk the keys in tiles of 64 through
 //     shared memory.  A thread makes RPT x 4 scores from 16-byte reads along the head and RPT x 4 DB outputs, two multiply-adds
-//     an instruction; P passes through shared memory, over the keys.  RPT is 8, and 1 or 2 where no request has more rows.
-//   keys: 64 keys stay in shared memory, the tiles of rows pass by; a thread adds up the weights of its 4 keys, the eight row groups
+//     an instruction; P passes through shared memory.  RPT is 8 (4 for heads above 128), and 1 where no request has more than 16 rows.
+//     A tile's values arrive while its scores are made, the next tile's keys while the values are used.
+//   keys: 64 keys stay in shared memory, the tiles of rows pass by; a thread adds up the weights of its 4 keys, the sixteen row groups
 //     meet in shared memory at the end.
-// What bounds them is multiply-adds: 4 D a pair in the first, 2 D in the second, of 128 a cycle and SM.
+// What bounds them is multiply-adds, 4 D a pair in the first and 2 D in the second, of 128 a cycle and SM, and beside them the 16-byte
+// reads of shared memory, four cycles each however many lanes read the same: 12 for 128 multiply-adds a thread in the scores, 16 for
+// 256 in the outputs.
 // Long walks over the keys are split over blocks where there are few tiles of rows, and rows into chunks in the keys' pass; two
 // small kernels join the parts in a fixed order.  No sum depends on the order in which blocks run.
 //
@@ -21,7 +24,7 @@
 
 namespace {
 
-constexpr int SA_THREADS = 128, SA_KEYS = 64;
+constexpr int SA_THREADS = 256, SA_KEYS = 64;
 
 struct TileArgs {
   ScoredArgs a;
@@ -36,17 +39,25 @@ template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bf
   return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
 
-// `rows` rows of d elements at base + at[r] into shared memory, `stride` floats apart, as fp32; at[r] < 0: zeros.  The last four
-// columns that d reaches into are filled up with zeros.
-template <typename T>
-__device__ __forceinline__ void load_rows(float* dst, int stride, const T* base, const long long* at, int rows, int d, bool vec) {
-  const int per_row = (d + 3) / 4;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < rows * per_row; i += SA_THREADS) {
-    const int r = i / per_row, c = (i - r * per_row) * 4;
+// ROWS rows of d elements at base + at[r] into shared memory, `stride` floats apart, as fp32, and committed as one group of
+// asynchronous copies (float32 rows that can be read by 16 bytes; others are there when this returns).  at[r] < 0: zeros.  The last
+// four columns that d reaches into are filled up with zeros.
+template <typename T, int DB, int ROWS>
+__device__ __forceinline__ void load_rows(float* dst, int stride, const T* base, const long long* at, int d, bool vec) {
+  constexpr int PER_ROW = 16 * DB;
+#pragma unroll
+  for (int i = threadIdx.x; i < ROWS * PER_ROW; i += SA_THREADS) {
+    const int r = i / PER_ROW, c = (i - r * PER_ROW) * 4;
+    if (c >= d) continue;
+    const T* src = base + at[r] + c;
+    const bool there = at[r] >= 0;
+    if (sizeof(T) == 4 && vec) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst + r * stride + c)), "l"(there ? src : base),
+                   "r"(there ? 16 : 0) : "memory");
+      continue;
+    }
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (at[r] >= 0) {
-      const T* src = base + at[r] + c;
+    if (there) {
       if (vec) {
         v = load4<T>(src);
       } else {
@@ -58,7 +69,11 @@ __device__ __forceinline__ void load_rows(float* dst, int stride, const T* base,
     }
     *reinterpret_cast<float4*>(dst + r * stride + c) = v;
   }
+  asm volatile("cp.async.commit_group;\n" ::: "memory");
 }
+// All groups but the last N have arrived (this thread's copies).
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 // s[i][k] = row (ty RPT + i) . key (tx + 16 k)
 template <int RPT>
@@ -100,14 +115,14 @@ __device__ __forceinline__ float scaled(float s, const ScoredArgs& a) {
 
 // DB: blocks of 64 elements of a head.
 template <typename T, int DB, int RPT>
-__global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_rows_kernel(const TileArgs t) {
+__global__ void __launch_bounds__(SA_THREADS, 1) scored_rows_kernel(const TileArgs t) {
   extern __shared__ __align__(16) float smem[];
-  __shared__ long long s_at[SA_KEYS], s_v[SA_KEYS];
-  constexpr int ROWS = 8 * RPT, DP = 64 * DB, STRIDE = DP + 4, PS = SA_KEYS + 4;
+  constexpr int ROWS = 16 * RPT, DP = 64 * DB, STRIDE = DP + 4, PS = SA_KEYS + 4;
+  __shared__ long long s_q[ROWS], s_at[2][SA_KEYS];      // where rows of q begin, and keys of this tile and the next
   float* Qs = smem;                       // [ROWS][STRIDE]
-  float* Ks = Qs + ROWS * STRIDE;         // [64][STRIDE], and then P [ROWS][PS]
+  float* Ks = Qs + ROWS * STRIDE;         // [64][STRIDE]
   float* Vs = Ks + SA_KEYS * STRIDE;      // [64][DP]
-  float* Ps = Ks;
+  float* Ps = Vs + SA_KEYS * DP;          // [ROWS][PS]
   pdl_prologue();
   const ScoredArgs& a = t.a;
   const int G = a.nq / a.nkv, kvh = blockIdx.y, tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, d = a.d;
@@ -131,9 +146,19 @@ __global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_rows_kerne
   const int all = total - n + r0 / G;                                          // every row sees keys up to here
   const int key_end = min(last + 1, key_begin + t.p.split_tiles * SA_KEYS);
   const T* pages = (const T*)a.pages;
-  if (tid < ROWS) s_at[tid] = tid < rows ? (long long)(first + (r0 + tid) / G) * a.q_stride + (long long)(kvh * G + (r0 + tid) % G) * d : -1;
+  const T* values = pages + (long long)a.nkv * a.page_size * d;               // the plane behind a page's keys
+  auto place = [&](int j0, long long* at) {
+    if (tid < SA_KEYS) at[tid] = j0 + tid < key_end ? key_row(a, seq, j0 + tid, kvh, 0) : -1;
+  };
+  for (int r = tid; r < ROWS; r += SA_THREADS)
+    s_q[r] = r < rows ? (long long)(first + (r0 + r) / G) * a.q_stride + (long long)(kvh * G + (r0 + r) % G) * d : -1;
+  place(key_begin, s_at[0]);
   __syncthreads();
-  load_rows<T>(Qs, STRIDE, (const T*)a.q, s_at, ROWS, d, t.vec);
+  if (key_begin < key_end) {
+    load_rows<T, DB, ROWS>(Qs, STRIDE, (const T*)a.q, s_q, d, t.vec);
+    load_rows<T, DB, SA_KEYS>(Ks, STRIDE, pages, s_at[0], d, t.vec);
+    load_rows<T, DB, SA_KEYS>(Vs, DP, values, s_at[0], d, t.vec);
+  }
 
   float m[RPT], l[RPT];
   f32x2 o[RPT][2 * DB];                   // columns 64 b + 4 tx .. + 3
@@ -147,31 +172,24 @@ __global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_rows_kerne
 #pragma unroll
     for (int c = 0; c < 2 * DB; ++c) o[i][c] = 0ull;
   }
-  for (int j0 = key_begin; j0 < key_end; j0 += SA_KEYS) {
-    __syncthreads();
-    if (tid < SA_KEYS) {
-      const int j = j0 + tid;
-      s_at[tid] = j < key_end ? key_row(a, seq, j, kvh, 0) : -1;
-      s_v[tid] = j < key_end ? key_row(a, seq, j, kvh, 1) : -1;
-    }
+  int cur = 0;
+  for (int j0 = key_begin; j0 < key_end; j0 += SA_KEYS, cur ^= 1) {
+    const long long* at = s_at[cur];
+    wait_loads<1>();                      // the keys
     // some row does not see some key of the tile
-    const bool masked = __syncthreads_or(tid < SA_KEYS && s_at[tid & (SA_KEYS - 1)] < 0) || j0 + SA_KEYS - 1 > all;
-    load_rows<T>(Ks, STRIDE, pages, s_at, SA_KEYS, d, t.vec);
-    load_rows<T>(Vs, DP, pages, s_v, SA_KEYS, d, t.vec);
-    __syncthreads();
+    const bool masked = __syncthreads_or(tid < SA_KEYS && at[tid & (SA_KEYS - 1)] < 0) || j0 + SA_KEYS - 1 > all;
+    place(j0 + SA_KEYS, s_at[cur ^ 1]);
     float s[RPT][4];
     tile_scores<RPT>(s, Qs, Ks, STRIDE, d, ty, tx);
-    uint32_t sees = 0xffffffffu;          // bit 4 i + k
+    __syncthreads();
+    load_rows<T, DB, SA_KEYS>(Ks, STRIDE, pages, s_at[cur ^ 1], d, t.vec);       // zeros behind the last tile
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       float top = -INFINITY;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         s[i][k] = scaled(s[i][k], a);
-        if (masked && (j0 + tx + 16 * k > hi[i] || s_at[tx + 16 * k] < 0)) {
-          s[i][k] = -INFINITY;
-          sees &= ~(1u << (4 * i + k));
-        }
+        if (masked && (j0 + tx + 16 * k > hi[i] || at[tx + 16 * k] < 0)) s[i][k] = -INFINITY;
         top = fmaxf(top, s[i][k]);
       }
 #pragma unroll
@@ -182,6 +200,7 @@ __global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_rows_kerne
       for (int k = 0; k < 4; ++k) {
         s[i][k] = scored_exp2(s[i][k] - use);
         sum += s[i][k];
+        Ps[(ty * RPT + i) * PS + tx + 16 * k] = s[i][k];
       }
       l[i] = fmaf(l[i], alpha, sum);      // this thread's keys; the sixteen threads of a row meet at the end
       m[i] = ref;
@@ -189,13 +208,16 @@ __global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_rows_kerne
 #pragma unroll
       for (int c = 0; c < 2 * DB; ++c) o[i][c] = f2_mul(o[i][c], aa);
     }
+    wait_loads<1>();                      // the values
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < RPT; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) Ps[(ty * RPT + i) * PS + tx + 16 * k] = s[i][k];
-    __syncthreads();
-    if (!masked) {
+    bool each = false;
+    if (masked) {                         // 0 times a value is nothing only if the value is a number
+      bool odd = false;
+      for (int i = tid; i < SA_KEYS * DP; i += SA_THREADS)
+        if (i % DP < d) odd |= !(fabsf(Vs[i]) < INFINITY);
+      each = __syncthreads_or(odd);
+    }
+    if (!each) {
 #pragma unroll 2
       for (int j = 0; j < SA_KEYS; j += 4) {
         float4 p[RPT];
@@ -221,7 +243,7 @@ __global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_rows_kerne
       }
     } else {
       for (int j = 0; j < SA_KEYS && j0 + j < key_end; ++j) {
-        if (s_at[j] < 0) continue;
+        if (at[j] < 0) continue;
         f32x2 v[2 * DB];
 #pragma unroll
         for (int b = 0; b < DB; ++b) {
@@ -239,7 +261,10 @@ __global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_rows_kerne
         }
       }
     }
+    __syncthreads();
+    load_rows<T, DB, SA_KEYS>(Vs, DP, values, s_at[cur ^ 1], d, t.vec);
   }
+  wait_loads<0>();
   T* out = (T*)a.out;
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
@@ -282,13 +307,13 @@ __global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_rows_kerne
 }
 
 template <typename T, int DB, int RPT>
-__global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_keys_kernel(const TileArgs t) {
+__global__ void __launch_bounds__(SA_THREADS, 1) scored_keys_kernel(const TileArgs t) {
   extern __shared__ __align__(16) float smem[];
-  __shared__ long long s_at[SA_KEYS];
-  __shared__ float s_lse[64], s_part[8][SA_KEYS];
-  constexpr int ROWS = 8 * RPT, STRIDE = 64 * DB + 4;
-  float* Qs = smem;                       // [ROWS][STRIDE]
-  float* Ks = Qs + ROWS * STRIDE;         // [64][STRIDE]
+  constexpr int ROWS = 16 * RPT, STRIDE = 64 * DB + 4;
+  __shared__ long long s_k[SA_KEYS], s_q[2][ROWS];
+  __shared__ float s_lse[2][ROWS], s_part[16][SA_KEYS];
+  float* Ks = smem;                       // [64][STRIDE]
+  float* Qs = Ks + SA_KEYS * STRIDE;      // [2][ROWS][STRIDE]
   pdl_prologue();
   const ScoredArgs& a = t.a;
   const int G = a.nq / a.nkv, kvh = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, d = a.d;
@@ -298,39 +323,50 @@ __global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 2 : 1) scored_keys_kerne
   int begin, end;
   chunk_range(t.p, n, G, total, key0, chunk, begin, end);
   if (t.p.chunks > 1 && begin >= end) return;
-  if (tid < SA_KEYS) s_at[tid] = key0 + tid < total ? key_row(a, seq, key0 + tid, kvh, 0) : -1;
-  __syncthreads();
-  load_rows<T>(Ks, STRIDE, (const T*)a.pages, s_at, SA_KEYS, d, t.vec);
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = begin; i0 < end; ++i0) {
-    const int r0 = i0 * ROWS, rows = min(ROWS, n * G - r0);
-    __syncthreads();
-    if (tid < ROWS) {
-      s_at[tid] = tid < rows ? (long long)(first + (r0 + tid) / G) * a.q_stride + (long long)(kvh * G + (r0 + tid) % G) * d : -1;
-      s_lse[tid] = tid < rows ? a.lse[(size_t)kvh * a.n_tokens * G + (size_t)first * G + r0 + tid] : INFINITY;
+  auto place = [&](int i0, int buf) {
+    for (int r = tid; r < ROWS; r += SA_THREADS) {
+      const int row = i0 * ROWS + r;
+      const bool in = i0 < end && row < n * G;
+      s_q[buf][r] = in ? (long long)(first + row / G) * a.q_stride + (long long)(kvh * G + row % G) * d : -1;
+      s_lse[buf][r] = in ? a.lse[(size_t)kvh * a.n_tokens * G + (size_t)first * G + row] : INFINITY;
     }
+  };
+  if (tid < SA_KEYS) s_k[tid] = key0 + tid < total ? key_row(a, seq, key0 + tid, kvh, 0) : -1;
+  place(begin, 0);
+  __syncthreads();
+  if (begin < end) {
+    load_rows<T, DB, SA_KEYS>(Ks, STRIDE, (const T*)a.pages, s_k, d, t.vec);
+    load_rows<T, DB, ROWS>(Qs, STRIDE, (const T*)a.q, s_q[0], d, t.vec);
+  }
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  int cur = 0;
+  for (int i0 = begin; i0 < end; ++i0, cur ^= 1) {
+    place(i0 + 1, cur ^ 1);
     __syncthreads();
-    load_rows<T>(Qs, STRIDE, (const T*)a.q, s_at, ROWS, d, t.vec);
+    load_rows<T, DB, ROWS>(Qs + (cur ^ 1) * ROWS * STRIDE, STRIDE, (const T*)a.q, s_q[cur ^ 1], d, t.vec);      // zeros behind the last tile
+    wait_loads<1>();
     __syncthreads();
     float s[RPT][4];
-    tile_scores<RPT>(s, Qs, Ks, STRIDE, d, ty, tx);
+    tile_scores<RPT>(s, Qs + cur * ROWS * STRIDE, Ks, STRIDE, d, ty, tx);
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
-      const int r = ty * RPT + i, hi = r < rows ? total - n + (r0 + r) / G : -1;
+      const int r = ty * RPT + i, row = i0 * ROWS + r, hi = row < n * G ? total - n + row / G : -1;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float p = scored_exp2(scaled(s[i][k], a) - s_lse[r]);
+        const float p = scored_exp2(scaled(s[i][k], a) - s_lse[cur][r]);
         if (key0 + tx + 16 * k <= hi) w[k] += p;
       }
     }
+    __syncthreads();
   }
+  wait_loads<0>();
 #pragma unroll
   for (int k = 0; k < 4; ++k) s_part[ty][tx + 16 * k] = w[k];
   __syncthreads();
   if (tid < SA_KEYS && key0 + tid < total) {
     float sum = 0.f;
 #pragma unroll
-    for (int y = 0; y < 8; ++y) sum += s_part[y][tid];
+    for (int y = 0; y < 16; ++y) sum += s_part[y][tid];
     if (t.p.chunks == 1) store_weight(a, seq, first, kvh, key0 + tid, key0 + tid - (total - n), sum);
     else t.p.w[(((size_t)seq * a.nkv + kvh) * t.p.chunks + chunk) * t.p.keys + key0 + tid] = sum;
   }
@@ -383,8 +419,9 @@ __global__ void __launch_bounds__(256) scored_join_keys_kernel(const ScoredArgs 
 template <typename T, int DB, int RPT>
 int launch_tiles(const TileArgs& t, cudaStream_t stream) {
   static std::atomic<uint64_t> rows_done{0}, keys_done{0};
-  constexpr int ROWS = 8 * RPT, STRIDE = 64 * DB + 4;
-  constexpr size_t rows_smem = sizeof(float) * (ROWS * STRIDE + SA_KEYS * STRIDE + SA_KEYS * 64 * DB), keys_smem = sizeof(float) * (ROWS + SA_KEYS) * STRIDE;
+  constexpr int ROWS = 16 * RPT, STRIDE = 64 * DB + 4;
+  constexpr size_t rows_smem = sizeof(float) * ((ROWS + SA_KEYS) * STRIDE + SA_KEYS * 64 * DB + ROWS * (SA_KEYS + 4));
+  constexpr size_t keys_smem = sizeof(float) * (2 * ROWS + SA_KEYS) * STRIDE;
   const ScoredArgs& a = t.a;
   const long long tiles = (long long)a.n_tokens * (a.nq / a.nkv) / ROWS + a.n_seqs, key_tiles = (long long)(t.p.keys / SA_KEYS) * t.p.chunks;
   NHV_REQUIRE(tiles < (1LL << 31) && key_tiles < (1LL << 31), "scored attention: %lld tiles of rows, %lld of keys are beyond the grid's reach", tiles, key_tiles);
@@ -397,35 +434,42 @@ int launch_tiles(const TileArgs& t, cudaStream_t stream) {
   return scored_join_keys(a, t.p, stream);
 }
 
-template <typename T, int RPT>
-int launch_tiles(const TileArgs& t, cudaStream_t stream) {
-  return t.a.d <= 64 ? launch_tiles<T, 1, RPT>(t, stream) : t.a.d <= 128 ? launch_tiles<T, 2, RPT>(t, stream) : launch_tiles<T, 4, RPT>(t, stream);
-}
-
-// Rows of a tile, by eight: 64, or 8 or 16 where no request has more (fp32 alone: bfloat16 has its own kernels for few rows).
-int rows_per_thread(int dtype, int max_new, int G) {
-  const long long rows = (long long)max_new * G;
-  return dtype == NHV_BF16 || rows > 16 ? 8 : rows > 8 ? 2 : 1;
+// Rows of a thread of the tiles' sixteen row groups.
+int rows_per_thread(int dtype, int max_new, int G, int d) {
+  // bfloat16 has kernels of its own for few rows
+  return dtype == NHV_F32 && (long long)max_new * G <= 16 ? 1 : d <= 128 ? 8 : 4;
 }
 
 size_t tile_parts(ScoredParts& p, int dtype, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
-  p.tile_rows = 8 * rows_per_thread(dtype, max_new, nq / nkv);
+  p.tile_rows = 16 * rows_per_thread(dtype, max_new, nq / nkv, d);
   p.tile_keys = SA_KEYS;
-  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, p.tile_rows, SA_KEYS, 2 * 148, 2 * 148);
+  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, p.tile_rows, SA_KEYS, p.tile_rows * SA_KEYS * d / 50.0, 148, 148);
 }
 
 }  // namespace
 
 size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d, int row_tile, int key_tile,
-                    int rows_at_once, int keys_at_once) {
+                    double tile_cycles, int rows_at_once, int keys_at_once) {
   const int G = nq / nkv;
-  // the rows' pass: parts of the keys only where whole walks would leave most SMs idle, and no part below eight tiles
+  // the rows' pass: parts of the keys where whole walks fill the SMs badly.  With `blocks` walks and `at_once` places, s parts take
+  // ceil(blocks s / at_once) / s walks' time, and each part's sums are written and read once, 8 bytes an element at some 30 bytes a
+  // cycle; no part is below `least` tiles.  Walks of a prompt without earlier keys are of every length, and their longest go first:
+  // there parts pay only if SMs would idle.
   const long long blocks = ((long long)n_tokens * G / row_tile + n_seqs) * nkv;        // at most
-  const int tiles = (max_keys + key_tile - 1) / key_tile;
-  long long splits = rows_at_once / blocks;
-  if (splits > tiles / 8) splits = tiles / 8;
-  if (splits < 1) splits = 1;
-  p.split_tiles = (int)((tiles + splits - 1) / splits);
+  const int tiles = (max_keys + key_tile - 1) / key_tile, least = key_tile * row_tile >= 128 * 128 ? 8 : 3;
+  const bool alike = max_keys >= 2 * max_new;
+  int splits = 1;
+  double best = 1e30;
+  const double sums = row_tile * d * 8 / 30.0 / (tile_cycles * tiles);
+  for (int s = 1; s <= 64 && (s == 1 || tiles / s >= least); ++s) {
+    const double waves = alike || blocks * s <= rows_at_once ? (double)((blocks * s + rows_at_once - 1) / rows_at_once) : (double)blocks * s / rows_at_once;
+    const double cost = waves / s + (s > 1 ? s * sums : 0.0);
+    if (cost < best - 1e-9) {
+      best = cost;
+      splits = s;
+    }
+  }
+  p.split_tiles = (tiles + splits - 1) / splits;
   p.splits = (tiles + p.split_tiles - 1) / p.split_tiles;
   // the keys' pass: chunks of rows so that a few blocks come to each place that runs at once
   const long long row_tiles = ((long long)max_new * G + p.tile_rows - 1) / p.tile_rows, key_tiles = (max_keys + p.tile_keys - 1) / p.tile_keys;
@@ -540,10 +584,10 @@ NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* o
   scored_place(plan.parts, scratch, n_tokens, nq, d);
   if (plan.many) return scored_long_launch(a, plan.parts, stream);
   const TileArgs t{a, plan.parts, d % 4 == 0 && q_stride % 4 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)kv_pages % 16 == 0};
-  if (dtype == NHV_BF16) return launch_tiles<__nv_bfloat16, 8>(t, stream);
-  switch (rows_per_thread(dtype, max_new, nq / nkv)) {
-    case 1: return launch_tiles<float, 1>(t, stream);
-    case 2: return launch_tiles<float, 2>(t, stream);
-    default: return launch_tiles<float, 8>(t, stream);
-  }
+  const int db = d <= 64 ? 1 : d <= 128 ? 2 : 4;
+  if (dtype == NHV_BF16)
+    return db == 1 ? launch_tiles<__nv_bfloat16, 1, 8>(t, stream) : db == 2 ? launch_tiles<__nv_bfloat16, 2, 8>(t, stream) : launch_tiles<__nv_bfloat16, 4, 4>(t, stream);
+  if (rows_per_thread(dtype, max_new, nq / nkv, d) == 1)
+    return db == 1 ? launch_tiles<float, 1, 1>(t, stream) : db == 2 ? launch_tiles<float, 2, 1>(t, stream) : launch_tiles<float, 4, 1>(t, stream);
+  return db == 1 ? launch_tiles<float, 1, 8>(t, stream) : db == 2 ? launch_tiles<float, 2, 8>(t, stream) : launch_tiles<float, 4, 4>(t, stream);
 }

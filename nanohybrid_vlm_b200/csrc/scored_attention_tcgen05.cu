@@ -743,7 +743,7 @@ size_t scored_long_plan(ScoredParts& p, int n_seqs, int n_tokens, int max_new, i
   const int G = nq / nkv, tokens = BM / G;
   p.tile_rows = tokens * G;
   p.tile_keys = BM;
-  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, (d <= 128 ? 2 : 1) * tokens * G, d <= 128 ? 128 : 64, SMS, 2 * SMS);
+  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, (d <= 128 ? 2 : 1) * tokens * G, d <= 128 ? 128 : 64, 2500.0, SMS, 2 * SMS);
 }
 
 int scored_long_launch(ScoredArgs a, const ScoredParts& parts, cudaStream_t stream) {
