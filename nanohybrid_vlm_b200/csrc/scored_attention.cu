@@ -544,35 +544,52 @@ static bool scored_wide(const void* q, int q_stride, const void* out, int out_st
   return q_stride % 8 == 0 && out_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)kv_pages % 16 == 0;
 }
 
-// Kilobytes of scratch that nhv_attention_scored wants for a call of these arguments.
-NHV_API int nhv_attention_scored_kilobytes(int dtype, const void* q, int q_stride, const void* out, int out_stride, const void* kv_pages, int n_seqs,
-                                           int n_tokens, int min_new, int max_new, int max_kv_len, int nq, int nkv, int d, int page_size, float scale) {
-  if (n_seqs <= 0 || nkv <= 0 || nq < nkv || d <= 0 || page_size <= 0 || max_kv_len <= 0) return 0;
-  return (int)(scored_plan(dtype, scored_wide(q, q_stride, out, out_stride, kv_pages), n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d, page_size, scale)
-                       .floats * sizeof(float) / 1024 + 1);
+// A call's arguments in one block: passing them one by one costs the host more than a launch.
+struct NhvScoredCall {
+  const void* q;
+  void* out;
+  const void* kv_pages;
+  const float* scores;
+  float* scores_out;
+  int* births;
+  const int* positions;
+  const int* block_table;
+  const int* cu_q;
+  const int* kv_len;
+  const float* sinks;
+  int dtype, q_stride, out_stride, bt_stride, n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d, page_size, n_pages;
+  float scale, softcap;
+};
+
+static ScoredPlan scored_plan(const NhvScoredCall& c) {
+  return scored_plan(c.dtype, scored_wide(c.q, c.q_stride, c.out, c.out_stride, c.kv_pages), c.n_seqs, c.n_tokens, c.min_new, c.max_new, c.max_kv_len,
+                     c.nq, c.nkv, c.d, c.page_size, c.scale);
 }
 
-NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* out, int out_stride, const void* kv_pages,
-                                 const float* scores, float* scores_out, int* births, const int* positions, const int* block_table,
-                                 int bt_stride, const int* cu_q, const int* kv_len, int n_seqs, int n_tokens, int min_new, int max_new,
-                                 int max_kv_len, int nq, int nkv, int d, int page_size, int n_pages, float scale, const float* sinks,
-                                 float softcap, float* work, int work_kilobytes, cudaStream_t stream) {
+// Kilobytes of scratch that nhv_attention_scored wants for these arguments.
+NHV_API int nhv_attention_scored_kilobytes(const NhvScoredCall* c) {
+  if (c->n_seqs <= 0 || c->nkv <= 0 || c->nq < c->nkv || c->d <= 0 || c->page_size <= 0 || c->max_kv_len <= 0) return 0;
+  return (int)(scored_plan(*c).floats * sizeof(float) / 1024 + 1);
+}
+
+NHV_API int nhv_attention_scored(const NhvScoredCall* c, float* work, int work_kilobytes, cudaStream_t stream) {
+  const int dtype = c->dtype, nq = c->nq, nkv = c->nkv, d = c->d, n_seqs = c->n_seqs, n_tokens = c->n_tokens, min_new = c->min_new, max_new = c->max_new,
+            max_kv_len = c->max_kv_len;
   NHV_REQUIRE(dtype == NHV_F32 || dtype == NHV_BF16, "scored attention: unknown type %d", dtype);
   NHV_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "scored attention: %d query heads do not divide into %d KV heads", nq, nkv);
   NHV_REQUIRE(d > 0 && d <= SA_MAX_D, "scored attention: head size %d is not in 1..%d", d, SA_MAX_D);
-  NHV_REQUIRE(page_size > 0 && n_pages > 0 && bt_stride >= 0 && nkv <= 65535, "scored attention: bad page geometry");
+  NHV_REQUIRE(c->page_size > 0 && c->n_pages > 0 && c->bt_stride >= 0 && nkv <= 65535, "scored attention: bad page geometry");
   NHV_REQUIRE(n_seqs >= 0 && n_tokens >= 0 && min_new >= 0 && max_new >= min_new && max_kv_len >= max_new,
               "scored attention: %d to %d new tokens with up to %d keys", min_new, max_new, max_kv_len);
-  NHV_REQUIRE(softcap >= 0.f, "scored attention: the cap on the scores is positive");
-  NHV_REQUIRE(!births == !positions || n_tokens == 0, "scored attention: births and positions go together");
+  NHV_REQUIRE(c->softcap >= 0.f, "scored attention: the cap on the scores is positive");
+  NHV_REQUIRE(!c->births == !c->positions || n_tokens == 0, "scored attention: births and positions go together");
   if (n_seqs == 0 || max_kv_len == 0) return 0;
   NHV_REQUIRE(n_seqs <= 65535, "scored attention: %d requests are beyond the grid's reach", n_seqs);
-  ScoredPlan plan = scored_plan(dtype, scored_wide(q, q_stride, out, out_stride, kv_pages), n_seqs, n_tokens, min_new, max_new, max_kv_len, nq, nkv, d,
-                                page_size, scale);
+  ScoredPlan plan = scored_plan(*c);
   NHV_REQUIRE((size_t)work_kilobytes * 1024 >= plan.floats * sizeof(float) && (uintptr_t)work % 16 == 0, "scored attention: %d kilobytes of scratch are too few",
               work_kilobytes);
-  ScoredArgs a{q, out, kv_pages, scores, scores_out, births, positions, block_table, cu_q, kv_len, sinks, work,
-               q_stride, out_stride, bt_stride, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages, max_kv_len, 0, 0x7fffffff, scale, softcap};
+  ScoredArgs a{c->q, c->out, c->kv_pages, c->scores, c->scores_out, c->births, c->positions, c->block_table, c->cu_q, c->kv_len, c->sinks, work,
+               c->q_stride, c->out_stride, c->bt_stride, n_seqs, n_tokens, nq, nkv, d, c->page_size, c->n_pages, max_kv_len, 0, 0x7fffffff, c->scale, c->softcap};
   float* scratch = work + ((size_t)n_tokens * nq + 3) / 4 * 4;
   if (plan.short_rows >= 0) {
     a.max_rows = plan.short_rows;
@@ -583,7 +600,7 @@ NHV_API int nhv_attention_scored(int dtype, const void* q, int q_stride, void* o
   }
   scored_place(plan.parts, scratch, n_tokens, nq, d);
   if (plan.many) return scored_long_launch(a, plan.parts, stream);
-  const TileArgs t{a, plan.parts, d % 4 == 0 && q_stride % 4 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)kv_pages % 16 == 0};
+  const TileArgs t{a, plan.parts, d % 4 == 0 && c->q_stride % 4 == 0 && (uintptr_t)c->q % 16 == 0 && (uintptr_t)c->kv_pages % 16 == 0};
   const int db = d <= 64 ? 1 : d <= 128 ? 2 : 4;
   if (dtype == NHV_BF16)
     return db == 1 ? launch_tiles<__nv_bfloat16, 1, 8>(t, stream) : db == 2 ? launch_tiles<__nv_bfloat16, 2, 8>(t, stream) : launch_tiles<__nv_bfloat16, 4, 4>(t, stream);

@@ -86,8 +86,8 @@ _SIGNATURES = {
     "nhv_map_difference": [I, P, I, P, I, P, F, F, I, I, I, P],
     "nhv_sandwich_stream": [I, P, P, P, P, P, P, I, I, F, F, F, F, I, P],
     "nhv_embed_rmsnorm": [I, P, P, P, P, I, I, I, F, F, P],
-    "nhv_attention_scored": [I, P, I, P, I, P, P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, I, I, I, F, P, F, P, I, P],
-    "nhv_attention_scored_kilobytes": [I, P, I, P, I, P, I, I, I, I, I, I, I, I, I, F],
+    "nhv_attention_scored": [ctypes.c_char_p, P, I, P],
+    "nhv_attention_scored_kilobytes": [ctypes.c_char_p],
     "nhv_select_keys": [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, P],
     "nhv_move_keys": [P, P, P, P, I, I, P, P, I, I, I, I, I, I, P],
     "nhv_decay_lowrank": [I, P, P, I, P, P, I, I, I, P],

@@ -10,6 +10,7 @@ that the 32-bit path never sees a reduced-precision matrix mode.
 from __future__ import annotations
 
 import os
+import struct
 import weakref
 
 import torch
@@ -1175,8 +1176,9 @@ def attention(out, q, kv_pages, tables, batch, nq: int, nkv: int, head_dim: int,
                        nq, nkv, head_dim, scale, window)
 
 
-def _page_geometry(kv_pages, nkv: int, scores, births, block_table, n_seqs: int, max_kv_len: int) -> tuple[int, int, int]:
-    """(number of pages, page size, head size), with what the kernels over scored pages assume checked."""
+def _check_scored_pages(kv_pages, nkv: int, scores, births, block_table, n_seqs: int, max_kv_len: int) -> None:
+    """What the kernels over scored pages assume, one ``KernelError`` each; called when the quick look of an entry point finds
+    something amiss."""
     _need_cuda(kv_pages, scores, births, block_table)
     if kv_pages is not None and (kv_pages.dim() != 5 or kv_pages.shape[1] != 2 or kv_pages.shape[2] != nkv or not kv_pages.is_contiguous()):
         raise KernelError(f"pages are [n_pages, 2, {nkv}, page_size, head_dim] and contiguous, not {tuple(kv_pages.shape)}")
@@ -1191,13 +1193,56 @@ def _page_geometry(kv_pages, nkv: int, scores, births, block_table, n_seqs: int,
         raise KernelError(f"the block table has a row of int32 pages for each of the {n_seqs} requests")
     if n_pages == 0 or page_size == 0 or max_kv_len > block_table.shape[1] * page_size:
         raise KernelError(f"{max_kv_len} keys do not fit a block table of {block_table.shape[1]} pages of {page_size}")
-    return n_pages, page_size, 0 if kv_pages is None else kv_pages.shape[4]
 
 
-def _int_array(name: str, t, n: int) -> None:
+def _check_int_array(name: str, t, n: int) -> None:
     _need_cuda(t)
     if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < n or t.stride(0) != 1:
         raise KernelError(f"{name} is an int32 array of {n} entries, not {tuple(t.shape)} {t.dtype}")
+
+
+def _int_array_ok(t, n: int) -> bool:
+    return t.is_cuda and t.dtype is torch.int32 and t.dim() == 1 and t.numel() >= n and t.is_contiguous()
+
+
+def _scored_pages_ok(scores, births, block_table, n_seqs: int, max_kv_len: int) -> bool:
+    shape, table = scores.shape, block_table.shape
+    return (scores.is_cuda and scores.dtype is torch.float32 and scores.is_contiguous() and len(shape) == 3 and shape[0] > 0
+            and (births is None or (births.is_cuda and births.dtype is torch.int32 and births.shape == shape and births.is_contiguous()))
+            and block_table.is_cuda and block_table.dtype is torch.int32 and len(table) == 2 and table[0] >= n_seqs
+            and block_table.stride(1) == 1 and 0 <= max_kv_len <= table[1] * shape[2])
+
+
+def _check_attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs, min_new, max_new, max_kv_len, nq, nkv, head_dim, births,
+                            positions, sinks, softcap, scores_out) -> None:
+    _check_scored_pages(kv_pages, nkv, scores, births, block_table, n_seqs, max_kv_len)
+    _need_cuda(out, q, sinks, scores_out)
+    if nq <= 0 or nkv <= 0 or nq % nkv:
+        raise KernelError(f"{nq} query heads do not divide into {nkv} KV heads")
+    if kv_pages.shape[4] != head_dim or not 0 < head_dim <= 256:
+        raise KernelError(f"attention with scores takes heads of 1 to 256 elements, the pages' own: not {head_dim} with pages of {kv_pages.shape[4]}")
+    if (q.dim() != 2 or q.shape != out.shape or q.shape[1] != nq * head_dim or q.stride(1) != 1 or out.stride(1) != 1
+            or not q.dtype == out.dtype == kv_pages.dtype):
+        raise KernelError(f"q and the output are [tokens, {nq * head_dim}] in the pages' type with neighbouring columns")
+    dtype_code(q)
+    T = q.shape[0]
+    _check_int_array("cu_q", cu_q, n_seqs + 1)
+    _check_int_array("kv_len", kv_len, n_seqs)
+    if (births is None) != (positions is None):
+        raise KernelError("births and positions go together")
+    if positions is not None:
+        _check_int_array("positions", positions, T)
+    if n_seqs < 0 or not 0 <= min_new <= max_new <= max_kv_len or not min_new * n_seqs <= T <= max_new * n_seqs:
+        raise KernelError(f"{T} new tokens of {n_seqs} requests are not {min_new} to {max_new} each, among {max_kv_len} keys")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != nq or not sinks.is_contiguous()):
+        raise KernelError(f"sinks are {nq} float32 numbers")
+    if softcap is not None and not softcap > 0:
+        raise KernelError("the cap on the scores is positive")
+    if scores_out.shape != scores.shape or scores_out.dtype != torch.float32 or not scores_out.is_contiguous():
+        raise KernelError(f"scores_out is float32 of the scores' shape {tuple(scores.shape)} and contiguous")
+
+
+_SCORED_CALL = struct.Struct("=11Q14i2f")
 
 
 def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs: int, min_new: int, max_new: int, max_kv_len: int,
@@ -1213,42 +1258,31 @@ def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs
     ``births`` [n_pages, nkv, page_size] int32: receives ``positions`` [T] int32 for the new keys.  ``sinks`` and ``softcap`` as in
     ``attention_tensor_core``.  ``min_new``, ``max_new``, ``max_kv_len``: the least and the most new tokens of a request, the most keys.
     Scores, weights and sums are float32 and added in a fixed order: the same call gives the same bits."""
-    n_pages, page_size, d = _page_geometry(kv_pages, nkv, scores, births, block_table, n_seqs, max_kv_len)
-    _need_cuda(out, q, sinks)
-    if nq <= 0 or nkv <= 0 or nq % nkv:
-        raise KernelError(f"{nq} query heads do not divide into {nkv} KV heads")
-    if d != head_dim or not 0 < head_dim <= 256:
-        raise KernelError(f"attention with scores takes heads of 1 to 256 elements, the pages' own: not {head_dim} with pages of {d}")
-    T = q.shape[0]
-    if (q.dim() != 2 or q.shape != out.shape or q.shape[1] != nq * head_dim or q.stride(1) != 1 or out.stride(1) != 1
-            or not q.dtype == out.dtype == kv_pages.dtype):
-        raise KernelError(f"q and the output are [tokens, {nq * head_dim}] in the pages' type with neighbouring columns")
-    _int_array("cu_q", cu_q, n_seqs + 1)
-    _int_array("kv_len", kv_len, n_seqs)
-    if (births is None) != (positions is None):
-        raise KernelError("births and positions go together")
-    if positions is not None:
-        _int_array("positions", positions, T)
-    if not 0 <= min_new <= max_new <= max_kv_len or not min_new * n_seqs <= T <= max_new * n_seqs:
-        raise KernelError(f"{T} new tokens of {n_seqs} requests are not {min_new} to {max_new} each, among {max_kv_len} keys")
-    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != nq or not sinks.is_contiguous()):
-        raise KernelError(f"sinks are {nq} float32 numbers")
-    if softcap is not None and not softcap > 0:
-        raise KernelError("the cap on the scores is positive")
     if scores_out is None:
         scores_out = scores
-    elif scores_out.shape != scores.shape or scores_out.dtype != torch.float32 or not scores_out.is_contiguous():
-        raise KernelError(f"scores_out is float32 of the scores' shape {tuple(scores.shape)} and contiguous")
-    _need_cuda(scores_out)
-    dt = dtype_code(q)
-    kilobytes = library.load_library().nhv_attention_scored_kilobytes(
-        dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv_pages.data_ptr(), n_seqs, T, min_new, max_new, max_kv_len, nq, nkv,
-        head_dim, page_size, float(scale))
+    pages, (T, columns), dtype = kv_pages.shape, q.shape if q.dim() == 2 else (-1, -1), q.dtype
+    if not (q.is_cuda and out.is_cuda and kv_pages.is_cuda and (dtype is torch.bfloat16 or dtype is torch.float32) and out.dtype is dtype
+            and kv_pages.dtype is dtype and nkv > 0 and nq > 0 and nq % nkv == 0 and 0 < head_dim <= 256 and columns == nq * head_dim
+            and q.stride(1) == 1 and out.shape == q.shape and out.stride(1) == 1 and kv_pages.is_contiguous()
+            and _scored_pages_ok(scores, births, block_table, n_seqs, max_kv_len)
+            and pages == (scores.shape[0], 2, nkv, scores.shape[2], head_dim) and scores.shape[1] == nkv
+            and n_seqs >= 0 and 0 <= min_new <= max_new <= max_kv_len and min_new * n_seqs <= T <= max_new * n_seqs
+            and _int_array_ok(cu_q, n_seqs + 1) and _int_array_ok(kv_len, n_seqs)
+            and (positions is None if births is None else positions is not None and _int_array_ok(positions, T))
+            and (scores_out is scores or scores_out.is_cuda and scores_out.dtype is torch.float32 and scores_out.shape == scores.shape
+                 and scores_out.is_contiguous())
+            and (softcap is None or softcap > 0)
+            and (sinks is None or sinks.is_cuda and sinks.dtype is torch.float32 and sinks.numel() == nq and sinks.is_contiguous())):
+        _check_attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs, min_new, max_new, max_kv_len, nq, nkv, head_dim,
+                                births, positions, sinks, softcap, scores_out)
+    given = _SCORED_CALL.pack(
+        q.data_ptr(), out.data_ptr(), kv_pages.data_ptr(), scores.data_ptr(), scores_out.data_ptr(), births.data_ptr() if births is not None else 0,
+        positions.data_ptr() if positions is not None else 0, block_table.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(),
+        sinks.data_ptr() if sinks is not None else 0, BF16 if dtype is torch.bfloat16 else F32, q.stride(0), out.stride(0), block_table.stride(0),
+        n_seqs, T, min_new, max_new, max_kv_len, nq, nkv, head_dim, pages[3], pages[0], scale, softcap or 0.0)
+    kilobytes = library.load_library().nhv_attention_scored_kilobytes(given)
     work = torch.empty(kilobytes * 256, dtype=torch.float32, device=q.device)
-    call("nhv_attention_scored", dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv_pages.data_ptr(),
-         scores.data_ptr(), scores_out.data_ptr(), _ptr(births), _ptr(positions), block_table.data_ptr(), block_table.stride(0),
-         cu_q.data_ptr(), kv_len.data_ptr(), n_seqs, T, min_new, max_new, max_kv_len, nq, nkv, head_dim, page_size, n_pages, float(scale),
-         _ptr(sinks), float(softcap or 0.0), work.data_ptr(), kilobytes, stream_ptr())
+    call("nhv_attention_scored", given, work.data_ptr(), kilobytes, stream_ptr())
 
 
 def select_keys(sources, targets, scores, births, block_table, kv_len, seen, budgets, n_seqs: int, max_kv_len: int, keep_first: int,
@@ -1260,42 +1294,55 @@ def select_keys(sources, targets, scores, births, block_table, kv_len, seen, bud
     ``budgets[i]`` largest of the first kv_len[i] slots stay, of equal ones those in the lowest slots.  ``sources``, ``targets`` [n_seqs,
     nkv, M] int32: the i-th kept slot at or above the budget and the i-th dropped slot below it, -1 behind the last.  M has to reach
     the largest kv_len[i] - budgets[i], or the largest budget if that is less (else the next check of the kernels raises)."""
-    nkv = scores.shape[1] if scores.dim() == 3 else 0
-    n_pages, page_size, _ = _page_geometry(None, nkv, scores, births, block_table, n_seqs, max_kv_len)
-    if births is None:
-        raise KernelError("the choice of keys needs their births")
-    for name, t in (("kv_len", kv_len), ("seen", seen), ("budgets", budgets)):
-        _int_array(name, t, n_seqs)
-    moves = _moves(sources, targets, n_seqs, nkv)
-    if keep_first < 0 or keep_recent < 0 or max_kv_len < 0:
-        raise KernelError("kept first and recent keys, and keys, are counted from 0")
+    n_pages, nkv, page_size = scores.shape if scores.dim() == 3 else (0, 0, 0)
+    moves = sources.shape[2] if sources.dim() == 3 else -1
+    if not (births is not None and _scored_pages_ok(scores, births, block_table, n_seqs, max_kv_len) and n_seqs >= 0
+            and _int_array_ok(kv_len, n_seqs) and _int_array_ok(seen, n_seqs) and _int_array_ok(budgets, n_seqs)
+            and _moves_ok(sources, targets, n_seqs, nkv) and keep_first >= 0 and keep_recent >= 0):
+        _check_scored_pages(None, nkv, scores, births, block_table, n_seqs, max_kv_len)
+        if births is None:
+            raise KernelError("the choice of keys needs their births")
+        for name, t in (("kv_len", kv_len), ("seen", seen), ("budgets", budgets)):
+            _check_int_array(name, t, n_seqs)
+        _check_moves(sources, targets, n_seqs, nkv)
+        raise KernelError(f"requests, keys, kept first and recent keys are counted from 0: {n_seqs}, {max_kv_len}, {keep_first}, {keep_recent}")
     call("nhv_select_keys", sources.data_ptr(), targets.data_ptr(), scores.data_ptr(), births.data_ptr(), block_table.data_ptr(),
          block_table.stride(0), kv_len.data_ptr(), seen.data_ptr(), budgets.data_ptr(), n_seqs, max_kv_len, nkv, page_size, n_pages, moves,
          keep_first, keep_recent, stream_ptr())
 
 
-def _moves(sources, targets, n_seqs: int, nkv: int) -> int:
+def _moves_ok(sources, targets, n_seqs: int, nkv: int) -> bool:
+    shape = sources.shape
+    return (sources.is_cuda and targets.is_cuda and sources.dtype is torch.int32 and targets.dtype is torch.int32 and len(shape) == 3
+            and shape[0] == n_seqs and shape[1] == nkv and targets.shape == shape and sources.is_contiguous() and targets.is_contiguous())
+
+
+def _check_moves(sources, targets, n_seqs: int, nkv: int) -> None:
     _need_cuda(sources, targets)
     for t in (sources, targets):
         if t.dim() != 3 or t.shape[:2] != (n_seqs, nkv) or t.dtype != torch.int32 or not t.is_contiguous():
             raise KernelError(f"sources and targets are [{n_seqs}, {nkv}, moves] int32 and contiguous, not {tuple(t.shape)} {t.dtype}")
     if sources.shape != targets.shape:
         raise KernelError("there are as many sources as targets")
-    return sources.shape[2]
 
 
 def move_keys(kv_pages, scores, births, block_table, sources, targets, n_seqs: int) -> None:
     """Carry out the moves of ``select_keys`` in place: key, value, score and birth of every source slot go to its target slot.
     Afterwards the request's keys fill its first min(kv_len, budget) slots.  Sources keep what they held."""
-    nkv = scores.shape[1] if scores.dim() == 3 else 0
-    n_pages, page_size, d = _page_geometry(kv_pages, nkv, scores, births, block_table, n_seqs, 0)
-    if births is None:
-        raise KernelError("the moves of keys take their births along")
-    dtype_code(kv_pages)
-    moves = _moves(sources, targets, n_seqs, nkv)
+    n_pages, nkv, page_size = scores.shape if scores.dim() == 3 else (0, 0, 0)
+    pages, dtype = kv_pages.shape, kv_pages.dtype
+    if not (births is not None and _scored_pages_ok(scores, births, block_table, n_seqs, 0) and _moves_ok(sources, targets, n_seqs, nkv)
+            and kv_pages.is_cuda and (dtype is torch.bfloat16 or dtype is torch.float32) and len(pages) == 5
+            and pages[:4] == (n_pages, 2, nkv, page_size) and kv_pages.is_contiguous()):
+        _check_scored_pages(kv_pages, nkv, scores, births, block_table, n_seqs, 0)
+        if births is None:
+            raise KernelError("the moves of keys take their births along")
+        dtype_code(kv_pages)
+        _check_moves(sources, targets, n_seqs, nkv)
+        raise KernelError(f"pages {tuple(pages)} do not go with scores {tuple(scores.shape)}")
     call("nhv_move_keys", kv_pages.data_ptr(), scores.data_ptr(), births.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-         block_table.shape[1], sources.data_ptr(), targets.data_ptr(), n_seqs, nkv, page_size, n_pages, moves, d * kv_pages.element_size(),
-         stream_ptr())
+         block_table.shape[1], sources.data_ptr(), targets.data_ptr(), n_seqs, nkv, page_size, n_pages, sources.shape[2],
+         pages[4] * (2 if dtype is torch.bfloat16 else 4), stream_ptr())
 
 
 FUSE_DECODE_QK = True             # tests switch it off to compare with the two-kernel form
