@@ -103,6 +103,14 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t (&r)[32], uint32_t tad
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], uint32_t taddr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -113,6 +121,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
         "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
@@ -143,6 +159,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+__device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
 // A pair of bfloat16 with what is not finite taken out; `bad` says whether there was any.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t v, bool& bad) {
@@ -158,6 +179,89 @@ __device__ __forceinline__ void cap32(uint32_t (&sr)[32], const NhvScoreCap& c) 
   nhv_cap_tile(s, c);
 #pragma unroll
   for (int i = 0; i < 32; ++i) sr[i] = __float_as_uint(s[i >> 2][i & 3]);
+}
+
+// What few tiles need, out of the way of what all need: scores capped and masked where they lie in tensor memory (32 columns at a
+// time); a key at or above `end` of the row's own, or without a page, gets -inf.
+template <int BN>
+__device__ __noinline__ void change_scores(uint32_t s_addr, const NhvScoreCap& cap, bool masked, bool missing, int key0, int row_hi, int total, const int* table,
+                                           int page_size, int n_pages) {
+#pragma unroll 1
+  for (int c = 0; c < BN; c += 32) {
+    uint32_t sr[32];
+    tmem_ld32_nowait(sr, s_addr + c);
+    tmem_ld_wait();
+    if (cap.in != 0.f) cap32(sr, cap);
+    if (masked) {
+      uint32_t gone = 0;
+      if (missing)
+        for (int i = 0; i < 32; ++i) {
+          const int page = table[min(key0 + c + i, total - 1) / page_size];
+          if (page < 0 || page >= n_pages) gone |= 1u << i;
+        }
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (key0 + c + i > row_hi || (gone >> i & 1u)) sr[i] = 0xFF800000u;
+    }
+    tmem_st32(s_addr + c, sr);
+  }
+  tmem_st_wait();
+}
+// A thread group's pass over a tile of values in shared memory: rows that are no key of the request become zeros, and, with
+// `finite`, so does what is not finite, each such key noted in bad[4].
+template <int DB, int BN>
+__device__ __noinline__ void clean_values(unsigned char* v, uint32_t* bad_keys, bool finite, bool missing, int key0, int total, const int* table,
+                                          int page_size, int n_pages) {
+  for (int id = threadIdx.x & 127; id < BN * DB * 8; id += 128) {
+    const int row = id / (DB * 8), rem = id - row * (DB * 8), at_key = min(key0 + row, total - 1);
+    uint4* at = reinterpret_cast<uint4*>(v + (rem >> 3) * (BN * 128) + row * 128 + ((rem & 7) << 4));
+    const int page = missing ? table[at_key / page_size] : 0;
+    if (key0 + row >= total || page < 0 || page >= n_pages) {
+      *at = make_uint4(0, 0, 0, 0);
+    } else if (finite) {
+      uint4 x = *at;
+      bool bad = false;
+      x.x = finite_pair(x.x, bad); x.y = finite_pair(x.y, bad); x.z = finite_pair(x.z, bad); x.w = finite_pair(x.w, bad);
+      if (bad) {
+        atomicOr(&bad_keys[row >> 5], 1u << (row & 31));
+        *at = x;
+      }
+    }
+  }
+  fence_async_smem();
+}
+// Values taken out above, back to a row that sees them: p v, of what is not finite in v, added to O in tensor memory.  `notes`: the 8 x 4
+// words of keys, from key `key0` on in tiles of BN.
+template <int DB, int BN>
+__device__ __noinline__ void return_values(uint32_t o_addr, const ScoredArgs& a, const uint32_t* notes, int seq, int kvh, int head, int token, int key0,
+                                           int row_hi, float m, float scale_log2) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < DB * 64; c0 += 32) {
+    uint32_t o[32];
+    tmem_ld32_nowait(o, o_addr + c0);
+    tmem_ld_wait();
+    for (int w = 0; w < 32; ++w)
+      for (uint32_t bits = notes[w]; bits; bits &= bits - 1) {
+        const int key = key0 + (w >> 2) * BN + (w & 3) * 32 + __ffs(bits) - 1;
+        if (key > row_hi) continue;
+        const long long k_at = key_row(a, seq, key, kvh, 0), v_at = key_row(a, seq, key, kvh, 1);
+        if (k_at < 0) continue;
+        const bf16* qr = (const bf16*)a.q + (size_t)token * a.q_stride + (size_t)head * a.d;
+        float s = 0.f;
+        for (int e = 0; e < a.d; ++e) s = fmaf(to_f32(qr[e]), to_f32(((const bf16*)a.pages)[k_at + e]), s);
+        if (a.softcap > 0.f) s = a.softcap * tanhf(s * a.scale / a.softcap) * SA_LOG2E;
+        else s *= scale_log2;
+        const float weight = scored_exp2(s + (m == -INFINITY ? 0.f : -m));
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float x = c0 + i < a.d ? to_f32(((const bf16*)a.pages)[v_at + c0 + i]) : 0.f;
+          if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(fmaf(weight, x, __uint_as_float(o[i])));
+        }
+      }
+    __syncwarp();
+    tmem_st32(o_addr + c0, o);
+  }
+  tmem_st_wait();
 }
 
 // Loads `BN` keys or values of a request, from key0 on, into one stage: boxes of p.box rows, which lie in one page each.  Boxes at
@@ -182,7 +286,7 @@ __device__ __forceinline__ void load_rows(unsigned char* stage, const LongArgs& 
   for (int b = 0; b < DB; ++b) tma_load_3d(stage + b * (BM * 128), &p.q_map, b * 64, kvh * G, token, bar);
 }
 
-template <int DB>
+template <int DB, bool CAP>
 __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kernel(const __grid_constant__ LongArgs p) {
   using C = Rows<DB>;
   constexpr int NQ = C::NQ, BN = C::BN, STAGES = C::STAGES;
@@ -191,12 +295,12 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
   uint64_t* full = bars;                   // [STAGES]
   uint64_t* empty = bars + 8;              // [STAGES]
   uint64_t* s_full = bars + 16;            // [NQ]
-  uint64_t* p_ready = bars + 18;           // [NQ]
-  uint64_t* o_full = bars + 20;            // [NQ]
-  uint64_t* q_full = bars + 22;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
-  int* s_abort = reinterpret_cast<int*>(bars + 25);
-  int* s_missing = reinterpret_cast<int*>(bars + 26);
+  uint64_t* p_ready = bars + 18;           // [NQ][2]: the halves of a tile's P
+  uint64_t* o_full = bars + 22;            // [NQ]
+  uint64_t* q_full = bars + 24;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
+  int* s_abort = reinterpret_cast<int*>(bars + 26);
+  int* s_missing = reinterpret_cast<int*>(bars + 27);
   uint32_t* s_bad = reinterpret_cast<uint32_t*>(bars + 32);       // [8 tiles][4]: keys whose values are not all finite
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* tiles = smem_raw + (((raw + 1024 + 1023u) & ~1023u) - raw);
@@ -212,7 +316,8 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
     }
     for (int q = 0; q < NQ; ++q) {
       mbar_init(&s_full[q], 1);
-      mbar_init(&p_ready[q], 128);
+      mbar_init(&p_ready[2 * q], 128);
+      mbar_init(&p_ready[2 * q + 1], 128);
       mbar_init(&o_full[q], 1);
     }
     mbar_init(q_full, 1);
@@ -255,6 +360,9 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
   const uint32_t tmem_base = *tmem_slot;
   const int n_tiles = max(nt[0], nt[1]);
 
+  // Registers go where the rows are: 384 threads start with 168 each, 64,512 in all; 128 x 80 + 256 x 208 = 63,488.
+  if (warp < 4) {
+  if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && n_tiles > 0) {
@@ -299,13 +407,15 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
                  kd + (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
         tc_commit(&s_full[q]);
       };
-      auto second_product = [&](int q, int j) {
+      auto second_product = [&](int q, int j, int half) {
         const uint64_t vd = v_desc + (uint64_t)(((2 * j + 1) % STAGES) * (C::STAGE >> 4));
         const uint32_t pa = tmem_base + C::S_COL + q * BN;           // P lies over the first half of S
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)                          // 8 columns of P and 16 rows of V per 16 keys
+        for (int i = 0; i < BN / 32; ++i) {                           // 8 columns of P and 16 rows of V per 16 keys
+          const int kk = half * (BN / 32) + i;
           tc_mma_a_tmem(tmem_base + C::O_COL + q * (DB * 64), pa + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), idesc_o,
                         (j > 0 || kk > 0) ? 1u : 0u);
+        }
       };
       if (ok) ok = stage_ready(0);
       if (ok) {
@@ -318,12 +428,16 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
         bool have_v = false, have_k = false;
         for (int q = 0; q < NQ && ok; ++q) {
           if (j >= nt[q]) continue;
-          ok = mbar_wait(&p_ready[q], (uint32_t)j & 1, 5);
+          ok = mbar_wait(&p_ready[2 * q], (uint32_t)j & 1, 5);
           if (ok && !have_v) ok = stage_ready(2 * j + 1);
           have_v = true;
           if (!ok) break;
           tc_fence_after();
-          second_product(q, j);
+          second_product(q, j, 0);
+          ok = mbar_wait(&p_ready[2 * q + 1], (uint32_t)j & 1, 5);
+          if (!ok) break;
+          tc_fence_after();
+          second_product(q, j, 1);
           if (j + 1 < nt[q]) {
             if (!have_k) ok = stage_ready(2 * j + 2);
             have_k = true;
@@ -341,7 +455,10 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
       if (!ok) *s_abort = 1;
     }
     __syncwarp();
-  } else if (warp >= 4 && seq >= 0) {
+  }
+  } else {
+  if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
+  if (seq >= 0) {
     // ------------------------------------------------------------------ softmax and output: a thread per row
     const int q = (warp - 4) >> 2, quarter = warp & 3, R = quarter * 32 + lane;
     const int tq = R / G, g = R - tq * G, token = t0 + q * p.tokens + tq;
@@ -356,119 +473,86 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
     float m = -INFINITY, l = 0.f;
     // the first tile of which some row of the block does not see all; the notes on values begin there
     const int first_edge = max(0, total - n + t0 + 1 - key_begin) / BN;
-    bool ok = true, any_bad = false;
+    bool ok = true;
+    const f32x2 scale2 = f2_pack(p.scale_log2, p.scale_log2);
     for (int j = 0; j < tiles_q; ++j) {
       const int key0 = key_begin + j * BN;
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[q], (uint32_t)j & 1, 6));
-      if (!ok) break;
-      tc_fence_after();
-      // the maximum first; scores that a cap or a mask changes go back to where they were
-      const bool edge = key0 + BN - 1 > all_hi;                        // some row does not see some key of the tile
-      const bool masked = edge || missing;
-      float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < BN / 32; ++c) {
-        uint32_t sr[32];
-        tmem_ld32_nowait(sr, s_addr + c * 32);
-        tmem_ld_wait();
-        if (p.cap.in != 0.f) cap32(sr, p.cap);
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (key0 + c * 32 + i > row_hi) sr[i] = 0xFF800000u;       // -inf
-          if (missing) {
-            for (int i = 0; i < 32; ++i) {
-              const int at = min(key0 + c * 32 + i, total - 1), page = table[at / a.page_size];
-              const bool gone = page < 0 || page >= a.n_pages;
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (k == i && gone) sr[k] = 0xFF800000u;
-            }
-          }
-        }
-        if (masked || p.cap.in != 0.f) tmem_st32(s_addr + c * 32, sr);
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          mx0 = max3(mx0, __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
-          mx1 = max3(mx1, __uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3]));
-        }
-      }
-      if (masked || p.cap.in != 0.f) tmem_st_wait();
-      float mx = fmaxf(mx0, mx1);
-      mx *= p.scale_log2;
-      const bool grow = mx > m + RESCALE_STEP;                         // also the first keys a row sees
-      float alpha = 1.f;
-      if (grow) {
-        alpha = scored_exp2(m - mx);                                   // 0 when the row had seen nothing
-        m = mx;
-        l *= alpha;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll 1
-        for (int c0 = 0; c0 < DB * 64; c0 += 32) {
-          uint32_t o[32];
-          tmem_ld32_nowait(o, o_addr + c0);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st32(o_addr + c0, o);
-        }
-      }
-      const float neg_ref = m == -INFINITY ? 0.f : -m;
-      float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
-#pragma unroll
-      for (int c = 0; c < BN / 64; ++c) {
-        uint32_t sr[2][32], pk[32];
-        tmem_ld32_nowait(sr[0], s_addr + c * 64);
-        tmem_ld32_nowait(sr[1], s_addr + c * 64 + 32);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          const float p0 = scored_exp2(fmaf(__uint_as_float(sr[i >> 5][i & 31]), p.scale_log2, neg_ref));
-          const float p1 = scored_exp2(fmaf(__uint_as_float(sr[i >> 5][(i & 31) + 1]), p.scale_log2, neg_ref));
-          const float p2 = scored_exp2(fmaf(__uint_as_float(sr[i >> 5][(i & 31) + 2]), p.scale_log2, neg_ref));
-          const float p3 = scored_exp2(fmaf(__uint_as_float(sr[i >> 5][(i & 31) + 3]), p.scale_log2, neg_ref));
-          pk[i >> 1] = pack_bf16(p0, p1);
-          pk[(i >> 1) + 1] = pack_bf16(p2, p3);
-          l0 += p0; l1 += p1; l2 += p2; l3 += p3;                      // the row's sum in fp32, before the rounding to bfloat16
-        }
-        tmem_st32(s_addr + c * 32, pk);
-      }
-      l += (l0 + l1) + (l2 + l3);
-      tmem_st_wait();
-      if ((masked || key0 + BN - 1 > total - n + t0) && (q == 0 || j >= nt[0])) {
-        // Values that some row of the block does not see: not finite ones, and rows that are no key of the request, are taken out.
-        // The first tile's group does it for both: its product comes first.
+      // Values that some row of the block does not see: the first tile's group looks them through for both, whose product comes first.
+      if ((missing || key0 + BN - 1 > total - n + t0) && (q == 0 || j >= nt[0])) {
         const int st = (2 * j + 1) % STAGES;
         ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)((2 * j + 1) / STAGES) & 1, 7));
         if (!ok) break;
-        unsigned char* v = kv_s + st * C::STAGE;
-        for (int id = threadIdx.x & 127; id < BN * DB * 8; id += 128) {
-          const int row = id / (DB * 8), rem = id - row * (DB * 8), at_key = min(key0 + row, total - 1);
-          uint4* at = reinterpret_cast<uint4*>(v + (rem >> 3) * (BN * 128) + row * 128 + ((rem & 7) << 4));
-          const int page = missing ? table[at_key / a.page_size] : 0;
-          if (key0 + row >= total || page < 0 || page >= a.n_pages) {
-            *at = make_uint4(0, 0, 0, 0);
-          } else if (j >= first_edge) {
-            uint4 x = *at;
-            bool bad = false;
-            x.x = finite_pair(x.x, bad); x.y = finite_pair(x.y, bad); x.z = finite_pair(x.z, bad); x.w = finite_pair(x.w, bad);
-            if (bad) {
-              atomicOr(&s_bad[((j - first_edge) & 7) * 4 + (row >> 5)], 1u << (row & 31));
-              *at = x;
-            }
+        clean_values<DB, BN>(kv_s + st * C::STAGE, &s_bad[((j - first_edge) & 7) * 4], j >= first_edge, missing, key0, total, table, a.page_size, a.n_pages);
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[q], (uint32_t)j & 1, 6));
+      if (!ok) break;
+      tc_fence_after();
+      const bool masked = key0 + BN - 1 > all_hi || missing;           // some row does not see some key of the tile
+      if (CAP || masked) change_scores<BN>(s_addr, p.cap, masked, missing, key0, row_hi, total, table, a.page_size, a.n_pages);
+      uint32_t sr[BN / 32][32];
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) tmem_ld32_nowait(sr[c], s_addr + c * 32);
+      tmem_ld_wait();
+      float mx0 = max3(__uint_as_float(sr[0][0]), __uint_as_float(sr[0][1]), __uint_as_float(sr[0][2]));
+      float mx1 = max3(__uint_as_float(sr[0][3]), __uint_as_float(sr[0][4]), __uint_as_float(sr[0][5]));
+#pragma unroll
+      for (int i = 6; i + 3 < BN; i += 4) {
+        mx0 = max3(mx0, __uint_as_float(sr[i >> 5][i & 31]), __uint_as_float(sr[(i + 1) >> 5][(i + 1) & 31]));
+        mx1 = max3(mx1, __uint_as_float(sr[(i + 2) >> 5][(i + 2) & 31]), __uint_as_float(sr[(i + 3) >> 5][(i + 3) & 31]));
+      }
+      const float mx = max3(mx0, mx1, fmaxf(__uint_as_float(sr[BN / 32 - 1][30]), __uint_as_float(sr[BN / 32 - 1][31]))) * p.scale_log2;
+      const bool grow = mx > m + RESCALE_STEP;                         // also the first keys a row sees
+      if (__any_sync(0xffffffffu, grow)) {
+        float alpha = 1.f;
+        if (grow) {
+          alpha = scored_exp2(m - mx);                                 // 0 when the row had seen nothing
+          m = mx;
+          l *= alpha;
+        }
+        if (j > 0) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < DB * 64; c0 += 16) {
+            uint32_t o[16];
+            tmem_ld16(o, o_addr + c0);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st16(o_addr + c0, o);
           }
         }
-        fence_async_smem();
       }
-      tc_fence_before();
-      mbar_arrive(&p_ready[q]);
+      const float neg_ref = m == -INFINITY ? 0.f : -m;
+      const f32x2 ref2 = f2_pack(neg_ref, neg_ref);
+      f32x2 l2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t pk[BN / 4];
+#pragma unroll
+        for (int i = 0; i < BN / 2; i += 2) {
+          const int at = half * (BN / 2) + i;
+          float x, y;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[at >> 5][at & 31]), __uint_as_float(sr[at >> 5][(at & 31) + 1])), scale2, ref2), x, y);
+          x = scored_exp2(x);
+          y = scored_exp2(y);
+          pk[i >> 1] = pack_bf16(x, y);
+          l2[(i >> 1) & 3] = f2_add(l2[(i >> 1) & 3], f2_pack(x, y));   // the row's sum in fp32, before the rounding to bfloat16
+        }
+#pragma unroll
+        for (int c = 0; c < BN / 4; c += 16) tmem_st16(s_addr + half * (BN / 4) + c, pk + c);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_ready[2 * q + half]);
+      }
+      l += f2_sum(f2_add(l2[0], l2[1]), f2_add(l2[2], l2[3]));
     }
     if (ok && tiles_q > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], 0, 8));
     if (ok) {
       tc_fence_after();
       // the notes on values: made before the products that o_full covers
+      bool any_bad = false;
       for (int i = 0; i < 32; ++i) any_bad |= *(volatile uint32_t*)&s_bad[i] != 0;
+      if (any_bad && tiles_q > 0)
+        return_values<DB, BN>(o_addr, a, s_bad, seq, kvh, kvh * G + g, first + token, key_begin + first_edge * BN, row_hi, m, p.scale_log2);
       const size_t row = (size_t)kvh * a.n_tokens * G + (size_t)(first + token) * G + g;
       const bool whole = p.parts.splits == 1;
       float inv = 1.f;
@@ -497,28 +581,6 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (valid && any_bad) {
-          // values taken out above, back to the rows that see them: p v, of what is not finite in v
-          for (int w = 0; w < 32; ++w) {
-            for (uint32_t bits = s_bad[w]; bits; bits &= bits - 1) {
-              const int key = key_begin + (first_edge + (w >> 2)) * BN + (w & 3) * 32 + __ffs(bits) - 1;
-              if (key > row_hi) continue;
-              const long long k_at = key_row(a, seq, key, kvh, 0), v_at = key_row(a, seq, key, kvh, 1);
-              if (k_at < 0) continue;
-              const bf16* qr = (const bf16*)a.q + (size_t)(first + token) * a.q_stride + (size_t)(kvh * G + g) * a.d;
-              float s = 0.f;
-              for (int e = 0; e < a.d; ++e) s = fmaf(to_f32(qr[e]), to_f32(((const bf16*)a.pages)[k_at + e]), s);
-              if (a.softcap > 0.f) s = a.softcap * tanhf(s * a.scale / a.softcap) * SA_LOG2E;
-              else s *= p.scale_log2;
-              const float weight = scored_exp2(s + (m == -INFINITY ? 0.f : -m));
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float x = c0 + i < a.d ? to_f32(((const bf16*)a.pages)[v_at + c0 + i]) : 0.f;
-                if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(fmaf(weight, x, __uint_as_float(o[i])));
-              }
-            }
-          }
-        }
         if (valid && whole) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -540,6 +602,7 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
     } else {
       *s_abort = 1;
     }
+  }
   }
   tc_fence_before();
   __syncthreads();
@@ -715,13 +778,13 @@ bool make_q_map(CUtensorMap* map, const ScoredArgs& a, int tokens) {
 
 int divisor(int a, int b) { return b == 0 ? a : divisor(b, a % b); }
 
-template <int DB>
+template <int DB, bool CAP>
 int launch_long(const LongArgs& p, int row_tiles, cudaStream_t stream) {
   static std::atomic<uint64_t> rows_done{0}, keys_done{0};
   const ScoredArgs& a = p.a;
-  NHV_CUDA(nhv_allow_smem((const void*)scored_rows_tcgen05_kernel<DB>, Rows<DB>::SMEM, rows_done), "scored attention (tcgen05)");
+  NHV_CUDA(nhv_allow_smem((const void*)scored_rows_tcgen05_kernel<DB, CAP>, Rows<DB>::SMEM, rows_done), "scored attention (tcgen05)");
   NHV_CUDA(nhv_allow_smem((const void*)scored_keys_tcgen05_kernel<DB>, Keys<DB>::SMEM, keys_done), "scored attention (tcgen05)");
-  NHV_CUDA(nhv_launch(scored_rows_tcgen05_kernel<DB>, dim3(a.nkv, row_tiles, p.parts.splits), Rows<DB>::THREADS, Rows<DB>::SMEM, stream, p),
+  NHV_CUDA(nhv_launch(scored_rows_tcgen05_kernel<DB, CAP>, dim3(a.nkv, row_tiles, p.parts.splits), Rows<DB>::THREADS, Rows<DB>::SMEM, stream, p),
            "scored attention (tcgen05)");
   int rc = scored_join_rows(NHV_BF16, a, p.parts, stream);
   if (rc) return rc;
@@ -763,10 +826,11 @@ int scored_long_launch(ScoredArgs a, const ScoredParts& parts, cudaStream_t stre
   const long long row_tiles = (long long)a.n_tokens / (nq_tiles * p.tokens) + a.n_seqs;
   NHV_REQUIRE(row_tiles <= 65535 && (long long)p.key_tiles * parts.chunks <= 65535, "scored attention (tcgen05): %lld tiles of rows, %d of keys in %d chunks are beyond the grid's reach",
               row_tiles, p.key_tiles, parts.chunks);
+  const bool cap = a.softcap > 0.f;
   switch (db) {
-    case 1: return launch_long<1>(p, (int)row_tiles, stream);
-    case 2: return launch_long<2>(p, (int)row_tiles, stream);
-    case 3: return launch_long<3>(p, (int)row_tiles, stream);
-    default: return launch_long<4>(p, (int)row_tiles, stream);
+    case 1: return cap ? launch_long<1, true>(p, (int)row_tiles, stream) : launch_long<1, false>(p, (int)row_tiles, stream);
+    case 2: return cap ? launch_long<2, true>(p, (int)row_tiles, stream) : launch_long<2, false>(p, (int)row_tiles, stream);
+    case 3: return cap ? launch_long<3, true>(p, (int)row_tiles, stream) : launch_long<3, false>(p, (int)row_tiles, stream);
+    default: return cap ? launch_long<4, true>(p, (int)row_tiles, stream) : launch_long<4, false>(p, (int)row_tiles, stream);
   }
 }
