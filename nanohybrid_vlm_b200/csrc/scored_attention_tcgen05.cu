@@ -2,12 +2,13 @@
 // the 5th-generation tensor cores: tcgen05.mma with the accumulators in tensor memory, operands brought by TMA.
 //
 // The rows' pass: O = softmax(Q K^T) V, and each row's log-sum.  A block owns two tiles of up to 128 rows (whole tokens; heads above
-// 128: one tile) of a KV head and walks the keys in tiles of 128 (heads above 128: 64).  Warp 0, one lane: TMA, keys and
-// values through one ring of stages, straight from the pages, in boxes of as many rows as divide the page size and 128.
-// Warp 1, one lane: the MMAs, S = Q K^T and O += P V.  Warps 4-7 and 8-11: one thread per row of the first and the second tile;
-// it reads its row of S, takes maximum and exponentials, writes P (bfloat16) over S.  While one tile is in its softmax the other's
-// products run.  The products of a tile run in order, so a finished S says that the P V before it is finished too: P may be
-// written and O rescaled without another wait.  O is rescaled only when a row's maximum grew by more than 2^8.
+// 128: one tile) of a KV head and walks the keys in tiles of 64.  Warp 0, one lane: TMA, keys and values through one ring of
+// stages, straight from the pages, in boxes of as many rows as divide the page size and 64.  Warp 1, one lane: the MMAs,
+// S = Q K^T into one of two buffers a tile of rows, and O += P V.  Warps 4-7 and 8-11: one thread per row of the first and the second
+// tile; it reads its row of S, takes maximum and exponentials, writes P (bfloat16) over S.  The next S is made while this one is in
+// the softmax.  O is rescaled only when a row's maximum grew by more than 2^8; then, and only then, the product before is waited for.
+//   Tried: tiles of 128 keys with one buffer of S (the softmax then waits for P V and the next Q K^T, 1,024 cycles of a step of 4,430:
+//   385 us for 1,024 tokens behind 16,384 keys); the same with two threads a row (458 us: the threads of a row meet for the maximum).
 //   Where the grid would leave SMs idle the keys are split over blocks, whose sums a small kernel joins.
 // The keys' pass: w[j] = sum over the rows that see j of exp2(s - log-sum).  S^T = K Q^T with the keys as M: a lane of tensor
 // memory is a key and its columns are rows, so a thread adds up its key's weights with no exchange at all.  The block's keys stay
@@ -34,17 +35,17 @@ constexpr int SMS = 148;
 
 template <int DB> struct Rows {                  // DB: blocks of 64 elements (128 bytes) of a head
   static constexpr int NQ = DB <= 2 ? 2 : 1;     // tiles of rows a block
-  static constexpr int BN = DB <= 2 ? 128 : 64;  // keys of a tile
+  static constexpr int BN = 64;                  // keys of a tile
   static constexpr int THREADS = 128 + NQ * 128;
   static constexpr int Q_BYTES = DB * BM * 128, STAGE = DB * BN * 128;
-  static constexpr int STAGES = DB == 1 ? 8 : 5;
-  static constexpr int SMEM = 1024 + 1024 + NQ * Q_BYTES + STAGES * STAGE;       // barriers and flags, alignment, tiles
-  static constexpr uint32_t S_COL = 0, O_COL = NQ * BN;
+  static constexpr int STAGES = DB == 1 ? 12 : DB == 2 ? 10 : 5;
+  static constexpr int SMEM = 1024 + 1024 + NQ * Q_BYTES + STAGES * STAGE;       // barriers and notes, alignment, tiles
+  static constexpr uint32_t S_COL = 0, O_COL = NQ * 2 * BN;      // two buffers of S a tile of rows
   static constexpr uint32_t TMEM_COLS = 512;
 };
 template <int DB> struct Keys {
   static constexpr int BN = 128;                 // rows of a tile = columns of S^T
-  static constexpr int THREADS = 192;
+  static constexpr int THREADS = 64 + 256;
   static constexpr int K_BYTES = DB * BM * 128, STAGE = DB * BN * 128;
   static constexpr int STAGES = DB == 1 ? 4 : DB == 2 ? 2 : 1;     // two blocks an SM (tensor memory has room for two), above 128 one
   static constexpr int SMEM = 1024 + 1024 + 1024 + K_BYTES + STAGES * STAGE;
@@ -75,6 +76,15 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+// One lane of a converged warp.  MMAs are issued under this and not under `lane == 0`, with what they are made from the same in every
+// lane by a shuffle: their operands live in the warp's uniform registers, and where the compiler cannot see that a value is the
+// same in all lanes, each MMA took about 137 cycles to issue, whatever its size (506 -> 335 us for the rows of 1,024 tokens behind
+// 16,384 keys).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
 }
 __device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -164,7 +174,8 @@ __device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
+// 256 threads meet.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 256;\n" ::"r"(id) : "memory"); }
 // A pair of bfloat16 with what is not finite taken out; `bad` says whether there was any.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t v, bool& bad) {
   const bool lo = (v & 0x7f80u) == 0x7f80u, hi = (v & 0x7f800000u) == 0x7f800000u;
@@ -208,7 +219,7 @@ __device__ __noinline__ void change_scores(uint32_t s_addr, const NhvScoreCap& c
   tmem_st_wait();
 }
 // A thread group's pass over a tile of values in shared memory: rows that are no key of the request become zeros, and, with
-// `finite`, so does what is not finite, each such key noted in bad[4].
+// `finite`, so does what is not finite, each such key noted in bad_keys[2].
 template <int DB, int BN>
 __device__ __noinline__ void clean_values(unsigned char* v, uint32_t* bad_keys, bool finite, bool missing, int key0, int total, const int* table,
                                           int page_size, int n_pages) {
@@ -230,7 +241,7 @@ __device__ __noinline__ void clean_values(unsigned char* v, uint32_t* bad_keys, 
   }
   fence_async_smem();
 }
-// Values taken out above, back to a row that sees them: p v, of what is not finite in v, added to O in tensor memory.  `notes`: the 8 x 4
+// Values taken out above, back to a row that sees them: p v, of what is not finite in v, added to O in tensor memory.  `notes`: the 8 x 2
 // words of keys, from key `key0` on in tiles of BN.
 template <int DB, int BN>
 __device__ __noinline__ void return_values(uint32_t o_addr, const ScoredArgs& a, const uint32_t* notes, int seq, int kvh, int head, int token, int key0,
@@ -240,9 +251,9 @@ __device__ __noinline__ void return_values(uint32_t o_addr, const ScoredArgs& a,
     uint32_t o[32];
     tmem_ld32_nowait(o, o_addr + c0);
     tmem_ld_wait();
-    for (int w = 0; w < 32; ++w)
+    for (int w = 0; w < 16; ++w)
       for (uint32_t bits = notes[w]; bits; bits &= bits - 1) {
-        const int key = key0 + (w >> 2) * BN + (w & 3) * 32 + __ffs(bits) - 1;
+        const int key = key0 + (w >> 1) * BN + (w & 1) * 32 + __ffs(bits) - 1;
         if (key > row_hi) continue;
         const long long k_at = key_row(a, seq, key, kvh, 0), v_at = key_row(a, seq, key, kvh, 1);
         if (k_at < 0) continue;
@@ -264,20 +275,59 @@ __device__ __noinline__ void return_values(uint32_t o_addr, const ScoredArgs& a,
   tmem_st_wait();
 }
 
-// Loads `BN` keys or values of a request, from key0 on, into one stage: boxes of p.box rows, which lie in one page each.  Boxes at
-// or behind `total` and those without a page bring some other row of the pool: their scores are replaced and their values cleared.
-template <int DB, int BN>
-__device__ __forceinline__ void load_tile(unsigned char* stage, const LongArgs& p, const int* table, int key0, int total, int kvh, int plane, uint64_t* bar) {
-  mbar_expect_tx(bar, DB * BN * 128);
-  const int step = p.box < BN ? p.box : BN;
-  for (int r = 0; r < BN; r += step) {
-    const int j = key0 + r < total ? key0 + r : total - 1;
-    int page = table[j / p.a.page_size];
-    page = page < 0 || page >= p.a.n_pages ? 0 : page;
-    const int row = ((page * 2 + plane) * p.a.nkv + kvh) * p.a.page_size + (j % p.a.page_size) / step * step;
-#pragma unroll
-    for (int b = 0; b < DB; ++b) tma_load_2d(stage + b * (BN * 128) + r * 128, &p.kv_map, b * 64, row, bar);
+// Where tiles of BN keys lie: a lane per box of rows, which lie in one page each.  A lane asks for the page of its box a tile ahead (one
+// lane that looked each tile up and then sent for it took 1,900 cycles a tile).  Boxes at or behind `total` and those without a page
+// bring some other row: their scores are replaced and their values cleared.
+template <int BN>
+struct BoxWalk {
+  const int* table;
+  int at, off, last_at, last_off, key, total, page;        // page index and place of the lane's box, and of the request's last box
+  int page_size, step;
+  __device__ __forceinline__ BoxWalk(const LongArgs& p, int seq, int key0, int total_, int lane)
+      : table(p.a.block_table + (size_t)seq * p.a.bt_stride), total(total_), page_size(p.a.page_size), step(p.box < BN ? p.box : BN) {
+    key = key0 + lane * step;
+    at = key / page_size;
+    off = key - at * page_size;
+    last_at = (total - 1) / page_size;
+    last_off = (total - 1 - last_at * page_size) / step * step;
+    ask();
   }
+  __device__ __forceinline__ void ask() { page = table[key < total ? at : last_at]; }
+  // the pool's row of the box asked for
+  __device__ __forceinline__ int row(const LongArgs& p, int kvh) const {
+    const int use = page < 0 || page >= p.a.n_pages ? 0 : page;
+    return (use * 2 * p.a.nkv + kvh) * page_size + (key < total ? off : last_off);
+  }
+  __device__ __forceinline__ void next() {                  // asks for the box of the next tile
+    key += BN;
+    off += BN;
+    while (off >= page_size) {
+      off -= page_size;
+      ++at;
+    }
+    ask();
+  }
+};
+// The warp's copy of a tile of keys (plane 0) or values (plane 1) into one stage.
+template <int DB, int BN>
+__device__ __forceinline__ void load_tile(unsigned char* stage, const LongArgs& p, int row, int plane, uint64_t* bar, int lane) {
+  const int step = p.box < BN ? p.box : BN;
+  if (step == BN) {                                         // one box, one lane, with what it needs the same in all
+    const int y = __shfl_sync(0xffffffffu, row, 0) + plane * p.a.nkv * p.a.page_size;
+    if (elect_one()) {
+      mbar_expect_tx(bar, DB * BN * 128);
+#pragma unroll
+      for (int b = 0; b < DB; ++b) tma_load_2d(stage + b * (BN * 128), &p.kv_map, b * 64, y, bar);
+    }
+  } else {
+    if (lane == 0) mbar_expect_tx(bar, DB * BN * 128);
+    __syncwarp();
+    if (lane * step < BN) {
+#pragma unroll
+      for (int b = 0; b < DB; ++b) tma_load_2d(stage + b * (BN * 128) + lane * step * 128, &p.kv_map, b * 64, row + plane * p.a.nkv * p.a.page_size, bar);
+    }
+  }
+  __syncwarp();
 }
 template <int DB>
 __device__ __forceinline__ void load_rows(unsigned char* stage, const LongArgs& p, int token, int kvh, int G, uint64_t* bar) {
@@ -293,32 +343,35 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
   extern __shared__ __align__(128) unsigned char smem_raw[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw);
   uint64_t* full = bars;                   // [STAGES]
-  uint64_t* empty = bars + 8;              // [STAGES]
-  uint64_t* s_full = bars + 16;            // [NQ]
-  uint64_t* p_ready = bars + 18;           // [NQ][2]: the halves of a tile's P
-  uint64_t* o_full = bars + 22;            // [NQ]
-  uint64_t* q_full = bars + 24;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
-  int* s_abort = reinterpret_cast<int*>(bars + 26);
-  int* s_missing = reinterpret_cast<int*>(bars + 27);
-  uint32_t* s_bad = reinterpret_cast<uint32_t*>(bars + 32);       // [8 tiles][4]: keys whose values are not all finite
+  uint64_t* empty = bars + 12;             // [STAGES]
+  uint64_t* s_full = bars + 24;            // [NQ][2]
+  uint64_t* p_ready = bars + 28;           // [NQ][2]: by buffer, since the rows may be a tile ahead of the products
+  uint64_t* o_full = bars + 32;            // [NQ]: after every product
+  uint64_t* o_last = bars + 34;            // [NQ]: after the last one
+  uint64_t* q_full = bars + 36;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 37);
+  int* s_abort = reinterpret_cast<int*>(bars + 38);
+  int* s_missing = reinterpret_cast<int*>(bars + 39);
+  uint32_t* s_bad = reinterpret_cast<uint32_t*>(bars + 40);       // [8 tiles][2]: keys whose values are not all finite
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* tiles = smem_raw + (((raw + 1024 + 1023u) & ~1023u) - raw);
   unsigned char* q_s = tiles;                          // [NQ][Q_BYTES]
   unsigned char* kv_s = q_s + NQ * C::Q_BYTES;         // [STAGES][STAGE]
 
   const ScoredArgs& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int q = 0; q < NQ; ++q) {
-      mbar_init(&s_full[q], 1);
+      mbar_init(&s_full[2 * q], 1);
+      mbar_init(&s_full[2 * q + 1], 1);
       mbar_init(&p_ready[2 * q], 128);
       mbar_init(&p_ready[2 * q + 1], 128);
       mbar_init(&o_full[q], 1);
+      mbar_init(&o_last[q], 1);
     }
     mbar_init(q_full, 1);
     *s_abort = 0;
@@ -327,7 +380,7 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
     asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&p.kv_map) : "memory");
     asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&p.q_map) : "memory");
   }
-  if (threadIdx.x < 32) s_bad[threadIdx.x] = 0;
+  if (threadIdx.x < 16) s_bad[threadIdx.x] = 0;
   if (warp == 1) tmem_alloc(tmem_slot, C::TMEM_COLS);
   pdl_prologue();
 
@@ -357,32 +410,38 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  const int n_tiles = max(nt[0], nt[1]);
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const int n_tiles = __shfl_sync(0xffffffffu, max(nt[0], nt[1]), 0);
+  nt[0] = __shfl_sync(0xffffffffu, nt[0], 0);
+  nt[1] = __shfl_sync(0xffffffffu, nt[1], 0);
 
-  // Registers go where the rows are: 384 threads start with 168 each, 64,512 in all; 128 x 80 + 256 x 208 = 63,488.
-  if (warp < 4) {
-  if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0 && n_tiles > 0) {
-      const int* table = a.block_table + (size_t)seq * a.bt_stride;
-      mbar_expect_tx(q_full, (uint32_t)((nt[0] > 0) + (nt[1] > 0)) * DB * p.tokens * G * 128);
-      for (int q = 0; q < NQ; ++q)
-        if (nt[q] > 0) {
+    if (n_tiles > 0) {
+      BoxWalk<BN> walk(p, seq, key_begin, total, lane);
+      if (lane == 0) {
+        mbar_expect_tx(q_full, (uint32_t)((nt[0] > 0) + (nt[1] > 0)) * DB * p.tokens * G * 128);
+        for (int q = 0; q < NQ; ++q)
+          if (nt[q] > 0) {
 #pragma unroll
-          for (int b = 0; b < DB; ++b) tma_load_3d(q_s + q * C::Q_BYTES + b * (BM * 128), &p.q_map, b * 64, kvh * G, first + t0 + q * p.tokens, q_full);
-        }
+            for (int b = 0; b < DB; ++b) tma_load_3d(q_s + q * C::Q_BYTES + b * (BM * 128), &p.q_map, b * 64, kvh * G, first + t0 + q * p.tokens, q_full);
+          }
+      }
+      __syncwarp();
       bool ok = true;
       int sent = 0;
-      for (int i = 0; i < 2 * n_tiles && ok; ++i) {
-        const int st = i % STAGES;
-        if (i >= STAGES) ok = mbar_wait(&empty[st], (uint32_t)(i / STAGES - 1) & 1, 1);
-        if (!ok) break;
-        load_tile<DB, BN>(kv_s + st * C::STAGE, p, table, key_begin + (i >> 1) * BN, total, kvh, i & 1, &full[st]);
-        sent = i + 1;
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int row = walk.row(p, kvh);
+        walk.next();
+        for (int plane = 0; plane < 2 && ok; ++plane) {
+          const int i = 2 * j + plane, st = i % STAGES;
+          if (i >= STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (uint32_t)(i / STAGES - 1) & 1, 1));
+          if (!ok) break;
+          load_tile<DB, BN>(kv_s + st * C::STAGE, p, row, plane, &full[st], lane);
+          sent = i + 1;
+        }
       }
-      if (!ok) {
+      if (!ok && lane == 0) {
         *s_abort = 1;
         mbar_wait(q_full, 0, 2);
         for (int i = max(0, sent - STAGES); i < sent; ++i) mbar_wait(&full[i % STAGES], (uint32_t)(i / STAGES) & 1, 2);
@@ -391,74 +450,70 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && n_tiles > 0) {
+    if (n_tiles > 0) {
       const uint32_t idesc_s = instr_desc(BM, BN, false), idesc_o = instr_desc(BM, DB * 64, true);
       const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024);
       const uint64_t k_desc = smem_desc(smem_u32(kv_s), 16, 1024);
       const uint64_t v_desc = smem_desc(smem_u32(kv_s), BN * 128, 1024);
-      bool ok = mbar_wait(q_full, 0, 3);
+      // every lane waits, and all go on or none
+      auto reached = [&](uint64_t* bar, uint32_t parity, int code) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, code)); };
+      bool ok = reached(q_full, 0, 3);
       tc_fence_after();
-      auto stage_ready = [&](int i) { return mbar_wait(&full[i % STAGES], (uint32_t)(i / STAGES) & 1, 4); };
+      auto stage_ready = [&](int i) { return reached(&full[i % STAGES], (uint32_t)(i / STAGES) & 1, 4); };
       auto first_product = [&](int q, int j) {
+        if (!elect_one()) return;
         const uint64_t kd = k_desc + (uint64_t)(((2 * j) % STAGES) * (C::STAGE >> 4)), qd = q_desc + (uint64_t)(q * (C::Q_BYTES >> 4));
 #pragma unroll
         for (int kk = 0; kk < DB * 4; ++kk)
-          tc_mma(tmem_base + C::S_COL + q * BN, qd + (uint64_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
+          tc_mma(tmem_base + C::S_COL + (2 * q + (j & 1)) * BN, qd + (uint64_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
                  kd + (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
-        tc_commit(&s_full[q]);
+        tc_commit(&s_full[2 * q + (j & 1)]);
       };
-      auto second_product = [&](int q, int j, int half) {
+      auto second_product = [&](int q, int j) {
+        if (!elect_one()) return;
         const uint64_t vd = v_desc + (uint64_t)(((2 * j + 1) % STAGES) * (C::STAGE >> 4));
-        const uint32_t pa = tmem_base + C::S_COL + q * BN;           // P lies over the first half of S
+        const uint32_t pa = tmem_base + C::S_COL + (2 * q + (j & 1)) * BN;       // P lies over the first half of S
 #pragma unroll
-        for (int i = 0; i < BN / 32; ++i) {                           // 8 columns of P and 16 rows of V per 16 keys
-          const int kk = half * (BN / 32) + i;
+        for (int kk = 0; kk < BN / 16; ++kk)                          // 8 columns of P and 16 rows of V per 16 keys
           tc_mma_a_tmem(tmem_base + C::O_COL + q * (DB * 64), pa + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), idesc_o,
                         (j > 0 || kk > 0) ? 1u : 0u);
-        }
+        tc_commit(&o_full[q]);
+        if (j == nt[q] - 1) tc_commit(&o_last[q]);
       };
       if (ok) ok = stage_ready(0);
       if (ok) {
         tc_fence_after();
         for (int q = 0; q < NQ; ++q)
           if (nt[q] > 0) first_product(q, 0);
-        tc_commit(&empty[0]);
+        if (elect_one()) tc_commit(&empty[0]);
+        __syncwarp();
       }
       for (int j = 0; j < n_tiles && ok; ++j) {
-        bool have_v = false, have_k = false;
+        // the next tile's S goes to the other buffer, whose P the products before have read
+        if (j + 1 < n_tiles) {
+          ok = stage_ready(2 * j + 2);
+          if (!ok) break;
+          tc_fence_after();
+          for (int q = 0; q < NQ; ++q)
+            if (j + 1 < nt[q]) first_product(q, j + 1);
+          if (elect_one()) tc_commit(&empty[(2 * j + 2) % STAGES]);
+          __syncwarp();
+        }
+        ok = stage_ready(2 * j + 1);
         for (int q = 0; q < NQ && ok; ++q) {
           if (j >= nt[q]) continue;
-          ok = mbar_wait(&p_ready[2 * q], (uint32_t)j & 1, 5);
-          if (ok && !have_v) ok = stage_ready(2 * j + 1);
-          have_v = true;
+          ok = reached(&p_ready[2 * q + (j & 1)], (uint32_t)(j >> 1) & 1, 5);
           if (!ok) break;
           tc_fence_after();
-          second_product(q, j, 0);
-          ok = mbar_wait(&p_ready[2 * q + 1], (uint32_t)j & 1, 5);
-          if (!ok) break;
-          tc_fence_after();
-          second_product(q, j, 1);
-          if (j + 1 < nt[q]) {
-            if (!have_k) ok = stage_ready(2 * j + 2);
-            have_k = true;
-            if (!ok) break;
-            tc_fence_after();
-            first_product(q, j + 1);
-          } else {
-            tc_commit(&o_full[q]);
-          }
+          second_product(q, j);
         }
-        if (!ok) break;
-        tc_commit(&empty[(2 * j + 1) % STAGES]);
-        if (j + 1 < n_tiles) tc_commit(&empty[(2 * j + 2) % STAGES]);
+        if (ok && elect_one()) tc_commit(&empty[(2 * j + 1) % STAGES]);
+        __syncwarp();
       }
       if (!ok) *s_abort = 1;
     }
     __syncwarp();
-  }
-  } else {
-  if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
-  if (seq >= 0) {
+  } else if (warp >= 4 && seq >= 0) {
     // ------------------------------------------------------------------ softmax and output: a thread per row
     const int q = (warp - 4) >> 2, quarter = warp & 3, R = quarter * 32 + lane;
     const int tq = R / G, g = R - tq * G, token = t0 + q * p.tokens + tq;
@@ -469,7 +524,7 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
     const bool missing = *s_missing != 0;
     const int* table = a.block_table + (size_t)seq * a.bt_stride;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_addr = lane_addr + C::S_COL + q * BN, o_addr = lane_addr + C::O_COL + q * (DB * 64);
+    const uint32_t s_base = lane_addr + C::S_COL + q * 2 * BN, o_addr = lane_addr + C::O_COL + q * (DB * 64);
     float m = -INFINITY, l = 0.f;
     // the first tile of which some row of the block does not see all; the notes on values begin there
     const int first_edge = max(0, total - n + t0 + 1 - key_begin) / BN;
@@ -477,14 +532,15 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
     const f32x2 scale2 = f2_pack(p.scale_log2, p.scale_log2);
     for (int j = 0; j < tiles_q; ++j) {
       const int key0 = key_begin + j * BN;
+      const uint32_t s_addr = s_base + (j & 1) * BN;
       // Values that some row of the block does not see: the first tile's group looks them through for both, whose product comes first.
       if ((missing || key0 + BN - 1 > total - n + t0) && (q == 0 || j >= nt[0])) {
         const int st = (2 * j + 1) % STAGES;
         ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)((2 * j + 1) / STAGES) & 1, 7));
         if (!ok) break;
-        clean_values<DB, BN>(kv_s + st * C::STAGE, &s_bad[((j - first_edge) & 7) * 4], j >= first_edge, missing, key0, total, table, a.page_size, a.n_pages);
+        clean_values<DB, BN>(kv_s + st * C::STAGE, &s_bad[((j - first_edge) & 7) * 2], j >= first_edge, missing, key0, total, table, a.page_size, a.n_pages);
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[q], (uint32_t)j & 1, 6));
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * q + (j & 1)], (uint32_t)(j >> 1) & 1, 6));
       if (!ok) break;
       tc_fence_after();
       const bool masked = key0 + BN - 1 > all_hi || missing;           // some row does not see some key of the tile
@@ -510,6 +566,10 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
           l *= alpha;
         }
         if (j > 0) {
+          // the product before must be complete (the one before that is, or this S would not be: a parity tells the two apart)
+          ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], (uint32_t)(j - 1) & 1, 8));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll 1
           for (int c0 = 0; c0 < DB * 64; c0 += 16) {
             uint32_t o[16];
@@ -524,33 +584,28 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
       const float neg_ref = m == -INFINITY ? 0.f : -m;
       const f32x2 ref2 = f2_pack(neg_ref, neg_ref);
       f32x2 l2[4] = {0ull, 0ull, 0ull, 0ull};
+      uint32_t pk[BN / 2];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t pk[BN / 4];
-#pragma unroll
-        for (int i = 0; i < BN / 2; i += 2) {
-          const int at = half * (BN / 2) + i;
-          float x, y;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[at >> 5][at & 31]), __uint_as_float(sr[at >> 5][(at & 31) + 1])), scale2, ref2), x, y);
-          x = scored_exp2(x);
-          y = scored_exp2(y);
-          pk[i >> 1] = pack_bf16(x, y);
-          l2[(i >> 1) & 3] = f2_add(l2[(i >> 1) & 3], f2_pack(x, y));   // the row's sum in fp32, before the rounding to bfloat16
-        }
-#pragma unroll
-        for (int c = 0; c < BN / 4; c += 16) tmem_st16(s_addr + half * (BN / 4) + c, pk + c);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_ready[2 * q + half]);
+      for (int i = 0; i < BN; i += 2) {
+        float x, y;
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[i >> 5][i & 31]), __uint_as_float(sr[i >> 5][(i & 31) + 1])), scale2, ref2), x, y);
+        x = scored_exp2(x);
+        y = scored_exp2(y);
+        pk[i >> 1] = pack_bf16(x, y);
+        l2[(i >> 1) & 3] = f2_add(l2[(i >> 1) & 3], f2_pack(x, y));     // the row's sum in fp32, before the rounding to bfloat16
       }
+      tmem_st32(s_addr, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_ready[2 * q + (j & 1)]);
       l += f2_sum(f2_add(l2[0], l2[1]), f2_add(l2[2], l2[3]));
     }
-    if (ok && tiles_q > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[q], 0, 8));
+    if (ok && tiles_q > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_last[q], 0, 8));
     if (ok) {
       tc_fence_after();
       // the notes on values: made before the products that o_full covers
       bool any_bad = false;
-      for (int i = 0; i < 32; ++i) any_bad |= *(volatile uint32_t*)&s_bad[i] != 0;
+      for (int i = 0; i < 16; ++i) any_bad |= *(volatile uint32_t*)&s_bad[i] != 0;
       if (any_bad && tiles_q > 0)
         return_values<DB, BN>(o_addr, a, s_bad, seq, kvh, kvh * G + g, first + token, key_begin + first_edge * BN, row_hi, m, p.scale_log2);
       const size_t row = (size_t)kvh * a.n_tokens * G + (size_t)(first + token) * G + g;
@@ -603,7 +658,6 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
       *s_abort = 1;
     }
   }
-  }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -612,7 +666,7 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
   }
 }
 
-template <int DB>
+template <int DB, bool CAP>
 __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_keys_tcgen05_kernel(const __grid_constant__ LongArgs p) {
   using C = Keys<DB>;
   constexpr int STAGES = C::STAGES;
@@ -625,14 +679,15 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
   uint64_t* k_full = bars + 12;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
   int* s_abort = reinterpret_cast<int*>(bars + 15);
-  float* s_lse = reinterpret_cast<float*>(smem_raw + 1024);        // [2][128]
+  float* s_part = reinterpret_cast<float*>(bars + 32);             // [128]
+  float* s_lse = reinterpret_cast<float*>(smem_raw + 1024);        // [2][128], negated
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* tiles = smem_raw + (((raw + 2048 + 1023u) & ~1023u) - raw);
   unsigned char* k_s = tiles;
   unsigned char* q_s = k_s + C::K_BYTES;               // [STAGES][STAGE]
 
   const ScoredArgs& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -640,7 +695,7 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&s_free[s], 128);
+      mbar_init(&s_free[s], 256);
     }
     mbar_init(k_full, 1);
     *s_abort = 0;
@@ -657,25 +712,28 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
   int begin = 0, end = 0;
   const bool mine = key0 < total && scored_takes(a, n);
   if (mine) chunk_range(p.parts, n, G, total, key0, chunk, begin, end);
-  const int n_tiles = max(0, end - begin);
+  const int n_tiles = __shfl_sync(0xffffffffu, max(0, end - begin), 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 0) {
-    if (lane == 0 && n_tiles > 0) {
-      load_tile<DB, BM>(k_s, p, a.block_table + (size_t)seq * a.bt_stride, key0, total, kvh, 0, k_full);
+    if (n_tiles > 0)
+      load_tile<DB, BM>(k_s, p, BoxWalk<BM>(p, seq, key0, total, lane).row(p, kvh), 0, k_full, lane);
+    if (n_tiles > 0) {
       bool ok = true;
       int sent = 0;
+      const int token = __shfl_sync(0xffffffffu, first + begin * p.tokens, 0);
       for (int i = 0; i < n_tiles && ok; ++i) {
         const int st = i % STAGES;
-        if (i >= STAGES) ok = mbar_wait(&empty[st], (uint32_t)(i / STAGES - 1) & 1, 11);
+        if (i >= STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (uint32_t)(i / STAGES - 1) & 1, 11));
         if (!ok) break;
-        load_rows<DB>(q_s + st * C::STAGE, p, first + (begin + i) * p.tokens, kvh, G, &full[st]);
+        if (elect_one()) load_rows<DB>(q_s + st * C::STAGE, p, token + i * p.tokens, kvh, G, &full[st]);
+        __syncwarp();
         sent = i + 1;
       }
-      if (!ok) {
+      if (!ok && lane == 0) {
         *s_abort = 1;
         mbar_wait(k_full, 0, 12);
         for (int i = max(0, sent - STAGES); i < sent; ++i) mbar_wait(&full[i % STAGES], (uint32_t)(i / STAGES) & 1, 12);
@@ -683,30 +741,33 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && n_tiles > 0) {
+    if (n_tiles > 0) {
       const uint32_t idesc = instr_desc(BM, C::BN, false);
       const uint64_t k_desc = smem_desc(smem_u32(k_s), 16, 1024), q_desc = smem_desc(smem_u32(q_s), 16, 1024);
-      bool ok = mbar_wait(k_full, 0, 13);
+      bool ok = __all_sync(0xffffffffu, mbar_wait(k_full, 0, 13));
       for (int i = 0; i < n_tiles && ok; ++i) {
         const int st = i % STAGES, buf = i & 1;
-        ok = mbar_wait(&full[st], (uint32_t)(i / STAGES) & 1, 14);
-        if (ok && i >= 2) ok = mbar_wait(&s_free[buf], (uint32_t)(i / 2 - 1) & 1, 15);
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)(i / STAGES) & 1, 14));
+        if (ok && i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&s_free[buf], (uint32_t)(i / 2 - 1) & 1, 15));
         if (!ok) break;
         tc_fence_after();
-        const uint64_t qd = q_desc + (uint64_t)(st * (C::STAGE >> 4));
+        if (elect_one()) {
+          const uint64_t qd = q_desc + (uint64_t)(st * (C::STAGE >> 4));
 #pragma unroll
-        for (int kk = 0; kk < DB * 4; ++kk)
-          tc_mma(tmem_base + buf * C::BN, k_desc + (uint64_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
-                 qd + (uint64_t)(((kk >> 2) * (C::BN * 128) + (kk & 3) * 32) >> 4), idesc, kk > 0 ? 1u : 0u);
-        tc_commit(&empty[st]);
-        tc_commit(&s_full[buf]);
+          for (int kk = 0; kk < DB * 4; ++kk)
+            tc_mma(tmem_base + buf * C::BN, k_desc + (uint64_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
+                   qd + (uint64_t)(((kk >> 2) * (C::BN * 128) + (kk & 3) * 32) >> 4), idesc, kk > 0 ? 1u : 0u);
+          tc_commit(&empty[st]);
+          tc_commit(&s_full[buf]);
+        }
+        __syncwarp();
       }
       if (!ok) *s_abort = 1;
     }
     __syncwarp();
   } else if (mine) {
-    // ------------------------------------------------------------------ a thread per key
-    const int quarter = warp & 3, at = quarter * 32 + lane, key = key0 + at;
+    // ------------------------------------------------------------------ two threads per key, for half of the columns each
+    const int quarter = warp & 3, half = (warp - 2) >> 2, at = quarter * 32 + lane, key = key0 + at;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const float* lse = a.lse + ((size_t)kvh * a.n_tokens + first) * G;
     const int rows = n * G, tile_rows = p.tokens * G;
@@ -714,50 +775,62 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
       const int r = (begin + i) * tile_rows + at;
       return i < n_tiles && at < tile_rows && r < rows ? lse[r] : INFINITY;
     };
-    float next = lse_of(0), sum = 0.f;
+    const f32x2 scale2 = f2_pack(p.scale_log2, p.scale_log2);
+    float next = half == 0 ? lse_of(0) : 0.f, sum = 0.f;
     bool ok = true;
     for (int i = 0; i < n_tiles; ++i) {
       const int buf = i & 1, t_first = (begin + i) * p.tokens;
-      s_lse[buf * 128 + at] = next;
-      next = lse_of(i + 1);
-      group_sync(1);                                    // all come here in every round, also behind a wait that ran out
+      if (half == 0) {
+        s_lse[buf * 128 + at] = -next;
+        next = lse_of(i + 1);
+      }
+      pair_sync(1);                                     // all come here in every round, also behind a wait that ran out
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buf], (uint32_t)(i / 2) & 1, 16));
       if (!ok) continue;
       tc_fence_after();
+      uint32_t s[2][32];
+      tmem_ld32_nowait(s[0], lane_addr + buf * C::BN + half * 64);
+      tmem_ld32_nowait(s[1], lane_addr + buf * C::BN + half * 64 + 32);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(&s_free[buf]);
+      if (CAP) {
+        cap32(s[0], p.cap);
+        cap32(s[1], p.cap);
+      }
       // rows behind the request's last and those that do not see every key of the tile
       const bool masked = key0 + BM - 1 > total - n + t_first || (begin + i + 1) * tile_rows > rows || tile_rows < C::BN;
-      // the first column that this key is seen by, and the first behind the rows
-      const int lo = (key - (total - n) - t_first) * G, hi = min(tile_rows, rows - (begin + i) * tile_rows);
-      float w0 = 0.f, w1 = 0.f, w2 = 0.f, w3 = 0.f;
+      const float4* ls = reinterpret_cast<const float4*>(s_lse + buf * 128 + half * 64);
+      f32x2 w[4] = {0ull, 0ull, 0ull, 0ull};
+      if (!masked) {
 #pragma unroll
-      for (int c = 0; c < C::BN / 32; ++c) {
-        uint32_t s[32];
-        tmem_ld32_nowait(s, lane_addr + buf * C::BN + c * 32);
-        tmem_ld_wait();
-        if (c == C::BN / 32 - 1) {
-          tc_fence_before();
-          mbar_arrive(&s_free[buf]);
+        for (int k = 0; k < 64; k += 4) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(ls + (k >> 2));
+          float x0, x1, x2, x3;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[k >> 5][k & 31]), __uint_as_float(s[k >> 5][(k & 31) + 1])), scale2, v.x), x0, x1);
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[k >> 5][(k & 31) + 2]), __uint_as_float(s[k >> 5][(k & 31) + 3])), scale2, v.y), x2, x3);
+          w[(k >> 1) & 3] = f2_add(w[(k >> 1) & 3], f2_pack(scored_exp2(x0), scored_exp2(x1)));
+          w[((k >> 1) + 1) & 3] = f2_add(w[((k >> 1) + 1) & 3], f2_pack(scored_exp2(x2), scored_exp2(x3)));
         }
-        if (p.cap.in != 0.f) cap32(s, p.cap);
+      } else {
+        // the first column that sees this key, and the first behind the rows
+        const int lo = (key - (total - n) - t_first) * G - half * 64, hi = min(tile_rows, rows - (begin + i) * tile_rows) - half * 64;
+        const float* lf = reinterpret_cast<const float*>(ls);
+        float x = 0.f;
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 ls = *reinterpret_cast<const float4*>(s_lse + buf * 128 + c * 32 + k);
-          float x0 = scored_exp2(fmaf(__uint_as_float(s[k]), p.scale_log2, -ls.x)), x1 = scored_exp2(fmaf(__uint_as_float(s[k + 1]), p.scale_log2, -ls.y));
-          float x2 = scored_exp2(fmaf(__uint_as_float(s[k + 2]), p.scale_log2, -ls.z)), x3 = scored_exp2(fmaf(__uint_as_float(s[k + 3]), p.scale_log2, -ls.w));
-          if (masked) {
-            const int r = c * 32 + k;
-            x0 = r >= lo && r < hi ? x0 : 0.f;
-            x1 = r + 1 >= lo && r + 1 < hi ? x1 : 0.f;
-            x2 = r + 2 >= lo && r + 2 < hi ? x2 : 0.f;
-            x3 = r + 3 >= lo && r + 3 < hi ? x3 : 0.f;
-          }
-          w0 += x0; w1 += x1; w2 += x2; w3 += x3;
+        for (int k = 0; k < 64; ++k) {
+          const float e = scored_exp2(fmaf(__uint_as_float(s[k >> 5][k & 31]), p.scale_log2, lf[k]));
+          x += k >= lo && k < hi ? e : 0.f;
         }
+        w[0] = f2_pack(x, 0.f);
       }
-      sum += (w0 + w1) + (w2 + w3);
+      sum += f2_sum(f2_add(w[0], w[1]), f2_add(w[2], w[3]));
     }
     if (!ok) *s_abort = 1;
-    else if (key < total) {
+    if (half == 1) s_part[at] = sum;
+    pair_sync(1);
+    if (ok && half == 0 && key < total) {
+      sum += s_part[at];
       if (p.parts.chunks == 1) store_weight(a, seq, first, kvh, key, key - (total - n), sum);
       else if (n_tiles > 0) p.parts.w[(((size_t)seq * a.nkv + kvh) * p.parts.chunks + chunk) * p.parts.keys + key] = sum;
     }
@@ -783,12 +856,12 @@ int launch_long(const LongArgs& p, int row_tiles, cudaStream_t stream) {
   static std::atomic<uint64_t> rows_done{0}, keys_done{0};
   const ScoredArgs& a = p.a;
   NHV_CUDA(nhv_allow_smem((const void*)scored_rows_tcgen05_kernel<DB, CAP>, Rows<DB>::SMEM, rows_done), "scored attention (tcgen05)");
-  NHV_CUDA(nhv_allow_smem((const void*)scored_keys_tcgen05_kernel<DB>, Keys<DB>::SMEM, keys_done), "scored attention (tcgen05)");
+  NHV_CUDA(nhv_allow_smem((const void*)scored_keys_tcgen05_kernel<DB, CAP>, Keys<DB>::SMEM, keys_done), "scored attention (tcgen05)");
   NHV_CUDA(nhv_launch(scored_rows_tcgen05_kernel<DB, CAP>, dim3(a.nkv, row_tiles, p.parts.splits), Rows<DB>::THREADS, Rows<DB>::SMEM, stream, p),
            "scored attention (tcgen05)");
   int rc = scored_join_rows(NHV_BF16, a, p.parts, stream);
   if (rc) return rc;
-  NHV_CUDA(nhv_launch(scored_keys_tcgen05_kernel<DB>, dim3(a.nkv, p.key_tiles * p.parts.chunks, a.n_seqs), Keys<DB>::THREADS, Keys<DB>::SMEM, stream, p),
+  NHV_CUDA(nhv_launch(scored_keys_tcgen05_kernel<DB, CAP>, dim3(a.nkv, p.key_tiles * p.parts.chunks, a.n_seqs), Keys<DB>::THREADS, Keys<DB>::SMEM, stream, p),
            "scored attention (tcgen05)");
   return scored_join_keys(a, p.parts, stream);
 }
@@ -806,7 +879,7 @@ size_t scored_long_plan(ScoredParts& p, int n_seqs, int n_tokens, int max_new, i
   const int G = nq / nkv, tokens = BM / G;
   p.tile_rows = tokens * G;
   p.tile_keys = BM;
-  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, (d <= 128 ? 2 : 1) * tokens * G, d <= 128 ? 128 : 64, 2500.0, SMS, 2 * SMS);
+  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, (d <= 128 ? 2 : 1) * tokens * G, 64, 1400.0, SMS, 2 * SMS);
 }
 
 int scored_long_launch(ScoredArgs a, const ScoredParts& parts, cudaStream_t stream) {
@@ -817,8 +890,8 @@ int scored_long_launch(ScoredArgs a, const ScoredParts& parts, cudaStream_t stre
   p.parts = parts;
   p.tokens = BM / (a.nq / a.nkv);
   p.key_tiles = (int)(parts.keys / BM);
-  const int db = (a.d + 63) / 64, nq_tiles = db <= 2 ? 2 : 1, bn = db <= 2 ? 128 : 64;
-  p.box = divisor(a.page_size, bn);
+  const int db = (a.d + 63) / 64, nq_tiles = db <= 2 ? 2 : 1;
+  p.box = divisor(a.page_size, 64);
   const long long pool = (long long)a.n_pages * 2 * a.nkv * a.page_size;
   NHV_REQUIRE(pool < (1LL << 31), "scored attention (tcgen05): the pool's %lld rows are beyond a 32-bit coordinate", pool);
   NHV_REQUIRE(nhv_make_map_bf16(&p.kv_map, a.pages, pool, a.d, a.d, 64, p.box), "scored attention (tcgen05): cannot encode the tensor map of the pool");
