@@ -92,12 +92,14 @@ int scored_join_keys(const ScoredArgs& a, const ScoredParts& p, cudaStream_t str
 // ---- requests with few rows (scored_attention_short.cu): the keys are split over blocks, the scores kept for the second pass
 struct ShortPlan {
   int rows;                 // rows kept per key: the most of a request, rounded up to 2
-  int split_keys, splits;   // keys of a block, blocks of a request's KV head
+  int block_rows, row_blocks;       // rows of a block, blocks that share a request's rows
+  int split_keys, splits;   // keys of a block, parts of a request's keys
   int group;                // requests per pair of launches (the scores kept are bounded)
   size_t keys;              // places for keys of a (request, KV head)
   size_t floats;            // of scratch
 };
-// Whether requests of up to `rows` rows can go this way.
+// The most rows of a request that goes this way, and whether requests of up to `rows` rows can.
+int scored_short_rows(int d);
 bool scored_short_takes(int dtype, int rows, int d);
 ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d);
 // The requests with a.min_rows to a.max_rows rows: output, scores and births.  `work`: plan.floats floats.

@@ -452,17 +452,17 @@ size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int m
                     double tile_cycles, int rows_at_once, int keys_at_once) {
   const int G = nq / nkv;
   // the rows' pass: parts of the keys where whole walks fill the SMs badly.  With `blocks` walks and `at_once` places, s parts take
-  // ceil(blocks s / at_once) / s walks' time, and each part's sums are written and read once, 8 bytes an element at some 30 bytes a
-  // cycle; no part is below `least` tiles.  Walks of a prompt without earlier keys are of every length, and their longest go first:
-  // there parts pay only if SMs would idle.
+  // one s-th of a walk where all run at once, else the work's share and half a part more for the last ones to end; each part's sums
+  // are written and read once, 8 bytes an element at some 30 bytes a cycle.  One request's walks are alike but for the causal edge, and
+  // come in whole rounds.  No part is below `least` tiles.
   const long long blocks = ((long long)n_tokens * G / row_tile + n_seqs) * nkv;        // at most
   const int tiles = (max_keys + key_tile - 1) / key_tile, least = key_tile * row_tile >= 128 * 128 ? 8 : 3;
-  const bool alike = max_keys >= 2 * max_new;
+  const bool alike = n_seqs == 1 && max_keys >= 2 * max_new;
   int splits = 1;
   double best = 1e30;
   const double sums = row_tile * d * 8 / 30.0 / (tile_cycles * tiles);
   for (int s = 1; s <= 64 && (s == 1 || tiles / s >= least); ++s) {
-    const double waves = alike || blocks * s <= rows_at_once ? (double)((blocks * s + rows_at_once - 1) / rows_at_once) : (double)blocks * s / rows_at_once;
+    const double waves = alike || blocks * s <= rows_at_once ? (double)((blocks * s + rows_at_once - 1) / rows_at_once) : (double)blocks * s / rows_at_once + 0.5;
     const double cost = waves / s + (s > 1 ? s * sums : 0.0);
     if (cost < best - 1e-9) {
       best = cost;
@@ -522,7 +522,7 @@ static ScoredPlan scored_plan(int dtype, bool wide, int n_seqs, int n_tokens, in
   ScoredPlan p = {};
   p.wide = wide && d % 8 == 0;
   p.short_rows = -1;
-  const int G = nq / nkv, most = d <= 128 ? 16 : 8;
+  const int G = nq / nkv, most = scored_short_rows(d);
   size_t few = 0, rest = 0;
   if (p.wide && min_new <= most && scored_short_takes(dtype, min_new * G, d)) {
     p.short_rows = most;

@@ -1,7 +1,8 @@
-// Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), up to 16 of
+// Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), up to 32 of
 // them: decoded tokens, drafts.  All the work is to read the keys and values once.
 //
-// First kernel: a block per (part of a request's keys, KV head, request), its warps independent of one another.  A warp takes 16
+// First kernel: a block per (part of a request's keys, up to 16 of its rows, KV head, request), its warps independent of one
+// another; blocks for other rows of the same keys find them in L2.  A warp takes 16
 // keys at a time straight from the pages into registers and forms S^T = K Q^T (m16n8k16, the 16 keys as M, up to 8 rows as N) and
 // O^T += V^T P^T.  No shared memory is between the pages and the products: which element of a head stands at which index of the
 // product is free as long as both operands agree, so a lane takes 16 consecutive bytes of a row and its registers are the fragment
@@ -32,7 +33,7 @@ struct ShortArgs {
   float* part_o;            // [group][nkv][splits][rows][d]
   float* part_ml;           // [group][nkv][splits][rows][2]: reference and sum
   size_t keys;
-  int rows, split_keys, splits, first_seq;
+  int rows, block_rows, row_blocks, split_keys, splits, first_seq;
 };
 
 __device__ __forceinline__ uint4 load16(const void* p) {
@@ -64,15 +65,16 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
   pdl_prologue();
   const int seq = w.first_seq + blockIdx.z, kvh = blockIdx.y, G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), R = n * G, d = a.d;
-  const int begin = blockIdx.x * w.split_keys, end = min(total, begin + w.split_keys);
-  if (begin >= end || n <= 0 || !scored_takes(a, n)) return;
+  const int split = blockIdx.x / w.row_blocks, r0 = (blockIdx.x - split * w.row_blocks) * w.block_rows, RB = min(R - r0, w.block_rows);
+  const int begin = split * w.split_keys, end = min(total, begin + w.split_keys);
+  if (begin >= end || RB <= 0 || !scored_takes(a, n)) return;
   const int ra = lane >> 2, rc = lane & 3;
   const __nv_bfloat16* q = (const __nv_bfloat16*)a.q;
   const __nv_bfloat16* pages = (const __nv_bfloat16*)a.pages;
   const int* table = a.block_table + (size_t)seq * a.bt_stride;
   const size_t v_plane = (size_t)a.nkv * a.page_size * d;
 
-  // the product's B operand: row ra (+ 8), elements 32 i + 8 rc ..
+  // the product's B operand: row r0 + ra (+ 8), elements 32 i + 8 rc ..
   uint4 qf[NT][2 * DB];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -81,7 +83,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
     for (int i = 0; i < 2 * DB; ++i) {
       const int e = 32 * i + 8 * rc;
       qf[t][i] = make_uint4(0, 0, 0, 0);
-      if (r < R && e < d) qf[t][i] = *reinterpret_cast<const uint4*>(q + (size_t)(first + r / G) * a.q_stride + (size_t)(kvh * G + r % G) * d + e);
+      if (r < RB && e < d) qf[t][i] = *reinterpret_cast<const uint4*>(q + (size_t)(first + (r0 + r) / G) * a.q_stride + (size_t)(kvh * G + (r0 + r) % G) * d + e);
     }
   }
   float o[NT][DB][4][4];                          // O^T: element 64 b + 8 ra + 2 u (+ 1), rows 2 rc (+ 1)
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
       }
     }
   };
-  float* kept = w.kept + ((size_t)blockIdx.z * a.nkv + kvh) * w.keys * w.rows;
+  float* kept = w.kept + ((size_t)blockIdx.z * a.nkv + kvh) * w.keys * w.rows + r0;
   const float scale_log2 = w.cap.in != 0.f ? 1.0f : a.scale * SA_LOG2E;
 
   const int step = 16 * SH_WARPS;
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = j0 + ra + 8 * (e >> 1), r = t * 8 + 2 * rc + (e & 1);
-          bool sees = j < end && r < R && j <= total - n + r / G;
+          bool sees = j < end && r < RB && j <= total - n + (r0 + r) / G;
           if (BY16) sees = sees && at_page >= 0;
           else sees = sees && page_at(j) >= 0;
           if (!sees) s[t][e] = -INFINITY;
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
         top[t][e] = x;
         grow |= x > m[t][e] + SH_GROW;
       }
-      if (t * 8 + 2 * rc < w.rows) {
+      if (t * 8 + 2 * rc < RB) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (j0 + ra + 8 * h < end) *reinterpret_cast<float2*>(kept + (size_t)(j0 + ra + 8 * h) * w.rows + t * 8 + 2 * rc) = make_float2(s[t][2 * h], s[t][2 * h + 1]);
@@ -250,13 +252,13 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
       second_product(p);
     } else {
       // token by token, with the values up to its own key
-      for (int tok = 0; tok < n; ++tok) {
+      for (int tok = r0 / G; tok <= (r0 + RB - 1) / G; ++tok) {
         const int hi_key = total - n + tok;
-        if (tok + 1 < n && hi_key < j0) continue;             // earlier tokens see nothing of this tile
+        if (hi_key < j0) continue;                            // sees nothing of this tile
         uint32_t own[NT][2][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const bool mine = (t * 8 + ra) / G == tok;
+          const bool mine = (r0 + t * 8 + ra) / G == tok;
 #pragma unroll
           for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
   // the warps' sums joined
   const int row_len = d + 2;
   float* so = smem;
-  float* sml = smem + SH_WARPS * w.rows * row_len;
+  float* sml = smem + SH_WARPS * w.block_rows * row_len;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -292,35 +294,35 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
 #pragma unroll
       for (int k = 4; k < 32; k <<= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
       const int r = t * 8 + 2 * rc + e;
-      if (r < w.rows) {
+      if (r < w.block_rows) {
         if (ra == 0) {
-          sml[(warp * w.rows + r) * 2] = m[t][e];
-          sml[(warp * w.rows + r) * 2 + 1] = x;
+          sml[(warp * w.block_rows + r) * 2] = m[t][e];
+          sml[(warp * w.block_rows + r) * 2 + 1] = x;
         }
 #pragma unroll
         for (int b = 0; b < DB; ++b)
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int at = 64 * b + 8 * ra + 2 * u;
-            if (at < d) *reinterpret_cast<float2*>(so + (warp * w.rows + r) * row_len + at) = make_float2(o[t][b][u][e], o[t][b][u][2 + e]);
+            if (at < d) *reinterpret_cast<float2*>(so + (warp * w.block_rows + r) * row_len + at) = make_float2(o[t][b][u][e], o[t][b][u][2 + e]);
           }
       }
     }
   __syncthreads();
-  const size_t part = (((size_t)blockIdx.z * a.nkv + kvh) * w.splits + blockIdx.x) * w.rows;
-  for (int i = threadIdx.x; i < R * (d / 2); i += SH_THREADS) {
+  const size_t part = (((size_t)blockIdx.z * a.nkv + kvh) * w.splits + split) * w.rows + r0;
+  for (int i = threadIdx.x; i < RB * (d / 2); i += SH_THREADS) {
     const int r = i / (d / 2), c = 2 * (i - r * (d / 2));
     float ref = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < SH_WARPS; ++k) ref = fmaxf(ref, sml[(k * w.rows + r) * 2]);
+    for (int k = 0; k < SH_WARPS; ++k) ref = fmaxf(ref, sml[(k * w.block_rows + r) * 2]);
     const float use = ref == -INFINITY ? 0.f : ref;
     float sum = 0.f;
     float2 v = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < SH_WARPS; ++k) {
-      const float f = scored_exp2(sml[(k * w.rows + r) * 2] - use);
-      const float2 x = *reinterpret_cast<const float2*>(so + (k * w.rows + r) * row_len + c);
-      sum = fmaf(f, sml[(k * w.rows + r) * 2 + 1], sum);
+      const float f = scored_exp2(sml[(k * w.block_rows + r) * 2] - use);
+      const float2 x = *reinterpret_cast<const float2*>(so + (k * w.block_rows + r) * row_len + c);
+      sum = fmaf(f, sml[(k * w.block_rows + r) * 2 + 1], sum);
       v.x = fmaf(f, x.x, v.x);
       v.y = fmaf(f, x.y, v.y);
     }
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
 // Blocks [0, key_blocks): weights of `per_block` keys each, the others FIN_THREADS elements of the output each.
 template <typename T>
 __global__ void __launch_bounds__(FIN_THREADS) scored_short_finish_kernel(const ShortArgs w, const int key_blocks, const int per_block) {
-  __shared__ float s_ref[16], s_inv[16], s_lse[16];
+  __shared__ float s_ref[32], s_inv[32], s_lse[32];
   const ScoredArgs& a = w.a;
   pdl_prologue();
   const int seq = w.first_seq + blockIdx.z, kvh = blockIdx.y, G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -404,17 +406,24 @@ int launch_split(const ShortArgs& w, dim3 grid, size_t smem, cudaStream_t stream
 
 }  // namespace
 
+int scored_short_rows(int d) {
+  // a block's 16 rows of heads above 128 would need more registers than a thread has; from 32 rows on (two blocks for the same keys)
+  // the tcgen05 kernels are faster
+  return d <= 128 ? 32 : 8;
+}
+
 bool scored_short_takes(int dtype, int rows, int d) {
-  // 16 rows of heads above 128 would need more registers than a thread has
-  return dtype == NHV_BF16 && d % 8 == 0 && d <= SA_MAX_D && rows <= (d <= 128 ? 16 : 8);
+  return dtype == NHV_BF16 && d % 8 == 0 && d <= SA_MAX_D && rows <= scored_short_rows(d);
 }
 
 ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d) {
   ShortPlan p = {};
   p.rows = (max_rows + 1) / 2 * 2;
+  p.row_blocks = (p.rows + 15) / 16;
+  p.block_rows = (p.rows / p.row_blocks + (p.rows % p.row_blocks ? 1 : 0) + 1) / 2 * 2;
   // Four times as many blocks as run at once (three an SM), so that requests of unlike length even out, and no fewer than 64 keys a
   // block (a tile per warp).
-  const long long keys = (long long)n_seqs * nkv * max_keys, want = (keys + 4 * 444 - 1) / (4 * 444);
+  const long long keys = (long long)n_seqs * nkv * p.row_blocks * max_keys, want = (keys + 4 * 444 - 1) / (4 * 444);
   p.split_keys = (int)((want + 63) / 64 * 64);
   if (p.split_keys < 64) p.split_keys = 64;
   p.splits = (max_keys + p.split_keys - 1) / p.split_keys;
@@ -433,6 +442,8 @@ int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* w
   w.cap = nhv_score_cap(a.scale, a.softcap);
   w.keys = plan.keys;
   w.rows = plan.rows;
+  w.block_rows = plan.block_rows;
+  w.row_blocks = plan.row_blocks;
   w.split_keys = plan.split_keys;
   w.splits = plan.splits;
   const size_t pairs = (size_t)plan.group * a.nkv;
@@ -440,16 +451,16 @@ int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* w
   w.part_o = w.kept + pairs * plan.keys * plan.rows;
   w.part_ml = w.part_o + pairs * plan.splits * plan.rows * a.d;
   const int db = (a.d + 63) / 64;
-  const size_t smem = sizeof(float) * SH_WARPS * plan.rows * (a.d + 4);
+  const size_t smem = sizeof(float) * SH_WARPS * plan.block_rows * (a.d + 4);
   // weights: 256 keys a block, 1,024 where there are blocks enough
   const int per_block = (long long)plan.group * a.nkv * plan.keys > 4 * 1024 * 1024 / 8 ? 1024 : 256;
   const int key_blocks = (a.max_keys + per_block - 1) / per_block, out_blocks = (plan.rows * a.d + FIN_THREADS - 1) / FIN_THREADS;
   for (int s = 0; s < a.n_seqs; s += plan.group) {
     w.first_seq = s;
     const int count = a.n_seqs - s < plan.group ? a.n_seqs - s : plan.group;
-    const dim3 grid(plan.splits, a.nkv, count);
+    const dim3 grid(plan.splits * plan.row_blocks, a.nkv, count);
     int rc = 0;
-    if (plan.rows <= 8)
+    if (plan.block_rows <= 8)
       rc = db == 1 ? launch_split<1, 1>(w, grid, smem, stream) : db == 2 ? launch_split<2, 1>(w, grid, smem, stream)
            : db == 3 ? launch_split<3, 1>(w, grid, smem, stream) : launch_split<4, 1>(w, grid, smem, stream);
     else
