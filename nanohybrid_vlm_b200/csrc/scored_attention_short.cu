@@ -1,15 +1,16 @@
 // Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), up to 32 of
 // them: decoded tokens, drafts.  All the work is to read the keys and values once.
 //
-// First kernel: a block per (part of a request's keys, up to 16 of its rows, KV head, request), its warps independent of one
+// First kernel: a block per (part of a request's keys, up to 24 of its rows, KV head, request), its warps independent of one
 // another; blocks for other rows of the same keys find them in L2.  A warp takes 16
 // keys at a time straight from the pages into registers and forms S^T = K Q^T (m16n8k16, the 16 keys as M, up to 8 rows as N) and
 // O^T += V^T P^T.  No shared memory is between the pages and the products: which element of a head stands at which index of the
 // product is free as long as both operands agree, so a lane takes 16 consecutive bytes of a row and its registers are the fragment
 // as they are.  For V^T two keys' elements have to share a register, which one byte permutation each does.  The next keys'
 // loads are sent as soon as the products have used the registers; the next tile's page is looked up one tile ahead.
-//   P goes into the second product as two bfloat16 parts, the rounded value and what the rounding left (an error of 2^-16 where
-//   one part has 2^-9): the tensor pipe is idle most of the time here.
+//   P goes into the second product as two bfloat16 parts, the rounded value and what the rounding left (an error of 2^-17 where
+//   one part has 2^-9): the tensor pipe is idle most of the time here.  With more than 16 rows it is not, and P has one part, as in the
+//   tcgen05 kernels.
 //   The running maximum moves only when it grows by more than 2^8, so that most tiles leave the sums as they are.
 //   The warps' sums meet in shared memory; the block leaves one partial sum (fp32) and the scores of its keys.
 // Second kernel: the parts' sums are joined, a block per (request, KV head) for the output and blocks of keys for the weights: a
@@ -60,6 +61,7 @@ __device__ __forceinline__ float high_of(uint32_t v) { return __uint_as_float(v 
 // DB: blocks of 64 elements of a head; NT: blocks of 8 rows; BY16: pages hold a multiple of 16 keys.
 template <int DB, int NT, bool BY16>
 __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short_kernel(const ShortArgs w) {
+  constexpr int PARTS = NT <= 2 ? 2 : 1;          // of P
   extern __shared__ float smem[];                 // [warps][rows][d + 2] sums, then [warps][rows][2]
   const ScoredArgs& a = w.a;
   pdl_prologue();
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
       }
     }
   };
-  auto second_product = [&](const uint32_t (&p)[NT][2][2]) {
+  auto second_product = [&](const uint32_t (&p)[NT][PARTS][2]) {
 #pragma unroll
     for (int b = 0; b < DB; ++b) {
       const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vr[0][b]);
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           mma16816(o[t][b][u], a0, a1, a2, a3, p[t][0][0], p[t][0][1]);
-          mma16816(o[t][b][u], a0, a1, a2, a3, p[t][1][0], p[t][1][1]);
+          if (PARTS == 2) mma16816(o[t][b][u], a0, a1, a2, a3, p[t][PARTS - 1][0], p[t][PARTS - 1][1]);
         }
       }
     }
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
           }
         }
     }
-    uint32_t p[NT][2][2];                          // [rounded, what that left][keys 0-7, 8-15]
+    uint32_t p[NT][PARTS][2];                      // [rounded, what that left][keys 0-7, 8-15]
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
         }
         const uint32_t hi = pack2(x[0], x[1]);
         p[t][0][h] = transposed(hi);
-        p[t][1][h] = transposed(pack2(x[0] - low_of(hi), x[1] - high_of(hi)));
+        if (PARTS == 2) p[t][PARTS - 1][h] = transposed(pack2(x[0] - low_of(hi), x[1] - high_of(hi)));
       }
     if (!edge || n == 1) {
       second_product(p);
@@ -255,12 +257,12 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
       for (int tok = r0 / G; tok <= (r0 + RB - 1) / G; ++tok) {
         const int hi_key = total - n + tok;
         if (hi_key < j0) continue;                            // sees nothing of this tile
-        uint32_t own[NT][2][2];
+        uint32_t own[NT][PARTS][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const bool mine = (r0 + t * 8 + ra) / G == tok;
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
+          for (int k = 0; k < PARTS; ++k)
 #pragma unroll
             for (int h = 0; h < 2; ++h) own[t][k][h] = mine ? p[t][k][h] : 0u;
         }
@@ -419,7 +421,7 @@ bool scored_short_takes(int dtype, int rows, int d) {
 ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d) {
   ShortPlan p = {};
   p.rows = (max_rows + 1) / 2 * 2;
-  p.row_blocks = (p.rows + 15) / 16;
+  p.row_blocks = (p.rows + 23) / 24;
   p.block_rows = (p.rows / p.row_blocks + (p.rows % p.row_blocks ? 1 : 0) + 1) / 2 * 2;
   // Four times as many blocks as run at once (three an SM), so that requests of unlike length even out, and no fewer than 64 keys a
   // block (a tile per warp).
@@ -463,8 +465,10 @@ int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* w
     if (plan.block_rows <= 8)
       rc = db == 1 ? launch_split<1, 1>(w, grid, smem, stream) : db == 2 ? launch_split<2, 1>(w, grid, smem, stream)
            : db == 3 ? launch_split<3, 1>(w, grid, smem, stream) : launch_split<4, 1>(w, grid, smem, stream);
-    else
+    else if (plan.block_rows <= 16)
       rc = db == 1 ? launch_split<1, 2>(w, grid, smem, stream) : launch_split<2, 2>(w, grid, smem, stream);
+    else
+      rc = db == 1 ? launch_split<1, 3>(w, grid, smem, stream) : launch_split<2, 3>(w, grid, smem, stream);
     if (rc) return rc;
     NHV_CUDA(nhv_launch(scored_short_finish_kernel<__nv_bfloat16>, dim3(key_blocks + out_blocks, a.nkv, count), FIN_THREADS, 0, stream, w, key_blocks, per_block),
              "scored attention");
