@@ -272,6 +272,21 @@ class CacheManager:
                 freed += len(pages)
         return freed
 
+    def shrink(self, req_id, num_tokens: int) -> int:
+        """The request holds only the slots [0, num_tokens) from now on (keys were dropped and the others moved there): the pages
+        behind them go back.  Returns how many."""
+        if self.prefix_cache or self.has_windows or self.slots is not None:
+            raise ValueError("a request's pages can shrink only where every group keeps all keys, without prefix reuse and without state")
+        req = self._requests[req_id]
+        keep = -(-num_tokens // self.page_size)
+        freed = 0
+        for g, table in enumerate(req.tables):
+            self.pools[g].free(list(reversed(table[keep:])))
+            freed += len(table) - len(table[:keep])
+            del table[keep:]
+        req.num_tokens = min(req.num_tokens, num_tokens)
+        return freed
+
     def free(self, req_id) -> None:
         """The request has ended (or is preempted): everything it holds goes back."""
         req = self._requests.pop(req_id)

@@ -52,14 +52,15 @@ class CacheLayout:
     def needs_state_slots(self) -> bool:
         return any(isinstance(leaf, FixedStateNeed) for n in self.needs for leaf in leaves(n))
 
-    def page_bytes(self, page_size: int, dtype: torch.dtype) -> list[int]:
-        """Bytes that one page id of each group stands for (summed over the group's runs)."""
+    def page_bytes(self, page_size: int, dtype: torch.dtype, scored: bool = False) -> list[int]:
+        """Bytes that one page id of each group stands for (summed over the group's runs); ``scored``: with scores and births."""
         item = torch.empty((), dtype=dtype).element_size()
         out = [0] * len(self.groups)
         for need, groups in zip(self.needs, self.leaf_group):
             for leaf, g in zip(leaves(need), groups):
                 if g is not None:
                     out[g] += leaf.planes * leaf.num_kv_heads * page_size * leaf.row_dim * item
+                    out[g] += 8 * leaf.num_kv_heads * page_size if scored else 0
         return out
 
     def state_bytes_per_slot(self, dtype: torch.dtype) -> int:
@@ -76,8 +77,9 @@ class CacheLayout:
 
 class CacheStorage:
     def __init__(self, layout: CacheLayout, order, page_size: int, num_pages: list[int], num_state_slots: int,
-                 dtype: torch.dtype, device, poison: bool = False):
-        """``poison``: the pools start as NaN instead of zeros, so that a kernel that reads a slot which no step
+                 dtype: torch.dtype, device, poison: bool = False, scored: bool = False):
+        """``scored``: every paged run also keeps its keys' scores and births (8 bytes per token and KV head).
+        ``poison``: the pools start as NaN instead of zeros, so that a kernel that reads a slot which no step
         has written (beyond a request's tokens, or a page of another request) cannot go unnoticed."""
         self.layout = layout
         self.order = list(order)
@@ -88,6 +90,8 @@ class CacheStorage:
         self.leaf_tensors: list[list[tuple]] = []
         self.pages: list[torch.Tensor | None] = []
         self.states: list[torch.Tensor | None] = []
+        self.scores: list[torch.Tensor | None] = []     # per run, of its first paged entry
+        self.births: list[torch.Tensor | None] = []
         for need, groups in zip(layout.needs, layout.leaf_group):
             mine = []
             for leaf, g in zip(leaves(need), groups):
@@ -103,6 +107,10 @@ class CacheStorage:
             self.leaf_tensors.append(mine)
             self.pages.append(next((p for p, _ in mine if p is not None), None))
             self.states.append(next((s for _, s in mine if s is not None), None))
+            paged = self.pages[-1] if scored else None
+            shape = None if paged is None else (paged.shape[0], paged.shape[2], paged.shape[3])
+            self.scores.append(None if paged is None else torch.full(shape, fill, dtype=torch.float32, device=device))
+            self.births.append(None if paged is None else torch.zeros(shape, dtype=torch.int32, device=device))
 
     def view(self, run: int, cache_from: int | None, batch) -> CacheView:
         """What run ``run`` sees: its own pages and states; where it reads the pages of run ``cache_from``, those
@@ -121,10 +129,11 @@ class CacheStorage:
             if isinstance(n, SharedPagesNeed):
                 pages, g = next(lent)
                 return CacheView(pages=pages, tables=batch.groups[g], writes=False)
-            return CacheView(pages=pages, tables=batch.groups[g] if g is not None else None, state=state)
+            return CacheView(pages=pages, tables=batch.groups[g] if g is not None else None, state=state, scores=self.scores[run],
+                             births=self.births[run])
 
         return build(self.layout.needs[run])
 
     def bytes(self) -> int:
         return sum(t.numel() * t.element_size() for mine in self.leaf_tensors for pair in mine for t in pair
-                   if t is not None)
+                   if t is not None) + sum(t.numel() * 4 for t in self.scores + self.births if t is not None)

@@ -33,6 +33,9 @@ def _add_engine_options(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--decode-weight-copy", dest="decode_weight_copy", action="store_true", default=None,
                     help="keep a second copy of the matrices a decode step streams, laid out per SM (default: when it fits)")
     ap.add_argument("--no-decode-weight-copy", dest="decode_weight_copy", action="store_false")
+    ap.add_argument("--cache-budget", type=int, default=0, help="keys a request keeps per layer and KV head, by attention weight (0: all)")
+    ap.add_argument("--cache-first", type=int, default=4, help="with a budget: the first positions stay")
+    ap.add_argument("--cache-recent", type=int, default=-1, help="with a budget: the last positions stay (default: a quarter of it)")
     ap.add_argument("--profile-ranges", action="store_true", help="NVTX ranges around the step and every layer run")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--random-weights", action="store_true",
@@ -51,7 +54,8 @@ def cmd_generate(args) -> int:
               gpu_memory_utilization=args.gpu_memory_utilization, kvcache_block_size=args.kvcache_block_size,
               num_kvcache_blocks=args.num_kvcache_blocks, scheduler_policy=args.scheduler_policy,
               enforce_eager=args.enforce_eager, seed=args.seed, enable_prefix_cache=args.enable_prefix_cache,
-              decode_weight_copy=args.decode_weight_copy, profile_ranges=args.profile_ranges,
+              decode_weight_copy=args.decode_weight_copy, profile_ranges=args.profile_ranges, cache_budget=args.cache_budget,
+              cache_first=args.cache_first, cache_recent=args.cache_recent,
               random_weights_seed=args.seed if args.random_weights else None)
     sp = SamplingParams(temperature=args.temperature, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos,
                         seed=args.sampling_seed)

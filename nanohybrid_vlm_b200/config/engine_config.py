@@ -5,7 +5,7 @@ point fills from keyword arguments (nanovllm/engine/llm_engine.py:179-181).  The
 options that belong to its hybrid (GDN, vision, joint prefix cache) path are absent.
 Options that the reference does not have: ``dtype`` (run the checkpoint in another
 precision; ``"float32"`` is the true 32-bit path), ``seed``, ``decode_weight_copy``,
-``async_decode``, ``profile_ranges`` and ``poison_cache``.
+``async_decode``, ``profile_ranges``, ``poison_cache`` and the three of a bounded cache.
 """
 from __future__ import annotations
 
@@ -41,6 +41,10 @@ class Config:
                                              # one step late and the extra token dropped.  Needs the CUDA graphs.
     profile_ranges: bool = False             # NVTX ranges around the step, every layer run, the final norm and the head,
                                              # for profilers that filter or group by range
+    cache_budget: int = 0                    # keys a request keeps per layer and KV head (0: all): beyond that, and a page more, those
+                                             # that have gathered the least attention weight are dropped; decode steps run without graphs
+    cache_first: int = 4                     # with cache_budget: the keys of the first positions stay whatever they gathered
+    cache_recent: int = -1                   # with cache_budget: and those of the last positions (-1: a quarter of the budget)
     poison_cache: bool = False               # fill the cache pools with NaN at start: a read of a slot that no step
                                              # wrote shows in the logits (tests, replay)
     dtype: str | torch.dtype | None = None   # None: the checkpoint's own
@@ -62,6 +66,15 @@ class Config:
             raise ConfigError("max_num_batched_tokens, max_num_seqs and max_model_len must be positive")
         if not 0.0 < self.gpu_memory_utilization <= 1.0:
             raise ConfigError("gpu_memory_utilization must be in (0, 1]")
+        if self.cache_budget:
+            if self.cache_recent < 0:
+                self.cache_recent = self.cache_budget // 4
+            if self.cache_budget < 0 or self.cache_first < 0 or self.cache_first + self.cache_recent >= self.cache_budget:
+                raise ConfigError("cache_budget must be positive and larger than cache_first and cache_recent together")
+            if self.enable_prefix_cache:
+                raise ConfigError("cache_budget drops keys of a request, whose pages then hold no prefix that others could share")
+            self.enable_prefix_cache = False
+            self.enforce_eager = True
         self.architecture, self.model_config = load_model_config(self.model)
         self.dtype = parse_dtype(self.dtype) if self.dtype is not None else self.model_config.dtype
         if self.dtype not in (torch.bfloat16, torch.float32):

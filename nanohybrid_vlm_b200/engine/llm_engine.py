@@ -95,7 +95,7 @@ class LLMEngine:
         self.scheduler = Scheduler(self.model_runner.cache, max_num_seqs=config.max_num_seqs,
                                    max_num_batched_tokens=config.max_num_batched_tokens,
                                    max_model_len=config.max_model_len, eos=config.eos,
-                                   policy=config.scheduler_policy, max_portion=max_portion)
+                                   policy=config.scheduler_policy, max_portion=max_portion, cache_budget=config.cache_budget)
         self.request_metrics: dict[int, RequestMetrics] = {}
         self.h2d_bytes = 0
         self.d2h_bytes = 0
@@ -199,8 +199,9 @@ class LLMEngine:
         for s in seqs:
             start, n = s.num_cached_tokens, s.num_scheduled_tokens
             last = start + n == len(s)
-            items.append(StepItem(s.seq_id, [0 if t == PENDING else t for t in s.token_ids[start:start + n]], start,
-                                  [n - 1] if last else []))
+            # in a bounded cache the next free slot is not the next position any more
+            items.append(StepItem(s.seq_id, [0 if t == PENDING else t for t in s.token_ids[start:start + n]], s.num_kept_tokens,
+                                  [n - 1] if last else [], list(range(start, start + n)) if s.num_dropped_tokens else None))
             if last:
                 sampled.append(s)
             m = self.request_metrics[s.seq_id]
@@ -219,6 +220,11 @@ class LLMEngine:
             outputs += self._resolve(previous)
         if not self.async_decode:
             outputs += self._drain()                          # every step is read before the next is planned
+        over = self.scheduler.over_budget(seqs)
+        if over:
+            runner.drop_keys([(s.seq_id, s.num_kept_tokens, s.num_cached_tokens) for s in over])
+            for s in over:
+                self.scheduler.dropped(s)
         stats.elapsed = perf_counter() - t0
         return outputs, stats
 

@@ -66,10 +66,15 @@ class ModelRunner:
             num_slots = 0
         elif num_slots < 0:
             num_slots = config.max_num_seqs
+        possible = CacheManager.prefix_cache_possible(self.layout.groups, num_slots)
+        if config.cache_budget:
+            mixers = [self.model.blocks[run.layer].cache_owner for run in spec.order]
+            if not possible or any(run.cache_from is not None or not getattr(m, "scores_keys", False) for run, m in zip(spec.order, mixers)):
+                raise ValueError("cache_budget needs a model whose every layer attends to all keys of its own cache and adds up their "
+                                 "weights (gqa_attention without a window)")
         num_pages = self._size_pools(num_slots)
         config.num_kvcache_blocks, config.num_state_slots = num_pages, num_slots
         counts = [num_pages] * len(self.layout.groups)
-        possible = CacheManager.prefix_cache_possible(self.layout.groups, num_slots)
         if config.enable_prefix_cache and not possible:
             raise ValueError("enable_prefix_cache=True, but this model has layers with a window or with per-request "
                              "state, which shared pages cannot rebuild")
@@ -77,7 +82,7 @@ class ModelRunner:
         self.cache = CacheManager(self.layout.groups, self.page_size, counts, num_slots,
                                   enable_prefix_cache=config.enable_prefix_cache)
         self.storage = CacheStorage(self.layout, spec.order, self.page_size, counts, num_slots, self.dtype, self.device,
-                                    poison=config.poison_cache)
+                                    poison=config.poison_cache, scored=config.cache_budget > 0)
         self.builder = BatchBuilder(self.cache, self.vocab_size, self.device,
                                     max_tokens=config.max_num_batched_tokens, max_seqs=config.max_num_seqs,
                                     max_pages_per_seq=self.max_pages_per_seq, position_axes=spec.position_axes)
@@ -118,11 +123,16 @@ class ModelRunner:
         T = self.config.max_num_batched_tokens
         per_token = (3 * widest + 6 * self.model.spec.hidden_size) * item
         logits = self.config.max_num_seqs * self.vocab_size * (4 + item)
-        return 2 * T * per_token + 2 * logits + (256 << 20) + self.model.scratch_bytes(T, min(T, self.config.max_num_seqs))
+        requests = min(T, self.config.max_num_seqs)
+        scored = 0
+        if self.config.cache_budget:
+            scored = max(self.model.blocks[run.layer].cache_owner.scored_scratch_bytes(T, requests, self.config.max_model_len, self.page_size)
+                         for run in self.model.spec.order)
+        return 2 * T * per_token + 2 * logits + (256 << 20) + self.model.scratch_bytes(T, requests) + scored
 
     def _size_pools(self, num_slots: int) -> int:
         cfg = self.config
-        per_page = sum(self.layout.page_bytes(self.page_size, self.dtype))
+        per_page = sum(self.layout.page_bytes(self.page_size, self.dtype, scored=cfg.cache_budget > 0))
         useful = cfg.max_num_seqs * self.max_pages_per_seq       # more pages than this can never be held
         if cfg.num_kvcache_blocks > 0:
             return cfg.num_kvcache_blocks
@@ -224,6 +234,28 @@ class ModelRunner:
         slot[0][:bucket + 1].copy_(tokens, non_blocking=True)     # tokens and health word, before the next replay overwrites them
         slot[1].record()
         return InFlight(n, bucket, tokens, slot)
+
+    @torch.no_grad()
+    def drop_keys(self, requests: list[tuple]) -> None:
+        """Cut requests down to ``cache_budget`` keys in every layer and KV head: ``requests`` holds (request, slots it fills, position of
+        its next token).  The caller gives the pages behind the budget back (``CacheManager.shrink``)."""
+        cfg = self.config
+        tables = [self.cache.block_table(r) for r, _, _ in requests]
+        width, n = max(len(t) for t in tables), len(requests)
+        host = torch.full((n, width + 3), -1, dtype=torch.int32)
+        for i, (table, (_, kept, seen)) in enumerate(zip(tables, requests)):
+            host[i, :len(table)] = torch.tensor(table, dtype=torch.int32)
+            host[i, width:] = torch.tensor([kept, seen, cfg.cache_budget], dtype=torch.int32)
+        arrays = host.to(self.device)
+        table, (kept, seen, budgets) = arrays[:, :width], arrays[:, width:].t().contiguous()
+        most = max(k for _, k, _ in requests)
+        for pages, scores, births in zip(self.storage.pages, self.storage.scores, self.storage.births):
+            if scores is None:
+                continue
+            sources = torch.empty((n, scores.shape[1], min(cfg.cache_budget, most - cfg.cache_budget)), dtype=torch.int32, device=self.device)
+            targets = torch.empty_like(sources)
+            ops.select_keys(sources, targets, scores, births, table, kept, seen, budgets, n, most, cfg.cache_first, cfg.cache_recent)
+            ops.move_keys(pages, scores, births, table, sources, targets, n)
 
     def _bucket(self, items) -> int | None:
         if not self.graph_buckets or len(items) > self.graph_buckets[-1]:

@@ -42,13 +42,14 @@ class SchedulePlan:
 
 class Scheduler:
     def __init__(self, cache: CacheManager, *, max_num_seqs: int, max_num_batched_tokens: int, max_model_len: int,
-                 eos: int = -1, policy: str = "decode_first", max_portion: int | None = None):
+                 eos: int = -1, policy: str = "decode_first", max_portion: int | None = None, cache_budget: int = 0):
         self.cache = cache
         self.max_num_seqs = max_num_seqs
         self.max_num_batched_tokens = max_num_batched_tokens
         self.max_model_len = max_model_len
         self.eos = eos
         self.policy = policy
+        self.cache_budget = cache_budget        # keys a request keeps (0: all)
         self.max_portion = max_portion          # test hook: no portion of a prompt is longer than this
         self.waiting: deque[Sequence] = deque()
         self.running: deque[Sequence] = deque()
@@ -63,6 +64,8 @@ class Scheduler:
             raise ValueError(f"prompt of {len(seq)} tokens leaves no room to generate within max_model_len "
                              f"{self.max_model_len}")
         most = min(len(seq) + seq.max_tokens - 1, self.max_model_len)   # the last token chosen is never fed back
+        if self.cache_budget:       # the whole prompt, then no more than a page above the budget
+            most = min(most, max(len(seq), self.cache_budget + self.cache.page_size))
         for g, pool in enumerate(self.cache.pools):
             if -(-most // self.cache.page_size) > pool.num_pages:
                 raise ValueError(f"request of up to {most} tokens can never fit the cache "
@@ -117,7 +120,7 @@ class Scheduler:
         for seq in list(self.running):
             if seq.status != SequenceStatus.RUNNING or budget == 0 or len(plan.seqs) >= self.max_num_seqs:
                 continue
-            n = len(seq)
+            n = len(seq) - seq.num_dropped_tokens
             while not (self.cache.covers(seq.seq_id, n) or self.cache.can_allocate(seq.seq_id, n)):
                 victim = self._pick_victim(scheduled, exclude=seq)
                 if victim is None:
@@ -148,11 +151,25 @@ class Scheduler:
         self.num_recomputed_tokens += seq.num_cached_tokens
         seq.num_preemptions += 1
         seq.num_cached_tokens = 0
+        seq.num_dropped_tokens = 0
         seq.num_scheduled_tokens = 0
         seq.status = SequenceStatus.WAITING
         self.running.remove(seq)
         self.waiting.append(seq)
         plan.preempted_seq_ids.append(seq.seq_id)
+
+    # ------------------------------------------------------------------ a bounded cache
+    def over_budget(self, seqs: list[Sequence]) -> list[Sequence]:
+        """Those of the requests that hold a page more than the cache's budget and will go on: their keys are to be dropped."""
+        if not self.cache_budget:
+            return []
+        return [s for s in seqs if s.status == SequenceStatus.RUNNING and not s.finishing
+                and s.num_kept_tokens >= self.cache_budget + self.cache.page_size]
+
+    def dropped(self, seq: Sequence) -> None:
+        """The request's keys have been cut down to the budget."""
+        seq.num_dropped_tokens = seq.num_cached_tokens - self.cache_budget
+        self.cache.shrink(seq.seq_id, self.cache_budget)
 
     # ------------------------------------------------------------------ a step whose tokens are read later
     def advance(self, seqs: list[Sequence]) -> list[int]:

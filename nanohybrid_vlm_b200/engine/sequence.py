@@ -26,6 +26,7 @@ class Sequence:
         self.num_prompt_tokens = len(token_ids)
         self.num_cached_tokens = 0          # tokens whose keys/values (and state) are in the cache
         self.num_scheduled_tokens = 0       # tokens of the step being run
+        self.num_dropped_tokens = 0         # of the cached ones, those whose keys a bounded cache has dropped
         self.temperature = sampling_params.temperature
         self.max_tokens = sampling_params.max_tokens
         self.ignore_eos = sampling_params.ignore_eos
@@ -35,6 +36,11 @@ class Sequence:
 
     def __len__(self) -> int:
         return len(self.token_ids)
+
+    @property
+    def num_kept_tokens(self) -> int:
+        """Slots that its cached tokens take."""
+        return self.num_cached_tokens - self.num_dropped_tokens
 
     @property
     def num_tokens(self) -> int:

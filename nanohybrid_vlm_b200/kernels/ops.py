@@ -1285,6 +1285,14 @@ def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs
     call("nhv_attention_scored", given, work.data_ptr(), kilobytes, stream_ptr())
 
 
+def attention_scored_scratch_bytes(dtype, n_seqs: int, n_tokens: int, min_new: int, max_new: int, max_kv_len: int, nq: int, nkv: int,
+                                   head_dim: int, page_size: int) -> int:
+    """What ``attention_scored`` takes as scratch for a call of these sizes (freed when the call returns to its stream)."""
+    given = _SCORED_CALL.pack(*[0] * 11, BF16 if dtype is torch.bfloat16 else F32, nq * head_dim, nq * head_dim, 0, n_seqs, n_tokens, min_new,
+                              max_new, max_kv_len, nq, nkv, head_dim, page_size, 1, 1.0, 0.0)
+    return 1024 * library.load_library().nhv_attention_scored_kilobytes(given)
+
+
 def select_keys(sources, targets, scores, births, block_table, kv_len, seen, budgets, n_seqs: int, max_kv_len: int, keep_first: int,
                 keep_recent: int) -> None:
     """Which keys leave a cache that is to hold ``budgets[i]`` keys of request i, said as moves that close the gaps.

@@ -63,6 +63,11 @@ class GQAttention(Mixer):
         q_w = self.w_q_norm_weight if self.qk_norm else None
         k_w = self.w_k_norm_weight if self.qk_norm else None
         o = self.new(T, self.q_size)
+        if cache.scores is not None:
+            self.attend_scored(o, qkv, q_w, k_w, table, rotary_dim, batch, cache)
+            y = self.new(T, self.env.hidden_size)
+            ops.linear(y, o, self.w_o_proj_weight)
+            return y
         # a step of single tokens: the decode kernel takes qkv as it is (norm, rotation and store inside it)
         if not ops.attention_decode_fused(o, qkv, cache.pages, cache.tables, batch, self.nq, self.nkv, self.d,
                                           self.scale, self.window or 0, q_w, k_w, table, rotary_dim, self.eps,
@@ -75,6 +80,28 @@ class GQAttention(Mixer):
         y = self.new(T, self.env.hidden_size)
         ops.linear(y, o, self.w_o_proj_weight)
         return y
+
+    scores_keys = True
+
+    def scored_scratch_bytes(self, tokens: int, requests: int, keys: int, page_size: int) -> int:
+        """The most that attention with scored keys takes in a step of up to so many tokens, requests and keys of a request."""
+        longest = min(tokens, keys)
+        return max(ops.attention_scored_scratch_bytes(self.env.dtype, requests, min(tokens, requests), 1, 1, keys, self.nq, self.nkv, self.d, page_size),
+                   ops.attention_scored_scratch_bytes(self.env.dtype, requests, tokens, 1, longest, keys, self.nq, self.nkv, self.d, page_size),
+                   ops.attention_scored_scratch_bytes(self.env.dtype, 1, longest, longest, longest, keys, self.nq, self.nkv, self.d, page_size))
+
+    def attend_scored(self, o, qkv, q_w, k_w, table, rotary_dim, batch, cache):
+        """Attention in a cache that drops keys: the store, then the kernels that add up every key's weight."""
+        q = self.new(qkv.shape[0], self.q_size)
+        ops.qk_norm_rope_store(qkv, q, cache.pages, cache.tables.slot_mapping, batch.positions, q_w, k_w, table, rotary_dim, self.nq,
+                               self.nkv, self.d, self.eps, self.norm_offset)
+        news = batch.host_cu_q
+        least = batch.carried.get("least_new_tokens")
+        if least is None:
+            least = batch.carried["least_new_tokens"] = min(b - a for a, b in zip(news, news[1:]))
+        ops.attention_scored(o, q, cache.pages, cache.scores, cache.tables.block_tables, batch.cu_q, batch.kv_len, batch.n_seqs, least,
+                             batch.max_new_tokens, batch.max_kv_len, self.nq, self.nkv, self.d, self.scale, births=cache.births,
+                             positions=batch.positions)
 
     def attend(self, o, q, batch, cache):
         ops.attention(o, q, cache.pages, cache.tables, batch, self.nq, self.nkv, self.d, self.scale,

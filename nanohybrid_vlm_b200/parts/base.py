@@ -166,12 +166,16 @@ class CacheView:
     ``writes`` False if the run must not store keys and values.
     Fixed state: ``state`` [num_slots, *shape]; the step's slots are ``batch.state_slots``.
     Composite need: ``children``, one view per entry of the need.
+    ``scores``, ``births`` [num_pages, kv_heads, page_size]: in an engine that bounds its cache, the attention weight that each
+    key has gathered and the position it stands for; the mixer keeps both (``Mixer.scores_keys``).
     """
     pages: torch.Tensor | None = None
     tables: Any = None
     writes: bool = True
     state: torch.Tensor | None = None
     children: tuple = ()
+    scores: torch.Tensor | None = None
+    births: torch.Tensor | None = None
 
 
 @dataclass
@@ -209,6 +213,9 @@ class Mixer(Part):
         pass an RMS norm over the model width with that weight (eps: ``self.side_eps``).  A block that norms the mixer's
         output anyway does these norms in the same kernel.  Default: the terms of ``forward_terms``, no norms."""
         return tuple((t, c, None) for t, c in self.forward_terms(x, batch, cache))
+
+    # True: where the run's view has scores, the mixer adds up its keys' attention weights there, so that the engine may drop keys
+    scores_keys = False
 
     def cache_need(self) -> "PagedKVNeed | FixedStateNeed | CompositeNeed | None":
         return None
