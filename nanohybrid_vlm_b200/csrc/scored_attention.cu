@@ -380,22 +380,47 @@ __global__ void __launch_bounds__(256) scored_join_rows_kernel(const ScoredArgs 
   const size_t rows = (size_t)a.nkv * a.n_tokens * G, row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int kvh = (int)(row / ((size_t)a.n_tokens * G)), r = (int)(row - (size_t)kvh * a.n_tokens * G), token = r / G, head = kvh * G + r % G;
-  int seq = 0;
-  while (seq + 1 < a.n_seqs && a.cu_q[seq + 1] <= token) ++seq;
+  int seq = 0;                            // how many requests end at or before the token
+  for (int s = 0; s < a.n_seqs; s += 32) seq += __popc(__ballot_sync(0xffffffffu, s + lane < a.n_seqs && a.cu_q[s + lane + 1] <= token));
+  if (seq >= a.n_seqs) return;
   if (!scored_takes(a, a.cu_q[seq + 1] - a.cu_q[seq])) return;
+  // a lane per part: its sum's reference and factor
   const float sink = a.sinks ? a.sinks[head] * SA_LOG2E : -INFINITY;
-  float ref = sink;
-  for (int s = 0; s < p.splits; ++s) ref = fmaxf(ref, p.ml[(s * rows + row) * 2]);
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < p.splits) ml = *reinterpret_cast<const float2*>(p.ml + (lane * rows + row) * 2);
+  float ref = fmaxf(sink, warp_max(ml.x));
   if (ref == -INFINITY) ref = 0.f;
-  float sum = scored_exp2(sink - ref);
-  for (int s = 0; s < p.splits; ++s) sum = fmaf(p.ml[(s * rows + row) * 2 + 1], scored_exp2(p.ml[(s * rows + row) * 2] - ref), sum);
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const float f = scored_exp2(ml.x - ref), sum = warp_sum(f * ml.y) + scored_exp2(sink - ref), inv = sum == 0.f ? 0.f : 1.0f / sum;
   T* dst = (T*)a.out + (size_t)token * a.out_stride + (size_t)head * a.d;
-  for (int c = lane; c < a.d; c += 32) {
-    float v = 0.f;
+  if (a.d % 4 == 0) {
+    for (int c0 = 0; c0 < a.d; c0 += 128) {
+      const int c = c0 + 4 * lane;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) v = fmaf(scored_exp2(p.ml[(s * rows + row) * 2] - ref), p.o[(s * rows + row) * a.d + c], v);
-    dst[c] = from_f32<T>(v * inv);
+      for (int s = 0; s < p.splits; ++s) {
+        const float fs = __shfl_sync(0xffffffffu, f, s);
+        if (c < a.d) {
+          const float4 x = *reinterpret_cast<const float4*>(p.o + (s * rows + row) * a.d + c);
+          v.x = fmaf(fs, x.x, v.x); v.y = fmaf(fs, x.y, v.y); v.z = fmaf(fs, x.z, v.z); v.w = fmaf(fs, x.w, v.w);
+        }
+      }
+      if (c < a.d) {
+        dst[c] = from_f32<T>(v.x * inv);
+        dst[c + 1] = from_f32<T>(v.y * inv);
+        dst[c + 2] = from_f32<T>(v.z * inv);
+        dst[c + 3] = from_f32<T>(v.w * inv);
+      }
+    }
+  } else {
+    for (int c0 = 0; c0 < a.d; c0 += 32) {
+      const int c = c0 + lane;
+      float v = 0.f;
+      for (int s = 0; s < p.splits; ++s) {
+        const float fs = __shfl_sync(0xffffffffu, f, s);
+        if (c < a.d) v = fmaf(fs, p.o[(s * rows + row) * a.d + c], v);
+      }
+      if (c < a.d) dst[c] = from_f32<T>(v * inv);
+    }
   }
   if (lane == 0) a.lse[row] = sum == 0.f ? INFINITY : ref + log2f(sum);
 }
@@ -406,13 +431,13 @@ __global__ void __launch_bounds__(256) scored_join_keys_kernel(const ScoredArgs 
   const int seq = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
   const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
   if (key >= total || !scored_takes(a, n)) return;
+  // the chunks from the first that sees the key's tile to the last that has rows
+  const int G = a.nq / a.nkv, t = key / p.tile_keys * p.tile_keys - (total - n), first_tile = t > 0 ? t * G / p.tile_rows : 0;
+  const int tiles = (n * G + p.tile_rows - 1) / p.tile_rows, end = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
+  const float* w = p.w + ((size_t)seq * a.nkv + kvh) * p.chunks * p.keys + key;
   float sum = 0.f;
-#pragma unroll 4
-  for (int c = 0; c < p.chunks; ++c) {
-    int begin, end;
-    chunk_range(p, n, a.nq / a.nkv, total, key / p.tile_keys * p.tile_keys, c, begin, end);
-    if (begin < end) sum += p.w[(((size_t)seq * a.nkv + kvh) * p.chunks + c) * p.keys + key];
-  }
+#pragma unroll 8
+  for (int c = first_tile / p.chunk_tiles; c < end; ++c) sum += w[c * p.keys];
   store_weight(a, seq, first, kvh, key, key - (total - n), sum);
 }
 
@@ -461,7 +486,7 @@ size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int m
   int splits = 1;
   double best = 1e30;
   const double sums = row_tile * d * 8 / 30.0 / (tile_cycles * tiles);
-  for (int s = 1; s <= 64 && (s == 1 || tiles / s >= least); ++s) {
+  for (int s = 1; s <= 32 && (s == 1 || tiles / s >= least); ++s) {
     const double waves = alike || blocks * s <= rows_at_once ? (double)((blocks * s + rows_at_once - 1) / rows_at_once) : (double)blocks * s / rows_at_once + 0.5;
     const double cost = waves / s + (s > 1 ? s * sums : 0.0);
     if (cost < best - 1e-9) {
@@ -471,11 +496,12 @@ size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int m
   }
   p.split_tiles = (tiles + splits - 1) / splits;
   p.splits = (tiles + p.split_tiles - 1) / p.split_tiles;
-  // the keys' pass: chunks of rows so that a few blocks come to each place that runs at once
+  // the keys' pass: chunks of rows so that two blocks come to each place that runs at once, of eight tiles at least (eight blocks and four
+  // tiles: 100 against 90 us for a prompt of 2,048 tokens)
   const long long row_tiles = ((long long)max_new * G + p.tile_rows - 1) / p.tile_rows, key_tiles = (max_keys + p.tile_keys - 1) / p.tile_keys;
   const long long pairs = ((long long)n_tokens * G / p.tile_rows + n_seqs) * key_tiles * nkv;
-  long long chunk = pairs / (keys_at_once * 8LL);
-  if (chunk < 4) chunk = 4;
+  long long chunk = pairs / (keys_at_once * 2LL);
+  if (chunk < 8) chunk = 8;
   if (chunk > row_tiles) chunk = row_tiles < 1 ? 1 : row_tiles;
   p.chunk_tiles = (int)chunk;
   p.chunks = (int)((row_tiles + chunk - 1) / chunk);

@@ -23,7 +23,7 @@
 
 namespace {
 
-constexpr int SH_WARPS = 4, SH_THREADS = SH_WARPS * 32, FIN_THREADS = 256;
+constexpr int SH_WARPS = 4, SH_THREADS = SH_WARPS * 32, FIN_THREADS = 256, FIN_KEYS = 4;
 constexpr float SH_GROW = 8.0f;                  // log2 units
 constexpr size_t SH_MOST_SCORES = (size_t)1 << 28;        // floats of scores kept at once (1 GiB)
 
@@ -380,16 +380,60 @@ __global__ void __launch_bounds__(FIN_THREADS) scored_short_finish_kernel(const 
     return;
   }
   const float* kept = w.kept + ((size_t)blockIdx.z * a.nkv + kvh) * w.keys * w.rows;
-  const int end = min(total, (int)(blockIdx.x + 1) * per_block);
-#pragma unroll 4
-  for (int j = blockIdx.x * per_block + threadIdx.x; j < end; j += FIN_THREADS) {
-    float sum = 0.f;
-    for (int r = 0; r < R; r += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(kept + (size_t)j * w.rows + r);
-      sum += scored_exp2(x.x - s_lse[r]);
-      if (r + 1 < R) sum += scored_exp2(x.y - s_lse[r + 1]);
+  const int end = min(total, (int)(blockIdx.x + 1) * per_block), old = total - n, j0 = blockIdx.x * per_block + threadIdx.x;
+  // four keys a thread: their pages, their old scores and the rows' scores are asked for together
+  int page[FIN_KEYS];
+  size_t at[FIN_KEYS];
+  float sum[FIN_KEYS];
+#pragma unroll
+  for (int k = 0; k < FIN_KEYS; ++k) {
+    const int j = j0 + k * FIN_THREADS;
+    page[k] = j < end ? a.block_table[(size_t)seq * a.bt_stride + j / a.page_size] : -1;
+    sum[k] = 0.f;
+  }
+  if (w.rows % 4 == 0) {
+#pragma unroll 2
+    for (int r = 0; r < R; r += 4) {
+      float4 x[FIN_KEYS];
+#pragma unroll
+      for (int k = 0; k < FIN_KEYS; ++k) x[k] = *reinterpret_cast<const float4*>(kept + (size_t)min(j0 + k * FIN_THREADS, end - 1) * w.rows + r);
+#pragma unroll
+      for (int k = 0; k < FIN_KEYS; ++k) {
+        sum[k] += scored_exp2(x[k].x - s_lse[r]);
+        if (r + 1 < R) sum[k] += scored_exp2(x[k].y - s_lse[r + 1]);
+        if (r + 2 < R) sum[k] += scored_exp2(x[k].z - s_lse[r + 2]);
+        if (r + 3 < R) sum[k] += scored_exp2(x[k].w - s_lse[r + 3]);
+      }
     }
-    store_weight(a, seq, first, kvh, j, j - (total - n), sum);
+  } else {
+#pragma unroll 2
+    for (int r = 0; r < R; r += 2) {
+      float2 x[FIN_KEYS];
+#pragma unroll
+      for (int k = 0; k < FIN_KEYS; ++k) x[k] = *reinterpret_cast<const float2*>(kept + (size_t)min(j0 + k * FIN_THREADS, end - 1) * w.rows + r);
+#pragma unroll
+      for (int k = 0; k < FIN_KEYS; ++k) {
+        sum[k] += scored_exp2(x[k].x - s_lse[r]);
+        if (r + 1 < R) sum[k] += scored_exp2(x[k].y - s_lse[r + 1]);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < FIN_KEYS; ++k) {
+    const int j = j0 + k * FIN_THREADS;
+    at[k] = 0;
+    if (page[k] >= a.n_pages) page[k] = -1;
+    if (page[k] >= 0) {
+      at[k] = ((size_t)page[k] * a.nkv + kvh) * a.page_size + j % a.page_size;
+      if (j < old) sum[k] += a.scores[at[k]];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < FIN_KEYS; ++k) {
+    const int j = j0 + k * FIN_THREADS;
+    if (page[k] < 0) continue;
+    a.scores_out[at[k]] = sum[k];
+    if (j >= old && a.births) a.births[at[k]] = a.positions[first + j - old];
   }
 }
 
@@ -454,8 +498,7 @@ int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* w
   w.part_ml = w.part_o + pairs * plan.splits * plan.rows * a.d;
   const int db = (a.d + 63) / 64;
   const size_t smem = sizeof(float) * SH_WARPS * plan.block_rows * (a.d + 4);
-  // weights: 256 keys a block, 1,024 where there are blocks enough
-  const int per_block = (long long)plan.group * a.nkv * plan.keys > 4 * 1024 * 1024 / 8 ? 1024 : 256;
+  const int per_block = FIN_KEYS * FIN_THREADS;
   const int key_blocks = (a.max_keys + per_block - 1) / per_block, out_blocks = (plan.rows * a.d + FIN_THREADS - 1) / FIN_THREADS;
   for (int s = 0; s < a.n_seqs; s += plan.group) {
     w.first_seq = s;

@@ -182,14 +182,34 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t v, bool& bad) {
   bad |= lo | hi;
   return (lo ? 0u : v & 0xffffu) | (hi ? 0u : v & 0xffff0000u);
 }
-// 32 scores capped (see nhv_cap_tile).
+// 32 scores capped (see nhv_cap_tile): where a warp's are all small, two at a time by the polynomial.
 __device__ __forceinline__ void cap32(uint32_t (&sr)[32], const NhvScoreCap& c) {
-  float s[8][4];
+  float m0 = 0.f, m1 = 0.f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) s[i >> 2][i & 3] = __uint_as_float(sr[i]);
-  nhv_cap_tile(s, c);
+  for (int i = 0; i < 32; i += 4) {
+    m0 = max3(m0, fabsf(__uint_as_float(sr[i])), fabsf(__uint_as_float(sr[i + 1])));
+    m1 = max3(m1, fabsf(__uint_as_float(sr[i + 2])), fabsf(__uint_as_float(sr[i + 3])));
+  }
+  if (__all_sync(0xffffffffu, fmaxf(m0, m1) <= c.small)) {
+    const f32x2 z2 = f2_pack(c.z, c.z), k0 = f2_pack(c.c[0], c.c[0]), k1 = f2_pack(c.c[1], c.c[1]), k2 = f2_pack(c.c[2], c.c[2]),
+                k3 = f2_pack(c.c[3], c.c[3]), k4 = f2_pack(c.c[4], c.c[4]);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) sr[i] = __float_as_uint(s[i >> 2][i & 3]);
+    for (int i = 0; i < 32; i += 2) {
+      const f32x2 z = f2_mul(f2_pack(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), z2), t = f2_mul(z, z);
+      float x, y;
+      f2_unpack(f2_mul(z, f2_fma(f2_fma(f2_fma(f2_fma(k4, t, k3), t, k2), t, k1), t, k0)), x, y);
+      sr[i] = __float_as_uint(x);
+      sr[i + 1] = __float_as_uint(y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float x = __uint_as_float(sr[i]), y = __uint_as_float(sr[i + 1]);
+      nhv_cap_scores(x, y, c);
+      sr[i] = __float_as_uint(x);
+      sr[i + 1] = __float_as_uint(y);
+    }
+  }
 }
 
 // What few tiles need, out of the way of what all need: scores capped and masked where they lie in tensor memory (32 columns at a
@@ -544,11 +564,15 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
       if (!ok) break;
       tc_fence_after();
       const bool masked = key0 + BN - 1 > all_hi || missing;           // some row does not see some key of the tile
-      if (CAP || masked) change_scores<BN>(s_addr, p.cap, masked, missing, key0, row_hi, total, table, a.page_size, a.n_pages);
+      if (masked) change_scores<BN>(s_addr, p.cap, masked, missing, key0, row_hi, total, table, a.page_size, a.n_pages);
       uint32_t sr[BN / 32][32];
 #pragma unroll
       for (int c = 0; c < BN / 32; ++c) tmem_ld32_nowait(sr[c], s_addr + c * 32);
       tmem_ld_wait();
+      if (CAP && !masked) {
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) cap32(sr[c], p.cap);
+      }
       float mx0 = max3(__uint_as_float(sr[0][0]), __uint_as_float(sr[0][1]), __uint_as_float(sr[0][2]));
       float mx1 = max3(__uint_as_float(sr[0][3]), __uint_as_float(sr[0][4]), __uint_as_float(sr[0][5]));
 #pragma unroll
@@ -688,6 +712,23 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
 
   const ScoredArgs& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  // Blocks without work (requests of unlike length, chunks that see nothing of a tile) leave before they take tensor memory.  The others
+  // have taken theirs when they let the next kernel in, so that none of this kernel's blocks can wait for what that one holds.
+  pdl_wait();
+  const int G = a.nq / a.nkv, kvh = blockIdx.x, seq = blockIdx.z;
+  const int chunk = blockIdx.y / p.key_tiles, key0 = (blockIdx.y - chunk * p.key_tiles) * BM;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
+  if (key0 >= total || !scored_takes(a, n)) return;
+  int begin = 0, end = 0;
+  chunk_range(p.parts, n, G, total, key0, chunk, begin, end);
+  if (begin >= end && p.parts.chunks > 1) return;
+  // Rows of a stage behind a tile's last (groups that do not divide 128) are never copied to: zeros, whose weights the log-sum of +inf
+  // makes none.
+  for (int i = threadIdx.x; i < (BM - p.tokens * G) * 8 * DB * STAGES; i += C::THREADS) {
+    const int block = i / ((BM - p.tokens * G) * 8), at = i - block * ((BM - p.tokens * G) * 8);
+    *reinterpret_cast<uint4*>(q_s + block * (BM * 128) + p.tokens * G * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_async_smem();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -704,18 +745,11 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
     asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&p.q_map) : "memory");
   }
   if (warp == 1) tmem_alloc(tmem_slot, C::TMEM_COLS);
-  pdl_prologue();
-
-  const int G = a.nq / a.nkv, kvh = blockIdx.x, seq = blockIdx.z;
-  const int chunk = blockIdx.y / p.key_tiles, key0 = (blockIdx.y - chunk * p.key_tiles) * BM;
-  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
-  int begin = 0, end = 0;
-  const bool mine = key0 < total && scored_takes(a, n);
-  if (mine) chunk_range(p.parts, n, G, total, key0, chunk, begin, end);
   const int n_tiles = __shfl_sync(0xffffffffu, max(0, end - begin), 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_launch_dependents();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == 0) {
@@ -765,7 +799,7 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
       if (!ok) *s_abort = 1;
     }
     __syncwarp();
-  } else if (mine) {
+  } else {
     // ------------------------------------------------------------------ two threads per key, for half of the columns each
     const int quarter = warp & 3, half = (warp - 2) >> 2, at = quarter * 32 + lane, key = key0 + at;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
@@ -799,7 +833,7 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
         cap32(s[1], p.cap);
       }
       // rows behind the request's last and those that do not see every key of the tile
-      const bool masked = key0 + BM - 1 > total - n + t_first || (begin + i + 1) * tile_rows > rows || tile_rows < C::BN;
+      const bool masked = key0 + BM - 1 > total - n + t_first || (begin + i + 1) * tile_rows > rows;
       const float4* ls = reinterpret_cast<const float4*>(s_lse + buf * 128 + half * 64);
       f32x2 w[4] = {0ull, 0ull, 0ull, 0ull};
       if (!masked) {
