@@ -99,7 +99,7 @@ struct ShortPlan {
   size_t floats;            // of scratch
 };
 // The most rows of a request that goes this way, and whether requests of up to `rows` rows can.
-int scored_short_rows(int d);
+int scored_short_rows(int dtype, int d);
 bool scored_short_takes(int dtype, int rows, int d);
 ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d);
 // The requests with a.min_rows to a.max_rows rows: output, scores and births.  `work`: plan.floats floats.

@@ -8,7 +8,7 @@
 // the tensor-core kernels of scored_attention_short.cu and scored_attention_tcgen05.cu refuse).
 //   rows: 256 threads hold 16 RPT rows (row = token * G + head, of one request and KV head) and walk the keys in tiles of 64 through
 //     shared memory.  A thread makes RPT x 4 scores from 16-byte reads along the head and RPT x 4 DB outputs, two multiply-adds
-//     an instruction; P passes through shared memory.  RPT is 8 (4 for heads above 128), and 1 where no request has more than 16 rows.
+//     an instruction; P passes through shared memory.  RPT is 8 (4 for heads above 128).
 //     A tile's values arrive while its scores are made, the next tile's keys while the values are used.
 //   keys: 64 keys stay in shared memory, the tiles of rows pass by; a thread adds up the weights of its 4 keys, the sixteen row groups
 //     meet in shared memory at the end.
@@ -460,13 +460,10 @@ int launch_tiles(const TileArgs& t, cudaStream_t stream) {
 }
 
 // Rows of a thread of the tiles' sixteen row groups.
-int rows_per_thread(int dtype, int max_new, int G, int d) {
-  // bfloat16 has kernels of its own for few rows
-  return dtype == NHV_F32 && (long long)max_new * G <= 16 ? 1 : d <= 128 ? 8 : 4;
-}
+int rows_per_thread(int d) { return d <= 128 ? 8 : 4; }
 
-size_t tile_parts(ScoredParts& p, int dtype, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
-  p.tile_rows = 16 * rows_per_thread(dtype, max_new, nq / nkv, d);
+size_t tile_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
+  p.tile_rows = 16 * rows_per_thread(d);
   p.tile_keys = SA_KEYS;
   return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, p.tile_rows, SA_KEYS, p.tile_rows * SA_KEYS * d / 50.0, 148, 148);
 }
@@ -546,9 +543,9 @@ struct ScoredPlan {
 static ScoredPlan scored_plan(int dtype, bool wide, int n_seqs, int n_tokens, int min_new, int max_new, int max_keys, int nq, int nkv, int d,
                               int page_size, float scale) {
   ScoredPlan p = {};
-  p.wide = wide && d % 8 == 0;
+  p.wide = wide && d % (dtype == NHV_F32 ? 4 : 8) == 0;
   p.short_rows = -1;
-  const int G = nq / nkv, most = scored_short_rows(d);
+  const int G = nq / nkv, most = scored_short_rows(dtype, d);
   size_t few = 0, rest = 0;
   if (p.wide && min_new <= most && scored_short_takes(dtype, min_new * G, d)) {
     p.short_rows = most;
@@ -560,7 +557,7 @@ static ScoredPlan scored_plan(int dtype, bool wide, int n_seqs, int n_tokens, in
   if (p.rest) {
     p.many = p.wide && scored_long_takes(dtype, nq, nkv, d, page_size, scale);
     rest = p.many ? scored_long_plan(p.parts, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d)
-                  : tile_parts(p.parts, dtype, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d);
+                  : tile_parts(p.parts, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d);
   }
   p.floats = ((size_t)n_tokens * nq + 3) / 4 * 4 + (few > rest ? few : rest);       // one after the other in the same scratch
   return p;
@@ -630,7 +627,5 @@ NHV_API int nhv_attention_scored(const NhvScoredCall* c, float* work, int work_k
   const int db = d <= 64 ? 1 : d <= 128 ? 2 : 4;
   if (dtype == NHV_BF16)
     return db == 1 ? launch_tiles<__nv_bfloat16, 1, 8>(t, stream) : db == 2 ? launch_tiles<__nv_bfloat16, 2, 8>(t, stream) : launch_tiles<__nv_bfloat16, 4, 4>(t, stream);
-  if (rows_per_thread(dtype, max_new, nq / nkv, d) == 1)
-    return db == 1 ? launch_tiles<float, 1, 1>(t, stream) : db == 2 ? launch_tiles<float, 2, 1>(t, stream) : launch_tiles<float, 4, 1>(t, stream);
   return db == 1 ? launch_tiles<float, 1, 8>(t, stream) : db == 2 ? launch_tiles<float, 2, 8>(t, stream) : launch_tiles<float, 4, 4>(t, stream);
 }

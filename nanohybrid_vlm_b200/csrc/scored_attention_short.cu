@@ -58,6 +58,29 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float low_of(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high_of(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// The sums of a block's warps (in shared memory, rows of `row_len`) joined and written as the block's part.
+__device__ __forceinline__ void join_warps(const ShortArgs& w, const float* so, const float* sml, int row_len, size_t part, int rows, int d) {
+  for (int i = threadIdx.x; i < rows * (d / 2); i += SH_THREADS) {
+    const int r = i / (d / 2), c = 2 * (i - r * (d / 2));
+    float ref = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < SH_WARPS; ++k) ref = fmaxf(ref, sml[(k * w.block_rows + r) * 2]);
+    const float use = ref == -INFINITY ? 0.f : ref;
+    float sum = 0.f;
+    float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < SH_WARPS; ++k) {
+      const float f = scored_exp2(sml[(k * w.block_rows + r) * 2] - use);
+      const float2 x = *reinterpret_cast<const float2*>(so + (k * w.block_rows + r) * row_len + c);
+      sum = fmaf(f, sml[(k * w.block_rows + r) * 2 + 1], sum);
+      v.x = fmaf(f, x.x, v.x);
+      v.y = fmaf(f, x.y, v.y);
+    }
+    *reinterpret_cast<float2*>(w.part_o + (part + r) * d + c) = v;
+    if (c == 0) *reinterpret_cast<float2*>(w.part_ml + (part + r) * 2) = make_float2(ref, sum);
+  }
+}
+
 // DB: blocks of 64 elements of a head; NT: blocks of 8 rows; BY16: pages hold a multiple of 16 keys.
 template <int DB, int NT, bool BY16>
 __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short_kernel(const ShortArgs w) {
@@ -311,26 +334,209 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
       }
     }
   __syncthreads();
-  const size_t part = (((size_t)blockIdx.z * a.nkv + kvh) * w.splits + split) * w.rows + r0;
-  for (int i = threadIdx.x; i < RB * (d / 2); i += SH_THREADS) {
-    const int r = i / (d / 2), c = 2 * (i - r * (d / 2));
-    float ref = -INFINITY;
+  join_warps(w, so, sml, row_len, (((size_t)blockIdx.z * a.nkv + kvh) * w.splits + split) * w.rows + r0, RB, d);
+}
+
+// The same for float32, on the CUDA cores.  LPK lanes share a key, 4 EV / 4 elements each: a key's row is read in one piece, and
+// what a row of the product needs of q and O stands in registers.  A warp takes U x 32 / LPK keys at a time; the lanes' parts of the U x RB
+// scores are added by halves (a lane keeps half of its numbers and sends the other half), which costs about one shuffle a score and
+// leaves each score in one lane, where its exponential is taken once.  P goes back to all lanes by a shuffle.
+template <int LPK, int EV, int RB, bool BY_PAGE>
+__global__ void __launch_bounds__(SH_THREADS, EV == 8 ? 2 : 3) scored_short_f32_kernel(const ShortArgs w) {
+  extern __shared__ float smem[];                 // [warps][rows][d + 2] sums, then [warps][rows][2]
+  constexpr int U = RB * EV >= 32 ? 4 : 8, KPI = 32 / LPK, BATCH = U * KPI, N = U * RB;
+  constexpr int P = N > LPK ? N / LPK : 1, DUP = LPK > N ? LPK / N : 1;       // scores of a lane; lanes that hold the same one
+  const ScoredArgs& a = w.a;
+  pdl_prologue();
+  const int seq = w.first_seq + blockIdx.z, kvh = blockIdx.y, G = a.nq / a.nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), R = n * G, d = a.d;
+  const int split = blockIdx.x / w.row_blocks, r0 = (blockIdx.x - split * w.row_blocks) * w.block_rows, rows = min(R - r0, w.block_rows);
+  const int begin = split * w.split_keys, end = min(total, begin + w.split_keys);
+  if (begin >= end || rows <= 0 || !scored_takes(a, n)) return;
+  const int kk = lane / LPK, in_key = lane % LPK;
+  const float* q = (const float*)a.q;
+  const float* pages = (const float*)a.pages;
+  const int* table = a.block_table + (size_t)seq * a.bt_stride;
+  const size_t v_plane = (size_t)a.nkv * a.page_size * d;
+  // elements 4 in_key .. of every block of 4 LPK
+  float qf[RB][EV], o[RB][EV], m[RB];
 #pragma unroll
-    for (int k = 0; k < SH_WARPS; ++k) ref = fmaxf(ref, sml[(k * w.block_rows + r) * 2]);
-    const float use = ref == -INFINITY ? 0.f : ref;
-    float sum = 0.f;
-    float2 v = make_float2(0.f, 0.f);
+  for (int r = 0; r < RB; ++r) {
+    m[r] = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < SH_WARPS; ++k) {
-      const float f = scored_exp2(sml[(k * w.block_rows + r) * 2] - use);
-      const float2 x = *reinterpret_cast<const float2*>(so + (k * w.block_rows + r) * row_len + c);
-      sum = fmaf(f, sml[(k * w.block_rows + r) * 2 + 1], sum);
-      v.x = fmaf(f, x.x, v.x);
-      v.y = fmaf(f, x.y, v.y);
+    for (int e = 0; e < EV; e += 4) {
+      const int at = e * LPK + 4 * in_key;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < rows && at < d) x = *reinterpret_cast<const float4*>(q + (size_t)(first + (r0 + r) / G) * a.q_stride + (size_t)(kvh * G + (r0 + r) % G) * d + at);
+      qf[r][e] = x.x; qf[r][e + 1] = x.y; qf[r][e + 2] = x.z; qf[r][e + 3] = x.w;
+      o[r][e] = o[r][e + 1] = o[r][e + 2] = o[r][e + 3] = 0.f;
     }
-    *reinterpret_cast<float2*>(w.part_o + (part + r) * d + c) = v;
-    if (c == 0) *reinterpret_cast<float2*>(w.part_ml + (part + r) * 2) = make_float2(ref, sum);
   }
+  float l[P], x[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) l[i] = 0.f;
+  float4 kr[U][EV / 4], vr[U][EV / 4];
+  auto row_at = [&](int j, int j0) -> const float* {
+    if (j >= end) return nullptr;
+    const int jp = BY_PAGE ? j0 : j, at = jp / a.page_size, page = table[at];
+    if (page < 0 || page >= a.n_pages) return nullptr;
+    return pages + (((size_t)page * 2 * a.nkv + kvh) * a.page_size + (j - at * a.page_size)) * d;
+  };
+  auto load = [&](float4 (&dst)[U][EV / 4], int j0, size_t plane) -> uint32_t {       // a bit for every u whose key is there
+    uint32_t there = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float* row = row_at(j0 + u * KPI + kk, j0);
+      there |= row ? 1u << u : 0u;
+#pragma unroll
+      for (int e = 0; e < EV / 4; ++e) {
+        const int at = e * 4 * LPK + 4 * in_key;
+        dst[u][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row && at < d) {
+          const uint4 v = load16(row + plane + at);
+          dst[u][e] = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+        }
+      }
+    }
+    return there;
+  };
+  float* kept = w.kept + ((size_t)blockIdx.z * a.nkv + kvh) * w.keys * w.rows + r0;
+  // the lane's scores: number i of the batch's U x RB is key i / RB, row i % RB
+  const int i0 = in_key / DUP * P;
+  const bool first_copy = in_key % DUP == 0;
+  const int step = BATCH * SH_WARPS;
+  int j0 = begin + BATCH * warp;
+  uint32_t there = 0;
+  if (j0 < end) {
+    there = load(kr, j0, 0);
+    load(vr, j0, v_plane);
+  }
+  for (; j0 < end; j0 += step) {
+    float s[N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        float t = 0.f;
+#pragma unroll
+        for (int e = 0; e < EV / 4; ++e) {
+          t = fmaf(qf[r][4 * e], kr[u][e].x, t);
+          t = fmaf(qf[r][4 * e + 1], kr[u][e].y, t);
+          t = fmaf(qf[r][4 * e + 2], kr[u][e].z, t);
+          t = fmaf(qf[r][4 * e + 3], kr[u][e].w, t);
+        }
+        s[u * RB + r] = t;
+      }
+    const uint32_t there_next = load(kr, j0 + step, 0);
+    int count = N;
+#pragma unroll
+    for (int bit = LPK / 2; bit > 0; bit >>= 1) {
+      if (count > 1) {
+        count >>= 1;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+          if (i < count) {
+            const bool upper = lane & bit;
+            const float mine = upper ? s[i + count] : s[i], other = upper ? s[i] : s[i + count];
+            s[i] = mine + __shfl_xor_sync(0xffffffffu, other, bit);
+          }
+      } else {
+        s[0] += __shfl_xor_sync(0xffffffffu, s[0], bit);
+      }
+    }
+    const bool edge = j0 + BATCH - 1 > total - n;
+    bool grow = false;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int r = (i0 + i) % RB, j = j0 + (i0 + i) / RB * KPI + kk;
+      float t = s[i] * a.scale;
+      if (a.softcap > 0.f) t = a.softcap * tanhf(t / a.softcap);
+      t *= SA_LOG2E;
+      bool sees = (there >> (i0 + i) / RB & 1u) && r < rows;
+      if (edge) sees = sees && j <= total - n + (r0 + r) / G;
+      x[i] = sees ? t : -INFINITY;
+      if (first_copy && j < end && r < rows) kept[(size_t)j * w.rows + r] = x[i];
+      float ref = m[0];
+#pragma unroll
+      for (int k = 1; k < RB; ++k) ref = r == k ? m[k] : ref;
+      grow |= x[i] > ref + SH_GROW;
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < P; ++i) top = fmaxf(top, (i0 + i) % RB == r ? x[i] : -INFINITY);
+        top = warp_max(top);
+        if (top > m[r] + SH_GROW) {
+          const float alpha = scored_exp2(m[r] - top);
+          m[r] = top;
+#pragma unroll
+          for (int i = 0; i < P; ++i)
+            if ((i0 + i) % RB == r) l[i] *= alpha;
+#pragma unroll
+          for (int e = 0; e < EV; ++e) o[r][e] *= alpha;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int r = (i0 + i) % RB;
+      float ref = m[0];
+#pragma unroll
+      for (int k = 1; k < RB; ++k) ref = r == k ? m[k] : ref;
+      x[i] = scored_exp2(x[i] - (ref == -INFINITY ? 0.f : ref));
+      l[i] += x[i];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const int i = u * RB + r;
+        const float p = __shfl_sync(0xffffffffu, x[i % P], kk * LPK + i / P * DUP);
+        // where some row does not see some key, a value out of sight is left out: it may be no number
+        if (!edge || (j0 + u * KPI + kk <= total - n + (r0 + r) / G)) {
+#pragma unroll
+          for (int e = 0; e < EV / 4; ++e) {
+            o[r][4 * e] = fmaf(p, vr[u][e].x, o[r][4 * e]);
+            o[r][4 * e + 1] = fmaf(p, vr[u][e].y, o[r][4 * e + 1]);
+            o[r][4 * e + 2] = fmaf(p, vr[u][e].z, o[r][4 * e + 2]);
+            o[r][4 * e + 3] = fmaf(p, vr[u][e].w, o[r][4 * e + 3]);
+          }
+        }
+      }
+    load(vr, j0 + step, v_plane);
+    there = there_next;
+  }
+  // the warps' sums joined
+  const int row_len = d + 4;
+  float* so = smem;
+  float* sml = smem + SH_WARPS * w.block_rows * row_len;
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) sum += first_copy && (i0 + i) % RB == r ? l[i] : 0.f;
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int e = 0; e < EV; ++e)
+#pragma unroll
+      for (int bit = LPK; bit < 32; bit <<= 1) o[r][e] += __shfl_xor_sync(0xffffffffu, o[r][e], bit);
+    if (r >= w.block_rows) continue;
+    if (lane == 0) {
+      sml[(warp * w.block_rows + r) * 2] = m[r];
+      sml[(warp * w.block_rows + r) * 2 + 1] = sum;
+    }
+    if (kk == 0) {
+#pragma unroll
+      for (int e = 0; e < EV; e += 4) {
+        const int at = e * LPK + 4 * in_key;
+        if (at < d) *reinterpret_cast<float4*>(so + (warp * w.block_rows + r) * row_len + at) = make_float4(o[r][e], o[r][e + 1], o[r][e + 2], o[r][e + 3]);
+      }
+    }
+  }
+  __syncthreads();
+  join_warps(w, so, sml, row_len, (((size_t)blockIdx.z * a.nkv + kvh) * w.splits + split) * w.rows + r0, rows, d);
 }
 
 // Blocks [0, key_blocks): weights of `per_block` keys each, the others FIN_THREADS elements of the output each.
@@ -450,22 +656,38 @@ int launch_split(const ShortArgs& w, dim3 grid, size_t smem, cudaStream_t stream
   return 0;
 }
 
+template <int LPK, int EV, int RB>
+int launch_f32(const ShortArgs& w, dim3 grid, size_t smem, cudaStream_t stream) {
+  constexpr int BATCH = (RB * EV >= 32 ? 4 : 8) * 32 / LPK;
+  if (w.a.page_size % BATCH == 0)
+    NHV_CUDA(nhv_launch(scored_short_f32_kernel<LPK, EV, RB, true>, grid, SH_THREADS, smem, stream, w), "scored attention");
+  else
+    NHV_CUDA(nhv_launch(scored_short_f32_kernel<LPK, EV, RB, false>, grid, SH_THREADS, smem, stream, w), "scored attention");
+  return 0;
+}
+template <int LPK, int EV>
+int launch_f32(const ShortArgs& w, dim3 grid, size_t smem, cudaStream_t stream) {
+  return w.block_rows <= 2 ? launch_f32<LPK, EV, 2>(w, grid, smem, stream) : w.block_rows <= 4 ? launch_f32<LPK, EV, 4>(w, grid, smem, stream)
+                                                                                                : launch_f32<LPK, EV, 8>(w, grid, smem, stream);
+}
+
 }  // namespace
 
-int scored_short_rows(int d) {
-  // a block's 16 rows of heads above 128 would need more registers than a thread has; from 32 rows on (two blocks for the same keys)
-  // the tcgen05 kernels are faster
-  return d <= 128 ? 32 : 8;
+int scored_short_rows(int dtype, int d) {
+  // float32: blocks of 8 rows, from 16 rows on the tiles of scored_attention.cu are as fast.  bfloat16: a block's 16 rows of heads above
+  // 128 would need more registers than a thread has; from 32 rows on the tcgen05 kernels are faster.
+  return dtype == NHV_F32 ? 16 : d <= 128 ? 32 : 8;
 }
 
 bool scored_short_takes(int dtype, int rows, int d) {
-  return dtype == NHV_BF16 && d % 8 == 0 && d <= SA_MAX_D && rows <= scored_short_rows(d);
+  return d % (dtype == NHV_F32 ? 4 : 8) == 0 && d <= SA_MAX_D && rows <= scored_short_rows(dtype, d);
 }
 
 ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d) {
   ShortPlan p = {};
   p.rows = (max_rows + 1) / 2 * 2;
-  p.row_blocks = (p.rows + 23) / 24;
+  const int most = dtype == NHV_F32 ? 8 : 24;
+  p.row_blocks = (p.rows + most - 1) / most;
   p.block_rows = (p.rows / p.row_blocks + (p.rows % p.row_blocks ? 1 : 0) + 1) / 2 * 2;
   // Four times as many blocks as run at once (three an SM), so that requests of unlike length even out, and no fewer than 64 keys a
   // block (a tile per warp).
@@ -497,7 +719,7 @@ int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* w
   w.part_o = w.kept + pairs * plan.keys * plan.rows;
   w.part_ml = w.part_o + pairs * plan.splits * plan.rows * a.d;
   const int db = (a.d + 63) / 64;
-  const size_t smem = sizeof(float) * SH_WARPS * plan.block_rows * (a.d + 4);
+  const size_t smem = sizeof(float) * SH_WARPS * plan.block_rows * (a.d + 6);
   const int per_block = FIN_KEYS * FIN_THREADS;
   const int key_blocks = (a.max_keys + per_block - 1) / per_block, out_blocks = (plan.rows * a.d + FIN_THREADS - 1) / FIN_THREADS;
   for (int s = 0; s < a.n_seqs; s += plan.group) {
@@ -505,7 +727,10 @@ int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* w
     const int count = a.n_seqs - s < plan.group ? a.n_seqs - s : plan.group;
     const dim3 grid(plan.splits * plan.row_blocks, a.nkv, count);
     int rc = 0;
-    if (plan.block_rows <= 8)
+    if (dtype == NHV_F32)
+      rc = a.d <= 32 ? launch_f32<8, 4>(w, grid, smem, stream) : a.d <= 64 ? launch_f32<16, 4>(w, grid, smem, stream)
+           : a.d <= 128 ? launch_f32<32, 4>(w, grid, smem, stream) : launch_f32<32, 8>(w, grid, smem, stream);
+    else if (plan.block_rows <= 8)
       rc = db == 1 ? launch_split<1, 1>(w, grid, smem, stream) : db == 2 ? launch_split<2, 1>(w, grid, smem, stream)
            : db == 3 ? launch_split<3, 1>(w, grid, smem, stream) : launch_split<4, 1>(w, grid, smem, stream);
     else if (plan.block_rows <= 16)
@@ -513,8 +738,9 @@ int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* w
     else
       rc = db == 1 ? launch_split<1, 3>(w, grid, smem, stream) : launch_split<2, 3>(w, grid, smem, stream);
     if (rc) return rc;
-    NHV_CUDA(nhv_launch(scored_short_finish_kernel<__nv_bfloat16>, dim3(key_blocks + out_blocks, a.nkv, count), FIN_THREADS, 0, stream, w, key_blocks, per_block),
-             "scored attention");
+    const dim3 all(key_blocks + out_blocks, a.nkv, count);
+    if (dtype == NHV_F32) NHV_CUDA(nhv_launch(scored_short_finish_kernel<float>, all, FIN_THREADS, 0, stream, w, key_blocks, per_block), "scored attention");
+    else NHV_CUDA(nhv_launch(scored_short_finish_kernel<__nv_bfloat16>, all, FIN_THREADS, 0, stream, w, key_blocks, per_block), "scored attention");
   }
   return 0;
 }
