@@ -136,7 +136,17 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
     }
     return page < 0 || j >= end ? nullptr : pages + (((size_t)page * 2 * a.nkv + kvh) * a.page_size + off) * d;
   };
+  // a tile whose keys are all there and whose heads fill the lanes is read without a check a key
+  const bool full = BY16 && d == 64 * DB;
   auto load_keys = [&](int j0, int page, int off) {
+    if (full && page >= 0 && j0 + 16 <= end) {
+      const __nv_bfloat16* row = pages + (((size_t)page * 2 * a.nkv + kvh) * a.page_size + off + ra) * (64 * DB) + 8 * rc;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2 * DB; ++i) kr[h][i] = load16(row + h * 8 * 64 * DB + 32 * i);
+      return;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const __nv_bfloat16* row = row_at(j0 + ra + 8 * h, page, off, ra + 8 * h);
@@ -148,6 +158,14 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
     }
   };
   auto load_values = [&](int j0, int page, int off) {
+    if (full && page >= 0 && j0 + 16 <= end) {
+      const __nv_bfloat16* row = pages + v_plane + (((size_t)page * 2 * a.nkv + kvh) * a.page_size + off + 2 * rc) * (64 * DB) + 8 * ra;
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int b = 0; b < DB; ++b) vr[h][b] = load16(row + ((h & 1) + 8 * (h >> 1)) * 64 * DB + 64 * b);
+      return;
+    }
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
       const int in_tile = 2 * rc + (h & 1) + 8 * (h >> 1);
@@ -383,6 +401,26 @@ __global__ void __launch_bounds__(SH_THREADS, EV == 8 ? 2 : 3) scored_short_f32_
     return pages + (((size_t)page * 2 * a.nkv + kvh) * a.page_size + (j - at * a.page_size)) * d;
   };
   auto load = [&](float4 (&dst)[U][EV / 4], int j0, size_t plane) -> uint32_t {       // a bit for every u whose key is there
+    if (BY_PAGE && j0 + BATCH <= end) {                     // a whole batch in one page: no check a key (552 -> 220 us for 64 requests)
+      const float* row = row_at(j0, j0);
+      if (row) {
+        row += plane + (size_t)kk * d + 4 * in_key;
+#pragma unroll
+        for (int e = 0; e < EV / 4; ++e) {
+          if (e * 4 * LPK + 4 * in_key < d) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const uint4 v = load16(row + (size_t)(u * KPI) * d + e * 4 * LPK);
+              dst[u][e] = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) dst[u][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
+        return 0xffffffffu;
+      }
+    }
     uint32_t there = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -488,23 +526,27 @@ __global__ void __launch_bounds__(SH_THREADS, EV == 8 ? 2 : 3) scored_short_f32_
       x[i] = scored_exp2(x[i] - (ref == -INFINITY ? 0.f : ref));
       l[i] += x[i];
     }
+    auto second_product = [&](bool all) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        const int i = u * RB + r;
-        const float p = __shfl_sync(0xffffffffu, x[i % P], kk * LPK + i / P * DUP);
-        // where some row does not see some key, a value out of sight is left out: it may be no number
-        if (!edge || (j0 + u * KPI + kk <= total - n + (r0 + r) / G)) {
+        for (int r = 0; r < RB; ++r) {
+          const int i = u * RB + r;
+          const float p = __shfl_sync(0xffffffffu, x[i % P], kk * LPK + i / P * DUP);
+          // where some row does not see some key, a value out of sight is left out: it may be no number
+          if (all || (j0 + u * KPI + kk <= total - n + (r0 + r) / G)) {
 #pragma unroll
-          for (int e = 0; e < EV / 4; ++e) {
-            o[r][4 * e] = fmaf(p, vr[u][e].x, o[r][4 * e]);
-            o[r][4 * e + 1] = fmaf(p, vr[u][e].y, o[r][4 * e + 1]);
-            o[r][4 * e + 2] = fmaf(p, vr[u][e].z, o[r][4 * e + 2]);
-            o[r][4 * e + 3] = fmaf(p, vr[u][e].w, o[r][4 * e + 3]);
+            for (int e = 0; e < EV / 4; ++e) {
+              o[r][4 * e] = fmaf(p, vr[u][e].x, o[r][4 * e]);
+              o[r][4 * e + 1] = fmaf(p, vr[u][e].y, o[r][4 * e + 1]);
+              o[r][4 * e + 2] = fmaf(p, vr[u][e].z, o[r][4 * e + 2]);
+              o[r][4 * e + 3] = fmaf(p, vr[u][e].w, o[r][4 * e + 3]);
+            }
           }
         }
-      }
+    };
+    if (!edge || n == 1) second_product(true);
+    else second_product(false);
     load(vr, j0 + step, v_plane);
     there = there_next;
   }
