@@ -275,6 +275,47 @@ def test_requests_without_keys_and_entries_without_pages(ops):
         assert torch.equal(c.of(scores_out, 1, 0), c.of(c.scores, 1, 0))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 24])
+def test_offsets_beyond_32_bits(ops, dtype, new):
+    """The pages in use stand at the end of a pool of more than 2^32 elements, and half of them at its start."""
+    c = Case([new, 1], [90, 70], 4, 2, 64, 64, dtype, seed=8)
+    n_pages = 2 ** 32 // c.pages[0].numel() + 5
+    shift = n_pages - c.n_pages
+    where = torch.tensor([i if i % 2 else i + shift for i in range(c.n_pages)])
+    pages = torch.empty(n_pages, *c.pages.shape[1:], dtype=dtype, device="cuda")
+    scores, births = torch.empty(n_pages, 2, 64, device="cuda"), torch.empty(n_pages, 2, 64, dtype=torch.int32, device="cuda")
+    pages[where], scores[where], births[where] = c.pages.cuda(), c.scores.cuda(), c.births.cuda()
+    table = torch.where(c.table >= 0, where[c.table.long().clamp(min=0)].int(), c.table).cuda()
+    out = torch.full_like(c.q, math.nan).cuda()
+    ops.attention_scored(out, c.q.cuda(), pages, scores, table, c.cu_t, c.lens_t, 2, 1, new, 90, 4, 2, 64, c.scale, births=births,
+                         positions=i32(c.positions))
+    ops.raise_wait_errors()
+    c.check(out.cpu(), scores[where].cpu(), births[where].cpu())
+    before = pages[where].cpu()
+    moves = torch.tensor([[[64, 66, 80]] * 2, [[65, 69, -1]] * 2], dtype=torch.int32), torch.tensor([[[3, 0, 63]] * 2, [[1, 2, -1]] * 2], dtype=torch.int32)
+    ops.move_keys(pages, scores, births, table, moves[0].cuda(), moves[1].cuda(), 2)
+    for s in range(2):
+        for a, b in zip(moves[0][s, 0].tolist(), moves[1][s, 0].tolist()):
+            if a >= 0:
+                before[int(c.table[s, b // 64]), :, :, b % 64] = before[int(c.table[s, a // 64]), :, :, a % 64]
+    assert torch.equal(pages[where].cpu().nan_to_num(7.0), before.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lengths_far_below_the_longest_allowed(ops, dtype):
+    """The caller's bound on the lengths is what the scratch is sized by: beyond its largest size the requests go in groups."""
+    c = Case([1, 2, 1, 2, 0], [90, 70, 1, 129, 20], 16, 2, 64, 64, dtype, seed=9)
+    bound = 2 ** 21
+    table = torch.full((5, bound // 64), -1, dtype=torch.int32)
+    table[:, :c.table.shape[1]] = c.table
+    scores, births, out = c.scores.cuda(), c.births.cuda(), torch.full_like(c.q, math.nan).cuda()
+    ops.attention_scored(out, c.q.cuda(), c.pages.cuda(), scores, table.cuda(), c.cu_t, c.lens_t, 5, 0, 2, bound, 16, 2, 64, c.scale,
+                         births=births, positions=i32(c.positions))
+    ops.raise_wait_errors()
+    c.check(out.cpu(), scores.cpu(), births.cpu())
+
+
 def test_refusals_of_attention(ops):
     from nanohybrid_vlm_b200.kernels.library import KernelError
     c = Case([2, 1], [40, 30], 4, 2, 64, 16, torch.bfloat16)
@@ -388,6 +429,15 @@ def test_the_keys_that_stay(ops, nkv, page, lens, budgets, ties, keep_first, kee
     p = Pool(lens, nkv, page, seed=page + len(lens))
     scores, births = p.random(ties, order=page != 32)
     p.check(ops, scores, births, [2 * L + 1 for L in lens], budgets, keep_first, keep_recent)
+
+
+@pytest.mark.parametrize("ties", [False, True])
+@pytest.mark.parametrize("budget", [4096, 330000])
+def test_more_keys_than_the_blocks_hold(ops, ties, budget):
+    """Beyond what the blocks of a cluster keep in shared memory the keys are read again in each pass."""
+    p = Pool([350000, 400], 1, 256, seed=11)
+    scores, births = p.random(ties)
+    p.check(ops, scores, births, [700001, 801], [budget, 300], 4, 512)
 
 
 def test_scores_that_are_alike_infinite_or_no_numbers(ops):
