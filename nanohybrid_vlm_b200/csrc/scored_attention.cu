@@ -4,32 +4,36 @@
 //   scores_out[g][j] = (j < L - n ? scores[g][j] : 0) + sum over t and the heads of g of p[j];     births[g][j] = position, j new
 // A key's sum needs the rows' final normaliser, so there are two passes: the rows' (output and log-sum), then the keys'.
 //
-// The entry point, and kernels for any type, size and page size that compute in fp32 on the CUDA cores (the 32-bit path, and what
-// the tensor-core kernels of scored_attention_short.cu and scored_attention_tcgen05.cu refuse).
-//   rows: 256 threads hold 16 RPT rows (row = token * G + head, of one request and KV head) and walk the keys in tiles of 64 through
-//     shared memory.  A thread makes RPT x 4 scores from 16-byte reads along the head and RPT x 4 DB outputs, two multiply-adds
-//     an instruction; P passes through shared memory.  RPT is 8 (4 for heads above 128).
-//     A tile's values arrive while its scores are made, the next tile's keys while the values are used.
-//   keys: 64 keys stay in shared memory, the tiles of rows pass by; a thread adds up the weights of its 4 keys, the sixteen row groups
-//     meet in shared memory at the end.
-// What bounds them is multiply-adds, 4 D a pair in the first and 2 D in the second, of 128 a cycle and SM, and beside them the 16-byte
-// reads of shared memory, four cycles each however many lanes read the same: 12 for 128 multiply-adds a thread in the scores, 16 for
-// 256 in the outputs.
+// The entry point, and kernels for any type, size and page size in 32 bits (the float32 path, and what the tensor-core kernels of
+// scored_attention_short.cu and scored_attention_tcgen05.cu refuse).  Products are those of tf32 halves, x y = hi hi + hi lo + lo hi:
+// three products of the tensor cores take less than one of the CUDA cores, whose 16-byte reads of shared memory took as long again
+// (float32 prompts of 90 to 400 tokens among 400 to 777 keys: 376 us with those, 304 us so, and no less exact).
+//   rows: four warps hold 16 rows each (row = token * G + head, of one request and KV head) and walk the keys in tiles of 32 through
+//     shared memory; scores stay in registers as the weights of the second product.  Tiles of 32 let three blocks run on an SM (64: two
+//     blocks, 236 against 197 us).  A tile's values arrive while its scores are made, the next tile's keys while the values are used.
+//   keys: 64 keys stay in shared memory, the tiles of 64 rows pass by; a lane adds up the weights of its 16 keys, the rows' lanes and
+//     warps meet at the end.
+// What bounds them is the cutting into halves beside the products, with three warps a scheduler: the tensor cores are busy for 36 % of
+// the rows' pass and 43 % of the keys', the schedulers for 41 %.
 // Long walks over the keys are split over blocks where there are few tiles of rows, and rows into chunks in the keys' pass; two
 // small kernels join the parts in a fixed order.  No sum depends on the order in which blocks run.
 //
-// A key out of sight may hold anything: its score is replaced, and in tiles of which some row sees only a part its value is left
-// out of that row's sum instead of being multiplied by 0.
+// A key out of sight may hold anything: its score is replaced, and where a tile's sum is not finite its odd values are left out of
+// the products and given to the rows that see them.
+#include <type_traits>
+
 #include "nhv_scored.cuh"
 
 namespace {
 
-constexpr int SA_THREADS = 256, SA_KEYS = 64;
+constexpr int SA_THREADS = 128, SA_WARPS = SA_THREADS / 32, SA_ROWS = 16 * SA_WARPS;
+constexpr int ROWS_KEYS = 32, KEYS_KEYS = 64;     // keys of a tile in the rows' pass and in the keys' pass
 
 struct TileArgs {
   ScoredArgs a;
   ScoredParts p;
   int vec;                  // rows of q and of the pages can be read four elements at a time
+  int vec_out;              // and rows of the output written
 };
 
 template <typename T> __device__ __forceinline__ float4 load4(const T* p);
@@ -75,37 +79,107 @@ __device__ __forceinline__ void load_rows(float* dst, int stride, const T* base,
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
-// s[i][k] = row (ty RPT + i) . key (tx + 16 k)
-template <int RPT>
-__device__ __forceinline__ void tile_scores(float (&s)[RPT][4], const float* Qs, const float* Ks, int stride, int d, int ty, int tx) {
-  f32x2 acc[RPT][4];
+// A float32 as two tf32 numbers of 11 bits each: hi its nearest (NEAR: what a row brings) or its first bits (one instruction less: what
+// the keys bring; hi lo of one operand that errs to either side leaves no bias), lo what is left of it but for the last bits (3 2^-23
+// of x at most).  A bfloat16 is a tf32 as it is.  What is not finite, or rounds to that, gives no finite hi + lo.
+struct Halves {
+  uint32_t hi, lo;
+};
+template <bool EXACT, bool NEAR>
+__device__ __forceinline__ Halves halves(float x) {
+  if (EXACT) return {__float_as_uint(x), 0u};
+  const uint32_t hi = (__float_as_uint(x) + (NEAR ? 0x1000u : 0u)) & 0xffffe000u;
+  return {hi, __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u};
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// a b[u], u < N, from halves: the products of two upper ones go to c, the small ones to rest.  A_EXACT, B_EXACT: without lower halves.
+template <bool A_EXACT, bool B_EXACT, int N>
+__device__ __forceinline__ void mma_halves(float (&c)[N][4], float (&rest)[N][4], const Halves (&a)[4], const Halves (&b)[N][2]) {
 #pragma unroll
-  for (int i = 0; i < RPT; ++i)
+  for (int u = 0; u < N; ++u) mma_tf32(c[u], a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[u][0].hi, b[u][1].hi);
+  if (!A_EXACT) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[i][k] = 0ull;
-  for (int c = 0; c < d; c += 4) {
-    f32x2 kk[4][2];
+    for (int u = 0; u < N; ++u) mma_tf32(rest[u], a[0].lo, a[1].lo, a[2].lo, a[3].lo, b[u][0].hi, b[u][1].hi);
+  }
+  if (!B_EXACT) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(Ks + (tx + 16 * k) * stride + c);
-      kk[k][0] = v.x;
-      kk[k][1] = v.y;
-    }
+    for (int u = 0; u < N; ++u) mma_tf32(rest[u], a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[u][0].lo, b[u][1].lo);
+  }
+}
+
+// Columns of a tile's rows that no load fills, up to the next block of 64.
+template <int DP>
+__device__ __forceinline__ void clear_columns(float* dst, int stride, int rows, int d) {
+  const int from = (d + 3) / 4 * 4, n = DP - from;
+  for (int i = threadIdx.x; i < rows * n; i += SA_THREADS) dst[i / n * stride + from + i % n] = 0.f;
+}
+
+// The scores of 16 rows and 8 NT keys by a warp: s[c][e] is row g + 8 (e >> 1), key 8 c + 2 t + (e & 1), g = lane / 4, t = lane % 4.
+// Which column of the head is which of a step's eight is the same for both operands, so a lane reads four columns in a row.  The tensor
+// cores cut an accumulator off at each step, so large products meet there for 16 columns only, and the small ones apart (one
+// accumulator for all: errors 5 times as large).
+template <bool EXACT, int NT>
+__device__ __forceinline__ void tile_scores(float (&s)[NT][4], const float* Qw, const float* Ks, int stride, int d) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float rest[NT][4];
 #pragma unroll
-    for (int i = 0; i < RPT; ++i) {
-      const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(Qs + (ty * RPT + i) * stride + c);
+  for (int c = 0; c < NT; ++c)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[i][k] = f2_fma(q.y, kk[k][1], f2_fma(q.x, kk[k][0], acc[i][k]));
+    for (int e = 0; e < 4; ++e) s[c][e] = rest[c][e] = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < d; c += 16) {
+    const float4 x = *reinterpret_cast<const float4*>(Qw + g * stride + c + 4 * t), y = *reinterpret_cast<const float4*>(Qw + (g + 8) * stride + c + 4 * t);
+    const Halves a0[4] = {halves<EXACT, true>(x.x), halves<EXACT, true>(y.x), halves<EXACT, true>(x.y), halves<EXACT, true>(y.y)};
+    const Halves a1[4] = {halves<EXACT, true>(x.z), halves<EXACT, true>(y.z), halves<EXACT, true>(x.w), halves<EXACT, true>(y.w)};
+#pragma unroll
+    for (int k = 0; k < NT; k += 2) {
+      Halves b0[2][2], b1[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float4 v = *reinterpret_cast<const float4*>(Ks + (8 * (k + u) + g) * stride + c + 4 * t);
+        b0[u][0] = halves<EXACT, false>(v.x);
+        b0[u][1] = halves<EXACT, false>(v.y);
+        b1[u][0] = halves<EXACT, false>(v.z);
+        b1[u][1] = halves<EXACT, false>(v.w);
+      }
+      float part[2][4] = {}, (&small)[2][4] = *reinterpret_cast<float(*)[2][4]>(&rest[k]);
+      mma_halves<EXACT, EXACT>(part, small, a0, b0);
+      mma_halves<EXACT, EXACT>(part, small, a1, b1);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[k + u][e] += part[u][e];
     }
   }
+  float odd = 0.f;
 #pragma unroll
-  for (int i = 0; i < RPT; ++i)
+  for (int c = 0; c < NT; ++c)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float x, y;
-      f2_unpack(acc[i][k], x, y);
-      s[i][k] = x + y;
+    for (int e = 0; e < 4; ++e) {
+      s[c][e] += rest[c][e];
+      odd = fmaf(s[c][e], 0.f, odd);
     }
+  if (__builtin_expect(__any_sync(0xffffffffu, odd != 0.f), 0)) {              // what is not finite is made again from the products themselves
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+      float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int i = 0; i < d; ++i) {
+        const float x = Qw[g * stride + i], y = Qw[(g + 8) * stride + i];
+        const float k0 = Ks[(8 * c + 2 * t) * stride + i], k1 = Ks[(8 * c + 2 * t + 1) * stride + i];
+        z[0] = fmaf(x, k0, z[0]);
+        z[1] = fmaf(x, k1, z[1]);
+        z[2] = fmaf(y, k0, z[2]);
+        z[3] = fmaf(y, k1, z[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[c][e] = fabsf(s[c][e]) < INFINITY ? s[c][e] : z[e];
+    }
+  }
 }
 // in log2 units
 __device__ __forceinline__ float scaled(float s, const ScoredArgs& a) {
@@ -113,25 +187,30 @@ __device__ __forceinline__ float scaled(float s, const ScoredArgs& a) {
   return (a.softcap > 0.f ? a.softcap * tanhf(s / a.softcap) : s) * SA_LOG2E;
 }
 
+// Floats between rows of the tiles in shared memory: 16-byte reads by 8 lanes of two rows (queries, keys) or of four rows two apart
+// (values) meet no bank twice.
+constexpr int qk_stride(int db) { return 64 * db + 16; }
+constexpr int v_stride(int db) { return 64 * db + 4; }
+
 // DB: blocks of 64 elements of a head.
-template <typename T, int DB, int RPT>
-__global__ void __launch_bounds__(SA_THREADS, 1) scored_rows_kernel(const TileArgs t) {
+template <typename T, int DB>
+__global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 3 : 1) scored_rows_kernel(const TileArgs t) {
   extern __shared__ __align__(16) float smem[];
-  constexpr int ROWS = 16 * RPT, DP = 64 * DB, STRIDE = DP + 4, PS = SA_KEYS + 4;
-  __shared__ long long s_q[ROWS], s_at[2][SA_KEYS];      // where rows of q begin, and keys of this tile and the next
-  float* Qs = smem;                       // [ROWS][STRIDE]
-  float* Ks = Qs + ROWS * STRIDE;         // [64][STRIDE]
-  float* Vs = Ks + SA_KEYS * STRIDE;      // [64][DP]
-  float* Ps = Vs + SA_KEYS * DP;          // [ROWS][PS]
+  constexpr int DP = 64 * DB, STRIDE = qk_stride(DB), VS = v_stride(DB);
+  constexpr bool EXACT = sizeof(T) == 2;
+  __shared__ long long s_q[SA_ROWS], s_at[2][ROWS_KEYS];   // where rows of q begin, and keys of this tile and the next
+  float* Qs = smem;                       // [64][STRIDE]
+  float* Ks = Qs + SA_ROWS * STRIDE;      // [32][STRIDE]
+  float* Vs = Ks + ROWS_KEYS * STRIDE;      // [32][VS]
   pdl_prologue();
   const ScoredArgs& a = t.a;
-  const int G = a.nq / a.nkv, kvh = blockIdx.y, tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, d = a.d;
+  const int G = a.nq / a.nkv, kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tt = lane & 3, d = a.d;
   // which request, which rows: the last ones, which see the most, come first
   int tile = blockIdx.x, seq = -1;
   for (int s = 0; s < a.n_seqs; ++s) {
     const int n = a.cu_q[s + 1] - a.cu_q[s];
     if (!scored_takes(a, n)) continue;
-    const int nt = (n * G + ROWS - 1) / ROWS;
+    const int nt = (n * G + SA_ROWS - 1) / SA_ROWS;
     if (tile < nt) {
       seq = s;
       tile = nt - 1 - tile;
@@ -140,138 +219,158 @@ __global__ void __launch_bounds__(SA_THREADS, 1) scored_rows_kernel(const TileAr
     tile -= nt;
   }
   if (seq < 0) return;
-  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), r0 = tile * ROWS;
-  const int rows = min(ROWS, n * G - r0), key_begin = (int)blockIdx.z * t.p.split_tiles * SA_KEYS;
+  const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys), r0 = tile * SA_ROWS;
+  const int rows = min(SA_ROWS, n * G - r0), key_begin = (int)blockIdx.z * t.p.split_tiles * ROWS_KEYS;
   const int last = min(total - n + (r0 + rows - 1) / G, total - 1);            // the newest key that a row of the tile sees
   const int all = total - n + r0 / G;                                          // every row sees keys up to here
-  const int key_end = min(last + 1, key_begin + t.p.split_tiles * SA_KEYS);
+  const int key_end = min(last + 1, key_begin + t.p.split_tiles * ROWS_KEYS);
   const T* pages = (const T*)a.pages;
   const T* values = pages + (long long)a.nkv * a.page_size * d;               // the plane behind a page's keys
   auto place = [&](int j0, long long* at) {
-    if (tid < SA_KEYS) at[tid] = j0 + tid < key_end ? key_row(a, seq, j0 + tid, kvh, 0) : -1;
+    if (tid < ROWS_KEYS) at[tid] = j0 + tid < key_end ? key_row(a, seq, j0 + tid, kvh, 0) : -1;
   };
-  for (int r = tid; r < ROWS; r += SA_THREADS)
+  for (int r = tid; r < SA_ROWS; r += SA_THREADS)
     s_q[r] = r < rows ? (long long)(first + (r0 + r) / G) * a.q_stride + (long long)(kvh * G + (r0 + r) % G) * d : -1;
   place(key_begin, s_at[0]);
+  if (d <= DP - 4) {
+    clear_columns<DP>(Qs, STRIDE, SA_ROWS + ROWS_KEYS, d);
+    clear_columns<DP>(Vs, VS, ROWS_KEYS, d);
+  }
   __syncthreads();
   if (key_begin < key_end) {
-    load_rows<T, DB, ROWS>(Qs, STRIDE, (const T*)a.q, s_q, d, t.vec);
-    load_rows<T, DB, SA_KEYS>(Ks, STRIDE, pages, s_at[0], d, t.vec);
-    load_rows<T, DB, SA_KEYS>(Vs, DP, values, s_at[0], d, t.vec);
+    load_rows<T, DB, SA_ROWS>(Qs, STRIDE, (const T*)a.q, s_q, d, t.vec);
+    load_rows<T, DB, ROWS_KEYS>(Ks, STRIDE, pages, s_at[0], d, t.vec);
+    load_rows<T, DB, ROWS_KEYS>(Vs, VS, values, s_at[0], d, t.vec);
   }
 
-  float m[RPT], l[RPT];
-  f32x2 o[RPT][2 * DB];                   // columns 64 b + 4 tx .. + 3
-  int hi[RPT];
+  // rows g and g + 8 of the warp's sixteen; o[b][u][2 i + e]: row i, column 32 b + 8 tt + 4 e + u
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[2 * DB][4][4];
+  int hi[2];
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int r = ty * RPT + i;
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * warp + g + 8 * i;
     hi[i] = r < rows ? min(total - n + (r0 + r) / G, total - 1) : -1;
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-#pragma unroll
-    for (int c = 0; c < 2 * DB; ++c) o[i][c] = 0ull;
   }
+#pragma unroll
+  for (int b = 0; b < 2 * DB; ++b)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[b][u][e] = 0.f;
   int cur = 0;
-  for (int j0 = key_begin; j0 < key_end; j0 += SA_KEYS, cur ^= 1) {
+  for (int j0 = key_begin; j0 < key_end; j0 += ROWS_KEYS, cur ^= 1) {
     const long long* at = s_at[cur];
     wait_loads<1>();                      // the keys
     // some row does not see some key of the tile
-    const bool masked = __syncthreads_or(tid < SA_KEYS && at[tid & (SA_KEYS - 1)] < 0) || j0 + SA_KEYS - 1 > all;
-    place(j0 + SA_KEYS, s_at[cur ^ 1]);
-    float s[RPT][4];
-    tile_scores<RPT>(s, Qs, Ks, STRIDE, d, ty, tx);
+    const bool masked = __syncthreads_or(tid < ROWS_KEYS && at[tid & (ROWS_KEYS - 1)] < 0) || j0 + ROWS_KEYS - 1 > all;
+    place(j0 + ROWS_KEYS, s_at[cur ^ 1]);
+    float s[ROWS_KEYS / 8][4];
+    tile_scores<EXACT, ROWS_KEYS / 8>(s, Qs + 16 * warp * STRIDE, Ks, STRIDE, d);
     __syncthreads();
-    load_rows<T, DB, SA_KEYS>(Ks, STRIDE, pages, s_at[cur ^ 1], d, t.vec);       // zeros behind the last tile
+    load_rows<T, DB, ROWS_KEYS>(Ks, STRIDE, pages, s_at[cur ^ 1], d, t.vec);       // zeros behind the last tile
+    float top[2] = {-INFINITY, -INFINITY}, alpha[2];
 #pragma unroll
-    for (int i = 0; i < RPT; ++i) {
-      float top = -INFINITY;
+    for (int c = 0; c < ROWS_KEYS / 8; ++c)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        s[i][k] = scaled(s[i][k], a);
-        if (masked && (j0 + tx + 16 * k > hi[i] || at[tx + 16 * k] < 0)) s[i][k] = -INFINITY;
-        top = fmaxf(top, s[i][k]);
+      for (int e = 0; e < 4; ++e) {
+        const int j = 8 * c + 2 * tt + (e & 1);
+        s[c][e] = scaled(s[c][e], a);
+        if (masked && (j0 + j > hi[e >> 1] || at[j] < 0)) s[c][e] = -INFINITY;
+        top[e >> 1] = fmaxf(top[e >> 1], s[c][e]);
       }
 #pragma unroll
-      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float ref = fmaxf(m[i], top), use = ref == -INFINITY ? 0.f : ref, alpha = scored_exp2(m[i] - use);
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        s[i][k] = scored_exp2(s[i][k] - use);
-        sum += s[i][k];
-        Ps[(ty * RPT + i) * PS + tx + 16 * k] = s[i][k];
-      }
-      l[i] = fmaf(l[i], alpha, sum);      // this thread's keys; the sixteen threads of a row meet at the end
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      const float ref = fmaxf(m[i], top[i]), use = ref == -INFINITY ? 0.f : ref;
+      alpha[i] = scored_exp2(m[i] - use);
       m[i] = ref;
-      const f32x2 aa = f2_pack(alpha, alpha);
-#pragma unroll
-      for (int c = 0; c < 2 * DB; ++c) o[i][c] = f2_mul(o[i][c], aa);
+      top[i] = use;
     }
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < ROWS_KEYS / 8; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[c][e] = scored_exp2(s[c][e] - top[e >> 1]);
+        sum[e >> 1] += s[c][e];
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) l[i] = fmaf(l[i], alpha[i], sum[i]);           // this lane's keys; the four lanes of a row meet at the end
     wait_loads<1>();                      // the values
     __syncthreads();
-    bool each = false;
-    if (masked) {                         // 0 times a value is nothing only if the value is a number
-      bool odd = false;
-      for (int i = tid; i < SA_KEYS * DP; i += SA_THREADS)
-        if (i % DP < d) odd |= !(fabsf(Vs[i]) < INFINITY);
-      each = __syncthreads_or(odd);
-    }
-    if (!each) {
-#pragma unroll 2
-      for (int j = 0; j < SA_KEYS; j += 4) {
-        float4 p[RPT];
 #pragma unroll
-        for (int i = 0; i < RPT; ++i) p[i] = *reinterpret_cast<const float4*>(Ps + (ty * RPT + i) * PS + j);
+    for (int b = 0; b < 2 * DB; ++b) {
+      if (32 * b >= d) continue;
+      // a tile's products are added up apart: an accumulator that is cut off at each step stays short
+      float acc[4][4], rest[4][4];
+      auto products = [&](auto all) {       // or those of the values that have halves
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f32x2 v[2 * DB];
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int b = 0; b < DB; ++b) {
-            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(Vs + (j + k) * DP + 64 * b + 4 * tx);
-            v[2 * b] = x.x;
-            v[2 * b + 1] = x.y;
+          for (int e = 0; e < 4; ++e) acc[u][e] = rest[u][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < ROWS_KEYS / 8; ++c) {
+          float4 x = *reinterpret_cast<const float4*>(Vs + (8 * c + 2 * tt) * VS + 32 * b + 4 * g);
+          float4 y = *reinterpret_cast<const float4*>(Vs + (8 * c + 2 * tt + 1) * VS + 32 * b + 4 * g);
+          if (!decltype(all)::value) {
+            x = make_float4(fabsf(x.x) < INFINITY ? x.x : 0.f, fabsf(x.y) < INFINITY ? x.y : 0.f, fabsf(x.z) < INFINITY ? x.z : 0.f, fabsf(x.w) < INFINITY ? x.w : 0.f);
+            y = make_float4(fabsf(y.x) < INFINITY ? y.x : 0.f, fabsf(y.y) < INFINITY ? y.y : 0.f, fabsf(y.z) < INFINITY ? y.z : 0.f, fabsf(y.w) < INFINITY ? y.w : 0.f);
           }
+          const Halves p[4] = {halves<false, true>(s[c][0]), halves<false, true>(s[c][2]), halves<false, true>(s[c][1]), halves<false, true>(s[c][3])};
+          const Halves v[4][2] = {{halves<EXACT, false>(x.x), halves<EXACT, false>(y.x)}, {halves<EXACT, false>(x.y), halves<EXACT, false>(y.y)},
+                                  {halves<EXACT, false>(x.z), halves<EXACT, false>(y.z)}, {halves<EXACT, false>(x.w), halves<EXACT, false>(y.w)}};
+          mma_halves<false, EXACT>(acc, rest, p, v);
+        }
 #pragma unroll
-          for (int i = 0; i < RPT; ++i) {
-            const float pk = k == 0 ? p[i].x : k == 1 ? p[i].y : k == 2 ? p[i].z : p[i].w;
-            const f32x2 pp = f2_pack(pk, pk);
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int c = 0; c < 2 * DB; ++c) o[i][c] = f2_fma(pp, v[c], o[i][c]);
+          for (int e = 0; e < 4; ++e) acc[u][e] += rest[u][e];
+      };
+      products(std::true_type{});
+      float odd = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd = fmaf(acc[u][e], 0.f, odd);
+      if (__builtin_expect(__any_sync(0xffffffffu, odd != 0.f), 0)) {          // a value is not finite: only who sees it multiplies by it
+        products(std::false_type{});
+#pragma unroll
+        for (int c = 0; c < ROWS_KEYS / 8; ++c)
+#pragma unroll 1
+          for (int x = 0; x < 8; ++x) {
+            const int j = 8 * c + x, from = (lane & ~3) | (x >> 1);
+            const float even0 = __shfl_sync(0xffffffffu, s[c][0], from), odd0 = __shfl_sync(0xffffffffu, s[c][1], from);
+            const float even1 = __shfl_sync(0xffffffffu, s[c][2], from), odd1 = __shfl_sync(0xffffffffu, s[c][3], from);
+            const float p0 = x & 1 ? odd0 : even0, p1 = x & 1 ? odd1 : even1;
+            const bool there = at[j] >= 0, sees0 = there && j0 + j <= hi[0], sees1 = there && j0 + j <= hi[1];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float v = Vs[j * VS + 32 * b + 8 * tt + 4 * e + u];
+                if (fabsf(v) < INFINITY) continue;
+                if (sees0) acc[u][e] = fmaf(p0, v, acc[u][e]);
+                if (sees1) acc[u][2 + e] = fmaf(p1, v, acc[u][2 + e]);
+              }
           }
-        }
       }
-    } else {
-      for (int j = 0; j < SA_KEYS && j0 + j < key_end; ++j) {
-        if (at[j] < 0) continue;
-        f32x2 v[2 * DB];
 #pragma unroll
-        for (int b = 0; b < DB; ++b) {
-          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(Vs + j * DP + 64 * b + 4 * tx);
-          v[2 * b] = x.x;
-          v[2 * b + 1] = x.y;
-        }
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-          if (j0 + j > hi[i]) continue;
-          const float pk = Ps[(ty * RPT + i) * PS + j];
-          const f32x2 pp = f2_pack(pk, pk);
-#pragma unroll
-          for (int c = 0; c < 2 * DB; ++c) o[i][c] = f2_fma(pp, v[c], o[i][c]);
-        }
-      }
+        for (int e = 0; e < 4; ++e) o[b][u][e] = fmaf(o[b][u][e], alpha[e >> 1], acc[u][e]);
     }
     __syncthreads();
-    load_rows<T, DB, SA_KEYS>(Vs, DP, values, s_at[cur ^ 1], d, t.vec);
+    load_rows<T, DB, ROWS_KEYS>(Vs, VS, values, s_at[cur ^ 1], d, t.vec);
   }
   wait_loads<0>();
   T* out = (T*)a.out;
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
+  for (int i = 0; i < 2; ++i) {
     float sum = l[i];
-#pragma unroll
-    for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    const int r = ty * RPT + i;
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    const int r = 16 * warp + g + 8 * i;
     if (r >= rows) continue;
     const int token = first + (r0 + r) / G, head = kvh * G + (r0 + r) % G;
     const size_t row = (size_t)kvh * a.n_tokens * G + (size_t)first * G + r0 + r;
@@ -282,91 +381,110 @@ __global__ void __launch_bounds__(SA_THREADS, 1) scored_rows_kernel(const TileAr
       const float f = scored_exp2(m[i] - use);
       sum = fmaf(sum, f, scored_exp2(sink - use));
       inv = sum == 0.f ? 0.f : f / sum;
-      if (tx == 0) a.lse[row] = sum == 0.f ? INFINITY : use + log2f(sum);
-    } else if (tx == 0) {
+      if (tt == 0) a.lse[row] = sum == 0.f ? INFINITY : use + log2f(sum);
+    } else if (tt == 0) {
       float* ml = t.p.ml + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * 2;
       ml[0] = m[i];
       ml[1] = sum;
     }
+    T* dst = out + (size_t)token * a.out_stride + (size_t)head * d;
+    float* part = t.p.o + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * d;
 #pragma unroll
-    for (int c = 0; c < 2 * DB; ++c) {
-      float x, y;
-      f2_unpack(o[i][c], x, y);
-      const int at = 64 * (c >> 1) + 4 * tx + 2 * (c & 1);
-      if (whole) {
-        T* dst = out + (size_t)token * a.out_stride + (size_t)head * d + at;
-        if (at < d) dst[0] = from_f32<T>(x * inv);
-        if (at + 1 < d) dst[1] = from_f32<T>(y * inv);
-      } else {
-        float* dst = t.p.o + ((size_t)blockIdx.z * a.nkv * a.n_tokens * G + row) * d + at;
-        if (at < d) dst[0] = x;
-        if (at + 1 < d) dst[1] = y;
+    for (int b = 0; b < 2 * DB; ++b)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int at = 32 * b + 8 * tt + 4 * e;
+        if (at >= d) continue;
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = o[b][u][2 * i + e] * inv;
+        if (d % 4 == 0 && (!whole || (sizeof(T) == 4 && t.vec_out))) {
+          *reinterpret_cast<float4*>(whole ? (float*)dst + at : part + at) = make_float4(x[0], x[1], x[2], x[3]);
+          continue;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (at + u >= d) continue;
+          if (whole) dst[at + u] = from_f32<T>(x[u]);
+          else part[at + u] = x[u];
+        }
       }
-    }
   }
 }
 
-template <typename T, int DB, int RPT>
-__global__ void __launch_bounds__(SA_THREADS, 1) scored_keys_kernel(const TileArgs t) {
+template <typename T, int DB>
+__global__ void __launch_bounds__(SA_THREADS, DB <= 2 ? 3 : 1) scored_keys_kernel(const TileArgs t) {
   extern __shared__ __align__(16) float smem[];
-  constexpr int ROWS = 16 * RPT, STRIDE = 64 * DB + 4;
-  __shared__ long long s_k[SA_KEYS], s_q[2][ROWS];
-  __shared__ float s_lse[2][ROWS], s_part[16][SA_KEYS];
+  constexpr int STRIDE = qk_stride(DB);
+  constexpr bool EXACT = sizeof(T) == 2;
+  __shared__ long long s_k[KEYS_KEYS], s_q[2][SA_ROWS];
+  __shared__ float s_lse[2][SA_ROWS], s_part[SA_WARPS][KEYS_KEYS];
   float* Ks = smem;                       // [64][STRIDE]
-  float* Qs = Ks + SA_KEYS * STRIDE;      // [2][ROWS][STRIDE]
+  float* Qs = Ks + KEYS_KEYS * STRIDE;      // [64][STRIDE]
   pdl_prologue();
   const ScoredArgs& a = t.a;
-  const int G = a.nq / a.nkv, kvh = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, d = a.d;
-  const int tiles = (int)(t.p.keys / SA_KEYS), chunk = blockIdx.x / tiles, key0 = (blockIdx.x - chunk * tiles) * SA_KEYS;
+  const int G = a.nq / a.nkv, kvh = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tt = lane & 3, d = a.d;
+  const int tiles = (int)(t.p.keys / KEYS_KEYS), chunk = blockIdx.x / tiles, key0 = (blockIdx.x - chunk * tiles) * KEYS_KEYS;
   const int first = a.cu_q[seq], n = a.cu_q[seq + 1] - first, total = min(a.kv_len[seq], a.max_keys);
   if (key0 >= total || !scored_takes(a, n)) return;
   int begin, end;
   chunk_range(t.p, n, G, total, key0, chunk, begin, end);
   if (t.p.chunks > 1 && begin >= end) return;
   auto place = [&](int i0, int buf) {
-    for (int r = tid; r < ROWS; r += SA_THREADS) {
-      const int row = i0 * ROWS + r;
+    for (int r = tid; r < SA_ROWS; r += SA_THREADS) {
+      const int row = i0 * SA_ROWS + r;
       const bool in = i0 < end && row < n * G;
       s_q[buf][r] = in ? (long long)(first + row / G) * a.q_stride + (long long)(kvh * G + row % G) * d : -1;
       s_lse[buf][r] = in ? a.lse[(size_t)kvh * a.n_tokens * G + (size_t)first * G + row] : INFINITY;
     }
   };
-  if (tid < SA_KEYS) s_k[tid] = key0 + tid < total ? key_row(a, seq, key0 + tid, kvh, 0) : -1;
+  if (tid < KEYS_KEYS) s_k[tid] = key0 + tid < total ? key_row(a, seq, key0 + tid, kvh, 0) : -1;
   place(begin, 0);
+  if (d <= 64 * DB - 4) clear_columns<64 * DB>(Ks, STRIDE, KEYS_KEYS + SA_ROWS, d);
   __syncthreads();
   if (begin < end) {
-    load_rows<T, DB, SA_KEYS>(Ks, STRIDE, (const T*)a.pages, s_k, d, t.vec);
-    load_rows<T, DB, ROWS>(Qs, STRIDE, (const T*)a.q, s_q[0], d, t.vec);
+    load_rows<T, DB, KEYS_KEYS>(Ks, STRIDE, (const T*)a.pages, s_k, d, t.vec);
+    load_rows<T, DB, SA_ROWS>(Qs, STRIDE, (const T*)a.q, s_q[0], d, t.vec);
   }
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  float w[8][2];                          // keys 8 c + 2 tt + e
+#pragma unroll
+  for (int c = 0; c < 8; ++c) w[c][0] = w[c][1] = 0.f;
   int cur = 0;
   for (int i0 = begin; i0 < end; ++i0, cur ^= 1) {
+    wait_loads<0>();
+    __syncthreads();
     place(i0 + 1, cur ^ 1);
+    float s[8][4];
+    tile_scores<EXACT, KEYS_KEYS / 8>(s, Qs + 16 * warp * STRIDE, Ks, STRIDE, d);
     __syncthreads();
-    load_rows<T, DB, ROWS>(Qs + (cur ^ 1) * ROWS * STRIDE, STRIDE, (const T*)a.q, s_q[cur ^ 1], d, t.vec);      // zeros behind the last tile
-    wait_loads<1>();
-    __syncthreads();
-    float s[RPT][4];
-    tile_scores<RPT>(s, Qs + cur * ROWS * STRIDE, Ks, STRIDE, d, ty, tx);
+    load_rows<T, DB, SA_ROWS>(Qs, STRIDE, (const T*)a.q, s_q[cur ^ 1], d, t.vec);        // zeros behind the last tile
 #pragma unroll
-    for (int i = 0; i < RPT; ++i) {
-      const int r = ty * RPT + i, row = i0 * ROWS + r, hi = row < n * G ? total - n + row / G : -1;
+    for (int i = 0; i < 2; ++i) {
+      const int r = 16 * warp + g + 8 * i, row = i0 * SA_ROWS + r, hi = row < n * G ? total - n + row / G : -1;
+      const float lse = s_lse[cur][r];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float p = scored_exp2(scaled(s[i][k], a) - s_lse[cur][r]);
-        if (key0 + tx + 16 * k <= hi) w[k] += p;
-      }
+      for (int c = 0; c < 8; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p = scored_exp2(scaled(s[c][2 * i + e], a) - lse);
+          if (key0 + 8 * c + 2 * tt + e <= hi) w[c][e] += p;
+        }
     }
-    __syncthreads();
   }
   wait_loads<0>();
 #pragma unroll
-  for (int k = 0; k < 4; ++k) s_part[ty][tx + 16 * k] = w[k];
+  for (int c = 0; c < 8; ++c)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) w[c][e] += __shfl_xor_sync(0xffffffffu, w[c][e], x);
+      if (g == 0) s_part[warp][8 * c + 2 * tt + e] = w[c][e];
+    }
   __syncthreads();
-  if (tid < SA_KEYS && key0 + tid < total) {
+  if (tid < KEYS_KEYS && key0 + tid < total) {
     float sum = 0.f;
 #pragma unroll
-    for (int y = 0; y < 16; ++y) sum += s_part[y][tid];
+    for (int y = 0; y < SA_WARPS; ++y) sum += s_part[y][tid];
     if (t.p.chunks == 1) store_weight(a, seq, first, kvh, key0 + tid, key0 + tid - (total - n), sum);
     else t.p.w[(((size_t)seq * a.nkv + kvh) * t.p.chunks + chunk) * t.p.keys + key0 + tid] = sum;
   }
@@ -441,31 +559,28 @@ __global__ void __launch_bounds__(256) scored_join_keys_kernel(const ScoredArgs 
   store_weight(a, seq, first, kvh, key, key - (total - n), sum);
 }
 
-template <typename T, int DB, int RPT>
+template <typename T, int DB>
 int launch_tiles(const TileArgs& t, cudaStream_t stream) {
   static std::atomic<uint64_t> rows_done{0}, keys_done{0};
-  constexpr int ROWS = 16 * RPT, STRIDE = 64 * DB + 4;
-  constexpr size_t rows_smem = sizeof(float) * ((ROWS + SA_KEYS) * STRIDE + SA_KEYS * 64 * DB + ROWS * (SA_KEYS + 4));
-  constexpr size_t keys_smem = sizeof(float) * (2 * ROWS + SA_KEYS) * STRIDE;
+  constexpr size_t rows_smem = sizeof(float) * ((SA_ROWS + ROWS_KEYS) * qk_stride(DB) + ROWS_KEYS * v_stride(DB));
+  constexpr size_t keys_smem = sizeof(float) * (SA_ROWS + KEYS_KEYS) * qk_stride(DB);
   const ScoredArgs& a = t.a;
-  const long long tiles = (long long)a.n_tokens * (a.nq / a.nkv) / ROWS + a.n_seqs, key_tiles = (long long)(t.p.keys / SA_KEYS) * t.p.chunks;
+  const long long tiles = (long long)a.n_tokens * (a.nq / a.nkv) / SA_ROWS + a.n_seqs, key_tiles = (long long)(t.p.keys / KEYS_KEYS) * t.p.chunks;
   NHV_REQUIRE(tiles < (1LL << 31) && key_tiles < (1LL << 31), "scored attention: %lld tiles of rows, %lld of keys are beyond the grid's reach", tiles, key_tiles);
-  NHV_CUDA(nhv_allow_smem((const void*)scored_rows_kernel<T, DB, RPT>, (int)rows_smem, rows_done), "scored attention");
-  NHV_CUDA(nhv_allow_smem((const void*)scored_keys_kernel<T, DB, RPT>, (int)keys_smem, keys_done), "scored attention");
-  NHV_CUDA(nhv_launch(scored_rows_kernel<T, DB, RPT>, dim3((unsigned)tiles, a.nkv, t.p.splits), SA_THREADS, rows_smem, stream, t), "scored attention");
+  NHV_CUDA(nhv_allow_smem((const void*)scored_rows_kernel<T, DB>, (int)rows_smem, rows_done), "scored attention");
+  NHV_CUDA(nhv_allow_smem((const void*)scored_keys_kernel<T, DB>, (int)keys_smem, keys_done), "scored attention");
+  NHV_CUDA(nhv_launch(scored_rows_kernel<T, DB>, dim3((unsigned)tiles, a.nkv, t.p.splits), SA_THREADS, rows_smem, stream, t), "scored attention");
   int rc = scored_join_rows(sizeof(T) == 4 ? NHV_F32 : NHV_BF16, a, t.p, stream);
   if (rc) return rc;
-  NHV_CUDA(nhv_launch(scored_keys_kernel<T, DB, RPT>, dim3((unsigned)key_tiles, a.nkv, a.n_seqs), SA_THREADS, keys_smem, stream, t), "scored attention");
+  NHV_CUDA(nhv_launch(scored_keys_kernel<T, DB>, dim3((unsigned)key_tiles, a.nkv, a.n_seqs), SA_THREADS, keys_smem, stream, t), "scored attention");
   return scored_join_keys(a, t.p, stream);
 }
 
-// Rows of a thread of the tiles' sixteen row groups.
-int rows_per_thread(int d) { return d <= 128 ? 8 : 4; }
-
 size_t tile_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
-  p.tile_rows = 16 * rows_per_thread(d);
-  p.tile_keys = SA_KEYS;
-  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, p.tile_rows, SA_KEYS, p.tile_rows * SA_KEYS * d / 50.0, 148, 148);
+  p.tile_rows = SA_ROWS;
+  p.tile_keys = KEYS_KEYS;
+  const int at_once = d <= 128 ? 3 * 148 : 148;
+  return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, SA_ROWS, ROWS_KEYS, SA_ROWS * ROWS_KEYS * d / 30.0, at_once, at_once);
 }
 
 }  // namespace
@@ -623,9 +738,10 @@ NHV_API int nhv_attention_scored(const NhvScoredCall* c, float* work, int work_k
   }
   scored_place(plan.parts, scratch, n_tokens, nq, d);
   if (plan.many) return scored_long_launch(a, plan.parts, stream);
-  const TileArgs t{a, plan.parts, d % 4 == 0 && c->q_stride % 4 == 0 && (uintptr_t)c->q % 16 == 0 && (uintptr_t)c->kv_pages % 16 == 0};
+  const TileArgs t{a, plan.parts, d % 4 == 0 && c->q_stride % 4 == 0 && (uintptr_t)c->q % 16 == 0 && (uintptr_t)c->kv_pages % 16 == 0,
+                   c->out_stride % 4 == 0 && (uintptr_t)c->out % 16 == 0};
   const int db = d <= 64 ? 1 : d <= 128 ? 2 : 4;
   if (dtype == NHV_BF16)
-    return db == 1 ? launch_tiles<__nv_bfloat16, 1, 8>(t, stream) : db == 2 ? launch_tiles<__nv_bfloat16, 2, 8>(t, stream) : launch_tiles<__nv_bfloat16, 4, 4>(t, stream);
-  return db == 1 ? launch_tiles<float, 1, 8>(t, stream) : db == 2 ? launch_tiles<float, 2, 8>(t, stream) : launch_tiles<float, 4, 4>(t, stream);
+    return db == 1 ? launch_tiles<__nv_bfloat16, 1>(t, stream) : db == 2 ? launch_tiles<__nv_bfloat16, 2>(t, stream) : launch_tiles<__nv_bfloat16, 4>(t, stream);
+  return db == 1 ? launch_tiles<float, 1>(t, stream) : db == 2 ? launch_tiles<float, 2>(t, stream) : launch_tiles<float, 4>(t, stream);
 }
