@@ -94,9 +94,11 @@ struct ShortPlan {
   int rows;                 // rows kept per key: the most of a request, rounded up to 2
   int block_rows, row_blocks;       // rows of a block, blocks that share a request's rows
   int split_keys, splits;   // keys of a block, parts of a request's keys
+  int cluster;              // blocks that finish a (request, KV head) in one launch, or 0
   int group;                // requests per pair of launches (the scores kept are bounded)
   size_t keys;              // places for keys of a (request, KV head)
   size_t floats;            // of scratch
+  size_t smem;              // bytes of a block
 };
 // The most rows of a request that goes this way, and whether requests of up to `rows` rows can.
 int scored_short_rows(int dtype, int d);
