@@ -11,6 +11,10 @@
 //     each block counting its own and reading the others' counts through the cluster; then every warp goes over its own run of slots
 //     three times, without a barrier inside: keys equal to the bound are counted, then sources and targets, then written.
 //   moves: a warp for eight moves, whose loads are all sent before the first store: K row, V row, score and birth.
+//
+// What bounds them: the choice reads 8 bytes a key and is a chain of counts, meetings and prefix sums (64 requests of 2,304 keys and 8
+// heads 19 us, eight of 20,000 to 40,000 keys 32 us, against 2 and 3 us of reading); the moves are bound by memory (137 MB in 28 us,
+// 242 MB in 44 us, 4.9 and 5.5 TB/s of the 6.5 that a copy has).
 #include "nhv_common.cuh"
 
 namespace {
