@@ -195,6 +195,22 @@ def test_many_requests(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page,new,cap,sinks", [
+    (4, 1, 128, 64, 1, None, True),
+    (8, 1, 128, 16, 2, 30.0, False),
+    (3, 3, 40, 7, 2, 5.0, True),
+    (8, 8, 64, 8, 1, None, False),
+    (16, 1, 32, 48, 1, 20.0, True),
+    (2, 1, 256, 32, 1, None, True),
+])
+def test_more_blocks_than_run_at_once(ops, dtype, nq, nkv, d, page, new, cap, sinks):
+    """Few rows a request, of so many requests that parts and weights are brought together by a kernel of their own; some bring nothing."""
+    lens = [3 + (53 * i) % 127 for i in range(120)]
+    c = Case([(new * (i % 5 > 0)) for i in range(120)], lens, nq, nkv, d, page, dtype, cap=cap, sinks=sinks, seed=12)
+    c.check(*c.run(ops))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lengths", ["single", "prompts"])
 def test_in_place_rows_apart_and_a_wide_table(ops, dtype, lengths):
     c = Case(*LENGTHS[lengths], 8, 2, 64, 64, dtype, seed=5, width=3)
