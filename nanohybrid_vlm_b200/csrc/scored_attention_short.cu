@@ -347,7 +347,6 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
     const bool edge = j0 + 15 > total - n;
     if (w.cap.in != 0.f) nhv_cap_tile(s, w.cap);
     bool grow = false;
-    float top[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -363,13 +362,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
         }
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x = fmaxf(s[t][e], s[t][2 + e]);
-#pragma unroll
-        for (int k = 4; k < 32; k <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
-        top[t][e] = x;
-        grow |= x > m[t][e] + SH_GROW;
-      }
+      for (int e = 0; e < 2; ++e) grow |= fmaxf(s[t][e], s[t][2 + e]) > m[t][e] + SH_GROW;       // over the lanes only where it does
       if (t * 8 + 2 * rc < RB) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -381,9 +374,12 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (top[t][e] > m[t][e] + SH_GROW) {
-            const float alpha = scored_exp2(m[t][e] - top[t][e]);      // 0 when the row had seen nothing
-            m[t][e] = top[t][e];
+          float top = fmaxf(s[t][e], s[t][2 + e]);
+#pragma unroll
+          for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+          if (top > m[t][e] + SH_GROW) {
+            const float alpha = scored_exp2(m[t][e] - top);            // 0 when the row had seen nothing
+            m[t][e] = top;
             l[t][e] *= alpha;
 #pragma unroll
             for (int b = 0; b < DB; ++b)
