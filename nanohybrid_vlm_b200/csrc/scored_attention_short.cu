@@ -19,7 +19,7 @@
 //
 // What bounds it is reading the pages: 64 decoded tokens over 1,500 to 2,304 keys each (474 MB), 32 heads on 8 of 128, 101 us in both
 // kernels, of them 88 in the first at 5.4 TB/s; three over 65,000 to 98,000 keys 175 us.  With 20 rows a request (drafts) it is the
-// instructions of the products and exponentials: 136 us for 311 MB.
+// instructions of the products and exponentials, with two blocks an SM to hide them: 120 us for 311 MB.
 //
 // A key out of sight may hold anything: its score is replaced, its value not loaded.  Where only some of a request's rows see a
 // key (several new tokens), the second product is made token by token with the values that the token sees.
@@ -866,13 +866,14 @@ ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, i
   const int most = dtype == NHV_F32 ? 8 : 24;
   p.row_blocks = (p.rows + most - 1) / most;
   p.block_rows = (p.rows / p.row_blocks + (p.rows % p.row_blocks ? 1 : 0) + 1) / 2 * 2;
-  // Four times as many blocks as run at once (three an SM), so that requests of unlike length even out, and no fewer than 64 keys a
-  // block (a tile per warp).
-  const long long keys = (long long)n_seqs * nkv * p.row_blocks * max_keys, want = (keys + 4 * 444 - 1) / (4 * 444);
+  // Four times as many blocks as run at once (three times: drafts 120 -> 125 us, 64 decoded tokens 101 -> 103), so that requests of
+  // unlike length even out, and no fewer than 64 keys a block (a tile per warp).
+  const int an_sm = dtype == NHV_F32 ? (d <= 128 ? 3 : 2) : p.block_rows * ((d + 63) / 64) <= 16 ? 3 : 2, at_once = 148 * an_sm;
+  const long long keys = (long long)n_seqs * nkv * p.row_blocks * max_keys, want = (keys + 4 * at_once - 1) / (4 * at_once);
   p.split_keys = (int)((want + 63) / 64 * 64);
   if (p.split_keys < 64) p.split_keys = 64;
   p.splits = (max_keys + p.split_keys - 1) / p.split_keys;
-  // Where a request's parts are few, their scores stay in shared memory and all blocks run at once (three an SM), a cluster of blocks
+  // Where a request's parts are few, their scores stay in shared memory and all blocks run at once, a cluster of blocks
   // finishes the request and KV head alone, without a second launch: one request of 517 keys 18.4 -> 15.3 us a call, as long on the
   // device (9.8 against 9.5; float32 13.1 against 11.3), four of 1,000 keys 14.6 -> 11.6 there (float32 19.6 -> 16.3).  With more
   // blocks than that the wait for the slowest of a cluster costs more than the second kernel (64 requests 101 -> 119 us).
@@ -881,7 +882,7 @@ ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, i
     while (blocks < p.splits && blocks < SH_MOST_CLUSTER) blocks *= 2;
     const int keys = (max_keys + blocks * 64 - 1) / (blocks * 64) * 64;
     const size_t smem = sizeof(float) * (short_sums(p.block_rows, d) + short_part(p.block_rows, d) + (size_t)keys * p.rows);
-    if (smem <= 72 * 1024 && (long long)n_seqs * nkv * blocks <= 3 * 148) {
+    if (smem <= 72 * 1024 && (long long)n_seqs * nkv * blocks <= at_once) {
       p.cluster = p.splits = blocks;
       p.split_keys = keys;
       p.smem = smem;
