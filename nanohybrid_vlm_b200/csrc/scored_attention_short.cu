@@ -851,9 +851,10 @@ int launch_f32(const ShortArgs& w, dim3 grid, size_t smem, cudaStream_t stream) 
 }  // namespace
 
 int scored_short_rows(int dtype, int d) {
-  // float32: blocks of 8 rows, from 16 rows on the tiles of scored_attention.cu are as fast.  bfloat16: a block's 16 rows of heads above
-  // 128 would need more registers than a thread has; from 32 rows on the tcgen05 kernels are faster.
-  return dtype == NHV_F32 ? 16 : d <= 128 ? 32 : 8;
+  // float32: blocks of 8 rows; 24 rows take 153 us where the tiles of scored_attention.cu take 245 (8 requests of 2,000 keys), 32 rows 197.
+  // bfloat16: a block's 16 rows of heads above 128 would need more registers than a thread has; from 32 rows on the tcgen05 kernels are
+  // faster.
+  return dtype == NHV_F32 ? 32 : d <= 128 ? 32 : 8;
 }
 
 bool scored_short_takes(int dtype, int rows, int d) {
