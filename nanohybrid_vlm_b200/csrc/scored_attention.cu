@@ -631,7 +631,7 @@ void scored_place(ScoredParts& p, float* work, int n_tokens, int nq, int d) {
 }
 
 int scored_join_rows(int dtype, const ScoredArgs& a, const ScoredParts& p, cudaStream_t stream) {
-  if (p.splits <= 1) return 0;
+  if (p.splits <= 1 || a.n_tokens == 0) return 0;
   const dim3 grid((unsigned)(((long long)a.n_tokens * a.nq + 7) / 8));
   if (dtype == NHV_F32) NHV_CUDA(nhv_launch(scored_join_rows_kernel<float>, grid, 256, 0, stream, a, p), "scored attention");
   else NHV_CUDA(nhv_launch(scored_join_rows_kernel<__nv_bfloat16>, grid, 256, 0, stream, a, p), "scored attention");

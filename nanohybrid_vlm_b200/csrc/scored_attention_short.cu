@@ -863,7 +863,7 @@ bool scored_short_takes(int dtype, int rows, int d) {
 
 ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d) {
   ShortPlan p = {};
-  p.rows = (max_rows + 1) / 2 * 2;
+  p.rows = max_rows > 1 ? (max_rows + 1) / 2 * 2 : 2;      // requests that bring nothing go this way too: their scores pass through
   const int most = dtype == NHV_F32 ? 8 : 24;
   p.row_blocks = (p.rows + most - 1) / most;
   p.block_rows = (p.rows / p.row_blocks + (p.rows % p.row_blocks ? 1 : 0) + 1) / 2 * 2;

@@ -553,3 +553,25 @@ def test_moves_beyond_the_table_move_nothing(ops):
     pages, sc, bi = p.pages.cuda(), p.scores.cuda(), p.births.cuda()
     ops.move_keys(pages, sc, bi, p.table.cuda(), bad, to, 1)
     assert torch.equal(pages.cpu(), p.pages) and torch.equal(bi.cpu(), p.births)
+
+
+# ---------------------------------------------------------------- steps that bring nothing
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page", [(4, 2, 64, 16), (64, 1, 128, 64), (3, 3, 33, 5), (2, 1, 256, 7)])
+@pytest.mark.parametrize("lens", [[40, 0, 7], [20000], [3 + i % 90 for i in range(130)]])
+def test_a_step_without_new_tokens_passes_the_scores_through(ops, dtype, nq, nkv, d, page, lens):
+    c = Case([0] * len(lens), [min(L, 90) for L in lens], nq, nkv, d, page, dtype, seed=13)
+    scores_out = torch.full_like(c.scores, 5.0).cuda()
+    q = torch.empty(0, nq * d, dtype=dtype, device="cuda")
+    births = c.births.cuda()
+    longest = max(lens)
+    table = torch.full((len(lens), -(-longest // page)), -1, dtype=torch.int32)
+    table[:, :c.table.shape[1]] = c.table[:, :table.shape[1]]
+    ops.attention_scored(torch.empty_like(q), q, c.pages.cuda(), c.scores.cuda(), table.cuda(), c.cu_t, c.lens_t, len(lens), 0, 0, longest, nq, nkv, d,
+                         c.scale, births=births, positions=i32([]), scores_out=scores_out)
+    ops.raise_wait_errors()
+    touched = c.check(c.q, scores_out.cpu(), births.cpu(), rows=slice(0))
+    assert (scores_out.cpu()[~touched] == 5.0).all()
+    for s in range(len(lens)):
+        for g in range(nkv):
+            assert torch.equal(c.of(scores_out.cpu(), s, g), c.of(c.scores, s, g))
