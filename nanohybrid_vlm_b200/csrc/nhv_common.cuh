@@ -203,6 +203,9 @@ __device__ __forceinline__ float nhv_cap_small(float raw, const NhvScoreCap& c) 
   const float z = raw * c.z, t = z * z;
   return z * fmaf(fmaf(fmaf(fmaf(c.c[4], t, c.c[3]), t, c.c[2]), t, c.c[1]), t, c.c[0]);
 }
+// The bound on the exponent makes the cap of a score that is no number; with KEEP such a score stays what it was, and the one that
+// shares its reciprocal does not notice.
+template <bool KEEP = false>
 __device__ __forceinline__ void nhv_cap_scores(float& a, float& b, const NhvScoreCap& c) {
   float ea, eb, r;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(ea) : "f"(fminf(a * c.in, 60.f)));
@@ -211,11 +214,12 @@ __device__ __forceinline__ void nhv_cap_scores(float& a, float& b, const NhvScor
   eb += 1.f;
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(ea * eb));
   r *= -2.0f * c.out;
-  a = fmaf(r, eb, c.out);
-  b = fmaf(r, ea, c.out);
+  const float x = fmaf(r, eb, c.out), y = fmaf(r, ea, c.out);
+  a = KEEP && a != a ? a : x;
+  b = KEEP && b != b ? b : y;
 }
 // The scores of a warp's tile, N groups of four a thread (scores that a mask replaces later may be anything).
-template <int N>
+template <int N, bool KEEP = false>
 __device__ __forceinline__ void nhv_cap_tile(float (&s)[N][4], const NhvScoreCap& c) {
   float m = 0.f;
 #pragma unroll
@@ -229,8 +233,8 @@ __device__ __forceinline__ void nhv_cap_tile(float (&s)[N][4], const NhvScoreCap
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      nhv_cap_scores(s[j][0], s[j][1], c);
-      nhv_cap_scores(s[j][2], s[j][3], c);
+      nhv_cap_scores<KEEP>(s[j][0], s[j][1], c);
+      nhv_cap_scores<KEEP>(s[j][2], s[j][3], c);
     }
   }
 }

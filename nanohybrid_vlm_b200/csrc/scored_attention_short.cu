@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
 
     // scores in log2 units; -inf for what a row does not see
     const bool edge = j0 + 15 > total - n;
-    if (w.cap.in != 0.f) nhv_cap_tile(s, w.cap);
+    if (w.cap.in != 0.f) nhv_cap_tile<NT, true>(s, w.cap);
     bool grow = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {

@@ -210,7 +210,7 @@ __device__ __forceinline__ void cap32(uint32_t (&sr)[32], const NhvScoreCap& c) 
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       float x = __uint_as_float(sr[i]), y = __uint_as_float(sr[i + 1]);
-      nhv_cap_scores(x, y, c);
+      nhv_cap_scores<true>(x, y, c);
       sr[i] = __float_as_uint(x);
       sr[i + 1] = __float_as_uint(y);
     }

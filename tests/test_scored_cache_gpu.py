@@ -575,3 +575,40 @@ def test_a_step_without_new_tokens_passes_the_scores_through(ops, dtype, nq, nkv
     for s in range(len(lens)):
         for g in range(nkv):
             assert torch.equal(c.of(scores_out.cpu(), s, g), c.of(c.scores, s, g))
+
+
+# ---------------------------------------------------------------- numbers that are none, and infinite ones, in sight
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page", [(4, 2, 128, 64), (6, 2, 32, 8), (2, 2, 64, 256), (3, 1, 33, 7)])
+@pytest.mark.parametrize("cap,spread", [(None, 1.5), (30.0, 1.5), (30.0, 60.0), (2.0, 20.0)])
+def test_scores_that_are_no_numbers_stay_so_under_a_cap(ops, dtype, nq, nkv, d, page, cap, spread):
+    """The key of the 46th new token is no number: nobody before it notices, and from it on nothing is a number, whether the tile's other
+    scores are small or beyond half the cap.  The same for a query, alone among its request's."""
+    n, G = 80, nq // nkv
+    c = Case([n, 1, 50, 3], [n + 40, 30, 50, 90], nq, nkv, d, page, dtype, cap=cap, spread=spread, seed=d)
+    clean, scores_clean, _ = c.run(ops)
+    bad, pages = 40 + 45, c.pages.clone()
+    c.pages[int(c.table[0, bad // page]), 0, :, bad % page] = math.nan
+    c.pages[int(c.table[1, 20 // page]), 0, :, 20 % page, d // 2] = math.nan           # an old key of a single token
+    out, scores_out, _ = c.run(ops)
+    c.pages = pages
+    assert torch.equal(out[:45], clean[:45]) and torch.equal(out[n + 1:], clean[n + 1:])
+    assert torch.isnan(out[45:n + 1].float()).all()
+    for g in range(nkv):
+        assert torch.isnan(c.of(scores_out, 0, g)).all() and torch.isnan(c.of(scores_out, 1, g)).all()
+        for s in (2, 3):
+            assert torch.equal(c.of(scores_out, s, g), c.of(scores_clean, s, g))
+    q = c.q.clone()
+    rows = [7, n, n + 1 + 20, n + 1 + 50 + 1]               # a token of each request, with its first head of the last KV head
+    head = (nkv - 1) * G
+    for r in rows:
+        q[r, head * d] = math.nan
+    out, scores_out, _ = c.run(ops, q=q)
+    for t in range(q.shape[0]):
+        got, want = out[t].view(nq, d), clean[t].view(nq, d)
+        if t in rows:
+            assert torch.isnan(got[head].float()).all()
+            got, want = torch.cat([got[:head], got[head + 1:]]), torch.cat([want[:head], want[head + 1:]])
+        assert torch.equal(got, want)
+    for s, (r, L, new) in enumerate(zip((7, 0, 20, 1), c.lens, c.news)):
+        assert torch.isnan(c.of(scores_out, s, nkv - 1)[:L - new + r + 1]).all()           # every key that the query sees
