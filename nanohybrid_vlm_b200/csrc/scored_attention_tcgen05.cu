@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
   chunk_range(p.parts, n, G, total, key0, chunk, begin, end);
   if (begin >= end && p.parts.chunks > 1) return;
   // Rows of a stage behind a tile's last (groups that do not divide 128) are never copied to: zeros, whose weights the log-sum of +inf
-  // makes none.
+  // makes none.  A tile has more than 64 rows.
   for (int i = threadIdx.x; i < (BM - p.tokens * G) * 8 * DB * STAGES; i += C::THREADS) {
     const int block = i / ((BM - p.tokens * G) * 8), at = i - block * ((BM - p.tokens * G) * 8);
     *reinterpret_cast<uint4*>(q_s + block * (BM * 128) + p.tokens * G * 128 + at * 16) = make_uint4(0, 0, 0, 0);
@@ -833,6 +833,15 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
       tmem_ld_wait();
       tc_fence_before();
       mbar_arrive(&s_free[buf]);
+      if (half == 1 && tile_rows < BM) {                // the rows of zeros: a key that is not finite gives no number there
+        const int spare = tile_rows - 64;
+#pragma unroll
+        for (int k = 0; k < 64; k += 8) {
+          if (k + 8 <= spare) continue;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[k >> 5][(k & 31) + e] = k + e >= spare ? 0u : s[k >> 5][(k & 31) + e];
+        }
+      }
       if (CAP) {
         cap32(s[0], p.cap);
         cap32(s[1], p.cap);

@@ -612,3 +612,23 @@ def test_scores_that_are_no_numbers_stay_so_under_a_cap(ops, dtype, nq, nkv, d, 
         assert torch.equal(got, want)
     for s, (r, L, new) in enumerate(zip((7, 0, 20, 1), c.lens, c.news)):
         assert torch.isnan(c.of(scores_out, s, nkv - 1)[:L - new + r + 1]).all()           # every key that the query sees
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page", [(6, 2, 64, 64), (5, 1, 128, 16), (4, 1, 128, 64), (7, 7, 40, 8)])
+@pytest.mark.parametrize("news,lens", [([200, 3, 1], [700, 300, 65]), ([1, 2], [40, 90])])
+def test_keys_of_minus_infinity_weigh_nothing(ops, dtype, nq, nkv, d, page, news, lens):
+    """A key that every query's product with is minus infinity is a key of no weight, as one of -1e30 is."""
+    c = Case(news, lens, nq, nkv, d, page, dtype, seed=17)
+    c.q.view(-1, nq, d)[:, :, 3] = c.q.view(-1, nq, d)[:, :, 3].abs() + 0.5
+    got = []
+    for value in (-1e30, -math.inf):
+        for s, L in enumerate(lens):
+            for j in (5, L // 2, L - news[s]):              # the last one is the first new token's own
+                c.pages[int(c.table[s, j // page]), 0, :, j % page, 3] = value
+        got.append(c.run(ops))
+    assert not torch.isnan(got[0][0].float()).any()
+    assert torch.equal(got[0][0], got[1][0])
+    for s in range(len(lens)):
+        for g in range(nkv):
+            assert torch.equal(c.of(got[0][1], s, g), c.of(got[1][1], s, g))
