@@ -65,6 +65,13 @@ __device__ __forceinline__ float scored_exp2(float x) {     // 2^x; -inf gives 0
   return y;
 }
 
+// A pair of bfloat16 with what is not finite taken out; `bad` says whether there was any.
+__device__ __forceinline__ uint32_t finite_pair(uint32_t v, bool& bad) {
+  const bool lo = (v & 0x7f80u) == 0x7f80u, hi = (v & 0x7f800000u) == 0x7f800000u;
+  bad |= lo | hi;
+  return (lo ? 0u : v & 0xffffu) | (hi ? 0u : v & 0xffff0000u);
+}
+
 // Parts of the two passes: the keys of a request cut for the rows' pass (`splits`), its rows cut for the keys' pass (`chunks`).
 struct ScoredParts {
   float* o;                 // [splits][nkv][n_tokens * G][d], with splits > 1

@@ -22,7 +22,7 @@
 // instructions of the products and exponentials, with two blocks an SM to hide them: 120 us for 311 MB.
 //
 // A key out of sight may hold anything: its score is replaced, its value not loaded.  Where only some of a request's rows see a
-// key (several new tokens), the second product is made token by token with the values that the token sees.
+// key (several new tokens), what is not finite in the values is left out of the second product and given to the rows that see it.
 #include "nhv_scored.cuh"
 
 namespace {
@@ -319,6 +319,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
   const float scale_log2 = w.cap.in != 0.f ? 1.0f : a.scale * SA_LOG2E;
 
   const int step = 16 * SH_WARPS;
+  int odd_tile = -1;
   int j0 = RB > 0 ? begin + 16 * warp : end;      // a request that brings nothing keeps its scores
   int page = page_at(j0), off = BY16 ? j0 % a.page_size : 0;
   int page_next = page_at(j0 + step);
@@ -409,33 +410,18 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
     if (!edge || n == 1) {
       second_product(p);
     } else {
-      // token by token, with the values up to its own key
-      for (int tok = r0 / G; tok <= (r0 + RB - 1) / G; ++tok) {
-        const int hi_key = total - n + tok;
-        if (hi_key < j0) continue;                            // sees nothing of this tile
-        uint32_t own[NT][PARTS][2];
+      // some row does not see some key: what is not finite in the values comes behind the walk, to the rows that see it.  Such a tile
+      // touches the request's last 32 keys, so a warp, which takes every fourth, meets one at most.
+      bool odd = false;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const bool mine = (r0 + t * 8 + ra) / G == tok;
+      for (int h = 0; h < 4; ++h)
 #pragma unroll
-          for (int k = 0; k < PARTS; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) own[t][k][h] = mine ? p[t][k][h] : 0u;
+        for (int b = 0; b < DB; ++b) {
+          vr[h][b].x = finite_pair(vr[h][b].x, odd); vr[h][b].y = finite_pair(vr[h][b].y, odd);
+          vr[h][b].z = finite_pair(vr[h][b].z, odd); vr[h][b].w = finite_pair(vr[h][b].w, odd);
         }
-        uint4 all[4][DB];
-#pragma unroll
-        for (int h = 0; h < 4; ++h)
-#pragma unroll
-          for (int b = 0; b < DB; ++b) {
-            all[h][b] = vr[h][b];
-            if (j0 + 2 * rc + (h & 1) + 8 * (h >> 1) > hi_key) vr[h][b] = make_uint4(0, 0, 0, 0);
-          }
-        second_product(own);
-#pragma unroll
-        for (int h = 0; h < 4; ++h)
-#pragma unroll
-          for (int b = 0; b < DB; ++b) vr[h][b] = all[h][b];
-      }
+      if (__any_sync(0xffffffffu, odd)) odd_tile = j0;
+      second_product(p);
     }
     load_values(j0 + step, page, off);
   }
@@ -466,6 +452,22 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
           }
       }
     }
+  if (odd_tile >= 0) {
+    // the values left out above, to this warp's sums: an element of the head a lane
+    __syncwarp();
+    for (int j = odd_tile; j < min(odd_tile + 16, end); ++j) {
+      const int at = page_at(j), sees_from = max(0, (j - (total - n)) * G - r0);
+      for (int c = lane; c < d && at >= 0; c += 32) {
+        const float v = to_f32(pages[v_plane + (((size_t)at * 2 * a.nkv + kvh) * a.page_size + j % a.page_size) * d + c]);
+        if (fabsf(v) < INFINITY) continue;
+        for (int r = sees_from; r < RB; ++r) {
+          const float ref = sml[(warp * w.block_rows + r) * 2];
+          float& sum = so[(warp * w.block_rows + r) * row_len + c];
+          sum = fmaf(scored_exp2(kept[(size_t)j * w.rows + r] - (ref == -INFINITY ? 0.f : ref)), v, sum);
+        }
+      }
+    }
+  }
   __syncthreads();
   if (w.cluster) {
     finish_in_cluster<__nv_bfloat16>(w, smem, row_len, seq, kvh, first, n, total, begin, end);

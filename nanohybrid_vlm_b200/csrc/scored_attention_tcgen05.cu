@@ -181,12 +181,6 @@ __device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
 }
 // 256 threads meet.
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 256;\n" ::"r"(id) : "memory"); }
-// A pair of bfloat16 with what is not finite taken out; `bad` says whether there was any.
-__device__ __forceinline__ uint32_t finite_pair(uint32_t v, bool& bad) {
-  const bool lo = (v & 0x7f80u) == 0x7f80u, hi = (v & 0x7f800000u) == 0x7f800000u;
-  bad |= lo | hi;
-  return (lo ? 0u : v & 0xffffu) | (hi ? 0u : v & 0xffff0000u);
-}
 // 32 scores capped (see nhv_cap_tile): where a warp's are all small, two at a time by the polynomial.
 __device__ __forceinline__ void cap32(uint32_t (&sr)[32], const NhvScoreCap& c) {
   float m0 = 0.f, m1 = 0.f;

@@ -632,3 +632,26 @@ def test_keys_of_minus_infinity_weigh_nothing(ops, dtype, nq, nkv, d, page, news
     for s in range(len(lens)):
         for g in range(nkv):
             assert torch.equal(c.of(got[0][1], s, g), c.of(got[1][1], s, g))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page,n", [(4, 2, 128, 64, 8), (2, 2, 64, 8, 5), (20, 4, 96, 16, 6), (3, 1, 40, 24, 4), (2, 1, 256, 64, 4), (8, 1, 32, 256, 4)])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_values_of_later_tokens_do_not_reach_earlier_ones_among_few(ops, dtype, nq, nkv, d, page, n, what):
+    """The same for drafts: few tokens of several requests, the value of each of them no number in turn."""
+    c = Case([n, n, 1], [n + 150, n, 30], nq, nkv, d, page, dtype, seed=d)
+    clean, scores_clean, _ = c.run(ops)
+    for bad in range(n):
+        pages = c.pages.clone()
+        for s in (0, 1):
+            j = c.lens[s] - n + bad
+            c.pages[int(c.table[s, j // page]), 1, :, j % page] = what
+        out, scores_out, _ = c.run(ops)
+        c.pages = pages
+        for s in (0, 1):
+            assert torch.equal(out[s * n:s * n + bad], clean[s * n:s * n + bad])
+            assert not torch.isfinite(out[s * n + bad:(s + 1) * n].float()).any()
+        assert torch.equal(out[2 * n:], clean[2 * n:])
+        for s in range(3):
+            for g in range(nkv):
+                assert torch.equal(c.of(scores_out, s, g), c.of(scores_clean, s, g))
