@@ -8,9 +8,10 @@
 // product is free as long as both operands agree, so a lane takes 16 consecutive bytes of a row and its registers are the fragment
 // as they are.  For V^T two keys' elements have to share a register, which one byte permutation each does.  The next keys'
 // loads are sent as soon as the products have used the registers; the next tile's page is looked up one tile ahead.
-//   P goes into the second product as two bfloat16 parts, the rounded value and what the rounding left (an error of 2^-17 where
-//   one part has 2^-9): the tensor pipe is idle most of the time here.  With more than 16 rows it is not, and P has one part, as in the
-//   tcgen05 kernels.
+//   P goes into the second product as two bfloat16 parts, its first 8 bits and what they leave (an error of 2^-15 where one part
+//   has 2^-8): the tensor pipe is idle most of the time here.  Neither part is negative, and the second none only where P is: an
+//   infinite value times P is as infinite in parts as whole.  With more than 16 rows the pipe is not idle, and P has one part, as in
+//   the tcgen05 kernels.
 //   The running maximum moves only when it grows by more than 2^8, so that most tiles leave the sums as they are.
 //   The warps' sums meet in shared memory; the block leaves one partial sum (fp32) and the scores of its keys.
 // Second kernel, or the same blocks as a cluster where few suffice: the parts' sums are joined, a block per (request, KV head) for the output and blocks of keys for the weights: a
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
           }
         }
     }
-    uint32_t p[NT][PARTS][2];                      // [rounded, what that left][keys 0-7, 8-15]
+    uint32_t p[NT][PARTS][2];                      // [first bits, what they leave][keys 0-7, 8-15], or [rounded]
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -403,9 +404,13 @@ __global__ void __launch_bounds__(SH_THREADS, DB * NT <= 2 ? 3 : 2) scored_short
           x[e] = scored_exp2(s[t][2 * h + e] - (m[t][e] == -INFINITY ? 0.f : m[t][e]));
           l[t][e] += x[e];
         }
-        const uint32_t hi = pack2(x[0], x[1]);
-        p[t][0][h] = transposed(hi);
-        if (PARTS == 2) p[t][PARTS - 1][h] = transposed(pack2(x[0] - low_of(hi), x[1] - high_of(hi)));
+        if (PARTS == 2) {
+          const uint32_t hi = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x7632);
+          p[t][0][h] = transposed(hi);
+          p[t][PARTS - 1][h] = transposed(pack2(fmaxf(x[0] - low_of(hi), x[0] * 0x1p-20f), fmaxf(x[1] - high_of(hi), x[1] * 0x1p-20f)));
+        } else {
+          p[t][0][h] = transposed(pack2(x[0], x[1]));
+        }
       }
     if (!edge || n == 1) {
       second_product(p);

@@ -655,3 +655,25 @@ def test_values_of_later_tokens_do_not_reach_earlier_ones_among_few(ops, dtype, 
         for s in range(3):
             for g in range(nkv):
                 assert torch.equal(c.of(scores_out, s, g), c.of(scores_clean, s, g))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page", [(4, 2, 128, 64), (2, 2, 64, 16), (20, 1, 32, 8), (12, 2, 96, 64), (2, 1, 256, 64)])
+@pytest.mark.parametrize("lengths", ["single", "few", "prompts"])
+@pytest.mark.parametrize("what", [math.inf, -math.inf])
+def test_infinite_values_in_sight(ops, dtype, nq, nkv, d, page, lengths, what):
+    """One element of a value is infinite: so is that element of every output that sees it, and nothing else changes."""
+    c = Case(*LENGTHS[lengths], nq, nkv, d, page, dtype, seed=19, spread=0.5)
+    clean, scores_clean, _ = c.run(ops)
+    e, slots = d - 3, [L * 2 // 3 for L in c.lens]
+    for s, j in enumerate(slots):
+        c.pages[int(c.table[s, j // page]), 1, :, j % page, e] = what
+    out, scores_out, _ = c.run(ops)
+    for s, (n, L) in enumerate(zip(c.news, c.lens)):
+        for t in range(n):
+            got, want = out[c.cu[s] + t].view(nq, d), clean[c.cu[s] + t].view(nq, d).clone()
+            if slots[s] <= L - n + t:
+                want[:, e] = what
+            assert torch.equal(got, want), (s, t)
+        for g in range(nkv):
+            assert torch.equal(c.of(scores_out, s, g), c.of(scores_clean, s, g))
