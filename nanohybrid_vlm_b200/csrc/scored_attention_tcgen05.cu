@@ -181,15 +181,16 @@ __device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
 }
 // 256 threads meet.
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 256;\n" ::"r"(id) : "memory"); }
-// 32 scores capped (see nhv_cap_tile): where a warp's are all small, two at a time by the polynomial.
-__device__ __forceinline__ void cap32(uint32_t (&sr)[32], const NhvScoreCap& c) {
+// 32 scores capped (see nhv_cap_tile): where a warp's are all small, two at a time by the polynomial.  A lane that does not count has no
+// say in that, or the last bits of the others would go by what lies about in shared memory and in pages' unused slots.
+__device__ __forceinline__ void cap32(uint32_t (&sr)[32], const NhvScoreCap& c, bool counts) {
   float m0 = 0.f, m1 = 0.f;
 #pragma unroll
   for (int i = 0; i < 32; i += 4) {
     m0 = max3(m0, fabsf(__uint_as_float(sr[i])), fabsf(__uint_as_float(sr[i + 1])));
     m1 = max3(m1, fabsf(__uint_as_float(sr[i + 2])), fabsf(__uint_as_float(sr[i + 3])));
   }
-  if (__all_sync(0xffffffffu, fmaxf(m0, m1) <= c.small)) {
+  if (__all_sync(0xffffffffu, !counts || fmaxf(m0, m1) <= c.small)) {
     const f32x2 z2 = f2_pack(c.z, c.z), k0 = f2_pack(c.c[0], c.c[0]), k1 = f2_pack(c.c[1], c.c[1]), k2 = f2_pack(c.c[2], c.c[2]),
                 k3 = f2_pack(c.c[3], c.c[3]), k4 = f2_pack(c.c[4], c.c[4]);
 #pragma unroll
@@ -221,18 +222,23 @@ __device__ __noinline__ void change_scores(uint32_t s_addr, const NhvScoreCap& c
     uint32_t sr[32];
     tmem_ld32_nowait(sr, s_addr + c);
     tmem_ld_wait();
-    if (cap.in != 0.f) cap32(sr, cap);
+    uint32_t gone = 0;
     if (masked) {
-      uint32_t gone = 0;
       if (missing)
         for (int i = 0; i < 32; ++i) {
           const int page = table[min(key0 + c + i, total - 1) / page_size];
           if (page < 0 || page >= n_pages) gone |= 1u << i;
         }
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (key0 + c + i > row_hi || (gone >> i & 1u)) sr[i] = 0xFF800000u;
+      for (int i = 0; i < 32; ++i) gone |= key0 + c + i > row_hi ? 1u << i : 0u;
     }
+    if (cap.in != 0.f) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sr[i] = gone >> i & 1u ? 0u : sr[i];
+      cap32(sr, cap, true);
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) sr[i] = gone >> i & 1u ? 0xFF800000u : sr[i];
     tmem_st32(s_addr + c, sr);
   }
   tmem_st_wait();
@@ -570,7 +576,7 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
       tmem_ld_wait();
       if (CAP && !masked) {
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) cap32(sr[c], p.cap);
+        for (int c = 0; c < BN / 32; ++c) cap32(sr[c], p.cap, valid);
       }
       float mx0 = max3(__uint_as_float(sr[0][0]), __uint_as_float(sr[0][1]), __uint_as_float(sr[0][2]));
       float mx1 = max3(__uint_as_float(sr[0][3]), __uint_as_float(sr[0][4]), __uint_as_float(sr[0][5]));
@@ -722,7 +728,7 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
   chunk_range(p.parts, n, G, total, key0, chunk, begin, end);
   if (begin >= end && p.parts.chunks > 1) return;
   // Rows of a stage behind a tile's last (groups that do not divide 128) are never copied to: zeros, whose weights the log-sum of +inf
-  // makes none.  A tile has more than 64 rows.
+  // makes none.
   for (int i = threadIdx.x; i < (BM - p.tokens * G) * 8 * DB * STAGES; i += C::THREADS) {
     const int block = i / ((BM - p.tokens * G) * 8), at = i - block * ((BM - p.tokens * G) * 8);
     *reinterpret_cast<uint4*>(q_s + block * (BM * 128) + p.tokens * G * 128 + at * 16) = make_uint4(0, 0, 0, 0);
@@ -801,6 +807,7 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
   } else {
     // ------------------------------------------------------------------ two threads per key, for half of the columns each
     const int quarter = warp & 3, half = (warp - 2) >> 2, at = quarter * 32 + lane, key = key0 + at;
+    const bool counts = !CAP || (key < total && key_row(a, seq, key, kvh, 0) >= 0);
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const float* lse = a.lse + ((size_t)kvh * a.n_tokens + first) * G;
     const int rows = n * G, tile_rows = p.tokens * G;
@@ -827,18 +834,20 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
       tmem_ld_wait();
       tc_fence_before();
       mbar_arrive(&s_free[buf]);
-      if (half == 1 && tile_rows < BM) {                // the rows of zeros: a key that is not finite gives no number there
-        const int spare = tile_rows - 64;
+      // the rows of zeros: a key that is not finite gives no number there; under a cap those of the next request too, which are none of
+      // this one's business
+      const int own = (CAP ? min(tile_rows, rows - (begin + i) * tile_rows) : tile_rows) - half * 64;
+      if (CAP ? own < 64 : half == 1 && tile_rows < BM) {
 #pragma unroll
         for (int k = 0; k < 64; k += 8) {
-          if (k + 8 <= spare) continue;
+          if (k + 8 <= own) continue;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[k >> 5][(k & 31) + e] = k + e >= spare ? 0u : s[k >> 5][(k & 31) + e];
+          for (int e = 0; e < 8; ++e) s[k >> 5][(k & 31) + e] = k + e >= own ? 0u : s[k >> 5][(k & 31) + e];
         }
       }
       if (CAP) {
-        cap32(s[0], p.cap);
-        cap32(s[1], p.cap);
+        cap32(s[0], p.cap, counts);
+        cap32(s[1], p.cap, counts);
       }
       // rows behind the request's last and those that do not see every key of the tile
       const bool masked = key0 + BM - 1 > total - n + t_first || (begin + i + 1) * tile_rows > rows;
@@ -856,7 +865,7 @@ __global__ void __launch_bounds__(Keys<DB>::THREADS, DB <= 2 ? 2 : 1) scored_key
         }
       } else {
         // the first column that sees this key, and the first behind the rows
-        const int lo = (key - (total - n) - t_first) * G - half * 64, hi = min(tile_rows, rows - (begin + i) * tile_rows) - half * 64;
+        const int lo = (key - (total - n) - t_first) * G - half * 64, hi = CAP ? own : min(tile_rows, rows - (begin + i) * tile_rows) - half * 64;
         const float* lf = reinterpret_cast<const float*>(ls);
         float x = 0.f;
 #pragma unroll

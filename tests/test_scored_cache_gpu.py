@@ -677,3 +677,30 @@ def test_infinite_values_in_sight(ops, dtype, nq, nkv, d, page, lengths, what):
             assert torch.equal(got, want), (s, t)
         for g in range(nkv):
             assert torch.equal(c.of(scores_out, s, g), c.of(scores_clean, s, g))
+
+
+@pytest.mark.parametrize("nq,nkv,d,page", [(6, 2, 32, 8), (4, 2, 64, 64), (5, 1, 128, 16), (3, 1, 192, 64)])
+def test_capped_scores_do_not_depend_on_what_lies_about(ops, nq, nkv, d, page):
+    """Unused slots of the request's pages, entries without a page, the next request's queries and what the launch before left in shared
+    memory: none of it shows, not in the last bit either."""
+    c = Case([80, 3, 50, 1], [117, 30, 350, 70], nq, nkv, d, page, torch.bfloat16, cap=30.0, seed=d)
+    c.table[2, 1] = -1
+    before = Case([300], [300], nq, nkv, d, page, torch.bfloat16, cap=30.0, seed=1)
+    empty, results = torch.isnan(c.pages), []
+    for fill in (0.0, 5000.0):
+        c.pages[empty] = fill
+        before.q = torch.full_like(before.q, fill)
+        before.run(ops)
+        q = c.q.clone()
+        if fill:
+            q[83:133] *= 100                                # the third request's, behind those of the first two in a tile
+        results.append(c.run(ops, q=q))
+    (out, scores, _), (out2, scores2, _) = results
+    assert torch.equal(out[:83], out2[:83]) and torch.equal(out[133:], out2[133:])
+    for s in (0, 1, 3):
+        for g in range(nkv):
+            assert torch.equal(c.of(scores, s, g), c.of(scores2, s, g))
+    out3, scores3, _ = c.run(ops)
+    assert torch.equal(out3, out)
+    held = [j for j in range(350) if j // page != 1]
+    assert torch.equal(c.of(scores3, 2, 0)[held], c.of(scores, 2, 0)[held])
