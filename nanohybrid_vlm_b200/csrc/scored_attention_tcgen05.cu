@@ -632,10 +632,11 @@ __global__ void __launch_bounds__(Rows<DB>::THREADS, 1) scored_rows_tcgen05_kern
     if (ok && tiles_q > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_last[q], 0, 8));
     if (ok) {
       tc_fence_after();
-      // the notes on values: made before the products that o_full covers
+      // The notes on values: made before the products that o_full covers.  The other group may be noting keys that no row of this tile
+      // sees, so lanes may read different words; what follows is the whole warp's business and takes one decision.
       bool any_bad = false;
       for (int i = 0; i < 16; ++i) any_bad |= *(volatile uint32_t*)&s_bad[i] != 0;
-      if (any_bad && tiles_q > 0)
+      if (__any_sync(0xffffffffu, any_bad) && tiles_q > 0)
         return_values<DB, BN>(o_addr, a, s_bad, seq, kvh, kvh * G + g, first + token, key_begin + first_edge * BN, row_hi, m, p.scale_log2);
       const size_t row = (size_t)kvh * a.n_tokens * G + (size_t)(first + token) * G + g;
       const bool whole = p.parts.splits == 1;

@@ -704,3 +704,22 @@ def test_capped_scores_do_not_depend_on_what_lies_about(ops, nq, nkv, d, page):
     assert torch.equal(out3, out)
     held = [j for j in range(350) if j // page != 1]
     assert torch.equal(c.of(scores3, 2, 0)[held], c.of(scores, 2, 0)[held])
+
+
+@pytest.mark.parametrize("nq,nkv,d,page", [(4, 2, 128, 64), (6, 2, 64, 8), (1, 1, 32, 16), (8, 1, 256, 64)])
+@pytest.mark.parametrize("first", [0, 70])
+def test_odd_values_that_only_the_second_tile_of_a_block_sees(ops, nq, nkv, d, page, first):
+    """A block's two tiles of rows end at unlike keys: what the later one finds in its own last keys is its own business."""
+    n, old = 150, 90
+    c = Case([n, 2], [n + old, 64], nq, nkv, d, page, torch.bfloat16, seed=d)
+    clean, scores_clean, _ = c.run(ops)
+    for bad in range(first, n, 13):
+        pages = c.pages.clone()
+        for j in range(old + bad, old + n, 29):
+            c.pages[int(c.table[0, j // page]), 1, :, j % page] = math.nan if j % 2 else math.inf
+        out, scores_out, _ = c.run(ops)
+        c.pages = pages
+        assert torch.equal(out[:bad], clean[:bad]) and torch.equal(out[n:], clean[n:])
+        assert not torch.isfinite(out[bad:n].float()).any()
+        for g in range(nkv):
+            assert torch.equal(c.of(scores_out, 0, g), c.of(scores_clean, 0, g)) and torch.equal(c.of(scores_out, 1, g), c.of(scores_clean, 1, g))
