@@ -364,7 +364,7 @@ NHV_API int nhv_select_keys(int* sources, int* targets, const float* scores, con
   NHV_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && max_kv_len >= 0 && max_moves >= 0 && nkv <= 65535, "choice of keys: %d requests, %d keys, %d moves", n_seqs,
               max_kv_len, max_moves);
   NHV_REQUIRE(keep_first >= 0 && keep_recent >= 0, "choice of keys: kept first and recent keys are counted from 0");
-  if (n_seqs == 0 || max_moves == 0) return 0;
+  if (n_seqs == 0) return 0;                          // without room for moves the kernel still says whether some were needed
   ChoiceArgs a{scores, births, block_table, kv_len, seen, budgets, sources, targets, bt_stride, nkv, page_size, n_pages, max_moves,
                keep_first, keep_recent, max_kv_len};
   a.page_shift = -1;

@@ -723,3 +723,19 @@ def test_odd_values_that_only_the_second_tile_of_a_block_sees(ops, nq, nkv, d, p
         assert not torch.isfinite(out[bad:n].float()).any()
         for g in range(nkv):
             assert torch.equal(c.of(scores_out, 0, g), c.of(scores_clean, 0, g)) and torch.equal(c.of(scores_out, 1, g), c.of(scores_clean, 1, g))
+
+
+def test_no_room_at_all_for_moves(ops):
+    from nanohybrid_vlm_b200.kernels.library import KernelError
+    p = Pool([64, 10], 1, 16, seed=2)
+    p.random(False)
+    p.select(ops, [64, 10], [64, 10], 0, 0, room=0)         # nobody is over the budget
+    ops.raise_wait_errors()
+    p.select(ops, [64, 10], [0, 10], 0, 0, room=0)          # nothing stays: no moves either
+    ops.raise_wait_errors()
+    births = [torch.arange(n, dtype=torch.int32).view(1, -1) + 5 for n in (64, 10)]
+    p.fill([torch.arange(n).float().view(1, -1) for n in (64, 10)], births)     # the best keys stand last
+    p.select(ops, [64, 10], [63, 10], 0, 0, room=0)
+    with pytest.raises(KernelError, match="key_eviction"):
+        ops.raise_wait_errors()
+    ops.raise_wait_errors()
