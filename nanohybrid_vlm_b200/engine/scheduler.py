@@ -21,6 +21,10 @@ Policy, after nanovllm/engine/scheduler.py (queues :133-134, budget :544-547, po
   preempted: its pages go back, it returns to the tail of ``waiting`` and is later
   recomputed from its first token, generated tokens included.  If there is no other, the
   request preempts itself.
+* With a bounded cache (``cache_budget``) a request's keys are cut down to the budget when its prompt is done, if that is a page
+  above the budget or more, and then whenever it holds a page more.  A preempted request is computed again under the same rule: in
+  portions that end where its keys were cut before, so that its tokens see the keys that they saw, and it never needs more
+  pages than it did.  It is admitted with the pages up to the first cut and gets the others portion by portion.
 * A step that can schedule nothing raises: the engine would spin.
 """
 from __future__ import annotations
@@ -82,25 +86,39 @@ class Scheduler:
         if not strict_prefill:
             budget = self._schedule_decodes(plan, budget, scheduled)
 
-        while self.waiting and budget > 0 and len(plan.seqs) < self.max_num_seqs:
-            seq = self.waiting[0]
+        at, stuck = 0, False        # a request that waits for its keys to be dropped, or for a page behind that, lets others pass
+        while at < len(self.waiting) and budget > 0 and len(plan.seqs) < self.max_num_seqs:
+            seq = self.waiting[at]
+            upto = min(len(seq), self._next_cut(seq)) if self.cache_budget else len(seq)
             if seq.seq_id not in self.cache:
+                # one at a time is computed again from cut to cut, and while it waits for a page nobody takes one before it
+                if stuck or (at > 0 and upto < len(seq)):
+                    break
                 live = self.cache.num_live()
-                if live >= self.max_num_seqs or not self.cache.can_admit(seq.seq_id, seq.token_ids):
+                tokens = seq.token_ids if upto == len(seq) else seq.token_ids[:upto]
+                if live >= self.max_num_seqs or not self.cache.can_admit(seq.seq_id, tokens):
                     break
                 # leading pages that an earlier request left in the cache are shared, not computed again
-                seq.num_cached_tokens = self.cache.admit(seq.seq_id, seq.token_ids)
+                seq.num_cached_tokens = self.cache.admit(seq.seq_id, tokens)
+            elif seq.num_dropped_tokens:
+                slots = upto - seq.num_dropped_tokens
+                if not self.cache.can_allocate(seq.seq_id, slots):
+                    at, stuck = at + 1, True
+                    continue
+                self.cache.allocate(seq.seq_id, slots)
             remaining = len(seq) - seq.num_cached_tokens
-            n = min(remaining, budget, self.max_portion or remaining)
+            n = min(upto - seq.num_cached_tokens, budget, self.max_portion or remaining)
             seq.num_scheduled_tokens = n
             plan.seqs.append(seq)
             scheduled.add(seq.seq_id)
             plan.num_prefill_tokens += n
             budget -= n
             if n == remaining:
-                self.waiting.popleft()
+                del self.waiting[at]
                 seq.status = SequenceStatus.RUNNING
                 self.running.append(seq)
+            elif n == upto - seq.num_cached_tokens:
+                at += 1
             else:
                 break   # a prompt was cut: the budget (or the portion limit) is used up for this step
 
@@ -159,12 +177,16 @@ class Scheduler:
         plan.preempted_seq_ids.append(seq.seq_id)
 
     # ------------------------------------------------------------------ a bounded cache
+    def _next_cut(self, seq: Sequence) -> int:
+        """How many tokens of the request are cached when its keys are cut down to the budget the next time."""
+        full = self.cache_budget + self.cache.page_size
+        return seq.num_dropped_tokens + full if seq.num_dropped_tokens else max(seq.num_prompt_tokens, full)
+
     def over_budget(self, seqs: list[Sequence]) -> list[Sequence]:
         """Those of the requests that hold a page more than the cache's budget and will go on: their keys are to be dropped."""
         if not self.cache_budget:
             return []
-        return [s for s in seqs if s.status == SequenceStatus.RUNNING and not s.finishing
-                and s.num_kept_tokens >= self.cache_budget + self.cache.page_size]
+        return [s for s in seqs if not s.is_finished and not s.finishing and s.num_cached_tokens >= self._next_cut(s)]
 
     def dropped(self, seq: Sequence) -> None:
         """The request's keys have been cut down to the budget."""

@@ -163,3 +163,38 @@ def test_models_that_cannot_drop_keys_say_so(tmp_path):
     write_model(str(tmp_path), KIL_A, 0)
     with pytest.raises(ValueError, match="cache_budget"):
         LLM(str(tmp_path), dtype="float32", cache_budget=32, num_kvcache_blocks=16, max_num_seqs=2, max_model_len=64)
+
+
+@pytest.mark.parametrize("name,lengths,new,budget,first,recent,pages", [("A", (40, 50, 30), 70, 40, 2, 8, 9), ("B", (20, 33, 9, 41), 60, 20, 1, 5, 10)])
+def test_preempted_requests_keep_what_they_kept(name, lengths, new, budget, first, recent, pages, model_dirs, plain_models):
+    """Requests that give way and are computed again hold the same keys behind it as the plain model, which nobody interrupts."""
+    from nanohybrid_vlm_b200 import SamplingParams
+    page = 16 if name == "A" else 8
+    prompts = prompts_for(name, lengths, seed=11)
+    llm = make_llm(model_dirs[name], name, cache_budget=budget, cache_first=first, cache_recent=recent, max_num_batched_tokens=64, num_kvcache_blocks=pages)
+    ids = [llm.add_request(p, SamplingParams(temperature=0.0, max_tokens=new, ignore_eos=True)) for p in prompts]
+    plains = {i: PlainBounded(plain_models[name], budget, page, first, recent) for i in ids}
+    fed, outputs = {i: list(p) for i, p in zip(ids, prompts)}, {}
+    live = {i: s for i, s in zip(ids, llm.scheduler.waiting)}
+    after_preemption = 0
+    while not llm.is_finished():
+        outputs.update(llm.step()[0])
+        for i in [i for i in llm.last_sampled_ids if i in plains]:
+            lg = plains[i].step(fed[i])
+            token = outputs[i][-1] if i in outputs else live[i].token_ids[-1]
+            assert lg[token] >= lg.max() - 2e-4, (i, len(live[i]), float(lg.max() - lg[token]))
+            fed[i] = [token]
+            if plains[i].cut() < 1e-4:                      # so close that rounding decides: the two may part here
+                del plains[i]
+            if i in outputs or i not in plains:
+                continue
+            kept = len(plains[i].heads[0][0])
+            births, scores = held_by_engine(llm, i, kept)
+            assert live[i].num_kept_tokens == kept and births == plains[i].births()
+            for a, b in zip(scores, plains[i].heads):
+                want = torch.tensor([[x[3] for x in kv] for kv in b], dtype=torch.float64)
+                assert torch.allclose(a.cpu().double().sort(1).values, want.sort(1).values, rtol=1e-3, atol=1e-6)
+            after_preemption += live[i].num_preemptions > 0 and live[i].num_dropped_tokens > page
+    assert llm.scheduler.num_preemptions > 0 and after_preemption > 20
+    assert all(len(outputs[i]) == new for i in ids)
+    llm.model_runner.cache.check()
