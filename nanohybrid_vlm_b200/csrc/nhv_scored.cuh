@@ -115,6 +115,8 @@ ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, i
 int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* work, cudaStream_t stream);
 
 // ---- requests with many rows, bfloat16 (scored_attention_tcgen05.cu)
-bool scored_long_takes(int dtype, int nq, int nkv, int d, int page_size, float scale);
+bool scored_long_takes(int dtype, int nq, int nkv, int d, int page_size, int q_stride, float scale);
 size_t scored_long_plan(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d);     // floats of scratch
+// Whether the pool's rows fit a copy's 32-bit coordinate and the tiles the grid.
+bool scored_long_reaches(const ScoredParts& p, int n_seqs, int n_tokens, int nq, int nkv, int d, int page_size, int n_pages);
 int scored_long_launch(ScoredArgs a, const ScoredParts& p, cudaStream_t stream);

@@ -656,7 +656,7 @@ struct ScoredPlan {
 };
 
 static ScoredPlan scored_plan(int dtype, bool wide, int n_seqs, int n_tokens, int min_new, int max_new, int max_keys, int nq, int nkv, int d,
-                              int page_size, float scale) {
+                              int page_size, int n_pages, int q_stride, float scale) {
   ScoredPlan p = {};
   p.wide = wide && d % (dtype == NHV_F32 ? 4 : 8) == 0;
   p.short_rows = -1;
@@ -670,9 +670,12 @@ static ScoredPlan scored_plan(int dtype, bool wide, int n_seqs, int n_tokens, in
   }
   p.rest = p.short_rows < 0 || max_new > most || max_new * G > most;
   if (p.rest) {
-    p.many = p.wide && scored_long_takes(dtype, nq, nkv, d, page_size, scale);
-    rest = p.many ? scored_long_plan(p.parts, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d)
-                  : tile_parts(p.parts, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d);
+    p.many = p.wide && scored_long_takes(dtype, nq, nkv, d, page_size, q_stride, scale);
+    if (p.many) {
+      rest = scored_long_plan(p.parts, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d);
+      p.many = scored_long_reaches(p.parts, n_seqs, n_tokens, nq, nkv, d, page_size, n_pages);
+    }
+    if (!p.many) rest = tile_parts(p.parts, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d);
   }
   p.floats = ((size_t)n_tokens * nq + 3) / 4 * 4 + (few > rest ? few : rest);       // one after the other in the same scratch
   return p;
@@ -701,7 +704,7 @@ struct NhvScoredCall {
 
 static ScoredPlan scored_plan(const NhvScoredCall& c) {
   return scored_plan(c.dtype, scored_wide(c.q, c.q_stride, c.out, c.out_stride, c.kv_pages), c.n_seqs, c.n_tokens, c.min_new, c.max_new, c.max_kv_len,
-                     c.nq, c.nkv, c.d, c.page_size, c.scale);
+                     c.nq, c.nkv, c.d, c.page_size, c.n_pages, c.q_stride, c.scale);
 }
 
 // Kilobytes of scratch that nhv_attention_scored wants for these arguments.
@@ -729,19 +732,27 @@ NHV_API int nhv_attention_scored(const NhvScoredCall* c, float* work, int work_k
   ScoredArgs a{c->q, c->out, c->kv_pages, c->scores, c->scores_out, c->births, c->positions, c->block_table, c->cu_q, c->kv_len, c->sinks, work,
                c->q_stride, c->out_stride, c->bt_stride, n_seqs, n_tokens, nq, nkv, d, c->page_size, c->n_pages, max_kv_len, 0, 0x7fffffff, c->scale, c->softcap};
   float* scratch = work + ((size_t)n_tokens * nq + 3) / 4 * 4;
-  if (plan.short_rows >= 0) {
-    a.max_rows = plan.short_rows;
-    const int rc = scored_short_launch(dtype, a, plan.few, scratch, stream);
-    if (rc || !plan.rest) return rc;
+  // The requests of many rows first: whatever can be refused is refused before anything is launched, or scores in place would hold some
+  // requests' weights already.
+  if (plan.rest) {
     a.min_rows = plan.short_rows + 1;
-    a.max_rows = 0x7fffffff;
+    scored_place(plan.parts, scratch, n_tokens, nq, d);
+    int rc;
+    if (plan.many) {
+      rc = scored_long_launch(a, plan.parts, stream);
+    } else {
+      const TileArgs t{a, plan.parts, d % 4 == 0 && c->q_stride % 4 == 0 && (uintptr_t)c->q % 16 == 0 && (uintptr_t)c->kv_pages % 16 == 0,
+                       c->out_stride % 4 == 0 && (uintptr_t)c->out % 16 == 0};
+      const int db = d <= 64 ? 1 : d <= 128 ? 2 : 4;
+      if (dtype == NHV_BF16)
+        rc = db == 1 ? launch_tiles<__nv_bfloat16, 1>(t, stream) : db == 2 ? launch_tiles<__nv_bfloat16, 2>(t, stream) : launch_tiles<__nv_bfloat16, 4>(t, stream);
+      else
+        rc = db == 1 ? launch_tiles<float, 1>(t, stream) : db == 2 ? launch_tiles<float, 2>(t, stream) : launch_tiles<float, 4>(t, stream);
+    }
+    if (rc) return rc;
   }
-  scored_place(plan.parts, scratch, n_tokens, nq, d);
-  if (plan.many) return scored_long_launch(a, plan.parts, stream);
-  const TileArgs t{a, plan.parts, d % 4 == 0 && c->q_stride % 4 == 0 && (uintptr_t)c->q % 16 == 0 && (uintptr_t)c->kv_pages % 16 == 0,
-                   c->out_stride % 4 == 0 && (uintptr_t)c->out % 16 == 0};
-  const int db = d <= 64 ? 1 : d <= 128 ? 2 : 4;
-  if (dtype == NHV_BF16)
-    return db == 1 ? launch_tiles<__nv_bfloat16, 1>(t, stream) : db == 2 ? launch_tiles<__nv_bfloat16, 2>(t, stream) : launch_tiles<__nv_bfloat16, 4>(t, stream);
-  return db == 1 ? launch_tiles<float, 1>(t, stream) : db == 2 ? launch_tiles<float, 2>(t, stream) : launch_tiles<float, 4>(t, stream);
+  if (plan.short_rows < 0) return 0;
+  a.min_rows = 0;
+  a.max_rows = plan.short_rows;
+  return scored_short_launch(dtype, a, plan.few, scratch, stream);
 }

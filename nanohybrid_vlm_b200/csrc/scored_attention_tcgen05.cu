@@ -923,8 +923,16 @@ int launch_long(const LongArgs& p, int row_tiles, cudaStream_t stream) {
 NHV_API int nhv_scored_tcgen05_error() { return nhv_wait_error_take(); }
 NHV_API void* nhv_scored_tcgen05_error_word() { return nhv_wait_error_address(); }
 
-bool scored_long_takes(int dtype, int nq, int nkv, int d, int page_size, float scale) {
-  return scale > 0.f && dtype == NHV_BF16 && d % 8 == 0 && d <= SA_MAX_D && nq / nkv <= BM && page_size % 8 == 0;
+// Tiles of rows in the grid: at most one that is not full a request.
+static long long long_row_tiles(int n_seqs, int n_tokens, int G, int d) { return (long long)n_tokens / ((d <= 128 ? 2 : 1) * (BM / G)) + n_seqs; }
+
+bool scored_long_takes(int dtype, int nq, int nkv, int d, int page_size, int q_stride, float scale) {
+  return scale > 0.f && dtype == NHV_BF16 && d % 8 == 0 && d <= SA_MAX_D && nq / nkv <= BM && page_size % 8 == 0 && q_stride > 0;
+}
+
+bool scored_long_reaches(const ScoredParts& p, int n_seqs, int n_tokens, int nq, int nkv, int d, int page_size, int n_pages) {
+  const long long pool = (long long)n_pages * 2 * nkv * page_size, key_tiles = (long long)(p.keys / BM) * p.chunks;
+  return pool < (1LL << 31) && key_tiles <= 65535 && long_row_tiles(n_seqs, n_tokens, nq / nkv, d) <= 65535;
 }
 
 size_t scored_long_plan(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
@@ -942,15 +950,12 @@ int scored_long_launch(ScoredArgs a, const ScoredParts& parts, cudaStream_t stre
   p.parts = parts;
   p.tokens = BM / (a.nq / a.nkv);
   p.key_tiles = (int)(parts.keys / BM);
-  const int db = (a.d + 63) / 64, nq_tiles = db <= 2 ? 2 : 1;
+  const int db = (a.d + 63) / 64;
   p.box = divisor(a.page_size, 64);
-  const long long pool = (long long)a.n_pages * 2 * a.nkv * a.page_size;
-  NHV_REQUIRE(pool < (1LL << 31), "scored attention (tcgen05): the pool's %lld rows are beyond a 32-bit coordinate", pool);
-  NHV_REQUIRE(nhv_make_map_bf16(&p.kv_map, a.pages, pool, a.d, a.d, 64, p.box), "scored attention (tcgen05): cannot encode the tensor map of the pool");
+  NHV_REQUIRE(nhv_make_map_bf16(&p.kv_map, a.pages, (long long)a.n_pages * 2 * a.nkv * a.page_size, a.d, a.d, 64, p.box),
+              "scored attention (tcgen05): cannot encode the tensor map of the pool");
   NHV_REQUIRE(make_q_map(&p.q_map, a, p.tokens), "scored attention (tcgen05): cannot encode the tensor map of q");
-  const long long row_tiles = (long long)a.n_tokens / (nq_tiles * p.tokens) + a.n_seqs;
-  NHV_REQUIRE(row_tiles <= 65535 && (long long)p.key_tiles * parts.chunks <= 65535, "scored attention (tcgen05): %lld tiles of rows, %d of keys in %d chunks are beyond the grid's reach",
-              row_tiles, p.key_tiles, parts.chunks);
+  const long long row_tiles = long_row_tiles(a.n_seqs, a.n_tokens, a.nq / a.nkv, a.d);
   const bool cap = a.softcap > 0.f;
   switch (db) {
     case 1: return cap ? launch_long<1, true>(p, (int)row_tiles, stream) : launch_long<1, false>(p, (int)row_tiles, stream);

@@ -739,3 +739,57 @@ def test_no_room_at_all_for_moves(ops):
     with pytest.raises(KernelError, match="key_eviction"):
         ops.raise_wait_errors()
     ops.raise_wait_errors()
+
+
+# ---------------------------------------------------------------- sizes beyond what the tcgen05 kernels reach
+def test_a_pool_of_more_rows_than_a_32_bit_coordinate_reaches(ops):
+    """bfloat16 heads of 8: the pool's rows pass 2^31.  A request of many rows beside one of few, scores in place."""
+    c = Case([24, 1], [90, 70], 4, 2, 8, 64, torch.bfloat16, seed=21)
+    n_pages = 2 ** 31 // (2 * 2 * 64) + 5
+    shift = n_pages - c.n_pages
+    where = torch.tensor([i if i % 2 else i + shift for i in range(c.n_pages)])
+    pages = torch.empty(n_pages, *c.pages.shape[1:], dtype=torch.bfloat16, device="cuda")
+    scores, births = torch.empty(n_pages, 2, 64, device="cuda"), torch.empty(n_pages, 2, 64, dtype=torch.int32, device="cuda")
+    pages[where], scores[where], births[where] = c.pages.cuda(), c.scores.cuda(), c.births.cuda()
+    table = torch.where(c.table >= 0, where[c.table.long().clamp(min=0)].int(), c.table).cuda()
+    out = torch.full_like(c.q, math.nan).cuda()
+    ops.attention_scored(out, c.q.cuda(), pages, scores, table, c.cu_t, c.lens_t, 2, 1, 24, 90, 4, 2, 8, c.scale, births=births,
+                         positions=i32(c.positions))
+    ops.raise_wait_errors()
+    c.check(out.cpu(), scores[where].cpu(), births[where].cpu())
+
+
+def test_more_tiles_of_rows_than_a_grid_has_places(ops):
+    """53,000 requests of one token with 64 query heads: more tiles of rows than the tcgen05 kernels' grid has."""
+    S, nq, d, page, L = 53000, 64, 8, 8, 3
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(S, nq * d, generator=g, device="cuda").bfloat16()
+    pages = torch.randn(S, 2, 1, page, d, generator=g, device="cuda").bfloat16()
+    scores = torch.rand(S, 1, page, generator=g, device="cuda")
+    table = torch.randperm(S, generator=g, device="cuda").int().view(S, 1)
+    out, after = torch.empty_like(q), torch.zeros_like(scores)
+    ops.attention_scored(out, q, pages, scores, table, torch.arange(S + 1, dtype=torch.int32, device="cuda"),
+                         torch.full((S,), L, dtype=torch.int32, device="cuda"), S, 1, 1, L, nq, 1, d, d ** -0.5, scores_out=after)
+    ops.raise_wait_errors()
+    at = table[:, 0].long()
+    k, v = pages[at, 0, 0, :L].double(), pages[at, 1, 0, :L].double()
+    p = torch.softmax(q.view(S, nq, d).double() @ k.transpose(1, 2) * d ** -0.5, -1)
+    unit = 2 * 2 ** -8 + 2 ** -15                           # the weights and the output, each rounded once; the 32-bit sums
+    assert ((out.view(S, nq, d).double() - p @ v).abs() <= p @ v.abs() * unit).all()
+    old = scores[at, 0, :L].double()
+    old[:, L - 1:] = 0
+    assert torch.allclose(after[at, 0, :L].double(), old + p.sum(1), rtol=2 ** -15, atol=0)
+    assert (after[:, :, L:] == 0).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_queries_that_are_one_row_for_all_tokens(ops, new):
+    """q with rows no distance apart: what no copy by tiles can describe is done without it."""
+    c = Case([new, 1], [90, 70], 4, 2, 64, 64, torch.bfloat16, seed=23)
+    c.q[:] = c.q[:1].clone()
+    first, second = c.q[:1].cuda().expand(c.q.shape[0], -1), torch.full_like(c.q, math.nan).cuda()
+    scores, births = c.scores.cuda(), c.births.cuda()
+    ops.attention_scored(second, first, c.pages.cuda(), scores, c.table.cuda(), c.cu_t, c.lens_t, 2, 1, new, 90, 4, 2, 64, c.scale, births=births,
+                         positions=i32(c.positions))
+    ops.raise_wait_errors()
+    c.check(second.cpu(), scores.cpu(), births.cpu())
