@@ -6,6 +6,8 @@
 
 constexpr float SA_LOG2E = 1.4426950408889634f;
 constexpr int SA_MAX_D = 256;
+constexpr int SA_MOST_SPLITS = 32;                        // parts of a request's keys in the rows' pass
+constexpr size_t SA_MOST_SUMS = (size_t)1 << 28;          // floats of their sums (1 GiB)
 
 struct ScoredArgs {
   const void* q;
@@ -92,6 +94,8 @@ __device__ __forceinline__ void chunk_range(const ScoredParts& p, int n, int G, 
 // about `tile_cycles` for one of each; blocks that run at once in either pass.
 size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d, int row_tile, int key_tile,
                     double tile_cycles, int rows_at_once, int keys_at_once);
+// The most scratch of any call of up to so many requests and tokens, and keys of a request.
+size_t scored_most_parts(int n_seqs, int n_tokens, int max_keys, int nq, int nkv, int d, int tile_rows, int tile_keys, int keys_at_once);
 void scored_place(ScoredParts& p, float* work, int n_tokens, int nq, int d);
 int scored_join_rows(int dtype, const ScoredArgs& a, const ScoredParts& p, cudaStream_t stream);
 int scored_join_keys(const ScoredArgs& a, const ScoredParts& p, cudaStream_t stream);
@@ -111,12 +115,14 @@ struct ShortPlan {
 int scored_short_rows(int dtype, int d);
 bool scored_short_takes(int dtype, int rows, int d);
 ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, int nkv, int d);
+size_t scored_short_most(int dtype, int n_seqs, int max_keys, int G, int nkv, int d);      // floats, for any call of up to these sizes
 // The requests with a.min_rows to a.max_rows rows: output, scores and births.  `work`: plan.floats floats.
 int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* work, cudaStream_t stream);
 
 // ---- requests with many rows, bfloat16 (scored_attention_tcgen05.cu)
 bool scored_long_takes(int dtype, int nq, int nkv, int d, int page_size, int q_stride, float scale);
 size_t scored_long_plan(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d);     // floats of scratch
+size_t scored_long_most(int n_seqs, int n_tokens, int max_keys, int nq, int nkv, int d);
 // Whether the pool's rows fit a copy's 32-bit coordinate and the tiles the grid.
 bool scored_long_reaches(const ScoredParts& p, int n_seqs, int n_tokens, int nq, int nkv, int d, int page_size, int n_pages);
 int scored_long_launch(ScoredArgs a, const ScoredParts& p, cudaStream_t stream);

@@ -576,10 +576,12 @@ int launch_tiles(const TileArgs& t, cudaStream_t stream) {
   return scored_join_keys(a, t.p, stream);
 }
 
+int tiles_at_once(int d) { return d <= 128 ? 3 * 148 : 148; }
+
 size_t tile_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int max_keys, int nq, int nkv, int d) {
   p.tile_rows = SA_ROWS;
   p.tile_keys = KEYS_KEYS;
-  const int at_once = d <= 128 ? 3 * 148 : 148;
+  const int at_once = tiles_at_once(d);
   return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, SA_ROWS, ROWS_KEYS, SA_ROWS * ROWS_KEYS * d / 30.0, at_once, at_once);
 }
 
@@ -591,14 +593,14 @@ size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int m
   // the rows' pass: parts of the keys where whole walks fill the SMs badly.  With `blocks` walks and `at_once` places, s parts take
   // one s-th of a walk where all run at once, else the work's share and half a part more for the last ones to end; each part's sums
   // are written and read once, 8 bytes an element at some 30 bytes a cycle.  One request's walks are alike but for the causal edge, and
-  // come in whole rounds.  No part is below `least` tiles.
+  // come in whole rounds.  No part is below `least` tiles, and the sums of all parts fit 1 GiB.
   const long long blocks = ((long long)n_tokens * G / row_tile + n_seqs) * nkv;        // at most
   const int tiles = (max_keys + key_tile - 1) / key_tile, least = key_tile * row_tile >= 128 * 128 ? 8 : 3;
   const bool alike = n_seqs == 1 && max_keys >= 2 * max_new;
   int splits = 1;
   double best = 1e30;
   const double sums = row_tile * d * 8 / 30.0 / (tile_cycles * tiles);
-  for (int s = 1; s <= 32 && (s == 1 || tiles / s >= least); ++s) {
+  for (int s = 1; s <= SA_MOST_SPLITS && (s == 1 || (tiles / s >= least && s * ((size_t)n_tokens * nq * (d + 2)) <= SA_MOST_SUMS)); ++s) {
     const double waves = alike || blocks * s <= rows_at_once ? (double)((blocks * s + rows_at_once - 1) / rows_at_once) : (double)blocks * s / rows_at_once + 0.5;
     const double cost = waves / s + (s > 1 ? s * sums : 0.0);
     if (cost < best - 1e-9) {
@@ -621,6 +623,14 @@ size_t scored_parts(ScoredParts& p, int n_seqs, int n_tokens, int max_new, int m
   p.keys = (size_t)key_tiles * p.tile_keys;
   const size_t rows = (size_t)n_tokens * nq;
   return (p.splits > 1 ? p.splits * rows * (d + 2) : 0) + (p.chunks > 1 ? (size_t)n_seqs * nkv * p.chunks * p.keys : 0) + 8;
+}
+
+// Of the rows' pass what the plan allows.  Of the keys' pass: a chunk has at least 8/9 of its share of the pairs of tiles, so a (request, KV
+// head) has at most 9/8 2 keys_at_once / (key tiles x KV heads) chunks and one that is not full, of so many keys each.
+size_t scored_most_parts(int n_seqs, int n_tokens, int max_keys, int nq, int nkv, int d, int tile_rows, int tile_keys, int keys_at_once) {
+  const size_t sums = SA_MOST_SPLITS * ((size_t)n_tokens * nq * (d + 2)), keys = ((size_t)max_keys + tile_keys - 1) / tile_keys * tile_keys;
+  const bool chunks = ((long long)n_tokens * (nq / nkv) + tile_rows - 1) / tile_rows > 8;
+  return (sums < SA_MOST_SUMS ? sums : SA_MOST_SUMS) + (chunks ? n_seqs * ((size_t)keys_at_once * 9 / 4 * tile_keys + nkv * keys) : 0) + 8;
 }
 
 void scored_place(ScoredParts& p, float* work, int n_tokens, int nq, int d) {
@@ -711,6 +721,19 @@ static ScoredPlan scored_plan(const NhvScoredCall& c) {
 NHV_API int nhv_attention_scored_kilobytes(const NhvScoredCall* c) {
   if (c->n_seqs <= 0 || c->nkv <= 0 || c->nq < c->nkv || c->d <= 0 || c->page_size <= 0 || c->max_kv_len <= 0) return 0;
   return (int)(scored_plan(*c).floats * sizeof(float) / 1024 + 1);
+}
+
+// The most of any call of up to c->n_seqs requests with c->n_tokens new tokens in all and c->max_kv_len keys each.
+NHV_API int nhv_attention_scored_most_kilobytes(const NhvScoredCall* c) {
+  if (c->n_seqs <= 0 || c->nkv <= 0 || c->nq < c->nkv || c->d <= 0 || c->page_size <= 0 || c->max_kv_len <= 0) return 0;
+  size_t most = scored_short_most(c->dtype, c->n_seqs, c->max_kv_len, c->nq / c->nkv, c->nkv, c->d);
+  const size_t tiles = scored_most_parts(c->n_seqs, c->n_tokens, c->max_kv_len, c->nq, c->nkv, c->d, SA_ROWS, KEYS_KEYS, tiles_at_once(c->d));
+  if (tiles > most) most = tiles;
+  if (c->nq / c->nkv <= 128) {
+    const size_t rows = scored_long_most(c->n_seqs, c->n_tokens, c->max_kv_len, c->nq, c->nkv, c->d);
+    if (rows > most) most = rows;
+  }
+  return (int)((((size_t)c->n_tokens * c->nq + 3) / 4 * 4 + most) * sizeof(float) / 1024 + 1);
 }
 
 NHV_API int nhv_attention_scored(const NhvScoredCall* c, float* work, int work_kilobytes, cudaStream_t stream) {

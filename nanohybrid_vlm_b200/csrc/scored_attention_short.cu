@@ -899,13 +899,22 @@ ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, i
     }
   }
   p.smem = sizeof(float) * short_sums(p.block_rows, d);
-  p.keys = (size_t)p.splits * p.split_keys;
+  p.keys = ((size_t)max_keys + 63) / 64 * 64;
   const size_t per_request = (size_t)nkv * p.rows * (p.keys + (size_t)p.splits * (d + 2));
   p.group = (int)(SH_MOST_SCORES / per_request);
   if (p.group < 1) p.group = 1;
   if (p.group > n_seqs) p.group = n_seqs;
   p.floats = per_request * p.group;
   return p;
+}
+
+// A request has at most 4 blocks that run at once / (requests x KV heads) parts and one that is not full.
+size_t scored_short_most(int dtype, int n_seqs, int max_keys, int G, int nkv, int d) {
+  const int rows = scored_short_rows(dtype, d);
+  if (!scored_short_takes(dtype, G, d)) return 0;
+  auto sum = [&](size_t n) { return n * nkv * rows * (((size_t)max_keys + 63) / 64 * 64) + (4 * 3 * 148 + n * nkv) * rows * (d + 2); };
+  const size_t one = sum(1) > SH_MOST_SCORES ? sum(1) : SH_MOST_SCORES, all = sum(n_seqs);
+  return all < one ? all : one;
 }
 
 int scored_short_launch(int dtype, ScoredArgs a, const ShortPlan& plan, float* work, cudaStream_t stream) {

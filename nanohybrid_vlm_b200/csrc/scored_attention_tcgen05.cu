@@ -942,6 +942,11 @@ size_t scored_long_plan(ScoredParts& p, int n_seqs, int n_tokens, int max_new, i
   return scored_parts(p, n_seqs, n_tokens, max_new, max_keys, nq, nkv, d, (d <= 128 ? 2 : 1) * tokens * G, 64, 1400.0, SMS, 2 * SMS);
 }
 
+size_t scored_long_most(int n_seqs, int n_tokens, int max_keys, int nq, int nkv, int d) {
+  const int G = nq / nkv;
+  return scored_most_parts(n_seqs, n_tokens, max_keys, nq, nkv, d, BM / G * G, BM, 2 * SMS);
+}
+
 int scored_long_launch(ScoredArgs a, const ScoredParts& parts, cudaStream_t stream) {
   LongArgs p;
   p.a = a;

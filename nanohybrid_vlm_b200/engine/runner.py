@@ -126,7 +126,7 @@ class ModelRunner:
         requests = min(T, self.config.max_num_seqs)
         scored = 0
         if self.config.cache_budget:
-            scored = max(self.model.blocks[run.layer].cache_owner.scored_scratch_bytes(T, requests, self.config.max_model_len, self.page_size)
+            scored = max(self.model.blocks[run.layer].cache_owner.scored_scratch_bytes(T, requests, self.config.max_model_len)
                          for run in self.model.spec.order)
         return 2 * T * per_token + 2 * logits + (256 << 20) + self.model.scratch_bytes(T, requests) + scored
 

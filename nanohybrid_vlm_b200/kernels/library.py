@@ -88,6 +88,7 @@ _SIGNATURES = {
     "nhv_embed_rmsnorm": [I, P, P, P, P, I, I, I, F, F, P],
     "nhv_attention_scored": [ctypes.c_char_p, P, I, P],
     "nhv_attention_scored_kilobytes": [ctypes.c_char_p],
+    "nhv_attention_scored_most_kilobytes": [ctypes.c_char_p],
     "nhv_select_keys": [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, P],
     "nhv_move_keys": [P, P, P, P, I, I, P, P, I, I, I, I, I, I, P],
     "nhv_decay_lowrank": [I, P, P, I, P, P, I, I, I, P],

@@ -1293,6 +1293,13 @@ def attention_scored_scratch_bytes(dtype, n_seqs: int, n_tokens: int, min_new: i
     return 1024 * library.load_library().nhv_attention_scored_kilobytes(given)
 
 
+def attention_scored_most_scratch_bytes(dtype, n_seqs: int, n_tokens: int, max_kv_len: int, nq: int, nkv: int, head_dim: int) -> int:
+    """A bound on the scratch of every call of ``attention_scored`` with up to so many requests, new tokens in all and keys of a request."""
+    given = _SCORED_CALL.pack(*[0] * 11, BF16 if dtype is torch.bfloat16 else F32, nq * head_dim, nq * head_dim, 0, n_seqs, n_tokens, 0, n_tokens,
+                              max_kv_len, nq, nkv, head_dim, 1, 1, 1.0, 0.0)
+    return 1024 * library.load_library().nhv_attention_scored_most_kilobytes(given)
+
+
 def select_keys(sources, targets, scores, births, block_table, kv_len, seen, budgets, n_seqs: int, max_kv_len: int, keep_first: int,
                 keep_recent: int) -> None:
     """Which keys leave a cache that is to hold ``budgets[i]`` keys of request i, said as moves that close the gaps.

@@ -83,12 +83,9 @@ class GQAttention(Mixer):
 
     scores_keys = True
 
-    def scored_scratch_bytes(self, tokens: int, requests: int, keys: int, page_size: int) -> int:
+    def scored_scratch_bytes(self, tokens: int, requests: int, keys: int) -> int:
         """The most that attention with scored keys takes in a step of up to so many tokens, requests and keys of a request."""
-        longest = min(tokens, keys)
-        return max(ops.attention_scored_scratch_bytes(self.env.dtype, requests, min(tokens, requests), 1, 1, keys, self.nq, self.nkv, self.d, page_size),
-                   ops.attention_scored_scratch_bytes(self.env.dtype, requests, tokens, 1, longest, keys, self.nq, self.nkv, self.d, page_size),
-                   ops.attention_scored_scratch_bytes(self.env.dtype, 1, longest, longest, longest, keys, self.nq, self.nkv, self.d, page_size))
+        return ops.attention_scored_most_scratch_bytes(self.env.dtype, requests, tokens, keys, self.nq, self.nkv, self.d)
 
     def attend_scored(self, o, qkv, q_w, k_w, table, rotary_dim, batch, cache):
         """Attention in a cache that drops keys: the store, then the kernels that add up every key's weight."""
