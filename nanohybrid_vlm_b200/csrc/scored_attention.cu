@@ -753,12 +753,15 @@ NHV_API int nhv_attention_scored(const NhvScoredCall* c, float* work, int work_k
   NHV_REQUIRE((size_t)work_kilobytes * 1024 >= plan.floats * sizeof(float) && (uintptr_t)work % 16 == 0, "scored attention: %d kilobytes of scratch are too few",
               work_kilobytes);
   ScoredArgs a{c->q, c->out, c->kv_pages, c->scores, c->scores_out, c->births, c->positions, c->block_table, c->cu_q, c->kv_len, c->sinks, work,
-               c->q_stride, c->out_stride, c->bt_stride, n_seqs, n_tokens, nq, nkv, d, c->page_size, c->n_pages, max_kv_len, 0, 0x7fffffff, c->scale, c->softcap};
+               c->q_stride, c->out_stride, c->bt_stride, n_seqs, n_tokens, nq, nkv, d, c->page_size, c->n_pages, max_kv_len, 0, 0, c->scale, c->softcap};
   float* scratch = work + ((size_t)n_tokens * nq + 3) / 4 * 4;
+  // the scratch is for requests of up to max_new tokens: none takes one that brings more
+  const int most_rows = max_new < 0x7fffffff / (nq / nkv) ? max_new * (nq / nkv) : 0x7fffffff;
   // The requests of many rows first: whatever can be refused is refused before anything is launched, or scores in place would hold some
   // requests' weights already.
   if (plan.rest) {
     a.min_rows = plan.short_rows + 1;
+    a.max_rows = most_rows;
     scored_place(plan.parts, scratch, n_tokens, nq, d);
     int rc;
     if (plan.many) {
@@ -776,6 +779,6 @@ NHV_API int nhv_attention_scored(const NhvScoredCall* c, float* work, int work_k
   }
   if (plan.short_rows < 0) return 0;
   a.min_rows = 0;
-  a.max_rows = plan.short_rows;
+  a.max_rows = plan.short_rows < most_rows ? plan.short_rows : most_rows;
   return scored_short_launch(dtype, a, plan.few, scratch, stream);
 }

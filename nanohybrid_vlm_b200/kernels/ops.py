@@ -1256,7 +1256,8 @@ def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs
     weights, summed over the tokens and over the query heads of a KV head, are added to the scores of the request's keys
     (new keys start from nothing) and written to ``scores_out`` (None: ``scores`` itself; slots of no request stay as they are).
     ``births`` [n_pages, nkv, page_size] int32: receives ``positions`` [T] int32 for the new keys.  ``sinks`` and ``softcap`` as in
-    ``attention_tensor_core``.  ``min_new``, ``max_new``, ``max_kv_len``: the least and the most new tokens of a request, the most keys.
+    ``attention_tensor_core``.  ``min_new``, ``max_new``, ``max_kv_len``: the least and the most new tokens of a request, the most keys
+    (a request that brings more than ``max_new`` is left out, keys beyond ``max_kv_len`` are not looked at).
     Scores, weights and sums are float32 and added in a fixed order: the same call gives the same bits."""
     if scores_out is None:
         scores_out = scores

@@ -793,3 +793,26 @@ def test_queries_that_are_one_row_for_all_tokens(ops, new):
                          positions=i32(c.positions))
     ops.raise_wait_errors()
     c.check(second.cpu(), scores.cpu(), births.cpu())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page", [(4, 2, 64, 64), (8, 1, 33, 7)])
+@pytest.mark.parametrize("news,most", [([1, 4, 0, 1], 2), ([40, 200, 1, 0], 100), ([1, 90, 1, 1], 30)])
+def test_requests_that_bring_more_than_was_said_are_left_out(ops, dtype, nq, nkv, d, page, news, most):
+    c = Case(news, [300, 250, 70, 20], nq, nkv, d, page, dtype, seed=25)
+    want, want_scores, want_births = c.run(ops)
+    out, scores, births = torch.full_like(c.q, 9.0).cuda(), c.scores.cuda(), c.births.cuda()
+    ops.attention_scored(out, c.q.cuda(), c.pages.cuda(), scores, c.table.cuda(), c.cu_t, c.lens_t, 4, min(news), most, 300, nq, nkv, d, c.scale,
+                         births=births, positions=i32(c.positions))
+    ops.raise_wait_errors()
+    out, scores, births = out.cpu(), scores.cpu(), births.cpu()
+    big = slice(news[0], news[0] + news[1])
+    assert (out[big] == 9.0).all()
+    assert torch.equal(c.of(scores, 1, 0).nan_to_num(-1.0), c.of(c.scores, 1, 0).nan_to_num(-1.0)) and torch.equal(c.of(births, 1, 0), c.of(c.births, 1, 0))
+    rest = torch.ones(c.q.shape[0], dtype=torch.bool)
+    rest[big] = False
+    unit = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -18      # the same sums in other parts: a rounding of the output, or of 32-bit sums
+    assert torch.allclose(out[rest].double(), want[rest].double(), rtol=unit, atol=unit)
+    for s in (0, 2, 3):
+        for g in range(nkv):
+            assert torch.allclose(c.of(scores, s, g), c.of(want_scores, s, g), rtol=2.0 ** -15, atol=0) and torch.equal(c.of(births, s, g), c.of(want_births, s, g))
