@@ -1,5 +1,5 @@
-// Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), up to 32 of
-// them: decoded tokens, drafts.  All the work is to read the keys and values once.
+// Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), up to 8 to 32 of
+// them (scored_short_rows): decoded tokens, drafts.  All the work is to read the keys and values once.
 //
 // First kernel: a block per (part of a request's keys, up to 24 of its rows, KV head, request), its warps independent of one
 // another; blocks for other rows of the same keys find them in L2.  A warp takes 16
@@ -858,10 +858,13 @@ int launch_f32(const ShortArgs& w, dim3 grid, size_t smem, cudaStream_t stream) 
 }  // namespace
 
 int scored_short_rows(int dtype, int d) {
-  // float32: blocks of 8 rows; 24 rows take 153 us where the tiles of scored_attention.cu take 245 (8 requests of 2,000 keys), 32 rows 197.
-  // bfloat16: a block's 16 rows of heads above 128 would need more registers than a thread has; from 32 rows on the tcgen05 kernels are
-  // faster.
-  return dtype == NHV_F32 ? 32 : d <= 128 ? 32 : 8;
+  // float32: as many as the arrays of the second kernel hold.  Against the tiles of scored_attention.cu, 8 requests of 2,000 keys, 8 KV heads
+  // of 128: 24 rows 155 us and 247, 32 rows 199 and 277; heads of 256 319 and 729; the tiles win only for 64 requests of 300 keys with heads
+  // of 64 (179 and 171).
+  // bfloat16: against the tcgen05 kernels, heads of 128, 24 rows: 2 requests of 20,000 keys 87 us and 96, 64 of 2,000 keys 255 and 291, 64 of
+  // 300 107 and 96, 8 of 2,000 63 and 47; 32 rows: 112 and 96, 375 and 291, 138 and 96, 75 and 47.  Heads of 64, 32 rows: 81 and 81, 229
+  // and 315, 89 and 86, 54 and 44.  A block's 16 rows of heads above 128 would need more registers than a thread has.
+  return dtype == NHV_F32 ? 32 : d <= 64 ? 32 : d <= 128 ? 24 : 8;
 }
 
 bool scored_short_takes(int dtype, int rows, int d) {
