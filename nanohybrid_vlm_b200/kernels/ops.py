@@ -1226,6 +1226,8 @@ def _check_attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len,
         raise KernelError(f"q and the output are [tokens, {nq * head_dim}] in the pages' type with neighbouring columns")
     dtype_code(q)
     T = q.shape[0]
+    if T and out.data_ptr() == q.data_ptr():
+        raise KernelError("the output has memory of its own: q is read again when the keys' weights are added up")
     _check_int_array("cu_q", cu_q, n_seqs + 1)
     _check_int_array("kv_len", kv_len, n_seqs)
     if (births is None) != (positions is None):
@@ -1250,8 +1252,8 @@ def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs
                      softcap: float | None = None, scores_out=None) -> None:
     """Causal attention of the step's new tokens over the paged cache, with the weight that every cached key received.
 
-    out, q [T, nq * head_dim] (rows may lie further apart), pages [n_pages, 2, nkv, page_size, head_dim] with the new keys and values
-    stored, scores [n_pages, nkv, page_size] float32: what the keys have gathered so far.  Of request i, tokens cu_q[i] .. cu_q[i + 1]
+    out, q [T, nq * head_dim] (rows may lie further apart, out not over q), pages [n_pages, 2, nkv, page_size, head_dim] with the new
+    keys and values stored, scores [n_pages, nkv, page_size] float32: what the keys have gathered so far.  Of request i, tokens cu_q[i] .. cu_q[i + 1]
     are new and its keys are the first kv_len[i] slots of its pages; a token sees all slots up to its own.  The new tokens'
     weights, summed over the tokens and over the query heads of a KV head, are added to the scores of the request's keys
     (new keys start from nothing) and written to ``scores_out`` (None: ``scores`` itself; slots of no request stay as they are).
@@ -1265,6 +1267,7 @@ def attention_scored(out, q, kv_pages, scores, block_table, cu_q, kv_len, n_seqs
     if not (q.is_cuda and out.is_cuda and kv_pages.is_cuda and (dtype is torch.bfloat16 or dtype is torch.float32) and out.dtype is dtype
             and kv_pages.dtype is dtype and nkv > 0 and nq > 0 and nq % nkv == 0 and 0 < head_dim <= 256 and columns == nq * head_dim
             and q.stride(1) == 1 and out.shape == q.shape and out.stride(1) == 1 and kv_pages.is_contiguous()
+            and (T == 0 or out.data_ptr() != q.data_ptr())
             and _scored_pages_ok(scores, births, block_table, n_seqs, max_kv_len)
             and pages == (scores.shape[0], 2, nkv, scores.shape[2], head_dim) and scores.shape[1] == nkv
             and n_seqs >= 0 and 0 <= min_new <= max_new <= max_kv_len and min_new * n_seqs <= T <= max_new * n_seqs

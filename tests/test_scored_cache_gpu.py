@@ -816,3 +816,13 @@ def test_requests_that_bring_more_than_was_said_are_left_out(ops, dtype, nq, nkv
     for s in (0, 2, 3):
         for g in range(nkv):
             assert torch.allclose(c.of(scores, s, g), c.of(want_scores, s, g), rtol=2.0 ** -15, atol=0) and torch.equal(c.of(births, s, g), c.of(want_births, s, g))
+
+
+def test_an_output_over_the_queries_is_refused(ops):
+    """The second pass reads the queries again: in place the weights would be those of the outputs."""
+    from nanohybrid_vlm_b200.kernels.library import KernelError
+    c = Case([40, 1], [60, 30], 4, 2, 64, 64, torch.bfloat16, seed=27)
+    q, scores = c.q.cuda(), c.scores.cuda()
+    with pytest.raises(KernelError, match="memory of its own"):
+        ops.attention_scored(q, q, c.pages.cuda(), scores, c.table.cuda(), c.cu_t, c.lens_t, 2, 1, 40, 60, 4, 2, 64, c.scale)
+    assert torch.equal(q.cpu(), c.q) and torch.equal(scores.cpu().nan_to_num(-1.0), c.scores.nan_to_num(-1.0))
