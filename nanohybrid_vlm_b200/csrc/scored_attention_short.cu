@@ -1,26 +1,25 @@
-// Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), up to 8 to 32 of
-// them (scored_short_rows): decoded tokens, drafts.  All the work is to read the keys and values once.
+// Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), 8 to 32 of
+// them at most (scored_short_rows): decoded tokens, drafts.  All the work is to read the keys and values once.
 //
 // First kernel: a block per (part of a request's keys, up to 24 of its rows, KV head, request), its warps independent of one
-// another; blocks for other rows of the same keys find them in L2.  A warp takes 16
-// keys at a time straight from the pages into registers and forms S^T = K Q^T (m16n8k16, the 16 keys as M, up to 8 rows as N) and
-// O^T += V^T P^T.  No shared memory is between the pages and the products: which element of a head stands at which index of the
+// another; blocks for other rows of the same keys find them in L2.  A warp takes 16 keys at a time straight from the pages into
+// registers and forms S^T = K Q^T (m16n8k16, the 16 keys as M, up to 8 rows as N) and O^T += V^T P^T.  No shared memory is between the pages and the products: which element of a head stands at which index of the
 // product is free as long as both operands agree, so a lane takes 16 consecutive bytes of a row and its registers are the fragment
 // as they are.  For V^T two keys' elements have to share a register, which one byte permutation each does.  The next keys'
 // loads are sent as soon as the products have used the registers; the next tile's page is looked up one tile ahead.
 //   P goes into the second product as two bfloat16 parts, its first 8 bits and what they leave (an error of 2^-15 where one part
 //   has 2^-8): the tensor pipe is idle most of the time here.  Neither part is negative, and the second none only where P is: an
 //   infinite value times P is as infinite in parts as whole.  With more than 16 rows the pipe is not idle, and P has one part, as in
-//   the tcgen05 kernels.
+//   the tcgen05 kernels (error of the output against 64 bits 2.3e-3, with two parts 1.7e-3, which is the output's own rounding).
 //   The running maximum moves only when it grows by more than 2^8, so that most tiles leave the sums as they are.
 //   The warps' sums meet in shared memory; the block leaves one partial sum (fp32) and the scores of its keys.
-// Second kernel, or the same blocks as a cluster where few suffice: the parts' sums are joined, a block per (request, KV head) for the output and blocks of keys for the weights: a
-// thread per key adds exp2(score - log-sum) over the rows.  Two kernels instead of one that reads the keys twice: a score is 4
+// Second kernel, or the same blocks as a cluster where few suffice: the parts' sums are joined, blocks of the output's elements and
+// blocks of keys for the weights: a thread per key adds exp2(score - log-sum) over the rows.  Two kernels instead of one that reads the keys twice: a score is 4
 // bytes a row where a key is 2 d.
 //
-// What bounds it is reading the pages: 64 decoded tokens over 1,500 to 2,304 keys each (474 MB), 32 heads on 8 of 128, 101 us in both
-// kernels, of them 88 in the first at 5.4 TB/s; three over 65,000 to 98,000 keys 175 us.  With 20 rows a request (drafts) it is the
-// instructions of the products and exponentials, with two blocks an SM to hide them: 120 us for 311 MB.
+// What bounds it is reading the pages: 64 decoded tokens over 1,200 to 2,304 keys each (474 MB), 32 heads on 8 of 128, 99 us in both
+// kernels, of them 85 in the first at 5.6 TB/s; three over 65,000 to 98,000 keys 174 us.  With 20 rows a request (drafts) it is the
+// instructions of the products and exponentials, with two blocks an SM to hide them: 121 us for 311 MB.
 //
 // A key out of sight may hold anything: its score is replaced, its value not loaded.  Where only some of a request's rows see a
 // key (several new tokens), what is not finite in the values is left out of the second product and given to the rows that see it.
@@ -877,7 +876,7 @@ ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, i
   const int most = dtype == NHV_F32 ? 8 : 24;
   p.row_blocks = (p.rows + most - 1) / most;
   p.block_rows = (p.rows / p.row_blocks + (p.rows % p.row_blocks ? 1 : 0) + 1) / 2 * 2;
-  // Four times as many blocks as run at once (three times: drafts 120 -> 125 us, 64 decoded tokens 101 -> 103), so that requests of
+  // Four times as many blocks as run at once (three times took 4 and 2 % longer for drafts and 64 decoded tokens), so that requests of
   // unlike length even out, and no fewer than 64 keys a block (a tile per warp).
   const int an_sm = dtype == NHV_F32 ? (d <= 128 ? 3 : 2) : p.block_rows * ((d + 63) / 64) <= 16 ? 3 : 2, at_once = 148 * an_sm;
   const long long keys = (long long)n_seqs * nkv * p.row_blocks * max_keys, want = (keys + 4 * at_once - 1) / (4 * at_once);
@@ -887,7 +886,7 @@ ShortPlan scored_short_plan(int dtype, int n_seqs, int max_rows, int max_keys, i
   // Where a request's parts are few, their scores stay in shared memory and all blocks run at once, a cluster of blocks
   // finishes the request and KV head alone, without a second launch: one request of 517 keys 18.4 -> 15.3 us a call, as long on the
   // device (9.8 against 9.5; float32 13.1 against 11.3), four of 1,000 keys 14.6 -> 11.6 there (float32 19.6 -> 16.3).  With more
-  // blocks than that the wait for the slowest of a cluster costs more than the second kernel (64 requests 101 -> 119 us).
+  // blocks than that the wait for the slowest of a cluster costs more than the second kernel (64 requests 18 % longer).
   if (p.row_blocks == 1 && p.splits <= 2 * SH_MOST_CLUSTER) {
     int blocks = 1;
     while (blocks < p.splits && blocks < SH_MOST_CLUSTER) blocks *= 2;
