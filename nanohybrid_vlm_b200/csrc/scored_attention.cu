@@ -668,6 +668,7 @@ struct ScoredPlan {
 static ScoredPlan scored_plan(int dtype, bool wide, int n_seqs, int n_tokens, int min_new, int max_new, int max_keys, int nq, int nkv, int d,
                               int page_size, int n_pages, int q_stride, float scale) {
   ScoredPlan p = {};
+  if (n_tokens == 0) min_new = max_new = 0;       // whatever the caller's bounds say: no rows to make maps of
   p.wide = wide && d % (dtype == NHV_F32 ? 4 : 8) == 0;
   p.short_rows = -1;
   const int G = nq / nkv, most = scored_short_rows(dtype, d);

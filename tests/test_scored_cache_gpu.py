@@ -826,3 +826,15 @@ def test_an_output_over_the_queries_is_refused(ops):
     with pytest.raises(KernelError, match="memory of its own"):
         ops.attention_scored(q, q, c.pages.cuda(), scores, c.table.cuda(), c.cu_t, c.lens_t, 2, 1, 40, 60, 4, 2, 64, c.scale)
     assert torch.equal(q.cpu(), c.q) and torch.equal(scores.cpu().nan_to_num(-1.0), c.scores.nan_to_num(-1.0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page", [(16, 2, 128, 64), (64, 1, 64, 8), (33, 1, 40, 7)])
+def test_bounds_above_what_a_step_without_new_tokens_brings(ops, dtype, nq, nkv, d, page):
+    c = Case([0, 0, 0], [90, 0, 33], nq, nkv, d, page, dtype, seed=29)
+    scores, births = c.scores.cuda(), c.births.cuda()
+    q = torch.empty(0, nq * d, dtype=dtype, device="cuda")
+    ops.attention_scored(torch.empty_like(q), q, c.pages.cuda(), scores, c.table.cuda(), c.cu_t, c.lens_t, 3, 0, 60, 90, nq, nkv, d, c.scale, births=births,
+                         positions=i32([]))
+    ops.raise_wait_errors()
+    assert torch.equal(scores.cpu().nan_to_num(-1.0), c.scores.nan_to_num(-1.0)) and torch.equal(births.cpu(), c.births)
