@@ -65,6 +65,21 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float low_of(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high_of(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// The weight of keys j0, j0 + step, .. from their kept scores, where some row's sum is no number: a row that does not see a key adds nothing.
+__device__ __forceinline__ void careful_weights(const ScoredArgs& a, const float* kept, int stride, const float* lse, int rows, int seq, int first, int kvh,
+                                                int j0, int step, int end, int old) {
+#pragma unroll 1
+  for (int j = j0; j < end; j += step) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+      const float x = kept[(size_t)j * stride + r];
+      sum += x == -INFINITY ? 0.f : scored_exp2(x - lse[r]);
+    }
+    store_weight(a, seq, first, kvh, j, j - old, sum);
+  }
+}
+
 // The sums of a block's warps (in shared memory, rows of `row_len`) joined: the block's part, d floats a row, and its references and sums.
 __device__ __forceinline__ void join_warps(const ShortArgs& w, const float* so, const float* sml, int row_len, float* part_o, float* part_ml, int rows, int d) {
   for (int i = threadIdx.x; i < rows * (d / 2); i += SH_THREADS) {
@@ -152,6 +167,7 @@ __device__ __forceinline__ void finish_in_cluster(const ShortArgs& w, float* sme
   };
   ask(begin + threadIdx.x);
   cluster_wait();
+  bool odd = false;                               // some row's sum is no number
   for (int r = warp; r < R; r += SH_WARPS) {
     const float sink = a.sinks ? a.sinks[kvh * G + r % G] * SA_LOG2E : -INFINITY;
     float2 ml = make_float2(-INFINITY, 0.f);
@@ -160,8 +176,9 @@ __device__ __forceinline__ void finish_in_cluster(const ShortArgs& w, float* sme
     const float f = scored_exp2(ml.x - use), sum = warp_sum(f * ml.y) + scored_exp2(sink - use);
     if (lane < w.cluster) s_f[r][lane] = sum == 0.f ? 0.f : f * (1.0f / sum);
     if (lane == 0) s_lse[r] = sum == 0.f ? INFINITY : use + log2f(sum);
+    odd |= sum != sum;
   }
-  __syncthreads();
+  odd = __syncthreads_or(odd);
   for (int i = blockIdx.x * SH_THREADS + threadIdx.x; i < R * (d / 4); i += w.cluster * SH_THREADS) {
     const int r = i / (d / 4), c = 4 * (i - r * (d / 4));
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -177,7 +194,8 @@ __device__ __forceinline__ void finish_in_cluster(const ShortArgs& w, float* sme
     else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
   }
   cluster_arrive();                               // nothing of the others is read behind this
-  for (int j0 = begin + threadIdx.x; j0 < end; j0 += FIN_KEYS * SH_THREADS) {
+  if (odd) careful_weights(a, kept - (ptrdiff_t)begin * w.rows, w.rows, s_lse, R, seq, first, kvh, begin + threadIdx.x, SH_THREADS, end, old);
+  for (int j0 = odd ? end : begin + threadIdx.x; j0 < end; j0 += FIN_KEYS * SH_THREADS) {
 #pragma unroll
     for (int k = 0; k < FIN_KEYS; ++k) {
       const int j = j0 + k * SH_THREADS;
@@ -728,6 +746,7 @@ __global__ void __launch_bounds__(FIN_THREADS) scored_short_finish_kernel(const 
   if (output ? i - (int)threadIdx.x >= R * d : (int)blockIdx.x * per_block >= total) return;
   const int parts = (total + w.split_keys - 1) / w.split_keys;
   const size_t part = ((size_t)blockIdx.z * a.nkv + kvh) * w.splits * w.rows;
+  bool odd = false;                               // some row's sum is no number
   for (int r = warp; r < R; r += FIN_THREADS / 32) {
     const float sink = a.sinks ? a.sinks[kvh * G + r % G] * SA_LOG2E : -INFINITY;
     float ref = sink, sum = 0.f;
@@ -745,8 +764,9 @@ __global__ void __launch_bounds__(FIN_THREADS) scored_short_finish_kernel(const 
       s_inv[r] = sum == 0.f ? 0.f : 1.0f / sum;
       s_lse[r] = sum == 0.f ? INFINITY : use + log2f(sum);
     }
+    odd |= sum != sum;
   }
-  __syncthreads();
+  odd = __syncthreads_or(odd);
   if (output) {
     if (i >= R * d) return;
     const int r = i / d, c = i - r * d;
@@ -762,6 +782,10 @@ __global__ void __launch_bounds__(FIN_THREADS) scored_short_finish_kernel(const 
   }
   const float* kept = w.kept + ((size_t)blockIdx.z * a.nkv + kvh) * w.keys * w.rows;
   const int end = min(total, (int)(blockIdx.x + 1) * per_block), old = total - n, j0 = blockIdx.x * per_block + threadIdx.x;
+  if (odd) {
+    careful_weights(a, kept, w.rows, s_lse, R, seq, first, kvh, j0, FIN_THREADS, end, old);
+    return;
+  }
   // four keys a thread: their pages, their old scores and the rows' scores are asked for together
   int page[FIN_KEYS];
   size_t at[FIN_KEYS];

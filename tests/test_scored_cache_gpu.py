@@ -838,3 +838,21 @@ def test_bounds_above_what_a_step_without_new_tokens_brings(ops, dtype, nq, nkv,
                          positions=i32([]))
     ops.raise_wait_errors()
     assert torch.equal(scores.cpu().nan_to_num(-1.0), c.scores.nan_to_num(-1.0)) and torch.equal(births.cpu(), c.births)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nkv,d,page,copies", [(4, 2, 128, 64, 1), (3, 1, 40, 24, 1), (20, 4, 96, 16, 1), (2, 2, 64, 64, 100), (8, 1, 256, 32, 60)])
+def test_a_query_that_is_no_number_weighs_on_no_key_that_it_does_not_see(ops, dtype, nq, nkv, d, page, copies):
+    """Few tokens a request, of few requests (one launch) and of many (two): keys behind the token's own do not notice."""
+    n = 4 if nq // nkv < 8 else 1
+    c = Case([n, 1] * copies, [40 + n, 30] * copies, nq, nkv, d, page, dtype, seed=31)
+    _, clean, _ = c.run(ops)
+    q = c.q.clone()
+    q[c.cu[0]] = math.nan                                   # the first request's first token
+    out, scores, _ = c.run(ops, q=q)
+    assert torch.isnan(out[0].float()).all() and not torch.isnan(out[1:].float()).any()
+    for g in range(nkv):
+        got, want = c.of(scores, 0, g), c.of(clean, 0, g)
+        assert torch.isnan(got[:41]).all() and torch.equal(got[41:], want[41:])
+        for s in range(1, 2 * copies):
+            assert torch.equal(c.of(scores, s, g), c.of(clean, s, g))
