@@ -18,7 +18,7 @@
 // bytes a row where a key is 2 d.
 //
 // What bounds it is reading the pages: 64 decoded tokens over 1,200 to 2,304 keys each (474 MB), 32 heads on 8 of 128, 99 us in both
-// kernels, of them 85 in the first at 5.6 TB/s; three over 65,000 to 98,000 keys 174 us.  With 20 rows a request (drafts) it is the
+// kernels, of them 85 in the first at 5.6 TB/s; three over 65,000 to 98,000 keys 173 to 181 us.  With 20 rows a request (drafts) it is the
 // instructions of the products and exponentials, with two blocks an SM to hide them: 121 us for 311 MB.
 //
 // A key out of sight may hold anything: its score is replaced, its value not loaded.  Where only some of a request's rows see a
