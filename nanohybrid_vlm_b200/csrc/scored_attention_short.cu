@@ -1,28 +1,29 @@
-// Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), 8 to 32 of
-// them at most (scored_short_rows): decoded tokens, drafts.  All the work is to read the keys and values once.
+// Attention with scored keys for requests that bring few rows (a row: a new token and a query head of one KV head), 8 to 32 of them at
+// most (scored_short_rows): decoded tokens, drafts.  All the work is to read the keys and values once.
 //
-// First kernel: a block per (part of a request's keys, up to 24 of its rows, KV head, request), its warps independent of one
-// another; blocks for other rows of the same keys find them in L2.  A warp takes 16 keys at a time straight from the pages into
-// registers and forms S^T = K Q^T (m16n8k16, the 16 keys as M, up to 8 rows as N) and O^T += V^T P^T.  No shared memory is between the pages and the products: which element of a head stands at which index of the
-// product is free as long as both operands agree, so a lane takes 16 consecutive bytes of a row and its registers are the fragment
-// as they are.  For V^T two keys' elements have to share a register, which one byte permutation each does.  The next keys'
-// loads are sent as soon as the products have used the registers; the next tile's page is looked up one tile ahead.
-//   P goes into the second product as two bfloat16 parts, its first 8 bits and what they leave (an error of 2^-15 where one part
-//   has 2^-8): the tensor pipe is idle most of the time here.  Neither part is negative, and the second none only where P is: an
-//   infinite value times P is as infinite in parts as whole.  With more than 16 rows the pipe is not idle, and P has one part, as in
-//   the tcgen05 kernels (error of the output against 64 bits 2.3e-3, with two parts 1.7e-3, which is the output's own rounding).
+// First kernel: a block per (part of a request's keys, up to 24 of its rows, KV head, request), its warps independent of one another;
+// blocks for other rows of the same keys find them in L2.  A warp takes 16 keys at a time straight from the pages into registers and
+// forms S^T = K Q^T (m16n8k16, the 16 keys as M, up to 8 rows as N) and O^T += V^T P^T.  No shared memory is between the pages and the
+// products: which element of a head stands at which index of the product is free as long as both operands agree, so a lane takes 16
+// consecutive bytes of a row and its registers are the fragment as they are.  For V^T two keys' elements have to share a register, which
+// one byte permutation each does.  The next keys' loads are sent as soon as the products have used the registers; the next tile's page is
+// looked up one tile ahead.
+//   P goes into the second product as two bfloat16 parts, its first 8 bits and what they leave (an error of 2^-15 where one part has
+//   2^-8): the tensor pipe is idle most of the time here.  Neither part is negative, and the second none only where P is: an infinite
+//   value times P is as infinite in parts as whole.  With more than 16 rows the pipe is not idle, and P has one part, as in the tcgen05
+//   kernels (error of the output against 64 bits 2.3e-3, with two parts 1.7e-3, which is the output's own rounding).
 //   The running maximum moves only when it grows by more than 2^8, so that most tiles leave the sums as they are.
 //   The warps' sums meet in shared memory; the block leaves one partial sum (fp32) and the scores of its keys.
 // Second kernel, or the same blocks as a cluster where few suffice: the parts' sums are joined, blocks of the output's elements and
-// blocks of keys for the weights: a thread per key adds exp2(score - log-sum) over the rows.  Two kernels instead of one that reads the keys twice: a score is 4
-// bytes a row where a key is 2 d.
+// blocks of keys for the weights: a thread per key adds exp2(score - log-sum) over the rows.  Two kernels instead of one that reads the
+// keys twice: a score is 4 bytes a row where a key is 2 d.
 //
 // What bounds it is reading the pages: 64 decoded tokens over 1,200 to 2,304 keys each (474 MB), 32 heads on 8 of 128, 99 us in both
-// kernels, of them 85 in the first at 5.6 TB/s; three over 65,000 to 98,000 keys 173 to 181 us.  With 20 rows a request (drafts) it is the
-// instructions of the products and exponentials, with two blocks an SM to hide them: 121 us for 311 MB.
+// kernels, of them 85 in the first at 5.6 TB/s; three over 65,000 to 98,000 keys 173 to 181 us.  With 20 rows a request (drafts) it is
+// the instructions of the products and exponentials, with two blocks an SM to hide them: 121 us for 311 MB.
 //
-// A key out of sight may hold anything: its score is replaced, its value not loaded.  Where only some of a request's rows see a
-// key (several new tokens), what is not finite in the values is left out of the second product and given to the rows that see it.
+// A key out of sight may hold anything: its score is replaced, its value not loaded.  Where only some of a request's rows see a key
+// (several new tokens), what is not finite in the values is left out of the second product and given to the rows that see it.
 #include "nhv_scored.cuh"
 
 namespace {
