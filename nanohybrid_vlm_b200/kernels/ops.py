@@ -49,7 +49,10 @@ try:                # the current stream's handle without an object around it: 0
 
     def stream_ptr() -> int:
         return _cuda_getCurrentRawStream(_cuda_getDevice())
+
+    _current_device = _cuda_getDevice
 except ImportError:
+    _current_device = torch.cuda.current_device
 
     def stream_ptr() -> int:
         return torch.cuda.current_stream().cuda_stream
@@ -1858,6 +1861,115 @@ def linear_simt(out, x, weight) -> None:
     N = weight.shape[0]
     call("nhv_gemm_nt_simt", dtype_code(x), out.data_ptr(), x.data_ptr(), weight.data_ptr(), M, N, K, x.stride(0), K,
          N, int(out.dtype == torch.float32 and x.dtype != torch.float32), stream_ptr())
+
+
+# ---------------------------------------------------------------- 8-bit integers
+# Rows of 8-bit integers with a float32 scale each (integer times scale is the value), and their products.
+INT8_LONGEST_SUM = 131071
+INT8_ROW_BYTES = 16     # rows made here start at multiples of this, which the fast products read 16 bytes at a time
+
+
+def new_int8(rows: int, width: int, device) -> torch.Tensor:
+    """An uninitialised int8 matrix [rows, width] whose rows start at multiples of 16 bytes, as ``linear_int8`` reads them fastest."""
+    pitch = -(-width // INT8_ROW_BYTES) * INT8_ROW_BYTES
+    return torch.empty((rows, pitch), dtype=torch.int8, device=device)[:, :width]
+
+
+def _same_device(*tensors) -> None:
+    """All tensors on the current device, the one whose stream the kernel is launched on."""
+    _need_cuda(*tensors)
+    current = _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != current:
+            raise KernelError(f"tensors and stream belong together: a tensor lies on {t.device}, the current device is cuda:{current}")
+
+
+def _int8_rows_ok(t, rows: int, width: int) -> bool:
+    return (t.dtype is torch.int8 and t.shape == (rows, width) and (t.stride(1) == 1 or width == 1)
+            and (rows <= 1 or t.stride(0) >= width))
+
+
+def _check_int8_rows(name: str, t, rows: int, width: int) -> None:
+    if not _int8_rows_ok(t, rows, width):
+        raise KernelError(f"{name} are int8 [{rows}, {width}] with neighbouring columns and rows that do not overlap, not "
+                          f"{tuple(t.shape)} {t.dtype} with strides {t.stride()}")
+
+
+def _check_scales(name: str, t, n: int) -> None:
+    if t.dtype is not torch.float32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        raise KernelError(f"{name} are {n} float32 numbers side by side, not {tuple(t.shape)} {t.dtype}")
+
+
+def _rows_int8(kind: int, q, scales, x, rows: int, width: int, x_stride: int, residual=None, weight=None, eps: float = 0.0, offset: float = 0.0,
+               write_residual: bool = False) -> None:
+    _check_int8_rows("the rows to write", q, rows, width)
+    _check_scales("scales", scales, rows)
+    if width < 1:
+        raise KernelError("rows of no elements have no scale")
+    dtype = dtype_code(x)
+    _same_device(q, scales, x, residual, weight)
+    call("nhv_rows_int8", kind, dtype, q.data_ptr(), q.stride(0) if rows > 1 else width, scales.data_ptr(), x.data_ptr(), x_stride,
+         _ptr(residual), _ptr(weight), rows, width, float(eps), float(offset), int(write_residual), stream_ptr())
+
+
+def quantize_rows(q, scales, x) -> None:
+    """q [n, width] int8, scales [n] float32 = the rows of x [n, width] in 8 bits: a = max |x[r]|, scales[r] = a / 127, q = 127 x / a rounded to
+    the nearest integer, ties to even.  Rows of q and x may lie further apart.  A row of zeros has the scale 0; one that holds an
+    infinity or a NaN has the scale NaN and zeros."""
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise KernelError(f"x is a matrix with neighbouring columns, not {tuple(x.shape)} with strides {x.stride()}")
+    rows, width = x.shape
+    _rows_int8(0, q, scales, x, rows, width, x.stride(0) if rows > 1 else width)
+
+
+def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual: bool = True, weight_offset: float = 0.0) -> None:
+    """``rmsnorm`` with its output in 8 bits: q [n, width] int8 and scales [n] as ``quantize_rows`` gives them for norm(x (+ residual)) *
+    (weight + weight_offset), which is held in 32 bits and rounded once.  With a residual and write_residual the sum, rounded to x's
+    type, replaces the residual."""
+    width = x.shape[-1] if x.dim() else 0
+    _contig("x", x)
+    if weight.dtype != x.dtype or weight.numel() != width or not weight.is_contiguous():
+        raise KernelError(f"the norm's weight is {width} numbers in x's type side by side, not {tuple(weight.shape)} {weight.dtype}")
+    if residual is not None:
+        _contig("residual", residual)
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise KernelError(f"the residual has x's shape and type, not {tuple(residual.shape)} {residual.dtype}")
+        if write_residual and residual.data_ptr() == x.data_ptr() and x.numel():
+            raise KernelError("the residual has memory of its own: its sum with x is written there")
+    rows = x.numel() // width if width else 0
+    _rows_int8(1, q, scales, x, rows, width, width, residual, weight, eps, weight_offset, write_residual and residual is not None)
+
+
+def silu_mul_int8(q, scales, gate_up) -> None:
+    """``silu_mul`` with its output in 8 bits: q [n, inter] int8 and scales [n] as ``quantize_rows`` gives them for silu(gate) * up, which is held
+    in 32 bits; gate_up [n, 2 * inter] with the gate in the first half of each row."""
+    _contig("gate_up", gate_up)
+    if gate_up.dim() != 2 or gate_up.shape[1] % 2:
+        raise KernelError(f"gate_up is [n, 2 * inter], not {tuple(gate_up.shape)}")
+    rows, inter = gate_up.shape[0], gate_up.shape[1] // 2
+    _rows_int8(2, q, scales, gate_up, rows, inter, 2 * inter)
+
+
+def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
+    """out[T, N] = (x[T, K] @ weight[N, K]^T) * x_scales[:, None] * weight_scales[None] for int8 x and weight, float32 scales and out in
+    bfloat16 or float32.  The sums are exact (K up to 131,071), so an output does not depend on how the work is cut or batched.
+    Rows of all three matrices may lie further apart; x and weight are read fastest where their rows start at multiples of 16
+    bytes (``new_int8``)."""
+    if x.dim() != 2 or weight.dim() != 2 or out.dim() != 2:
+        raise KernelError("linear_int8 takes matrices: x [T, K], weight [N, K], out [T, N]")
+    (T, K), N = x.shape, weight.shape[0]
+    _check_int8_rows("x's rows", x, T, K)
+    _check_int8_rows("the weight's rows", weight, N, K)
+    _check_scales("x_scales", x_scales, T)
+    _check_scales("weight_scales", weight_scales, N)
+    if out.shape != (T, N) or (out.stride(1) != 1 and N > 1) or (T > 1 and out.stride(0) < N):
+        raise KernelError(f"out is [{T}, {N}] with neighbouring columns and rows that do not overlap, not {tuple(out.shape)} with strides {out.stride()}")
+    if not 0 < K <= INT8_LONGEST_SUM:
+        raise KernelError(f"a sum over 1 to {INT8_LONGEST_SUM} products of 8-bit integers is exact in 32 bits, not over {K}")
+    dtype = dtype_code(out)
+    _same_device(out, x, x_scales, weight, weight_scales)
+    call("nhv_gemm_int8", out.data_ptr(), dtype, out.stride(0) if T > 1 else N, x.data_ptr(), x.stride(0) if T > 1 else K, x_scales.data_ptr(),
+         weight.data_ptr(), weight.stride(0) if N > 1 else K, weight_scales.data_ptr(), T, N, K, stream_ptr())
 
 
 # ---------------------------------------------------------------- bounded waits that ran out
