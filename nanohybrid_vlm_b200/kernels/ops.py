@@ -1866,6 +1866,7 @@ def linear_simt(out, x, weight) -> None:
 # ---------------------------------------------------------------- 8-bit integers
 # Rows of 8-bit integers with a float32 scale each (integer times scale is the value), and their products.
 INT8_LONGEST_SUM = 131071
+INT8_WAY = 0
 INT8_ROW_BYTES = 16     # rows made here start at multiples of this, which the fast products read 16 bytes at a time
 
 
@@ -1968,8 +1969,8 @@ def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
         raise KernelError(f"a sum over 1 to {INT8_LONGEST_SUM} products of 8-bit integers is exact in 32 bits, not over {K}")
     dtype = dtype_code(out)
     _same_device(out, x, x_scales, weight, weight_scales)
-    call("nhv_gemm_int8", out.data_ptr(), dtype, out.stride(0) if T > 1 else N, x.data_ptr(), x.stride(0) if T > 1 else K, x_scales.data_ptr(),
-         weight.data_ptr(), weight.stride(0) if N > 1 else K, weight_scales.data_ptr(), T, N, K, stream_ptr())
+    call("nhv_gemm_int8", out.data_ptr(), dtype, out.stride(0) if T > 1 else N, x.data_ptr(), x.stride(0) if T > 1 else -(-K // 16) * 16, x_scales.data_ptr(),
+         weight.data_ptr(), weight.stride(0) if N > 1 else -(-K // 16) * 16, weight_scales.data_ptr(), T, N, K, _sm_count(x.device), INT8_WAY, stream_ptr())
 
 
 # ---------------------------------------------------------------- bounded waits that ran out
@@ -1993,7 +1994,8 @@ def _register_library_sources() -> None:
     import ctypes
     from .library import load_library
     lib = load_library()
-    for name in ("gemm_slab", "gemm_stream_k", "gemm_tcgen05", "moe_tcgen05", "gemm_f32_tcgen05", "key_eviction", "scored_tcgen05"):
+    for name in ("gemm_slab", "gemm_stream_k", "gemm_tcgen05", "moe_tcgen05", "gemm_f32_tcgen05", "key_eviction", "scored_tcgen05",
+                 "gemm_int8"):
         word = getattr(lib, f"nhv_{name}_error_word")
         word.restype, word.argtypes = ctypes.c_void_p, []
         take = getattr(lib, f"nhv_{name}_error")
