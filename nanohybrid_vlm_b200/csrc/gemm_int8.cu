@@ -93,11 +93,11 @@ __device__ __forceinline__ uint32_t in_block(uint32_t mine, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(mine), "r"(rank));
   return a;
 }
-__device__ __forceinline__ int4 load_cluster4(uint32_t at) {
-  int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-  return v;
+__device__ __forceinline__ void store_cluster4(uint32_t at, int a, int b, int c, int d) {
+  asm volatile("st.shared::cluster.v4.s32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
@@ -108,6 +108,7 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(r));
   return r != 0;
 }
+__device__ __forceinline__ uint32_t same_in_all(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 template <int GROUP>
@@ -194,29 +195,163 @@ struct alignas(64) Mapped {
   Product p;
   int nt;             // tokens of a tile: the boxes of x_map, a multiple of 16
   int tiles_t, tiles_n, group;
+  int rows, stages, w_bytes, ring_bytes;      // few tokens: rows of the weight of a tile, and the ring
+  int share, parts_bytes;                     // tokens that a block of a cluster finishes, and room for all parts of theirs
 };
 
-// ---- few tokens: 128 rows of the weight on the MMA's M axis, up to NT tokens on its N axis.
-constexpr int SPLIT_THREADS = 192;     // producer warp, MMA warp, four epilogue warps
-constexpr int W_BYTES = 128 * BK;
+// ---- up to eight tokens: the weight streams through registers into mma.sync, 16 rows beside the tokens
+constexpr int STREAM_WARPS = 16, STREAM_CHUNKS = 4, STREAM_DEPTH = 2;
+constexpr int STREAM_LD = 12;          // of a row's sums: eight tokens, and four so that the lanes' banks differ
 
-template <int NT, int STAGES>
+__device__ __forceinline__ void mma_sync(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load_once(const int8_t* at) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
+  return v;
+}
+// The first n of a word's four bytes, zeros for the others.
+__device__ __forceinline__ uint32_t kept_bytes(uint32_t v, int n) { return n >= 4 ? v : n <= 0 ? 0u : v & ((1u << (8 * n)) - 1u); }
+
+struct StreamPlan {
+  int along_k, chunks;      // warps that share K, and the 64-byte pieces that each takes at a time
+};
+
+__global__ void __launch_bounds__(STREAM_WARPS * 32, 1) product_stream_kernel(const Product p, const StreamPlan plan) {
+  extern __shared__ int sums[];                                  // [rows][STREAM_LD]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int r0 = (int)((long long)p.N * blockIdx.x / gridDim.x), rows = (int)((long long)p.N * (blockIdx.x + 1) / gridDim.x) - r0;
+  pdl_launch_dependents();
+  const int8_t* w = p.w + (long long)r0 * p.w_stride;
+  if (threadIdx.x == 0) {
+    // asked into L2, which is where all copies meet: nothing that is read here is used
+    const long long bytes = (long long)(rows - 1) * p.w_stride;
+    const uint32_t ask = (uint32_t)(bytes < 65536 ? bytes : 65536);
+    if (rows > 1) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(w), "r"(ask) : "memory");
+  }
+  for (int i = threadIdx.x; i < rows * STREAM_LD; i += STREAM_WARPS * 32) sums[i] = 0;
+  __syncthreads();
+  pdl_wait();
+  const int wk = plan.along_k, step = plan.chunks * 64, kw = warp % wk, nw = warp / wk, wn = STREAM_WARPS / wk;
+  const int f0 = rows * nw / wn, f1 = rows * (nw + 1) / wn;      // this warp's rows, from r0
+  const int mine = (f1 - f0 + 15) / 16, passes = (p.K + wk * step - 1) / (wk * step), items = mine * passes;
+  uint4 b[STREAM_DEPTH][2][STREAM_CHUNKS];
+  int pass = 0, group = 0;                                       // of what is loaded next
+  auto load = [&](uint4 (&v)[2][STREAM_CHUNKS]) {
+    const int k = (pass * wk + kw) * step + q * 16;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = f0 + group * 16 + h * 8 + g;
+      const int8_t* at = w + (long long)r * p.w_stride + k;
+#pragma unroll
+      for (int c = 0; c < STREAM_CHUNKS; ++c)
+        v[h][c] = r < f1 && c < plan.chunks && k + c * 64 < p.K ? load_once(at + c * 64) : make_uint4(0, 0, 0, 0);
+    }
+    if (++group == mine) {
+      group = 0;
+      ++pass;
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < STREAM_DEPTH; ++d)
+    if (d < items) load(b[d]);
+  uint32_t x[STREAM_CHUNKS][4];
+  int at_pass = -1, left = 0, row = 0;
+  for (int i = 0; i < items; i += STREAM_DEPTH) {
+#pragma unroll
+    for (int d = 0; d < STREAM_DEPTH; ++d) {
+      if (i + d >= items) break;
+      if (left == 0) {                                           // the tokens' next pieces
+        left = mine;
+        row = f0;
+        ++at_pass;
+#pragma unroll
+        for (int c = 0; c < STREAM_CHUNKS; ++c) {
+          const int k = (at_pass * wk + kw) * step + c * 64 + q * 16;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (g < p.T && c < plan.chunks && k < p.K) {
+            v = *reinterpret_cast<const uint4*>(p.x + (long long)g * p.x_stride + k);
+            // what lies behind a row is anybody's: zeros in x make it count for nothing, in the weight too
+            if (k + 16 > p.K) v = make_uint4(kept_bytes(v.x, p.K - k), kept_bytes(v.y, p.K - k - 4), kept_bytes(v.z, p.K - k - 8), kept_bytes(v.w, p.K - k - 12));
+          }
+          x[c][0] = v.x; x[c][1] = v.y; x[c][2] = v.z; x[c][3] = v.w;
+        }
+      }
+      // A lane's 16 bytes of a row are its places of two MMAs: which column of K stands where is the same for both operands.
+      int acc[4] = {};
+#pragma unroll
+      for (int c = 0; c < STREAM_CHUNKS; ++c) {
+        const uint4 u = b[d][0][c], v = b[d][1][c];
+        const uint32_t lo[4] = {u.x, v.x, u.y, v.y}, hi[4] = {u.z, v.z, u.w, v.w};
+        mma_sync(acc, lo, x[c][0], x[c][1]);
+        mma_sync(acc, hi, x[c][2], x[c][3]);
+      }
+      if (i + d + STREAM_DEPTH < items) load(b[d]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = row + (e >> 1) * 8 + g, t = 2 * q + (e & 1);
+        if (r < f1 && t < p.T) atomicAdd(&sums[r * STREAM_LD + t], acc[e]);      // integers: the order does not matter
+      }
+      row += 16;
+      --left;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * p.T; i += STREAM_WARPS * 32) {
+    const int t = i / rows, r = i - t * rows;
+    store_out(p, t, r0 + r, scaled(sums[r * STREAM_LD + t], p.x_scales[t], p.w_scales[r0 + r]));
+  }
+}
+
+int stream_product(const Product& p, int sms, cudaStream_t stream) {
+  constexpr int MOST_ROWS = 4096;                                // of a block: 192 KB of sums
+  const long long blocks = (long long)sms * ((p.N + (long long)sms * MOST_ROWS - 1) / ((long long)sms * MOST_ROWS));
+  const int grid = (int)(blocks < p.N ? blocks : p.N), rows = (p.N + grid - 1) / grid, pieces = (p.K + 63) / 64;
+  StreamPlan plan = {1, 1};
+  while (plan.along_k < STREAM_WARPS && plan.along_k * STREAM_CHUNKS < pieces) plan.along_k *= 2;
+  const int passes = (pieces + plan.along_k * STREAM_CHUNKS - 1) / (plan.along_k * STREAM_CHUNKS);
+  plan.chunks = (pieces + passes * plan.along_k - 1) / (passes * plan.along_k);
+  static std::atomic<uint64_t> allowed{0};
+  NHV_CUDA(nhv_allow_smem((const void*)product_stream_kernel, MOST_ROWS * STREAM_LD * 4, allowed), "linear_int8");
+  NHV_CUDA(nhv_launch(product_stream_kernel, dim3(grid), dim3(STREAM_WARPS * 32), (size_t)rows * STREAM_LD * 4, stream, p, plan), "linear_int8");
+  return 0;
+}
+
+// ---- few tokens: 128 rows of the weight on the MMA's M axis, up to NT tokens on its N axis.
+constexpr int SPLIT_THREADS = 320;     // producer warp, MMA warp, eight epilogue warps
+
+// One output of each of up to 16 tokens.
+template <typename O>
+__device__ __forceinline__ void store_column16(O* at, long long stride, const int (&v)[16], const float* xs, float ws, int tokens) {
+  if (tokens >= 16) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) at[j * stride] = from_f32<O>(scaled(v[j], xs[j], ws));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < tokens) at[j * stride] = from_f32<O>(scaled(v[j], xs[j], ws));
+  }
+}
 __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __grid_constant__ Mapped m) {
-  constexpr int STAGE_BYTES = W_BYTES + NT * BK;
-  constexpr uint32_t COLUMNS = NT < 32 ? 32 : NT;
-  static_assert((size_t)STAGES * STAGE_BYTES >= (size_t)NT * 512, "the sums are parked over the ring");
+  const int STAGES = m.stages, W_BYTES = m.w_bytes, STAGE_BYTES = W_BYTES + m.nt * BK;
+  const int tall = m.rows > 128 ? 2 : 1;                         // accumulators: 128 rows each
+  const uint32_t COLUMNS = tall * m.nt <= 32 ? 32 : tall * m.nt <= 64 ? 64 : tall * m.nt <= 128 ? 128 : tall * m.nt <= 256 ? 256 : 512;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* ring = smem_unaligned + ((1024 - (smem_u32(smem_unaligned) & 1023)) & 1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + (size_t)STAGES * STAGE_BYTES);
+  int* parts = reinterpret_cast<int*>(ring + m.ring_bytes);       // [part][share of the tokens / 4][tall * 128][4]
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + m.ring_bytes + m.parts_bytes);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   __shared__ int s_abort;
+  __shared__ float s_xs[256];
 
   const Product& p = m.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = (int)same_in_all(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int S = m.group, rank = S > 1 ? (int)cluster_rank() : 0;
-  const int n0 = (int)(blockIdx.x / S) * 128, t0 = (int)blockIdx.y * m.nt;
+  const int n0 = (int)(blockIdx.x / S) * m.rows, n_end = min(n0 + m.rows, p.N), t0 = (int)blockIdx.y * m.nt;
   const int tokens = min(m.nt, p.T - t0);
   const int kt = (p.K + BK - 1) / BK;
   const int k0 = (int)((long long)kt * rank / S), k1 = (int)((long long)kt * (rank + 1) / S);
@@ -234,94 +369,125 @@ __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __gr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = same_in_all(*tmem_slot);
   pdl_launch_dependents();
+  if (S > 1) cluster_arrive();
 
   if (warp == 0) {
     if (elect_one()) {
       const int n = k1 - k0;
+      asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&m.x_map) : "memory");
       for (int i = 0; i < min(n, STAGES); ++i) tma_prefetch_2d(&m.w_map, (k0 + i) * BK, n0);
       pdl_wait();
-      const uint32_t bytes = W_BYTES + m.nt * BK;                // zero-filled parts of a box count too
+      const uint32_t bytes = (m.rows + m.nt) * BK;                // zero-filled parts of a box count too
+      uint32_t s = 0, phase = 1;
       for (int i = 0; i < n; ++i) {
-        const int s = i % STAGES;
-        if (i >= STAGES && !mbar_wait(&empty[s], (uint32_t)((i / STAGES) - 1) & 1, 1)) { s_abort = 1; break; }
+        if (i >= STAGES && !mbar_wait(&empty[s], phase, 1)) { s_abort = 1; break; }
         unsigned char* dst = ring + (size_t)s * STAGE_BYTES;
         mbar_expect_tx(&full[s], bytes);
         tma_load_2d(dst, &m.w_map, (k0 + i) * BK, n0, &full[s]);
         tma_load_2d(dst + W_BYTES, &m.x_map, (k0 + i) * BK, t0, &full[s]);
+        if (++s == (uint32_t)STAGES) { s = 0; phase ^= 1; }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     const uint32_t idesc = instr_desc(128, m.nt);
+    const int n = (int)same_in_all(k1 - k0);
     bool ok = true;
-    for (int i = 0; i < k1 - k0; ++i) {
-      const int s = i % STAGES;
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (uint32_t)(i / STAGES) & 1, 2));
+    uint32_t s = 0, phase = 0;
+    const uint64_t first = smem_desc(same_in_all(smem_u32(ring)));
+    for (int i = 0; i < n; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase, 2));
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t a = smem_desc(smem_u32(ring) + s * STAGE_BYTES), b = a + (W_BYTES >> 4);
+        const uint64_t a = first + (uint64_t)(s * (uint32_t)(STAGE_BYTES >> 4)), b = a + (uint32_t)(W_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < BK / UMMA_K; ++kk)
           tc_mma<1>(tmem_base, a + kk * (UMMA_K >> 4), b + kk * (UMMA_K >> 4), idesc, (i > 0 || kk > 0) ? 1u : 0u);
+        if (tall == 2)
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk)
+            tc_mma<1>(tmem_base + (uint32_t)m.nt, a + (128 * BK >> 4) + kk * (UMMA_K >> 4), b + kk * (UMMA_K >> 4), idesc, (i > 0 || kk > 0) ? 1u : 0u);
         tc_commit<1>(&empty[s]);
-        if (i == k1 - k0 - 1) tc_commit<1>(acc_full);
+        if (i == n - 1) tc_commit<1>(acc_full);
       }
       __syncwarp();
+      if (++s == (uint32_t)STAGES) { s = 0; phase ^= 1; }
     }
     if (!ok) s_abort = 1;
   }
-  const int tid = (int)threadIdx.x - 64;                         // the epilogue's threads: 0 .. 127
-  int* parked = reinterpret_cast<int*>(ring);                    // [token][128]
   if (warp >= 2) {
+    const int tid = (int)threadIdx.x - 64;                       // 0 .. 255
     pdl_wait();
-    const int quarter = warp & 3, row = quarter * 32 + lane, n = n0 + row;      // the tensor-memory lanes that this warp may read
-    const float ws = n < p.N ? p.w_scales[n] : 0.f;
+    if (tid < tokens) s_xs[tid] = p.x_scales[t0 + tid];
+    asm volatile("bar.sync 1, 256;\n" ::: "memory");
+    // the tensor-memory lanes that this warp may read; every second piece of 16 tokens is its
+    const int quarter = warp & 3, row = quarter * 32 + lane, second = warp >= 6;
+    const float ws[2] = {n0 + row < n_end ? p.w_scales[n0 + row] : 0.f, n0 + 128 + row < n_end ? p.w_scales[n0 + 128 + row] : 0.f};
     const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, 3));
     tc_fence_after();
+    if (S > 1) cluster_wait();                                   // all blocks of the cluster run
     if (!ok) {
       s_abort = 1;
     } else {
-      const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16);
-      for (int c = 0; c < tokens; c += 16) {
-        int v[16];
-        tmem_ld16(v, at + c);
-        tmem_ld_wait();
+      for (int u = 0; u < tall; ++u) {
+        const int n = n0 + u * 128 + row;
+        const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(u * m.nt);
+        for (int c = second * 16; c < tokens; c += 32) {
+          int v[16];
+          tmem_ld16(v, at + c);
+          tmem_ld_wait();
+          if (S > 1) {                                           // four tokens' sums at a time to the block that finishes them
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (S > 1)
-            parked[(c + j) * 128 + row] = v[j];
-          else if (c + j < tokens && n < p.N)
-            store_out(p, t0 + c + j, n, scaled(v[j], p.x_scales[t0 + c + j], ws));
+            for (int j = 0; j < 16; j += 4) {
+              if (c + j >= tokens) break;
+              const int owner = (c + j) / m.share, four = (c + j - owner * m.share) >> 2;
+              const int* to = parts + (((rank * (m.share >> 2) + four) * tall * 128 + u * 128 + row) << 2);
+              store_cluster4(in_block(smem_u32(to), owner), v[j], v[j + 1], v[j + 2], v[j + 3]);
+            }
+          } else if (n < n_end) {
+            const long long o = (long long)(t0 + c) * p.out_stride + n;
+            if (p.out_f32)
+              store_column16(reinterpret_cast<float*>(p.out) + o, p.out_stride, v, s_xs + c, ws[u], tokens - c);
+            else
+              store_column16(reinterpret_cast<bf16*>(p.out) + o, p.out_stride, v, s_xs + c, ws[u], tokens - c);
+          }
         }
       }
     }
     tc_fence_before();
-  }
-  if (S > 1) {
-    __syncwarp();
-    cluster_sync();                                              // every block's sums are parked
-    if (warp >= 2) {
-      const int items = tokens * 32;
-      for (int i = items * rank / S + tid; i < items * (rank + 1) / S; i += 128) {
-        const int j = i >> 5, n = n0 + 4 * (i & 31);
-        const uint32_t mine = smem_u32(parked + i * 4);
-        int4 sum = make_int4(0, 0, 0, 0);
-        for (int q = 0; q < S; ++q) {
-          const int4 v = load_cluster4(in_block(mine, q));
-          sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-        }
-        const float xs = p.x_scales[t0 + j];
-        const int all[4] = {sum.x, sum.y, sum.z, sum.w};
+    if (S > 1) {
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();                                            // all parts have arrived
+      const int j0 = rank * m.share, fours = (min(tokens, j0 + m.share) - j0 + 3) >> 2;
+      for (int u = 0; u < tall; ++u) {
+        const int n = n0 + u * 128 + row;
+        for (int f = second; f < fours && n < n_end; f += 2) {
+          const int4* from = reinterpret_cast<const int4*>(parts) + f * tall * 128 + u * 128 + row;
+          int4 part[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < p.N) store_out(p, t0 + j, n + e, scaled(all[e], xs, p.w_scales[n + e]));
+          for (int q = 0; q < 8; ++q) part[q] = q < S ? from[q * (m.share >> 2) * tall * 128] : make_int4(0, 0, 0, 0);
+          int sum[4] = {};
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            sum[0] += part[q].x; sum[1] += part[q].y; sum[2] += part[q].z; sum[3] += part[q].w;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = j0 + f * 4 + e;
+            if (j < tokens) store_out(p, t0 + j, n, scaled(sum[e], s_xs[j], ws[u]));
+          }
+        }
       }
     }
+  } else if (S > 1) {
     __syncwarp();
-    cluster_sync();                                              // nobody leaves while its sums are read
+    cluster_wait();
+    cluster_arrive();
+    cluster_wait();
   }
   __syncthreads();
   if (s_abort) give_up_delay();                                  // let copies that may still be in flight land
@@ -329,12 +495,15 @@ __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __gr
   if (warp == 1) tmem_dealloc<1>(tmem_base, COLUMNS);
 }
 
-// ---- many tokens: pairs of blocks, 256 tokens on the MMA's M axis (128 a block), 256 outputs on its N axis (128 rows of the weight
-// in each block's shared memory), tiles handed out in turn to a grid of one pair for two SMs.
+// ---- many tokens: pairs of blocks, 256 tokens on the MMA's M axis (128 a block), TN outputs on its N axis (TN / 2 rows of the weight in
+// each block's shared memory), tiles handed out in turn to a grid of one pair for two SMs.
 constexpr int PAIR_THREADS = 320;      // producer warp, MMA warp, eight epilogue warps
-constexpr int PAIR_STAGES = 6;
-constexpr int HALF_BYTES = 128 * BK;   // an operand's half of a stage
-constexpr size_t PAIR_SMEM = 1024 + (size_t)PAIR_STAGES * 2 * HALF_BYTES + 8 * 128 * 4 + (2 * PAIR_STAGES + 4) * 8 + 16;
+template <int TN>
+struct Pair {
+  static constexpr int X_BYTES = 128 * BK, W_BYTES = TN / 2 * BK, STAGE = X_BYTES + W_BYTES;      // a block's half of a stage
+  static constexpr int STAGES = 196608 / STAGE;
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 8 * (TN / 2) * 4 + (2 * STAGES + 4) * 8 + 16;
+};
 
 __device__ __forceinline__ void store_row32(const Product& p, long long at, const float (&v)[32], int room) {
   if (p.out_f32) {
@@ -381,25 +550,27 @@ __device__ __forceinline__ void tile_place(const Mapped& m, int tile, int& tt, i
   tt = g * m.group + (r - tn * here);
 }
 
+template <int TN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) product_pair_kernel(const __grid_constant__ Mapped m) {
+  constexpr int STAGES = Pair<TN>::STAGES, STAGE = Pair<TN>::STAGE, X_BYTES = Pair<TN>::X_BYTES, HALF = TN / 2;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* ring = smem_unaligned + ((1024 - (smem_u32(smem_unaligned) & 1023)) & 1023);
-  float* scales = reinterpret_cast<float*>(ring + (size_t)PAIR_STAGES * 2 * HALF_BYTES);      // [8 warps][128]
-  uint64_t* full = reinterpret_cast<uint64_t*>(scales + 8 * 128);        // used in block 0, for both
-  uint64_t* empty = full + PAIR_STAGES;
-  uint64_t* acc_full = empty + PAIR_STAGES;      // [2]
+  float* scales = reinterpret_cast<float*>(ring + (size_t)STAGES * STAGE);      // [8 warps][HALF]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + 8 * HALF);        // used in block 0, for both
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;      // [2]
   uint64_t* acc_empty = acc_full + 2;            // [2], used in block 0
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   __shared__ int s_abort;
 
   const Product& p = m.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = (int)same_in_all(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
   const int tiles = m.tiles_t * m.tiles_n, kt = (p.K + BK - 1) / BK;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < PAIR_STAGES; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -415,7 +586,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) pro
   __syncthreads();
   cluster_sync();                                                // both blocks' barriers are there
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = same_in_all(*tmem_slot);
   pdl_launch_dependents();
   pdl_wait();
 
@@ -426,25 +597,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) pro
       for (int tile = pair; tile < tiles && ok; tile += pairs) {
         int tt, tn;
         tile_place(m, tile, tt, tn);
-        const int t0 = tt * 256 + (int)rank * 128, n0 = tn * 256 + (int)rank * 128;
+        const int t0 = tt * 256 + (int)rank * 128, n0 = tn * TN + (int)rank * HALF;
         for (int k = 0; k < kt; ++k, ++i) {
-          const int s = i % PAIR_STAGES;
-          if (i >= PAIR_STAGES && !mbar_wait(&empty[s], (uint32_t)((i / PAIR_STAGES) - 1) & 1, 1)) { ok = false; break; }
-          unsigned char* dst = ring + (size_t)s * 2 * HALF_BYTES;
+          const int s = i % STAGES;
+          if (i >= STAGES && !mbar_wait(&empty[s], (uint32_t)((i / STAGES) - 1) & 1, 1)) { ok = false; break; }
+          unsigned char* dst = ring + (size_t)s * STAGE;
           const uint32_t bar = in_block(smem_u32(&full[s]), 0);
-          if (rank == 0) mbar_expect_tx(&full[s], 4 * HALF_BYTES);      // zero-filled parts of a box count too
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * STAGE);      // zero-filled parts of a box count too
           tma_load_2d_pair(dst, &m.x_map, k * BK, t0, bar);
-          tma_load_2d_pair(dst + HALF_BYTES, &m.w_map, k * BK, n0, bar);
+          tma_load_2d_pair(dst + X_BYTES, &m.w_map, k * BK, n0, bar);
         }
       }
       // no block leaves before the last commits have reached it
-      for (int j = max(0, i - PAIR_STAGES); j < i && ok; ++j) ok = mbar_wait(&empty[j % PAIR_STAGES], (uint32_t)(j / PAIR_STAGES) & 1, 1);
+      for (int j = max(0, i - STAGES); j < i && ok; ++j) ok = mbar_wait(&empty[j % STAGES], (uint32_t)(j / STAGES) & 1, 1);
       if (!ok) s_abort = 1;
     }
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0) {
-      const uint32_t idesc = instr_desc(256, 256);
+      const uint32_t idesc = instr_desc(256, TN);
       bool ok = true;
       int i = 0, turn = 0;
       for (int tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
@@ -455,12 +626,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) pro
         }
         const uint32_t d = tmem_base + (uint32_t)((turn & 1) * 256);
         for (int k = 0; k < kt; ++k, ++i) {
-          const int s = i % PAIR_STAGES;
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (uint32_t)(i / PAIR_STAGES) & 1, 3));
+          const int s = i % STAGES;
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (uint32_t)(i / STAGES) & 1, 3));
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t a = smem_desc(smem_u32(ring) + s * 2 * HALF_BYTES), b = a + (HALF_BYTES >> 4);
+            const uint64_t a = smem_desc(smem_u32(ring) + s * STAGE), b = a + (X_BYTES >> 4);
 #pragma unroll
             for (int kk = 0; kk < BK / UMMA_K; ++kk)
               tc_mma<2>(d, a + kk * (UMMA_K >> 4), b + kk * (UMMA_K >> 4), idesc, (k > 0 || kk > 0) ? 1u : 0u);
@@ -473,17 +644,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) pro
       if (!ok) s_abort = 1;
     }
   } else {
-    const int quarter = warp & 3, half = warp >= 6 ? 128 : 0;      // lanes that this warp may read; its columns
-    float* mine = scales + (warp - 2) * 128;
+    const int quarter = warp & 3, half = warp >= 6 ? HALF : 0;      // lanes that this warp may read; its columns
+    float* mine = scales + (warp - 2) * HALF;
     int turn = 0;
     bool ok = true;
     for (int tile = pair; tile < tiles; tile += pairs, ++turn) {
       int tt, tn;
       tile_place(m, tile, tt, tn);
-      const int t = tt * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = tn * 256 + half;
+      const int t = tt * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = tn * TN + half;
       const float xs = t < p.T ? p.x_scales[t] : 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < HALF / 32; ++j) {
         const int n = n0 + j * 32 + lane;
         mine[j * 32 + lane] = n < p.N ? p.w_scales[n] : 0.f;
       }
@@ -492,12 +663,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) pro
       if (!ok) break;
       tc_fence_after();
       const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((turn & 1) * 256 + half);
-      for (int c = 0; c < 128; c += 32) {
+      for (int c = 0; c < HALF; c += 32) {
         int r[32];
         float v[32];
         tmem_ld32(r, at + c);
         tmem_ld_wait();
-        if (c == 96) {                                             // the accumulator is read: the MMAs may have it again
+        if (c == HALF - 32) {                                             // the accumulator is read: the MMAs may have it again
           tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_cluster(in_block(smem_u32(&acc_empty[turn & 1]), 0));
@@ -538,47 +709,119 @@ bool make_map(CUtensorMap* map, const void* base, long long rows, long long byte
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NT, int STAGES>
-int launch_split(const Mapped& m, cudaStream_t stream) {
-  constexpr size_t smem = 1024 + (size_t)STAGES * (W_BYTES + NT * BK) + (2 * STAGES + 1) * 8 + 16;
-  static_assert(smem <= 227 * 1024, "the ring must fit one block's shared memory");
+struct SplitPlan {
+  int nt, rows, parts, stages;
+};
+
+struct SplitSmem {
+  int w_bytes, ring_bytes, share, parts_bytes;
+  size_t all;
+};
+SplitSmem split_smem(const SplitPlan& plan) {
+  const int tall = plan.rows > 128 ? 2 : 1;
+  SplitSmem s;
+  s.w_bytes = (plan.rows * BK + 1023) / 1024 * 1024;
+  // the MMAs read 128 or 256 rows from a stage's start, whatever the stage holds
+  s.ring_bytes = (plan.stages - 1) * (s.w_bytes + plan.nt * BK) + tall * 128 * BK + plan.nt * BK;
+  s.share = ((plan.nt + plan.parts - 1) / plan.parts + 3) / 4 * 4;
+  s.parts_bytes = plan.parts > 1 ? plan.parts * s.share * tall * 512 : 0;
+  s.all = 1024 + (size_t)s.ring_bytes + s.parts_bytes + (2 * plan.stages + 1) * 8 + 16;
+  return s;
+}
+
+// Rows of a tile, parts of K and stages.  Times in us for 16 / 64 / 128 tokens.
+//   K in one part, a tile for each SM or, where that would be more than 96 rows, two: 12,288 x 4,096: 84 rows 11.3 / 12.2 / 13.6, 42 rows
+//   12.0 / 13.0 / 14.5; 24,576 x 4,096: 84 rows 18.8 / 19.2 / 22.1, 128 rows 19.9 / 20.5 / 23.4.
+//   Narrower weights: tiles of 128 rows, K over a cluster of blocks: 4,096 x 4,096 in 4 parts 5.8 / 7.8 / 9.4, in 1 with 28 rows 8.5 / 9.4 / 11.2.
+//   Up to 64 tokens two blocks share an SM (4,096 x 12,288 in 8 parts: 11.3 / 13.4, in 4: 11.8 / 14.4) unless a part would have fewer than 8
+//   stages (4,096 x 4,096 in 8 parts: 6.3 / 8.2); above, the room for the parts' sums leaves a second block no ring.  Clusters that
+//   would fill the SMs to the last do not all find their places at once (12,288 x 4,096 in 3 parts, 288 blocks: 15.1 / 19.6; 2,048 x 4,096 for
+//   128 tokens as 16 clusters of 8 13.4, as 32 of 4 with tiles of 64 rows 8.6).
+//   Short sums: K in one part, the tiles smaller: 4,096 x 1,024, 64 rows 3.6 / 4.1 / 5.1, 4 parts of 128 rows 3.6 / 5.3 / 8.8.
+SplitPlan split_plan(const Product& p, int sms) {
+  const int kt = (p.K + BK - 1) / BK;
+  SplitPlan plan;
+  plan.nt = p.T >= 128 ? 128 : (p.T + 15) / 16 * 16;
+  const bool shared = plan.nt <= 64;
+  plan.rows = shared || p.N > 64 * (sms * 7 / 8 / 4) ? 128 : 64;
+  const int tiles = (p.N + plan.rows - 1) / plan.rows, most_parts = shared ? 8 : 4;
+  plan.parts = (shared ? 2 * sms * 9 / 10 : sms * 7 / 8) / tiles;
+  if (plan.parts > most_parts) plan.parts = most_parts;
+  while (plan.parts > 1 && kt < 8 * plan.parts && tiles * plan.parts > sms) --plan.parts;
+  if (plan.parts > kt) plan.parts = kt;
+  if (plan.parts < 3 || (kt < 16 && p.N >= 24 * sms)) {
+    plan.parts = 1;
+    const long long slots = p.N > 96LL * sms ? 2 * sms : sms, waves = (p.N + 128LL * slots - 1) / (128LL * slots);
+    plan.rows = (int)((p.N + waves * slots - 1) / (waves * slots));
+    if (plan.rows < 32) plan.rows = p.N < 64 ? 64 : 32;
+  }
+  const size_t most = (plan.parts == 1 || shared ? 112 : 200) * 1024;
+  plan.stages = 8;
+  while (plan.stages > 1 && split_smem(plan).all > most) --plan.stages;
+  return plan;
+}
+
+int split_product(Mapped& m, const SplitPlan& plan, cudaStream_t stream) {
+  const Product& p = m.p;
+  NHV_REQUIRE(plan.rows >= 1 && plan.rows <= 256 && plan.nt >= 16 && plan.nt <= 256 && plan.nt % 16 == 0 && plan.stages >= 1 && plan.stages <= 16 && plan.parts >= 1 &&
+              plan.parts <= 8, "linear_int8: tiles of %d rows and %d tokens, %d stages, %d parts", plan.rows, plan.nt, plan.stages, plan.parts);
+  m.nt = plan.nt;
+  m.rows = plan.rows;
+  m.group = plan.parts;
+  m.stages = plan.stages;
+  m.tiles_t = (p.T + m.nt - 1) / m.nt;
+  m.tiles_n = (p.N + m.rows - 1) / m.rows;
+  const SplitSmem room = split_smem(plan);
+  m.w_bytes = room.w_bytes;
+  m.ring_bytes = room.ring_bytes;
+  m.share = room.share;
+  m.parts_bytes = room.parts_bytes;
+  NHV_REQUIRE(room.all <= 225 * 1024, "linear_int8: a ring of %d bytes", m.ring_bytes);
+  NHV_REQUIRE(make_map(&m.w_map, p.w, p.N, p.K, p.w_stride, m.rows) && make_map(&m.x_map, p.x, p.T, p.K, p.x_stride, m.nt),
+              "linear_int8: cannot encode the tensor maps");
   static std::atomic<uint64_t> allowed{0};
-  NHV_CUDA(nhv_allow_smem((const void*)product_split_kernel<NT, STAGES>, (int)smem, allowed), "linear_int8");
-  NHV_CUDA(nhv_launch_cluster(product_split_kernel<NT, STAGES>, dim3(m.tiles_n * m.group, m.tiles_t), dim3(SPLIT_THREADS), smem, stream, m.group, m),
+  NHV_CUDA(nhv_allow_smem((const void*)product_split_kernel, 225 * 1024, allowed), "linear_int8");
+  NHV_CUDA(nhv_launch_cluster(product_split_kernel, dim3(m.tiles_n * m.group, m.tiles_t), dim3(SPLIT_THREADS), room.all, stream, m.group, m),
            "linear_int8");
   return 0;
 }
 
-int split_product(Mapped& m, int parts, cudaStream_t stream) {
-  const Product& p = m.p;
-  m.nt = p.T >= 256 ? 256 : (p.T + 15) / 16 * 16;
-  m.tiles_t = (p.T + m.nt - 1) / m.nt;
-  m.tiles_n = (p.N + 127) / 128;
-  m.group = parts;
-  NHV_REQUIRE(make_map(&m.w_map, p.w, p.N, p.K, p.w_stride, 128) && make_map(&m.x_map, p.x, p.T, p.K, p.x_stride, m.nt),
-              "linear_int8: cannot encode the tensor maps");
-  if (m.nt <= 16) return launch_split<16, 5>(m, stream);
-  if (m.nt <= 32) return launch_split<32, 5>(m, stream);
-  if (m.nt <= 64) return launch_split<64, 4>(m, stream);
-  if (m.nt <= 128) return launch_split<128, 6>(m, stream);
-  return launch_split<256, 4>(m, stream);
-}
-
-int pair_product(Mapped& m, int sms, cudaStream_t stream) {
+template <int TN>
+int launch_pair(Mapped& m, int sms, cudaStream_t stream) {
   const Product& p = m.p;
   m.nt = 256;
   m.tiles_t = (p.T + 255) / 256;
-  m.tiles_n = (p.N + 255) / 256;
+  m.tiles_n = (p.N + TN - 1) / TN;
   m.group = m.tiles_t < 16 ? m.tiles_t : 16;
-  NHV_REQUIRE(make_map(&m.w_map, p.w, p.N, p.K, p.w_stride, 128) && make_map(&m.x_map, p.x, p.T, p.K, p.x_stride, 128),
+  NHV_REQUIRE(make_map(&m.w_map, p.w, p.N, p.K, p.w_stride, TN / 2) && make_map(&m.x_map, p.x, p.T, p.K, p.x_stride, 128),
               "linear_int8: cannot encode the tensor maps");
   const long long tiles = (long long)m.tiles_t * m.tiles_n;
   NHV_REQUIRE(tiles < (1LL << 30), "linear_int8: too many tiles");
   const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
   static std::atomic<uint64_t> allowed{0};
-  NHV_CUDA(nhv_allow_smem((const void*)product_pair_kernel, (int)PAIR_SMEM, allowed), "linear_int8");
-  NHV_CUDA(nhv_launch(product_pair_kernel, dim3(2 * pairs), dim3(PAIR_THREADS), PAIR_SMEM, stream, m), "linear_int8");
+  NHV_CUDA(nhv_allow_smem((const void*)product_pair_kernel<TN>, (int)Pair<TN>::SMEM, allowed), "linear_int8");
+  NHV_CUDA(nhv_launch(product_pair_kernel<TN>, dim3(2 * pairs), dim3(PAIR_THREADS), Pair<TN>::SMEM, stream, m), "linear_int8");
   return 0;
+}
+
+// The tiles' width: the one with the least turns * (width + 64), a turn being a tile for every pair, and 64 what a tile costs beside
+// its width.  us for widths 64 / 128 / 192 / 256: 256 tokens, 4,096 x 4,096 9.3 / 9.9 / - / 15.0; 256, 24,576 x 4,096 35.5 / 26.5 / 26.2 / 29.0; 512, 4,096 x 12,288
+// 32.4 / 23.1 / 31.0 / 36.0; 1,024, 4,096 x 12,288 - / 39.1 / 47.7 / 37.1; 2,048, 4,096 x 12,288 - / 90.7 / 84.2 / 75.4.
+int pair_product(Mapped& m, int sms, cudaStream_t stream) {
+  const long long tiles_t = (m.p.T + 255) / 256, pairs = sms / 2;
+  long long least = 0;
+  int width = 256;
+  for (int w = 256; w >= 64; w -= 64) {
+    const long long turns = (tiles_t * ((m.p.N + w - 1) / w) + pairs - 1) / pairs, cost = turns * (w + 64);
+    if (w == 256 || cost < least) {
+      least = cost;
+      width = w;
+    }
+  }
+  if (width == 64) return launch_pair<64>(m, sms, stream);
+  if (width == 128) return launch_pair<128>(m, sms, stream);
+  if (width == 192) return launch_pair<192>(m, sms, stream);
+  return launch_pair<256>(m, sms, stream);
 }
 
 }  // namespace
@@ -589,20 +832,20 @@ NHV_API int nhv_gemm_int8_error() { return nhv_wait_error_take(); }
 NHV_API void* nhv_gemm_int8_error_word() { return nhv_wait_error_address(); }
 
 NHV_API int nhv_gemm_int8(void* out, int out_dtype, long long out_stride, const void* x, long long x_stride, const float* x_scales,
-                          const void* w, long long w_stride, const float* w_scales, int T, int N, int K, int sms, int way, cudaStream_t stream) {
+                          const void* w, long long w_stride, const float* w_scales, int T, int N, int K, int sms, cudaStream_t stream) {
   if (T == 0 || N == 0) return 0;
   NHV_REQUIRE(T > 0 && N > 0 && K > 0 && K <= 131071, "linear_int8: a sum over 1 to 131,071 products is exact in 32 bits, not over %d", K);
   NHV_REQUIRE(out && x && w && x_scales && w_scales && (out_dtype == NHV_F32 || out_dtype == NHV_BF16), "linear_int8: bad arguments");
   const Product p = {(const int8_t*)x, (const int8_t*)w, x_scales, w_scales, out, x_stride, w_stride, out_stride, T, N, K, out_dtype == NHV_F32};
   const bool aligned = ((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_stride | (uintptr_t)w_stride) % 16 == 0;
-  if (aligned && way != 1) {
+  if (aligned) {
+    // us: 8 tokens, 4,096 x 4,096 / 6,144 x 4,096 / 4,096 x 12,288 through registers 5.0 / 6.3 / 10.6, on tcgen05 5.8 / 7.5 / 11.0; 16 tokens 6.2 / - / 13.6
+    // and 5.8 / 7.5 / 11.3.  128 tokens, 4,096 x 4,096 / 24,576 x 4,096 / 4,096 x 12,288: whole tiles of the weight 9.4 / 22.1 / 14.9, pairs 9.3 / 26.2 / 18.6
+    if (T <= 8) return stream_product(p, sms, stream);
     Mapped m;
     m.p = p;
-    if (way == 3 || (way == 0 && T > 256)) return pair_product(m, sms, stream);
-    const int tiles = (N + 127) / 128 * ((T + 255) / 256), kt = (K + BK - 1) / BK;
-    int parts = way >= 10 ? way - 10 : 2 * sms / tiles;
-    parts = parts < 1 ? 1 : parts > 8 ? 8 : parts;
-    return split_product(m, parts < kt ? parts : kt, stream);
+    if (T <= 128) return split_product(m, split_plan(p, sms), stream);
+    return pair_product(m, sms, stream);
   }
   const int rows = (T + TILE - 1) / TILE;
   NHV_REQUIRE(rows <= 65535, "linear_int8: %d tokens are more than a call takes", T);

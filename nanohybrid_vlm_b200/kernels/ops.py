@@ -1866,7 +1866,6 @@ def linear_simt(out, x, weight) -> None:
 # ---------------------------------------------------------------- 8-bit integers
 # Rows of 8-bit integers with a float32 scale each (integer times scale is the value), and their products.
 INT8_LONGEST_SUM = 131071
-INT8_WAY = 0
 INT8_ROW_BYTES = 16     # rows made here start at multiples of this, which the fast products read 16 bytes at a time
 
 
@@ -1970,7 +1969,7 @@ def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
     dtype = dtype_code(out)
     _same_device(out, x, x_scales, weight, weight_scales)
     call("nhv_gemm_int8", out.data_ptr(), dtype, out.stride(0) if T > 1 else N, x.data_ptr(), x.stride(0) if T > 1 else -(-K // 16) * 16, x_scales.data_ptr(),
-         weight.data_ptr(), weight.stride(0) if N > 1 else -(-K // 16) * 16, weight_scales.data_ptr(), T, N, K, _sm_count(x.device), INT8_WAY, stream_ptr())
+         weight.data_ptr(), weight.stride(0) if N > 1 else -(-K // 16) * 16, weight_scales.data_ptr(), T, N, K, _sm_count(x.device), stream_ptr())
 
 
 # ---------------------------------------------------------------- bounded waits that ran out
