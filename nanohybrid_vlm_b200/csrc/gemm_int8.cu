@@ -2,6 +2,8 @@
 //
 // The sum is exact in 32 bits (K <= 131,071: K * 128 * 128 < 2^31), so no cut of K and no order of adding changes an output: only the
 // conversion of the sum to a float and the products with the two scales round, and the store once more.
+#include <string.h>
+
 #define NHV_WAIT_LIMIT (1u << 22)
 #include "nhv_async.cuh"
 
@@ -831,13 +833,22 @@ NHV_API int nhv_gemm_int8_error() { return nhv_wait_error_take(); }
 // The device address of the error word, for kernels that report it with the step's result.
 NHV_API void* nhv_gemm_int8_error_word() { return nhv_wait_error_address(); }
 
-NHV_API int nhv_gemm_int8(void* out, int out_dtype, long long out_stride, const void* x, long long x_stride, const float* x_scales,
-                          const void* w, long long w_stride, const float* w_scales, int T, int N, int K, int sms, cudaStream_t stream) {
+// What a call is given, one after the other, in one block.
+struct ProductCall {
+  long long out, x, x_scales, w, w_scales, out_stride, x_stride, w_stride;
+  int out_dtype, T, N, K, sms;
+};
+
+NHV_API int nhv_gemm_int8(const void* given, cudaStream_t stream) {
+  ProductCall c;
+  memcpy(&c, given, sizeof(c));
+  const int T = c.T, N = c.N, K = c.K, sms = c.sms;
   if (T == 0 || N == 0) return 0;
   NHV_REQUIRE(T > 0 && N > 0 && K > 0 && K <= 131071, "linear_int8: a sum over 1 to 131,071 products is exact in 32 bits, not over %d", K);
-  NHV_REQUIRE(out && x && w && x_scales && w_scales && (out_dtype == NHV_F32 || out_dtype == NHV_BF16), "linear_int8: bad arguments");
-  const Product p = {(const int8_t*)x, (const int8_t*)w, x_scales, w_scales, out, x_stride, w_stride, out_stride, T, N, K, out_dtype == NHV_F32};
-  const bool aligned = ((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_stride | (uintptr_t)w_stride) % 16 == 0;
+  NHV_REQUIRE(c.out && c.x && c.w && c.x_scales && c.w_scales && (c.out_dtype == NHV_F32 || c.out_dtype == NHV_BF16) && sms > 1, "linear_int8: bad arguments");
+  const Product p = {(const int8_t*)c.x, (const int8_t*)c.w, (const float*)c.x_scales, (const float*)c.w_scales, (void*)c.out,
+                     c.x_stride, c.w_stride, c.out_stride, T, N, K, c.out_dtype == NHV_F32};
+  const bool aligned = (c.x | c.w | c.x_stride | c.w_stride) % 16 == 0;
   if (aligned) {
     // us: 8 tokens, 4,096 x 4,096 / 6,144 x 4,096 / 4,096 x 12,288 through registers 5.0 / 6.3 / 10.6, on tcgen05 5.8 / 7.5 / 11.0; 16 tokens 6.2 / - / 13.6
     // and 5.8 / 7.5 / 11.3.  128 tokens, 4,096 x 4,096 / 24,576 x 4,096 / 4,096 x 12,288: whole tiles of the weight 9.4 / 22.1 / 14.9, pairs 9.3 / 26.2 / 18.6

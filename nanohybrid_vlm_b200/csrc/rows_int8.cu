@@ -9,6 +9,8 @@
 // The quotient is rounded correctly before it is rounded to an integer (Markstein's correction of a product with the
 // reciprocal, 1990: r = t - q a exactly by one fused multiply-add, q + r / a), so rows in bfloat16 give the integers of the
 // definition, ties included.  |q| is at most 127.
+#include <string.h>
+
 #include "nhv_vec8.cuh"
 
 namespace {
@@ -28,21 +30,22 @@ struct Args {
   int write_residual;
 };
 
-// What a row's elements are divided by.  The factor m (a power of two) keeps every intermediate of rows of very small and very
+// What a row's elements are divided by.  A factor (a power of two) keeps every intermediate of rows of very small and very
 // large values in range.
 struct Divisor {
-  float m, a, inv;
+  float m, a, inv;       // m: 127 times the factor
 };
 __device__ __forceinline__ Divisor divisor_of(float a) {
   Divisor d;
-  d.m = a < 0x1p-60f ? 0x1p100f : (a > 0x1p100f ? 0x1p-100f : 1.0f);
-  d.a = a * d.m;
+  const float m = a < 0x1p-60f ? 0x1p100f : (a > 0x1p100f ? 0x1p-100f : 1.0f);
+  d.m = 127.0f * m;
+  d.a = a * m;
   d.inv = 1.0f / d.a;
   return d;
 }
 // The integer in the low byte: 1.5 * 2^23 + q has q's two's complement there, rounded to nearest, ties to even.
 __device__ __forceinline__ uint32_t rounded_byte(float y, const Divisor& d) {
-  const float t = y * d.m * 127.0f;
+  const float t = y * d.m;
   float q = t * d.inv;
   q = fmaf(fmaf(-q, d.a, t), d.inv, q);
   return __float_as_uint(q + 12582912.0f);
@@ -130,33 +133,290 @@ template <typename T, int KIND>
 int launch_any(const Args& p, int n_rows, cudaStream_t stream) {
   int threads = 32;
   while (threads < 1024 && threads * 4 < p.width) threads <<= 1;
-  if (p.width <= KEPT_WIDTH) {
+  if (KIND == ROW_NORM || p.width <= KEPT_WIDTH) {
+    NHV_REQUIRE(p.width <= KEPT_WIDTH, "rmsnorm_int8: width %d is beyond the %d floats that a row buffer holds", p.width, KEPT_WIDTH);
     static std::atomic<uint64_t> allowed{0};
     NHV_CUDA(nhv_allow_smem((const void*)rows_kernel<T, KIND, true>, KEPT_WIDTH * 4, allowed), "rows_int8");
     NHV_CUDA(nhv_launch(rows_kernel<T, KIND, true>, dim3(n_rows), dim3(threads), (size_t)p.width * 4, stream, p), "rows_int8");
   } else {
-    NHV_REQUIRE(KIND != ROW_NORM, "rmsnorm_int8: width %d is beyond the %d floats that a row buffer holds", p.width, KEPT_WIDTH);
-    NHV_CUDA(nhv_launch(rows_kernel<T, KIND == ROW_NORM ? ROW_PLAIN : KIND, false>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
+    NHV_CUDA(nhv_launch(rows_kernel<T, KIND, false>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
   }
   return 0;
 }
 
+// ---------------------------------------------------------------- widths in eights, rows on 16-byte boundaries
+// A thread keeps CH pieces of eight elements of its row in registers from the one read to the one write.
+template <typename T> struct Piece;
+template <> struct Piece<bf16> {
+  uint4 v;
+  __device__ __forceinline__ void load(const void* row, int i) { v = reinterpret_cast<const uint4*>(row)[i]; }
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[2 * i] = __uint_as_float(w[i] << 16);
+      o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Piece<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const void* row, int i) {
+    a = reinterpret_cast<const float4*>(row)[2 * i];
+    b = reinterpret_cast<const float4*>(row)[2 * i + 1];
+  }
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+    o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
+  }
+};
+
+template <typename T, int KIND, int CH, int MOST>
+__global__ void __launch_bounds__(MOST) rows8_kernel(const Args p) {
+  __shared__ float sums[32];
+  __shared__ uint32_t tops[32];
+  pdl_prologue();
+  const long long r = blockIdx.x;
+  const int pieces = p.width >> 3;
+  const T* x = reinterpret_cast<const T*>(p.x) + r * p.x_stride;
+  T* residual = KIND == ROW_NORM && p.residual ? reinterpret_cast<T*>(p.residual) + r * (long long)p.width : nullptr;
+  Piece<T> one[CH], two[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c < pieces) {
+      one[i].load(x, c);
+      if (KIND == ROW_UNIT) two[i].load(x + p.width, c);
+      if (KIND == ROW_NORM && residual) two[i].load(residual, c);
+    }
+  }
+  float y[CH][8];
+  float ss = 0.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c >= pieces) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[i][e] = 0.f;
+      continue;
+    }
+    one[i].get(y[i]);
+    if (KIND == ROW_UNIT || (KIND == ROW_NORM && residual)) {
+      float u[8];
+      two[i].get(u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[i][e] = KIND == ROW_UNIT ? silu_times<T>(y[i][e], u[e]) : y[i][e] + u[e];
+      if (KIND == ROW_NORM && p.write_residual) nhv_store8(residual + 8 * c, y[i]);
+    }
+    if (KIND == ROW_NORM) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(y[i][e], y[i][e], ss);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, magnitude(y[i][e]));
+    }
+  }
+  if (KIND == ROW_NORM) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (c < pieces) one[i].load(p.weight, c);                  // on its way beside the sum
+    }
+    const float rstd = 1.0f / sqrtf(all_sum(ss, sums) / (float)p.width + p.eps);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      if (threadIdx.x + i * blockDim.x >= pieces) continue;
+      float w[8];
+      one[i].get(w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[i][e] = y[i][e] * rstd * (w[e] + p.weight_offset);
+        top = max(top, magnitude(y[i][e]));
+      }
+    }
+  }
+  const float a = __uint_as_float(all_max(top, tops));
+  const bool finite = a < __int_as_float(0x7f800000), some = finite && a > 0.f;
+  if (threadIdx.x == 0) p.scales[r] = finite ? a / 127.0f : __int_as_float(0x7fc00000);
+  const Divisor d = divisor_of(some ? a : 1.0f);
+  int8_t* q = p.q + r * p.q_stride;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c >= pieces) continue;
+    uint2 out = make_uint2(0, 0);
+    if (some) {
+      uint32_t b[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = rounded_byte(y[i][e], d);
+      out = make_uint2(four_bytes(b[0], b[1], b[2], b[3]), four_bytes(b[4], b[5], b[6], b[7]));
+    }
+    *reinterpret_cast<uint2*>(q + 8 * c) = out;
+  }
+}
+
+// Wider rows: the row in 32 bits in shared memory, so that two blocks share an SM and one reads while the other writes.
+constexpr int WIDE_THREADS = 512;
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
+template <typename T, int KIND>
+__global__ void __launch_bounds__(WIDE_THREADS, 2) rows8_wide_kernel(const Args p) {
+  extern __shared__ float4 kept[];               // first and second halves of the eights: neighbouring threads, neighbouring 16 bytes
+  __shared__ float sums[32];
+  __shared__ uint32_t tops[32];
+  pdl_prologue();
+  const long long r = blockIdx.x;
+  const int pieces = p.width >> 3;
+  const T* x = reinterpret_cast<const T*>(p.x) + r * p.x_stride;
+  T* residual = KIND == ROW_NORM && p.residual ? reinterpret_cast<T*>(p.residual) + r * (long long)p.width : nullptr;
+  float ss = 0.f;
+  uint32_t top = 0;
+  const bool pair = KIND == ROW_UNIT || (KIND == ROW_NORM && residual);
+  auto take = [&](int c, const Piece<T>& one, const Piece<T>& two) {
+    float y[8], u[8];
+    one.get(y);
+    if (pair) {
+      two.get(u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = KIND == ROW_UNIT ? silu_times<T>(y[e], u[e]) : y[e] + u[e];
+      if (KIND == ROW_NORM && p.write_residual) nhv_store8(residual + 8 * c, y);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (KIND == ROW_NORM) ss = fmaf(y[e], y[e], ss);
+      else top = max(top, magnitude(y[e]));
+    }
+    kept[c] = make_float4(y[0], y[1], y[2], y[3]);
+    kept[pieces + c] = make_float4(y[4], y[5], y[6], y[7]);
+  };
+  if (sizeof(T) == 2) {
+    // A thread's pieces of both operands lie where its sums will, all of them on their way at once.
+    const T* second = KIND == ROW_UNIT ? x + p.width : residual;
+    for (int c = threadIdx.x; c < pieces; c += WIDE_THREADS) {
+      copy16(&kept[c], x + 8 * c);
+      if (pair) copy16(&kept[pieces + c], second + 8 * c);
+    }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+#pragma unroll 2
+    for (int c = threadIdx.x; c < pieces; c += WIDE_THREADS) {
+      Piece<T> one, two;
+      one.load(&kept[c], 0);
+      if (pair) two.load(&kept[pieces + c], 0);
+      take(c, one, two);
+    }
+  } else {
+    constexpr int CH = 2;
+    for (int c0 = threadIdx.x; c0 < pieces; c0 += CH * WIDE_THREADS) {
+      Piece<T> one[CH], two[CH];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int c = c0 + i * WIDE_THREADS;
+        if (c >= pieces) continue;
+        one[i].load(x, c);
+        if (KIND == ROW_UNIT) two[i].load(x + p.width, c);
+        if (KIND == ROW_NORM && residual) two[i].load(residual, c);
+      }
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        if (c0 + i * WIDE_THREADS < pieces) take(c0 + i * WIDE_THREADS, one[i], two[i]);
+    }
+  }
+  if (KIND == ROW_NORM) {
+    const float rstd = 1.0f / sqrtf(all_sum(ss, sums) / (float)p.width + p.eps);
+    for (int c = threadIdx.x; c < pieces; c += WIDE_THREADS) {
+      Piece<T> weight;
+      weight.load(p.weight, c);
+      float w[8];
+      weight.get(w);
+      const float4 a = kept[c], b = kept[pieces + c];
+      float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = y[e] * rstd * (w[e] + p.weight_offset);
+        top = max(top, magnitude(y[e]));
+      }
+      kept[c] = make_float4(y[0], y[1], y[2], y[3]);
+      kept[pieces + c] = make_float4(y[4], y[5], y[6], y[7]);
+    }
+  }
+  const float a = __uint_as_float(all_max(top, tops));
+  const bool finite = a < __int_as_float(0x7f800000), some = finite && a > 0.f;
+  if (threadIdx.x == 0) p.scales[r] = finite ? a / 127.0f : __int_as_float(0x7fc00000);
+  const Divisor d = divisor_of(some ? a : 1.0f);
+  int8_t* q = p.q + r * p.q_stride;
+  for (int c = threadIdx.x; c < pieces; c += WIDE_THREADS) {
+    const float4 y = kept[c], z = kept[pieces + c];
+    uint2 out = make_uint2(0, 0);
+    if (some)
+      out = make_uint2(four_bytes(rounded_byte(y.x, d), rounded_byte(y.y, d), rounded_byte(y.z, d), rounded_byte(y.w, d)),
+                       four_bytes(rounded_byte(z.x, d), rounded_byte(z.y, d), rounded_byte(z.z, d), rounded_byte(z.w, d)));
+    *reinterpret_cast<uint2*>(q + 8 * c) = out;
+  }
+}
+
+template <typename T, int KIND, int CH>
+int launch_eights(const Args& p, int n_rows, cudaStream_t stream) {
+  const int threads = ((p.width / 8 + CH - 1) / CH + 31) / 32 * 32;
+  if (threads <= 256)
+    NHV_CUDA(nhv_launch(rows8_kernel<T, KIND, CH, 256>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
+  else
+    NHV_CUDA(nhv_launch(rows8_kernel<T, KIND, CH, 1024>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
+  return 0;
+}
+
+// Which kernel and how many pieces a thread; us a call for 1 / 2 / 4 pieces, bfloat16: the norm of 8 rows of 4,096 2.0 / 2.1 / 2.3, of 512 5.3 / 5.8 /
+// 5.5, of 2,048 14.1 / 11.9 / 12.4, of 8,191 of 5,120 64 / 52 / 50; 24,576 plain rows of 4,096 74 / 62 / 58; the unit of 8 rows of 12,288 2.8 / 2.7 / 3.0,
+// of 2,048 27.7 / 27.8 / 25.7.  Kept in shared memory / registers: the unit of 2,048 rows of 16,384 32 / 34, of 25,600 54 / 74, of 512 rows 17 / 22, of 8 (the
+// registers' way) 4.9; of 2,048 rows of 4,096 and 12,288 48 / 30 (8,192 rows) and 27 / 25.  In 32 bits the way goes by the width alone: it decides in which order a norm's squares are added.
+template <typename T, int KIND>
+int launch_row(const Args& p, int n_rows, cudaStream_t stream) {
+  const long long item = sizeof(T);
+  const bool aligned = p.width % 8 == 0 && ((uintptr_t)p.x | (uintptr_t)(p.x_stride * item) | (uintptr_t)(p.width * item) | (uintptr_t)p.residual |
+                                            (uintptr_t)p.weight) % 16 == 0 && ((uintptr_t)p.q | (uintptr_t)p.q_stride) % 8 == 0;
+  if (!aligned || p.width > KEPT_WIDTH) return launch_any<T, KIND>(p, n_rows, stream);
+  const int pieces = p.width / 8;
+  if (pieces > (sizeof(T) == 2 && n_rows < 512 ? 4096 : 2047)) {
+    static std::atomic<uint64_t> allowed{0};
+    NHV_CUDA(nhv_allow_smem((const void*)rows8_wide_kernel<T, KIND>, KEPT_WIDTH * 4, allowed), "rows_int8");
+    NHV_CUDA(nhv_launch(rows8_wide_kernel<T, KIND>, dim3(n_rows), dim3(WIDE_THREADS), (size_t)p.width * 4, stream, p), "rows_int8");
+    return 0;
+  }
+  int each = sizeof(T) == 4 ? (pieces <= 256 ? 1 : 2) : n_rows < 1024 ? 1 : KIND == ROW_NORM && pieces <= 512 ? 2 : 4;
+  while (each * 1024 < pieces) each *= 2;
+  while (each > 1 && pieces <= 32 * (each / 2)) each /= 2;
+  if (each == 1) return launch_eights<T, KIND, 1>(p, n_rows, stream);
+  if (each == 2) return launch_eights<T, KIND, 2>(p, n_rows, stream);
+  return launch_eights<T, KIND, 4>(p, n_rows, stream);
+}
+
 template <typename T>
 int launch_kind(int kind, const Args& p, int n_rows, cudaStream_t stream) {
-  if (kind == ROW_PLAIN) return launch_any<T, ROW_PLAIN>(p, n_rows, stream);
-  if (kind == ROW_NORM) return launch_any<T, ROW_NORM>(p, n_rows, stream);
-  return launch_any<T, ROW_UNIT>(p, n_rows, stream);
+  if (kind == ROW_PLAIN) return launch_row<T, ROW_PLAIN>(p, n_rows, stream);
+  if (kind == ROW_NORM) return launch_row<T, ROW_NORM>(p, n_rows, stream);
+  return launch_row<T, ROW_UNIT>(p, n_rows, stream);
 }
 
 }  // namespace
 
+// What a call is given, one after the other, in one block.
+struct RowsCall {
+  long long q, scales, x, residual, weight, q_stride, x_stride;
+  int kind, dtype, n_rows, width, write_residual;
+  float eps, weight_offset;
+};
+
 // kind: 0 the rows of x, 1 their RMS norm (residual may be null), 2 silu(first half) * second half of rows of 2 * width.
-NHV_API int nhv_rows_int8(int kind, int dtype, void* q, long long q_stride, float* scales, const void* x, long long x_stride, void* residual,
-                          const void* weight, int n_rows, int width, float eps, float weight_offset, int write_residual, cudaStream_t stream) {
-  if (n_rows == 0) return 0;
-  NHV_REQUIRE(n_rows > 0 && width > 0 && width <= (1 << 30) && q && scales && x, "rows_int8: bad sizes");
-  NHV_REQUIRE(kind >= ROW_PLAIN && kind <= ROW_UNIT && (kind != ROW_NORM || weight), "rows_int8: bad arguments");
-  NHV_REQUIRE(dtype == NHV_F32 || dtype == NHV_BF16, "rows_int8: unknown dtype %d", dtype);
-  const Args p = {(int8_t*)q, scales, x, residual, weight, q_stride, x_stride, width, eps, weight_offset, write_residual};
-  return dtype == NHV_F32 ? launch_kind<float>(kind, p, n_rows, stream) : launch_kind<bf16>(kind, p, n_rows, stream);
+NHV_API int nhv_rows_int8(const void* given, cudaStream_t stream) {
+  RowsCall c;
+  memcpy(&c, given, sizeof(c));
+  if (c.n_rows == 0) return 0;
+  NHV_REQUIRE(c.n_rows > 0 && c.width > 0 && c.width <= (1 << 30) && c.q && c.scales && c.x, "rows_int8: bad sizes");
+  NHV_REQUIRE(c.kind >= ROW_PLAIN && c.kind <= ROW_UNIT && (c.kind != ROW_NORM || c.weight), "rows_int8: bad arguments");
+  NHV_REQUIRE(c.dtype == NHV_F32 || c.dtype == NHV_BF16, "rows_int8: unknown dtype %d", c.dtype);
+  const Args p = {(int8_t*)c.q, (float*)c.scales, (const void*)c.x, (void*)c.residual, (const void*)c.weight, c.q_stride, c.x_stride, c.width,
+                  c.eps, c.weight_offset, c.write_residual};
+  return c.dtype == NHV_F32 ? launch_kind<float>(c.kind, p, c.n_rows, stream) : launch_kind<bf16>(c.kind, p, c.n_rows, stream);
 }

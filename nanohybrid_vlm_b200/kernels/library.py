@@ -91,8 +91,8 @@ _SIGNATURES = {
     "nhv_attention_scored_most_kilobytes": [ctypes.c_char_p],
     "nhv_select_keys": [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, P],
     "nhv_move_keys": [P, P, P, P, I, I, P, P, I, I, I, I, I, I, P],
-    "nhv_rows_int8": [I, I, P, ctypes.c_longlong, P, P, ctypes.c_longlong, P, P, I, I, F, F, I, P],
-    "nhv_gemm_int8": [P, I, ctypes.c_longlong, P, ctypes.c_longlong, P, P, ctypes.c_longlong, P, I, I, I, I, P],
+    "nhv_rows_int8": [ctypes.c_char_p, P],
+    "nhv_gemm_int8": [ctypes.c_char_p, P],
     "nhv_decay_lowrank": [I, P, P, I, P, P, I, I, I, P],
 }
 

@@ -1871,8 +1871,7 @@ INT8_ROW_BYTES = 16     # rows made here start at multiples of this, which the f
 
 def new_int8(rows: int, width: int, device) -> torch.Tensor:
     """An uninitialised int8 matrix [rows, width] whose rows start at multiples of 16 bytes, as ``linear_int8`` reads them fastest."""
-    pitch = -(-width // INT8_ROW_BYTES) * INT8_ROW_BYTES
-    return torch.empty((rows, pitch), dtype=torch.int8, device=device)[:, :width]
+    return torch.empty_strided((rows, width), (-(-width // INT8_ROW_BYTES) * INT8_ROW_BYTES, 1), dtype=torch.int8, device=device)
 
 
 def _same_device(*tensors) -> None:
@@ -1885,8 +1884,10 @@ def _same_device(*tensors) -> None:
 
 
 def _int8_rows_ok(t, rows: int, width: int) -> bool:
-    return (t.dtype is torch.int8 and t.shape == (rows, width) and (t.stride(1) == 1 or width == 1)
-            and (rows <= 1 or t.stride(0) >= width))
+    if t.dtype is not torch.int8 or t.shape != (rows, width):
+        return False
+    stride, step = t.stride()
+    return (step == 1 or width == 1) and (stride >= width or rows <= 1)
 
 
 def _check_int8_rows(name: str, t, rows: int, width: int) -> None:
@@ -1895,9 +1896,16 @@ def _check_int8_rows(name: str, t, rows: int, width: int) -> None:
                           f"{tuple(t.shape)} {t.dtype} with strides {t.stride()}")
 
 
+def _scales_ok(t, n: int) -> bool:
+    return t.dtype is torch.float32 and t.shape == (n,) and (n <= 1 or t.stride(0) == 1)
+
+
 def _check_scales(name: str, t, n: int) -> None:
-    if t.dtype is not torch.float32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+    if not _scales_ok(t, n):
         raise KernelError(f"{name} are {n} float32 numbers side by side, not {tuple(t.shape)} {t.dtype}")
+
+
+_ROWS_CALL = struct.Struct("=7q5i2f")
 
 
 def _rows_int8(kind: int, q, scales, x, rows: int, width: int, x_stride: int, residual=None, weight=None, eps: float = 0.0, offset: float = 0.0,
@@ -1908,8 +1916,9 @@ def _rows_int8(kind: int, q, scales, x, rows: int, width: int, x_stride: int, re
         raise KernelError("rows of no elements have no scale")
     dtype = dtype_code(x)
     _same_device(q, scales, x, residual, weight)
-    call("nhv_rows_int8", kind, dtype, q.data_ptr(), q.stride(0) if rows > 1 else width, scales.data_ptr(), x.data_ptr(), x_stride,
-         _ptr(residual), _ptr(weight), rows, width, float(eps), float(offset), int(write_residual), stream_ptr())
+    call("nhv_rows_int8", _ROWS_CALL.pack(
+        q.data_ptr(), scales.data_ptr(), x.data_ptr(), residual.data_ptr() if residual is not None else 0, weight.data_ptr() if weight is not None else 0,
+        q.stride(0) if rows > 1 else width, x_stride, kind, dtype, rows, width, write_residual, eps, offset), stream_ptr())
 
 
 def quantize_rows(q, scales, x) -> None:
@@ -1950,6 +1959,9 @@ def silu_mul_int8(q, scales, gate_up) -> None:
     _rows_int8(2, q, scales, gate_up, rows, inter, 2 * inter)
 
 
+_PRODUCT_CALL = struct.Struct("=8q5i")
+
+
 def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
     """out[T, N] = (x[T, K] @ weight[N, K]^T) * x_scales[:, None] * weight_scales[None] for int8 x and weight, float32 scales and out in
     bfloat16 or float32.  The sums are exact (K up to 131,071), so an output does not depend on how the work is cut or batched.
@@ -1962,14 +1974,17 @@ def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
     _check_int8_rows("the weight's rows", weight, N, K)
     _check_scales("x_scales", x_scales, T)
     _check_scales("weight_scales", weight_scales, N)
-    if out.shape != (T, N) or (out.stride(1) != 1 and N > 1) or (T > 1 and out.stride(0) < N):
+    stride, step = out.stride()
+    if out.shape != (T, N) or (step != 1 and N > 1) or (stride < N and T > 1):
         raise KernelError(f"out is [{T}, {N}] with neighbouring columns and rows that do not overlap, not {tuple(out.shape)} with strides {out.stride()}")
     if not 0 < K <= INT8_LONGEST_SUM:
         raise KernelError(f"a sum over 1 to {INT8_LONGEST_SUM} products of 8-bit integers is exact in 32 bits, not over {K}")
     dtype = dtype_code(out)
     _same_device(out, x, x_scales, weight, weight_scales)
-    call("nhv_gemm_int8", out.data_ptr(), dtype, out.stride(0) if T > 1 else N, x.data_ptr(), x.stride(0) if T > 1 else -(-K // 16) * 16, x_scales.data_ptr(),
-         weight.data_ptr(), weight.stride(0) if N > 1 else -(-K // 16) * 16, weight_scales.data_ptr(), T, N, K, _sm_count(x.device), stream_ptr())
+    pitch = -(-K // INT8_ROW_BYTES) * INT8_ROW_BYTES                 # of a single row, whose stride may be anything
+    call("nhv_gemm_int8", _PRODUCT_CALL.pack(
+        out.data_ptr(), x.data_ptr(), x_scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), stride if T > 1 else N, x.stride(0) if T > 1 else pitch,
+        weight.stride(0) if N > 1 else pitch, dtype, T, N, K, _sm_count(x.device)), stream_ptr())
 
 
 # ---------------------------------------------------------------- bounded waits that ran out
