@@ -17,6 +17,7 @@ struct Product {
   void* out;
   long long x_stride, w_stride, out_stride;
   int T, N, K, out_f32;
+  int boxes;             // rows of out start at multiples of 16 bytes
 };
 
 __device__ __forceinline__ float scaled(int sum, float xs, float ws) { return (float)sum * xs * ws; }
@@ -29,55 +30,38 @@ __device__ __forceinline__ void store_out(const Product& p, int t, int n, float 
     reinterpret_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(v);
 }
 
-// ---------------------------------------------------------------- any size, any alignment
-// A tile of 64 x 64 outputs a block, 64 columns of K at a time through shared memory, four products of bytes an instruction.
-constexpr int TILE = 64, WORDS = 16;
-
-__device__ __forceinline__ int word_at(const int8_t* row, int k, int K) {
-  uint32_t v = 0;
+// ---------------------------------------------------------------- rows that start anywhere
+// Laid out anew with rows at multiples of 16 bytes, which all products read: a thread's 16 bytes of the copy come from the words that hold
+// them, and no word is read that holds none of the row's.
+__global__ void __launch_bounds__(256) align_rows_kernel(uint4* __restrict__ out, const int8_t* __restrict__ in, long long stride, long long pieces, int per_row,
+                                                         int K) {
+  pdl_prologue();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= pieces) return;
+  const long long row = i / per_row;
+  const int k = (int)(i - row * per_row) * 16;
+  const uintptr_t from = (uintptr_t)in + row * stride + k, end = from + min(16, K - k);
+  const uint32_t shift = (uint32_t)(from & 3) * 8;
+  uint32_t w[5];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (k + i < K) v |= (uint32_t)(uint8_t)row[k + i] << (8 * i);
-  return (int)v;
+  for (int j = 0; j < 5; ++j) {
+    const uintptr_t at = (from & ~(uintptr_t)3) + 4 * j;
+    w[j] = at < end ? *reinterpret_cast<const uint32_t*>(at) : 0u;
+  }
+  out[i] = make_uint4(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift), __funnelshift_r(w[2], w[3], shift),
+                      __funnelshift_r(w[3], w[4], shift));
 }
 
-__global__ void __launch_bounds__(256) product_any_kernel(const Product p) {
-  __shared__ int xs[TILE][WORDS + 1], ws[TILE][WORDS + 1];
-  pdl_prologue();
-  const int t0 = blockIdx.y * TILE, n0 = blockIdx.x * TILE, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int sum[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += 4 * WORDS) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < TILE * WORDS; i += 256) {
-      const int r = i / WORDS, c = i % WORDS;
-      xs[r][c] = t0 + r < p.T ? word_at(p.x + (long long)(t0 + r) * p.x_stride, k0 + 4 * c, p.K) : 0;
-      ws[r][c] = n0 + r < p.N ? word_at(p.w + (long long)(n0 + r) * p.w_stride, k0 + 4 * c, p.K) : 0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < WORDS; ++c) {
-      int a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = xs[ty + 16 * i][c];
-        b[i] = ws[tx + 16 * i][c];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum[i][j] = __dp4a(a[i], b[j], sum[i][j]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = t0 + ty + 16 * i;
-    if (t >= p.T) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx + 16 * j;
-      if (n < p.N) store_out(p, t, n, scaled(sum[i][j], p.x_scales[t], p.w_scales[n]));
-    }
-  }
+int align_rows(const int8_t** rows, long long* stride, void* copy, int n, int K, cudaStream_t stream) {
+  if (((uintptr_t)*rows | (uintptr_t)*stride) % 16 == 0) return 0;
+  NHV_REQUIRE(copy && (uintptr_t)copy % 16 == 0, "linear_int8: rows that start between multiples of 16 bytes come with room for a copy");
+  const int per_row = (K + 15) / 16;
+  const long long pieces = (long long)n * per_row, blocks = (pieces + 255) / 256;
+  NHV_REQUIRE(blocks < (1LL << 31), "linear_int8: too many rows");
+  NHV_CUDA(nhv_launch(align_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, (uint4*)copy, *rows, *stride, pieces, per_row, K), "linear_int8");
+  *rows = (const int8_t*)copy;
+  *stride = (long long)per_row * 16;
+  return 0;
 }
 
 // ---------------------------------------------------------------- tcgen05 (8-bit integers, 32-bit sums in tensor memory)
@@ -193,7 +177,7 @@ constexpr int BK = 128;                // columns of K per stage: one 128-byte s
 constexpr int UMMA_K = 32;
 
 struct alignas(64) Mapped {
-  CUtensorMap w_map, x_map;
+  CUtensorMap w_map, x_map, out_map;
   Product p;
   int nt;             // tokens of a tile: the boxes of x_map, a multiple of 16
   int tiles_t, tiles_n, group;
@@ -500,48 +484,64 @@ __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __gr
 // ---- many tokens: pairs of blocks, 256 tokens on the MMA's M axis (128 a block), TN outputs on its N axis (TN / 2 rows of the weight in
 // each block's shared memory), tiles handed out in turn to a grid of one pair for two SMs.
 constexpr int PAIR_THREADS = 320;      // producer warp, MMA warp, eight epilogue warps
+constexpr int TURN = 2560;             // bytes of a warp's outputs on their way out: 32 rows of 64 bytes, or of 17 floats; whole 512s for the swizzle
 template <int TN>
 struct Pair {
   static constexpr int X_BYTES = 128 * BK, W_BYTES = TN / 2 * BK, STAGE = X_BYTES + W_BYTES;      // a block's half of a stage
   static constexpr int STAGES = 196608 / STAGE;
-  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 8 * (TN / 2) * 4 + (2 * STAGES + 4) * 8 + 16;
+  static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + 8 * (TN / 2) * 4 + 8 * TURN + (2 * STAGES + 4) * 8 + 16;
 };
 
-__device__ __forceinline__ void store_row32(const Product& p, long long at, const float (&v)[32], int room) {
-  if (p.out_f32) {
-    float* o = reinterpret_cast<float*>(p.out) + at;
-    if (room >= 32 && ((uintptr_t)o & 31) == 0) {
+// A warp's 32 outputs of 32 rows from (t0, n0): 64 bytes of each row at a time through 2 KB of shared memory in the 64-byte swizzle, from where
+// a TMA store takes them while the warp goes on; what lies behind out's rows and columns is not written.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, unsigned char* box, const uint32_t (&w)[16], int n, int t, int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");      // the last one has read the box
+  __syncwarp();
+  const uint32_t at = smem_u32(box) + lane * 64, turn = (lane >> 1) & 3;
 #pragma unroll
-      for (int i = 0; i < 32; i += 8)
-        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(o + i), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]),
-                     "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7]) : "memory");
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < room) o[i] = v[i];
-    }
-    return;
-  }
-  bf16* o = reinterpret_cast<bf16*>(p.out) + at;
+  for (int i = 0; i < 4; ++i)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at + ((i ^ turn) << 4)), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]),
+                 "r"(w[4 * i + 3]) : "memory");
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  __syncwarp();
+  if (lane == 0)
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
+                 "cp.async.bulk.commit_group;\n" ::"l"((uint64_t)map), "r"(n), "r"(t), "r"(smem_u32(box)) : "memory");
+}
+__device__ __forceinline__ void store_rows32(const CUtensorMap* map, unsigned char* box, const float (&v)[32], bool f32, int n0, int t0, int lane) {
   uint32_t w[16];
+  if (f32) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  if (room >= 32 && ((uintptr_t)o & 31) == 0) {
+    for (int h = 0; h < 32; h += 16) {
 #pragma unroll
-    for (int i = 0; i < 16; i += 8)
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(o + 2 * i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]),
-                   "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7]) : "memory");
-  } else if (room >= 32 && ((uintptr_t)o & 3) == 0) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) reinterpret_cast<uint32_t*>(o)[i] = w[i];
+      for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[h + i]);
+      store_box(map, box, w, n0 + h, t0, lane);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < room) o[i] = __float2bfloat16_rn(v[i]);
+    for (int i = 0; i < 16; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    store_box(map, box, w, n0, t0, lane);
   }
+}
+// The same where rows start at odd places: 16 columns of two rows at a time, lanes side by side.
+template <typename O>
+__device__ __forceinline__ void store_turned(O* out, const Product& p, float* mine, const float (&v)[32], int t0, int n0, int lane) {
+#pragma unroll
+  for (int h = 0; h < 32; h += 16) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) mine[lane * 17 + j] = v[h + j];
+    __syncwarp();
+    const int n = n0 + h + (lane & 15), t = t0 + (lane >> 4), rows = n < p.N ? p.T - t : 0;
+    O* at = out + (long long)t * p.out_stride + n;
+#pragma unroll
+    for (int r = 0; r < 32; r += 2)
+      if (r < rows) at[r * p.out_stride] = from_f32<O>(mine[(r + (lane >> 4)) * 17 + (lane & 15)]);
+  }
+  __syncwarp();
 }
 
 // The tile'th tile: `group` tiles of tokens after one another beside the same rows of the weight, then the next rows.
@@ -557,7 +557,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) pro
   constexpr int STAGES = Pair<TN>::STAGES, STAGE = Pair<TN>::STAGE, X_BYTES = Pair<TN>::X_BYTES, HALF = TN / 2;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* ring = smem_unaligned + ((1024 - (smem_u32(smem_unaligned) & 1023)) & 1023);
-  float* scales = reinterpret_cast<float*>(ring + (size_t)STAGES * STAGE);      // [8 warps][HALF]
+  unsigned char* boxes = ring + (size_t)STAGES * STAGE;                // [8 warps][TURN]
+  float* scales = reinterpret_cast<float*>(boxes + 8 * TURN);      // [8 warps][HALF]
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + 8 * HALF);        // used in block 0, for both
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;      // [2]
@@ -683,10 +684,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) pro
           v[j + 2] = scaled(r[j + 2], xs, ws.z);
           v[j + 3] = scaled(r[j + 3], xs, ws.w);
         }
-        if (t < p.T && n0 + c < p.N) store_row32(p, (long long)t * p.out_stride + n0 + c, v, p.N - n0 - c);
+        if (n0 + c >= p.N || t - lane >= p.T) continue;
+        unsigned char* box = boxes + (warp - 2) * TURN;
+        if (p.boxes)
+          store_rows32(&m.out_map, box, v, p.out_f32, n0 + c, t - lane, lane);
+        else if (p.out_f32)
+          store_turned(reinterpret_cast<float*>(p.out), p, reinterpret_cast<float*>(box), v, t - lane, n0 + c, lane);
+        else
+          store_turned(reinterpret_cast<bf16*>(p.out), p, reinterpret_cast<float*>(box), v, t - lane, n0 + c, lane);
       }
       __syncwarp();
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
     if (!ok) s_abort = 1;
   }
   __syncthreads();
@@ -696,8 +705,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) pro
   if (warp == 1) tmem_dealloc<2>(tmem_base, 512);
 }
 
-// A tensor map over rows of bytes, read in boxes of 128 bytes x `rows_of_box` rows with the 128-byte swizzle.
-bool make_map(CUtensorMap* map, const void* base, long long rows, long long bytes, long long stride, int rows_of_box) {
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long columns, long long stride_bytes, int box_columns,
+                int box_rows, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   static PFN_cuTensorMapEncodeTiled_v12000 encode = []() -> PFN_cuTensorMapEncodeTiled_v12000 {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -705,10 +714,21 @@ bool make_map(CUtensorMap* map, const void* base, long long rows, long long byte
     return (PFN_cuTensorMapEncodeTiled_v12000)fn;
   }();
   if (!encode) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
-  const cuuint32_t box[2] = {BK, (cuuint32_t)rows_of_box}, steps[2] = {1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows}, steps[2] = {1, 1};
+  return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Rows of bytes, read in boxes of 128 bytes x `box_rows` rows with the 128-byte swizzle.
+bool make_map(CUtensorMap* map, const void* base, long long rows, long long bytes, long long stride, int box_rows) {
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, bytes, stride, BK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+// The output, written in boxes of 64 bytes x 32 rows with the 64-byte swizzle.
+bool make_out_map(CUtensorMap* map, const Product& p) {
+  const int item = p.out_f32 ? 4 : 2;
+  return encode_map(map, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.out, p.T, p.N, p.out_stride * item, 64 / item, 32,
+                    CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
 struct SplitPlan {
@@ -795,8 +815,8 @@ int launch_pair(Mapped& m, int sms, cudaStream_t stream) {
   m.tiles_t = (p.T + 255) / 256;
   m.tiles_n = (p.N + TN - 1) / TN;
   m.group = m.tiles_t < 16 ? m.tiles_t : 16;
-  NHV_REQUIRE(make_map(&m.w_map, p.w, p.N, p.K, p.w_stride, TN / 2) && make_map(&m.x_map, p.x, p.T, p.K, p.x_stride, 128),
-              "linear_int8: cannot encode the tensor maps");
+  NHV_REQUIRE(make_map(&m.w_map, p.w, p.N, p.K, p.w_stride, TN / 2) && make_map(&m.x_map, p.x, p.T, p.K, p.x_stride, 128) &&
+              (!p.boxes || make_out_map(&m.out_map, p)), "linear_int8: cannot encode the tensor maps");
   const long long tiles = (long long)m.tiles_t * m.tiles_n;
   NHV_REQUIRE(tiles < (1LL << 30), "linear_int8: too many tiles");
   const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
@@ -835,7 +855,7 @@ NHV_API void* nhv_gemm_int8_error_word() { return nhv_wait_error_address(); }
 
 // What a call is given, one after the other, in one block.
 struct ProductCall {
-  long long out, x, x_scales, w, w_scales, out_stride, x_stride, w_stride;
+  long long out, x, x_scales, w, w_scales, x_copy, w_copy, out_stride, x_stride, w_stride;      // the copies: room for rows that start anywhere, or 0
   int out_dtype, T, N, K, sms;
 };
 
@@ -846,20 +866,16 @@ NHV_API int nhv_gemm_int8(const void* given, cudaStream_t stream) {
   if (T == 0 || N == 0) return 0;
   NHV_REQUIRE(T > 0 && N > 0 && K > 0 && K <= 131071, "linear_int8: a sum over 1 to 131,071 products is exact in 32 bits, not over %d", K);
   NHV_REQUIRE(c.out && c.x && c.w && c.x_scales && c.w_scales && (c.out_dtype == NHV_F32 || c.out_dtype == NHV_BF16) && sms > 1, "linear_int8: bad arguments");
-  const Product p = {(const int8_t*)c.x, (const int8_t*)c.w, (const float*)c.x_scales, (const float*)c.w_scales, (void*)c.out,
-                     c.x_stride, c.w_stride, c.out_stride, T, N, K, c.out_dtype == NHV_F32};
-  const bool aligned = (c.x | c.w | c.x_stride | c.w_stride) % 16 == 0;
-  if (aligned) {
-    // us: 8 tokens, 4,096 x 4,096 / 6,144 x 4,096 / 4,096 x 12,288 through registers 5.0 / 6.3 / 10.6, on tcgen05 5.8 / 7.5 / 11.0; 16 tokens 6.2 / - / 13.6
-    // and 5.8 / 7.5 / 11.3.  128 tokens, 4,096 x 4,096 / 24,576 x 4,096 / 4,096 x 12,288: whole tiles of the weight 9.4 / 22.1 / 14.9, pairs 9.3 / 26.2 / 18.6
-    if (T <= 8) return stream_product(p, sms, stream);
-    Mapped m;
-    m.p = p;
-    if (T <= 128) return split_product(m, split_plan(p, sms), stream);
-    return pair_product(m, sms, stream);
-  }
-  const int rows = (T + TILE - 1) / TILE;
-  NHV_REQUIRE(rows <= 65535, "linear_int8: %d tokens are more than a call takes", T);
-  NHV_CUDA(nhv_launch(product_any_kernel, dim3((N + TILE - 1) / TILE, rows), dim3(256), 0, stream, p), "linear_int8");
-  return 0;
+  Product p = {(const int8_t*)c.x, (const int8_t*)c.w, (const float*)c.x_scales, (const float*)c.w_scales, (void*)c.out,
+                     c.x_stride, c.w_stride, c.out_stride, T, N, K, c.out_dtype == NHV_F32,
+                     (c.out | c.out_stride * (c.out_dtype == NHV_F32 ? 4 : 2)) % 16 == 0};
+  if (int e = align_rows(&p.x, &p.x_stride, (void*)c.x_copy, T, K, stream)) return e;
+  if (int e = align_rows(&p.w, &p.w_stride, (void*)c.w_copy, N, K, stream)) return e;
+  // us: 8 tokens, 4,096 x 4,096 / 6,144 x 4,096 / 4,096 x 12,288 through registers 5.0 / 6.3 / 10.6, on tcgen05 5.8 / 7.5 / 11.0; 16 tokens 6.2 / - / 13.6 and 5.8 /
+  // 7.5 / 11.3.  128 tokens, 4,096 x 4,096 / 24,576 x 4,096 / 4,096 x 12,288: whole tiles of the weight 9.4 / 22.1 / 14.9, pairs 9.3 / 26.2 / 18.6.
+  if (T <= 8) return stream_product(p, sms, stream);
+  Mapped m;
+  m.p = p;
+  if (T <= 128) return split_product(m, split_plan(p, sms), stream);
+  return pair_product(m, sms, stream);
 }

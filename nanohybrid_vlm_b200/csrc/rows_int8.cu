@@ -399,6 +399,60 @@ int launch_kind(int kind, const Args& p, int n_rows, cudaStream_t stream) {
   return launch_row<T, ROW_UNIT>(p, n_rows, stream);
 }
 
+// ---------------------------------------------------------------- and back
+// out[r, c] = q[r, c] * scale[r], rounded once.  Bounded by memory: 16 integers a thread where the rows allow it (24,576 rows of 4,096 to
+// bfloat16 48 us, 6.2 TB/s).
+struct BackArgs {
+  const int8_t* q;
+  const float* scales;
+  void* out;
+  long long q_stride, out_stride;
+  int n_rows, width;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) values16_kernel(const BackArgs p) {
+  pdl_prologue();
+  const int pieces = p.width >> 4;
+  const long long step = (long long)gridDim.x * 256, all = (long long)p.n_rows * pieces;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
+    const long long r = i / pieces;
+    const int c = (int)(i - r * pieces) * 16;
+    const uint4 v = *reinterpret_cast<const uint4*>(p.q + r * p.q_stride + c);
+    const float s = p.scales[r];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    T* out = reinterpret_cast<T*>(p.out) + r * p.out_stride + c;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = (float)(int8_t)(w[2 * h + (e >> 2)] >> (8 * (e & 3))) * s;
+      nhv_store8(out + 8 * h, y);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) values_kernel(const BackArgs p) {
+  pdl_prologue();
+  for (long long r = blockIdx.x; r < p.n_rows; r += gridDim.x) {
+    const float s = p.scales[r];
+    for (int c = threadIdx.x; c < p.width; c += 256) reinterpret_cast<T*>(p.out)[r * p.out_stride + c] = from_f32<T>((float)p.q[r * p.q_stride + c] * s);
+  }
+}
+
+template <typename T>
+int launch_back(const BackArgs& p, cudaStream_t stream) {
+  const bool eights = p.width % 16 == 0 && ((uintptr_t)p.q | (uintptr_t)p.q_stride | (uintptr_t)p.out | (uintptr_t)(p.out_stride * sizeof(T))) % 16 == 0;
+  if (eights) {
+    const long long blocks = ((long long)p.n_rows * (p.width / 16) + 255) / 256;
+    NHV_CUDA(nhv_launch(values16_kernel<T>, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, stream, p), "dequantize_rows");
+  } else {
+    NHV_CUDA(nhv_launch(values_kernel<T>, dim3(p.n_rows), dim3(256), 0, stream, p), "dequantize_rows");
+  }
+  return 0;
+}
+
 }  // namespace
 
 // What a call is given, one after the other, in one block.
@@ -419,4 +473,12 @@ NHV_API int nhv_rows_int8(const void* given, cudaStream_t stream) {
   const Args p = {(int8_t*)c.q, (float*)c.scales, (const void*)c.x, (void*)c.residual, (const void*)c.weight, c.q_stride, c.x_stride, c.width,
                   c.eps, c.weight_offset, c.write_residual};
   return c.dtype == NHV_F32 ? launch_kind<float>(c.kind, p, c.n_rows, stream) : launch_kind<bf16>(c.kind, p, c.n_rows, stream);
+}
+
+NHV_API int nhv_rows_from_int8(void* out, int dtype, long long out_stride, const void* q, long long q_stride, const float* scales, int n_rows, int width,
+                               cudaStream_t stream) {
+  if (n_rows == 0 || width == 0) return 0;
+  NHV_REQUIRE(n_rows > 0 && width > 0 && out && q && scales && (dtype == NHV_F32 || dtype == NHV_BF16), "dequantize_rows: bad arguments");
+  const BackArgs p = {(const int8_t*)q, scales, out, q_stride, out_stride, n_rows, width};
+  return dtype == NHV_F32 ? launch_back<float>(p, stream) : launch_back<bf16>(p, stream);
 }

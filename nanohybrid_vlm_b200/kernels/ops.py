@@ -1959,14 +1959,37 @@ def silu_mul_int8(q, scales, gate_up) -> None:
     _rows_int8(2, q, scales, gate_up, rows, inter, 2 * inter)
 
 
-_PRODUCT_CALL = struct.Struct("=8q5i")
+def dequantize_rows(out, q, scales) -> None:
+    """out[n, width] = q * scales[:, None]: the values that rows of 8-bit integers stand for, rounded once to out's type (bfloat16 or float32).
+    Rows of out and q may lie further apart."""
+    if out.dim() != 2 or (out.stride(1) != 1 and out.shape[1] > 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
+        raise KernelError(f"out is a matrix with neighbouring columns and rows that do not overlap, not {tuple(out.shape)} with strides {out.stride()}")
+    rows, width = out.shape
+    _check_int8_rows("the rows to read", q, rows, width)
+    _check_scales("scales", scales, rows)
+    dtype = dtype_code(out)
+    _same_device(out, q, scales)
+    call("nhv_rows_from_int8", out.data_ptr(), dtype, out.stride(0) if rows > 1 else width, q.data_ptr(), q.stride(0) if rows > 1 else width,
+         scales.data_ptr(), rows, width, stream_ptr())
+
+
+_PRODUCT_CALL = struct.Struct("=10q5i")
+
+
+def _int8_copy(t, pitch: int):
+    """Room for a copy of rows that do not start at multiples of 16 bytes, or None."""
+    rows = t.shape[0]
+    if not (t.data_ptr() | t.stride(0) if rows > 1 else t.data_ptr()) % INT8_ROW_BYTES:
+        return None
+    return torch.empty(rows * pitch, dtype=torch.int8, device=t.device)
+
 
 
 def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
     """out[T, N] = (x[T, K] @ weight[N, K]^T) * x_scales[:, None] * weight_scales[None] for int8 x and weight, float32 scales and out in
     bfloat16 or float32.  The sums are exact (K up to 131,071), so an output does not depend on how the work is cut or batched.
-    Rows of all three matrices may lie further apart; x and weight are read fastest where their rows start at multiples of 16
-    bytes (``new_int8``)."""
+    Rows of all three matrices may lie further apart.  Rows of x and weight that do not start at multiples of 16 bytes (those of
+    ``new_int8`` do) are copied first, each call."""
     if x.dim() != 2 or weight.dim() != 2 or out.dim() != 2:
         raise KernelError("linear_int8 takes matrices: x [T, K], weight [N, K], out [T, N]")
     (T, K), N = x.shape, weight.shape[0]
@@ -1981,10 +2004,14 @@ def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
         raise KernelError(f"a sum over 1 to {INT8_LONGEST_SUM} products of 8-bit integers is exact in 32 bits, not over {K}")
     dtype = dtype_code(out)
     _same_device(out, x, x_scales, weight, weight_scales)
-    pitch = -(-K // INT8_ROW_BYTES) * INT8_ROW_BYTES                 # of a single row, whose stride may be anything
+    if T == 0 or N == 0:
+        return
+    pitch = -(-K // INT8_ROW_BYTES) * INT8_ROW_BYTES
+    x_copy, w_copy = _int8_copy(x, pitch), _int8_copy(weight, pitch)
     call("nhv_gemm_int8", _PRODUCT_CALL.pack(
-        out.data_ptr(), x.data_ptr(), x_scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), stride if T > 1 else N, x.stride(0) if T > 1 else pitch,
-        weight.stride(0) if N > 1 else pitch, dtype, T, N, K, _sm_count(x.device)), stream_ptr())
+        out.data_ptr(), x.data_ptr(), x_scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), x_copy.data_ptr() if x_copy is not None else 0,
+        w_copy.data_ptr() if w_copy is not None else 0, stride if T > 1 else N, x.stride(0) if T > 1 else pitch, weight.stride(0) if N > 1 else pitch,
+        dtype, T, N, K, _sm_count(x.device)), stream_ptr())
 
 
 # ---------------------------------------------------------------- bounded waits that ran out

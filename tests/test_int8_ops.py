@@ -84,6 +84,15 @@ def test_rows_of_other_inputs_refused():
         ops.silu_mul_int8(gate_up=torch.zeros(20, 4).t(), **rows())
 
 
+def test_values_refused():
+    q, s = torch.zeros(4, 10, dtype=I8), torch.zeros(4)
+    for out, q_, s_, text in ((torch.empty(4, 11), q, s, "rows to read"), (torch.empty(4, 10).t(), q, s, "neighbouring"),
+                              (torch.empty(10).expand(4, 10), q, s, "do not overlap"), (torch.empty(4, 10), q, torch.zeros(3), "scales"),
+                              (torch.empty(4, 10, dtype=torch.float16), q, s, "float32 or bfloat16"), (torch.empty(4, 10), q, s, "GPU only")):
+        with pytest.raises(KernelError, match=text):
+            ops.dequantize_rows(out, q_, s_)
+
+
 @pytest.mark.parametrize("width, pitch", [(1, 16), (16, 16), (17, 32), (4096, 4096)])
 def test_room_for_rows(width, pitch):
     t = ops.new_int8(3, width, "cpu")

@@ -296,12 +296,26 @@ def test_rows_of_strided_inputs(ops):
         check_rows(q, s, x.double(), 0.0, exact=dtype == BF)
 
 
+@pytest.mark.parametrize("n,width,pitch,pad", [(1, 1, 16, 0), (3, 16, 16, 0), (5, 33, 16, 3), (300, 4096, 16, 0), (7, 48, 1, 1), (2, 100000, 16, 0)])
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_values(ops, n, width, pitch, pad, dtype):
+    """Integer times scale, rounded once: to 32 bits and, for bfloat16, from there once more (the product's 8 and 24 bits do not fit 32)."""
+    g = gen(width)
+    q, s = ints(g, n, width, pitch), torch.randn(n, generator=g, device="cuda")
+    s[n // 2] = math.nan if n > 2 else 0.0
+    whole = torch.full((n, width + pad), 3.0, dtype=dtype, device="cuda")
+    ops.dequantize_rows(whole[:, :width], q, s)
+    assert torch.equal(whole[:, :width].nan_to_num(nan=77), (q.float() * s[:, None]).to(dtype).nan_to_num(nan=77)) and (whole[:, width:] == 3).all()
+
+
 def test_no_rows(ops):
     e = lambda *shape: torch.empty(*shape, dtype=BF, device="cuda")      # noqa: E731
     q, s = ops.new_int8(0, 64, "cuda"), torch.empty(0, device="cuda")
     ops.quantize_rows(q, s, e(0, 64))
     ops.silu_mul_int8(q, s, e(0, 128))
     ops.rmsnorm_int8(q, s, e(0, 64), e(64), 1e-6, residual=e(0, 64))
+    ops.dequantize_rows(e(0, 64), q, s)
+    ops.dequantize_rows(e(3, 0), ops.new_int8(3, 0, "cuda"), torch.empty(3, device="cuda"))
 
 
 # ------------------------------------------------------------------------------------------------ together
