@@ -185,7 +185,8 @@ def _own(state):
     else:
         ops.quantize_rows(q, scales, state["x"])
     values = torch.empty((case["rows"], case["width"]), dtype=torch.bfloat16, device="cuda")
-    out = {"values": torch.mul(q, scales[:, None], out=values), "scales": scales}
+    ops.dequantize_rows(values, q, scales)
+    out = {"values": values, "scales": scales}
     if case["residual"]:
         out["residual"] = state["residual"]
     return out
