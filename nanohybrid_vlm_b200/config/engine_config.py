@@ -5,7 +5,7 @@ point fills from keyword arguments (nanovllm/engine/llm_engine.py:179-181).  The
 options that belong to its hybrid (GDN, vision, joint prefix cache) path are absent.
 Options that the reference does not have: ``dtype`` (run the checkpoint in another
 precision; ``"float32"`` is the true 32-bit path), ``seed``, ``decode_weight_copy``,
-``async_decode``, ``profile_ranges``, ``poison_cache`` and the three of a bounded cache.
+``async_decode``, ``profile_ranges``, ``quantization``, ``poison_cache`` and the three of a bounded cache.
 """
 from __future__ import annotations
 
@@ -45,6 +45,8 @@ class Config:
                                              # that have gathered the least attention weight are dropped; decode steps run without graphs
     cache_first: int = 4                     # with cache_budget: the keys of the first positions stay whatever they gathered
     cache_recent: int = -1                   # with cache_budget: and those of the last positions (-1: a quarter of the budget)
+    quantization: str | None = None          # "int8": the layers' matrices as 8-bit integers with a scale per output channel, what they
+                                             # multiply rounded to 8 bits with a scale per token (half the weights' bytes)
     poison_cache: bool = False               # fill the cache pools with NaN at start: a read of a slot that no step
                                              # wrote shows in the logits (tests, replay)
     dtype: str | torch.dtype | None = None   # None: the checkpoint's own
@@ -66,6 +68,8 @@ class Config:
             raise ConfigError("max_num_batched_tokens, max_num_seqs and max_model_len must be positive")
         if not 0.0 < self.gpu_memory_utilization <= 1.0:
             raise ConfigError("gpu_memory_utilization must be in (0, 1]")
+        if self.quantization not in (None, "int8"):
+            raise ConfigError(f"quantization must be None or 'int8', got {self.quantization!r}")
         if self.cache_budget:
             if self.cache_recent < 0:
                 self.cache_recent = self.cache_budget // 4

@@ -12,7 +12,7 @@ from dataclasses import dataclass, replace
 import torch
 
 from .. import parts as _registered_parts  # noqa: F401  (importing the package registers the built-in parts)
-from ..parts.base import (BLOCKS, EMBEDDINGS, HEADS, NORMS, BuildEnv, FixedStateNeed, PagedKVNeed, Part, need_leaves,
+from ..parts.base import (BLOCKS, EMBEDDINGS, HEADS, NORMS, BuildEnv, FixedStateNeed, Int8Rows, PagedKVNeed, Part, need_leaves,
                           with_shared_pages)
 from ..parts.spec import ModelSpec, ParamDecl, PartUse
 
@@ -87,8 +87,16 @@ class CausalLM:
             self.head.tie(self.embedding)
         self.tensors = tensors
 
+    def to_int8(self) -> None:
+        """Hold the matrices of all layers as 8-bit integers with a scale per output channel, and multiply by them so; embedding, head and
+        norms stay as they are.  Raises ``ValueError`` where a layer has no such form."""
+        names = {(id(bp.owner), bp.local): bp.name for bp in self.param_table()}
+        for part in {id(p): p for block in self.blocks for p in block.int8_parts()}.values():
+            for local, rows in part.to_int8().items():
+                self.tensors[names[id(part), local]] = rows
+
     def weight_bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in self.tensors.values())
+        return sum(t.bytes() if isinstance(t, Int8Rows) else t.numel() * t.element_size() for t in self.tensors.values())
 
     def streamed_weights(self) -> list[tuple[torch.Tensor, int]]:
         """Every matrix that a decode step streams once (each once, though several parts may share it)."""

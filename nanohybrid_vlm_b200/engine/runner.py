@@ -56,6 +56,9 @@ class ModelRunner:
         else:
             materialize_random(self.model, random_weights_seed)
         self.vocab_size = spec.vocab_size
+        if config.quantization is not None:
+            self.model.to_int8()
+            torch.cuda.empty_cache()     # the rounded matrices' memory: the cache is sized by what the device has free
         self.decode_copy_bytes = self._prepare_decode_weights()
 
         self.layout = CacheLayout.from_needs(self.model.cache_needs())

@@ -12,7 +12,7 @@ checkpoint's q_proj / k_proj / v_proj (nanovllm/layers/linear.py:153-167);
 from __future__ import annotations
 
 from ..kernels import ops
-from .base import MIXERS, Mixer, PagedKVNeed
+from .base import MIXERS, Int8Rows, Mixer, PagedKVNeed, project
 from .spec import ParamDecl, Source
 
 
@@ -51,13 +51,18 @@ class GQAttention(Mixer):
     def cache_need(self):
         return PagedKVNeed(self.nkv, self.d, self.window)
 
+    def int8_weights(self):
+        return ("qkv_proj.weight", "o_proj.weight")
+
     def streamed_weights(self):
+        if isinstance(self.w_o_proj_weight, Int8Rows):
+            return []
         return [(self.w_qkv_proj_weight, 0), (self.w_o_proj_weight, 0)]
 
     def forward(self, x, batch, cache):
         T = x.shape[0]
         qkv = self.new(T, self.q_size + 2 * self.kv_size)
-        ops.linear(qkv, x, self.w_qkv_proj_weight)
+        project(qkv, x, self.w_qkv_proj_weight)
         rot = self.position.rotary() if self.position is not None else None
         table, rotary_dim = rot if rot is not None else (None, 0)
         q_w = self.w_q_norm_weight if self.qk_norm else None
@@ -66,7 +71,7 @@ class GQAttention(Mixer):
         if cache.scores is not None:
             self.attend_scored(o, qkv, q_w, k_w, table, rotary_dim, batch, cache)
             y = self.new(T, self.env.hidden_size)
-            ops.linear(y, o, self.w_o_proj_weight)
+            project(y, o, self.w_o_proj_weight)
             return y
         # a step of single tokens: the decode kernel takes qkv as it is (norm, rotation and store inside it)
         if not ops.attention_decode_fused(o, qkv, cache.pages, cache.tables, batch, self.nq, self.nkv, self.d,
@@ -78,7 +83,7 @@ class GQAttention(Mixer):
                 q_w, k_w, table, rotary_dim, self.nq, self.nkv, self.d, self.eps, self.norm_offset)
             self.attend(o, q, batch, cache)
         y = self.new(T, self.env.hidden_size)
-        ops.linear(y, o, self.w_o_proj_weight)
+        project(y, o, self.w_o_proj_weight)
         return y
 
     scores_keys = True

@@ -16,6 +16,7 @@ from typing import Any
 
 import torch
 
+from ..kernels import ops
 from .spec import ParamDecl, PartSpec
 
 
@@ -110,6 +111,41 @@ def with_shared_pages(need):
     return need
 
 
+class Int8Rows:
+    """A matrix whose rows are 8-bit integers with a float32 scale each: a weight (a scale per output channel), or what a norm hands to
+    the projections that read it (a scale per token)."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        self.values, self.scales = values, scales
+
+    @classmethod
+    def room(cls, rows: int, width: int, device) -> "Int8Rows":
+        return cls(ops.new_int8(rows, width, device), torch.empty(rows, dtype=torch.float32, device=device))
+
+    @classmethod
+    def of(cls, x: torch.Tensor) -> "Int8Rows":
+        rows = cls.room(*x.shape, x.device)
+        ops.quantize_rows(rows.values, rows.scales, x)
+        return rows
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    def bytes(self) -> int:
+        return self.values.shape[0] * (self.values.stride(0) + 4)
+
+
+def project(out: torch.Tensor, x, weight) -> None:
+    """out = x weight^T, by 8-bit integers where the weight is held in them (x is then rounded to them here, unless its norm did that)."""
+    if isinstance(weight, Int8Rows):
+        if not isinstance(x, Int8Rows):
+            x = Int8Rows.of(x)
+        ops.linear_int8(out, x.values, x.scales, weight.values, weight.scales)
+    else:
+        ops.linear(out, x, weight)
+
+
 class BuildEnv:
     """What a part may know about its surroundings."""
 
@@ -147,6 +183,19 @@ class Part:
         ``kernels.ops`` streams them (0: plain product, 1: fp32 logits, 2: [gate; up] rows with SiLU).  The
         engine may keep a second copy of each, laid out for the weight-streaming kernel.  Default: none."""
         return []
+
+    def int8_weights(self) -> tuple[str, ...]:
+        """The local names of the matrices that the part can multiply by as 8-bit integers (``to_int8``).  Default: none."""
+        return ()
+
+    def to_int8(self) -> dict[str, Int8Rows]:
+        """Round those matrices to 8-bit integers with a scale per output channel, in their places; the part lets go of the originals."""
+        made = {}
+        for name in self.int8_weights():
+            at = "w_" + name.replace(".", "_")
+            made[name] = Int8Rows.of(getattr(self, at))
+            setattr(self, at, made[name])
+        return made
 
     def scratch_bytes(self, tokens: int, requests: int) -> int:
         """What a step of up to so many tokens and requests takes on the device beside the tensors that are as wide as one
@@ -323,6 +372,11 @@ class Block:
         self.parts = dict(parts)
         for name, obj in parts.items():
             setattr(self, name, obj)
+
+    def int8_parts(self) -> tuple[Part, ...]:
+        """For an engine that multiplies in 8-bit integers: the parts whose matrices are rounded to them, after the block has told its
+        norms to round what those parts read.  Default: the block cannot."""
+        raise ValueError(f"block {self.spec.kind!r} has no form in 8-bit integers")
 
     @property
     def cache_owner(self) -> Mixer | None:

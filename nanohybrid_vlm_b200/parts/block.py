@@ -15,6 +15,16 @@ from .spec import ParamDecl, Source
 
 
 class PreNormResidualBlock(Block):
+    def int8_parts(self):
+        for name in ("mixer", "ffn"):
+            if not self.parts[name].int8_weights():
+                raise ValueError(f"{self.parts[name].spec.kind!r} has no form in 8-bit integers")
+        for name in ("mixer_norm", "ffn_norm"):
+            if not hasattr(self.parts[name], "give_int8"):
+                raise ValueError(f"norm {self.parts[name].spec.kind!r} gives no 8-bit integers")
+            self.parts[name].give_int8()
+        return self.parts["mixer"], self.parts["ffn"]
+
     def forward(self, hidden, residual, batch, cache):
         if residual is None:
             residual = hidden

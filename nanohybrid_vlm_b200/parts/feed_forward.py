@@ -7,7 +7,7 @@ then up, packed from gate_proj / up_proj (nanovllm/layers/linear.py:102-108);
 from __future__ import annotations
 
 from ..kernels import ops
-from .base import FEED_FORWARDS, FeedForward
+from .base import FEED_FORWARDS, FeedForward, Int8Rows, project
 from .spec import ParamDecl, Source
 
 
@@ -25,9 +25,26 @@ class SwiGLU(FeedForward):
         ]
 
     def streamed_weights(self):
+        if isinstance(self.w_down_proj_weight, Int8Rows):
+            return []
         return [(self.w_gate_up_proj_weight, 2), (self.w_down_proj_weight, 0)]
 
+    def int8_weights(self):
+        return ("gate_up_proj.weight", "down_proj.weight")
+
+    def forward_int8(self, x):
+        T = x.shape[0]
+        gate_up = self.new(T, 2 * self.inter)
+        project(gate_up, x, self.w_gate_up_proj_weight)
+        act = Int8Rows.room(T, self.inter, self.env.device)
+        ops.silu_mul_int8(act.values, act.scales, gate_up)
+        y = self.new(T, self.env.hidden_size)
+        project(y, act, self.w_down_proj_weight)
+        return y
+
     def forward(self, x, batch):
+        if isinstance(self.w_down_proj_weight, Int8Rows):
+            return self.forward_int8(x)
         T = x.shape[0]
         act = self.new(T, self.inter)
         if not ops.swiglu_first_half(act, x, self.w_gate_up_proj_weight):

@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from ..kernels import ops
-from .base import NORMS, Norm, Pending
+from .base import NORMS, Int8Rows, Norm, Pending
 from .spec import ParamDecl, Source
 
 
@@ -85,8 +85,22 @@ class RMSNorm(Norm):
         new = streams if streams.shape[1] == S else self.new(streams.shape[0], S, self.width, dtype=torch.float32)
         return self._streams(x, streams, S, connection.read, new, None), new
 
+    def give_int8(self) -> None:
+        """From here on ``forward`` and ``forward_add`` over tensors return :class:`Int8Rows`."""
+        self._plain_only()
+        self.int8 = True
+
+    int8 = False
+
+    def _to_int8(self, x, residual=None):
+        out = Int8Rows.room(x.shape[0], self.width, x.device)
+        ops.rmsnorm_int8(out.values, out.scales, x, self.w_weight, self.eps, residual=residual, weight_offset=self.weight_offset)
+        return out
+
     def forward(self, x):
         self._plain_only()
+        if self.int8:
+            return self._to_int8(x)
         out = self.new(*x.shape)
         ops.rmsnorm(out, x, self.w_weight, self.eps, weight_offset=self.weight_offset)
         return out
@@ -123,6 +137,8 @@ class RMSNorm(Norm):
                                groups=self.groups)
             return out
         self._plain_only()
+        if self.int8:
+            return self._to_int8(x, residual)
         out = self.new(*x.shape)
         ops.rmsnorm(out, x, self.w_weight, self.eps, residual=residual, weight_offset=self.weight_offset)
         return out

@@ -97,3 +97,11 @@ def test_values_refused():
 def test_room_for_rows(width, pitch):
     t = ops.new_int8(3, width, "cpu")
     assert t.shape == (3, width) and t.dtype == I8 and t.stride() == (pitch, 1)
+
+
+def test_engine_option(model_dirs):
+    from nanohybrid_vlm_b200.config import Config
+    from nanohybrid_vlm_b200.config.model_config import ConfigError
+    assert Config(model_dirs["A"], quantization="int8").quantization == "int8" and Config(model_dirs["A"]).quantization is None
+    with pytest.raises(ConfigError, match="int8"):
+        Config(model_dirs["A"], quantization="int4")
