@@ -159,7 +159,7 @@ def bench_ours(args) -> dict:
         llm = LLM(d, random_weights_seed=SEED, kvcache_block_size=PAGE, num_kvcache_blocks=pages,
                   max_model_len=CONTEXT, max_num_seqs=max_b, max_num_batched_tokens=8192, seed=SEED,
                   enforce_eager=args.eager, async_decode=not args.sync,
-                  decode_weight_copy=False if args.no_weight_copy else None)
+                  decode_weight_copy=False if args.no_weight_copy else None, quantization=args.quantization)
     runner = llm.model_runner
     params = SamplingParams(temperature=0.0, max_tokens=CONTEXT - PROMPT_LEN, ignore_eos=True)
 
@@ -1023,6 +1023,8 @@ def main() -> int:
     ap.add_argument("--sync", action="store_true", help="read every decode step's tokens before the next is launched (async_decode off)")
     ap.add_argument("--no-weight-copy", action="store_true",
                     help="decode from the row-major matrices (no per-SM copies of the weights: half the weight memory)")
+    ap.add_argument("--quantization", default=None, choices=["int8"],
+                    help="the layers' matrices in 8-bit integers (with --only decode or --only prefill: the benchmark's line is for bfloat16)")
     ap.add_argument("--requests", type=int, default=0, help="fewer requests than the workload names (trying it out)")
     ap.add_argument("--breakdown", action="store_true",
                     help="time by kind of kernel in an eager run with --layers layers (default 2); prints one JSON line")
@@ -1034,6 +1036,8 @@ def main() -> int:
     if args.gpus != 1:
         print(f"bench.py measures a single-GPU engine: --gpus {args.gpus} is not supported (N=1 only)")
         return 2
+    if args.quantization and (args.only == "all" or args.workload != "8b" or args.designs or args.breakdown or args.impl == "reference"):
+        ap.error("--quantization goes with --only decode or --only prefill of the 8b workload")
     if args.warmup < 3:
         args.warmup = 3
     if args.designs:

@@ -185,126 +185,6 @@ struct alignas(64) Mapped {
   int share, parts_bytes;                     // tokens that a block of a cluster finishes, and room for all parts of theirs
 };
 
-// ---- up to eight tokens: the weight streams through registers into mma.sync, 16 rows beside the tokens
-constexpr int STREAM_WARPS = 16, STREAM_CHUNKS = 4, STREAM_DEPTH = 2;
-constexpr int STREAM_LD = 12;          // of a row's sums: eight tokens, and four so that the lanes' banks differ
-
-__device__ __forceinline__ void mma_sync(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
-               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint4 load_once(const int8_t* at) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at));
-  return v;
-}
-// The first n of a word's four bytes, zeros for the others.
-__device__ __forceinline__ uint32_t kept_bytes(uint32_t v, int n) { return n >= 4 ? v : n <= 0 ? 0u : v & ((1u << (8 * n)) - 1u); }
-
-struct StreamPlan {
-  int along_k, chunks;      // warps that share K, and the 64-byte pieces that each takes at a time
-};
-
-__global__ void __launch_bounds__(STREAM_WARPS * 32, 1) product_stream_kernel(const Product p, const StreamPlan plan) {
-  extern __shared__ int sums[];                                  // [rows][STREAM_LD]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int r0 = (int)((long long)p.N * blockIdx.x / gridDim.x), rows = (int)((long long)p.N * (blockIdx.x + 1) / gridDim.x) - r0;
-  pdl_launch_dependents();
-  const int8_t* w = p.w + (long long)r0 * p.w_stride;
-  if (threadIdx.x == 0) {
-    // asked into L2, which is where all copies meet: nothing that is read here is used
-    const long long bytes = (long long)(rows - 1) * p.w_stride;
-    const uint32_t ask = (uint32_t)(bytes < 65536 ? bytes : 65536);
-    if (rows > 1) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(w), "r"(ask) : "memory");
-  }
-  for (int i = threadIdx.x; i < rows * STREAM_LD; i += STREAM_WARPS * 32) sums[i] = 0;
-  __syncthreads();
-  pdl_wait();
-  const int wk = plan.along_k, step = plan.chunks * 64, kw = warp % wk, nw = warp / wk, wn = STREAM_WARPS / wk;
-  const int f0 = rows * nw / wn, f1 = rows * (nw + 1) / wn;      // this warp's rows, from r0
-  const int mine = (f1 - f0 + 15) / 16, passes = (p.K + wk * step - 1) / (wk * step), items = mine * passes;
-  uint4 b[STREAM_DEPTH][2][STREAM_CHUNKS];
-  int pass = 0, group = 0;                                       // of what is loaded next
-  auto load = [&](uint4 (&v)[2][STREAM_CHUNKS]) {
-    const int k = (pass * wk + kw) * step + q * 16;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = f0 + group * 16 + h * 8 + g;
-      const int8_t* at = w + (long long)r * p.w_stride + k;
-#pragma unroll
-      for (int c = 0; c < STREAM_CHUNKS; ++c)
-        v[h][c] = r < f1 && c < plan.chunks && k + c * 64 < p.K ? load_once(at + c * 64) : make_uint4(0, 0, 0, 0);
-    }
-    if (++group == mine) {
-      group = 0;
-      ++pass;
-    }
-  };
-#pragma unroll
-  for (int d = 0; d < STREAM_DEPTH; ++d)
-    if (d < items) load(b[d]);
-  uint32_t x[STREAM_CHUNKS][4];
-  int at_pass = -1, left = 0, row = 0;
-  for (int i = 0; i < items; i += STREAM_DEPTH) {
-#pragma unroll
-    for (int d = 0; d < STREAM_DEPTH; ++d) {
-      if (i + d >= items) break;
-      if (left == 0) {                                           // the tokens' next pieces
-        left = mine;
-        row = f0;
-        ++at_pass;
-#pragma unroll
-        for (int c = 0; c < STREAM_CHUNKS; ++c) {
-          const int k = (at_pass * wk + kw) * step + c * 64 + q * 16;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (g < p.T && c < plan.chunks && k < p.K) {
-            v = *reinterpret_cast<const uint4*>(p.x + (long long)g * p.x_stride + k);
-            // what lies behind a row is anybody's: zeros in x make it count for nothing, in the weight too
-            if (k + 16 > p.K) v = make_uint4(kept_bytes(v.x, p.K - k), kept_bytes(v.y, p.K - k - 4), kept_bytes(v.z, p.K - k - 8), kept_bytes(v.w, p.K - k - 12));
-          }
-          x[c][0] = v.x; x[c][1] = v.y; x[c][2] = v.z; x[c][3] = v.w;
-        }
-      }
-      // A lane's 16 bytes of a row are its places of two MMAs: which column of K stands where is the same for both operands.
-      int acc[4] = {};
-#pragma unroll
-      for (int c = 0; c < STREAM_CHUNKS; ++c) {
-        const uint4 u = b[d][0][c], v = b[d][1][c];
-        const uint32_t lo[4] = {u.x, v.x, u.y, v.y}, hi[4] = {u.z, v.z, u.w, v.w};
-        mma_sync(acc, lo, x[c][0], x[c][1]);
-        mma_sync(acc, hi, x[c][2], x[c][3]);
-      }
-      if (i + d + STREAM_DEPTH < items) load(b[d]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = row + (e >> 1) * 8 + g, t = 2 * q + (e & 1);
-        if (r < f1 && t < p.T) atomicAdd(&sums[r * STREAM_LD + t], acc[e]);      // integers: the order does not matter
-      }
-      row += 16;
-      --left;
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * p.T; i += STREAM_WARPS * 32) {
-    const int t = i / rows, r = i - t * rows;
-    store_out(p, t, r0 + r, scaled(sums[r * STREAM_LD + t], p.x_scales[t], p.w_scales[r0 + r]));
-  }
-}
-
-int stream_product(const Product& p, int sms, cudaStream_t stream) {
-  constexpr int MOST_ROWS = 4096;                                // of a block: 192 KB of sums
-  const long long blocks = (long long)sms * ((p.N + (long long)sms * MOST_ROWS - 1) / ((long long)sms * MOST_ROWS));
-  const int grid = (int)(blocks < p.N ? blocks : p.N), rows = (p.N + grid - 1) / grid, pieces = (p.K + 63) / 64;
-  StreamPlan plan = {1, 1};
-  while (plan.along_k < STREAM_WARPS && plan.along_k * STREAM_CHUNKS < pieces) plan.along_k *= 2;
-  const int passes = (pieces + plan.along_k * STREAM_CHUNKS - 1) / (plan.along_k * STREAM_CHUNKS);
-  plan.chunks = (pieces + passes * plan.along_k - 1) / (passes * plan.along_k);
-  static std::atomic<uint64_t> allowed{0};
-  NHV_CUDA(nhv_allow_smem((const void*)product_stream_kernel, MOST_ROWS * STREAM_LD * 4, allowed), "linear_int8");
-  NHV_CUDA(nhv_launch(product_stream_kernel, dim3(grid), dim3(STREAM_WARPS * 32), (size_t)rows * STREAM_LD * 4, stream, p, plan), "linear_int8");
-  return 0;
-}
-
 // ---- few tokens: 128 rows of the weight on the MMA's M axis, up to NT tokens on its N axis.
 constexpr int SPLIT_THREADS = 320;     // producer warp, MMA warp, eight epilogue warps
 
@@ -871,9 +751,9 @@ NHV_API int nhv_gemm_int8(const void* given, cudaStream_t stream) {
                      (c.out | c.out_stride * (c.out_dtype == NHV_F32 ? 4 : 2)) % 16 == 0};
   if (int e = align_rows(&p.x, &p.x_stride, (void*)c.x_copy, T, K, stream)) return e;
   if (int e = align_rows(&p.w, &p.w_stride, (void*)c.w_copy, N, K, stream)) return e;
-  // us: 8 tokens, 4,096 x 4,096 / 6,144 x 4,096 / 4,096 x 12,288 through registers 5.0 / 6.3 / 10.6, on tcgen05 5.8 / 7.5 / 11.0; 16 tokens 6.2 / - / 13.6 and 5.8 /
-  // 7.5 / 11.3.  128 tokens, 4,096 x 4,096 / 24,576 x 4,096 / 4,096 x 12,288: whole tiles of the weight 9.4 / 22.1 / 14.9, pairs 9.3 / 26.2 / 18.6.
-  if (T <= 8) return stream_product(p, sms, stream);
+  // us, 128 tokens, 4,096 x 4,096 / 24,576 x 4,096 / 4,096 x 12,288: whole tiles of the weight 9.4 / 22.1 / 14.9, pairs 9.3 / 26.2 / 18.6; 256 tokens 12.7 / 33 / 19.5 and 9.3 /
+  // 26.2 / 18.6.  Up to 8 tokens the weight through registers into mma.sync was tried: alone 5.0 / 18.5 / 10.6 against 6.0 / 18.3 / 11.0, but in a decode step,
+  // behind other kernels, 7.2 / 31.5 / 18.3 against 5.1 / 17.8 / 8.5 (its blocks fill an SM, so that none starts under the kernel before)
   Mapped m;
   m.p = p;
   if (T <= 128) return split_product(m, split_plan(p, sms), stream);
