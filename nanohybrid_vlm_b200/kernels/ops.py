@@ -1910,15 +1910,20 @@ _ROWS_CALL = struct.Struct("=7q5i2f")
 
 def _rows_int8(kind: int, q, scales, x, rows: int, width: int, x_stride: int, residual=None, weight=None, eps: float = 0.0, offset: float = 0.0,
                write_residual: bool = False) -> None:
-    _check_int8_rows("the rows to write", q, rows, width)
-    _check_scales("scales", scales, rows)
-    if width < 1:
-        raise KernelError("rows of no elements have no scale")
-    dtype = dtype_code(x)
-    _same_device(q, scales, x, residual, weight)
+    dtype, device, step = x.dtype, _current_device() if x.is_cuda else -1, q.stride()
+    if not (width > 0 and q.dtype is torch.int8 and q.shape == (rows, width) and step[1] == 1 and step[0] >= width and scales.shape == (rows,)
+            and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32)
+            and x.get_device() == q.get_device() == scales.get_device() == device >= 0 and (weight is None or weight.get_device() == device)
+            and (residual is None or residual.get_device() == device)):
+        _check_int8_rows("the rows to write", q, rows, width)
+        _check_scales("scales", scales, rows)
+        if width < 1:
+            raise KernelError("rows of no elements have no scale")
+        dtype_code(x)
+        _same_device(q, scales, x, residual, weight)
     call("nhv_rows_int8", _ROWS_CALL.pack(
         q.data_ptr(), scales.data_ptr(), x.data_ptr(), residual.data_ptr() if residual is not None else 0, weight.data_ptr() if weight is not None else 0,
-        q.stride(0) if rows > 1 else width, x_stride, kind, dtype, rows, width, write_residual, eps, offset), stream_ptr())
+        step[0] if rows > 1 else width, x_stride, kind, BF16 if dtype is torch.bfloat16 else F32, rows, width, write_residual, eps, offset), stream_ptr())
 
 
 def quantize_rows(q, scales, x) -> None:
@@ -1976,20 +1981,8 @@ def dequantize_rows(out, q, scales) -> None:
 _PRODUCT_CALL = struct.Struct("=10q5i")
 
 
-def _int8_copy(t, pitch: int):
-    """Room for a copy of rows that do not start at multiples of 16 bytes, or None."""
-    rows = t.shape[0]
-    if not (t.data_ptr() | t.stride(0) if rows > 1 else t.data_ptr()) % INT8_ROW_BYTES:
-        return None
-    return torch.empty(rows * pitch, dtype=torch.int8, device=t.device)
-
-
-
-def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
-    """out[T, N] = (x[T, K] @ weight[N, K]^T) * x_scales[:, None] * weight_scales[None] for int8 x and weight, float32 scales and out in
-    bfloat16 or float32.  The sums are exact (K up to 131,071), so an output does not depend on how the work is cut or batched.
-    Rows of all three matrices may lie further apart.  Rows of x and weight that do not start at multiples of 16 bytes (those of
-    ``new_int8`` do) are copied first, each call."""
+def _check_linear_int8(out, x, x_scales, weight, weight_scales) -> None:
+    """What ``linear_int8`` assumes, one ``KernelError`` each; called when its quick look finds something amiss."""
     if x.dim() != 2 or weight.dim() != 2 or out.dim() != 2:
         raise KernelError("linear_int8 takes matrices: x [T, K], weight [N, K], out [T, N]")
     (T, K), N = x.shape, weight.shape[0]
@@ -2002,16 +1995,37 @@ def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
         raise KernelError(f"out is [{T}, {N}] with neighbouring columns and rows that do not overlap, not {tuple(out.shape)} with strides {out.stride()}")
     if not 0 < K <= INT8_LONGEST_SUM:
         raise KernelError(f"a sum over 1 to {INT8_LONGEST_SUM} products of 8-bit integers is exact in 32 bits, not over {K}")
-    dtype = dtype_code(out)
+    dtype_code(out)
     _same_device(out, x, x_scales, weight, weight_scales)
-    if T == 0 or N == 0:
-        return
+
+
+def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
+    """out[T, N] = (x[T, K] @ weight[N, K]^T) * x_scales[:, None] * weight_scales[None] for int8 x and weight, float32 scales and out in
+    bfloat16 or float32.  The sums are exact (K up to 131,071), so an output does not depend on how the work is cut or batched.
+    Rows of all three matrices may lie further apart.  Rows of x and weight that do not start at multiples of 16 bytes (those of
+    ``new_int8`` do) are copied first, each call."""
+    shape, rows, dtype, device = x.shape, weight.shape, out.dtype, _current_device() if x.is_cuda else -1
+    T, K, N = (*shape, rows[0]) if len(shape) == len(rows) == 2 else (0, 0, 0)
+    x_step, w_step, out_step = x.stride(), weight.stride(), out.stride()
+    if not (T > 0 and N > 0 and 0 < K <= INT8_LONGEST_SUM and rows[1] == K and out.shape == (T, N) and x.dtype is torch.int8
+            and weight.dtype is torch.int8 and (dtype is torch.bfloat16 or dtype is torch.float32) and x_step[1] == w_step[1] == out_step[1] == 1
+            and x_step[0] >= K and w_step[0] >= K and out_step[0] >= N and x_scales.shape == (T,) and weight_scales.shape == (N,)
+            and x_scales.dtype is torch.float32 and weight_scales.dtype is torch.float32 and x_scales.is_contiguous() and weight_scales.is_contiguous()
+            and x.get_device() == weight.get_device() == out.get_device() == x_scales.get_device() == weight_scales.get_device() == device >= 0):
+        _check_linear_int8(out, x, x_scales, weight, weight_scales)
+        if T == 0 or N == 0:
+            return
     pitch = -(-K // INT8_ROW_BYTES) * INT8_ROW_BYTES
-    x_copy, w_copy = _int8_copy(x, pitch), _int8_copy(weight, pitch)
+    x_at, w_at = x.data_ptr(), weight.data_ptr()
+    x_pitch, w_pitch = x_step[0] if T > 1 else pitch, w_step[0] if N > 1 else pitch      # a single row's stride may be anything
+    x_copy = w_copy = None
+    if (x_at | w_at | x_pitch | w_pitch) % INT8_ROW_BYTES:
+        x_copy = torch.empty(T * pitch, dtype=torch.int8, device=x.device) if (x_at | x_pitch) % INT8_ROW_BYTES else None
+        w_copy = torch.empty(N * pitch, dtype=torch.int8, device=x.device) if (w_at | w_pitch) % INT8_ROW_BYTES else None
     call("nhv_gemm_int8", _PRODUCT_CALL.pack(
-        out.data_ptr(), x.data_ptr(), x_scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), x_copy.data_ptr() if x_copy is not None else 0,
-        w_copy.data_ptr() if w_copy is not None else 0, stride if T > 1 else N, x.stride(0) if T > 1 else pitch, weight.stride(0) if N > 1 else pitch,
-        dtype, T, N, K, _sm_count(x.device)), stream_ptr())
+        out.data_ptr(), x_at, x_scales.data_ptr(), w_at, weight_scales.data_ptr(), x_copy.data_ptr() if x_copy is not None else 0,
+        w_copy.data_ptr() if w_copy is not None else 0, out_step[0] if T > 1 else N, x_pitch, w_pitch, BF16 if dtype is torch.bfloat16 else F32, T, N, K,
+        _sm_count(x.device)), stream_ptr())
 
 
 # ---------------------------------------------------------------- bounded waits that ran out
