@@ -1921,8 +1921,11 @@ def _rows_int8(kind: int, q, scales, x, rows: int, width: int, x_stride: int, re
             raise KernelError("rows of no elements have no scale")
         dtype_code(x)
         _same_device(q, scales, x, residual, weight)
+    q_at, x_at = q.data_ptr(), x.data_ptr()
+    if q_at == x_at and rows:
+        raise KernelError("the 8-bit rows have memory of their own: other rows are still read from what lies there")
     call("nhv_rows_int8", _ROWS_CALL.pack(
-        q.data_ptr(), scales.data_ptr(), x.data_ptr(), residual.data_ptr() if residual is not None else 0, weight.data_ptr() if weight is not None else 0,
+        q_at, scales.data_ptr(), x_at, residual.data_ptr() if residual is not None else 0, weight.data_ptr() if weight is not None else 0,
         step[0] if rows > 1 else width, x_stride, kind, BF16 if dtype is torch.bfloat16 else F32, rows, width, write_residual, eps, offset), stream_ptr())
 
 
@@ -1970,12 +1973,18 @@ def dequantize_rows(out, q, scales) -> None:
     if out.dim() != 2 or (out.stride(1) != 1 and out.shape[1] > 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
         raise KernelError(f"out is a matrix with neighbouring columns and rows that do not overlap, not {tuple(out.shape)} with strides {out.stride()}")
     rows, width = out.shape
-    _check_int8_rows("the rows to read", q, rows, width)
-    _check_scales("scales", scales, rows)
-    dtype = dtype_code(out)
-    _same_device(out, q, scales)
-    call("nhv_rows_from_int8", out.data_ptr(), dtype, out.stride(0) if rows > 1 else width, q.data_ptr(), q.stride(0) if rows > 1 else width,
-         scales.data_ptr(), rows, width, stream_ptr())
+    device, step, dtype = _current_device() if out.is_cuda else -1, q.stride(), out.dtype
+    if not (q.dtype is torch.int8 and q.shape == (rows, width) and step[1] == 1 and step[0] >= width and scales.shape == (rows,)
+            and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32)
+            and out.get_device() == q.get_device() == scales.get_device() == device >= 0):
+        _check_int8_rows("the rows to read", q, rows, width)
+        _check_scales("scales", scales, rows)
+        dtype_code(out)
+        _same_device(out, q, scales)
+    if out.data_ptr() == q.data_ptr() and rows and width:
+        raise KernelError("the values have memory of their own: other rows are still read from what lies there")
+    call("nhv_rows_from_int8", out.data_ptr(), BF16 if dtype is torch.bfloat16 else F32, out.stride(0) if rows > 1 else width, q.data_ptr(),
+         step[0] if rows > 1 else width, scales.data_ptr(), rows, width, stream_ptr())
 
 
 _PRODUCT_CALL = struct.Struct("=10q5i")
@@ -2016,14 +2025,16 @@ def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
         if T == 0 or N == 0:
             return
     pitch = -(-K // INT8_ROW_BYTES) * INT8_ROW_BYTES
-    x_at, w_at = x.data_ptr(), weight.data_ptr()
+    x_at, w_at, out_at = x.data_ptr(), weight.data_ptr(), out.data_ptr()
+    if out_at == x_at or out_at == w_at:
+        raise KernelError("the output has memory of its own: the operands are read again for other outputs")
     x_pitch, w_pitch = x_step[0] if T > 1 else pitch, w_step[0] if N > 1 else pitch      # a single row's stride may be anything
     x_copy = w_copy = None
     if (x_at | w_at | x_pitch | w_pitch) % INT8_ROW_BYTES:
         x_copy = torch.empty(T * pitch, dtype=torch.int8, device=x.device) if (x_at | x_pitch) % INT8_ROW_BYTES else None
         w_copy = torch.empty(N * pitch, dtype=torch.int8, device=x.device) if (w_at | w_pitch) % INT8_ROW_BYTES else None
     call("nhv_gemm_int8", _PRODUCT_CALL.pack(
-        out.data_ptr(), x_at, x_scales.data_ptr(), w_at, weight_scales.data_ptr(), x_copy.data_ptr() if x_copy is not None else 0,
+        out_at, x_at, x_scales.data_ptr(), w_at, weight_scales.data_ptr(), x_copy.data_ptr() if x_copy is not None else 0,
         w_copy.data_ptr() if w_copy is not None else 0, out_step[0] if T > 1 else N, x_pitch, w_pitch, BF16 if dtype is torch.bfloat16 else F32, T, N, K,
         _sm_count(x.device)), stream_ptr())
 

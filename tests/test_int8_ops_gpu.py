@@ -308,6 +308,19 @@ def test_values(ops, n, width, pitch, pad, dtype):
     assert torch.equal(whole[:, :width].nan_to_num(nan=77), (q.float() * s[:, None]).to(dtype).nan_to_num(nan=77)) and (whole[:, width:] == 3).all()
 
 
+def test_outputs_over_inputs_are_refused(ops):
+    from nanohybrid_vlm_b200.kernels.library import KernelError
+    x, s = torch.randn(4, 64, device="cuda"), torch.empty(4, device="cuda")
+    over = x.view(torch.int8)[:, :64]
+    for call in (lambda: ops.quantize_rows(over, s, x), lambda: ops.rmsnorm_int8(over, s, x, x[0].clone(), 1e-6),
+                 lambda: ops.silu_mul_int8(over[:, :32], s, x), lambda: ops.dequantize_rows(x, over, s)):
+        with pytest.raises(KernelError, match="memory of"):
+            call()
+    x = ops.new_int8(4, 64, "cuda").fill_(1)
+    with pytest.raises(KernelError, match="memory of"):
+        ops.linear_int8(x.view(torch.float32)[:, :4], x, s, x[:4].clone(), s)
+
+
 def test_no_rows(ops):
     e = lambda *shape: torch.empty(*shape, dtype=BF, device="cuda")      # noqa: E731
     q, s = ops.new_int8(0, 64, "cuda"), torch.empty(0, device="cuda")
