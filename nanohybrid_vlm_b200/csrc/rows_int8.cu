@@ -6,9 +6,13 @@
 // rounded once, to q.  A row of zeros has the scale 0; a row with an infinity or a NaN has the scale NaN and zeros, so that every
 // product with it is NaN.
 //
-// The quotient is rounded correctly before it is rounded to an integer (Markstein's correction of a product with the
+// Plain rows: the quotient is rounded correctly before it is rounded to an integer (Markstein's correction of a product with the
 // reciprocal, 1990: r = t - q a exactly by one fused multiply-add, q + r / a), so rows in bfloat16 give the integers of the
-// definition, ties included.  |q| is at most 127.
+// definition, ties included.  The others' y is rounded anyway: one fused multiply-add of y and 127 / a onto a number whose last bit is a
+// one gives the integer.  |q| is at most 127.
+//
+// The large kernels are bounded by memory with the issue slots not far behind (two thirds and three quarters of them used before the
+// arithmetic went by pairs), hence pairs of floats, maxima of three and integers in the low bits of floats.
 #include <string.h>
 
 #include "nhv_vec8.cuh"
@@ -30,25 +34,35 @@ struct Args {
   int write_residual;
 };
 
+__device__ __forceinline__ f32x2 both(float v) { return f2_pack(v, v); }
+__device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // What a row's elements are divided by.  A factor (a power of two) keeps every intermediate of rows of very small and very
 // large values in range.
 struct Divisor {
-  float m, a, inv;       // m: 127 times the factor
+  float m, a, inv;       // the factor; the row's largest and its reciprocal, with the factor
 };
 __device__ __forceinline__ Divisor divisor_of(float a) {
   Divisor d;
-  const float m = a < 0x1p-60f ? 0x1p100f : (a > 0x1p100f ? 0x1p-100f : 1.0f);
-  d.m = 127.0f * m;
-  d.a = a * m;
+  d.m = a < 0x1p-60f ? 0x1p100f : (a > 0x1p100f ? 0x1p-100f : 1.0f);
+  d.a = a * d.m;
   d.inv = 1.0f / d.a;
   return d;
 }
-// The integer in the low byte: 1.5 * 2^23 + q has q's two's complement there, rounded to nearest, ties to even.
+// 1.5 * 2^23 + q has q's two's complement in its low byte, rounded to nearest, ties to even.
+constexpr float LOW_BITS = 12582912.0f;
+
+template <bool EXACT>
 __device__ __forceinline__ uint32_t rounded_byte(float y, const Divisor& d) {
-  const float t = y * d.m;
+  if (!EXACT) return __float_as_uint(fmaf(y * d.m, 127.0f * d.inv, LOW_BITS));
+  const float t = y * (127.0f * d.m);
   float q = t * d.inv;
   q = fmaf(fmaf(-q, d.a, t), d.inv, q);
-  return __float_as_uint(q + 12582912.0f);
+  return __float_as_uint(q + LOW_BITS);
 }
 __device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
@@ -126,7 +140,7 @@ __global__ void rows_kernel(const Args p) {
   if (threadIdx.x == 0) p.scales[r] = finite ? a / 127.0f : __int_as_float(0x7fc00000);
   const Divisor d = divisor_of(some ? a : 1.0f);
   int8_t* q = p.q + r * p.q_stride;
-  for (int c = threadIdx.x; c < p.width; c += blockDim.x) q[c] = some ? (int8_t)rounded_byte(KEEP ? row[c] : value(c), d) : (int8_t)0;
+  for (int c = threadIdx.x; c < p.width; c += blockDim.x) q[c] = some ? (int8_t)rounded_byte<KIND == ROW_PLAIN>(KEEP ? row[c] : value(c), d) : (int8_t)0;
 }
 
 template <typename T, int KIND>
@@ -145,18 +159,20 @@ int launch_any(const Args& p, int n_rows, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------- widths in eights, rows on 16-byte boundaries
-// A thread keeps CH pieces of eight elements of its row in registers from the one read to the one write.
+// Eight elements as they lie in memory, and as four pairs.
+struct Eight {
+  f32x2 v[4];
+};
 template <typename T> struct Piece;
 template <> struct Piece<bf16> {
   uint4 v;
   __device__ __forceinline__ void load(const void* row, int i) { v = reinterpret_cast<const uint4*>(row)[i]; }
-  __device__ __forceinline__ void get(float (&o)[8]) const {
+  __device__ __forceinline__ Eight get() const {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    Eight o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[2 * i] = __uint_as_float(w[i] << 16);
-      o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; ++i) o.v[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    return o;
   }
 };
 template <> struct Piece<float> {
@@ -165,11 +181,80 @@ template <> struct Piece<float> {
     a = reinterpret_cast<const float4*>(row)[2 * i];
     b = reinterpret_cast<const float4*>(row)[2 * i + 1];
   }
-  __device__ __forceinline__ void get(float (&o)[8]) const {
-    o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
+  __device__ __forceinline__ Eight get() const {
+    Eight o = {{f2_pack(a.x, a.y), f2_pack(a.z, a.w), f2_pack(b.x, b.y), f2_pack(b.z, b.w)}};
+    return o;
   }
 };
+template <typename T>
+__device__ __forceinline__ void store(T* at, const Eight& y) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f2_unpack(y.v[i], f[2 * i], f[2 * i + 1]);
+  nhv_store8(at, f);
+}
+// max(top, the eight magnitudes); NaN stays
+__device__ __forceinline__ void raise_top(float& top, const Eight& y) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    f2_unpack(y.v[i], a, b);
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(a), "f"(b));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void silu_eight(Eight& g, const Eight& u) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    if (sizeof(T) == 4) {
+      float c, d;
+      f2_unpack(g.v[i], a, b);
+      f2_unpack(u.v[i], c, d);
+      g.v[i] = f2_pack(silu_times<float>(a, c), silu_times<float>(b, d));
+    } else {                                    // as silu_times<bf16>, by pairs
+      f2_unpack(f2_mul(g.v[i], both(-1.4426950408889634f)), a, b);
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+      f2_unpack(f2_add(f2_pack(a, b), both(1.0f)), a, b);
+      asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+      asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+      g.v[i] = f2_mul(f2_mul(g.v[i], f2_pack(a, b)), u.v[i]);
+    }
+  }
+}
+__device__ __forceinline__ void add_squares(f32x2 (&ss)[2], const Eight& y) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ss[i & 1] = f2_fma(y.v[i], y.v[i], ss[i & 1]);
+}
+// y * rstd * (w + offset)
+__device__ __forceinline__ void scale_eight(Eight& y, Eight w, float rstd, float offset) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (offset != 0.f) w.v[i] = f2_add(w.v[i], both(offset));
+    y.v[i] = f2_mul(f2_mul(y.v[i], both(rstd)), w.v[i]);
+  }
+}
+template <bool EXACT>
+__device__ __forceinline__ uint2 eight_bytes(Eight y, const Divisor& d) {
+  uint32_t b[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f32x2 z;
+    if (EXACT) {
+      const f32x2 t = f2_mul(y.v[i], both(127.0f * d.m)), inv = both(d.inv), q = f2_mul(t, inv);
+      z = f2_add(f2_fma(f2_fma(q, both(-d.a), t), inv, q), both(LOW_BITS));
+    } else {
+      if (d.m != 1.0f) y.v[i] = f2_mul(y.v[i], both(d.m));
+      z = f2_fma(y.v[i], both(127.0f * d.inv), both(LOW_BITS));
+    }
+    b[2 * i] = (uint32_t)z;
+    b[2 * i + 1] = (uint32_t)(z >> 32);
+  }
+  return make_uint2(four_bytes(b[0], b[1], b[2], b[3]), four_bytes(b[4], b[5], b[6], b[7]));
+}
 
+// A thread keeps CH pieces of its row in registers from the one read to the one write.
 template <typename T, int KIND, int CH, int MOST>
 __global__ void __launch_bounds__(MOST) rows8_kernel(const Args p) {
   __shared__ float sums[32];
@@ -189,32 +274,26 @@ __global__ void __launch_bounds__(MOST) rows8_kernel(const Args p) {
       if (KIND == ROW_NORM && residual) two[i].load(residual, c);
     }
   }
-  float y[CH][8];
-  float ss = 0.f;
-  uint32_t top = 0;
+  Eight y[CH];
+  f32x2 ss[2] = {0ull, 0ull};
+  float top = 0.f;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
     if (c >= pieces) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[i][e] = 0.f;
+      y[i].v[0] = y[i].v[1] = y[i].v[2] = y[i].v[3] = 0ull;
       continue;
     }
-    one[i].get(y[i]);
-    if (KIND == ROW_UNIT || (KIND == ROW_NORM && residual)) {
-      float u[8];
-      two[i].get(u);
+    y[i] = one[i].get();
+    if (KIND == ROW_UNIT) silu_eight<T>(y[i], two[i].get());
+    if (KIND == ROW_NORM && residual) {
+      const Eight u = two[i].get();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[i][e] = KIND == ROW_UNIT ? silu_times<T>(y[i][e], u[e]) : y[i][e] + u[e];
-      if (KIND == ROW_NORM && p.write_residual) nhv_store8(residual + 8 * c, y[i]);
+      for (int e = 0; e < 4; ++e) y[i].v[e] = f2_add(y[i].v[e], u.v[e]);
+      if (p.write_residual) store(residual + 8 * c, y[i]);
     }
-    if (KIND == ROW_NORM) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(y[i][e], y[i][e], ss);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, magnitude(y[i][e]));
-    }
+    if (KIND == ROW_NORM) add_squares(ss, y[i]);
+    else raise_top(top, y[i]);
   }
   if (KIND == ROW_NORM) {
 #pragma unroll
@@ -222,20 +301,15 @@ __global__ void __launch_bounds__(MOST) rows8_kernel(const Args p) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c < pieces) one[i].load(p.weight, c);                  // on its way beside the sum
     }
-    const float rstd = 1.0f / sqrtf(all_sum(ss, sums) / (float)p.width + p.eps);
+    const float rstd = 1.0f / sqrtf(all_sum(f2_sum(ss[0], ss[1]), sums) / (float)p.width + p.eps);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       if (threadIdx.x + i * blockDim.x >= pieces) continue;
-      float w[8];
-      one[i].get(w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[i][e] = y[i][e] * rstd * (w[e] + p.weight_offset);
-        top = max(top, magnitude(y[i][e]));
-      }
+      scale_eight(y[i], one[i].get(), rstd, p.weight_offset);
+      raise_top(top, y[i]);
     }
   }
-  const float a = __uint_as_float(all_max(top, tops));
+  const float a = __uint_as_float(all_max(__float_as_uint(top), tops));
   const bool finite = a < __int_as_float(0x7f800000), some = finite && a > 0.f;
   if (threadIdx.x == 0) p.scales[r] = finite ? a / 127.0f : __int_as_float(0x7fc00000);
   const Divisor d = divisor_of(some ? a : 1.0f);
@@ -243,28 +317,19 @@ __global__ void __launch_bounds__(MOST) rows8_kernel(const Args p) {
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
-    if (c >= pieces) continue;
-    uint2 out = make_uint2(0, 0);
-    if (some) {
-      uint32_t b[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) b[e] = rounded_byte(y[i][e], d);
-      out = make_uint2(four_bytes(b[0], b[1], b[2], b[3]), four_bytes(b[4], b[5], b[6], b[7]));
-    }
-    *reinterpret_cast<uint2*>(q + 8 * c) = out;
+    if (c < pieces) *reinterpret_cast<uint2*>(q + 8 * c) = some ? eight_bytes<KIND == ROW_PLAIN>(y[i], d) : make_uint2(0, 0);
   }
 }
 
 // Wider rows: the row in 32 bits in shared memory, so that two blocks share an SM and one reads while the other writes.
 constexpr int WIDE_THREADS = 512;
-
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
 
 template <typename T, int KIND>
 __global__ void __launch_bounds__(WIDE_THREADS, 2) rows8_wide_kernel(const Args p) {
-  extern __shared__ float4 kept[];               // first and second halves of the eights: neighbouring threads, neighbouring 16 bytes
+  extern __shared__ ulonglong2 kept[];           // first and second halves of the eights: neighbouring threads, neighbouring 16 bytes
   __shared__ float sums[32];
   __shared__ uint32_t tops[32];
   pdl_prologue();
@@ -272,25 +337,30 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) rows8_wide_kernel(const Args 
   const int pieces = p.width >> 3;
   const T* x = reinterpret_cast<const T*>(p.x) + r * p.x_stride;
   T* residual = KIND == ROW_NORM && p.residual ? reinterpret_cast<T*>(p.residual) + r * (long long)p.width : nullptr;
-  float ss = 0.f;
-  uint32_t top = 0;
+  f32x2 ss[2] = {0ull, 0ull};
+  float top = 0.f;
   const bool pair = KIND == ROW_UNIT || (KIND == ROW_NORM && residual);
+  auto keep = [&](int c, const Eight& y) {
+    kept[c] = make_ulonglong2(y.v[0], y.v[1]);
+    kept[pieces + c] = make_ulonglong2(y.v[2], y.v[3]);
+  };
+  auto kept_eight = [&](int c) -> Eight {
+    const ulonglong2 a = kept[c], b = kept[pieces + c];
+    Eight y = {{a.x, a.y, b.x, b.y}};
+    return y;
+  };
   auto take = [&](int c, const Piece<T>& one, const Piece<T>& two) {
-    float y[8], u[8];
-    one.get(y);
-    if (pair) {
-      two.get(u);
+    Eight y = one.get();
+    if (KIND == ROW_UNIT) silu_eight<T>(y, two.get());
+    if (KIND == ROW_NORM && pair) {
+      const Eight u = two.get();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = KIND == ROW_UNIT ? silu_times<T>(y[e], u[e]) : y[e] + u[e];
-      if (KIND == ROW_NORM && p.write_residual) nhv_store8(residual + 8 * c, y);
+      for (int e = 0; e < 4; ++e) y.v[e] = f2_add(y.v[e], u.v[e]);
+      if (p.write_residual) store(residual + 8 * c, y);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (KIND == ROW_NORM) ss = fmaf(y[e], y[e], ss);
-      else top = max(top, magnitude(y[e]));
-    }
-    kept[c] = make_float4(y[0], y[1], y[2], y[3]);
-    kept[pieces + c] = make_float4(y[4], y[5], y[6], y[7]);
+    if (KIND == ROW_NORM) add_squares(ss, y);
+    else raise_top(top, y);
+    keep(c, y);
   };
   if (sizeof(T) == 2) {
     // A thread's pieces of both operands lie where its sums will, all of them on their way at once.
@@ -325,36 +395,23 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) rows8_wide_kernel(const Args 
     }
   }
   if (KIND == ROW_NORM) {
-    const float rstd = 1.0f / sqrtf(all_sum(ss, sums) / (float)p.width + p.eps);
+    const float rstd = 1.0f / sqrtf(all_sum(f2_sum(ss[0], ss[1]), sums) / (float)p.width + p.eps);
     for (int c = threadIdx.x; c < pieces; c += WIDE_THREADS) {
       Piece<T> weight;
       weight.load(p.weight, c);
-      float w[8];
-      weight.get(w);
-      const float4 a = kept[c], b = kept[pieces + c];
-      float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[e] = y[e] * rstd * (w[e] + p.weight_offset);
-        top = max(top, magnitude(y[e]));
-      }
-      kept[c] = make_float4(y[0], y[1], y[2], y[3]);
-      kept[pieces + c] = make_float4(y[4], y[5], y[6], y[7]);
+      Eight y = kept_eight(c);
+      scale_eight(y, weight.get(), rstd, p.weight_offset);
+      raise_top(top, y);
+      keep(c, y);
     }
   }
-  const float a = __uint_as_float(all_max(top, tops));
+  const float a = __uint_as_float(all_max(__float_as_uint(top), tops));
   const bool finite = a < __int_as_float(0x7f800000), some = finite && a > 0.f;
   if (threadIdx.x == 0) p.scales[r] = finite ? a / 127.0f : __int_as_float(0x7fc00000);
   const Divisor d = divisor_of(some ? a : 1.0f);
   int8_t* q = p.q + r * p.q_stride;
-  for (int c = threadIdx.x; c < pieces; c += WIDE_THREADS) {
-    const float4 y = kept[c], z = kept[pieces + c];
-    uint2 out = make_uint2(0, 0);
-    if (some)
-      out = make_uint2(four_bytes(rounded_byte(y.x, d), rounded_byte(y.y, d), rounded_byte(y.z, d), rounded_byte(y.w, d)),
-                       four_bytes(rounded_byte(z.x, d), rounded_byte(z.y, d), rounded_byte(z.z, d), rounded_byte(z.w, d)));
-    *reinterpret_cast<uint2*>(q + 8 * c) = out;
-  }
+  for (int c = threadIdx.x; c < pieces; c += WIDE_THREADS)
+    *reinterpret_cast<uint2*>(q + 8 * c) = some ? eight_bytes<KIND == ROW_PLAIN>(kept_eight(c), d) : make_uint2(0, 0);
 }
 
 template <typename T, int KIND, int CH>
@@ -367,10 +424,12 @@ int launch_eights(const Args& p, int n_rows, cudaStream_t stream) {
   return 0;
 }
 
-// Which kernel and how many pieces a thread; us a call for 1 / 2 / 4 pieces, bfloat16: the norm of 8 rows of 4,096 2.0 / 2.1 / 2.3, of 512 5.3 / 5.8 /
-// 5.5, of 2,048 14.1 / 11.9 / 12.4, of 8,191 of 5,120 64 / 52 / 50; 24,576 plain rows of 4,096 74 / 62 / 58; the unit of 8 rows of 12,288 2.8 / 2.7 / 3.0,
-// of 2,048 27.7 / 27.8 / 25.7.  Kept in shared memory / registers: the unit of 2,048 rows of 16,384 32 / 34, of 25,600 54 / 74, of 512 rows 17 / 22, of 8 (the
-// registers' way) 4.9; of 2,048 rows of 4,096 and 12,288 48 / 30 (8,192 rows) and 27 / 25.  In 32 bits the way goes by the width alone: it decides in which order a norm's squares are added.
+// Which kernel and how many pieces a thread; us a call for 1 / 2 / 4 pieces, bfloat16 (before the arithmetic went by pairs, which took a tenth off):
+// the norm of 8 rows of 4,096 2.0 / 2.1 / 2.3, of 512 5.3 / 5.8 / 5.5, of 2,048 14.1 / 11.9 / 12.4, of 8,191 of 5,120 64 / 52 / 50; 24,576 plain rows of
+// 4,096 74 / 62 / 58; the unit of 8 rows of 12,288 2.8 / 2.7 / 3.0, of 2,048 27.7 / 27.8 / 25.7.  Kept in shared memory / registers: the unit of
+// 2,048 rows of 16,384 32 / 34, of 25,600 54 / 74, of 512 rows 17 / 22; of 8,192 rows of 4,096 48 / 30, of 2,048 of 12,288 27 / 25.  In 32 bits the way goes by the
+// width alone: it decides in which order a norm's squares are added.
+// Now: the norm of 8,191 rows of 5,120 47 us (6.2 TB/s), the unit of 2,048 of 25,600 46 (5.7), 24,576 plain rows of 4,096 47 (6.4), 8 rows of 4,096 1.3 to 2.1.
 template <typename T, int KIND>
 int launch_row(const Args& p, int n_rows, cudaStream_t stream) {
   const long long item = sizeof(T);
