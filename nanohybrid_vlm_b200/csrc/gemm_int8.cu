@@ -1,11 +1,28 @@
 // out[t, n] = (sum_k x[t, k] w[n, k]) * x_scales[t] * w_scales[n] for x [T, K] and w [N, K] of 8-bit integers; out bfloat16 or float32.
 //
 // The sum is exact in 32 bits (K <= 131,071: K * 128 * 128 < 2^31), so no cut of K and no order of adding changes an output: only the
-// conversion of the sum to a float and the products with the two scales round, and the store once more.
+// conversion of the sum to a float and the products with the two scales round (24 bits each), and the store once more.
+//
+// Two families on the tensor cores of the 5th generation, tcgen05.mma kind::i8 with 32-bit sums in tensor memory and both operands by TMA
+// (128-byte swizzle; what lies behind a matrix arrives as zeros, so no size needs padding):
+//   up to 128 tokens, where the weight's one read is the work: product_split_kernel, rows of the weight on the MMA's M axis;
+//   more, where the arithmetic is: product_pair_kernel, pairs of SMs on tiles of 256 tokens.
+// B200: 8 x 4,096 x 24,576 18 us (5.5 TB/s of weight; reading it alone takes 16.5), 64 x 12,288 x 4,096 13.4, 2,048 x 4,096 x 24,576 116 us in a prompt's step
+// (3.55 POP/s; back to back for a while the power cap leaves 2.7 to 3.2).
 #include <string.h>
 
+#ifndef NHV_WAIT_LIMIT
 #define NHV_WAIT_LIMIT (1u << 22)
+#endif
 #include "nhv_async.cuh"
+
+// Test builds only (tests compile this file into a library of its own with a short NHV_WAIT_LIMIT): the producers leave stage
+// NHV_TEST_DROP_UNIT unsent, so that the waits for it run out.
+#ifdef NHV_TEST_DROP_UNIT
+#define NHV_UNIT_IS_SENT(i) ((i) != (NHV_TEST_DROP_UNIT))
+#else
+#define NHV_UNIT_IS_SENT(i) true
+#endif
 
 namespace {
 
@@ -185,7 +202,20 @@ struct alignas(64) Mapped {
   int share, parts_bytes;                     // tokens that a block of a cluster finishes, and room for all parts of theirs
 };
 
-// ---- few tokens: 128 rows of the weight on the MMA's M axis, up to NT tokens on its N axis.
+// ---- up to 128 tokens: up to 128 rows of the weight on the MMA's M axis, the tokens on its N axis.
+//
+// A block takes a tile of the weight's rows and one part of K; the blocks of a tile are a cluster.  The tile's height is free: the TMA box has
+// that many rows, the MMA reads 128 from the stage's start and the sums of the rows behind are not looked at.  So the weight's rows divide
+// evenly over the SMs, whatever N is.  Warp roles: TMA producer, MMA issuer, eight epilogue warps.  Before it waits for the kernel before it the
+// producer asks its first stages into L2 (not into shared memory: the weight may be that kernel's output).
+//
+// With K in parts every block sends each token's sums to the one of the cluster that finishes the token, 16 bytes a lane into the other's
+// shared memory, and after one meeting that block adds them up, which is exact, and writes.  (Parked sums that the finisher reads
+// from the others, with two meetings: 64 x 12,288 x 4,096 13.6 us against 12.7, 64 x 4,096 x 4,096 8.7 against 7.2.)
+//
+// What bounds it: memory while a block streams (two blocks an SM, some 200 KB on their way); start and end of a launch, 3 us, beside that; with
+// 64 tokens and more also what the tiles read of x, from L2.  The MMA issuer's operands are the same in every lane and the compiler has to see
+// that (the warp's number by a shuffle, elect.sync): 407 -> 305 cycles a stage.
 constexpr int SPLIT_THREADS = 320;     // producer warp, MMA warp, eight epilogue warps
 
 // One output of each of up to 16 tokens.
@@ -202,17 +232,16 @@ __device__ __forceinline__ void store_column16(O* at, long long stride, const in
 }
 __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __grid_constant__ Mapped m) {
   const int STAGES = m.stages, W_BYTES = m.w_bytes, STAGE_BYTES = W_BYTES + m.nt * BK;
-  const int tall = m.rows > 128 ? 2 : 1;                         // accumulators: 128 rows each
-  const uint32_t COLUMNS = tall * m.nt <= 32 ? 32 : tall * m.nt <= 64 ? 64 : tall * m.nt <= 128 ? 128 : tall * m.nt <= 256 ? 256 : 512;
+  const uint32_t COLUMNS = m.nt <= 32 ? 32 : m.nt <= 64 ? 64 : 128;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* ring = smem_unaligned + ((1024 - (smem_u32(smem_unaligned) & 1023)) & 1023);
-  int* parts = reinterpret_cast<int*>(ring + m.ring_bytes);       // [part][share of the tokens / 4][tall * 128][4]
+  int* parts = reinterpret_cast<int*>(ring + m.ring_bytes);       // [part][share of the tokens / 4][128][4]
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + m.ring_bytes + m.parts_bytes);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   __shared__ int s_abort;
-  __shared__ float s_xs[256];
+  __shared__ float s_xs[128];
 
   const Product& p = m.p;
   const int warp = (int)same_in_all(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -249,10 +278,12 @@ __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __gr
       uint32_t s = 0, phase = 1;
       for (int i = 0; i < n; ++i) {
         if (i >= STAGES && !mbar_wait(&empty[s], phase, 1)) { s_abort = 1; break; }
-        unsigned char* dst = ring + (size_t)s * STAGE_BYTES;
-        mbar_expect_tx(&full[s], bytes);
-        tma_load_2d(dst, &m.w_map, (k0 + i) * BK, n0, &full[s]);
-        tma_load_2d(dst + W_BYTES, &m.x_map, (k0 + i) * BK, t0, &full[s]);
+        if (NHV_UNIT_IS_SENT(i)) {
+          unsigned char* dst = ring + (size_t)s * STAGE_BYTES;
+          mbar_expect_tx(&full[s], bytes);
+          tma_load_2d(dst, &m.w_map, (k0 + i) * BK, n0, &full[s]);
+          tma_load_2d(dst + W_BYTES, &m.x_map, (k0 + i) * BK, t0, &full[s]);
+        }
         if (++s == (uint32_t)STAGES) { s = 0; phase ^= 1; }
       }
     }
@@ -272,10 +303,6 @@ __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __gr
 #pragma unroll
         for (int kk = 0; kk < BK / UMMA_K; ++kk)
           tc_mma<1>(tmem_base, a + kk * (UMMA_K >> 4), b + kk * (UMMA_K >> 4), idesc, (i > 0 || kk > 0) ? 1u : 0u);
-        if (tall == 2)
-#pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            tc_mma<1>(tmem_base + (uint32_t)m.nt, a + (128 * BK >> 4) + kk * (UMMA_K >> 4), b + kk * (UMMA_K >> 4), idesc, (i > 0 || kk > 0) ? 1u : 0u);
         tc_commit<1>(&empty[s]);
         if (i == n - 1) tc_commit<1>(acc_full);
       }
@@ -290,36 +317,33 @@ __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __gr
     if (tid < tokens) s_xs[tid] = p.x_scales[t0 + tid];
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
     // the tensor-memory lanes that this warp may read; every second piece of 16 tokens is its
-    const int quarter = warp & 3, row = quarter * 32 + lane, second = warp >= 6;
-    const float ws[2] = {n0 + row < n_end ? p.w_scales[n0 + row] : 0.f, n0 + 128 + row < n_end ? p.w_scales[n0 + 128 + row] : 0.f};
+    const int quarter = warp & 3, row = quarter * 32 + lane, second = warp >= 6, n = n0 + row;
+    const float ws = n < n_end ? p.w_scales[n] : 0.f;
     const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, 3));
     tc_fence_after();
     if (S > 1) cluster_wait();                                   // all blocks of the cluster run
     if (!ok) {
       s_abort = 1;
     } else {
-      for (int u = 0; u < tall; ++u) {
-        const int n = n0 + u * 128 + row;
-        const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(u * m.nt);
-        for (int c = second * 16; c < tokens; c += 32) {
-          int v[16];
-          tmem_ld16(v, at + c);
-          tmem_ld_wait();
-          if (S > 1) {                                           // four tokens' sums at a time to the block that finishes them
+      const uint32_t at = tmem_base + ((uint32_t)(quarter * 32) << 16);
+      for (int c = second * 16; c < tokens; c += 32) {
+        int v[16];
+        tmem_ld16(v, at + c);
+        tmem_ld_wait();
+        if (S > 1) {                                             // four tokens' sums at a time to the block that finishes them
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              if (c + j >= tokens) break;
-              const int owner = (c + j) / m.share, four = (c + j - owner * m.share) >> 2;
-              const int* to = parts + (((rank * (m.share >> 2) + four) * tall * 128 + u * 128 + row) << 2);
-              store_cluster4(in_block(smem_u32(to), owner), v[j], v[j + 1], v[j + 2], v[j + 3]);
-            }
-          } else if (n < n_end) {
-            const long long o = (long long)(t0 + c) * p.out_stride + n;
-            if (p.out_f32)
-              store_column16(reinterpret_cast<float*>(p.out) + o, p.out_stride, v, s_xs + c, ws[u], tokens - c);
-            else
-              store_column16(reinterpret_cast<bf16*>(p.out) + o, p.out_stride, v, s_xs + c, ws[u], tokens - c);
+          for (int j = 0; j < 16; j += 4) {
+            if (c + j >= tokens) break;
+            const int owner = (c + j) / m.share, four = (c + j - owner * m.share) >> 2;
+            const int* to = parts + (((rank * (m.share >> 2) + four) * 128 + row) << 2);
+            store_cluster4(in_block(smem_u32(to), owner), v[j], v[j + 1], v[j + 2], v[j + 3]);
           }
+        } else if (n < n_end) {
+          const long long o = (long long)(t0 + c) * p.out_stride + n;
+          if (p.out_f32)
+            store_column16(reinterpret_cast<float*>(p.out) + o, p.out_stride, v, s_xs + c, ws, tokens - c);
+          else
+            store_column16(reinterpret_cast<bf16*>(p.out) + o, p.out_stride, v, s_xs + c, ws, tokens - c);
         }
       }
     }
@@ -329,23 +353,20 @@ __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __gr
       cluster_arrive();
       cluster_wait();                                            // all parts have arrived
       const int j0 = rank * m.share, fours = (min(tokens, j0 + m.share) - j0 + 3) >> 2;
-      for (int u = 0; u < tall; ++u) {
-        const int n = n0 + u * 128 + row;
-        for (int f = second; f < fours && n < n_end; f += 2) {
-          const int4* from = reinterpret_cast<const int4*>(parts) + f * tall * 128 + u * 128 + row;
-          int4 part[8];
+      for (int f = second; f < fours && n < n_end; f += 2) {
+        const int4* from = reinterpret_cast<const int4*>(parts) + f * 128 + row;
+        int4 part[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) part[q] = q < S ? from[q * (m.share >> 2) * tall * 128] : make_int4(0, 0, 0, 0);
-          int sum[4] = {};
+        for (int q = 0; q < 8; ++q) part[q] = q < S ? from[q * (m.share >> 2) * 128] : make_int4(0, 0, 0, 0);
+        int sum[4] = {};
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            sum[0] += part[q].x; sum[1] += part[q].y; sum[2] += part[q].z; sum[3] += part[q].w;
-          }
+        for (int q = 0; q < 8; ++q) {
+          sum[0] += part[q].x; sum[1] += part[q].y; sum[2] += part[q].z; sum[3] += part[q].w;
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = j0 + f * 4 + e;
-            if (j < tokens) store_out(p, t0 + j, n, scaled(sum[e], s_xs[j], ws[u]));
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + f * 4 + e;
+          if (j < tokens) store_out(p, t0 + j, n, scaled(sum[e], s_xs[j], ws));
         }
       }
     }
@@ -361,8 +382,12 @@ __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __gr
   if (warp == 1) tmem_dealloc<1>(tmem_base, COLUMNS);
 }
 
-// ---- many tokens: pairs of blocks, 256 tokens on the MMA's M axis (128 a block), TN outputs on its N axis (TN / 2 rows of the weight in
-// each block's shared memory), tiles handed out in turn to a grid of one pair for two SMs.
+// ---- more than 128 tokens: pairs of blocks (cta_group::2), 256 tokens on the MMA's M axis (128 a block), TN outputs on its N axis (TN / 2 rows of
+// the weight in each block's shared memory), tiles handed out in turn to a grid of one pair for two SMs.
+//
+// Bound by the tensor pipe (90 % of its cycles at 2,048 x 4,096 x 24,576) and, back to back, by the power cap.  A pair reads each operand's
+// bytes once for both SMs, two accumulators let a tile's MMAs run beside the last one's epilogue, and outputs leave by TMA stores from 2 KB a
+// warp (8,192 x 256 x 4,096 in bfloat16 25.8 -> 22.7 us, in float32 55 -> 40).  Block 0's barriers count both blocks' copies, commits reach both.
 constexpr int PAIR_THREADS = 320;      // producer warp, MMA warp, eight epilogue warps
 constexpr int TURN = 2560;             // bytes of a warp's outputs on their way out: 32 rows of 64 bytes, or of 17 floats; whole 512s for the swizzle
 template <int TN>
@@ -484,6 +509,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) pro
         for (int k = 0; k < kt; ++k, ++i) {
           const int s = i % STAGES;
           if (i >= STAGES && !mbar_wait(&empty[s], (uint32_t)((i / STAGES) - 1) & 1, 1)) { ok = false; break; }
+          if (!NHV_UNIT_IS_SENT(i)) continue;
           unsigned char* dst = ring + (size_t)s * STAGE;
           const uint32_t bar = in_block(smem_u32(&full[s]), 0);
           if (rank == 0) mbar_expect_tx(&full[s], 2 * STAGE);      // zero-filled parts of a box count too
@@ -620,13 +646,12 @@ struct SplitSmem {
   size_t all;
 };
 SplitSmem split_smem(const SplitPlan& plan) {
-  const int tall = plan.rows > 128 ? 2 : 1;
   SplitSmem s;
   s.w_bytes = (plan.rows * BK + 1023) / 1024 * 1024;
-  // the MMAs read 128 or 256 rows from a stage's start, whatever the stage holds
-  s.ring_bytes = (plan.stages - 1) * (s.w_bytes + plan.nt * BK) + tall * 128 * BK + plan.nt * BK;
+  // the MMAs read 128 rows from a stage's start, whatever lies there
+  s.ring_bytes = (plan.stages - 1) * (s.w_bytes + plan.nt * BK) + 128 * BK + plan.nt * BK;
   s.share = ((plan.nt + plan.parts - 1) / plan.parts + 3) / 4 * 4;
-  s.parts_bytes = plan.parts > 1 ? plan.parts * s.share * tall * 512 : 0;
+  s.parts_bytes = plan.parts > 1 ? plan.parts * s.share * 512 : 0;
   s.all = 1024 + (size_t)s.ring_bytes + s.parts_bytes + (2 * plan.stages + 1) * 8 + 16;
   return s;
 }
@@ -665,7 +690,7 @@ SplitPlan split_plan(const Product& p, int sms) {
 
 int split_product(Mapped& m, const SplitPlan& plan, cudaStream_t stream) {
   const Product& p = m.p;
-  NHV_REQUIRE(plan.rows >= 1 && plan.rows <= 256 && plan.nt >= 16 && plan.nt <= 256 && plan.nt % 16 == 0 && plan.stages >= 1 && plan.stages <= 16 && plan.parts >= 1 &&
+  NHV_REQUIRE(plan.rows >= 1 && plan.rows <= 128 && plan.nt >= 16 && plan.nt <= 128 && plan.nt % 16 == 0 && plan.stages >= 1 && plan.stages <= 16 && plan.parts >= 1 &&
               plan.parts <= 8, "linear_int8: tiles of %d rows and %d tokens, %d stages, %d parts", plan.rows, plan.nt, plan.stages, plan.parts);
   m.nt = plan.nt;
   m.rows = plan.rows;
