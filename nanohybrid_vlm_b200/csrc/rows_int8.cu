@@ -520,6 +520,7 @@ struct RowsCall {
   int kind, dtype, n_rows, width, write_residual;
   float eps, weight_offset;
 };
+static_assert(sizeof(RowsCall) == 88, "the block ends with four bytes that nobody reads");
 
 // kind: 0 the rows of x, 1 their RMS norm (residual may be null), 2 silu(first half) * second half of rows of 2 * width.
 NHV_API int nhv_rows_int8(const void* given, cudaStream_t stream) {
@@ -534,10 +535,17 @@ NHV_API int nhv_rows_int8(const void* given, cudaStream_t stream) {
   return c.dtype == NHV_F32 ? launch_kind<float>(c.kind, p, c.n_rows, stream) : launch_kind<bf16>(c.kind, p, c.n_rows, stream);
 }
 
-NHV_API int nhv_rows_from_int8(void* out, int dtype, long long out_stride, const void* q, long long q_stride, const float* scales, int n_rows, int width,
-                               cudaStream_t stream) {
-  if (n_rows == 0 || width == 0) return 0;
-  NHV_REQUIRE(n_rows > 0 && width > 0 && out && q && scales && (dtype == NHV_F32 || dtype == NHV_BF16), "dequantize_rows: bad arguments");
-  const BackArgs p = {(const int8_t*)q, scales, out, q_stride, out_stride, n_rows, width};
-  return dtype == NHV_F32 ? launch_back<float>(p, stream) : launch_back<bf16>(p, stream);
+struct BackCall {
+  long long out, q, scales, out_stride, q_stride;
+  int dtype, n_rows, width;
+};
+static_assert(sizeof(BackCall) == 56, "the block ends with four bytes that nobody reads");
+
+NHV_API int nhv_rows_from_int8(const void* given, cudaStream_t stream) {
+  BackCall c;
+  memcpy(&c, given, sizeof(c));
+  if (c.n_rows == 0 || c.width == 0) return 0;
+  NHV_REQUIRE(c.n_rows > 0 && c.width > 0 && c.out && c.q && c.scales && (c.dtype == NHV_F32 || c.dtype == NHV_BF16), "dequantize_rows: bad arguments");
+  const BackArgs p = {(const int8_t*)c.q, (const float*)c.scales, (void*)c.out, c.q_stride, c.out_stride, c.n_rows, c.width};
+  return c.dtype == NHV_F32 ? launch_back<float>(p, stream) : launch_back<bf16>(p, stream);
 }

@@ -92,7 +92,7 @@ _SIGNATURES = {
     "nhv_select_keys": [P, P, P, P, P, I, P, P, P, I, I, I, I, I, I, I, I, P],
     "nhv_move_keys": [P, P, P, P, I, I, P, P, I, I, I, I, I, I, P],
     "nhv_rows_int8": [ctypes.c_char_p, P],
-    "nhv_rows_from_int8": [P, I, ctypes.c_longlong, P, ctypes.c_longlong, P, I, I, P],
+    "nhv_rows_from_int8": [ctypes.c_char_p, P],
     "nhv_gemm_int8": [ctypes.c_char_p, P],
     "nhv_decay_lowrank": [I, P, P, I, P, P, I, I, I, P],
 }

@@ -1905,28 +1905,35 @@ def _check_scales(name: str, t, n: int) -> None:
         raise KernelError(f"{name} are {n} float32 numbers side by side, not {tuple(t.shape)} {t.dtype}")
 
 
-_ROWS_CALL = struct.Struct("=7q5i2f")
+_ROWS_CALL = struct.Struct("=7q5i2f4x")
+_BACK_CALL = struct.Struct("=5q3i4x")
 
 
-def _rows_int8(kind: int, q, scales, x, rows: int, width: int, x_stride: int, residual=None, weight=None, eps: float = 0.0, offset: float = 0.0,
-               write_residual: bool = False) -> None:
-    dtype, device, step = x.dtype, _current_device() if x.is_cuda else -1, q.stride()
-    if not (width > 0 and q.dtype is torch.int8 and q.shape == (rows, width) and step[1] == 1 and step[0] >= width and scales.shape == (rows,)
+def _int8_rows_quick(q, scales, x, rows: int, width: int) -> bool:
+    """The quick look at what all makers of 8-bit rows assume; where it says no, ``_check_rows_int8`` knows why, or that all is well."""
+    step, dtype = q.stride(), x.dtype
+    return (width > 0 and q.dtype is torch.int8 and q.shape == (rows, width) and step[1] == 1 and step[0] >= width and scales.shape == (rows,)
             and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32)
-            and x.get_device() == q.get_device() == scales.get_device() == device >= 0 and (weight is None or weight.get_device() == device)
-            and (residual is None or residual.get_device() == device)):
-        _check_int8_rows("the rows to write", q, rows, width)
-        _check_scales("scales", scales, rows)
-        if width < 1:
-            raise KernelError("rows of no elements have no scale")
-        dtype_code(x)
-        _same_device(q, scales, x, residual, weight)
+            and x.is_cuda and x.get_device() == q.get_device() == scales.get_device() == _current_device())
+
+
+def _check_rows_int8(q, scales, x, rows: int, width: int, *others) -> None:
+    _check_int8_rows("the 8-bit rows", q, rows, width)
+    _check_scales("scales", scales, rows)
+    if width < 1:
+        raise KernelError("rows of no elements have no scale")
+    dtype_code(x)
+    _same_device(q, scales, x, *others)
+
+
+def _rows_int8(kind: int, q, scales, x, rows: int, width: int, x_stride: int) -> None:
+    if not _int8_rows_quick(q, scales, x, rows, width):
+        _check_rows_int8(q, scales, x, rows, width)
     q_at, x_at = q.data_ptr(), x.data_ptr()
     if q_at == x_at and rows:
         raise KernelError("the 8-bit rows have memory of their own: other rows are still read from what lies there")
-    call("nhv_rows_int8", _ROWS_CALL.pack(
-        q_at, scales.data_ptr(), x_at, residual.data_ptr() if residual is not None else 0, weight.data_ptr() if weight is not None else 0,
-        step[0] if rows > 1 else width, x_stride, kind, BF16 if dtype is torch.bfloat16 else F32, rows, width, write_residual, eps, offset), stream_ptr())
+    call("nhv_rows_int8", _ROWS_CALL.pack(q_at, scales.data_ptr(), x_at, 0, 0, q.stride(0) if rows > 1 else width, x_stride, kind,
+                                          BF16 if x.dtype is torch.bfloat16 else F32, rows, width, 0, 0.0, 0.0), stream_ptr())
 
 
 def quantize_rows(q, scales, x) -> None:
@@ -1939,11 +1946,7 @@ def quantize_rows(q, scales, x) -> None:
     _rows_int8(0, q, scales, x, rows, width, x.stride(0) if rows > 1 else width)
 
 
-def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual: bool = True, weight_offset: float = 0.0) -> None:
-    """``rmsnorm`` with its output in 8 bits: q [n, width] int8 and scales [n] as ``quantize_rows`` gives them for norm(x (+ residual)) *
-    (weight + weight_offset), which is held in 32 bits and rounded once.  With a residual and write_residual the sum, rounded to x's
-    type, replaces the residual."""
-    width = x.shape[-1] if x.dim() else 0
+def _check_rmsnorm_int8(q, scales, x, weight, residual, write_residual: bool, rows: int, width: int) -> None:
     _contig("x", x)
     if weight.dtype != x.dtype or weight.numel() != width or not weight.is_contiguous():
         raise KernelError(f"the norm's weight is {width} numbers in x's type side by side, not {tuple(weight.shape)} {weight.dtype}")
@@ -1953,8 +1956,27 @@ def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual
             raise KernelError(f"the residual has x's shape and type, not {tuple(residual.shape)} {residual.dtype}")
         if write_residual and residual.data_ptr() == x.data_ptr() and x.numel():
             raise KernelError("the residual has memory of its own: its sum with x is written there")
+    _check_rows_int8(q, scales, x, rows, width, weight, residual)
+
+
+def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual: bool = True, weight_offset: float = 0.0) -> None:
+    """``rmsnorm`` with its output in 8 bits: q [n, width] int8 and scales [n] as ``quantize_rows`` gives them for norm(x (+ residual)) *
+    (weight + weight_offset), which is held in 32 bits and rounded once.  With a residual and write_residual the sum, rounded to x's
+    type, replaces the residual."""
+    shape, dtype = x.shape, x.dtype
+    width = shape[-1] if shape else 0
     rows = x.numel() // width if width else 0
-    _rows_int8(1, q, scales, x, rows, width, width, residual, weight, eps, weight_offset, write_residual and residual is not None)
+    x_at, residual_at, q_at = x.data_ptr(), 0 if residual is None else residual.data_ptr(), q.data_ptr()
+    if not (_int8_rows_quick(q, scales, x, rows, width) and x.is_contiguous() and weight.dtype is dtype and weight.shape == (width,)
+            and weight.is_contiguous() and weight.get_device() == x.get_device()
+            and (residual is None or (residual.shape == shape and residual.dtype is dtype and residual.is_contiguous() and residual_at != x_at
+                                      and residual.get_device() == x.get_device()))):
+        _check_rmsnorm_int8(q, scales, x, weight, residual, write_residual, rows, width)
+    if rows and (q_at == x_at or q_at == residual_at):
+        raise KernelError("the 8-bit rows have memory of their own: other rows are still read from what lies there")
+    call("nhv_rows_int8", _ROWS_CALL.pack(
+        q_at, scales.data_ptr(), x_at, residual_at, weight.data_ptr(), q.stride(0) if rows > 1 else width, width, 1, BF16 if dtype is torch.bfloat16 else F32,
+        rows, width, write_residual and residual is not None, eps, weight_offset), stream_ptr())
 
 
 def silu_mul_int8(q, scales, gate_up) -> None:
@@ -1963,31 +1985,30 @@ def silu_mul_int8(q, scales, gate_up) -> None:
     _contig("gate_up", gate_up)
     if gate_up.dim() != 2 or gate_up.shape[1] % 2:
         raise KernelError(f"gate_up is [n, 2 * inter], not {tuple(gate_up.shape)}")
-    rows, inter = gate_up.shape[0], gate_up.shape[1] // 2
-    _rows_int8(2, q, scales, gate_up, rows, inter, 2 * inter)
+    rows, both = gate_up.shape
+    _rows_int8(2, q, scales, gate_up, rows, both // 2, both)
 
 
 def dequantize_rows(out, q, scales) -> None:
     """out[n, width] = q * scales[:, None]: the values that rows of 8-bit integers stand for, rounded once to out's type (bfloat16 or float32).
     Rows of out and q may lie further apart."""
-    if out.dim() != 2 or (out.stride(1) != 1 and out.shape[1] > 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
-        raise KernelError(f"out is a matrix with neighbouring columns and rows that do not overlap, not {tuple(out.shape)} with strides {out.stride()}")
-    rows, width = out.shape
-    device, step, dtype = _current_device() if out.is_cuda else -1, q.stride(), out.dtype
-    if not (q.dtype is torch.int8 and q.shape == (rows, width) and step[1] == 1 and step[0] >= width and scales.shape == (rows,)
-            and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32)
-            and out.get_device() == q.get_device() == scales.get_device() == device >= 0):
-        _check_int8_rows("the rows to read", q, rows, width)
-        _check_scales("scales", scales, rows)
-        dtype_code(out)
-        _same_device(out, q, scales)
-    if out.data_ptr() == q.data_ptr() and rows and width:
+    shape, step = out.shape, out.stride()
+    if len(shape) != 2 or (step[1] != 1 and shape[1] > 1) or (step[0] < shape[1] and shape[0] > 1):
+        raise KernelError(f"out is a matrix with neighbouring columns and rows that do not overlap, not {tuple(shape)} with strides {step}")
+    rows, width = shape
+    if not _int8_rows_quick(q, scales, out, rows, width):
+        if width:
+            _check_rows_int8(q, scales, out, rows, width)
+        else:
+            return
+    out_at, q_at = out.data_ptr(), q.data_ptr()
+    if out_at == q_at and rows:
         raise KernelError("the values have memory of their own: other rows are still read from what lies there")
-    call("nhv_rows_from_int8", out.data_ptr(), BF16 if dtype is torch.bfloat16 else F32, out.stride(0) if rows > 1 else width, q.data_ptr(),
-         step[0] if rows > 1 else width, scales.data_ptr(), rows, width, stream_ptr())
+    call("nhv_rows_from_int8", _BACK_CALL.pack(out_at, q_at, scales.data_ptr(), step[0] if rows > 1 else width, q.stride(0) if rows > 1 else width,
+                                               BF16 if out.dtype is torch.bfloat16 else F32, rows, width), stream_ptr())
 
 
-_PRODUCT_CALL = struct.Struct("=10q5i")
+_PRODUCT_CALL = struct.Struct("=10q5i4x")
 
 
 def _check_linear_int8(out, x, x_scales, weight, weight_scales) -> None:

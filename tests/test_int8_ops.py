@@ -49,8 +49,8 @@ def rows(**other):
 
 
 @pytest.mark.parametrize("other, text", [
-    (dict(q=torch.empty(4, 11, dtype=I8)), "rows to write"),
-    (dict(q=torch.empty(4, 10, dtype=torch.int16)), "rows to write"),
+    (dict(q=torch.empty(4, 11, dtype=I8)), "8-bit rows"),
+    (dict(q=torch.empty(4, 10, dtype=torch.int16)), "8-bit rows"),
     (dict(q=torch.empty(10, dtype=I8).expand(4, 10)), "do not overlap"),
     (dict(scales=torch.empty(5)), "scales"),
     (dict(scales=torch.empty(4, dtype=torch.float64)), "scales"),
@@ -86,7 +86,7 @@ def test_rows_of_other_inputs_refused():
 
 def test_values_refused():
     q, s = torch.zeros(4, 10, dtype=I8), torch.zeros(4)
-    for out, q_, s_, text in ((torch.empty(4, 11), q, s, "rows to read"), (torch.empty(4, 10).t(), q, s, "neighbouring"),
+    for out, q_, s_, text in ((torch.empty(4, 11), q, s, "8-bit rows"), (torch.empty(4, 10).t(), q, s, "neighbouring"),
                               (torch.empty(10).expand(4, 10), q, s, "do not overlap"), (torch.empty(4, 10), q, torch.zeros(3), "scales"),
                               (torch.empty(4, 10, dtype=torch.float16), q, s, "float32 or bfloat16"), (torch.empty(4, 10), q, s, "GPU only")):
         with pytest.raises(KernelError, match=text):
@@ -105,3 +105,8 @@ def test_engine_option(model_dirs):
     assert Config(model_dirs["A"], quantization="int8").quantization == "int8" and Config(model_dirs["A"]).quantization is None
     with pytest.raises(ConfigError, match="int8"):
         Config(model_dirs["A"], quantization="int4")
+
+
+def test_call_blocks_have_the_size_of_the_librarys_structs():
+    """Eight-byte members come first, and a struct's size is a multiple of eight: the library reads so many bytes."""
+    assert (ops._ROWS_CALL.size, ops._BACK_CALL.size, ops._PRODUCT_CALL.size) == (88, 56, 104)

@@ -76,12 +76,16 @@ def test_products_of_many_tokens(ops, T, K, N, out):
     check_product(ops, T, K, N, out, seed=T)
 
 
+@pytest.mark.parametrize("T,K,N,out,pad", [(300, 320, 200, BF, 8), (257, 96, 1000, F, 4), (140, 64, 40, BF, 24), (60, 2048, 200, BF, 3)])
+def test_products_into_wider_rows(ops, T, K, N, out, pad):
+    """An output that is a slice of columns: what lies beside it stays."""
+    check_product(ops, T, K, N, out, out_pad=pad)
+
+
 @pytest.mark.parametrize("T", [1, 12, 40, 200, 1300])
 def test_sums_at_the_ends_of_32_bits(ops, T):
     """All products at the largest magnitude, -128 among them: K * 2^14 is just below 2^31."""
     K, N = 131071, 24
-    x = torch.full((T, K + 1), -128, dtype=torch.int8, device="cuda")[:, :K]
-    w = torch.full((N, K + 1), -128, dtype=torch.int8, device="cuda")[:, :K]
     x = ops.new_int8(T, K, "cuda").fill_(-128)
     w = ops.new_int8(N, K, "cuda").fill_(-128)
     w[1::2] = 127
@@ -316,6 +320,8 @@ def test_outputs_over_inputs_are_refused(ops):
                  lambda: ops.silu_mul_int8(over[:, :32], s, x), lambda: ops.dequantize_rows(x, over, s)):
         with pytest.raises(KernelError, match="memory of"):
             call()
+    with pytest.raises(KernelError, match="memory of"):
+        ops.rmsnorm_int8(over, s, x.clone(), x[0].clone(), 1e-6, residual=x)
     x = ops.new_int8(4, 64, "cuda").fill_(1)
     with pytest.raises(KernelError, match="memory of"):
         ops.linear_int8(x.view(torch.float32)[:, :4], x, s, x[:4].clone(), s)
