@@ -777,9 +777,10 @@ NHV_API int nhv_gemm_int8(const void* given, cudaStream_t stream) {
                      (c.out | c.out_stride * (c.out_dtype == NHV_F32 ? 4 : 2)) % 16 == 0};
   if (int e = align_rows(&p.x, &p.x_stride, (void*)c.x_copy, T, K, stream)) return e;
   if (int e = align_rows(&p.w, &p.w_stride, (void*)c.w_copy, N, K, stream)) return e;
-  // us, 128 tokens, 4,096 x 4,096 / 24,576 x 4,096 / 4,096 x 12,288: whole tiles of the weight 9.4 / 22.1 / 14.9, pairs 9.3 / 26.2 / 18.6; 256 tokens 12.7 / 33 / 19.5 and 9.3 /
-  // 26.2 / 18.6.  Up to 8 tokens the weight through registers into mma.sync was tried: alone 5.0 / 18.5 / 10.6 against 6.0 / 18.3 / 11.0, but in a decode step,
-  // behind other kernels, 7.2 / 31.5 / 18.3 against 5.1 / 17.8 / 8.5 (its blocks fill an SM, so that none starts under the kernel before)
+  // us, whole tiles of the weight / pairs: 128 tokens, 4,096 x 4,096 9.4 / 9.3, 24,576 x 4,096 22.1 / 26.2, 4,096 x 12,288 14.9 / 18.6; 256 tokens 12.7 / 9.3,
+  // 33 / 26.2, 19.5 / 18.6.  Up to 8 tokens the weight through registers into mma.sync was tried: alone 5.0, 18.5 and 10.6 against 6.0, 18.3 and 11.0,
+  // but in a decode step, behind other kernels, 7.2, 31.5 and 18.3 against 5.1, 17.8 and 8.5 (its blocks fill an SM, so that none starts under
+  // the kernel before).
   Mapped m;
   m.p = p;
   if (T <= 128) return split_product(m, split_plan(p, sms), stream);

@@ -160,3 +160,18 @@ def test_command_line(model_dirs, plain8):
     tokens = next(json.loads(x)["token_ids"] for x in r.stdout.splitlines() if x.startswith("{"))
     lg = plain8["A"].logits([5, 9, 2])[-1]
     assert len(tokens) == 4 and lg[tokens[0]] >= lg.max() - TOL * lg.norm()
+
+
+def test_replay(model_dirs, tmp_path):
+    """``bin/trace_run --quantization int8`` gives the runner's logits, bit for bit in float32."""
+    import json
+    import subprocess
+    import sys
+    from trace_tools import TRACE_RUN
+    tokens = prompts_for("A", (37,), seed=9)[0]
+    line = json.dumps({"step": 0, "entries": [{"id": "a", "tokens": tokens, "want": list(range(len(tokens)))}], "end": ["a"]})
+    r = subprocess.run([sys.executable, TRACE_RUN, "--model", model_dirs["A"], "--dtype", "float32", "--out", str(tmp_path), "--max-tokens", "64",
+                        "--quantization", "int8", "--poison"], input=line + "\n", capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    got = np.fromfile(tmp_path / "0.f32", dtype="<f4").reshape(len(tokens), -1)
+    assert np.array_equal(got, Driver(model_dirs["A"]).step([("a", tokens)])[0].cpu().numpy())
