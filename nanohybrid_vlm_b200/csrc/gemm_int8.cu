@@ -761,17 +761,28 @@ NHV_API void* nhv_gemm_int8_error_word() { return nhv_wait_error_address(); }
 // What a call is given, one after the other, in one block.
 struct ProductCall {
   long long out, x, x_scales, w, w_scales, x_copy, w_copy, out_stride, x_stride, w_stride;      // the copies: room for rows that start anywhere, or 0
-  int out_dtype, T, N, K, sms;
+  int out_dtype, T, N, K;
 };
-static_assert(sizeof(ProductCall) == 104, "the block ends with four bytes that nobody reads");
+
+// The SMs of the current device, asked for once.
+static int sm_count() {
+  static std::atomic<int> known[64];
+  int device = 0, n = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return 0;
+  if (device < 64) n = known[device].load(std::memory_order_relaxed);
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess && device < 64)
+    known[device].store(n, std::memory_order_relaxed);
+  return n;
+}
 
 NHV_API int nhv_gemm_int8(const void* given, cudaStream_t stream) {
   ProductCall c;
   memcpy(&c, given, sizeof(c));
-  const int T = c.T, N = c.N, K = c.K, sms = c.sms;
+  const int T = c.T, N = c.N, K = c.K, sms = sm_count();
   if (T == 0 || N == 0) return 0;
   NHV_REQUIRE(T > 0 && N > 0 && K > 0 && K <= 131071, "linear_int8: a sum over 1 to 131,071 products is exact in 32 bits, not over %d", K);
-  NHV_REQUIRE(c.out && c.x && c.w && c.x_scales && c.w_scales && (c.out_dtype == NHV_F32 || c.out_dtype == NHV_BF16) && sms > 1, "linear_int8: bad arguments");
+  NHV_REQUIRE(c.out && c.x && c.w && c.x_scales && c.w_scales && (c.out_dtype == NHV_F32 || c.out_dtype == NHV_BF16), "linear_int8: bad arguments");
+  NHV_REQUIRE(sms > 1, "linear_int8: the device does not say how many SMs it has");
   Product p = {(const int8_t*)c.x, (const int8_t*)c.w, (const float*)c.x_scales, (const float*)c.w_scales, (void*)c.out,
                      c.x_stride, c.w_stride, c.out_stride, T, N, K, c.out_dtype == NHV_F32,
                      (c.out | c.out_stride * (c.out_dtype == NHV_F32 ? 4 : 2)) % 16 == 0};

@@ -1909,14 +1909,6 @@ _ROWS_CALL = struct.Struct("=7q5i2f4x")
 _BACK_CALL = struct.Struct("=5q3i4x")
 
 
-def _int8_rows_quick(q, scales, x, rows: int, width: int) -> bool:
-    """The quick look at what all makers of 8-bit rows assume; where it says no, ``_check_rows_int8`` knows why, or that all is well."""
-    step, dtype = q.stride(), x.dtype
-    return (width > 0 and q.dtype is torch.int8 and q.shape == (rows, width) and step[1] == 1 and step[0] >= width and scales.shape == (rows,)
-            and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32)
-            and x.is_cuda and x.get_device() == q.get_device() == scales.get_device() == _current_device())
-
-
 def _check_rows_int8(q, scales, x, rows: int, width: int, *others) -> None:
     _check_int8_rows("the 8-bit rows", q, rows, width)
     _check_scales("scales", scales, rows)
@@ -1927,13 +1919,16 @@ def _check_rows_int8(q, scales, x, rows: int, width: int, *others) -> None:
 
 
 def _rows_int8(kind: int, q, scales, x, rows: int, width: int, x_stride: int) -> None:
-    if not _int8_rows_quick(q, scales, x, rows, width):
+    dtype, device, q_at, x_at = x.dtype, x.get_device(), q.data_ptr(), x.data_ptr()
+    if not (q.shape == (rows, width) and scales.shape == (rows,) and width > 0 and (step := q.stride())[1] == 1 and step[0] >= width
+            and q.dtype is torch.int8 and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32)
+            and 0 <= device == q.get_device() == scales.get_device() == _current_device()):
         _check_rows_int8(q, scales, x, rows, width)
-    q_at, x_at = q.data_ptr(), x.data_ptr()
+        step = (width,) if rows <= 1 else q.stride()
     if q_at == x_at and rows:
         raise KernelError("the 8-bit rows have memory of their own: other rows are still read from what lies there")
-    call("nhv_rows_int8", _ROWS_CALL.pack(q_at, scales.data_ptr(), x_at, 0, 0, q.stride(0) if rows > 1 else width, x_stride, kind,
-                                          BF16 if x.dtype is torch.bfloat16 else F32, rows, width, 0, 0.0, 0.0), stream_ptr())
+    call("nhv_rows_int8", _ROWS_CALL.pack(q_at, scales.data_ptr(), x_at, 0, 0, step[0], x_stride, kind, BF16 if dtype is torch.bfloat16 else F32, rows,
+                                          width, 0, 0.0, 0.0), stream_ptr())
 
 
 def quantize_rows(q, scales, x) -> None:
@@ -1963,20 +1958,22 @@ def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual
     """``rmsnorm`` with its output in 8 bits: q [n, width] int8 and scales [n] as ``quantize_rows`` gives them for norm(x (+ residual)) *
     (weight + weight_offset), which is held in 32 bits and rounded once.  With a residual and write_residual the sum, rounded to x's
     type, replaces the residual."""
-    shape, dtype = x.shape, x.dtype
+    shape, dtype, device = x.shape, x.dtype, x.get_device()
     width = shape[-1] if shape else 0
     rows = x.numel() // width if width else 0
     x_at, residual_at, q_at = x.data_ptr(), 0 if residual is None else residual.data_ptr(), q.data_ptr()
-    if not (_int8_rows_quick(q, scales, x, rows, width) and x.is_contiguous() and weight.dtype is dtype and weight.shape == (width,)
-            and weight.is_contiguous() and weight.get_device() == x.get_device()
+    if not (q.shape == (rows, width) and scales.shape == (rows,) and (step := q.stride())[1] == 1 and step[0] >= width and q.dtype is torch.int8
+            and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32) and x.is_contiguous()
+            and weight.dtype is dtype and weight.shape == (width,) and weight.is_contiguous()
+            and 0 <= device == q.get_device() == scales.get_device() == weight.get_device() == _current_device()
             and (residual is None or (residual.shape == shape and residual.dtype is dtype and residual.is_contiguous() and residual_at != x_at
-                                      and residual.get_device() == x.get_device()))):
+                                      and residual.get_device() == device))):
         _check_rmsnorm_int8(q, scales, x, weight, residual, write_residual, rows, width)
+        step = (width,) if rows <= 1 else q.stride()
     if rows and (q_at == x_at or q_at == residual_at):
         raise KernelError("the 8-bit rows have memory of their own: other rows are still read from what lies there")
-    call("nhv_rows_int8", _ROWS_CALL.pack(
-        q_at, scales.data_ptr(), x_at, residual_at, weight.data_ptr(), q.stride(0) if rows > 1 else width, width, 1, BF16 if dtype is torch.bfloat16 else F32,
-        rows, width, write_residual and residual is not None, eps, weight_offset), stream_ptr())
+    call("nhv_rows_int8", _ROWS_CALL.pack(q_at, scales.data_ptr(), x_at, residual_at, weight.data_ptr(), step[0], width, 1, BF16 if dtype is torch.bfloat16 else F32,
+                                          rows, width, write_residual and residual is not None, eps, weight_offset), stream_ptr())
 
 
 def silu_mul_int8(q, scales, gate_up) -> None:
@@ -1995,20 +1992,21 @@ def dequantize_rows(out, q, scales) -> None:
     shape, step = out.shape, out.stride()
     if len(shape) != 2 or (step[1] != 1 and shape[1] > 1) or (step[0] < shape[1] and shape[0] > 1):
         raise KernelError(f"out is a matrix with neighbouring columns and rows that do not overlap, not {tuple(shape)} with strides {step}")
-    rows, width = shape
-    if not _int8_rows_quick(q, scales, out, rows, width):
-        if width:
-            _check_rows_int8(q, scales, out, rows, width)
-        else:
+    (rows, width), dtype, device, out_at, q_at = shape, out.dtype, out.get_device(), out.data_ptr(), q.data_ptr()
+    if not (q.shape == shape and scales.shape == (rows,) and (q_step := q.stride())[1] == 1 and q_step[0] >= width > 0 and q.dtype is torch.int8
+            and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32)
+            and 0 <= device == q.get_device() == scales.get_device() == _current_device()):
+        if width == 0:
             return
-    out_at, q_at = out.data_ptr(), q.data_ptr()
+        _check_rows_int8(q, scales, out, rows, width)
+        q_step = (width,) if rows <= 1 else q.stride()
     if out_at == q_at and rows:
         raise KernelError("the values have memory of their own: other rows are still read from what lies there")
-    call("nhv_rows_from_int8", _BACK_CALL.pack(out_at, q_at, scales.data_ptr(), step[0] if rows > 1 else width, q.stride(0) if rows > 1 else width,
-                                               BF16 if out.dtype is torch.bfloat16 else F32, rows, width), stream_ptr())
+    call("nhv_rows_from_int8", _BACK_CALL.pack(out_at, q_at, scales.data_ptr(), step[0] if rows > 1 else width, q_step[0],
+                                               BF16 if dtype is torch.bfloat16 else F32, rows, width), stream_ptr())
 
 
-_PRODUCT_CALL = struct.Struct("=10q5i4x")
+_PRODUCT_CALL = struct.Struct("=10q4i")
 
 
 def _check_linear_int8(out, x, x_scales, weight, weight_scales) -> None:
@@ -2034,30 +2032,30 @@ def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
     bfloat16 or float32.  The sums are exact (K up to 131,071), so an output does not depend on how the work is cut or batched.
     Rows of all three matrices may lie further apart.  Rows of x and weight that do not start at multiples of 16 bytes (those of
     ``new_int8`` do) are copied first, each call."""
-    shape, rows, dtype, device = x.shape, weight.shape, out.dtype, _current_device() if x.is_cuda else -1
-    T, K, N = (*shape, rows[0]) if len(shape) == len(rows) == 2 else (0, 0, 0)
-    x_step, w_step, out_step = x.stride(), weight.stride(), out.stride()
-    if not (T > 0 and N > 0 and 0 < K <= INT8_LONGEST_SUM and rows[1] == K and out.shape == (T, N) and x.dtype is torch.int8
-            and weight.dtype is torch.int8 and (dtype is torch.bfloat16 or dtype is torch.float32) and x_step[1] == w_step[1] == out_step[1] == 1
-            and x_step[0] >= K and w_step[0] >= K and out_step[0] >= N and x_scales.shape == (T,) and weight_scales.shape == (N,)
-            and x_scales.dtype is torch.float32 and weight_scales.dtype is torch.float32 and x_scales.is_contiguous() and weight_scales.is_contiguous()
-            and x.get_device() == weight.get_device() == out.get_device() == x_scales.get_device() == weight_scales.get_device() == device >= 0):
+    try:
+        (T, K), (N, k) = x.shape, weight.shape
+        (x_pitch, x_step), (w_pitch, w_step), (out_pitch, out_step) = x.stride(), weight.stride(), out.stride()
+    except ValueError:                                            # no matrices: the check says so
+        _check_linear_int8(out, x, x_scales, weight, weight_scales)
+    dtype, device, out_at, x_at, w_at = out.dtype, x.get_device(), out.data_ptr(), x.data_ptr(), weight.data_ptr()
+    x_copy = w_copy = None
+    if not (K == k and out.shape == (T, N) and x_scales.shape == (T,) and weight_scales.shape == (N,) and x.dtype is torch.int8 and weight.dtype is torch.int8
+            and (dtype is torch.bfloat16 or dtype is torch.float32) and x_scales.dtype is torch.float32 and weight_scales.dtype is torch.float32
+            and x_step == w_step == out_step == 1 and x_pitch >= K and w_pitch >= K and out_pitch >= N and T > 0 and N > 0 and 0 < K <= INT8_LONGEST_SUM
+            and not (x_at | w_at | x_pitch | w_pitch) % INT8_ROW_BYTES and x_scales.is_contiguous() and weight_scales.is_contiguous()
+            and 0 <= device == weight.get_device() == out.get_device() == x_scales.get_device() == weight_scales.get_device() == _current_device()):
         _check_linear_int8(out, x, x_scales, weight, weight_scales)
         if T == 0 or N == 0:
             return
-    pitch = -(-K // INT8_ROW_BYTES) * INT8_ROW_BYTES
-    x_at, w_at, out_at = x.data_ptr(), weight.data_ptr(), out.data_ptr()
-    if out_at == x_at or out_at == w_at:
-        raise KernelError("the output has memory of its own: the operands are read again for other outputs")
-    x_pitch, w_pitch = x_step[0] if T > 1 else pitch, w_step[0] if N > 1 else pitch      # a single row's stride may be anything
-    x_copy = w_copy = None
-    if (x_at | w_at | x_pitch | w_pitch) % INT8_ROW_BYTES:
+        pitch = -(-K // INT8_ROW_BYTES) * INT8_ROW_BYTES
+        x_pitch, w_pitch, out_pitch = x_pitch if T > 1 else pitch, w_pitch if N > 1 else pitch, out_pitch if T > 1 else N      # a single row's may be anything
         x_copy = torch.empty(T * pitch, dtype=torch.int8, device=x.device) if (x_at | x_pitch) % INT8_ROW_BYTES else None
         w_copy = torch.empty(N * pitch, dtype=torch.int8, device=x.device) if (w_at | w_pitch) % INT8_ROW_BYTES else None
+    if out_at == x_at or out_at == w_at:
+        raise KernelError("the output has memory of its own: the operands are read again for other outputs")
     call("nhv_gemm_int8", _PRODUCT_CALL.pack(
-        out_at, x_at, x_scales.data_ptr(), w_at, weight_scales.data_ptr(), x_copy.data_ptr() if x_copy is not None else 0,
-        w_copy.data_ptr() if w_copy is not None else 0, out_step[0] if T > 1 else N, x_pitch, w_pitch, BF16 if dtype is torch.bfloat16 else F32, T, N, K,
-        _sm_count(x.device)), stream_ptr())
+        out_at, x_at, x_scales.data_ptr(), w_at, weight_scales.data_ptr(), 0 if x_copy is None else x_copy.data_ptr(), 0 if w_copy is None else w_copy.data_ptr(),
+        out_pitch, x_pitch, w_pitch, BF16 if dtype is torch.bfloat16 else F32, T, N, K), stream_ptr())
 
 
 # ---------------------------------------------------------------- bounded waits that ran out

@@ -25,8 +25,7 @@ def test_a_wait_that_runs_out(starved, T, K, N):
     from nanohybrid_vlm_b200.kernels import ops
     x, w = ops.new_int8(T, K, "cuda").fill_(2), ops.new_int8(N, K, "cuda").fill_(3)
     xs, ws, y = torch.ones(T, device="cuda"), torch.ones(N, device="cuda"), torch.zeros(T, N, device="cuda")
-    sms = torch.cuda.get_device_properties(0).multi_processor_count
-    given = ops._PRODUCT_CALL.pack(y.data_ptr(), x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), 0, 0, N, K, K, ops.F32, T, N, K, sms)
+    given = ops._PRODUCT_CALL.pack(y.data_ptr(), x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), 0, 0, N, K, K, ops.F32, T, N, K)
     assert starved.nhv_gemm_int8(given, torch.cuda.current_stream().cuda_stream) == 0, starved.nhv_last_error()
     torch.cuda.synchronize()
     assert starved.nhv_gemm_int8_error() in (1, 2, 3, 4)      # the producer's, the issuer's or the epilogue's wait, whichever ran out last
