@@ -657,34 +657,42 @@ SplitSmem split_smem(const SplitPlan& plan) {
 }
 
 // Rows of a tile, parts of K and stages.  Times in us for 16 / 64 / 128 tokens.
-//   K in one part, a tile for each SM or, where that would be more than 96 rows, two: 12,288 x 4,096: 84 rows 11.3 / 12.2 / 13.6, 42 rows
-//   12.0 / 13.0 / 14.5; 24,576 x 4,096: 84 rows 18.8 / 19.2 / 22.1, 128 rows 19.9 / 20.5 / 23.4.
-//   Narrower weights: tiles of 128 rows, K over a cluster of blocks: 4,096 x 4,096 in 4 parts 5.8 / 7.8 / 9.4, in 1 with 28 rows 8.5 / 9.4 / 11.2.
-//   Up to 64 tokens two blocks share an SM (4,096 x 12,288 in 8 parts: 11.3 / 13.4, in 4: 11.8 / 14.4) unless a part would have fewer than 8
-//   stages (4,096 x 4,096 in 8 parts: 6.3 / 8.2); above, the room for the parts' sums leaves a second block no ring.  Clusters that
-//   would fill the SMs to the last do not all find their places at once (12,288 x 4,096 in 3 parts, 288 blocks: 15.1 / 19.6; 2,048 x 4,096 for
-//   128 tokens as 16 clusters of 8 13.4, as 32 of 4 with tiles of 64 rows 8.6).
+//   K in one part, a tile for each SM or, where that would be more than 96 rows, two: 12,288 x 4,096: 84 rows 11.2 / 11.6 / 13.6, 42 rows
+//   12.0 / 13.0 / 14.5; 24,576 x 4,096: 84 rows 18.8 / 19.1 / 22.0, 128 rows 19.9 / 20.5 / 23.4.  With a tile for each SM and more than 32 tokens the ring
+//   takes most of the SM (10,240 x 4,096 - / 10.3 / 11.7, with half of it - / 10.8 / 13.9); else, and for short sums, half, so that the next kernel's
+//   block finds room (9.8 against 10.1 with most; 10,240 x 1,024 4.5 / 5.2, with most - / 5.3).
+//   Narrower weights: tiles of 128 rows, K over a cluster of blocks: 4,096 x 4,096 in 4 parts 5.7 / 7.1 / 9.3, in 1 with 28 rows 8.5 / 9.4 / 11.2;
+//   10,240 x 4,096 in 3 9.6 / 12.2, 8,192 x 12,288 in 4 - / 21.6, in 1 - / 23.2, hence the bounds on N with more than 32 tokens.  Up to 64 tokens two
+//   blocks share an SM (4,096 x 12,288 in 8 parts 11.0 / 13.2, in 4 11.8 / 13.0) unless a part would have fewer than 8 stages (4,096 x 4,096
+//   in 8 parts: 6.3 / 8.2); above, the room for the parts' sums leaves a second block no ring.  A block alone on its SM has four stages at
+//   least (4,096 x 4,096 with three - / 7.7).  Clusters that would fill the SMs to the last do not all find their places at once
+//   (12,288 x 4,096 in 3 parts, 288 blocks: 15.1 / 19.6; 2,048 x 4,096 for 128 tokens as 16 clusters of 8 13.4, as 32 of 4 with tiles of 64 rows
+//   8.6).
 //   Short sums: K in one part, the tiles smaller: 4,096 x 1,024, 64 rows 3.6 / 4.1 / 5.1, 4 parts of 128 rows 3.6 / 5.3 / 8.8.
 SplitPlan split_plan(const Product& p, int sms) {
   const int kt = (p.K + BK - 1) / BK;
   SplitPlan plan;
   plan.nt = p.T >= 128 ? 128 : (p.T + 15) / 16 * 16;
-  const bool shared = plan.nt <= 64;
+  const bool shared = plan.nt <= 64, few = plan.nt <= 32;
   plan.rows = shared || p.N > 64 * (sms * 7 / 8 / 4) ? 128 : 64;
-  const int tiles = (p.N + plan.rows - 1) / plan.rows, most_parts = shared ? 8 : 4;
+  int tiles = (p.N + plan.rows - 1) / plan.rows;
+  const int most_parts = shared ? 8 : 4;
   plan.parts = (shared ? 2 * sms * 9 / 10 : sms * 7 / 8) / tiles;
   if (plan.parts > most_parts) plan.parts = most_parts;
   while (plan.parts > 1 && kt < 8 * plan.parts && tiles * plan.parts > sms) --plan.parts;
   if (plan.parts > kt) plan.parts = kt;
-  if (plan.parts < 3 || (kt < 16 && p.N >= 24 * sms)) {
+  if (plan.parts < (shared || kt < 32 ? 3 : 2) || (kt < 16 && p.N >= 24 * sms) || (!few && p.N >= (shared ? 60 : 48) * sms)) {
     plan.parts = 1;
     const long long slots = p.N > 96LL * sms ? 2 * sms : sms, waves = (p.N + 128LL * slots - 1) / (128LL * slots);
     plan.rows = (int)((p.N + waves * slots - 1) / (waves * slots));
     if (plan.rows < 32) plan.rows = p.N < 64 ? 64 : 32;
+    tiles = (p.N + plan.rows - 1) / plan.rows;
   }
-  const size_t most = (plan.parts == 1 || shared ? 112 : 200) * 1024;
+  const bool alone = !few && kt >= 16 && (long long)tiles * plan.parts <= sms;
+  const size_t most = ((plan.parts == 1 ? alone : !shared) ? 200 : 112) * 1024;
+  const int least = alone && plan.parts <= 4 ? 4 : 1;
   plan.stages = 8;
-  while (plan.stages > 1 && split_smem(plan).all > most) --plan.stages;
+  while (plan.stages > least && split_smem(plan).all > most) --plan.stages;
   return plan;
 }
 
