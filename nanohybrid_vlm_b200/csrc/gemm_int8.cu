@@ -7,7 +7,7 @@
 // (128-byte swizzle; what lies behind a matrix arrives as zeros, so no size needs padding):
 //   up to 128 tokens, where the weight's one read is the work: product_split_kernel, rows of the weight on the MMA's M axis;
 //   more, where the arithmetic is: product_pair_kernel, pairs of SMs on tiles of 256 tokens.
-// B200: 8 x 4,096 x 24,576 18 us (5.5 TB/s of weight; reading it alone takes 16.5), 64 x 12,288 x 4,096 13.4, 2,048 x 4,096 x 24,576 116 us in a prompt's step
+// B200: 8 x 4,096 x 24,576 18 us (5.5 TB/s of weight; reading it alone takes 16.5), 64 x 12,288 x 4,096 13.2, 2,048 x 4,096 x 24,576 116 us in a prompt's step
 // (3.55 POP/s; back to back for a while the power cap leaves 2.7 to 3.2).
 #include <string.h>
 
@@ -740,8 +740,8 @@ int launch_pair(Mapped& m, int sms, cudaStream_t stream) {
 }
 
 // The tiles' width: the one with the least turns * (width + 64), a turn being a tile for every pair, and 64 what a tile costs beside
-// its width.  us for widths 64 / 128 / 192 / 256: 256 tokens, 4,096 x 4,096 9.3 / 9.9 / - / 15.0; 256, 24,576 x 4,096 35.5 / 26.5 / 26.2 / 29.0; 512, 4,096 x 12,288
-// 32.4 / 23.1 / 31.0 / 36.0; 1,024, 4,096 x 12,288 - / 39.1 / 47.7 / 37.1; 2,048, 4,096 x 12,288 - / 90.7 / 84.2 / 75.4.
+// its width.  us for widths 64 / 128 / 192 / 256: 256 tokens, 4,096 x 4,096 9.3 / 9.9 / - / 15.0, 24,576 x 4,096 35.5 / 26.5 / 26.2 / 29.0; 4,096 x 12,288, 512
+// tokens 32.4 / 23.1 / 31.0 / 36.0, 1,024 - / 39.1 / 47.7 / 37.1, 2,048 - / 90.7 / 84.2 / 75.4.
 int pair_product(Mapped& m, int sms, cudaStream_t stream) {
   const long long tiles_t = (m.p.T + 255) / 256, pairs = sms / 2;
   long long least = 0;
