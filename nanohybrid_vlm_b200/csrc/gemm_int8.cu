@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS) product_split_kernel(const __gr
     }
     __syncwarp();
   } else if (warp == 1) {
+    pdl_wait();                                                    // the waits' limit counts from here, however long the kernel before takes
     const uint32_t idesc = instr_desc(128, m.nt);
     const int n = (int)same_in_all(k1 - k0);
     bool ok = true;
