@@ -34,7 +34,7 @@ struct Product {
   void* out;
   long long x_stride, w_stride, out_stride;
   int T, N, K, out_f32;
-  int boxes;             // rows of out start at multiples of 16 bytes
+  int boxes;             // rows of out start and end at multiples of 16 bytes
 };
 
 __device__ __forceinline__ float scaled(int sum, float xs, float ws) { return (float)sum * xs * ws; }
@@ -399,7 +399,8 @@ struct Pair {
 };
 
 // A warp's 32 outputs of 32 rows from (t0, n0): 64 bytes of each row at a time through 2 KB of shared memory in the 64-byte swizzle, from where
-// a TMA store takes them while the warp goes on; what lies behind out's rows and columns is not written.
+// a TMA store takes them while the warp goes on; what lies behind out's rows and columns is not written.  A row ends at a multiple of 16 bytes
+// (Product::boxes): a store writes whole 16 bytes, with zeros behind the last column.
 __device__ __forceinline__ void store_box(const CUtensorMap* map, unsigned char* box, const uint32_t (&w)[16], int n, int t, int lane) {
   if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");      // the last one has read the box
   __syncwarp();
@@ -432,7 +433,7 @@ __device__ __forceinline__ void store_rows32(const CUtensorMap* map, unsigned ch
     store_box(map, box, w, n0, t0, lane);
   }
 }
-// The same where rows start at odd places: 16 columns of two rows at a time, lanes side by side.
+// The same where rows start or end at odd places: 16 columns of two rows at a time, lanes side by side.
 template <typename O>
 __device__ __forceinline__ void store_turned(O* out, const Product& p, float* mine, const float (&v)[32], int t0, int n0, int lane) {
 #pragma unroll
@@ -792,9 +793,10 @@ NHV_API int nhv_gemm_int8(const void* given, cudaStream_t stream) {
   NHV_REQUIRE(T > 0 && N > 0 && K > 0 && K <= 131071, "linear_int8: a sum over 1 to 131,071 products is exact in 32 bits, not over %d", K);
   NHV_REQUIRE(c.out && c.x && c.w && c.x_scales && c.w_scales && (c.out_dtype == NHV_F32 || c.out_dtype == NHV_BF16), "linear_int8: bad arguments");
   NHV_REQUIRE(sms > 1, "linear_int8: the device does not say how many SMs it has");
+  const long long item = c.out_dtype == NHV_F32 ? 4 : 2;
   Product p = {(const int8_t*)c.x, (const int8_t*)c.w, (const float*)c.x_scales, (const float*)c.w_scales, (void*)c.out,
                      c.x_stride, c.w_stride, c.out_stride, T, N, K, c.out_dtype == NHV_F32,
-                     (c.out | c.out_stride * (c.out_dtype == NHV_F32 ? 4 : 2)) % 16 == 0};
+                     (c.out | c.out_stride * item | N * item) % 16 == 0};
   if (int e = align_rows(&p.x, &p.x_stride, (void*)c.x_copy, T, K, stream)) return e;
   if (int e = align_rows(&p.w, &p.w_stride, (void*)c.w_copy, N, K, stream)) return e;
   // us, whole tiles of the weight / pairs: 128 tokens, 4,096 x 4,096 9.4 / 9.3, 24,576 x 4,096 22.1 / 26.2, 4,096 x 12,288 14.9 / 18.6; 256 tokens 12.7 / 9.3,

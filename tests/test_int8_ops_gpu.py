@@ -82,6 +82,13 @@ def test_products_into_wider_rows(ops, T, K, N, out, pad):
     check_product(ops, T, K, N, out, out_pad=pad)
 
 
+@pytest.mark.parametrize("T", [64, 366, 1025])
+@pytest.mark.parametrize("N,out,pad", [(55, BF, 1), (129, BF, 7), (300, BF, 4), (53, F, 3), (129, F, 7), (302, F, 2)])
+def test_products_whose_rows_end_inside_16_bytes(ops, T, N, out, pad):
+    """The rows start at multiples of 16 bytes and end between two: the rest of the last 16 bytes is not the output's."""
+    check_product(ops, T, 144, N, out, out_pad=pad, seed=N)
+
+
 @pytest.mark.parametrize("T", [1, 12, 40, 200, 1300])
 def test_sums_at_the_ends_of_32_bits(ops, T):
     """All products at the largest magnitude, -128 among them: K * 2^14 is just below 2^31."""
