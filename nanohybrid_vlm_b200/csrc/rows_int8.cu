@@ -70,7 +70,8 @@ __device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t 
 
 template <typename T> __device__ __forceinline__ float silu_times(float g, float u);
 template <> __device__ __forceinline__ float silu_times<float>(float g, float u) { return g / (1.0f + expf(-g)) * u; }
-// Rows in 16 bits: the fast exponential and division, about 2 ulp of 32 bits, next to inputs of 8 bits.
+// Rows in 16 bits: the fast exponential and division, about 2 ulp of 32 bits, next to inputs of 8 bits.  Gates below -87, where silu is
+// less than 2^-118, give 0, as in the product of units that stays in 16 bits.
 template <> __device__ __forceinline__ float silu_times<bf16>(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 // The block's sum and the block's largest magnitude (as the bits of a float that is not negative: their order is that of the

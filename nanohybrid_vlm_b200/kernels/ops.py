@@ -1957,7 +1957,7 @@ def _check_rmsnorm_int8(q, scales, x, weight, residual, write_residual: bool, ro
 def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual: bool = True, weight_offset: float = 0.0) -> None:
     """``rmsnorm`` with its output in 8 bits: q [n, width] int8 and scales [n] as ``quantize_rows`` gives them for norm(x (+ residual)) *
     (weight + weight_offset), which is held in 32 bits and rounded once.  With a residual and write_residual the sum, rounded to x's
-    type, replaces the residual."""
+    type, replaces the residual.  Widths up to 51,200."""
     shape, dtype, device = x.shape, x.dtype, x.get_device()
     width = shape[-1] if shape else 0
     rows = x.numel() // width if width else 0
