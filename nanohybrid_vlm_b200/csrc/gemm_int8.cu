@@ -9,6 +9,7 @@
 //   more, where the arithmetic is: product_pair_kernel, pairs of SMs on tiles of 256 tokens.
 // B200: 8 x 4,096 x 24,576 18 us (5.5 TB/s of weight; reading it alone takes 16.5), 64 x 12,288 x 4,096 13.2, 2,048 x 4,096 x 24,576 116 us in a prompt's step
 // (3.55 POP/s; back to back for a while the power cap leaves 2.7 to 3.2).
+#include <limits.h>
 #include <string.h>
 
 #ifndef NHV_WAIT_LIMIT
@@ -791,6 +792,7 @@ NHV_API int nhv_gemm_int8(const void* given, cudaStream_t stream) {
   const int T = c.T, N = c.N, K = c.K, sms = sm_count();
   if (T == 0 || N == 0) return 0;
   NHV_REQUIRE(T > 0 && N > 0 && K > 0 && K <= 131071, "linear_int8: a sum over 1 to 131,071 products is exact in 32 bits, not over %d", K);
+  NHV_REQUIRE(T <= INT_MAX - 511 && N <= INT_MAX - 511, "linear_int8: %d tokens and %d outputs: a tile's last row has no number in 32 bits", T, N);
   NHV_REQUIRE(c.out && c.x && c.w && c.x_scales && c.w_scales && (c.out_dtype == NHV_F32 || c.out_dtype == NHV_BF16), "linear_int8: bad arguments");
   NHV_REQUIRE(sms > 1, "linear_int8: the device does not say how many SMs it has");
   const long long item = c.out_dtype == NHV_F32 ? 4 : 2;

@@ -167,6 +167,34 @@ def test_streams_and_graphs(ops, T):
     assert ops.take_wait_errors() == []
 
 
+def far_apart(rows, width, stride, dtype):
+    """Rows whose last ones start more than 2^31 elements behind the first; most of the memory is never touched."""
+    assert (rows - 1) * stride > 2 ** 31
+    return torch.empty((rows - 1) * stride + width, dtype=dtype, device="cuda").as_strided((rows, width), (stride, 1))
+
+
+@pytest.mark.parametrize("T,odd", [(20, 0), (20, 1), (300, 0), (300, 1)])
+def test_product_offsets_beyond_32_bits(ops, T, odd):
+    """Rows of both operands and of the output lie far apart; with ``odd`` at places from which the operands are copied first."""
+    g = gen(T)
+    K, N, xp, wp = 80, 300, 2 ** 31 // (T - 2) // 16 * 16 + 64 + odd, 2 ** 31 // 298 // 16 * 16 + 64 + odd
+    x, w = far_apart(T, K, xp, torch.int8), far_apart(N, K, wp, torch.int8)
+    x.copy_(ints(g, T, K)), w.copy_(ints(g, N, K))
+    xs, ws = torch.rand(T, generator=g, device="cuda"), torch.rand(N, generator=g, device="cuda")
+    y = far_apart(T, N, xp, BF)
+    ops.linear_int8(y, x, xs, w, ws)
+    want = (x.double() @ w.double().t()) * xs.double()[:, None] * ws.double()[None]
+    assert ((y.double() - want).abs() <= (EIGHT[BF] + 3.1 * 2.0 ** -24) * want.abs()).all()
+
+
+def test_products_beyond_the_numbers_of_tiles_are_refused(ops):
+    """Sizes whose last tile has rows without a number in 32 bits; the call's own block says so, as no memory is that large."""
+    from nanohybrid_vlm_b200.kernels.library import KernelError, call
+    for T, N in ((2 ** 31 - 511, 1), (1, 2 ** 31 - 511)):
+        with pytest.raises(KernelError, match="no number"):
+            call("nhv_gemm_int8", ops._PRODUCT_CALL.pack(*[0] * 7, 1, 16, 16, 1, T, N, 16), ops.stream_ptr())
+
+
 # ------------------------------------------------------------------------------------------------ rows
 def definition(y):
     a = y.abs().amax(1)
@@ -226,6 +254,23 @@ def test_plain_rows_ties_and_ends_of_the_range(ops):
     x = torch.tensor([[3.3e38, -3.3e38, 1.0, 1.65e38]], device="cuda")
     ops.quantize_rows(q, s, x)
     assert q.tolist() == [[127, -127, 0, 64]] and torch.isfinite(s).all()
+
+
+@pytest.mark.parametrize("odd", [0, 1])
+def test_row_offsets_beyond_32_bits(ops, odd):
+    g = gen(7)
+    n, width, stride = 300, 1024, 2 ** 31 // 298 // 16 * 16 + 64 + odd
+    x, q, y = far_apart(n, width, stride, BF), far_apart(n, width, stride, torch.int8), far_apart(n, width, stride, BF)
+    x.copy_(torch.randn(n, width, generator=g, device="cuda"))
+    s = torch.empty(n, device="cuda")
+    ops.quantize_rows(q, s, x)
+    check_rows(q, s, x.double(), 0.0, exact=True)
+    ops.dequantize_rows(y, q, s)
+    assert torch.equal(y, (q.float() * s[:, None]).to(BF))
+    near = torch.randn(n, width, generator=g, device="cuda").to(BF)
+    ops.rmsnorm_int8(q, s, near, torch.ones(width, dtype=BF, device="cuda"), 1e-5)
+    y64 = near.double()
+    check_rows(q, s, y64 / torch.sqrt(y64.pow(2).mean(1, keepdim=True) + 1e-5), OFF_NORM)
 
 
 @pytest.mark.parametrize("width", [5, 264, 4096, 40000])
