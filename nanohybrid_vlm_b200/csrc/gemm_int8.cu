@@ -16,6 +16,7 @@
 #define NHV_WAIT_LIMIT (1u << 22)
 #endif
 #include "nhv_async.cuh"
+#include "nhv_overlap.h"
 
 // Test builds only (tests compile this file into a library of its own with a short NHV_WAIT_LIMIT): the producers leave stage
 // NHV_TEST_DROP_UNIT unsent, so that the waits for it run out.
@@ -794,8 +795,12 @@ NHV_API int nhv_gemm_int8(const void* given, cudaStream_t stream) {
   NHV_REQUIRE(T > 0 && N > 0 && K > 0 && K <= 131071, "linear_int8: a sum over 1 to 131,071 products is exact in 32 bits, not over %d", K);
   NHV_REQUIRE(T <= INT_MAX - 511 && N <= INT_MAX - 511, "linear_int8: %d tokens and %d outputs: a tile's last row has no number in 32 bits", T, N);
   NHV_REQUIRE(c.out && c.x && c.w && c.x_scales && c.w_scales && (c.out_dtype == NHV_F32 || c.out_dtype == NHV_BF16), "linear_int8: bad arguments");
-  NHV_REQUIRE(sms > 1, "linear_int8: the device does not say how many SMs it has");
   const long long item = c.out_dtype == NHV_F32 ? 4 : 2;
+  const NhvRows out = {c.out, T, c.out_stride * item, N * item};
+  NHV_REQUIRE(!nhv_rows_meet(out, {c.x, T, c.x_stride, K}) && !nhv_rows_meet(out, {c.w, N, c.w_stride, K}) &&
+              !nhv_rows_meet(out, {c.x_scales, 1, 0, 4LL * T}) && !nhv_rows_meet(out, {c.w_scales, 1, 0, 4LL * N}),
+              "the output has memory of its own: operands and scales are read again for other outputs");
+  NHV_REQUIRE(sms > 1, "linear_int8: the device does not say how many SMs it has");
   Product p = {(const int8_t*)c.x, (const int8_t*)c.w, (const float*)c.x_scales, (const float*)c.w_scales, (void*)c.out,
                      c.x_stride, c.w_stride, c.out_stride, T, N, K, c.out_dtype == NHV_F32,
                      (c.out | c.out_stride * item | N * item) % 16 == 0};

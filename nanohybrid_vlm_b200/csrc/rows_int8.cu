@@ -15,6 +15,7 @@
 // arithmetic went by pairs), hence pairs of floats, maxima of three and integers in the low bits of floats.
 #include <string.h>
 
+#include "nhv_overlap.h"
 #include "nhv_vec8.cuh"
 
 namespace {
@@ -531,6 +532,17 @@ NHV_API int nhv_rows_int8(const void* given, cudaStream_t stream) {
   NHV_REQUIRE(c.n_rows > 0 && c.width > 0 && c.width <= (1 << 30) && c.q && c.scales && c.x, "rows_int8: bad sizes");
   NHV_REQUIRE(c.kind >= ROW_PLAIN && c.kind <= ROW_UNIT && (c.kind != ROW_NORM || c.weight), "rows_int8: bad arguments");
   NHV_REQUIRE(c.dtype == NHV_F32 || c.dtype == NHV_BF16, "rows_int8: unknown dtype %d", c.dtype);
+  // A block reads its row while others write theirs: what is written shares no byte with anything else of the call.
+  const long long item = c.dtype == NHV_F32 ? 4 : 2, n = c.n_rows, w = c.width;
+  const NhvRows q = {c.q, n, c.q_stride, w}, scales = {c.scales, 1, 0, n * 4};
+  const NhvRows x = {c.x, n, c.x_stride * item, w * item * (c.kind == ROW_UNIT ? 2 : 1)};
+  const NhvRows weight = {c.weight, c.kind == ROW_NORM, 0, w * item}, residual = {c.residual, c.kind == ROW_NORM && c.residual, 0, n * w * item};
+  NHV_REQUIRE(!nhv_rows_meet(q, x) && !nhv_rows_meet(q, residual) && !nhv_rows_meet(q, weight) && !nhv_rows_meet(q, scales),
+              "the 8-bit rows have memory of their own: other rows are still read from what lies there");
+  NHV_REQUIRE(!nhv_rows_meet(scales, x) && !nhv_rows_meet(scales, residual) && !nhv_rows_meet(scales, weight),
+              "the scales have memory of their own: other rows are still read from what lies there");
+  NHV_REQUIRE(!c.write_residual || (!nhv_rows_meet(residual, x) && !nhv_rows_meet(residual, weight)),
+              "the residual has memory of its own: its sum with x is written there");
   const Args p = {(int8_t*)c.q, (float*)c.scales, (const void*)c.x, (void*)c.residual, (const void*)c.weight, c.q_stride, c.x_stride, c.width,
                   c.eps, c.weight_offset, c.write_residual};
   return c.dtype == NHV_F32 ? launch_kind<float>(c.kind, p, c.n_rows, stream) : launch_kind<bf16>(c.kind, p, c.n_rows, stream);
@@ -547,6 +559,9 @@ NHV_API int nhv_rows_from_int8(const void* given, cudaStream_t stream) {
   memcpy(&c, given, sizeof(c));
   if (c.n_rows == 0 || c.width == 0) return 0;
   NHV_REQUIRE(c.n_rows > 0 && c.width > 0 && c.out && c.q && c.scales && (c.dtype == NHV_F32 || c.dtype == NHV_BF16), "dequantize_rows: bad arguments");
+  const NhvRows out = {c.out, c.n_rows, c.out_stride * (c.dtype == NHV_F32 ? 4 : 2), (long long)c.width * (c.dtype == NHV_F32 ? 4 : 2)};
+  NHV_REQUIRE(!nhv_rows_meet(out, {c.q, c.n_rows, c.q_stride, c.width}) && !nhv_rows_meet(out, {c.scales, 1, 0, 4LL * c.n_rows}),
+              "the values have memory of their own: other rows are still read from what lies there");
   const BackArgs p = {(const int8_t*)c.q, (const float*)c.scales, (void*)c.out, c.q_stride, c.out_stride, c.n_rows, c.width};
   return c.dtype == NHV_F32 ? launch_back<float>(p, stream) : launch_back<bf16>(p, stream);
 }

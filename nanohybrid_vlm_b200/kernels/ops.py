@@ -1864,7 +1864,8 @@ def linear_simt(out, x, weight) -> None:
 
 
 # ---------------------------------------------------------------- 8-bit integers
-# Rows of 8-bit integers with a float32 scale each (integer times scale is the value), and their products.
+# Rows of 8-bit integers with a float32 scale each (integer times scale is the value), and their products.  Whether what a call
+# writes shares memory with what it reads is looked at by the library, row by row: columns of one buffer side by side do not.
 INT8_LONGEST_SUM = 131071
 INT8_ROW_BYTES = 16     # rows made here start at multiples of this, which the fast products read 16 bytes at a time
 
@@ -1919,15 +1920,13 @@ def _check_rows_int8(q, scales, x, rows: int, width: int, *others) -> None:
 
 
 def _rows_int8(kind: int, q, scales, x, rows: int, width: int, x_stride: int) -> None:
-    dtype, device, q_at, x_at = x.dtype, x.get_device(), q.data_ptr(), x.data_ptr()
+    dtype, device = x.dtype, x.get_device()
     if not (q.shape == (rows, width) and scales.shape == (rows,) and width > 0 and (step := q.stride())[1] == 1 and step[0] >= width
             and q.dtype is torch.int8 and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32)
             and 0 <= device == q.get_device() == scales.get_device() == _current_device()):
         _check_rows_int8(q, scales, x, rows, width)
         step = (width,) if rows <= 1 else q.stride()
-    if q_at == x_at and rows:
-        raise KernelError("the 8-bit rows have memory of their own: other rows are still read from what lies there")
-    call("nhv_rows_int8", _ROWS_CALL.pack(q_at, scales.data_ptr(), x_at, 0, 0, step[0], x_stride, kind, BF16 if dtype is torch.bfloat16 else F32, rows,
+    call("nhv_rows_int8", _ROWS_CALL.pack(q.data_ptr(), scales.data_ptr(), x.data_ptr(), 0, 0, step[0], x_stride, kind, BF16 if dtype is torch.bfloat16 else F32, rows,
                                           width, 0, 0.0, 0.0), stream_ptr())
 
 
@@ -1961,7 +1960,7 @@ def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual
     shape, dtype, device = x.shape, x.dtype, x.get_device()
     width = shape[-1] if shape else 0
     rows = x.numel() // width if width else 0
-    x_at, residual_at, q_at = x.data_ptr(), 0 if residual is None else residual.data_ptr(), q.data_ptr()
+    x_at, residual_at = x.data_ptr(), 0 if residual is None else residual.data_ptr()
     if not (q.shape == (rows, width) and scales.shape == (rows,) and (step := q.stride())[1] == 1 and step[0] >= width and q.dtype is torch.int8
             and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32) and x.is_contiguous()
             and weight.dtype is dtype and weight.shape == (width,) and weight.is_contiguous()
@@ -1970,9 +1969,7 @@ def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual
                                       and residual.get_device() == device))):
         _check_rmsnorm_int8(q, scales, x, weight, residual, write_residual, rows, width)
         step = (width,) if rows <= 1 else q.stride()
-    if rows and (q_at == x_at or q_at == residual_at):
-        raise KernelError("the 8-bit rows have memory of their own: other rows are still read from what lies there")
-    call("nhv_rows_int8", _ROWS_CALL.pack(q_at, scales.data_ptr(), x_at, residual_at, weight.data_ptr(), step[0], width, 1, BF16 if dtype is torch.bfloat16 else F32,
+    call("nhv_rows_int8", _ROWS_CALL.pack(q.data_ptr(), scales.data_ptr(), x_at, residual_at, weight.data_ptr(), step[0], width, 1, BF16 if dtype is torch.bfloat16 else F32,
                                           rows, width, write_residual and residual is not None, eps, weight_offset), stream_ptr())
 
 
@@ -1992,7 +1989,7 @@ def dequantize_rows(out, q, scales) -> None:
     shape, step = out.shape, out.stride()
     if len(shape) != 2 or (step[1] != 1 and shape[1] > 1) or (step[0] < shape[1] and shape[0] > 1):
         raise KernelError(f"out is a matrix with neighbouring columns and rows that do not overlap, not {tuple(shape)} with strides {step}")
-    (rows, width), dtype, device, out_at, q_at = shape, out.dtype, out.get_device(), out.data_ptr(), q.data_ptr()
+    (rows, width), dtype, device = shape, out.dtype, out.get_device()
     if not (q.shape == shape and scales.shape == (rows,) and (q_step := q.stride())[1] == 1 and q_step[0] >= width > 0 and q.dtype is torch.int8
             and scales.dtype is torch.float32 and scales.is_contiguous() and (dtype is torch.bfloat16 or dtype is torch.float32)
             and 0 <= device == q.get_device() == scales.get_device() == _current_device()):
@@ -2000,9 +1997,7 @@ def dequantize_rows(out, q, scales) -> None:
             return
         _check_rows_int8(q, scales, out, rows, width)
         q_step = (width,) if rows <= 1 else q.stride()
-    if out_at == q_at and rows:
-        raise KernelError("the values have memory of their own: other rows are still read from what lies there")
-    call("nhv_rows_from_int8", _BACK_CALL.pack(out_at, q_at, scales.data_ptr(), step[0] if rows > 1 else width, q_step[0],
+    call("nhv_rows_from_int8", _BACK_CALL.pack(out.data_ptr(), q.data_ptr(), scales.data_ptr(), step[0] if rows > 1 else width, q_step[0],
                                                BF16 if dtype is torch.bfloat16 else F32, rows, width), stream_ptr())
 
 
@@ -2037,7 +2032,7 @@ def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
         (x_pitch, x_step), (w_pitch, w_step), (out_pitch, out_step) = x.stride(), weight.stride(), out.stride()
     except ValueError:                                            # no matrices: the check says so
         _check_linear_int8(out, x, x_scales, weight, weight_scales)
-    dtype, device, out_at, x_at, w_at = out.dtype, x.get_device(), out.data_ptr(), x.data_ptr(), weight.data_ptr()
+    dtype, device, x_at, w_at = out.dtype, x.get_device(), x.data_ptr(), weight.data_ptr()
     x_copy = w_copy = None
     if not (K == k and out.shape == (T, N) and x_scales.shape == (T,) and weight_scales.shape == (N,) and x.dtype is torch.int8 and weight.dtype is torch.int8
             and (dtype is torch.bfloat16 or dtype is torch.float32) and x_scales.dtype is torch.float32 and weight_scales.dtype is torch.float32
@@ -2051,10 +2046,8 @@ def linear_int8(out, x, x_scales, weight, weight_scales) -> None:
         x_pitch, w_pitch, out_pitch = x_pitch if T > 1 else pitch, w_pitch if N > 1 else pitch, out_pitch if T > 1 else N      # a single row's may be anything
         x_copy = torch.empty(T * pitch, dtype=torch.int8, device=x.device) if (x_at | x_pitch) % INT8_ROW_BYTES else None
         w_copy = torch.empty(N * pitch, dtype=torch.int8, device=x.device) if (w_at | w_pitch) % INT8_ROW_BYTES else None
-    if out_at == x_at or out_at == w_at:
-        raise KernelError("the output has memory of its own: the operands are read again for other outputs")
     call("nhv_gemm_int8", _PRODUCT_CALL.pack(
-        out_at, x_at, x_scales.data_ptr(), w_at, weight_scales.data_ptr(), 0 if x_copy is None else x_copy.data_ptr(), 0 if w_copy is None else w_copy.data_ptr(),
+        out.data_ptr(), x_at, x_scales.data_ptr(), w_at, weight_scales.data_ptr(), 0 if x_copy is None else x_copy.data_ptr(), 0 if w_copy is None else w_copy.data_ptr(),
         out_pitch, x_pitch, w_pitch, BF16 if dtype is torch.bfloat16 else F32, T, N, K), stream_ptr())
 
 
