@@ -498,7 +498,8 @@ __global__ void __launch_bounds__(256) values_kernel(const BackArgs p) {
   pdl_prologue();
   for (long long r = blockIdx.x; r < p.n_rows; r += gridDim.x) {
     const float s = p.scales[r];
-    for (int c = threadIdx.x; c < p.width; c += 256) reinterpret_cast<T*>(p.out)[r * p.out_stride + c] = from_f32<T>((float)p.q[r * p.q_stride + c] * s);
+    for (unsigned c = threadIdx.x; c < (unsigned)p.width; c += 256)          // up to 2^31 - 1 columns: the last turn's end has no number in an int
+      reinterpret_cast<T*>(p.out)[r * p.out_stride + c] = from_f32<T>((float)p.q[r * p.q_stride + c] * s);
   }
 }
 

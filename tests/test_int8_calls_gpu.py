@@ -61,3 +61,17 @@ def test_columns_of_one_buffer(ops, T):
     assert torch.equal(x, was) and torch.equal(back, (q.float() * s[:, None]).to(BF))
     want = (q.double() @ w.double().t()) * s.double()[:, None] * ws.double()[None]
     assert ((y.double() - want).abs() <= 3.1 * 2.0 ** -24 * want.abs()).all()
+
+
+# ------------------------------------------------------------------------------------------------ the longest rows
+@pytest.mark.parametrize("width", [2 ** 31 - 1, 2 ** 31 - 16])
+def test_values_of_the_longest_rows(ops, width):
+    """One row of as many columns as 32 bits count: nothing before or behind it is touched."""
+    q = torch.empty(1, width, dtype=torch.int8, device="cuda")
+    q.random_(-127, 128, generator=gen(width % 97))
+    whole = torch.full((width + 512,), 3.0, dtype=BF, device="cuda")
+    s = torch.tensor([0.37], device="cuda")
+    ops.dequantize_rows(whole[256:256 + width][None], q, s)
+    for i in range(0, width, 2 ** 28):
+        assert torch.equal(whole[256 + i:256 + min(i + 2 ** 28, width)], (q[0, i:i + 2 ** 28].float() * s).to(BF))
+    assert (whole[:256] == 3).all() and (whole[256 + width:] == 3).all()
