@@ -46,7 +46,8 @@ class Config:
     cache_first: int = 4                     # with cache_budget: the keys of the first positions stay whatever they gathered
     cache_recent: int = -1                   # with cache_budget: and those of the last positions (-1: a quarter of the budget)
     quantization: str | None = None          # "int8": the layers' matrices as 8-bit integers with a scale per output channel, what they
-                                             # multiply rounded to 8 bits with a scale per token (half the weights' bytes)
+                                             # multiply rounded to 8 bits with a scale per token (half the weights' bytes,
+                                             # once they are loaded)
     poison_cache: bool = False               # fill the cache pools with NaN at start: a read of a slot that no step
                                              # wrote shows in the logits (tests, replay)
     dtype: str | torch.dtype | None = None   # None: the checkpoint's own

@@ -11,6 +11,7 @@ from dataclasses import dataclass, replace
 
 import torch
 
+from ..kernels import ops
 from .. import parts as _registered_parts  # noqa: F401  (importing the package registers the built-in parts)
 from ..parts.base import (BLOCKS, EMBEDDINGS, HEADS, NORMS, BuildEnv, FixedStateNeed, Int8Rows, PagedKVNeed, Part, need_leaves,
                           with_shared_pages)
@@ -87,11 +88,20 @@ class CausalLM:
             self.head.tie(self.embedding)
         self.tensors = tensors
 
+    def int8_parts(self) -> list[Part]:
+        """The parts that ``to_int8`` changes.  Raises ``ValueError`` where a layer has no such form; needs no tensors and changes nothing."""
+        parts = list({id(p): p for block in self.blocks for p in block.int8_parts()}.values())
+        for part in parts:
+            for decl in part.params():
+                if decl.name in part.int8_weights() and decl.shape[1] > ops.INT8_LONGEST_SUM:
+                    raise ValueError(f"{part.spec.kind!r} has no form in 8-bit integers for {decl.shape[1]} inputs: their sum does not fit 32 bits")
+        return parts
+
     def to_int8(self) -> None:
         """Hold the matrices of all layers as 8-bit integers with a scale per output channel, and multiply by them so; embedding, head and
-        norms stay as they are.  Raises ``ValueError`` where a layer has no such form."""
+        norms stay as they are.  Raises ``ValueError`` where a layer has no such form (``int8_parts``), and has changed nothing then."""
         names = {(id(bp.owner), bp.local): bp.name for bp in self.param_table()}
-        for part in {id(p): p for block in self.blocks for p in block.int8_parts()}.values():
+        for part in self.int8_parts():
             for local, rows in part.to_int8().items():
                 self.tensors[names[id(part), local]] = rows
 

@@ -51,6 +51,8 @@ class ModelRunner:
             spec = replace(spec, max_position=config.max_model_len)
         self.model = CausalLM(spec, self.dtype, self.device)
         self.model.profile_ranges = bool(config.profile_ranges)
+        if config.quantization is not None:
+            self.model.int8_parts()      # a model without such a form is refused before its weights are read
         if random_weights_seed is None:
             load_weights(self.model, config.model)
         else:

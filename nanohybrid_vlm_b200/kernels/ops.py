@@ -1867,6 +1867,7 @@ def linear_simt(out, x, weight) -> None:
 # Rows of 8-bit integers with a float32 scale each (integer times scale is the value), and their products.  Whether what a call
 # writes shares memory with what it reads is looked at by the library, row by row: columns of one buffer side by side do not.
 INT8_LONGEST_SUM = 131071
+INT8_WIDEST_NORM = 51200
 INT8_ROW_BYTES = 16     # rows made here start at multiples of this, which the fast products read 16 bytes at a time
 
 

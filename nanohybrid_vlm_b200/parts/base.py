@@ -189,7 +189,8 @@ class Part:
         return ()
 
     def to_int8(self) -> dict[str, Int8Rows]:
-        """Round those matrices to 8-bit integers with a scale per output channel, in their places; the part lets go of the originals."""
+        """Round those matrices to 8-bit integers with a scale per output channel, in their places; the part lets go of the originals.
+        A norm rounds what it gives from then on, and returns nothing."""
         made = {}
         for name in self.int8_weights():
             at = "w_" + name.replace(".", "_")
@@ -280,6 +281,8 @@ class FeedForward(Part):
 
 
 class Norm(Part):
+    gives_int8 = False      # whether ``to_int8`` makes it give :class:`Int8Rows`
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         raise NotImplementedError
 
@@ -374,8 +377,8 @@ class Block:
             setattr(self, name, obj)
 
     def int8_parts(self) -> tuple[Part, ...]:
-        """For an engine that multiplies in 8-bit integers: the parts whose matrices are rounded to them, after the block has told its
-        norms to round what those parts read.  Default: the block cannot."""
+        """For an engine that multiplies in 8-bit integers: the parts that ``to_int8`` is for, those whose matrices are rounded and the norms
+        in front of them.  Looks only, so that it may be asked before any tensor is there.  Default: the block cannot."""
         raise ValueError(f"block {self.spec.kind!r} has no form in 8-bit integers")
 
     @property

@@ -20,10 +20,9 @@ class PreNormResidualBlock(Block):
             if not self.parts[name].int8_weights():
                 raise ValueError(f"{self.parts[name].spec.kind!r} has no form in 8-bit integers")
         for name in ("mixer_norm", "ffn_norm"):
-            if not hasattr(self.parts[name], "give_int8"):
-                raise ValueError(f"norm {self.parts[name].spec.kind!r} gives no 8-bit integers")
-            self.parts[name].give_int8()
-        return self.parts["mixer"], self.parts["ffn"]
+            if not self.parts[name].gives_int8:
+                raise ValueError(f"norm {self.parts[name].spec.kind!r} gives no 8-bit integers as it is set up here")
+        return tuple(self.parts[name] for name in ("mixer_norm", "mixer", "ffn_norm", "ffn"))
 
     def forward(self, hidden, residual, batch, cache):
         if residual is None:

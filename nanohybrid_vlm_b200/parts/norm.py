@@ -85,12 +85,16 @@ class RMSNorm(Norm):
         new = streams if streams.shape[1] == S else self.new(streams.shape[0], S, self.width, dtype=torch.float32)
         return self._streams(x, streams, S, connection.read, new, None), new
 
-    def give_int8(self) -> None:
-        """From here on ``forward`` and ``forward_add`` over tensors return :class:`Int8Rows`."""
-        self._plain_only()
-        self.int8 = True
-
     int8 = False
+
+    @property
+    def gives_int8(self):
+        return self.groups == 1 and self.post_scale is None and self.width <= ops.INT8_WIDEST_NORM
+
+    def to_int8(self):
+        """From here on ``forward`` and ``forward_add`` over tensors return :class:`Int8Rows`."""
+        self.int8 = True
+        return {}
 
     def _to_int8(self, x, residual=None):
         out = Int8Rows.room(x.shape[0], self.width, x.device)
