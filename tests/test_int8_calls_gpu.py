@@ -75,3 +75,44 @@ def test_values_of_the_longest_rows(ops, width):
     for i in range(0, width, 2 ** 28):
         assert torch.equal(whole[256 + i:256 + min(i + 2 ** 28, width)], (q[0, i:i + 2 ** 28].float() * s).to(BF))
     assert (whole[:256] == 3).all() and (whole[256 + width:] == 3).all()
+
+
+# ------------------------------------------------------------------------------------------------ gates far from zero
+LARGEST = torch.finfo(BF).max
+
+
+@pytest.mark.parametrize("width", [264, 1031, 32776, 60001])         # pieces in registers, any width, shared memory, read again
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_gates_far_from_zero(ops, width, dtype):
+    """A row for each gate.  In 16 bits the unit is off by (9 + 1.25 |g|) * 2^-24 for negative gates g: the exponent of 2 is g log2 e, rounded, with log2 e
+    rounded (together 1.22 |g|), ex2 4, the sum 1, the reciprocal 2, two products 2; for positive ones the 9 alone.  In 32 bits: expf an ulp (2), the sum, the
+    division and the product 1 each.  Gates that give 0 have a unit below 2^-119."""
+    gates = [-20.0, -40.0, -60.0, -87.0, 30.0, 100.0, LARGEST] + ([-0.75] if dtype == BF else [-88.5])
+    none = [-100.0, -LARGEST] + ([-87.5, -88.5] if dtype == BF else [-89.0])
+    up = (2 * torch.rand(len(gates + none), width, generator=gen(width), device="cuda") - 1).to(BF).to(dtype)
+    gate = torch.tensor(gates + none, device="cuda").to(dtype)
+    assert gate.tolist() == pytest.approx(gates + none, rel=1e-6)
+    x = torch.cat([gate[:, None].expand(-1, width), up], 1)
+    q, s = ops.new_int8(len(gate), width, "cuda").fill_(55), torch.empty(len(gate), device="cuda")
+    ops.silu_mul_int8(q, s, x)
+    g64 = gate.double()[:, None]
+    y = g64 * torch.sigmoid(g64) * up.double()
+    for i, g in enumerate(gates):
+        check_rows(q[i:i + 1], s[i:i + 1], y[i:i + 1], ((9 + 1.25 * max(0.0, -g)) if dtype == BF else 5) * 2.0 ** -24)
+    assert y[len(gates):].abs().max() < 2.0 ** -119 and not s[len(gates):].any() and not q[len(gates):].any()
+
+
+@pytest.mark.parametrize("spread", [1.5, 12.0, 50.0])
+def test_a_row_does_not_depend_on_where_it_lies(ops, spread):
+    """The unit and plain rows, without a sum of their own, in either type: pieces of eight, single elements and shared memory give the same."""
+    for dtype, n, width in ((BF, 40, 4096), (F, 40, 4096), (BF, 700, 17000), (F, 20, 17000)):
+        g = gen(width + n)
+        x = (spread * torch.randn(n, 2 * width, generator=g, device="cuda")).to(dtype)
+        for call, given in ((ops.silu_mul_int8, x), (ops.quantize_rows, x[:, :width])):
+            q, s = ops.new_int8(n, width, "cuda"), torch.empty(n, device="cuda")
+            call(q, s, given)
+            odd, t = torch.empty(n, width + 1, dtype=torch.int8, device="cuda")[:, :width], torch.empty(n, device="cuda")
+            call(odd, t, given)
+            few, u = ops.new_int8(3, width, "cuda"), torch.empty(3, device="cuda")
+            call(few, u, given[:3])
+            assert torch.equal(q, odd) and torch.equal(s, t) and torch.equal(q[:3], few) and torch.equal(s[:3], u)
