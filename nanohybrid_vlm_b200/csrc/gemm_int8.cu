@@ -673,24 +673,24 @@ SplitSmem split_smem(const SplitPlan& plan) {
 //   (12,288 x 4,096 in 3 parts, 288 blocks: 15.1 / 19.6; 2,048 x 4,096 for 128 tokens as 16 clusters of 8 13.4, as 32 of 4 with tiles of 64 rows
 //   8.6).
 //   Short sums: K in one part, the tiles smaller: 4,096 x 1,024, 64 rows 3.6 / 4.1 / 5.1, 4 parts of 128 rows 3.6 / 5.3 / 8.8.
-SplitPlan split_plan(const Product& p, int sms) {
-  const int kt = (p.K + BK - 1) / BK;
+SplitPlan split_plan(int T, int N, int K, int sms) {
+  const int kt = (K + BK - 1) / BK;
   SplitPlan plan;
-  plan.nt = p.T >= 128 ? 128 : (p.T + 15) / 16 * 16;
+  plan.nt = T >= 128 ? 128 : (T + 15) / 16 * 16;
   const bool shared = plan.nt <= 64, few = plan.nt <= 32;
-  plan.rows = shared || p.N > 64 * (sms * 7 / 8 / 4) ? 128 : 64;
-  int tiles = (p.N + plan.rows - 1) / plan.rows;
+  plan.rows = shared || N > 64 * (sms * 7 / 8 / 4) ? 128 : 64;
+  int tiles = (N + plan.rows - 1) / plan.rows;
   const int most_parts = shared ? 8 : 4;
   plan.parts = (shared ? 2 * sms * 9 / 10 : sms * 7 / 8) / tiles;
   if (plan.parts > most_parts) plan.parts = most_parts;
   while (plan.parts > 1 && kt < 8 * plan.parts && tiles * plan.parts > sms) --plan.parts;
   if (plan.parts > kt) plan.parts = kt;
-  if (plan.parts < (shared || kt < 32 ? 3 : 2) || (kt < 16 && p.N >= 24 * sms) || (!few && p.N >= (shared ? 60 : 48) * sms)) {
+  if (plan.parts < (shared || kt < 32 ? 3 : 2) || (kt < 16 && N >= 24 * sms) || (!few && N >= (shared ? 60 : 48) * sms)) {
     plan.parts = 1;
-    const long long slots = p.N > 96LL * sms ? 2 * sms : sms, waves = (p.N + 128LL * slots - 1) / (128LL * slots);
-    plan.rows = (int)((p.N + waves * slots - 1) / (waves * slots));
-    if (plan.rows < 32) plan.rows = p.N < 64 ? 64 : 32;
-    tiles = (p.N + plan.rows - 1) / plan.rows;
+    const long long slots = N > 96LL * sms ? 2 * sms : sms, waves = (N + 128LL * slots - 1) / (128LL * slots);
+    plan.rows = (int)((N + waves * slots - 1) / (waves * slots));
+    if (plan.rows < 32) plan.rows = N < 64 ? 64 : 32;
+    tiles = (N + plan.rows - 1) / plan.rows;
   }
   const bool alone = !few && kt >= 16 && (long long)tiles * plan.parts <= sms;
   const size_t most = ((plan.parts == 1 ? alone : !shared) ? 200 : 112) * 1024;
@@ -746,17 +746,22 @@ int launch_pair(Mapped& m, int sms, cudaStream_t stream) {
 // The tiles' width: the one with the least turns * (width + 64), a turn being a tile for every pair, and 64 what a tile costs beside
 // its width.  us for widths 64 / 128 / 192 / 256: 256 tokens, 4,096 x 4,096 9.3 / 9.9 / - / 15.0, 24,576 x 4,096 35.5 / 26.5 / 26.2 / 29.0; 4,096 x 12,288, 512
 // tokens 32.4 / 23.1 / 31.0 / 36.0, 1,024 - / 39.1 / 47.7 / 37.1, 2,048 - / 90.7 / 84.2 / 75.4.
-int pair_product(Mapped& m, int sms, cudaStream_t stream) {
-  const long long tiles_t = (m.p.T + 255) / 256, pairs = sms / 2;
-  long long least = 0;
-  int width = 256;
+struct PairPlan {
+  int width;
+  long long tiles, turns;
+};
+PairPlan pair_plan(int T, int N, int sms) {
+  const long long tiles_t = (T + 255) / 256, pairs = sms / 2;
+  PairPlan plan = {};
   for (int w = 256; w >= 64; w -= 64) {
-    const long long turns = (tiles_t * ((m.p.N + w - 1) / w) + pairs - 1) / pairs, cost = turns * (w + 64);
-    if (w == 256 || cost < least) {
-      least = cost;
-      width = w;
-    }
+    const long long tiles = tiles_t * ((N + w - 1) / w), turns = (tiles + pairs - 1) / pairs;
+    if (w == 256 || turns * (w + 64) < plan.turns * (plan.width + 64)) plan = {w, tiles, turns};
   }
+  return plan;
+}
+
+int pair_product(Mapped& m, int sms, cudaStream_t stream) {
+  const int width = pair_plan(m.p.T, m.p.N, sms).width;
   if (width == 64) return launch_pair<64>(m, sms, stream);
   if (width == 128) return launch_pair<128>(m, sms, stream);
   if (width == 192) return launch_pair<192>(m, sms, stream);
@@ -769,6 +774,25 @@ int pair_product(Mapped& m, int sms, cudaStream_t stream) {
 NHV_API int nhv_gemm_int8_error() { return nhv_wait_error_take(); }
 // The device address of the error word, for kernels that report it with the step's result.
 NHV_API void* nhv_gemm_int8_error_word() { return nhv_wait_error_address(); }
+
+// How a product of these sizes is cut on a device with `sms` SMs, in `out`: 0 (K may be in parts) or 1 (pairs of SMs), tokens of a tile, outputs of a
+// tile, parts of K, stages of the ring, tiles, turns of a pair, bytes of shared memory of a block.
+NHV_API int nhv_gemm_int8_plan(int T, int N, int K, int sms, long long* out) {
+  NHV_REQUIRE(T > 0 && N > 0 && K > 0 && K <= 131071 && T <= INT_MAX - 511 && N <= INT_MAX - 511 && sms > 1 && out, "linear_int8: no plan for these sizes");
+  if (T <= 128) {
+    const SplitPlan plan = split_plan(T, N, K, sms);
+    const long long all[8] = {0, plan.nt, plan.rows, plan.parts, plan.stages, (N + plan.rows - 1) / plan.rows, 1, (long long)split_smem(plan).all};
+    memcpy(out, all, sizeof(all));
+  } else {
+    const PairPlan plan = pair_plan(T, N, sms);
+    const int stages[4] = {Pair<64>::STAGES, Pair<128>::STAGES, Pair<192>::STAGES, Pair<256>::STAGES};
+    const size_t smem[4] = {Pair<64>::SMEM, Pair<128>::SMEM, Pair<192>::SMEM, Pair<256>::SMEM};
+    const int i = plan.width / 64 - 1;
+    const long long all[8] = {1, 256, plan.width, 1, stages[i], plan.tiles, plan.turns, (long long)smem[i]};
+    memcpy(out, all, sizeof(all));
+  }
+  return 0;
+}
 
 // What a call is given, one after the other, in one block.
 struct ProductCall {
@@ -812,6 +836,6 @@ NHV_API int nhv_gemm_int8(const void* given, cudaStream_t stream) {
   // the kernel before).
   Mapped m;
   m.p = p;
-  if (T <= 128) return split_product(m, split_plan(p, sms), stream);
+  if (T <= 128) return split_product(m, split_plan(T, N, K, sms), stream);
   return pair_product(m, sms, stream);
 }

@@ -94,6 +94,7 @@ _SIGNATURES = {
     "nhv_rows_int8": [ctypes.c_char_p, P],
     "nhv_rows_from_int8": [ctypes.c_char_p, P],
     "nhv_gemm_int8": [ctypes.c_char_p, P],
+    "nhv_gemm_int8_plan": [I, I, I, I, P],
     "nhv_decay_lowrank": [I, P, P, I, P, P, I, I, I, P],
 }
 

@@ -12,6 +12,7 @@ from __future__ import annotations
 import os
 import struct
 import weakref
+from typing import NamedTuple
 
 import torch
 
@@ -2003,6 +2004,26 @@ def dequantize_rows(out, q, scales) -> None:
 
 
 _PRODUCT_CALL = struct.Struct("=10q4i")
+
+
+class Int8Plan(NamedTuple):
+    """How ``linear_int8`` cuts a product: see ``int8_plan``."""
+    pairs: int          # 1: pairs of SMs on tiles of 256 tokens; 0: all tokens beside rows of the weight, K perhaps in parts
+    tokens: int         # of a tile
+    outputs: int        # of a tile
+    parts: int          # of K, one block of a cluster each
+    stages: int         # of a block's ring
+    tiles: int
+    turns: int          # tiles that a pair takes after one another, at most
+    shared_bytes: int   # of a block
+
+
+def int8_plan(T: int, N: int, K: int, sms: int) -> Int8Plan:
+    """The plan that ``linear_int8`` makes for x [T, K] and weight [N, K] on a device with so many SMs; needs no device."""
+    import ctypes
+    out = (ctypes.c_longlong * 8)()
+    call("nhv_gemm_int8_plan", T, N, K, sms, ctypes.addressof(out))
+    return Int8Plan(*out)
 
 
 def _check_linear_int8(out, x, x_scales, weight, weight_scales) -> None:
