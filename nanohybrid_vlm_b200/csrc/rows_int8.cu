@@ -165,14 +165,16 @@ template <typename T, int KIND>
 int launch_any(const Args& p, int n_rows, cudaStream_t stream) {
   int threads = 32;
   while (threads < 1024 && threads * 4 < p.width) threads <<= 1;
-  if (KIND == ROW_NORM || p.width <= KEPT_WIDTH) {
-    NHV_REQUIRE(p.width <= KEPT_WIDTH, "rmsnorm_int8: width %d is beyond the %d floats that a row buffer holds", p.width, KEPT_WIDTH);
-    static std::atomic<uint64_t> allowed{0};
-    NHV_CUDA(nhv_allow_smem((const void*)rows_kernel<T, KIND, true>, KEPT_WIDTH * 4, allowed), "rows_int8");
-    NHV_CUDA(nhv_launch(rows_kernel<T, KIND, true>, dim3(n_rows), dim3(threads), (size_t)p.width * 4, stream, p), "rows_int8");
-  } else {
-    NHV_CUDA(nhv_launch(rows_kernel<T, KIND, false>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
+  if (p.width > KEPT_WIDTH) {
+    if constexpr (KIND == ROW_NORM)
+      NHV_REQUIRE(false, "rmsnorm_int8: width %d is beyond the %d floats that a row buffer holds", p.width, KEPT_WIDTH);
+    else
+      NHV_CUDA(nhv_launch(rows_kernel<T, KIND, false>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
+    return 0;
   }
+  static std::atomic<uint64_t> allowed{0};
+  NHV_CUDA(nhv_allow_smem((const void*)rows_kernel<T, KIND, true>, KEPT_WIDTH * 4, allowed), "rows_int8");
+  NHV_CUDA(nhv_launch(rows_kernel<T, KIND, true>, dim3(n_rows), dim3(threads), (size_t)p.width * 4, stream, p), "rows_int8");
   return 0;
 }
 
@@ -431,10 +433,13 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) rows8_wide_kernel(const Args 
 template <typename T, int KIND, int CH>
 int launch_eights(const Args& p, int n_rows, cudaStream_t stream) {
   const int threads = ((p.width / 8 + CH - 1) / CH + 31) / 32 * 32;
-  if (threads <= 256)
-    NHV_CUDA(nhv_launch(rows8_kernel<T, KIND, CH, 256>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
-  else
-    NHV_CUDA(nhv_launch(rows8_kernel<T, KIND, CH, 1024>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
+  if constexpr (sizeof(T) == 2 || CH > 1) {                       // one piece a thread of 32-bit rows: up to 256 pieces
+    if (threads > 256) {
+      NHV_CUDA(nhv_launch(rows8_kernel<T, KIND, CH, 1024>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
+      return 0;
+    }
+  }
+  NHV_CUDA(nhv_launch(rows8_kernel<T, KIND, CH, 256>, dim3(n_rows), dim3(threads), 0, stream, p), "rows_int8");
   return 0;
 }
 
@@ -461,8 +466,10 @@ int launch_row(const Args& p, int n_rows, cudaStream_t stream) {
   while (each * 1024 < pieces) each *= 2;
   while (each > 1 && pieces <= 32 * (each / 2)) each /= 2;
   if (each == 1) return launch_eights<T, KIND, 1>(p, n_rows, stream);
-  if (each == 2) return launch_eights<T, KIND, 2>(p, n_rows, stream);
-  return launch_eights<T, KIND, 4>(p, n_rows, stream);
+  if constexpr (sizeof(T) == 2) {                                 // 32-bit rows: up to 2,047 pieces, two a thread
+    if (each == 4) return launch_eights<T, KIND, 4>(p, n_rows, stream);
+  }
+  return launch_eights<T, KIND, 2>(p, n_rows, stream);
 }
 
 template <typename T>
