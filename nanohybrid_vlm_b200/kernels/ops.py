@@ -1958,7 +1958,7 @@ def _check_rmsnorm_int8(q, scales, x, weight, residual, write_residual: bool, ro
 def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual: bool = True, weight_offset: float = 0.0) -> None:
     """``rmsnorm`` with its output in 8 bits: q [n, width] int8 and scales [n] as ``quantize_rows`` gives them for norm(x (+ residual)) *
     (weight + weight_offset), which is held in 32 bits and rounded once.  With a residual and write_residual the sum, rounded to x's
-    type, replaces the residual.  Widths up to 51,200."""
+    type, replaces the residual.  Widths up to 51,200.  As in ``rmsnorm`` the squares are summed in 32 bits: a sum of 2^128 and more makes zeros."""
     shape, dtype, device = x.shape, x.dtype, x.get_device()
     width = shape[-1] if shape else 0
     rows = x.numel() // width if width else 0
@@ -1977,7 +1977,8 @@ def rmsnorm_int8(q, scales, x, weight, eps: float, residual=None, write_residual
 
 def silu_mul_int8(q, scales, gate_up) -> None:
     """``silu_mul`` with its output in 8 bits: q [n, inter] int8 and scales [n] as ``quantize_rows`` gives them for silu(gate) * up, which is held
-    in 32 bits; gate_up [n, 2 * inter] with the gate in the first half of each row."""
+    in 32 bits; gate_up [n, 2 * inter] with the gate in the first half of each row.  With bfloat16 rows the unit is off by up to
+    (9 + 1.25 max(0, -gate)) * 2^-24; gates below -87.3 (float32: -88.7) give 0."""
     _contig("gate_up", gate_up)
     if gate_up.dim() != 2 or gate_up.shape[1] % 2:
         raise KernelError(f"gate_up is [n, 2 * inter], not {tuple(gate_up.shape)}")
@@ -1986,7 +1987,7 @@ def silu_mul_int8(q, scales, gate_up) -> None:
 
 
 def dequantize_rows(out, q, scales) -> None:
-    """out[n, width] = q * scales[:, None]: the values that rows of 8-bit integers stand for, rounded once to out's type (bfloat16 or float32).
+    """out[n, width] = q * scales[:, None]: the values that rows of 8-bit integers stand for, in 32 bits, then in out's type (bfloat16 or float32).
     Rows of out and q may lie further apart."""
     shape, step = out.shape, out.stride()
     if len(shape) != 2 or (step[1] != 1 and shape[1] > 1) or (step[0] < shape[1] and shape[0] > 1):
